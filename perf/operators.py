@@ -126,7 +126,7 @@ def _weights(g, *shape):
     scale = torch.empty(n, device="cuda")
     for at in range(0, n, 16384):
         w = torch.empty(min(16384, n - at), k, device="cuda").normal_(0.0, 0.02, generator=g)
-        s = w.abs().amax(1) * (1.0 / 127.0)
+        s = w.abs().amax(1) / 127.0
         q[at:at + 16384, :k] = torch.round(w / s[:, None]).clamp_(-127, 127).to(torch.int8)
         scale[at:at + 16384] = s
     return q.view(*shape[:-1], -1)[..., :k], scale.view(shape[:-1])
@@ -161,7 +161,8 @@ def prepare(case, seed):
 # ---- one pass ----------------------------------------------------------------------------------------
 def _int8(x):
     """The integers and the scales of rows of 32-bit values."""
-    scale = x.abs().amax(-1, keepdim=True) * (1.0 / 127.0)
+    largest = x.abs().amax(-1, keepdim=True)
+    scale = largest / largest.new_full((), 127.0)                               # (a quotient: by a number torch would multiply by 1 / 127)
     return torch.where(scale > 0, torch.round(x / scale), 0.0), scale
 
 
