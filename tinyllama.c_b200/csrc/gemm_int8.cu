@@ -1,0 +1,170 @@
+// Products in 8-bit integers: out[m, n] (+)= a_scale[m] w_scale[n] sum_k a[m, k] w[n, k] + colbias[n], also gated (silu(gate) * up and
+// the like) and grouped by expert.  The sum of integers is exact in 32 bits while K <= 131,071 (128 * 128 * K < 2^31), so neither the
+// order of a sum nor how K is cut changes a result.
+//
+// Here: the product for operands in any layout, on the CUDA cores (dp4a: four products and their sum an instruction), tiles of 32 x
+// 64 results staged through shared memory 64 values of K at a time.
+#include "gemm_int8.cuh"
+
+namespace {
+
+constexpr int TM = 32, TN = 64, TKW = 16;          // a tile's rows and columns; K in words of four values
+
+// Four values from k on as one word, zeros past K.
+__device__ __forceinline__ int word_at(const int8_t* p, int k, int K, bool words) {
+  if (words && k + 4 <= K) return *reinterpret_cast<const int*>(p + k);
+  int v = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) if (k + i < K) v |= (int)(uint8_t)p[k + i] << (8 * i);
+  return v;
+}
+
+template <typename TO, bool GLU>
+__global__ void __launch_bounds__(256)
+int8_tile_kernel(Int8Args p) {
+  tlc_pdl(p.a, p.a_scale, p.w, p.out, p.offsets, p.order, p.wts);
+  constexpr int NW = GLU ? 2 : 1;
+  __shared__ int As[TM][TKW + 1], Ws[NW][TN][TKW + 1];
+  const int tid = threadIdx.x, n0 = blockIdx.y * TN;
+  int group = 0, row0, rows;
+  if (p.offsets) {                                  // which group's tile this is: the tiles before it are counted
+    int tile = blockIdx.x;
+    bool found = false;
+    for (; group < p.E; group++) {
+      const int count = p.offsets[group + 1] - p.offsets[group], tiles = (count + TM - 1) / TM;
+      if (tile < tiles) { found = true; break; }
+      tile -= tiles;
+    }
+    if (!found) return;
+    row0 = p.offsets[group] + tile * TM;
+    rows = min(TM, p.offsets[group + 1] - row0);
+  } else {
+    row0 = blockIdx.x * TM;
+    rows = min(TM, p.M - row0);
+  }
+  const bool words_a = ((uintptr_t)p.a | (uintptr_t)p.lda) % 4 == 0, words_w = ((uintptr_t)p.w | (uintptr_t)p.ldw) % 4 == 0;
+  const size_t w0 = (size_t)group * p.w_rows;
+  const int r2 = (tid >> 4) * 2, c0 = tid & 15;     // this thread's rows r2, r2 + 1 and columns c0 + 16 j
+  int acc[NW][2][4] = {};
+  for (int k0 = 0; k0 < p.K; k0 += 4 * TKW) {
+#pragma unroll
+    for (int i = 0; i < TM * TKW / 256; i++) {
+      const int r = (tid >> 4) + i * 16, k = k0 + 4 * (tid & 15);
+      As[r][tid & 15] = r < rows ? word_at(p.a + (size_t)(row0 + r) * p.lda, k, p.K, words_a) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < NW; u++)
+#pragma unroll
+      for (int i = 0; i < TN * TKW / 256; i++) {
+        const int n = (tid >> 4) + i * 16, k = k0 + 4 * (tid & 15);
+        Ws[u][n][tid & 15] = n0 + n < p.N ? word_at(p.w + (w0 + (size_t)u * p.N + n0 + n) * p.ldw, k, p.K, words_w) : 0;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < TKW; k++) {
+      const int a0 = As[r2][k], a1 = As[r2 + 1][k];
+#pragma unroll
+      for (int u = 0; u < NW; u++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int b = Ws[u][c0 + 16 * j][k];
+          acc[u][0][j] = __dp4a(a0, b, acc[u][0][j]);
+          acc[u][1][j] = __dp4a(a1, b, acc[u][1][j]);
+        }
+    }
+    __syncthreads();
+  }
+  TO* out = reinterpret_cast<TO*>(p.out);
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    if (r2 + i >= rows) continue;
+    const int row = row0 + r2 + i, pair = p.order ? p.order[row] : row;
+    float rs = p.a_scale[row];
+    if (p.w_out) rs *= p.wts[pair];
+    const float pw = p.w_in ? p.wts[pair] : 1.0f;
+    TO* o = out + (size_t)(p.scatter ? pair : row) * p.ldo;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int n = n0 + c0 + 16 * j;
+      if (n >= p.N) continue;
+      float v = int8_value(acc[0][i][j], rs, p.w_scale[w0 + n]);
+      if (p.colbias) v += p.colbias[n];
+      if (GLU || p.mode == I8_ACT) {
+        float u = 0.f;
+        if (GLU) {
+          u = int8_value(acc[NW - 1][i][j], rs, p.w_scale[w0 + p.N + n]);
+          if (p.colbias) u += p.colbias[p.N + n];
+        }
+        v = moe_pair_act<false>(p.act, 0, p.limit, p.alpha, pw, v, u);
+      } else if (p.mode == I8_ADD) {
+        v += to_f32(o[n]);
+      }
+      o[n] = from_f32<TO>(v);
+    }
+  }
+}
+
+template <typename TO>
+int run_tiles(const Int8Args& p, cudaStream_t stream) {
+  // grouped: an upper bound, the last blocks find no tile
+  const int tiles = p.offsets ? p.M / TM + (p.M < p.E ? p.M : p.E) : (p.M + TM - 1) / TM;
+  const dim3 grid(tiles, (p.N + TN - 1) / TN);
+  if (p.mode == I8_GLU) tlc_launch(int8_tile_kernel<TO, true>, grid, dim3(256), 0, stream, p);
+  else tlc_launch(int8_tile_kernel<TO, false>, grid, dim3(256), 0, stream, p);
+  TLC_CHECK_LAUNCH("linear_int8");
+  return 0;
+}
+
+int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
+  if (out_dtype == TLC_F32) return run_tiles<float>(p, stream);
+  if (out_dtype == TLC_BF16) return run_tiles<__nv_bfloat16>(p, stream);
+  return tlc_fail(-1, "linear_int8: unknown output dtype %d", out_dtype);
+}
+
+}  // namespace
+
+extern "C" int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_scale, void* a_int8, int ld_int8, const void* w, int ldw,
+                               const float* w_scale, void* out, int out_dtype, int ldo, const float* colbias, int accumulate, int M, int N,
+                               int K, int act, float limit, float alpha, cudaStream_t stream) {
+  if (M == 0 || N == 0) return 0;
+  TLC_REQUIRE(K > 0 && K <= 131071 && lda >= K && ldw >= K && ldo >= N && M > 0 && N > 0,
+              "linear_int8: bad sizes M=%d N=%d K=%d (at most 131071) lda=%d ldw=%d ldo=%d", M, N, K, lda, ldw, ldo);
+  TLC_REQUIRE(act < 0 || act == TLC_ACT_SILU || act == TLC_ACT_GELU_TANH || act == TLC_ACT_SWISH_CLAMPED, "linear_int8: unknown activation %d", act);
+  if (a_dtype != TLC_I8) {
+    if (int rc = tlc_rows_int8(a, a_dtype, lda, M, K, nullptr, 0.f, a_int8, ld_int8, a_scale, nullptr, 1, 0, stream)) return rc;
+    a = a_int8;
+    lda = ld_int8;
+  }
+  Int8Args p = {};
+  p.a = (const int8_t*)a; p.a_scale = a_scale; p.w = (const int8_t*)w; p.w_scale = w_scale; p.out = out; p.colbias = colbias;
+  p.lda = lda; p.ldw = ldw; p.ldo = ldo; p.M = M; p.N = N; p.K = K; p.w_rows = act >= 0 ? 2 * N : N;
+  p.mode = act >= 0 ? I8_GLU : accumulate ? I8_ADD : I8_PLAIN;
+  p.act = act; p.limit = limit; p.alpha = alpha;
+  return run(p, out_dtype, stream);
+}
+
+extern "C" int tlc_moe_experts_int8(const void* x, int x_dtype, int ldx, const void* wgu, int ldgu, const float* sgu, const void* wd, int ldd,
+                                    const float* sd, const int* order, const int* offsets, const float* wts, int T, int E, int top, int F,
+                                    int D, void* q, int ldq, float* scales, float* act, void* y, int y_dtype, int act_code, int w_out,
+                                    float limit, float alpha, cudaStream_t stream) {
+  if (T == 0) return 0;
+  const long long pairs = (long long)T * top;
+  TLC_REQUIRE(T > 0 && top >= 1 && E >= 1 && F >= 1 && D >= 1 && F <= 131071 && D <= 131071 && pairs < (1 << 30),
+              "moe_experts_int8: bad sizes T=%d E=%d top=%d F=%d D=%d", T, E, top, F, D);
+  TLC_REQUIRE(ldgu >= D && ldd >= F && ldq >= D && ldq >= F, "moe_experts_int8: rows shorter than the sizes (ld %d %d %d)", ldgu, ldd, ldq);
+  TLC_REQUIRE(act_code >= TLC_ACT_SILU && act_code <= TLC_ACT_RELU_SQUARED, "moe_experts_int8: unknown activation %d", act_code);
+  // the chosen rows, sorted by expert, rounded; both products read their rows from q
+  if (int rc = tlc_rows_int8(x, x_dtype, ldx, (int)pairs, D, nullptr, 0.f, q, ldq, scales, order, top, 0, stream)) return rc;
+  const bool gated = act_code != TLC_ACT_RELU_SQUARED;
+  Int8Args p = {};
+  p.a = (const int8_t*)q; p.a_scale = scales; p.w = (const int8_t*)wgu; p.w_scale = sgu; p.out = act;
+  p.lda = ldq; p.ldw = ldgu; p.ldo = F; p.M = (int)pairs; p.N = F; p.K = D; p.w_rows = gated ? 2 * F : F;
+  p.mode = gated ? I8_GLU : I8_ACT; p.act = act_code; p.limit = limit; p.alpha = alpha;
+  p.offsets = offsets; p.order = order; p.wts = wts; p.E = E; p.w_in = !w_out;
+  if (int rc = run(p, TLC_F32, stream)) return rc;
+  // the activation in 32 bits -> rounded row by row; a weight on the result only multiplies the row's scale
+  if (int rc = tlc_rows_int8(act, TLC_F32, F, (int)pairs, F, nullptr, 0.f, q, ldq, scales, nullptr, 1, 0, stream)) return rc;
+  p.w = (const int8_t*)wd; p.w_scale = sd; p.out = y; p.ldw = ldd; p.ldo = D; p.N = D; p.K = F; p.w_rows = D;
+  p.mode = I8_PLAIN; p.w_in = 0; p.w_out = w_out; p.scatter = 1;
+  return run(p, y_dtype, stream);
+}

@@ -1,0 +1,25 @@
+// What the kernels of the products in 8-bit integers share: the operands, and the groups (experts) of a grouped product.
+#pragma once
+#include "common.cuh"
+
+// out[m, n] (+)= a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + colbias[n], or gated: act(y[m, n]) * y[m, F + n] for a w of 2 F
+// rows (the gate's, then the up projection's).  Grouped (offsets not NULL): rows offsets[e] .. offsets[e + 1] - 1 of a are multiplied
+// by the rows e * w_rows .. of w; order [rows] is the pair (row of the step * top + choice) of every row, wts [pairs] the pairs'
+// weights.
+struct Int8Args {
+  const int8_t* a; const float* a_scale;
+  const int8_t* w; const float* w_scale;
+  void* out; const float* colbias;
+  int lda, ldw, ldo, M, N, K;           // N: columns of the result (gated: F, w has 2 F rows)
+  int w_rows;                           // rows of w, or of one group's
+  int mode;                             // I8_*
+  int act, w_in;                        // gated / I8_ACT: the activation; w_in: the pair's weight multiplies the products before it
+  float limit, alpha;
+  const int* offsets; const int* order; const float* wts;
+  int E;
+  int scatter, w_out;                   // result rows go where order says, times the pair's weight
+};
+enum { I8_PLAIN = 0, I8_ADD = 1, I8_ACT = 2, I8_GLU = 3 };
+
+// One result from its integer sum.  Both scales in 32 bits, one after the other: their product alone may leave the range.
+__device__ __forceinline__ float int8_value(int sum, float row_scale, float col_scale) { return __int2float_rn(sum) * row_scale * col_scale; }

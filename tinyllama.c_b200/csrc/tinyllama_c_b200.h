@@ -27,6 +27,7 @@
 
 #define TLC_F32 0
 #define TLC_BF16 1
+#define TLC_I8 2              /* activations of the products in 8-bit integers only */
 #define TLC_PAGE 64
 #define TLC_ACT_SILU 0       /* activations of gated products: z * sigmoid(z) */
 #define TLC_ACT_GELU_TANH 1  /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
@@ -415,6 +416,30 @@ void tlc_delta_rule_split(int threads);   /* threads that share the rows of a co
 int tlc_delta_rule(const float* qkv, int ld, int q_off, int k_off, int v_off, const float* beta, const float* decay,
                    float* state, const int* cu_seqlens, const int* slots, const int* start_pos, int B, int T, int H, int G,
                    int dk, int dv, float* y, int ldy, int ldd, cudaStream_t stream);
+
+/* ---- products in 8-bit integers (int8_rows.cu, gemm_int8.cu) --------------------------------------------------------
+ * tlc_rows_int8: rows of x [T, ldx] (float or bfloat16, K values each), or with norm_weight [K] their RMS norm, rounded to integers:
+ * scale[t] = max_k |v[t, k]| / 127, q[t, k] = rint(v[t, k] / scale[t]).  A row of zeros gets scale 0; a row with an infinity or a NaN
+ * the scale NaN and integers 0.  order not NULL: row i of the result is row order[i] / top of x.  boundary: the launch is followed by
+ * a step boundary, after which q may be the w of a product (which fetches w ahead of its wait on the kernel before it). */
+int tlc_rows_int8(const void* x, int x_dtype, int ldx, int T, int K, const float* norm_weight, float eps, void* q, int ldq,
+                  float* scale, const int* order, int top, int boundary, cudaStream_t stream);
+/* out[m, n] (+)= a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + colbias[n]: a [M, lda] int8 (a_dtype TLC_I8, a_scale [M] given), or
+ * float or bfloat16 rows, which are rounded first (a_int8 [M, ld_int8] and a_scale [M] are then scratch).  w [N, ldw] int8,
+ * w_scale [N], colbias [N] or NULL, out float or bfloat16; K at most 131071 (the sums are exact 32-bit integers).
+ * act >= 0 (TLC_ACT_SILU, TLC_ACT_GELU_TANH, TLC_ACT_SWISH_CLAMPED): gated, w has 2 N rows (N gate rows, then N up rows; w_scale,
+ * colbias [2 N]) and out[m, n] = act(y[m, n]) * y[m, N + n], or the clamped swish's form with limit and alpha; no accumulate. */
+int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_scale, void* a_int8, int ld_int8, const void* w, int ldw,
+                    const float* w_scale, void* out, int out_dtype, int ldo, const float* colbias, int accumulate, int M,
+                    int N, int K, int act, float limit, float alpha, cudaStream_t stream);
+/* The experts' feed-forwards over the pairs that tlc_moe_route sorted, in 8-bit integers: x [T, ldx] float or bfloat16;
+ * wgu int8 [E, 2F, ldgu] (TLC_ACT_RELU_SQUARED: [E, F, ldgu]) with scales sgu [E, 2F], wd int8 [E, D, ldd] with scales sd [E, D].
+ * Scratch: q int8 [T*top, ldq] (ldq >= D and F), scales [T*top], act float [T*top, F].  y [T*top, D] float or bfloat16: every
+ * pair's result.  Uses order, offsets and wts of the routing; any number of rows a tile it was made for will do. */
+int tlc_moe_experts_int8(const void* x, int x_dtype, int ldx, const void* wgu, int ldgu, const float* sgu, const void* wd, int ldd,
+                         const float* sd, const int* order, const int* offsets, const float* wts, int T, int E, int top, int F,
+                         int D, void* q, int ldq, float* scales, float* act, void* y, int y_dtype, int act_code, int w_out,
+                         float limit, float alpha, cudaStream_t stream);
 
 /* ---- mixture of experts (moe.cu) ------------------------------------------------------------------------
  * tlc_moe_route: logits float [T, ld] (E columns) -> per token its `top` experts by descending logit (lowest index

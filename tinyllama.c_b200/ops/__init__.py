@@ -18,7 +18,7 @@ import torch
 
 from ..csrc import build as _build
 
-F32, BF16 = 0, 1
+F32, BF16, I8 = 0, 1, 2      # I8: activations of the products in 8-bit integers
 PAGE = 64          # tokens per page of the key/value store (TLC_PAGE in tinyllama_c_b200.h)
 # What the kernels are built for; a part checks its sizes against these when it is constructed, so that a
 # configuration they do not cover is refused when the model is built, not at its first step.
@@ -160,6 +160,10 @@ _SIGNATURES = {
     "tlc_delta_rule_split": (None, [_i]),
     "tlc_delta_rule": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _i, _vp]),
     "tlc_moe_down": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
+    "tlc_rows_int8": (_i, [_vp, _i, _i, _i, _i, _vp, _f, _vp, _i, _vp, _vp, _i, _i, _vp]),
+    "tlc_linear_int8": (_i, [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _f, _f, _vp]),
+    "tlc_moe_experts_int8": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i,
+                                  _i, _i, _f, _f, _vp]),
     "tlc_argmax": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
     "tlc_sample": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _i, _f, _f, _f, _i, _f, _f, _vp, _vp]),
     "tlc_attention_decode_no_alloc": (_i, [_vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _i, _i,
@@ -1552,6 +1556,159 @@ def moe_identity(x: torch.Tensor, routing, top: int, n_experts: int, y: torch.Te
         raise KernelError("moe_identity: y contiguous float32 [T, top, D]")
     _call("tlc_moe_identity", x.data_ptr(), dtype_code(x.dtype), _rows(x, "moe input"), ids.data_ptr(), wts.data_ptr(), T, int(top),
           int(n_experts), D, y.data_ptr(), _stream())
+
+
+# ---- products in 8-bit integers ----------------------------------------------------------------------------
+# Weights as integers in -127..127 with one scale for each output channel, activations rounded to such integers row by row with one
+# scale a row; the sums are exact integers, multiplied by both scales.  Rows of integers start on 16-byte boundaries where the
+# functions here make them (int8_empty), which the tensor-core kernels need; operands in any other layout are multiplied on the CUDA
+# cores.
+INT8_MAX_K = 131071                      # 128 * 128 * K < 2^31: the sums of products stay exact in 32 bits
+
+
+def int8_empty(rows: int, k: int, device) -> torch.Tensor:
+    """An uninitialised int8 [rows, k] whose rows start on 16-byte boundaries."""
+    return torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
+
+
+def _rows_int8(x, q, scale, norm_weight=None, eps=0.0, boundary=0):
+    T, K = x.shape
+    _call("tlc_rows_int8", x.data_ptr(), dtype_code(x.dtype), _rows(x, "rows_int8 input"), T, K, _p(norm_weight), float(eps), q.data_ptr(),
+          q.stride(0), scale.data_ptr(), None, 1, boundary, _stream())
+    return q, scale
+
+
+def rows_int8(x: torch.Tensor):
+    """(q int8 [T, K], scale float32 [T]) of float32 or bfloat16 rows: scale[t] = max_k |x[t, k]| / 127, q = x / scale rounded to the
+    nearest integer (halves to even).  A row of zeros has scale 0; one that holds a NaN or an infinity has scale NaN and integers 0.
+    q is an operand a of linear_int8; for weights see weight_int8."""
+    _gpu(x)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise KernelError(f"rows_int8: rows [T, K] with K >= 1, got {tuple(x.shape)}")
+    return _rows_int8(x, int8_empty(x.shape[0], x.shape[1], x.device), torch.empty(x.shape[0], dtype=torch.float32, device=x.device))
+
+
+def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float):
+    """rows_int8 of the RMS norm x / sqrt(mean(x^2) + eps) * weight of every row, in one pass; weight float32 [K]."""
+    _gpu(x, weight)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise KernelError(f"rmsnorm_int8: rows [T, K] with K >= 1, got {tuple(x.shape)}")
+    _f32vec(weight, x.shape[1], "rmsnorm_int8 weight")
+    return _rows_int8(x, int8_empty(x.shape[0], x.shape[1], x.device), torch.empty(x.shape[0], dtype=torch.float32, device=x.device), weight, eps)
+
+
+def weight_int8(w: torch.Tensor):
+    """(q int8 [N, K] or [E, N, K], scale float32 [N] or [E, N]) of a weight matrix, or of one per expert: rows_int8 of its output
+    channels, for the w of the products below.  Made once, when weights are loaded; what follows on the stream starts after it."""
+    _gpu(w)
+    if w.dim() not in (2, 3) or w.shape[-1] < 1:
+        raise KernelError(f"weight_int8: a matrix [N, K] or matrices [E, N, K], got {tuple(w.shape)}")
+    rows = w.reshape(-1, w.shape[-1])
+    q = int8_empty(rows.shape[0], rows.shape[1], w.device)
+    scale = torch.empty(rows.shape[0], dtype=torch.float32, device=w.device)
+    _rows_int8(rows, q, scale, boundary=1)
+    cannot_repeat()
+    if w.dim() == 3:
+        ld = q.stride(0)
+        q = q.as_strided(tuple(w.shape), (w.shape[1] * ld, ld, 1))
+    return q, scale.view(w.shape[:-1])
+
+
+def _int8_operands(what, a, a_scale, w, w_scale, colbias, out, N):
+    """Checks what the two products below share; (a's type code, its row stride, the scale and the room for its integers)."""
+    _gpu(a, a_scale, w, w_scale, colbias, out)
+    if a.dim() != 2 or w.dim() != 2 or w.dtype != torch.int8 or w.shape[1] != a.shape[1] or tuple(out.shape) != (a.shape[0], N):
+        raise KernelError(f"{what}: shapes a{tuple(a.shape)} w{tuple(w.shape)} {w.dtype} out{tuple(out.shape)} do not agree")
+    M, K = a.shape
+    if not 1 <= K <= INT8_MAX_K:
+        raise KernelError(f"{what}: rows of {K} values; the sums are exact for 1 to {INT8_MAX_K}")
+    _f32vec(w_scale, w.shape[0], what + " weight scale")
+    _f32vec(colbias, w.shape[0], what + " colbias")
+    if a.dtype == torch.int8:
+        if a_scale is None:
+            raise KernelError(f"{what}: integer rows come with their scales (a_scale)")
+        _f32vec(a_scale, M, what + " a_scale")
+        return I8, a_scale, None, 0
+    if a_scale is not None:
+        raise KernelError(f"{what}: a_scale belongs to integer rows; a is {a.dtype}")
+    q, scale = int8_empty(M, K, a.device), torch.empty(M, dtype=torch.float32, device=a.device)
+    _note_owned(q, scale)
+    return dtype_code(a.dtype), scale, q, q.stride(0)
+
+
+def linear_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: torch.Tensor, a_scale: Optional[torch.Tensor] = None,
+                colbias: Optional[torch.Tensor] = None, accumulate: bool = False) -> None:
+    """out[m, n] (+)= a_scale[m] * w_scale[n] * (sum_k a[m, k] w[n, k]) + colbias[n] with exact sums of integers.
+
+    w int8 [N, K] and w_scale float32 [N] as weight_int8 makes them; a int8 [M, K] with a_scale float32 [M] (rows_int8,
+    rmsnorm_int8), or float32 or bfloat16 rows, which are rounded that way first.  out [M, N] float32 or bfloat16; a, w and out may
+    be row-strided views.  w is fetched while the kernel before may still run: it must not be the output of a kernel of the same
+    step (weight_int8 sees to that)."""
+    N = w.shape[0]
+    code, scale, q, ldq = _int8_operands("linear_int8", a, a_scale, w, w_scale, colbias, out, N)
+    _call("tlc_linear_int8", a.data_ptr(), code, _rows(a, "linear_int8 input"), scale.data_ptr(), _p(q), ldq, w.data_ptr(),
+          _rows(w, "linear_int8 weight"), w_scale.data_ptr(), out.data_ptr(), dtype_code(out.dtype), _rows(out, "linear_int8 output"),
+          _p(colbias), int(bool(accumulate)), a.shape[0], N, a.shape[1], -1, 0.0, 1.0, _stream())
+
+
+def linear_swiglu_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: torch.Tensor, a_scale: Optional[torch.Tensor] = None,
+                       colbias: Optional[torch.Tensor] = None, act: str = "silu", limit: float = 0.0, alpha: float = 1.0) -> None:
+    """out[m, f] = act(gate) * up with gate = y[m, f] and up = y[m, F + f] of the product y that linear_int8 makes with w [2F, K] (the
+    gate's rows, then the up projection's; not interleaved); act, limit and alpha as in glu()."""
+    if act not in DENSE_ACTS:
+        raise KernelError(f"linear_swiglu_int8: unknown activation '{act}'; known: {sorted(DENSE_ACTS)}")
+    F = w.shape[0] // 2
+    if w.shape[0] % 2:
+        raise KernelError(f"linear_swiglu_int8: {w.shape[0]} rows are not a gate's and as many of an up projection")
+    code, scale, q, ldq = _int8_operands("linear_swiglu_int8", a, a_scale, w, w_scale, colbias, out, F)
+    _call("tlc_linear_int8", a.data_ptr(), code, _rows(a, "linear_swiglu_int8 input"), scale.data_ptr(), _p(q), ldq, w.data_ptr(),
+          _rows(w, "linear_swiglu_int8 weight"), w_scale.data_ptr(), out.data_ptr(), dtype_code(out.dtype),
+          _rows(out, "linear_swiglu_int8 output"), _p(colbias), 0, a.shape[0], F, a.shape[1], DENSE_ACTS[act], float(limit), float(alpha),
+          _stream())
+
+
+def _expert_rows(w: torch.Tensor, what: str) -> int:
+    """Row stride of matrices [E, N, K] of integers whose rows are dense and follow one another."""
+    if w.dim() != 3 or w.dtype != torch.int8 or (w.shape[2] > 1 and w.stride(2) != 1)             or (w.shape[0] > 1 and w.stride(0) != w.shape[1] * w.stride(1)):
+        raise KernelError(f"{what}: int8 [E, N, K] with dense rows one after the other, got {tuple(w.shape)} {w.dtype} strides {w.stride()}")
+    return w.stride(1)
+
+
+def moe_experts_int8(x: torch.Tensor, w_gate_up: torch.Tensor, gate_up_scale: torch.Tensor, w_down: torch.Tensor, down_scale: torch.Tensor,
+                     routing, top: int, y: torch.Tensor, act_fn: str = "silu", weight_on: str = "input", limit: float = 0.0,
+                     alpha: float = 1.0) -> None:
+    """moe_experts() in 8-bit integers: y[t, k, :] for every chosen (token, expert) pair.  w_gate_up int8 [E, 2F, D] (without a gate,
+    act_fn "relu_squared", [E, F, D]) and w_down int8 [E, D, F] with their scales as weight_int8 makes them; x float32 or bfloat16
+    [T, D]; the activation between the products is rounded to integers from its 32-bit values.  y float32 or bfloat16
+    [T, top, D].  routing: what moe_route() or moe_route_tables() returned (for any number of rows a tile)."""
+    if act_fn not in MOE_ACTS or weight_on not in ("input", "output"):
+        raise KernelError(f"moe_experts_int8: unknown activation '{act_fn}' or weight placement '{weight_on}'")
+    _gpu(x, w_gate_up, gate_up_scale, w_down, down_scale, y)
+    ids, wts, order, offsets = routing[:4]
+    T, D = x.shape
+    E, N, _ = w_gate_up.shape
+    F = w_down.shape[-1]
+    ld_gu, ld_d = _expert_rows(w_gate_up, "moe_experts_int8 gate and up"), _expert_rows(w_down, "moe_experts_int8 down")
+    if N != (F if act_fn in UNGATED_ACTS else 2 * F) or w_gate_up.shape[2] != D or tuple(w_down.shape) != (E, D, F):
+        raise KernelError(f"moe_experts_int8: shapes x{tuple(x.shape)} w_gate_up{tuple(w_gate_up.shape)} w_down{tuple(w_down.shape)} do not agree")
+    if not (1 <= D <= INT8_MAX_K and 1 <= F <= INT8_MAX_K):
+        raise KernelError(f"moe_experts_int8: rows of {D} and {F} values; the sums are exact for 1 to {INT8_MAX_K}")
+    if weight_on == "input" and act_fn in UNGATED_ACTS:
+        raise KernelError("moe_experts_int8: an expert without a gate is not linear before its activation: the weight goes on its output")
+    pairs = T * top
+    if ids.numel() != pairs or order.numel() != pairs or offsets.numel() < E + 1:
+        raise KernelError(f"moe_experts_int8: a routing of {ids.numel()} pairs does not belong to {T} rows with {top} experts each of {E}")
+    _f32vec(gate_up_scale, E * N, "moe_experts_int8 gate and up scale")
+    _f32vec(down_scale, E * D, "moe_experts_int8 down scale")
+    if not y.is_contiguous() or y.numel() != pairs * D:
+        raise KernelError("moe_experts_int8: y must be contiguous [T, top, D]")
+    q = int8_empty(pairs, max(D, F), x.device)
+    work = torch.empty(pairs * (F + 1), dtype=torch.float32, device=x.device)          # the activation, the rows' scales
+    _note_owned(q, work)
+    _call("tlc_moe_experts_int8", x.data_ptr(), dtype_code(x.dtype), _rows(x, "moe_experts_int8 input"), w_gate_up.data_ptr(), ld_gu,
+          gate_up_scale.data_ptr(), w_down.data_ptr(), ld_d, down_scale.data_ptr(), order.data_ptr(), offsets.data_ptr(), wts.data_ptr(),
+          T, E, int(top), F, D, q.data_ptr(), q.stride(0), work.data_ptr() + 4 * pairs * F, work.data_ptr(), y.data_ptr(),
+          dtype_code(y.dtype), MOE_ACTS[act_fn], int(weight_on == "output"), float(limit), float(alpha), _stream())
 
 
 def qk_whole_norm(qkv: torch.Tensor, q_off: int, q_n: int, q_weight: torch.Tensor, k_off: int, k_n: int, k_weight: torch.Tensor,
