@@ -4,7 +4,9 @@
 //
 // Here: the product for operands in any layout, on the CUDA cores (dp4a: four products and their sum an instruction), tiles of 32 x
 // 64 results staged through shared memory 64 values of K at a time.
-#include "gemm_int8.cuh"
+#include "gemm_int8_tc.cuh"
+
+int tlc_int8_few(const Int8Args& p, int out_dtype, int nb, int sms, cudaStream_t stream);      // gemm_int8_few.cu
 
 namespace {
 
@@ -115,7 +117,24 @@ int run_tiles(const Int8Args& p, cudaStream_t stream) {
   return 0;
 }
 
+// Whether the copy engine takes the operands: rows that start on 16-byte boundaries, and gated weights whose rows come in eights.
+bool tensor_cores_take(const Int8Args& p) {
+  return ((uintptr_t)p.a | (uintptr_t)p.w | (uintptr_t)p.lda | (uintptr_t)p.ldw) % 16 == 0 && (p.mode != I8_GLU || p.N % 8 == 0) &&
+         tlc_error_words_here() != nullptr;
+}
+
 int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
+  static int sms = 0;
+  if (sms == 0) {
+    int dev = 0, n = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    sms = n > 0 ? n : 148;
+  }
+  if ((out_dtype == TLC_F32 || out_dtype == TLC_BF16) && tensor_cores_take(p)) {
+    const int rows = p.offsets ? (p.M + p.E - 1) / p.E * 3 / 2 : p.M;      // grouped: half as many again as a group has on average
+    return tlc_int8_few(p, out_dtype, rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, sms, stream);
+  }
   if (out_dtype == TLC_F32) return run_tiles<float>(p, stream);
   if (out_dtype == TLC_BF16) return run_tiles<__nv_bfloat16>(p, stream);
   return tlc_fail(-1, "linear_int8: unknown output dtype %d", out_dtype);
