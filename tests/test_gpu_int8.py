@@ -460,3 +460,55 @@ def test_weights_may_follow_at_once():
         again = torch.empty(8, 2048, device=DEV)
         ops.linear_int8(x, q, s, again)
         assert torch.equal(out, again)
+
+
+KERNELS = [(1, 0), (2, 16), (2, 32), (2, 64), (2, 128), (3, 128), (3, 256)]
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_every_kernel_gives_the_same_bits(kernel):
+    """The sums are exact, so a result does not depend on which kernel made it; it is compared with the CUDA cores'."""
+    g = gen(9)
+    for M, N, K in [(1, 200, 384), (40, 1000, 272), (129, 2050, 130), (515, 520, 1024), (300, 2048, 64)]:
+        a, sa, w, sw = integers(g, M, K), scales(g, M), integers(g, N, K), scales(g, N)
+        bias = normal(g, N)
+        w2, sw2 = integers(g, 2 * 136, K), scales(g, 2 * 136) * 0.1
+        for dtype in (torch.float32, torch.bfloat16):
+            old = normal(g, M, N, dtype=dtype)
+            got = []
+            for k in ((1, 0), kernel):
+                ops.linear_int8_kernel(*k)
+                try:
+                    outs = [torch.full((M, N), float("nan"), dtype=dtype, device=DEV), old.clone(), torch.full((M, 136), float("nan"), dtype=dtype, device=DEV)]
+                    ops.linear_int8(a, w, sw, outs[0], a_scale=sa, colbias=bias)
+                    ops.linear_int8(a, w, sw, outs[1], a_scale=sa, accumulate=True)
+                    ops.linear_swiglu_int8(a, w2, sw2, outs[2], a_scale=sa)
+                    got.append(outs)
+                finally:
+                    ops.linear_int8_kernel()
+            for x, y in zip(*got):
+                assert torch.equal(x, y)
+    ops.check_errors()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("T,E,top,F,D,act,weight_on", [(1, 4, 2, 64, 128, "silu", "input"), (200, 5, 3, 136, 272, "silu", "output"),
+                                                       (700, 3, 2, 72, 400, "silu", "input"), (33, 70, 4, 200, 128, "relu_squared", "output")])
+def test_every_kernel_gives_the_same_experts(kernel, T, E, top, F, D, act, weight_on):
+    g = gen(T)
+    x, logits = normal(g, T, D, dtype=torch.bfloat16), normal(g, T, E)
+    rows = F if act == "relu_squared" else 2 * F
+    wgu, sgu, wd, sd = integers(g, E, rows, D), scales(g, E, rows) * 0.2, integers(g, E, D, F), scales(g, E, D)
+    routing = ops.moe_route(logits, E, top, weights="softmax")
+    for dtype in (torch.float32, torch.bfloat16):
+        got = []
+        for k in ((1, 0), kernel):
+            ops.linear_int8_kernel(*k)
+            try:
+                y = torch.full((T, top, D), float("nan"), dtype=dtype, device=DEV)
+                ops.moe_experts_int8(x, wgu, sgu, wd, sd, routing, top, y, act_fn=act, weight_on=weight_on)
+                got.append(y)
+            finally:
+                ops.linear_int8_kernel()
+        assert torch.equal(*got)
+    ops.check_errors()

@@ -7,6 +7,7 @@
 #include "gemm_int8_tc.cuh"
 
 int tlc_int8_few(const Int8Args& p, int out_dtype, int nb, int sms, cudaStream_t stream);      // gemm_int8_few.cu
+int tlc_int8_wide(const Int8Args& p, int out_dtype, int nb, int pairs, cudaStream_t stream);   // gemm_int8_wide.cu
 
 namespace {
 
@@ -89,14 +90,11 @@ int8_tile_kernel(Int8Args p) {
     for (int j = 0; j < 4; j++) {
       const int n = n0 + c0 + 16 * j;
       if (n >= p.N) continue;
-      float v = int8_value(acc[0][i][j], rs, p.w_scale[w0 + n]);
-      if (p.colbias) v += p.colbias[n];
+      float v = int8_value(acc[0][i][j], rs, p.w_scale[w0 + n], p.colbias ? p.colbias[n] : 0.f);
       if (GLU || p.mode == I8_ACT) {
         float u = 0.f;
-        if (GLU) {
-          u = int8_value(acc[NW - 1][i][j], rs, p.w_scale[w0 + p.N + n]);
-          if (p.colbias) u += p.colbias[p.N + n];
-        }
+        if (GLU)
+          u = int8_value(acc[NW - 1][i][j], rs, p.w_scale[w0 + p.N + n], p.colbias ? p.colbias[p.N + n] : 0.f);
         v = moe_pair_act<false>(p.act, 0, p.limit, p.alpha, pw, v, u);
       } else if (p.mode == I8_ADD) {
         v += to_f32(o[n]);
@@ -123,6 +121,8 @@ bool tensor_cores_take(const Int8Args& p) {
          tlc_error_words_here() != nullptr;
 }
 
+int g_kernel = 0, g_rows = 0;        // test hook: which kernel, on tiles of how many activation rows
+
 int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
   static int sms = 0;
   if (sms == 0) {
@@ -131,9 +131,12 @@ int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     sms = n > 0 ? n : 148;
   }
-  if ((out_dtype == TLC_F32 || out_dtype == TLC_BF16) && tensor_cores_take(p)) {
+  if (g_kernel != 1 && (out_dtype == TLC_F32 || out_dtype == TLC_BF16) && tensor_cores_take(p)) {
     const int rows = p.offsets ? (p.M + p.E - 1) / p.E * 3 / 2 : p.M;      // grouped: half as many again as a group has on average
-    return tlc_int8_few(p, out_dtype, rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, sms, stream);
+    const int pairs = tlc_linear_pairs();
+    if (g_kernel == 3 ? pairs > 0 : g_kernel == 0 && rows > 128 && pairs > 0)
+      return tlc_int8_wide(p, out_dtype, g_kernel == 3 ? g_rows : 256, pairs, stream);
+    return tlc_int8_few(p, out_dtype, g_kernel == 2 ? g_rows : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, sms, stream);
   }
   if (out_dtype == TLC_F32) return run_tiles<float>(p, stream);
   if (out_dtype == TLC_BF16) return run_tiles<__nv_bfloat16>(p, stream);
@@ -141,6 +144,16 @@ int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
 }
 
 }  // namespace
+
+// Test hook: 0 = chosen by the sizes; 1 = the CUDA cores; 2 = tiles of 128 weight rows and 16, 32, 64 or 128 activation rows; 3 = pairs of
+// blocks on 256 weight rows and 128 or 256 activation rows, wherever they take the operands.
+extern "C" int tlc_linear_int8_kernel(int kernel, int rows) {
+  TLC_REQUIRE(kernel == 0 || kernel == 1 || (kernel == 2 && (rows == 16 || rows == 32 || rows == 64 || rows == 128)) ||
+              (kernel == 3 && (rows == 128 || rows == 256)), "linear_int8: there is no kernel %d with tiles of %d rows", kernel, rows);
+  g_kernel = kernel;
+  g_rows = rows;
+  return 0;
+}
 
 extern "C" int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_scale, void* a_int8, int ld_int8, const void* w, int ldw,
                                const float* w_scale, void* out, int out_dtype, int ldo, const float* colbias, int accumulate, int M, int N,

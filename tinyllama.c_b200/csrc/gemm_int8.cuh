@@ -21,5 +21,8 @@ struct Int8Args {
 };
 enum { I8_PLAIN = 0, I8_ADD = 1, I8_ACT = 2, I8_GLU = 3 };
 
-// One result from its integer sum.  Both scales in 32 bits, one after the other: their product alone may leave the range.
-__device__ __forceinline__ float int8_value(int sum, float row_scale, float col_scale) { return __int2float_rn(sum) * row_scale * col_scale; }
+// One result from its integer sum.  Both scales in 32 bits, one after the other: their product alone may leave the range.  The
+// operations are spelled out, so that every kernel rounds alike and a result does not depend on which one made it.
+__device__ __forceinline__ float int8_value(int sum, float row_scale, float col_scale, float bias) {
+  return __fmaf_rn(__fmul_rn(__int2float_rn(sum), row_scale), col_scale, bias);
+}

@@ -188,7 +188,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       for (int q = 0; q < 8; q++) { sum[0] += x[q].x; sum[1] += x[q].y; sum[2] += x[q].z; sum[3] += x[q].w; }
       float v[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = int8_value(sum[i], rs, cs[i]) + cb[i];
+      for (int i = 0; i < 4; i++) v[i] = int8_value(sum[i], rs, cs[i], cb[i]);
       if (GLU) {                                            // the up rows sit two lanes above their gate rows
 #pragma unroll
         for (int i = 0; i < 4; i++) {

@@ -1,0 +1,322 @@
+// Products in 8-bit integers of many rows on the 5th-generation tensor cores: pairs of blocks (clusters of two) on tiles of 256 weight
+// rows x NB = 128 or 256 activation rows, D[n, m] = sum_k w[n, k] a[m, k] by tcgen05.mma.cta_group::2 (kind::i8, M = 256, N = NB, K = 32).
+//
+// A pair keeps the tensor cores fed where a block alone cannot: each block stages its 128 weight rows and NB / 2 of the activation
+// rows (128 values of K a stage, copied by TMA with the 128-byte swizzle) and both halves serve both, so a block moves (128 + NB / 2)
+// rows in for 128 x NB products a value of K.  The block of rank 0 issues the products; each block finds its 128 weight rows of the
+// result in the lanes of its own tensor memory.  Two accumulators (2 x NB columns) let the results of one tile leave under the
+// products of the next; blocks are persistent and pairs walk the tiles.
+//
+// A lane holds one weight row, so its scale and bias stay in a register and neighbouring lanes write neighbouring columns of a row of
+// the result; 16-bit results are exchanged between neighbours so that a lane writes two of them at once.  Gated products have the
+// gate and up rows of 8 features in neighbouring groups of 8 lanes (load_weights): of two activation rows the gate's lanes finish
+// one and the up projection's lanes the other.
+//
+// Waits are bounded (codes 55-59); after one that ran out both blocks of a pair go to their common end.
+#include "gemm_int8_tc.cuh"
+#include <algorithm>
+#include <atomic>
+
+namespace {
+
+constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;       // loader warp, issuer warp, the results' warps (two a quarter of the lanes)
+
+template <int NB> struct Wide {
+  static constexpr int STAGES = NB == 256 ? 6 : 8;
+  static constexpr int W_BYTES = I8_ROWS * I8_K, X_BYTES = NB / 2 * I8_K;
+  static constexpr int TILES = STAGES * (W_BYTES + X_BYTES);
+  static constexpr int N_BARS = 2 * STAGES + 4;
+  static constexpr int TOTAL = TILES + N_BARS * 8 + 32 + 1024;
+};
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename TO, int NB, bool GLU, bool GROUPED>
+__global__ void __launch_bounds__(THREADS, 1)
+int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Int8Args p,
+                 int n_tiles, ErrWords* err) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  using S = Wide<NB>;
+  constexpr int STAGES = S::STAGES;
+  extern __shared__ uint8_t wide_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)wide_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* x_tiles = smem + STAGES * S::W_BYTES;
+  uint64_t* bars = (uint64_t*)(smem + S::TILES);
+  uint32_t* tmem_slot = (uint32_t*)(bars + S::N_BARS);
+  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+  const uint32_t acc_full0 = smem_u32(bars + 2 * STAGES), acc_empty0 = smem_u32(bars + 2 * STAGES + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long wait_limit = mbar_wait_limit(err);
+  const uint32_t rank = cluster_rank();
+  const int walker = (int)blockIdx.x >> 1, walkers = (int)gridDim.x >> 1;
+  const int num_k = (p.K + I8_K - 1) / I8_K;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+    for (int s = 0; s < 2; s++) { mbar_init(acc_full0 + 8 * s, 1); mbar_init(acc_empty0 + 8 * s, 2 * EPI_WARPS); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * NB) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cluster_sync();                                       // the other block's mbarriers are initialised too
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+
+  // Tiles: without groups the activation rows' tiles run fastest (pairs that run together share weights in the L2), with them the
+  // weight rows' (a group has few tiles of activation rows).
+  const int* offsets = p.offsets;
+  const int m_tiles = GROUPED ? 1 : (p.M + NB - 1) / NB;
+  int total = m_tiles * n_tiles;
+  if (GROUPED) {
+    tlc_wait(offsets);
+    int tiles = 0;
+    for (int e = lane; e < p.E; e += 32) tiles += (offsets[e + 1] - offsets[e] + NB - 1) / NB;
+    total = __reduce_add_sync(0xffffffffu, tiles) * n_tiles;
+  }
+  auto place = [&](int tile, int* group, int* row0, int* rows) -> int {      // ... and the tile's index along the weight rows
+    if constexpr (GROUPED) {
+      *group = 0; *row0 = 0; *rows = 0;
+      int8_group_tile(tile / n_tiles, NB, offsets, p.E, group, row0, rows);
+      return tile % n_tiles;
+    } else {
+      *group = 0;
+      *row0 = tile % m_tiles * NB;
+      *rows = min(NB, p.M - *row0);
+      return tile / m_tiles;
+    }
+  };
+
+  if (warp == 0) {                                      // ---- copies (one lane issues them) ----
+    int it = 0;
+    bool ok = true, waited = GROUPED;
+    // a pair's copies count on the mbarriers of the block of rank 0, whose issuer waits for them
+    const uint32_t full_bar0 = cluster_address(full0, 0);
+    int pending = 0;                                    // first stages whose activations are held back until the kernel before is through
+    const int first = min(STAGES, num_k);               // (all of them in the first tile)
+    for (int tile = walker; tile < total && ok; tile += walkers) {
+      int group, row0, rows;
+      const int n0 = place(tile, &group, &row0, &rows) * 2 * I8_ROWS + (int)rank * I8_ROWS;
+      const int m0 = row0 + (int)rank * (NB / 2);
+      if (lane == 0) {
+        for (int k = 0; k < num_k; k++, it++) {
+          const int s = it % STAGES;
+          ok = mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1, err, 55, wait_limit);
+          if (!ok) break;
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (S::W_BYTES + S::X_BYTES));
+          load_weights<GLU, true>(smem_u32(smem + s * S::W_BYTES), &map_w, full_bar0 + 8 * s, k * I8_K, n0, group);
+          if (!waited) {
+            pending++;
+            if (pending < first) continue;
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            waited = true;
+            for (int j = 0; j < pending; j++)
+              tma_load_2d_pair(smem_u32(x_tiles + j * S::X_BYTES), &map_x, full_bar0 + 8 * j, j * I8_K, m0);
+            continue;
+          }
+          tma_load_2d_pair(smem_u32(x_tiles + s * S::X_BYTES), &map_x, full_bar0 + 8 * s, k * I8_K, m0);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      it = __shfl_sync(0xffffffffu, it, 0);
+    }
+    if (lane == 0 && rank == 0 && (!ok || *(volatile int*)&err->flag != 0)) {
+      // something went wrong: let the copies still in flight land (a pair's count on these mbarriers)
+      for (int i = max(0, it - STAGES); i < it; i++)
+        mbar_wait(full0 + 8 * (i % STAGES), (i / STAGES) & 1, err, 56, wait_limit);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {                       // ---- products ----
+      constexpr uint32_t idesc = int8_desc(2 * I8_ROWS, NB);
+      int it = 0, local = 0;
+      bool ok = true;
+      for (int tile = walker; tile < total && ok; tile += walkers, local++) {
+        const int as = local & 1;
+        ok = mbar_wait(acc_empty0 + 8 * as, ((local >> 1) & 1) ^ 1, err, 57, wait_limit);     // both blocks have taken this half out
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem + (uint32_t)(as * NB);
+        for (int k = 0; k < num_k; k++, it++) {
+          const int s = it % STAGES;
+          ok = mbar_wait(full0 + 8 * s, (it / STAGES) & 1, err, 58, wait_limit);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t w_addr = smem_u32(smem + s * S::W_BYTES), x_addr = smem_u32(x_tiles + s * S::X_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < I8_K / I8_MMA_K; kk++)
+            int8_mma_pair(d, smem_desc(w_addr + kk * I8_MMA_K), smem_desc(x_addr + kk * I8_MMA_K), idesc, (k > 0 || kk > 0) ? 1u : 0u);
+          umma_commit_pair(empty0 + 8 * s);             // the slot is free in both blocks once these products have read it
+        }
+        if (ok) umma_commit_pair(acc_full0 + 8 * as);
+      }
+    }
+  } else {                                              // ---- results ----
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int row = quarter * 32 + lane;                // weight row of the block's tile
+    constexpr int CHUNKS = NB / 64;                     // pieces of 32 activation rows a warp takes
+    int local = 0;
+    bool ok = true;
+    const float* a_scale = p.a_scale;
+    const int* order = p.order;
+    const float* wts = p.wts;
+    TO* out = reinterpret_cast<TO*>(p.out);
+    tlc_wait(out, a_scale, order, wts);                 // `out` may still be read or written by the kernel before
+    const bool two = sizeof(TO) == 2 && (uintptr_t)out % 4 == 0 && p.ldo % 2 == 0;      // two 16-bit results at once
+    for (int tile = walker; tile < total && ok; tile += walkers, local++) {
+      const int as = local & 1;
+      int group, row0, rows;
+      const int n0 = place(tile, &group, &row0, &rows) * 2 * I8_ROWS + (int)rank * I8_ROWS;
+      const bool is_up = GLU && (lane & 8);
+      const int col = GLU ? (n0 >> 1) + ((row >> 4) << 3) + (row & 7) : n0 + row;        // column of the result
+      const bool in = col < p.N;
+      const size_t at = (size_t)group * p.w_rows + (is_up ? p.N : 0) + col;
+      const float cs = in ? p.w_scale[at] : 0.f, cb = in && p.colbias ? p.colbias[(is_up ? p.N : 0) + col] : 0.f;
+      float rs[CHUNKS], pw[CHUNKS];                     // of activation row `lane` of every piece
+      int to[CHUNKS];
+#pragma unroll
+      for (int c = 0; c < CHUNKS; c++) {
+        const int m = (half * CHUNKS + c) * 32 + lane;
+        const bool there = m < rows;
+        rs[c] = there ? a_scale[row0 + m] : 0.f;
+        to[c] = row0 + m;
+        pw[c] = 1.0f;
+        if (GROUPED && there) {
+          const int pair = order[row0 + m];
+          if (p.scatter) to[c] = pair;
+          if (p.w_out) rs[c] *= wts[pair];
+          if (p.w_in) pw[c] = wts[pair];
+        }
+      }
+      ok = mbar_wait(acc_full0 + 8 * as, (local >> 1) & 1, err, 59, wait_limit);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+      for (int c = 0; c < CHUNKS; c++) {
+        const int m0 = (half * CHUNKS + c) * 32;
+        if (m0 >= rows) break;
+        uint32_t r[32];
+        tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * NB + m0), r);
+        auto value = [&](int j) { return int8_value((int)r[j], __shfl_sync(0xffffffffu, rs[c], j), cs, cb); };
+        auto target = [&](int j) { return out + (size_t)(GROUPED ? __shfl_sync(0xffffffffu, to[c], j) : row0 + m0 + j) * p.ldo; };
+        if constexpr (GLU) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            // rows j, j + 1 -> y0 (the gate's lanes the first, the up projection's the second), rows j + 2, j + 3 -> y1
+            float y[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const float v0 = value(j + 2 * h), v1 = value(j + 2 * h + 1);
+              const float other = __shfl_xor_sync(0xffffffffu, is_up ? v0 : v1, 8);
+              const float w0 = GROUPED ? __shfl_sync(0xffffffffu, pw[c], j + 2 * h) : 1.0f, w1 = GROUPED ? __shfl_sync(0xffffffffu, pw[c], j + 2 * h + 1) : 1.0f;
+              y[h] = moe_pair_act<false>(p.act, 0, p.limit, p.alpha, is_up ? w1 : w0, is_up ? other : v0, is_up ? v1 : other);
+            }
+            const int mine = is_up ? 1 : 0;
+            if (two) {                                  // even lanes finish y0's row, odd lanes y1's
+              const float other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? y[0] : y[1], 1);
+              TO* t0 = target(j); TO* t1 = target(j + 1); TO* t2 = target(j + 2); TO* t3 = target(j + 3);
+              TO* t = (lane & 1) ? (mine ? t3 : t2) : (mine ? t1 : t0);
+              const int m = m0 + j + mine + 2 * (lane & 1);
+              if (in && m < rows)                       // (F is a multiple of 8: both columns are there)
+                *reinterpret_cast<uint32_t*>(t + (col & ~1)) = (lane & 1) ? pack2(other, y[1]) : pack2(y[0], other);
+            } else {
+#pragma unroll
+              for (int h = 0; h < 2; h++) {
+                TO* t0 = target(j + 2 * h); TO* t1 = target(j + 2 * h + 1);
+                if (in && m0 + j + 2 * h + mine < rows) (mine ? t1 : t0)[col] = from_f32<TO>(y[h]);
+              }
+            }
+          }
+        } else if (two && p.mode == I8_PLAIN) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {             // even lanes write row j, odd lanes row j + 1, two columns each
+            const float v0 = value(j), v1 = value(j + 1);
+            const float other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? v0 : v1, 1);
+            TO* t0 = target(j); TO* t1 = target(j + 1);
+            TO* t = ((lane & 1) ? t1 : t0) + (col & ~1);
+            if (m0 + j + (lane & 1) < rows) {
+              if ((col | 1) < p.N) *reinterpret_cast<uint32_t*>(t) = (lane & 1) ? pack2(other, v1) : pack2(v0, other);
+              else if ((col & ~1) < p.N) *t = from_f32<TO>((lane & 1) ? other : v0);      // the last column alone
+            }
+          }
+        } else {
+          float old[32];
+          if (p.mode == I8_ADD) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              const TO* t = target(j);
+              old[j] = in && m0 + j < rows ? to_f32(t[col]) : 0.f;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j++) {
+            float v = value(j);
+            TO* t = target(j);
+            if (p.mode == I8_ACT) v = moe_pair_act<false>(p.act, 0, p.limit, p.alpha, GROUPED ? __shfl_sync(0xffffffffu, pw[c], j) : 1.0f, v, 0.f);
+            else if (p.mode == I8_ADD) v += old[j];
+            if (in && m0 + j < rows) t[col] = from_f32<TO>(v);
+          }
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(cluster_address(acc_empty0 + 8 * as, 0));        // the issuer's block
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cluster_sync();                                       // neither block's memories are in use by the other any more
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NB) : "memory");
+}
+
+template <typename TO, int NB, bool GLU, bool GROUPED>
+int launch(const Int8Args& p, long long tiles, int n_tiles, int pairs, cudaStream_t stream) {
+  using S = Wide<NB>;
+  static std::atomic<bool> set{false};
+  if (!set) {
+    if (cudaFuncSetAttribute(int8_wide_kernel<TO, NB, GLU, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL) != cudaSuccess)
+      return tlc_fail(-2, "linear_int8: cannot reserve %d bytes of shared memory", S::TOTAL);
+    set = true;
+  }
+  CUtensorMap mw, mx;
+  if (int rc = tlc_int8_maps(p, NB / 2, &mw, &mx)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, pairs));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = S::TOTAL;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g_tlc_pdl ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, int8_wide_kernel<TO, NB, GLU, GROUPED>, mw, mx, p, n_tiles, tlc_error_words());
+  TLC_CHECK_LAUNCH("linear_int8 (pairs)");
+  return 0;
+}
+
+template <typename TO, int NB>
+int launch_of(const Int8Args& p, int pairs, cudaStream_t stream) {
+  const int n_tiles = ((p.mode == I8_GLU ? 2 : 1) * p.N + 2 * I8_ROWS - 1) / (2 * I8_ROWS);
+  const long long tiles = (long long)n_tiles * (p.offsets ? p.M / NB + std::min(p.M, p.E) : (p.M + NB - 1) / NB);    // (grouped: an upper bound)
+  if (p.mode == I8_GLU)
+    return p.offsets ? launch<TO, NB, true, true>(p, tiles, n_tiles, pairs, stream) : launch<TO, NB, true, false>(p, tiles, n_tiles, pairs, stream);
+  return p.offsets ? launch<TO, NB, false, true>(p, tiles, n_tiles, pairs, stream) : launch<TO, NB, false, false>(p, tiles, n_tiles, pairs, stream);
+}
+
+}  // namespace
+
+// nb: activation rows of a tile (128 or 256); pairs: how many pairs of blocks run at once.
+int tlc_int8_wide(const Int8Args& p, int out_dtype, int nb, int pairs, cudaStream_t stream) {
+  if (nb == 128) return out_dtype == TLC_F32 ? launch_of<float, 128>(p, pairs, stream) : launch_of<__nv_bfloat16, 128>(p, pairs, stream);
+  return out_dtype == TLC_F32 ? launch_of<float, 256>(p, pairs, stream) : launch_of<__nv_bfloat16, 256>(p, pairs, stream);
+}

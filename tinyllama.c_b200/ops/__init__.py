@@ -162,6 +162,7 @@ _SIGNATURES = {
     "tlc_moe_down": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
     "tlc_rows_int8": (_i, [_vp, _i, _i, _i, _i, _vp, _f, _vp, _i, _vp, _vp, _i, _i, _vp]),
     "tlc_linear_int8": (_i, [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _f, _f, _vp]),
+    "tlc_linear_int8_kernel": (_i, [_i, _i]),
     "tlc_moe_experts_int8": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i,
                                   _i, _i, _f, _f, _vp]),
     "tlc_argmax": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
@@ -1565,6 +1566,14 @@ def moe_identity(x: torch.Tensor, routing, top: int, n_experts: int, y: torch.Te
 # functions here make them (int8_empty), which the tensor-core kernels need; operands in any other layout are multiplied on the CUDA
 # cores.
 INT8_MAX_K = 131071                      # 128 * 128 * K < 2^31: the sums of products stay exact in 32 bits
+
+
+def linear_int8_kernel(kernel: int = 0, rows: int = 0) -> None:
+    """Which kernel the products in 8-bit integers take where it takes the operands: 0 chosen by the sizes, 1 the CUDA cores, 2 tiles of
+    128 weight rows and `rows` (16, 32, 64 or 128) activation rows, 3 pairs of blocks on tiles of 128 or 256.  For tests."""
+    lib = library()
+    if lib.tlc_linear_int8_kernel(int(kernel), int(rows)) != 0:
+        raise KernelError(f"linear_int8_kernel: {lib.tlc_last_error().decode()}")
 
 
 def int8_empty(rows: int, k: int, device) -> torch.Tensor:
