@@ -26,7 +26,7 @@ template <int NB> struct Wide {
   static constexpr int W_BYTES = I8_ROWS * I8_K, X_BYTES = NB / 2 * I8_K;
   static constexpr int TILES = STAGES * (W_BYTES + X_BYTES);
   static constexpr int N_BARS = 2 * STAGES + 4;
-  static constexpr int TOTAL = TILES + N_BARS * 8 + 32 + 1024;
+  static constexpr int TOTAL = TILES + N_BARS * 8 + 16 + EPI_WARPS * NB / 2 * 4 + 16 + 1024;      // ..., where tensor memory lies, scales
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -168,6 +168,7 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     TO* out = reinterpret_cast<TO*>(p.out);
     tlc_wait(out, a_scale, order, wts);                 // `out` may still be read or written by the kernel before
     const bool two = sizeof(TO) == 2 && (uintptr_t)out % 4 == 0 && p.ldo % 2 == 0;      // two 16-bit results at once
+    float* scales = reinterpret_cast<float*>(tmem_slot + 4) + (warp - 2) * (NB / 2);    // this warp's activation rows'
     for (int tile = walker; tile < total && ok; tile += walkers, local++) {
       const int as = local & 1;
       int group, row0, rows;
@@ -177,89 +178,112 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       const bool in = col < p.N;
       const size_t at = (size_t)group * p.w_rows + (is_up ? p.N : 0) + col;
       const float cs = in ? p.w_scale[at] : 0.f, cb = in && p.colbias ? p.colbias[(is_up ? p.N : 0) + col] : 0.f;
-      float rs[CHUNKS], pw[CHUNKS];                     // of activation row `lane` of every piece
+      float pw[CHUNKS];                                 // of activation row `lane` of every piece
       int to[CHUNKS];
+      __syncwarp();                                     // (the last tile's scales have been read)
 #pragma unroll
       for (int c = 0; c < CHUNKS; c++) {
         const int m = (half * CHUNKS + c) * 32 + lane;
         const bool there = m < rows;
-        rs[c] = there ? a_scale[row0 + m] : 0.f;
+        float rs = there ? a_scale[row0 + m] : 0.f;
         to[c] = row0 + m;
         pw[c] = 1.0f;
         if (GROUPED && there) {
           const int pair = order[row0 + m];
           if (p.scatter) to[c] = pair;
-          if (p.w_out) rs[c] *= wts[pair];
+          if (p.w_out) rs *= wts[pair];
           if (p.w_in) pw[c] = wts[pair];
         }
+        scales[c * 32 + lane] = rs;
       }
+      __syncwarp();
       ok = mbar_wait(acc_full0 + 8 * as, (local >> 1) & 1, err, 59, wait_limit);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
       for (int c = 0; c < CHUNKS; c++) {
-        const int m0 = (half * CHUNKS + c) * 32;
-        if (m0 >= rows) break;
+        const int m0 = (half * CHUNKS + c) * 32, left = rows - m0;               // activation rows of this piece
+        if (left <= 0) break;
         uint32_t r[32];
         tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * NB + m0), r);
-        auto value = [&](int j) { return int8_value((int)r[j], __shfl_sync(0xffffffffu, rs[c], j), cs, cb); };
-        auto target = [&](int j) { return out + (size_t)(GROUPED ? __shfl_sync(0xffffffffu, to[c], j) : row0 + m0 + j) * p.ldo; };
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 rs = *reinterpret_cast<const float4*>(scales + c * 32 + j);
+          v[j] = int8_value((int)r[j], rs.x, cs, cb);
+          v[j + 1] = int8_value((int)r[j + 1], rs.y, cs, cb);
+          v[j + 2] = int8_value((int)r[j + 2], rs.z, cs, cb);
+          v[j + 3] = int8_value((int)r[j + 3], rs.w, cs, cb);
+        }
+        // where this lane writes: row `mine` of every group of rows, found once and moved on (grouped: by the row's own index)
+        auto target = [&](const int j, const int mine) {
+          return GROUPED ? out + (size_t)__shfl_sync(0xffffffffu, to[c], j + mine) * p.ldo
+                         : out + (size_t)(row0 + m0 + mine) * p.ldo + (unsigned)(j * p.ldo);
+        };
         if constexpr (GLU) {
+          auto gated = [&](const auto act_of) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            // rows j, j + 1 -> y0 (the gate's lanes the first, the up projection's the second), rows j + 2, j + 3 -> y1
-            float y[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const float v0 = value(j + 2 * h), v1 = value(j + 2 * h + 1);
-              const float other = __shfl_xor_sync(0xffffffffu, is_up ? v0 : v1, 8);
-              const float w0 = GROUPED ? __shfl_sync(0xffffffffu, pw[c], j + 2 * h) : 1.0f, w1 = GROUPED ? __shfl_sync(0xffffffffu, pw[c], j + 2 * h + 1) : 1.0f;
-              y[h] = moe_pair_act<false>(p.act, 0, p.limit, p.alpha, is_up ? w1 : w0, is_up ? other : v0, is_up ? v1 : other);
-            }
-            const int mine = is_up ? 1 : 0;
-            if (two) {                                  // even lanes finish y0's row, odd lanes y1's
-              const float other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? y[0] : y[1], 1);
-              TO* t0 = target(j); TO* t1 = target(j + 1); TO* t2 = target(j + 2); TO* t3 = target(j + 3);
-              TO* t = (lane & 1) ? (mine ? t3 : t2) : (mine ? t1 : t0);
-              const int m = m0 + j + mine + 2 * (lane & 1);
-              if (in && m < rows)                       // (F is a multiple of 8: both columns are there)
-                *reinterpret_cast<uint32_t*>(t + (col & ~1)) = (lane & 1) ? pack2(other, y[1]) : pack2(y[0], other);
-            } else {
+            for (int j = 0; j < 32; j += 4) {
+              // rows j, j + 1 -> y0 (the gate's lanes the first, the up projection's the second), rows j + 2, j + 3 -> y1
+              float y[2];
 #pragma unroll
               for (int h = 0; h < 2; h++) {
-                TO* t0 = target(j + 2 * h); TO* t1 = target(j + 2 * h + 1);
-                if (in && m0 + j + 2 * h + mine < rows) (mine ? t1 : t0)[col] = from_f32<TO>(y[h]);
+                const float v0 = v[j + 2 * h], v1 = v[j + 2 * h + 1];
+                const float other = __shfl_xor_sync(0xffffffffu, is_up ? v0 : v1, 8);
+                const float w = GROUPED ? __shfl_sync(0xffffffffu, pw[c], j + 2 * h + (is_up ? 1 : 0)) : 1.0f;
+                y[h] = act_of(w, is_up ? other : v0, is_up ? v1 : other);
+              }
+              if (two) {                                // even lanes finish y0's row, odd lanes y1's
+                const int mine = (is_up ? 1 : 0) + 2 * (lane & 1);
+                const float other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? y[0] : y[1], 1);
+                TO* t = target(j, mine) + (col & ~1);
+                if (in && j + mine < left)              // (F is a multiple of 8: both columns are there)
+                  *reinterpret_cast<uint32_t*>(t) = (lane & 1) ? pack2(other, y[1]) : pack2(y[0], other);
+              } else {
+                const int mine = is_up ? 1 : 0;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                  TO* t = target(j + 2 * h, mine) + col;
+                  if (in && j + 2 * h + mine < left) *t = from_f32<TO>(y[h]);
+                }
               }
             }
-          }
+          };
+          if (p.act == TLC_ACT_SILU) gated([&](float w, float g, float u) { return GROUPED ? moe_pair_act<true>(TLC_ACT_SILU, 0, 0.f, 1.f, w, g, u) : silu_quick(g) * u; });
+          else gated([&](float w, float g, float u) { return moe_pair_act<true>(p.act, 0, p.limit, p.alpha, w, g, u); });
         } else if (two && p.mode == I8_PLAIN) {
+          const int mine = lane & 1;                    // even lanes write row j, odd lanes row j + 1, two columns each
+          const bool both = (col | 1) < p.N, one = (col & ~1) < p.N;
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {             // even lanes write row j, odd lanes row j + 1, two columns each
-            const float v0 = value(j), v1 = value(j + 1);
-            const float other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? v0 : v1, 1);
-            TO* t0 = target(j); TO* t1 = target(j + 1);
-            TO* t = ((lane & 1) ? t1 : t0) + (col & ~1);
-            if (m0 + j + (lane & 1) < rows) {
-              if ((col | 1) < p.N) *reinterpret_cast<uint32_t*>(t) = (lane & 1) ? pack2(other, v1) : pack2(v0, other);
-              else if ((col & ~1) < p.N) *t = from_f32<TO>((lane & 1) ? other : v0);      // the last column alone
+          for (int j = 0; j < 32; j += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, mine ? v[j] : v[j + 1], 1);
+            TO* t = target(j, mine) + (col & ~1);
+            if (j + mine < left) {
+              if (both) *reinterpret_cast<uint32_t*>(t) = mine ? pack2(other, v[j + 1]) : pack2(v[j], other);
+              else if (one) *t = from_f32<TO>(mine ? other : v[j]);              // the last column alone
             }
           }
         } else {
-          float old[32];
-          if (p.mode == I8_ADD) {
+          if (p.mode == I8_ACT) {
 #pragma unroll
             for (int j = 0; j < 32; j++) {
-              const TO* t = target(j);
-              old[j] = in && m0 + j < rows ? to_f32(t[col]) : 0.f;
+              const float w = GROUPED ? __shfl_sync(0xffffffffu, pw[c], j) : 1.0f;
+              v[j] = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, w, v[j], 0.f);
             }
+          } else if (p.mode == I8_ADD) {
+            float old[32];                              // (all in flight before the first is added)
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              const TO* t = target(j, 0) + col;
+              old[j] = in && j < left ? to_f32(*t) : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] += old[j];
           }
 #pragma unroll
           for (int j = 0; j < 32; j++) {
-            float v = value(j);
-            TO* t = target(j);
-            if (p.mode == I8_ACT) v = moe_pair_act<false>(p.act, 0, p.limit, p.alpha, GROUPED ? __shfl_sync(0xffffffffu, pw[c], j) : 1.0f, v, 0.f);
-            else if (p.mode == I8_ADD) v += old[j];
-            if (in && m0 + j < rows) t[col] = from_f32<TO>(v);
+            TO* t = target(j, 0) + col;
+            if (in && j < left) *t = from_f32<TO>(v[j]);
           }
         }
       }
