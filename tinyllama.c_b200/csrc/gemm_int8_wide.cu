@@ -19,14 +19,14 @@
 
 namespace {
 
-constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;       // loader warp, issuer warp, the results' warps (two a quarter of the lanes)
+constexpr int EPI_WARPS = 16, THREADS = 64 + 32 * EPI_WARPS;      // loader warp, issuer warp, the results' warps (four a quarter of the lanes)
 
 template <int NB> struct Wide {
   static constexpr int STAGES = NB == 256 ? 6 : 8;
   static constexpr int W_BYTES = I8_ROWS * I8_K, X_BYTES = NB / 2 * I8_K;
   static constexpr int TILES = STAGES * (W_BYTES + X_BYTES);
   static constexpr int N_BARS = 2 * STAGES + 4;
-  static constexpr int TOTAL = TILES + N_BARS * 8 + 16 + EPI_WARPS * NB / 2 * 4 + 16 + 1024;      // ..., where tensor memory lies, scales
+  static constexpr int TOTAL = TILES + N_BARS * 8 + 16 + 4 * NB * 3 * 4 + 16 + 1024;      // ..., where tensor memory lies, scales
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -157,9 +157,9 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       }
     }
   } else {                                              // ---- results ----
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, share = (warp - 2) >> 2;
     const int row = quarter * 32 + lane;                // weight row of the block's tile
-    constexpr int CHUNKS = NB / 64;                     // pieces of 32 activation rows a warp takes
+    constexpr int CHUNKS = NB / (8 * EPI_WARPS), MINE = 32 * CHUNKS;      // pieces of 32 activation rows a warp takes
     int local = 0;
     bool ok = true;
     const float* a_scale = p.a_scale;
@@ -168,7 +168,10 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     TO* out = reinterpret_cast<TO*>(p.out);
     tlc_wait(out, a_scale, order, wts);                 // `out` may still be read or written by the kernel before
     const bool two = sizeof(TO) == 2 && (uintptr_t)out % 4 == 0 && p.ldo % 2 == 0;      // two 16-bit results at once
-    float* scales = reinterpret_cast<float*>(tmem_slot + 4) + (warp - 2) * (NB / 2);    // this warp's activation rows'
+    // this warp's activation rows: scales, where their results go, the pairs' weights
+    float* scales = reinterpret_cast<float*>(tmem_slot + 4) + (warp - 2) * (MINE * (GROUPED ? 3 : 1));
+    int* to = reinterpret_cast<int*>(scales + MINE);
+    float* pw = scales + 2 * MINE;
     for (int tile = walker; tile < total && ok; tile += walkers, local++) {
       const int as = local & 1;
       int group, row0, rows;
@@ -178,21 +181,18 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       const bool in = col < p.N;
       const size_t at = (size_t)group * p.w_rows + (is_up ? p.N : 0) + col;
       const float cs = in ? p.w_scale[at] : 0.f, cb = in && p.colbias ? p.colbias[(is_up ? p.N : 0) + col] : 0.f;
-      float pw[CHUNKS];                                 // of activation row `lane` of every piece
-      int to[CHUNKS];
       __syncwarp();                                     // (the last tile's scales have been read)
 #pragma unroll
       for (int c = 0; c < CHUNKS; c++) {
-        const int m = (half * CHUNKS + c) * 32 + lane;
+        const int m = (share * CHUNKS + c) * 32 + lane;
         const bool there = m < rows;
         float rs = there ? a_scale[row0 + m] : 0.f;
-        to[c] = row0 + m;
-        pw[c] = 1.0f;
-        if (GROUPED && there) {
-          const int pair = order[row0 + m];
-          if (p.scatter) to[c] = pair;
-          if (p.w_out) rs *= wts[pair];
-          if (p.w_in) pw[c] = wts[pair];
+        if (GROUPED) {
+          const int pair = there ? order[row0 + m] : 0;
+          const float w = there ? wts[pair] : 0.f;
+          if (p.w_out) rs *= w;
+          to[c * 32 + lane] = p.scatter ? pair : row0 + m;
+          pw[c * 32 + lane] = p.w_in ? w : 1.0f;
         }
         scales[c * 32 + lane] = rs;
       }
@@ -200,9 +200,9 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       ok = mbar_wait(acc_full0 + 8 * as, (local >> 1) & 1, err, 59, wait_limit);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
+#pragma unroll 1                                        // (the code of one piece is long enough)
       for (int c = 0; c < CHUNKS; c++) {
-        const int m0 = (half * CHUNKS + c) * 32, left = rows - m0;               // activation rows of this piece
+        const int m0 = (share * CHUNKS + c) * 32, left = rows - m0;               // activation rows of this piece
         if (left <= 0) break;
         uint32_t r[32];
         tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * NB + m0), r);
@@ -217,7 +217,7 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
         // where this lane writes: row `mine` of every group of rows, found once and moved on (grouped: by the row's own index)
         auto target = [&](const int j, const int mine) {
-          return GROUPED ? out + (size_t)__shfl_sync(0xffffffffu, to[c], j + mine) * p.ldo
+          return GROUPED ? out + (size_t)to[c * 32 + j + mine] * p.ldo
                          : out + (size_t)(row0 + m0 + mine) * p.ldo + (unsigned)(j * p.ldo);
         };
         if constexpr (GLU) {
@@ -230,7 +230,7 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
               for (int h = 0; h < 2; h++) {
                 const float v0 = v[j + 2 * h], v1 = v[j + 2 * h + 1];
                 const float other = __shfl_xor_sync(0xffffffffu, is_up ? v0 : v1, 8);
-                const float w = GROUPED ? __shfl_sync(0xffffffffu, pw[c], j + 2 * h + (is_up ? 1 : 0)) : 1.0f;
+                const float w = GROUPED ? pw[c * 32 + j + 2 * h + (is_up ? 1 : 0)] : 1.0f;
                 y[h] = act_of(w, is_up ? other : v0, is_up ? v1 : other);
               }
               if (two) {                                // even lanes finish y0's row, odd lanes y1's
@@ -267,7 +267,7 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
           if (p.mode == I8_ACT) {
 #pragma unroll
             for (int j = 0; j < 32; j++) {
-              const float w = GROUPED ? __shfl_sync(0xffffffffu, pw[c], j) : 1.0f;
+              const float w = GROUPED ? pw[c * 32 + j] : 1.0f;
               v[j] = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, w, v[j], 0.f);
             }
           } else if (p.mode == I8_ADD) {
