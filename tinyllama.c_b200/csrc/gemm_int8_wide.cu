@@ -29,11 +29,6 @@ template <int NB> struct Wide {
   static constexpr int TOTAL = TILES + N_BARS * 8 + 16 + 4 * NB * 3 * 4 + 16 + 1024;      // ..., where tensor memory lies, scales
 };
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
 template <typename TO, int NB, bool GLU, bool GROUPED>
 __global__ void __launch_bounds__(THREADS, 1)
 int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Int8Args p,
@@ -159,7 +154,8 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   } else {                                              // ---- results ----
     const int quarter = warp & 3, share = (warp - 2) >> 2;
     const int row = quarter * 32 + lane;                // weight row of the block's tile
-    constexpr int CHUNKS = NB / (8 * EPI_WARPS), MINE = 32 * CHUNKS;      // pieces of 32 activation rows a warp takes
+    constexpr int CHUNKS = NB / (8 * EPI_WARPS), MINE = 32 * CHUNKS;      // activation rows a warp takes, 32 CHUNKS of them
+    constexpr int PIECE = 16;                           // ..., so many at a time
     int local = 0;
     bool ok = true;
     const float* a_scale = p.a_scale;
@@ -167,7 +163,6 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const float* wts = p.wts;
     TO* out = reinterpret_cast<TO*>(p.out);
     tlc_wait(out, a_scale, order, wts);                 // `out` may still be read or written by the kernel before
-    const bool two = sizeof(TO) == 2 && (uintptr_t)out % 4 == 0 && p.ldo % 2 == 0;      // two 16-bit results at once
     // this warp's activation rows: scales, where their results go, the pairs' weights
     float* scales = reinterpret_cast<float*>(tmem_slot + 4) + (warp - 2) * (MINE * (GROUPED ? 3 : 1));
     int* to = reinterpret_cast<int*>(scales + MINE);
@@ -200,89 +195,54 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       ok = mbar_wait(acc_full0 + 8 * as, (local >> 1) & 1, err, 59, wait_limit);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1                                        // (the code of one piece is long enough)
-      for (int c = 0; c < CHUNKS; c++) {
-        const int m0 = (share * CHUNKS + c) * 32, left = rows - m0;               // activation rows of this piece
+#pragma unroll 1                                        // (a piece's code stays near the scheduler)
+      for (int m1 = 0; m1 < MINE; m1 += PIECE) {
+        const int m0 = share * MINE + m1, left = rows - m0;                      // activation rows of this piece
         if (left <= 0) break;
-        uint32_t r[32];
-        tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * NB + m0), r);
-        float v[32];
+        uint32_t r[PIECE];
+        tmem_ldn(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * NB + m0), r);
+        float v[PIECE];
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 rs = *reinterpret_cast<const float4*>(scales + c * 32 + j);
+        for (int j = 0; j < PIECE; j += 4) {
+          const float4 rs = *reinterpret_cast<const float4*>(scales + m1 + j);
           v[j] = int8_value((int)r[j], rs.x, cs, cb);
           v[j + 1] = int8_value((int)r[j + 1], rs.y, cs, cb);
           v[j + 2] = int8_value((int)r[j + 2], rs.z, cs, cb);
           v[j + 3] = int8_value((int)r[j + 3], rs.w, cs, cb);
         }
-        // where this lane writes: row `mine` of every group of rows, found once and moved on (grouped: by the row's own index)
+        // where this lane writes row j + mine of the piece (grouped: by the row's own index)
+        TO* base = out + (size_t)(row0 + m0) * p.ldo + col;
         auto target = [&](const int j, const int mine) {
-          return GROUPED ? out + (size_t)to[c * 32 + j + mine] * p.ldo
-                         : out + (size_t)(row0 + m0 + mine) * p.ldo + (unsigned)(j * p.ldo);
+          return GROUPED ? out + (size_t)to[m1 + j + mine] * p.ldo + col : base + (unsigned)((j + mine) * p.ldo);
         };
         if constexpr (GLU) {
+          const int mine = is_up ? 1 : 0;
           auto gated = [&](const auto act_of) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              // rows j, j + 1 -> y0 (the gate's lanes the first, the up projection's the second), rows j + 2, j + 3 -> y1
-              float y[2];
-#pragma unroll
-              for (int h = 0; h < 2; h++) {
-                const float v0 = v[j + 2 * h], v1 = v[j + 2 * h + 1];
-                const float other = __shfl_xor_sync(0xffffffffu, is_up ? v0 : v1, 8);
-                const float w = GROUPED ? pw[c * 32 + j + 2 * h + (is_up ? 1 : 0)] : 1.0f;
-                y[h] = act_of(w, is_up ? other : v0, is_up ? v1 : other);
-              }
-              if (two) {                                // even lanes finish y0's row, odd lanes y1's
-                const int mine = (is_up ? 1 : 0) + 2 * (lane & 1);
-                const float other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? y[0] : y[1], 1);
-                TO* t = target(j, mine) + (col & ~1);
-                if (in && j + mine < left)              // (F is a multiple of 8: both columns are there)
-                  *reinterpret_cast<uint32_t*>(t) = (lane & 1) ? pack2(other, y[1]) : pack2(y[0], other);
-              } else {
-                const int mine = is_up ? 1 : 0;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                  TO* t = target(j + 2 * h, mine) + col;
-                  if (in && j + 2 * h + mine < left) *t = from_f32<TO>(y[h]);
-                }
-              }
+            for (int j = 0; j < PIECE; j += 2) {        // of rows j and j + 1 the gate's lanes finish the first, the up projection's the second
+              const float other = __shfl_xor_sync(0xffffffffu, is_up ? v[j] : v[j + 1], 8);
+              const float w = GROUPED ? pw[m1 + j + mine] : 1.0f;
+              const float y = act_of(w, is_up ? other : v[j], is_up ? v[j + 1] : other);
+              TO* t = target(j, mine);
+              if (in && j + mine < left) *t = from_f32<TO>(y);
             }
           };
           if (p.act == TLC_ACT_SILU) gated([&](float w, float g, float u) { return GROUPED ? moe_pair_act<true>(TLC_ACT_SILU, 0, 0.f, 1.f, w, g, u) : silu_quick(g) * u; });
           else gated([&](float w, float g, float u) { return moe_pair_act<true>(p.act, 0, p.limit, p.alpha, w, g, u); });
-        } else if (two && p.mode == I8_PLAIN) {
-          const int mine = lane & 1;                    // even lanes write row j, odd lanes row j + 1, two columns each
-          const bool both = (col | 1) < p.N, one = (col & ~1) < p.N;
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float other = __shfl_xor_sync(0xffffffffu, mine ? v[j] : v[j + 1], 1);
-            TO* t = target(j, mine) + (col & ~1);
-            if (j + mine < left) {
-              if (both) *reinterpret_cast<uint32_t*>(t) = mine ? pack2(other, v[j + 1]) : pack2(v[j], other);
-              else if (one) *t = from_f32<TO>(mine ? other : v[j]);              // the last column alone
-            }
-          }
         } else {
           if (p.mode == I8_ACT) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              const float w = GROUPED ? pw[c * 32 + j] : 1.0f;
-              v[j] = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, w, v[j], 0.f);
-            }
+            for (int j = 0; j < PIECE; j++) v[j] = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, GROUPED ? pw[m1 + j] : 1.0f, v[j], 0.f);
           } else if (p.mode == I8_ADD) {
-            float old[32];                              // (all in flight before the first is added)
+            float old[PIECE];                           // (all in flight before the first is added)
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              const TO* t = target(j, 0) + col;
-              old[j] = in && j < left ? to_f32(*t) : 0.f;
-            }
+            for (int j = 0; j < PIECE; j++) old[j] = in && j < left ? to_f32(*target(j, 0)) : 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] += old[j];
+            for (int j = 0; j < PIECE; j++) v[j] += old[j];
           }
 #pragma unroll
-          for (int j = 0; j < 32; j++) {
-            TO* t = target(j, 0) + col;
+          for (int j = 0; j < PIECE; j++) {
+            TO* t = target(j, 0);
             if (in && j < left) *t = from_f32<TO>(v[j]);
           }
         }
