@@ -183,6 +183,7 @@ extern "C" int tlc_moe_experts_int8(const void* x, int x_dtype, int ldx, const v
   const long long pairs = (long long)T * top;
   TLC_REQUIRE(T > 0 && top >= 1 && E >= 1 && F >= 1 && D >= 1 && F <= 131071 && D <= 131071 && pairs < (1 << 30),
               "moe_experts_int8: bad sizes T=%d E=%d top=%d F=%d D=%d", T, E, top, F, D);
+  TLC_REQUIRE(E <= TLC_INT8_GROUPS, "moe_experts_int8: %d experts (at most %d)", E, TLC_INT8_GROUPS);
   TLC_REQUIRE(ldgu >= D && ldd >= F && ldq >= D && ldq >= F, "moe_experts_int8: rows shorter than the sizes (ld %d %d %d)", ldgu, ldd, ldq);
   TLC_REQUIRE(act_code >= TLC_ACT_SILU && act_code <= TLC_ACT_RELU_SQUARED, "moe_experts_int8: unknown activation %d", act_code);
   // the chosen rows, sorted by expert, rounded; both products read their rows from q

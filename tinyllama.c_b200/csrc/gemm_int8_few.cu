@@ -23,7 +23,7 @@ template <int NB> struct Few {
   static constexpr int W_BYTES = I8_ROWS * I8_K, X_BYTES = NB * I8_K;
   static constexpr int TILES = STAGES * (W_BYTES + X_BYTES);
   static constexpr int N_BARS = 2 * STAGES + 1;
-  static constexpr int TOTAL = TILES + N_BARS * 8 + 32 + 1024;
+  static constexpr int TOTAL = TILES + N_BARS * 8 + 32 + 3 * NB * 4 + 1024;      // ..., where tensor memory lies, the rows' numbers
   static_assert(NB * I8_ROWS * 4 <= TILES, "the sums take the stages' place");
 };
 
@@ -50,6 +50,10 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   int* part = reinterpret_cast<int*>(smem);
   uint64_t* bars = (uint64_t*)(smem + S::TILES);
   uint32_t* tmem_slot = (uint32_t*)(bars + S::N_BARS);
+  // the tile's activation rows: scale, where the result goes, the pair's weight
+  float* row_scale = reinterpret_cast<float*>(tmem_slot + 4);
+  int* row_to = reinterpret_cast<int*>(row_scale + NB);
+  float* row_weight = row_scale + 2 * NB;
   const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), acc_full = smem_u32(bars + 2 * STAGES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -147,6 +151,19 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     const int* order = p.order;
     const float* wts = p.wts;
     tlc_wait(a_scale, out, order, wts);                     // `out` may still be read or written by the kernel before
+    if (row < min(rows, NB)) {
+      float rs = a_scale[row0 + row], w = 1.0f;
+      int to = row0 + row;
+      if (GROUPED) {
+        const int pair = order[row0 + row];
+        w = wts[pair];
+        if (p.w_out) rs *= w;
+        if (p.scatter) to = pair;
+      }
+      row_scale[row] = rs;
+      row_to[row] = to;
+      row_weight[row] = w;
+    }
     mbar_wait(acc_full, 0, err, 53, wait_limit);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -158,11 +175,10 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       for (int j = 0; j < CW; j++) part[(c * CW + j) * I8_ROWS + row] = n_k > 0 ? (int)r[j] : 0;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    if (split > 1) {                                        // every block's sums are in its shared memory
+    asm volatile("bar.sync 1, 128;" ::: "memory");          // the rows' numbers, and this block's sums
+    if (split > 1) {                                        // ... and those of the others of the cluster
       asm volatile("barrier.cluster.arrive.release;" ::: "memory");
       asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-    } else {
-      asm volatile("bar.sync 1, 128;" ::: "memory");
     }
     const int* src[8];
 #pragma unroll
@@ -170,16 +186,8 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     const bool vec = c0 + 4 <= p.N && ((size_t)p.ldo * sizeof(TO)) % (4 * sizeof(TO)) == 0 && (uintptr_t)out % (4 * sizeof(TO)) == 0;
 #pragma unroll 1
     for (int m = m_begin + quarter; m < m_end; m += 4) {
-      const int at = row0 + m;
-      float rs = a_scale[at], pw = 1.0f;
-      size_t to = at;
-      if (GROUPED) {
-        const int pair = order[at];
-        if (p.scatter) to = pair;
-        if (p.w_out) rs *= wts[pair];
-        if (p.w_in) pw = wts[pair];
-      }
-      TO* o = out + to * p.ldo + c0;
+      const float rs = row_scale[m], pw = GROUPED && p.w_in ? row_weight[m] : 1.0f;
+      TO* o = out + (size_t)row_to[m] * p.ldo + c0;
       int4 x[8];
 #pragma unroll
       for (int q = 0; q < 8; q++) x[q] = q < split ? *reinterpret_cast<const int4*>(src[q] + m * I8_ROWS) : make_int4(0, 0, 0, 0);

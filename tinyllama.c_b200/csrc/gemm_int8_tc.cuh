@@ -51,6 +51,15 @@ __device__ __forceinline__ void load_weights(uint32_t dst, const CUtensorMap* ma
   }
 }
 
+// Waits for the loads from tensor memory; what they brought counts as written here, so that nothing uses it earlier.
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
 // Which group's which rows the tile-th tile of `rows_a_tile` sorted rows covers: a warp adds up the groups' tiles, 32 groups at a
 // time.  Returns false past the last tile.  (All lanes get the results.)
 __device__ __forceinline__ bool int8_group_tile(int tile, int rows_a_tile, const int* offsets, int E, int* group, int* row0, int* rows) {

@@ -26,7 +26,7 @@ template <int NB> struct Wide {
   static constexpr int W_BYTES = I8_ROWS * I8_K, X_BYTES = NB / 2 * I8_K;
   static constexpr int TILES = STAGES * (W_BYTES + X_BYTES);
   static constexpr int N_BARS = 2 * STAGES + 4;
-  static constexpr int TOTAL = TILES + N_BARS * 8 + 16 + 4 * NB * 3 * 4 + 16 + 1024;      // ..., where tensor memory lies, scales
+  static constexpr int TOTAL = TILES + N_BARS * 8 + 16 + 4 * NB * 3 * 4 + 1024;     // ..., where tensor memory lies, the rows' numbers (and the groups' offsets)
 };
 
 template <typename TO, int NB, bool GLU, bool GROUPED>
@@ -66,26 +66,33 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 
   // Tiles: without groups the activation rows' tiles run fastest (pairs that run together share weights in the L2), with them the
   // weight rows' (a group has few tiles of activation rows).
-  const int* offsets = p.offsets;
+  int* offsets = reinterpret_cast<int*>(tmem_slot + 4 + 12 * NB);      // (the groups' offsets, a copy)
   const int m_tiles = GROUPED ? 1 : (p.M + NB - 1) / NB;
   int total = m_tiles * n_tiles;
   if (GROUPED) {
-    tlc_wait(offsets);
+    const int* from = p.offsets;
+    tlc_wait(from);
+    for (int e = threadIdx.x; e <= p.E; e += THREADS) offsets[e] = from[e];
+    __syncthreads();
     int tiles = 0;
     for (int e = lane; e < p.E; e += 32) tiles += (offsets[e + 1] - offsets[e] + NB - 1) / NB;
     total = __reduce_add_sync(0xffffffffu, tiles) * n_tiles;
   }
-  auto place = [&](int tile, int* group, int* row0, int* rows) -> int {      // ... and the tile's index along the weight rows
+  struct Place { int group, row0, rows, n; };
+  auto place = [&](int tile) {
+    Place at;
     if constexpr (GROUPED) {
-      *group = 0; *row0 = 0; *rows = 0;
-      int8_group_tile(tile / n_tiles, NB, offsets, p.E, group, row0, rows);
-      return tile % n_tiles;
+      at.group = at.row0 = at.rows = 0;
+      int8_group_tile(tile / n_tiles, NB, offsets, p.E, &at.group, &at.row0, &at.rows);
+      at.n = tile % n_tiles;
     } else {
-      *group = 0;
-      *row0 = tile % m_tiles * NB;
-      *rows = min(NB, p.M - *row0);
-      return tile / m_tiles;
+      at.group = 0;
+      at.n = tile / m_tiles;
+      at.row0 = (tile - at.n * m_tiles) * NB;
+      at.rows = min(NB, p.M - at.row0);
     }
+    at.n = at.n * 2 * I8_ROWS + (int)rank * I8_ROWS;    // its first weight row (gated: of the interleaved ones) in this block
+    return at;
   };
 
   if (warp == 0) {                                      // ---- copies (one lane issues them) ----
@@ -96,16 +103,15 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     int pending = 0;                                    // first stages whose activations are held back until the kernel before is through
     const int first = min(STAGES, num_k);               // (all of them in the first tile)
     for (int tile = walker; tile < total && ok; tile += walkers) {
-      int group, row0, rows;
-      const int n0 = place(tile, &group, &row0, &rows) * 2 * I8_ROWS + (int)rank * I8_ROWS;
-      const int m0 = row0 + (int)rank * (NB / 2);
+      const Place at = place(tile);
+      const int m0 = at.row0 + (int)rank * (NB / 2);
       if (lane == 0) {
         for (int k = 0; k < num_k; k++, it++) {
           const int s = it % STAGES;
           ok = mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1, err, 55, wait_limit);
           if (!ok) break;
           if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (S::W_BYTES + S::X_BYTES));
-          load_weights<GLU, true>(smem_u32(smem + s * S::W_BYTES), &map_w, full_bar0 + 8 * s, k * I8_K, n0, group);
+          load_weights<GLU, true>(smem_u32(smem + s * S::W_BYTES), &map_w, full_bar0 + 8 * s, k * I8_K, at.n, at.group);
           if (!waited) {
             pending++;
             if (pending < first) continue;
@@ -167,40 +173,60 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     float* scales = reinterpret_cast<float*>(tmem_slot + 4) + (warp - 2) * (MINE * (GROUPED ? 3 : 1));
     int* to = reinterpret_cast<int*>(scales + MINE);
     float* pw = scales + 2 * MINE;
-    for (int tile = walker; tile < total && ok; tile += walkers, local++) {
-      const int as = local & 1;
-      int group, row0, rows;
-      const int n0 = place(tile, &group, &row0, &rows) * 2 * I8_ROWS + (int)rank * I8_ROWS;
-      const bool is_up = GLU && (lane & 8);
-      const int col = GLU ? (n0 >> 1) + ((row >> 4) << 3) + (row & 7) : n0 + row;        // column of the result
+    const bool is_up = GLU && (lane & 8);
+    // what a tile needs beside its sums, asked for a tile ahead: this lane's column's scale and bias, this warp's rows' numbers
+    Place at, next;
+    float cs, cb, n_cs = 0.f, n_cb = 0.f, n_rs[CHUNKS], n_pw[CHUNKS];
+    int n_to[CHUNKS];
+    auto column = [&](const Place& t) { return GLU ? (t.n >> 1) + ((row >> 4) << 3) + (row & 7) : t.n + row; };
+    auto fetch = [&](int tile) {
+      next = place(tile);
+      const int col = column(next);
       const bool in = col < p.N;
-      const size_t at = (size_t)group * p.w_rows + (is_up ? p.N : 0) + col;
-      const float cs = in ? p.w_scale[at] : 0.f, cb = in && p.colbias ? p.colbias[(is_up ? p.N : 0) + col] : 0.f;
-      __syncwarp();                                     // (the last tile's scales have been read)
+      n_cs = in ? p.w_scale[(size_t)next.group * p.w_rows + (is_up ? p.N : 0) + col] : 0.f;
+      n_cb = in && p.colbias ? p.colbias[(is_up ? p.N : 0) + col] : 0.f;
 #pragma unroll
       for (int c = 0; c < CHUNKS; c++) {
-        const int m = (share * CHUNKS + c) * 32 + lane;
-        const bool there = m < rows;
-        float rs = there ? a_scale[row0 + m] : 0.f;
+        const int m = share * MINE + c * 32 + lane;
+        const bool there = m < next.rows;
+        n_rs[c] = there ? a_scale[next.row0 + m] : 0.f;
         if (GROUPED) {
-          const int pair = there ? order[row0 + m] : 0;
-          const float w = there ? wts[pair] : 0.f;
-          if (p.w_out) rs *= w;
-          to[c * 32 + lane] = p.scatter ? pair : row0 + m;
-          pw[c * 32 + lane] = p.w_in ? w : 1.0f;
+          const int pair = there ? order[next.row0 + m] : 0;
+          n_pw[c] = there ? wts[pair] : 0.f;
+          n_to[c] = p.scatter ? pair : next.row0 + m;
         }
-        scales[c * 32 + lane] = rs;
+      }
+    };
+    if (walker < total) fetch(walker);
+    for (int tile = walker; tile < total && ok; tile += walkers, local++) {
+      const int as = local & 1;
+      at = next;
+      cs = n_cs;
+      cb = n_cb;
+      const int col = column(at);                       // of the result
+      const bool in = col < p.N;
+      __syncwarp();                                     // (the last tile's numbers have been read)
+#pragma unroll
+      for (int c = 0; c < CHUNKS; c++) {
+        const int m = c * 32 + lane;
+        scales[m] = GROUPED && p.w_out ? n_rs[c] * n_pw[c] : n_rs[c];
+        if (GROUPED) {
+          to[m] = n_to[c];
+          pw[m] = p.w_in ? n_pw[c] : 1.0f;
+        }
       }
       __syncwarp();
+      if (tile + walkers < total) fetch(tile + walkers);
       ok = mbar_wait(acc_full0 + 8 * as, (local >> 1) & 1, err, 59, wait_limit);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * NB + share * MINE);
+      uint32_t r[PIECE];
+      tmem_ld16_nowait(acc, r);
 #pragma unroll 1                                        // (a piece's code stays near the scheduler)
       for (int m1 = 0; m1 < MINE; m1 += PIECE) {
-        const int m0 = share * MINE + m1, left = rows - m0;                      // activation rows of this piece
-        if (left <= 0) break;
-        uint32_t r[PIECE];
-        tmem_ldn(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * NB + m0), r);
+        const int m0 = share * MINE + m1, left = at.rows - m0;                   // activation rows of this piece
+        tmem_wait16(r);
         float v[PIECE];
 #pragma unroll
         for (int j = 0; j < PIECE; j += 4) {
@@ -210,8 +236,16 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
           v[j + 2] = int8_value((int)r[j + 2], rs.z, cs, cb);
           v[j + 3] = int8_value((int)r[j + 3], rs.w, cs, cb);
         }
+        if (m1 + PIECE < MINE) {
+          tmem_ld16_nowait(acc + (uint32_t)(m1 + PIECE), r);                     // the next piece, under this one's stores
+        } else {                                        // all taken out: the accumulator goes back to the issuer's block
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(cluster_address(acc_empty0 + 8 * as, 0));
+        }
+        if (left <= 0) continue;
         // where this lane writes row j + mine of the piece (grouped: by the row's own index)
-        TO* base = out + (size_t)(row0 + m0) * p.ldo + col;
+        TO* base = out + (size_t)(at.row0 + m0) * p.ldo + col;
         auto target = [&](const int j, const int mine) {
           return GROUPED ? out + (size_t)to[m1 + j + mine] * p.ldo + col : base + (unsigned)((j + mine) * p.ldo);
         };
@@ -247,9 +281,6 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
           }
         }
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(cluster_address(acc_empty0 + 8 * as, 0));        // the issuer's block
     }
   }
   __syncwarp();
@@ -263,7 +294,8 @@ int launch(const Int8Args& p, long long tiles, int n_tiles, int pairs, cudaStrea
   using S = Wide<NB>;
   static std::atomic<bool> set{false};
   if (!set) {
-    if (cudaFuncSetAttribute(int8_wide_kernel<TO, NB, GLU, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL) != cudaSuccess)
+    if (cudaFuncSetAttribute(int8_wide_kernel<TO, NB, GLU, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             S::TOTAL + (GROUPED ? (TLC_INT8_GROUPS + 1) * (int)sizeof(int) : 0)) != cudaSuccess)
       return tlc_fail(-2, "linear_int8: cannot reserve %d bytes of shared memory", S::TOTAL);
     set = true;
   }
@@ -272,7 +304,7 @@ int launch(const Int8Args& p, long long tiles, int n_tiles, int pairs, cudaStrea
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, pairs));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = S::TOTAL;
+  cfg.dynamicSmemBytes = S::TOTAL + (GROUPED ? ((size_t)p.E + 1) * sizeof(int) : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
