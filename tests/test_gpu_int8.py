@@ -120,6 +120,20 @@ def test_halves_go_to_the_even_integer_and_the_lowest_integer_is_minus_127():
     assert q[0].tolist() == [127, 0, 2, 2, 0, -2, -126, -127] and float(scale) == 1.0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_integers_are_those_of_the_quotients(dtype):
+    """Integer by integer what dividing in 32 bits and rounding gives, over many magnitudes (one row in 128 of 16-bit rows is full of
+    quotients that are halves exactly)."""
+    g = gen(11)
+    for K in (8, 64, 2048):
+        x = normal(g, (1 << 22) // K, K) * torch.empty((1 << 22) // K, 1, device=DEV).uniform_(-30, 30, generator=g).exp2()
+        x = x.to(dtype)
+        q, scale = ops.rows_int8(x)
+        largest = x.float().abs().amax(1)
+        s = largest / torch.full((), 127.0, device=DEV)
+        assert torch.equal(scale, s) and torch.equal(q, torch.round(x.float() / s[:, None]).to(torch.int8))
+
+
 def test_rows_of_strided_and_unaligned_views():
     g = gen(3)
     big = normal(g, 9, 700, dtype=torch.bfloat16)

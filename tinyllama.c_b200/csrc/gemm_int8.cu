@@ -132,11 +132,13 @@ int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
     sms = n > 0 ? n : 148;
   }
   if (g_kernel != 1 && (out_dtype == TLC_F32 || out_dtype == TLC_BF16) && tensor_cores_take(p)) {
-    const int rows = p.offsets ? (p.M + p.E - 1) / p.E * 3 / 2 : p.M;      // grouped: half as many again as a group has on average
     const int pairs = tlc_linear_pairs();
-    if (g_kernel == 3 ? pairs > 0 : g_kernel == 0 && rows > 128 && pairs > 0)
-      return tlc_int8_wide(p, out_dtype, g_kernel == 3 ? g_rows : 256, pairs, stream);
-    return tlc_int8_few(p, out_dtype, g_kernel == 2 ? g_rows : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, sms, stream);
+    if (g_kernel == 3 && pairs > 0) return tlc_int8_wide(p, out_dtype, g_rows, pairs, stream);
+    if (g_kernel == 2) return tlc_int8_few(p, out_dtype, g_rows, sms, stream);
+    const int rows = p.offsets ? (p.M + p.E - 1) / p.E : p.M;              // of a group, on average
+    if (pairs > 0 && rows > (p.offsets ? 24 : 128)) return tlc_int8_wide(p, out_dtype, p.offsets && rows <= 110 ? 128 : 256, pairs, stream);
+    const int most = p.offsets ? rows * 3 / 2 : rows;                      // (a group may well have half as many again)
+    return tlc_int8_few(p, out_dtype, most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : 128, sms, stream);
   }
   if (out_dtype == TLC_F32) return run_tiles<float>(p, stream);
   if (out_dtype == TLC_BF16) return run_tiles<__nv_bfloat16>(p, stream);

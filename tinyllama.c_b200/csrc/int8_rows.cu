@@ -5,115 +5,163 @@
 //
 // The norm's factor r = 1 / sqrt(mean + eps) is the same for a whole row and cancels in v / s, so the integers are those of
 // p = x w and only the scale is multiplied by r: the row's sum of squares and its largest |p| come from one trip through the
-// block, and a row is read once (up to 16,384 values a block keeps it in registers).
+// row's warps, and a row is read once (up to 16,384 values stay in registers).
+//
+// Few rows: as many threads a row as it has pieces of eight values, for the shortest way through (1 x 2,048 1.4 us).  Rows that fill the
+// GPU: several pieces a thread and several rows a block, so that enough loads are on their way: 8,192 x 2,560 bfloat16 values 12.3 us
+// (63 MB, 5.1 TB/s), 16,384 x 1,024 float values 12.6 us (6.7 TB/s); a block a row took 27.5 and 18.6.
 //
 // The largest magnitude is a maximum of bit patterns without their sign: an infinity or a NaN is larger than every number there,
 // and a row that holds one gets the scale NaN and zeros, so that whatever is multiplied by it is NaN.  A row of zeros (or of values
 // below 127 x 2^-126) gets the scale 0.  Both divisions are IEEE's, not products with a reciprocal: with a largest magnitude of
 // 127 x 2^j, as one bfloat16 row in 128 has, v / s is often a half exactly, and the rounding to even should see it.
 #include "common.cuh"
+#include <algorithm>
 
 namespace {
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Eight values as they lie in memory (a 16- or 32-byte piece), and as numbers: apart, so that all of a thread's loads are on their way
+// before the first is looked at.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
+  __device__ __forceinline__ void numbers(float (&v)[8]) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w; }
+};
+template <> struct Piece<__nv_bfloat16> {
+  uint4 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void numbers(float (&v)[8]) const {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-
-// Eight values from column k on, zeros past K; vec: rows start on 16-byte boundaries, and so does every eighth column.
-template <typename T> __device__ __forceinline__ void row8(const T* x, int k, int K, bool vec, float (&v)[8]) {
-  if (vec && k + 8 <= K) return load8(x + k, v);
+    for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+};
+// Eight values from column k on, zeros past K, in any layout.
+template <typename T> __device__ __forceinline__ void row8(const T* x, int k, int K, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] = k + i < K ? to_f32(x[k + i]) : 0.f;
 }
-__device__ __forceinline__ void store8(int8_t* q, int k, int K, bool vec, const int (&n)[8]) {
-  if (vec && k + 8 <= K) {
-    uint2 o = make_uint2(0u, 0u);
+__device__ __forceinline__ void store8(int8_t* q, int k, int K, uint2 n) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) { o.x |= (uint32_t)(n[i] & 255) << (8 * i); o.y |= (uint32_t)(n[4 + i] & 255) << (8 * i); }
-    *reinterpret_cast<uint2*>(q + k) = o;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; i++) if (k + i < K) q[k + i] = (int8_t)n[i];
+  for (int i = 0; i < 8; i++) if (k + i < K) q[k + i] = (int8_t)((i < 4 ? n.x : n.y) >> (8 * (i & 3)));
 }
 
-// A block a row.  NI: pieces of eight values that a thread keeps in registers (0: it reads the row a second time).
-// order: row i of the result is row order[i] / top of x (the sorted pairs of a routing).
+// The larger magnitude; a NaN stays.
+__device__ __forceinline__ float larger(float m, float v) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v)));
+  return m;
+}
+// Eight integers nearest to the quotients v / s (halves to even) as bytes, inv = 1 / s correctly rounded.  A first quotient v inv is
+// mended by its remainder, which a fused multiply-add gives exactly, times inv (Markstein, IBM Journal of Research and Development 34,
+// 1990): the IEEE quotient, without the general division's cases, which do not arise here (s is no denormal and |v / s| <= 127).
+// Adding 1.5 * 2^23 rounds it to an integer and leaves that in the sum's low bits; conversions would go through the special-function
+// unit, at a quarter of the rate.
+__device__ __forceinline__ uint2 eight_nearest(const float (&v)[8], float s, float inv) {
+  uint32_t b[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const float first = __fmul_rn(v[i], inv), quotient = __fmaf_rn(__fmaf_rn(-first, s, v[i]), inv, first);
+    b[i] = __float_as_uint(__fadd_rn(quotient, 12582912.0f));
+  }
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+
+// `warps` warps a row, blockDim / (32 warps) rows a block.  NI > 0: rows of pieces that start on 16-byte boundaries, at most NI a
+// thread, which keeps them in registers; 0: any layout and length, and the row is read a second time.  order: row i of the result is
+// row order[i] / top of x (a routing's sorted pairs).
 template <typename T, int NI, bool NORM>
 __global__ void __launch_bounds__(512)
-int8_rows_kernel(const T* __restrict__ x, int ldx, int K, const float* __restrict__ w, float eps, int8_t* __restrict__ q, int ldq,
-                 float* __restrict__ scale, const int* __restrict__ order, int top, int vec_x, int vec_q, int vec_w) {
+int8_rows_kernel(const T* __restrict__ x, int ldx, int rows, int K, const float* __restrict__ w, float eps, int8_t* __restrict__ q, int ldq,
+                 float* __restrict__ scale, const int* __restrict__ order, int top, int warps) {
   tlc_pdl(x, q, scale, order);
   __shared__ unsigned red_max[16];
   __shared__ float red_sum[16];
-  const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nw = blockDim.x >> 5;
-  const T* xr = x + (size_t)(order ? order[row] / top : row) * ldx;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = warp / warps * warps, tid = threadIdx.x - 32 * first, threads = 32 * warps;     // of the row's warps
+  const int row = blockIdx.x * ((blockDim.x >> 5) / warps) + warp / warps;
+  const bool there = row < rows;
+  const T* xr = x + (size_t)(there ? (order ? order[row] / top : row) : 0) * ldx;
   int8_t* qr = q + (size_t)row * ldq;
-  constexpr int N = NI > 0 ? NI : 1;
-  float v[N][8];
-  unsigned largest = 0;
-  float sum = 0.f;
-  auto fetch = [&](int c, float (&u)[8]) {                    // p of piece c, and what it adds to the row's statistics
-    row8(xr, 8 * c, K, vec_x, u);
-    if (NORM) {
-      float g[8];
-      row8(w, 8 * c, K, vec_w, g);
-#pragma unroll
-      for (int i = 0; i < 8; i++) { sum += u[i] * u[i]; u[i] *= g[i]; }
-    }
-  };
   const int pieces = (K + 7) >> 3;
-  if (NI > 0) {
+  constexpr int N = NI > 0 ? NI : 1;
+  Piece<T> raw[N];
+  Piece<float> gain[NORM ? N : 1];
+  float magnitude = 0.f, sum = 0.f;
+  auto weigh = [&](float (&u)[8], const float (&g)[8], bool counts) {        // p of a piece, and what it adds to the row's statistics
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-      const int c = tid + j * blockDim.x;
-      if (c < pieces) {
-        fetch(c, v[j]);
-#pragma unroll
-        for (int i = 0; i < 8; i++) largest = max(largest, __float_as_uint(v[j][i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; i++) {
+      if (NORM) {
+        if (counts) sum += u[i] * u[i];
+        u[i] *= g[i];
       }
+      magnitude = larger(magnitude, u[i]);
     }
-  } else {
-    for (int c = tid; c < pieces; c += blockDim.x) {
-      fetch(c, v[0]);
-#pragma unroll
-      for (int i = 0; i < 8; i++) largest = max(largest, __float_as_uint(v[0][i]) & 0x7fffffffu);
-    }
-  }
-  largest = __reduce_max_sync(0xffffffffu, largest);
-  if (NORM) sum = warp_sum(sum);
-  if (lane == 0) { red_max[warp] = largest; if (NORM) red_sum[warp] = sum; }
-  __syncthreads();
-  largest = __reduce_max_sync(0xffffffffu, lane < nw ? red_max[lane] : 0u);
-  const float s = __fdiv_rn(__uint_as_float(largest), 127.0f);
-  const bool finite = largest < 0x7f800000u, some = finite && s >= 1.17549435e-38f;
-  if (tid < 32) {
-    float r = 1.0f;
-    if (NORM) r = rsqrtf(warp_sum(lane < nw ? red_sum[lane] : 0.f) / (float)K + eps);
-    if (lane == 0) scale[row] = !finite ? __uint_as_float(0x7fc00000u) : some ? s * r : 0.f;
-  }
-  auto leave = [&](int c, const float (&u)[8]) {
-    int n[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) n[i] = some ? __float2int_rn(__fdiv_rn(u[i], s)) : 0;
-    store8(qr, 8 * c, K, vec_q, n);
   };
-  if (NI > 0) {
+  if constexpr (NI > 0) {
+#pragma unroll
+    for (int j = 0; j < N; j++) {                             // (past the last piece: that piece again)
+      const int c = min(tid + j * threads, pieces - 1);
+      raw[j].load(xr + 8 * c);
+      if constexpr (NORM) gain[j].load(w + 8 * c);
+    }
 #pragma unroll
     for (int j = 0; j < N; j++) {
-      const int c = tid + j * blockDim.x;
-      if (c < pieces) leave(c, v[j]);
+      float u[8], g[8] = {};
+      raw[j].numbers(u);
+      if constexpr (NORM) gain[j].numbers(g);
+      weigh(u, g, tid + j * threads < pieces);
     }
   } else {
-    for (int c = tid; c < pieces; c += blockDim.x) { fetch(c, v[0]); leave(c, v[0]); }
+    for (int c = tid; c < pieces; c += threads) {
+      float u[8], g[8] = {};
+      row8(xr, 8 * c, K, u);
+      if (NORM) row8(w, 8 * c, K, g);
+      weigh(u, g, true);
+    }
+  }
+  unsigned largest = __reduce_max_sync(0xffffffffu, __float_as_uint(magnitude));
+  if (NORM) sum = warp_sum(sum);
+  if (warps > 1) {
+    if (lane == 0) { red_max[warp] = largest; if (NORM) red_sum[warp] = sum; }
+    __syncthreads();
+    largest = __reduce_max_sync(0xffffffffu, lane < warps ? red_max[first + lane] : 0u);
+    if (NORM) sum = warp_sum(lane < warps ? red_sum[first + lane] : 0.f);
+  }
+  if (!there) return;
+  const float s = __fdiv_rn(__uint_as_float(largest), 127.0f), inv = __frcp_rn(s);
+  const bool finite = largest < 0x7f800000u, some = finite && s >= 1.17549435e-38f;
+  if (tid == 0) {
+    const float r = NORM ? rsqrtf(sum / (float)K + eps) : 1.0f;
+    scale[row] = !finite ? __uint_as_float(0x7fc00000u) : some ? s * r : 0.f;
+  }
+  if constexpr (NI > 0) {
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const int c = tid + j * threads;
+      if (c >= pieces) break;
+      float u[8];
+      raw[j].numbers(u);
+      if constexpr (NORM) {
+        float g[8];
+        gain[j].numbers(g);
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] *= g[i];
+      }
+      *reinterpret_cast<uint2*>(qr + 8 * c) = some ? eight_nearest(u, s, inv) : make_uint2(0u, 0u);
+    }
+  } else {
+    for (int c = tid; c < pieces; c += threads) {
+      float u[8], g[8] = {};
+      row8(xr, 8 * c, K, u);
+      if (NORM) {
+        row8(w, 8 * c, K, g);
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] *= g[i];
+      }
+      store8(qr, 8 * c, K, some ? eight_nearest(u, s, inv) : make_uint2(0u, 0u));
+    }
   }
 }
 
@@ -122,15 +170,21 @@ __global__ void int8_boundary_kernel() {}
 template <typename T, bool NORM>
 int rows_of(const T* x, int ldx, int T_, int K, const float* w, float eps, int8_t* q, int ldq, float* scale, const int* order, int top,
             cudaStream_t stream) {
-  const int vec_x = (uintptr_t)x % 16 == 0 && ((size_t)ldx * sizeof(T)) % 16 == 0, vec_q = (uintptr_t)q % 8 == 0 && ldq % 8 == 0;
-  const int vec_w = NORM && (uintptr_t)w % 16 == 0;
+  const bool whole = (uintptr_t)x % 16 == 0 && ((size_t)ldx * sizeof(T)) % 16 == 0 && (uintptr_t)q % 8 == 0 && ldq % 8 == 0 && K % 8 == 0 &&
+                     (!NORM || (uintptr_t)w % 16 == 0);
   const int pieces = (K + 7) / 8;
-  const int threads = pieces <= 128 ? 128 : pieces <= 256 ? 256 : 512;
-#define TLC_ROWS(NI_) tlc_launch(int8_rows_kernel<T, NI_, NORM>, dim3(T_), dim3(threads), 0, stream, x, ldx, K, w, eps, q, ldq, scale, \
-                                 order, top, vec_x, vec_q, vec_w)
-  if (pieces <= threads) TLC_ROWS(1);
-  else if (pieces <= 2 * threads) TLC_ROWS(2);
-  else if (pieces <= 4 * threads) TLC_ROWS(4);
+  // a thread's pieces: one for few rows, or from 592 rows (four blocks an SM) on 64 or 96 bytes of it at most.  One, four, six pieces:
+  // 128 x 2,048 (bfloat16) 1.4, 1.7, 1.7 us; 1,024 x 2,560 3.7, 3.5, 3.7; 8,192 x 2,560 18.7, 13.4, 12.3
+  const int per_thread = T_ < 592 ? 1 : sizeof(T) == 2 ? 6 : 4;
+  const int warps = std::min(16, (pieces + 32 * per_thread - 1) / (32 * per_thread));
+  const int block_rows = T_ < 592 ? 1 : std::max(1, 8 / warps), threads = 32 * warps * block_rows;
+#define TLC_ROWS(NI_) tlc_launch(int8_rows_kernel<T, NI_, NORM>, dim3((T_ + block_rows - 1) / block_rows), dim3(threads), 0, stream, x, \
+                                 ldx, T_, K, w, eps, q, ldq, scale, order, top, warps)
+  if (!whole) TLC_ROWS(0);
+  else if (pieces <= 32 * warps) TLC_ROWS(1);
+  else if (pieces <= 64 * warps) TLC_ROWS(2);
+  else if (pieces <= 128 * warps) TLC_ROWS(4);
+  else if (pieces <= 192 * warps) TLC_ROWS(6);
   else TLC_ROWS(0);
 #undef TLC_ROWS
   TLC_CHECK_LAUNCH("rows_int8");
