@@ -1578,13 +1578,22 @@ def linear_int8_kernel(kernel: int = 0, rows: int = 0) -> None:
 
 def int8_empty(rows: int, k: int, device) -> torch.Tensor:
     """An uninitialised int8 [rows, k] whose rows start on 16-byte boundaries."""
+    if k % 16 == 0:
+        return torch.empty((rows, k), dtype=torch.int8, device=device)
     return torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
 
 
-def _rows_int8(x, q, scale, norm_weight=None, eps=0.0, boundary=0):
+def _rows_int8(x, what, norm_weight=None, eps=0.0, boundary=0):
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise KernelError(f"{what}: rows [T, K] with K >= 1, got {tuple(x.shape)}")
     T, K = x.shape
-    _call("tlc_rows_int8", x.data_ptr(), dtype_code(x.dtype), _rows(x, "rows_int8 input"), T, K, _p(norm_weight), float(eps), q.data_ptr(),
-          q.stride(0), scale.data_ptr(), None, 1, boundary, _stream())
+    if norm_weight is not None:
+        _f32vec(norm_weight, K, what + " weight")
+    _gpu(x, norm_weight)
+    code, ldx = dtype_code(x.dtype), _rows(x, what + " input")
+    q, scale = int8_empty(T, K, x.device), torch.empty(T, dtype=torch.float32, device=x.device)
+    _call("tlc_rows_int8", x.data_ptr(), code, ldx, T, K, _p(norm_weight), eps, q.data_ptr(), (K + 15) // 16 * 16, scale.data_ptr(), None, 1,
+          boundary, _stream())
     return q, scale
 
 
@@ -1592,19 +1601,12 @@ def rows_int8(x: torch.Tensor):
     """(q int8 [T, K], scale float32 [T]) of float32 or bfloat16 rows: scale[t] = max_k |x[t, k]| / 127, q = x / scale rounded to the
     nearest integer (halves to even).  A row of zeros has scale 0; one that holds a NaN or an infinity has scale NaN and integers 0.
     q is an operand a of linear_int8; for weights see weight_int8."""
-    _gpu(x)
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise KernelError(f"rows_int8: rows [T, K] with K >= 1, got {tuple(x.shape)}")
-    return _rows_int8(x, int8_empty(x.shape[0], x.shape[1], x.device), torch.empty(x.shape[0], dtype=torch.float32, device=x.device))
+    return _rows_int8(x, "rows_int8")
 
 
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float):
     """rows_int8 of the RMS norm x / sqrt(mean(x^2) + eps) * weight of every row, in one pass; weight float32 [K]."""
-    _gpu(x, weight)
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise KernelError(f"rmsnorm_int8: rows [T, K] with K >= 1, got {tuple(x.shape)}")
-    _f32vec(weight, x.shape[1], "rmsnorm_int8 weight")
-    return _rows_int8(x, int8_empty(x.shape[0], x.shape[1], x.device), torch.empty(x.shape[0], dtype=torch.float32, device=x.device), weight, eps)
+    return _rows_int8(x, "rmsnorm_int8", weight, float(eps))
 
 
 def weight_int8(w: torch.Tensor):
@@ -1613,37 +1615,53 @@ def weight_int8(w: torch.Tensor):
     _gpu(w)
     if w.dim() not in (2, 3) or w.shape[-1] < 1:
         raise KernelError(f"weight_int8: a matrix [N, K] or matrices [E, N, K], got {tuple(w.shape)}")
-    rows = w.reshape(-1, w.shape[-1])
-    q = int8_empty(rows.shape[0], rows.shape[1], w.device)
-    scale = torch.empty(rows.shape[0], dtype=torch.float32, device=w.device)
-    _rows_int8(rows, q, scale, boundary=1)
+    q, scale = _rows_int8(w.reshape(-1, w.shape[-1]), "weight_int8", boundary=1)
     cannot_repeat()
     if w.dim() == 3:
-        ld = q.stride(0)
+        ld = (w.shape[2] + 15) // 16 * 16
         q = q.as_strided(tuple(w.shape), (w.shape[1] * ld, ld, 1))
     return q, scale.view(w.shape[:-1])
 
 
-def _int8_operands(what, a, a_scale, w, w_scale, colbias, out, N):
-    """Checks what the two products below share; (a's type code, its row stride, the scale and the room for its integers)."""
-    _gpu(a, a_scale, w, w_scale, colbias, out)
-    if a.dim() != 2 or w.dim() != 2 or w.dtype != torch.int8 or w.shape[1] != a.shape[1] or tuple(out.shape) != (a.shape[0], N):
+def _linear_int8(what, a, a_scale, w, w_scale, colbias, out, N, accumulate, act, limit, alpha):
+    """What the two products below share.  (The checks stand here one by one: a decode step makes hundreds of these calls.)"""
+    if a.dim() != 2 or w.dim() != 2 or out.dim() != 2:
+        raise KernelError(f"{what}: matrices are wanted, got a{tuple(a.shape)} w{tuple(w.shape)} out{tuple(out.shape)}")
+    (M, K), (rows, k), (m, n) = a.shape, w.shape, out.shape
+    if w.dtype != torch.int8 or k != K or m != M or n != N:
         raise KernelError(f"{what}: shapes a{tuple(a.shape)} w{tuple(w.shape)} {w.dtype} out{tuple(out.shape)} do not agree")
-    M, K = a.shape
     if not 1 <= K <= INT8_MAX_K:
         raise KernelError(f"{what}: rows of {K} values; the sums are exact for 1 to {INT8_MAX_K}")
-    _f32vec(w_scale, w.shape[0], what + " weight scale")
-    _f32vec(colbias, w.shape[0], what + " colbias")
+    if not (a.is_cuda and w.is_cuda and out.is_cuda and w_scale.is_cuda):
+        _gpu(a, w, out, w_scale)
+    if w_scale.dtype != torch.float32 or w_scale.numel() != rows or not w_scale.is_contiguous():
+        _f32vec(w_scale, rows, what + " weight scale")
+    bias = None
+    if colbias is not None:
+        _gpu(colbias)
+        _f32vec(colbias, rows, what + " colbias")
+        bias = colbias.data_ptr()
+    (lda, ea), (ldw, ew), (ldo, eo) = a.stride(), w.stride(), out.stride()
+    if (ea != 1 and K > 1) or (ew != 1 and K > 1) or (eo != 1 and N > 1):
+        raise KernelError(f"{what}: rows must be dense, got strides {a.stride()}, {w.stride()}, {out.stride()}")
+    lda, ldw, ldo = lda if M > 1 else max(lda, K), ldw if rows > 1 else max(ldw, K), ldo if M > 1 else max(ldo, N)
     if a.dtype == torch.int8:
         if a_scale is None:
             raise KernelError(f"{what}: integer rows come with their scales (a_scale)")
+        _gpu(a_scale)
         _f32vec(a_scale, M, what + " a_scale")
-        return I8, a_scale, None, 0
-    if a_scale is not None:
-        raise KernelError(f"{what}: a_scale belongs to integer rows; a is {a.dtype}")
-    q, scale = int8_empty(M, K, a.device), torch.empty(M, dtype=torch.float32, device=a.device)
-    _note_owned(q, scale)
-    return dtype_code(a.dtype), scale, q, q.stride(0)
+        code, scale, q, ldq = I8, a_scale.data_ptr(), None, 0
+    else:
+        if a_scale is not None:
+            raise KernelError(f"{what}: a_scale belongs to integer rows; a is {a.dtype}")
+        code, ldq = dtype_code(a.dtype), (K + 15) // 16 * 16
+        room = torch.empty(M * (ldq + 4), dtype=torch.int8, device=a.device)       # the rows' integers, then their scales
+        if _notes.calls is not None:
+            _note_owned(room)
+        q = room.data_ptr()
+        scale = q + M * ldq
+    _call("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, w.data_ptr(), ldw, w_scale.data_ptr(), out.data_ptr(),
+          dtype_code(out.dtype), ldo, bias, accumulate, M, N, K, act, limit, alpha, _stream())
 
 
 def linear_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: torch.Tensor, a_scale: Optional[torch.Tensor] = None,
@@ -1654,11 +1672,7 @@ def linear_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: to
     rmsnorm_int8), or float32 or bfloat16 rows, which are rounded that way first.  out [M, N] float32 or bfloat16; a, w and out may
     be row-strided views.  w is fetched while the kernel before may still run: it must not be the output of a kernel of the same
     step (weight_int8 sees to that)."""
-    N = w.shape[0]
-    code, scale, q, ldq = _int8_operands("linear_int8", a, a_scale, w, w_scale, colbias, out, N)
-    _call("tlc_linear_int8", a.data_ptr(), code, _rows(a, "linear_int8 input"), scale.data_ptr(), _p(q), ldq, w.data_ptr(),
-          _rows(w, "linear_int8 weight"), w_scale.data_ptr(), out.data_ptr(), dtype_code(out.dtype), _rows(out, "linear_int8 output"),
-          _p(colbias), int(bool(accumulate)), a.shape[0], N, a.shape[1], -1, 0.0, 1.0, _stream())
+    _linear_int8("linear_int8", a, a_scale, w, w_scale, colbias, out, w.shape[0], 1 if accumulate else 0, -1, 0.0, 1.0)
 
 
 def linear_swiglu_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: torch.Tensor, a_scale: Optional[torch.Tensor] = None,
@@ -1667,14 +1681,9 @@ def linear_swiglu_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, 
     gate's rows, then the up projection's; not interleaved); act, limit and alpha as in glu()."""
     if act not in DENSE_ACTS:
         raise KernelError(f"linear_swiglu_int8: unknown activation '{act}'; known: {sorted(DENSE_ACTS)}")
-    F = w.shape[0] // 2
     if w.shape[0] % 2:
         raise KernelError(f"linear_swiglu_int8: {w.shape[0]} rows are not a gate's and as many of an up projection")
-    code, scale, q, ldq = _int8_operands("linear_swiglu_int8", a, a_scale, w, w_scale, colbias, out, F)
-    _call("tlc_linear_int8", a.data_ptr(), code, _rows(a, "linear_swiglu_int8 input"), scale.data_ptr(), _p(q), ldq, w.data_ptr(),
-          _rows(w, "linear_swiglu_int8 weight"), w_scale.data_ptr(), out.data_ptr(), dtype_code(out.dtype),
-          _rows(out, "linear_swiglu_int8 output"), _p(colbias), 0, a.shape[0], F, a.shape[1], DENSE_ACTS[act], float(limit), float(alpha),
-          _stream())
+    _linear_int8("linear_swiglu_int8", a, a_scale, w, w_scale, colbias, out, w.shape[0] // 2, 0, DENSE_ACTS[act], float(limit), float(alpha))
 
 
 def _expert_rows(w: torch.Tensor, what: str) -> int:
@@ -1712,12 +1721,15 @@ def moe_experts_int8(x: torch.Tensor, w_gate_up: torch.Tensor, gate_up_scale: to
     _f32vec(down_scale, E * D, "moe_experts_int8 down scale")
     if not y.is_contiguous() or y.numel() != pairs * D:
         raise KernelError("moe_experts_int8: y must be contiguous [T, top, D]")
-    q = int8_empty(pairs, max(D, F), x.device)
-    work = torch.empty(pairs * (F + 1), dtype=torch.float32, device=x.device)          # the activation, the rows' scales
-    _note_owned(q, work)
+    # the rows' integers (the activation's after them in the same place), the activation, the rows' scales
+    ldq = (max(D, F) + 15) // 16 * 16
+    room = torch.empty(pairs * (ldq + 4 * F + 4), dtype=torch.int8, device=x.device)
+    _note_owned(room)
+    q = room.data_ptr()
+    act = q + pairs * ldq
     _call("tlc_moe_experts_int8", x.data_ptr(), dtype_code(x.dtype), _rows(x, "moe_experts_int8 input"), w_gate_up.data_ptr(), ld_gu,
           gate_up_scale.data_ptr(), w_down.data_ptr(), ld_d, down_scale.data_ptr(), order.data_ptr(), offsets.data_ptr(), wts.data_ptr(),
-          T, E, int(top), F, D, q.data_ptr(), q.stride(0), work.data_ptr() + 4 * pairs * F, work.data_ptr(), y.data_ptr(),
+          T, E, int(top), F, D, q, ldq, act + 4 * pairs * F, act, y.data_ptr(),
           dtype_code(y.dtype), MOE_ACTS[act_fn], int(weight_on == "output"), float(limit), float(alpha), _stream())
 
 
