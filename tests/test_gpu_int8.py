@@ -476,14 +476,14 @@ def test_weights_may_follow_at_once():
         assert torch.equal(out, again)
 
 
-KERNELS = [(1, 0), (2, 16), (2, 32), (2, 64), (2, 128), (3, 128), (3, 256)]
+KERNELS = [(4, 0), (2, 16), (2, 32), (2, 64), (2, 128), (3, 128), (3, 256)]
 
 
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_every_kernel_gives_the_same_bits(kernel):
     """The sums are exact, so a result does not depend on which kernel made it; it is compared with the CUDA cores'."""
     g = gen(9)
-    for M, N, K in [(1, 200, 384), (40, 1000, 272), (129, 2050, 130), (515, 520, 1024), (300, 2048, 64)]:
+    for M, N, K in [(1, 200, 384), (3, 77, 2049), (8, 300, 4096), (40, 1000, 272), (129, 2050, 130), (515, 520, 1024), (300, 2048, 64)]:
         a, sa, w, sw = integers(g, M, K), scales(g, M), integers(g, N, K), scales(g, N)
         bias = normal(g, N)
         w2, sw2 = integers(g, 2 * 136, K), scales(g, 2 * 136) * 0.1
@@ -506,7 +506,8 @@ def test_every_kernel_gives_the_same_bits(kernel):
 
 
 @pytest.mark.parametrize("kernel", KERNELS)
-@pytest.mark.parametrize("T,E,top,F,D,act,weight_on", [(1, 4, 2, 64, 128, "silu", "input"), (200, 5, 3, 136, 272, "silu", "output"),
+@pytest.mark.parametrize("T,E,top,F,D,act,weight_on", [(1, 4, 2, 64, 128, "silu", "input"), (2, 9, 4, 129, 400, "silu", "output"),
+                                                       (5, 3, 3, 65, 80, "relu_squared", "output"), (200, 5, 3, 136, 272, "silu", "output"),
                                                        (700, 3, 2, 72, 400, "silu", "input"), (33, 70, 4, 200, 128, "relu_squared", "output")])
 def test_every_kernel_gives_the_same_experts(kernel, T, E, top, F, D, act, weight_on):
     g = gen(T)

@@ -5,8 +5,13 @@
 // Here: the product for operands in any layout, on the CUDA cores (dp4a: four products and their sum an instruction), tiles of 32 x
 // 64 results staged through shared memory 64 values of K at a time.
 #include "gemm_int8_tc.cuh"
+#include <algorithm>
+#include <atomic>
 
 int tlc_int8_few(const Int8Args& p, int out_dtype, int nb, int sms, cudaStream_t stream);      // gemm_int8_few.cu
+int tlc_int8_few_split(long long tiles, int num_k, int sms);
+int tlc_int8_skinny(const void* x, int x_dtype, const Int8Args& p, int out_dtype, int sms, cudaStream_t stream);   // gemm_int8_skinny.cu
+int tlc_int8_skinny_pairs(const void* x, int x_dtype, const Int8Args& p, const int* ids, int per_row, int out_dtype, int sms, cudaStream_t stream);
 int tlc_int8_wide(const Int8Args& p, int out_dtype, int nb, int pairs, cudaStream_t stream);   // gemm_int8_wide.cu
 
 namespace {
@@ -121,24 +126,50 @@ bool tensor_cores_take(const Int8Args& p) {
          tlc_error_words_here() != nullptr;
 }
 
-int g_kernel = 0, g_rows = 0;        // test hook: which kernel, on tiles of how many activation rows
-
-int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
-  static int sms = 0;
+int sm_count() {
+  static std::atomic<int> sms{0};
   if (sms == 0) {
     int dev = 0, n = 0;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     sms = n > 0 ? n : 148;
   }
+  return sms;
+}
+
+int g_kernel = 0, g_rows = 0;        // test hook: which kernel, on tiles of how many activation rows
+
+int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
+  const int sms = sm_count();
   if (g_kernel != 1 && (out_dtype == TLC_F32 || out_dtype == TLC_BF16) && tensor_cores_take(p)) {
     const int pairs = tlc_linear_pairs();
     if (g_kernel == 3 && pairs > 0) return tlc_int8_wide(p, out_dtype, g_rows, pairs, stream);
     if (g_kernel == 2) return tlc_int8_few(p, out_dtype, g_rows, sms, stream);
-    const int rows = p.offsets ? (p.M + p.E - 1) / p.E : p.M;              // of a group, on average
-    if (pairs > 0 && rows > (p.offsets ? 24 : 128)) return tlc_int8_wide(p, out_dtype, p.offsets && rows <= 110 ? 128 : 256, pairs, stream);
-    const int most = p.offsets ? rows * 3 / 2 : rows;                      // (a group may well have half as many again)
-    return tlc_int8_few(p, out_dtype, most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : 128, sms, stream);
+    if (p.offsets) {
+      // Rows of a group, on average.  From 25 on pairs of blocks, which stay and stream through the groups one after the other; microseconds
+      // of a whole feed-forward with tiles of 128 rows by single blocks, of 128 and of 256 rows by pairs: 25 rows (32 experts) 61, 56, 60;
+      // 73 rows (64 experts) 129, 88, 99; 188 rows (32 experts) 151, 99, 84.  Below, 5 rows (32 experts) 48 with tiles of 16, 51 by pairs.
+      const int rows = (p.M + p.E - 1) / p.E, most = rows * 3 / 2;         // (a group may well have half as many again)
+      if (pairs > 0 && rows > 24) return tlc_int8_wide(p, out_dtype, rows <= 110 ? 128 : 256, pairs, stream);
+      return tlc_int8_few(p, out_dtype, most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : 128, sms, stream);
+    }
+    if (p.M <= 64) return tlc_int8_few(p, out_dtype, p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64, sms, stream);
+    // More rows: whichever of three is through first by what a K-step and the way in and out take (microseconds, measured): tiles of 64
+    // or 128 rows by single blocks that share K, where the tiles are few, or tiles of 256 rows by pairs.  For 129, 512 and 1,031 rows
+    // (64, 128, pairs): 2,560 -> 1,537 6.3 8.5 10.5, 9.1 9.4 11.5, 12.9 12.3 11.6; 8,192 -> 2,560 10.9 13.3 23.2, 25.9 19.6 24.3,
+    // 49.9 32.4 25.8; 2,048 -> 8,240 11.7 11.2 9.7, 23.4 17.0 12.7, 45.5 33.7 23.9.
+    const int num_k = (p.K + I8_K - 1) / I8_K, w_rows = p.mode == I8_GLU ? 2 * p.N : p.N;
+    auto single = [&](int nb, float way, float step) {
+      const long long tiles = (long long)((w_rows + I8_ROWS - 1) / I8_ROWS) * ((p.M + nb - 1) / nb);
+      const int split = tlc_int8_few_split(tiles, num_k, sms);
+      return way + step * (float)((tiles * split + 2 * sms - 1) / (2 * sms) * ((num_k + split - 1) / split));
+    };
+    const float by64 = single(64, 4.7f, 0.36f), by128 = single(128, 6.5f, 0.46f);
+    if (pairs > 0) {
+      const long long tiles = (long long)((w_rows + 2 * I8_ROWS - 1) / (2 * I8_ROWS)) * ((p.M + 255) / 256);
+      if (4.6f + 0.32f * (float)((tiles + pairs - 1) / pairs * num_k) <= std::min(by64, by128)) return tlc_int8_wide(p, out_dtype, 256, pairs, stream);
+    }
+    return tlc_int8_few(p, out_dtype, by64 <= by128 ? 64 : 128, sms, stream);
   }
   if (out_dtype == TLC_F32) return run_tiles<float>(p, stream);
   if (out_dtype == TLC_BF16) return run_tiles<__nv_bfloat16>(p, stream);
@@ -148,10 +179,10 @@ int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
 }  // namespace
 
 // Test hook: 0 = chosen by the sizes; 1 = the CUDA cores; 2 = tiles of 128 weight rows and 16, 32, 64 or 128 activation rows; 3 = pairs of
-// blocks on 256 weight rows and 128 or 256 activation rows, wherever they take the operands.
+// blocks on 256 weight rows and 128 or 256 activation rows; 4 = the kernel of up to 4 rows, wherever they take the operands.
 extern "C" int tlc_linear_int8_kernel(int kernel, int rows) {
   TLC_REQUIRE(kernel == 0 || kernel == 1 || (kernel == 2 && (rows == 16 || rows == 32 || rows == 64 || rows == 128)) ||
-              (kernel == 3 && (rows == 128 || rows == 256)), "linear_int8: there is no kernel %d with tiles of %d rows", kernel, rows);
+              (kernel == 3 && (rows == 128 || rows == 256)) || kernel == 4, "linear_int8: there is no kernel %d with tiles of %d rows", kernel, rows);
   g_kernel = kernel;
   g_rows = rows;
   return 0;
@@ -164,21 +195,30 @@ extern "C" int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_sca
   TLC_REQUIRE(K > 0 && K <= 131071 && lda >= K && ldw >= K && ldo >= N && M > 0 && N > 0,
               "linear_int8: bad sizes M=%d N=%d K=%d (at most 131071) lda=%d ldw=%d ldo=%d", M, N, K, lda, ldw, ldo);
   TLC_REQUIRE(act < 0 || act == TLC_ACT_SILU || act == TLC_ACT_GELU_TANH || act == TLC_ACT_SWISH_CLAMPED, "linear_int8: unknown activation %d", act);
-  if (a_dtype != TLC_I8) {
-    if (int rc = tlc_rows_int8(a, a_dtype, lda, M, K, nullptr, 0.f, a_int8, ld_int8, a_scale, nullptr, 1, 0, stream)) return rc;
-    a = a_int8;
-    lda = ld_int8;
-  }
   Int8Args p = {};
   p.a = (const int8_t*)a; p.a_scale = a_scale; p.w = (const int8_t*)w; p.w_scale = w_scale; p.out = out; p.colbias = colbias;
   p.lda = lda; p.ldw = ldw; p.ldo = ldo; p.M = M; p.N = N; p.K = K; p.w_rows = act >= 0 ? 2 * N : N;
   p.mode = act >= 0 ? I8_GLU : accumulate ? I8_ADD : I8_PLAIN;
   p.act = act; p.limit = limit; p.alpha = alpha;
+  TLC_REQUIRE(a_dtype == TLC_I8 || a_dtype == TLC_F32 || a_dtype == TLC_BF16, "linear_int8: unknown type %d of the rows", a_dtype);
+  TLC_REQUIRE(out_dtype == TLC_F32 || out_dtype == TLC_BF16, "linear_int8: unknown output dtype %d", out_dtype);
+  // Up to 4 rows of at most 8,192 values in all (2 where they are still to be rounded, which every block does), weights in 16-byte pieces
+  // and up to 24 MB of them: the kernel that takes the rows as they are.  Microseconds there and on the tensor cores (rounding
+  // included): 1 x 2,048 -> 2,048 2.5, 4.5; 1 x 2,048 -> 8,240 5.2, 6.4; 1 x 8,192 -> 2,560 7.6, 7.6; 2 x 4,096 -> 2,048 5.1, 5.7;
+  // 2 x 8,192 -> 2,560 9.4, 7.6; 4 x 2,048 -> 8,240 7.5, 6.6 (integers given 5.6, 6.0); 1 x 2,560 -> 2 x 8,192 11.2, 10.1.
+  const bool takes = M <= 4 && (long long)(M == 3 ? 4 : M) * K <= TLC_INT8_SKINNY && ((uintptr_t)w | (uintptr_t)ldw) % 16 == 0;
+  const bool skinny = M <= (a_dtype == TLC_I8 ? 4 : 2) && (long long)p.w_rows * K <= 24 << 20;
+  if (takes && (g_kernel == 0 ? skinny : g_kernel == 4)) return tlc_int8_skinny(a, a_dtype, p, out_dtype, sm_count(), stream);
+  if (a_dtype != TLC_I8) {
+    if (int rc = tlc_rows_int8(a, a_dtype, lda, M, K, nullptr, 0.f, a_int8, ld_int8, a_scale, nullptr, 1, 0, stream)) return rc;
+    p.a = (const int8_t*)a_int8;
+    p.lda = ld_int8;
+  }
   return run(p, out_dtype, stream);
 }
 
 extern "C" int tlc_moe_experts_int8(const void* x, int x_dtype, int ldx, const void* wgu, int ldgu, const float* sgu, const void* wd, int ldd,
-                                    const float* sd, const int* order, const int* offsets, const float* wts, int T, int E, int top, int F,
+                                    const float* sd, const int* ids, const int* order, const int* offsets, const float* wts, int T, int E, int top, int F,
                                     int D, void* q, int ldq, float* scales, float* act, void* y, int y_dtype, int act_code, int w_out,
                                     float limit, float alpha, cudaStream_t stream) {
   if (T == 0) return 0;
@@ -188,18 +228,30 @@ extern "C" int tlc_moe_experts_int8(const void* x, int x_dtype, int ldx, const v
   TLC_REQUIRE(E <= TLC_INT8_GROUPS, "moe_experts_int8: %d experts (at most %d)", E, TLC_INT8_GROUPS);
   TLC_REQUIRE(ldgu >= D && ldd >= F && ldq >= D && ldq >= F, "moe_experts_int8: rows shorter than the sizes (ld %d %d %d)", ldgu, ldd, ldq);
   TLC_REQUIRE(act_code >= TLC_ACT_SILU && act_code <= TLC_ACT_RELU_SQUARED, "moe_experts_int8: unknown activation %d", act_code);
-  // the chosen rows, sorted by expert, rounded; both products read their rows from q
-  if (int rc = tlc_rows_int8(x, x_dtype, ldx, (int)pairs, D, nullptr, 0.f, q, ldq, scales, order, top, 0, stream)) return rc;
+  TLC_REQUIRE((x_dtype == TLC_F32 || x_dtype == TLC_BF16) && (y_dtype == TLC_F32 || y_dtype == TLC_BF16), "moe_experts_int8: unknown dtype %d or %d",
+              x_dtype, y_dtype);
   const bool gated = act_code != TLC_ACT_RELU_SQUARED;
   Int8Args p = {};
   p.a = (const int8_t*)q; p.a_scale = scales; p.w = (const int8_t*)wgu; p.w_scale = sgu; p.out = act;
   p.lda = ldq; p.ldw = ldgu; p.ldo = F; p.M = (int)pairs; p.N = F; p.K = D; p.w_rows = gated ? 2 * F : F;
   p.mode = gated ? I8_GLU : I8_ACT; p.act = act_code; p.limit = limit; p.alpha = alpha;
   p.offsets = offsets; p.order = order; p.wts = wts; p.E = E; p.w_in = !w_out;
+  Int8Args d = p;                                         // the second product
+  d.w = (const int8_t*)wd; d.w_scale = sd; d.out = y; d.ldw = ldd; d.ldo = D; d.N = D; d.K = F; d.w_rows = D;
+  d.mode = I8_PLAIN; d.w_in = 0; d.w_out = w_out; d.scatter = 1;
+  // A few pairs: each a product of one row, which the kernel rounds itself.  Microseconds there and in the four launches below (2,048 x
+  // 1,024, 32 experts): 4 pairs 11.6, 16.4; 8 pairs 17.1, 20.7; 12 pairs 23.4, 23.2
+  if ((g_kernel == 0 || g_kernel == 4) && pairs <= 8 && D <= TLC_INT8_SKINNY && F <= TLC_INT8_SKINNY &&
+      ((uintptr_t)wgu | (uintptr_t)wd | (uintptr_t)ldgu | (uintptr_t)ldd) % 16 == 0) {
+    p.lda = ldx;
+    d.lda = F;
+    if (int rc = tlc_int8_skinny_pairs(x, x_dtype, p, ids, top, TLC_F32, sm_count(), stream)) return rc;
+    return tlc_int8_skinny_pairs(act, TLC_F32, d, ids, 1, y_dtype, sm_count(), stream);
+  }
+  // the chosen rows, sorted by expert, rounded; both products read their rows from q
+  if (int rc = tlc_rows_int8(x, x_dtype, ldx, (int)pairs, D, nullptr, 0.f, q, ldq, scales, order, top, 0, stream)) return rc;
   if (int rc = run(p, TLC_F32, stream)) return rc;
   // the activation in 32 bits -> rounded row by row; a weight on the result only multiplies the row's scale
   if (int rc = tlc_rows_int8(act, TLC_F32, F, (int)pairs, F, nullptr, 0.f, q, ldq, scales, nullptr, 1, 0, stream)) return rc;
-  p.w = (const int8_t*)wd; p.w_scale = sd; p.out = y; p.ldw = ldd; p.ldo = D; p.N = D; p.K = F; p.w_rows = D;
-  p.mode = I8_PLAIN; p.w_in = 0; p.w_out = w_out; p.scatter = 1;
-  return run(p, y_dtype, stream);
+  return run(d, y_dtype, stream);
 }

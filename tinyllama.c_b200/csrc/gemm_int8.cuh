@@ -19,6 +19,7 @@ struct Int8Args {
   int E;
   int scatter, w_out;                   // result rows go where order says, times the pair's weight
 };
+constexpr int TLC_INT8_SKINNY = 8192;     // values of activation rows in the kernel of up to 4 rows, at most
 constexpr int TLC_INT8_GROUPS = 4096;     // at most (as a routing)
 enum { I8_PLAIN = 0, I8_ADD = 1, I8_ACT = 2, I8_GLU = 3 };
 

@@ -304,14 +304,18 @@ int tlc_int8_maps(const Int8Args& p, int box_rows, CUtensorMap* weights, CUtenso
   return tlc_tensor_map_int8(p.a, 2, dims, strides, box, rows);
 }
 
+// Blocks a tile: as many (1, 2, 4, 8) as bring the grid to two blocks an SM, each with two K-steps or more.
+int tlc_int8_few_split(long long tiles, int num_k, int sms) {
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= 2 * sms && num_k / (split * 2) >= 2) split *= 2;
+  return split;
+}
+
 // nb: activation rows of a tile (16, 32, 64 or 128).
 int tlc_int8_few(const Int8Args& p, int out_dtype, int nb, int sms, cudaStream_t stream) {
   const int token_tiles = p.offsets ? p.M / nb + std::min(p.M, p.E) : (p.M + nb - 1) / nb;     // (grouped: an upper bound)
   const long long tiles = (long long)(((p.mode == I8_GLU ? 2 : 1) * p.N + I8_ROWS - 1) / I8_ROWS) * token_tiles;
-  // blocks a tile: as many as bring the grid to two blocks an SM, each with two K-steps or more
-  const int num_k = (p.K + I8_K - 1) / I8_K;
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= 2 * sms && num_k / (split * 2) >= 2) split *= 2;
+  const int split = tlc_int8_few_split(tiles, (p.K + I8_K - 1) / I8_K, sms);
 #define TLC_I8_NB(TO_) (nb == 16 ? launch_of<TO_, 16>(p, token_tiles, split, stream) : nb == 32 ? launch_of<TO_, 32>(p, token_tiles, split, stream) \
                         : nb == 64 ? launch_of<TO_, 64>(p, token_tiles, split, stream) : launch_of<TO_, 128>(p, token_tiles, split, stream))
   return out_dtype == TLC_F32 ? TLC_I8_NB(float) : TLC_I8_NB(__nv_bfloat16);

@@ -1,0 +1,239 @@
+// Products in 8-bit integers of up to 4 rows on the CUDA cores, rows rounded in the same kernel.
+//
+// The weights are streamed once, a warp two rows of them at a time (a feature's gate and up row, or neighbours), a lane 16 bytes of
+// every 512, four such pieces of both rows on their way together; dp4a multiplies them with the activation rows, which every block
+// keeps as integers in shared memory, and a warp reduction adds the lanes' sums, exactly.  Rows given in 16 or 32 bits are rounded by
+// every block for itself (they are small and come from the L2): a decode step's product is one launch, without tensor maps and without
+// room for the integers.  The first pieces of the weights are asked for before the wait on the kernel before.
+//
+// What bounds it: for small matrices the way from launch to last store (1 x 2,048 -> 2,048 2.5 us, of which the 4 MB are 0.65; the
+// tensor cores' kernel and the one that rounds for it 4.5), then the weights' stream (8,240 x 2,048 5.2 us, 17 MB at 3.3 TB/s; there
+// 6.4).  From about 24 MB on the tensor cores' ring keeps more on its way (gated 16,384 x 2,560: 11.2 us here, 10.1 there).
+#include "gemm_int8.cuh"
+#include "int8_round.cuh"
+#include <algorithm>
+
+namespace {
+
+constexpr int THREADS = 256, WARPS = THREADS / 32, AHEAD = 4;      // pieces of 512 bytes of a weight row on their way together
+
+// 16 values from k on, zeros past K.
+__device__ __forceinline__ int4 sixteen(const int8_t* p, int k, int K) {
+  if (k + 16 <= K) return __ldg(reinterpret_cast<const int4*>(p + k));
+  int v[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; i++) if (k + i < K) v[i >> 2] |= (int)(uint8_t)p[k + i] << (8 * (i & 3));
+  return make_int4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ int dot16(int4 a, int4 b, int c) { return __dp4a(a.w, b.w, __dp4a(a.z, b.z, __dp4a(a.y, b.y, __dp4a(a.x, b.x, c)))); }
+
+// The block's copy of the activation rows: integers in xs [MR][ld], scales.
+template <int MR> __device__ __forceinline__ void stage(const int8_t* x, int ldx, const float* a_scale, int M, int K, int8_t* xs, int ld, float* scale, unsigned*) {
+  for (int i = threadIdx.x; i < MR * (ld / 16); i += THREADS) {
+    const int m = i / (ld / 16), k = 16 * (i - m * (ld / 16));
+    int4 v = make_int4(0, 0, 0, 0);
+    if (m < M && (((uintptr_t)x | (uintptr_t)ldx) & 15) == 0) v = sixteen(x + (size_t)m * ldx, k, K);
+    else if (m < M) {
+      int w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 16; j++) if (k + j < K) w[j >> 2] |= (int)(uint8_t)x[(size_t)m * ldx + k + j] << (8 * (j & 3));
+      v = make_int4(w[0], w[1], w[2], w[3]);
+    }
+    *reinterpret_cast<int4*>(xs + (size_t)m * ld + k) = v;
+  }
+  if (threadIdx.x < MR) scale[threadIdx.x] = threadIdx.x < M ? a_scale[threadIdx.x] : 0.f;
+  __syncthreads();
+}
+template <int MR, typename T>
+__device__ __forceinline__ void stage(const T* x, int ldx, const float*, int M, int K, int8_t* xs, int ld, float* scale, unsigned* red) {
+  const bool whole = (uintptr_t)x % 16 == 0 && ((size_t)ldx * sizeof(T)) % 16 == 0;
+  const int pieces = ld / 8, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;      // (zeros from K to ld)
+  auto piece = [&](int m, int c, float (&v)[8]) {
+    const T* p = x + (size_t)m * ldx + 8 * c;
+    if (whole && 8 * c + 8 <= K) {
+      Piece<T> raw;
+      raw.load(p);
+      raw.numbers(v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = 8 * c + i < K ? to_f32(p[i]) : 0.f;
+    }
+  };
+  // the largest magnitudes of all rows, one meeting of the block
+#pragma unroll
+  for (int m = 0; m < MR; m++) {
+    float magnitude = 0.f;
+    if (m < M)
+      for (int c = threadIdx.x; c < pieces; c += THREADS) {
+        float v[8];
+        piece(m, c, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) magnitude = larger(magnitude, v[i]);
+      }
+    const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(magnitude));
+    if (lane == 0) red[m * WARPS + warp] = most;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int m = 0; m < MR; m++) {
+    bool some;
+    const unsigned largest = __reduce_max_sync(0xffffffffu, red[m * WARPS + (lane & (WARPS - 1))]);
+    const float s = int8_scale(largest, &some), inv = __frcp_rn(s);
+    if (threadIdx.x == 0) scale[m] = int8_told(largest, some, s);
+    for (int c = threadIdx.x; c < pieces; c += THREADS) {
+      uint2 n = make_uint2(0u, 0u);
+      if (some) {
+        float v[8];
+        piece(m, c, v);
+        n = eight_nearest(v, s, inv);
+      }
+      *reinterpret_cast<uint2*>(xs + (size_t)m * ld + 8 * c) = n;
+    }
+  }
+  __syncthreads();
+}
+
+// MR: rows the kernel is built for (M of them are there).  GROUPED (MR = 1): blocks of blockIdx.y take the pair of that number, row
+// pair / per_row of x times the weights of expert ids[pair].
+template <typename TX, typename TO, int MR, bool GLU, bool GROUPED>
+__global__ void __launch_bounds__(THREADS, 2)
+int8_skinny_kernel(const TX* __restrict__ x, Int8Args p, const int* __restrict__ ids, int per_row) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  extern __shared__ __align__(16) int8_t skinny_rows[];
+  __shared__ float scale[MR];
+  __shared__ unsigned red[MR * WARPS];
+  const int lane = threadIdx.x & 31, ld = (p.K + 15) & ~15;
+  const int warps = gridDim.x * WARPS, items = GLU ? p.N : (p.N + 1) / 2;
+  const int8_t* rows[2];
+  auto rows_of = [&](int item) {                          // the two weight rows of an item (past the last: that one again)
+    const int n0 = GLU ? item : 2 * item, n1 = GLU ? p.N + item : min(2 * item + 1, p.N - 1);
+    rows[0] = p.w + (size_t)n0 * p.ldw;
+    rows[1] = p.w + (size_t)n1 * p.ldw;
+  };
+  int4 w[2][AHEAD];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const int k = k0 + 512 * j + 16 * lane;
+        w[r][j] = k < p.K ? sixteen(rows[r], k, p.K) : make_int4(0, 0, 0, 0);
+      }
+  };
+  // a warp's items: one from each block in turn, so that few items spread over all SMs
+  int item = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
+  const float* a_scale = p.a_scale;
+  const float* wts = p.wts;
+  TO* out = reinterpret_cast<TO*>(p.out);
+  float share = 1.0f;
+  if (GROUPED) {
+    tlc_wait(x, ids, wts, out);                           // (which weights it takes depends on the routing)
+    const int pair = blockIdx.y, expert = ids[pair];
+    if (expert >= p.E) return;                            // an output of the router without weights
+    p.w += (size_t)expert * p.w_rows * p.ldw;
+    p.w_scale += (size_t)expert * p.w_rows;
+    x += (size_t)(pair / per_row) * p.lda;
+    out += (size_t)pair * p.ldo;
+    share = wts[pair];
+  }
+  if (item < items) {
+    rows_of(item);
+    fetch(0);
+  }
+  if (!GROUPED) tlc_wait(x, a_scale, out);
+  stage<MR>(x, p.lda, a_scale, GROUPED ? 1 : p.M, p.K, skinny_rows, ld, scale, red);
+  for (; item < items; item += warps) {
+    int acc[2][MR] = {};
+    for (int k0 = 0; k0 < p.K; k0 += 512 * AHEAD) {
+      int4 now[2][AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; j++) { now[0][j] = w[0][j]; now[1][j] = w[1][j]; }
+      // the next pieces, of this item or the next one, under these pieces' products
+      const int next = item + warps;
+      if (k0 + 512 * AHEAD < p.K) fetch(k0 + 512 * AHEAD);
+      else if (next < items) {
+        rows_of(next);
+        fetch(0);
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; j++) {
+        const int k = k0 + 512 * j + 16 * lane;
+        if (k0 + 512 * j >= p.K) break;
+#pragma unroll
+        for (int m = 0; m < MR; m++) {
+          const int4 a = k < ld ? *reinterpret_cast<const int4*>(skinny_rows + (size_t)m * ld + k) : make_int4(0, 0, 0, 0);
+          acc[0][m] = dot16(now[0][j], a, acc[0][m]);
+          acc[1][m] = dot16(now[1][j], a, acc[1][m]);
+        }
+      }
+    }
+    // lane 2 m + r (gated: lane m) takes row m's result of weight row r
+    int mine = 0, up = 0;
+#pragma unroll
+    for (int m = 0; m < MR; m++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const int sum = __reduce_add_sync(0xffffffffu, acc[r][m]);
+        if (GLU) {
+          if (lane == m) { if (r == 0) mine = sum; else up = sum; }
+        } else if (lane == 2 * m + r) {
+          mine = sum;
+        }
+      }
+    const int m = GLU ? lane : lane >> 1, n = GLU ? item : 2 * item + (lane & 1);
+    if (m < (GROUPED ? 1 : p.M) && n < p.N) {
+      TO* o = out + (size_t)m * p.ldo + n;
+      const float rs = GROUPED && p.w_out ? scale[m] * share : scale[m], pw = GROUPED && p.w_in ? share : 1.0f;
+      float v = int8_value(mine, rs, p.w_scale[n], p.colbias ? p.colbias[n] : 0.f);
+      if (GLU) {
+        const float u = int8_value(up, rs, p.w_scale[p.N + n], p.colbias ? p.colbias[p.N + n] : 0.f);
+        v = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, pw, v, u);
+      } else if (p.mode == I8_ACT) {
+        v = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, pw, v, 0.f);
+      } else if (p.mode == I8_ADD) {
+        v += to_f32(*o);
+      }
+      *o = from_f32<TO>(v);
+    }
+  }
+}
+
+template <typename TX, typename TO, int MR, bool GLU, bool GROUPED = false>
+int launch(const void* x, const Int8Args& p, const int* ids, int per_row, int sms, cudaStream_t stream) {
+  const size_t smem = (size_t)MR * ((p.K + 15) & ~15);       // (TLC_INT8_SKINNY and the rows' ends at most)
+  const int items = GLU ? p.N : (p.N + 1) / 2, places = GROUPED ? std::max(1, 2 * sms / p.M) : 2 * sms;
+  tlc_launch(int8_skinny_kernel<TX, TO, MR, GLU, GROUPED>, dim3(std::min((items + WARPS - 1) / WARPS, places), GROUPED ? p.M : 1), dim3(THREADS), smem,
+             stream, (const TX*)x, p, ids, per_row);
+  TLC_CHECK_LAUNCH("linear_int8 (up to 4 rows)");
+  return 0;
+}
+
+template <typename TX, typename TO>
+int launch_of(const void* x, const Int8Args& p, int sms, cudaStream_t stream) {
+#define TLC_SKINNY(MR_) (p.mode == I8_GLU ? launch<TX, TO, MR_, true>(x, p, nullptr, 1, sms, stream) : launch<TX, TO, MR_, false>(x, p, nullptr, 1, sms, stream))
+  return p.M == 1 ? TLC_SKINNY(1) : p.M == 2 ? TLC_SKINNY(2) : TLC_SKINNY(4);
+#undef TLC_SKINNY
+}
+
+template <typename TX, typename TO>
+int launch_pairs(const void* x, const Int8Args& p, const int* ids, int per_row, int sms, cudaStream_t stream) {
+  return p.mode == I8_GLU ? launch<TX, TO, 1, true, true>(x, p, ids, per_row, sms, stream) : launch<TX, TO, 1, false, true>(x, p, ids, per_row, sms, stream);
+}
+
+}  // namespace
+
+// x [M, p.lda] of x_dtype (TLC_I8: p.a_scale holds the scales).
+int tlc_int8_skinny(const void* x, int x_dtype, const Int8Args& p, int out_dtype, int sms, cudaStream_t stream) {
+  if (out_dtype == TLC_F32)
+    return x_dtype == TLC_I8 ? launch_of<int8_t, float>(x, p, sms, stream) : x_dtype == TLC_F32 ? launch_of<float, float>(x, p, sms, stream)
+                                                                          : launch_of<__nv_bfloat16, float>(x, p, sms, stream);
+  return x_dtype == TLC_I8 ? launch_of<int8_t, __nv_bfloat16>(x, p, sms, stream)
+                           : x_dtype == TLC_F32 ? launch_of<float, __nv_bfloat16>(x, p, sms, stream) : launch_of<__nv_bfloat16, __nv_bfloat16>(x, p, sms, stream);
+}
+
+// p.M pairs, each a product of its own: row pair / per_row of x (float or bfloat16), the weights of expert ids[pair], row `pair` of the result.
+int tlc_int8_skinny_pairs(const void* x, int x_dtype, const Int8Args& p, const int* ids, int per_row, int out_dtype, int sms, cudaStream_t stream) {
+  if (out_dtype == TLC_F32)
+    return x_dtype == TLC_F32 ? launch_pairs<float, float>(x, p, ids, per_row, sms, stream) : launch_pairs<__nv_bfloat16, float>(x, p, ids, per_row, sms, stream);
+  return x_dtype == TLC_F32 ? launch_pairs<float, __nv_bfloat16>(x, p, ids, per_row, sms, stream) : launch_pairs<__nv_bfloat16, __nv_bfloat16>(x, p, ids, per_row, sms, stream);
+}

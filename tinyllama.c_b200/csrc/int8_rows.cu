@@ -15,28 +15,11 @@
 // and a row that holds one gets the scale NaN and zeros, so that whatever is multiplied by it is NaN.  A row of zeros (or of values
 // below 127 x 2^-126) gets the scale 0.  Both divisions are IEEE's, not products with a reciprocal: with a largest magnitude of
 // 127 x 2^j, as one bfloat16 row in 128 has, v / s is often a half exactly, and the rounding to even should see it.
-#include "common.cuh"
+#include "int8_round.cuh"
 #include <algorithm>
 
 namespace {
 
-// Eight values as they lie in memory (a 16- or 32-byte piece), and as numbers: apart, so that all of a thread's loads are on their way
-// before the first is looked at.
-template <typename T> struct Piece;
-template <> struct Piece<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
-  __device__ __forceinline__ void numbers(float (&v)[8]) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w; }
-};
-template <> struct Piece<__nv_bfloat16> {
-  uint4 u;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void numbers(float (&v)[8]) const {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-  }
-};
 // Eight values from column k on, zeros past K, in any layout.
 template <typename T> __device__ __forceinline__ void row8(const T* x, int k, int K, float (&v)[8]) {
 #pragma unroll
@@ -45,27 +28,6 @@ template <typename T> __device__ __forceinline__ void row8(const T* x, int k, in
 __device__ __forceinline__ void store8(int8_t* q, int k, int K, uint2 n) {
 #pragma unroll
   for (int i = 0; i < 8; i++) if (k + i < K) q[k + i] = (int8_t)((i < 4 ? n.x : n.y) >> (8 * (i & 3)));
-}
-
-// The larger magnitude; a NaN stays.
-__device__ __forceinline__ float larger(float m, float v) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v)));
-  return m;
-}
-// Eight integers nearest to the quotients v / s (halves to even) as bytes, inv = 1 / s correctly rounded.  A first quotient v inv is
-// mended by its remainder, which a fused multiply-add gives exactly, times inv (Markstein, IBM Journal of Research and Development 34,
-// 1990): the IEEE quotient, without the general division's cases, which do not arise here (s is no denormal and |v / s| <= 127).
-// Adding 1.5 * 2^23 rounds it to an integer and leaves that in the sum's low bits; conversions would go through the special-function
-// unit, at a quarter of the rate.
-__device__ __forceinline__ uint2 eight_nearest(const float (&v)[8], float s, float inv) {
-  uint32_t b[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float first = __fmul_rn(v[i], inv), quotient = __fmaf_rn(__fmaf_rn(-first, s, v[i]), inv, first);
-    b[i] = __float_as_uint(__fadd_rn(quotient, 12582912.0f));
-  }
-  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
-                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
 // `warps` warps a row, blockDim / (32 warps) rows a block.  NI > 0: rows of pieces that start on 16-byte boundaries, at most NI a
@@ -130,11 +92,11 @@ int8_rows_kernel(const T* __restrict__ x, int ldx, int rows, int K, const float*
     if (NORM) sum = warp_sum(lane < warps ? red_sum[first + lane] : 0.f);
   }
   if (!there) return;
-  const float s = __fdiv_rn(__uint_as_float(largest), 127.0f), inv = __frcp_rn(s);
-  const bool finite = largest < 0x7f800000u, some = finite && s >= 1.17549435e-38f;
+  bool some;
+  const float s = int8_scale(largest, &some), inv = __frcp_rn(s);
   if (tid == 0) {
     const float r = NORM ? rsqrtf(sum / (float)K + eps) : 1.0f;
-    scale[row] = !finite ? __uint_as_float(0x7fc00000u) : some ? s * r : 0.f;
+    scale[row] = int8_told(largest, some, s * r);
   }
   if constexpr (NI > 0) {
 #pragma unroll

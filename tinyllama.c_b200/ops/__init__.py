@@ -163,7 +163,7 @@ _SIGNATURES = {
     "tlc_rows_int8": (_i, [_vp, _i, _i, _i, _i, _vp, _f, _vp, _i, _vp, _vp, _i, _i, _vp]),
     "tlc_linear_int8": (_i, [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _f, _f, _vp]),
     "tlc_linear_int8_kernel": (_i, [_i, _i]),
-    "tlc_moe_experts_int8": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i,
+    "tlc_moe_experts_int8": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i,
                                   _i, _i, _f, _f, _vp]),
     "tlc_argmax": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
     "tlc_sample": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _i, _f, _f, _f, _i, _f, _f, _vp, _vp]),
@@ -1459,9 +1459,7 @@ def moe_route(logits: torch.Tensor, n_experts: int, top: int, tile_rows: int = 3
         raise KernelError("moe_route: float32 logits [T, >= E]")
     dev = logits.device
     ints = torch.empty(2 * T * top + 2 * (n_experts + 1), dtype=torch.int32, device=dev)
-    ids, order = ints[:T * top], ints[T * top:2 * T * top]
-    offsets = ints[2 * T * top:2 * T * top + n_experts + 1]
-    tile_off = ints[2 * T * top + n_experts + 1:]
+    ids, order, offsets, tile_off = ints.split_with_sizes((T * top, T * top, n_experts + 1, n_experts + 1))
     wts = torch.empty(T * top, dtype=torch.float32, device=dev)
     global _launches
     _launches += 1                      # (two kernels)
@@ -1570,7 +1568,8 @@ INT8_MAX_K = 131071                      # 128 * 128 * K < 2^31: the sums of pro
 
 def linear_int8_kernel(kernel: int = 0, rows: int = 0) -> None:
     """Which kernel the products in 8-bit integers take where it takes the operands: 0 chosen by the sizes, 1 the CUDA cores, 2 tiles of
-    128 weight rows and `rows` (16, 32, 64 or 128) activation rows, 3 pairs of blocks on tiles of 128 or 256.  For tests."""
+    128 weight rows and `rows` (16, 32, 64 or 128) activation rows, 3 pairs of blocks on tiles of 128 or 256, 4 the kernel of up to 4 rows.
+    For tests."""
     lib = library()
     if lib.tlc_linear_int8_kernel(int(kernel), int(rows)) != 0:
         raise KernelError(f"linear_int8_kernel: {lib.tlc_last_error().decode()}")
@@ -1587,12 +1586,20 @@ def _rows_int8(x, what, norm_weight=None, eps=0.0, boundary=0):
     if x.dim() != 2 or x.shape[1] < 1:
         raise KernelError(f"{what}: rows [T, K] with K >= 1, got {tuple(x.shape)}")
     T, K = x.shape
+    weight = None
     if norm_weight is not None:
+        _gpu(norm_weight)
         _f32vec(norm_weight, K, what + " weight")
-    _gpu(x, norm_weight)
-    code, ldx = dtype_code(x.dtype), _rows(x, what + " input")
-    q, scale = int8_empty(T, K, x.device), torch.empty(T, dtype=torch.float32, device=x.device)
-    _call("tlc_rows_int8", x.data_ptr(), code, ldx, T, K, _p(norm_weight), eps, q.data_ptr(), (K + 15) // 16 * 16, scale.data_ptr(), None, 1,
+        weight = norm_weight.data_ptr()
+    if not x.is_cuda:
+        _gpu(x)
+    code, dev = dtype_code(x.dtype), x.device
+    ldx, dense = x.stride()
+    if T < 2 or (dense != 1 and K > 1):
+        ldx = _rows(x, what + " input")
+    q = torch.empty((T, K), dtype=torch.int8, device=dev) if K % 16 == 0 else int8_empty(T, K, dev)
+    scale = torch.empty(T, dtype=torch.float32, device=dev)
+    _call("tlc_rows_int8", x.data_ptr(), code, ldx, T, K, weight, eps, q.data_ptr(), (K + 15) // 16 * 16, scale.data_ptr(), None, 1,
           boundary, _stream())
     return q, scale
 
@@ -1702,21 +1709,22 @@ def moe_experts_int8(x: torch.Tensor, w_gate_up: torch.Tensor, gate_up_scale: to
     [T, top, D].  routing: what moe_route() or moe_route_tables() returned (for any number of rows a tile)."""
     if act_fn not in MOE_ACTS or weight_on not in ("input", "output"):
         raise KernelError(f"moe_experts_int8: unknown activation '{act_fn}' or weight placement '{weight_on}'")
-    _gpu(x, w_gate_up, gate_up_scale, w_down, down_scale, y)
     ids, wts, order, offsets = routing[:4]
-    T, D = x.shape
-    E, N, _ = w_gate_up.shape
-    F = w_down.shape[-1]
+    if x.dim() != 2:
+        raise KernelError(f"moe_experts_int8: rows [T, D], got {tuple(x.shape)}")
     ld_gu, ld_d = _expert_rows(w_gate_up, "moe_experts_int8 gate and up"), _expert_rows(w_down, "moe_experts_int8 down")
-    if N != (F if act_fn in UNGATED_ACTS else 2 * F) or w_gate_up.shape[2] != D or tuple(w_down.shape) != (E, D, F):
+    (T, D), (E, N, Dw), (Ed, Dd, F) = x.shape, w_gate_up.shape, w_down.shape
+    if N != (F if act_fn in UNGATED_ACTS else 2 * F) or Dw != D or Ed != E or Dd != D:
         raise KernelError(f"moe_experts_int8: shapes x{tuple(x.shape)} w_gate_up{tuple(w_gate_up.shape)} w_down{tuple(w_down.shape)} do not agree")
     if not (1 <= D <= INT8_MAX_K and 1 <= F <= INT8_MAX_K):
         raise KernelError(f"moe_experts_int8: rows of {D} and {F} values; the sums are exact for 1 to {INT8_MAX_K}")
     if weight_on == "input" and act_fn in UNGATED_ACTS:
         raise KernelError("moe_experts_int8: an expert without a gate is not linear before its activation: the weight goes on its output")
     pairs = T * top
-    if ids.numel() != pairs or order.numel() != pairs or offsets.numel() < E + 1:
+    if ids.numel() != pairs or order.numel() != pairs or wts.numel() != pairs or offsets.numel() < E + 1:
         raise KernelError(f"moe_experts_int8: a routing of {ids.numel()} pairs does not belong to {T} rows with {top} experts each of {E}")
+    if not (x.is_cuda and w_gate_up.is_cuda and w_down.is_cuda and y.is_cuda and gate_up_scale.is_cuda and down_scale.is_cuda and ids.is_cuda):
+        _gpu(x, w_gate_up, w_down, y, gate_up_scale, down_scale, ids)
     _f32vec(gate_up_scale, E * N, "moe_experts_int8 gate and up scale")
     _f32vec(down_scale, E * D, "moe_experts_int8 down scale")
     if not y.is_contiguous() or y.numel() != pairs * D:
@@ -1724,13 +1732,14 @@ def moe_experts_int8(x: torch.Tensor, w_gate_up: torch.Tensor, gate_up_scale: to
     # the rows' integers (the activation's after them in the same place), the activation, the rows' scales
     ldq = (max(D, F) + 15) // 16 * 16
     room = torch.empty(pairs * (ldq + 4 * F + 4), dtype=torch.int8, device=x.device)
-    _note_owned(room)
+    if _notes.calls is not None:
+        _note_owned(room)
     q = room.data_ptr()
     act = q + pairs * ldq
     _call("tlc_moe_experts_int8", x.data_ptr(), dtype_code(x.dtype), _rows(x, "moe_experts_int8 input"), w_gate_up.data_ptr(), ld_gu,
-          gate_up_scale.data_ptr(), w_down.data_ptr(), ld_d, down_scale.data_ptr(), order.data_ptr(), offsets.data_ptr(), wts.data_ptr(),
-          T, E, int(top), F, D, q, ldq, act + 4 * pairs * F, act, y.data_ptr(),
-          dtype_code(y.dtype), MOE_ACTS[act_fn], int(weight_on == "output"), float(limit), float(alpha), _stream())
+          gate_up_scale.data_ptr(), w_down.data_ptr(), ld_d, down_scale.data_ptr(), ids.data_ptr(), order.data_ptr(), offsets.data_ptr(),
+          wts.data_ptr(), T, E, top, F, D, q, ldq, act + 4 * pairs * F, act, y.data_ptr(), dtype_code(y.dtype), MOE_ACTS[act_fn],
+          1 if weight_on == "output" else 0, float(limit), float(alpha), _stream())
 
 
 def qk_whole_norm(qkv: torch.Tensor, q_off: int, q_n: int, q_weight: torch.Tensor, k_off: int, k_n: int, k_weight: torch.Tensor,
