@@ -23,6 +23,7 @@ from .parts import (ChunkRequest, KVRequest, LayerRun, LayerSpec, Part, PartSpec
                     register_feed_forward, register_mixer, register_norm, register_position)
 from .sampling import GREEDY, Sampler, SamplingParams
 from .weights import WeightError, build_model, load_model, write_random_model
+from .weights.loader import weight_format
 
 __all__ = ["LLM", "SamplingParams", "GREEDY", "load_model", "write_random_model", "Cache", "StepEntry", "step",
            "generate", "GenerationResult", "Continuation", "register_architecture", "register_mixer", "register_feed_forward",
@@ -37,15 +38,21 @@ class LLM:
     allows, at most 256)."""
 
     def __init__(self, model_dir, dtype: Union[str, torch.dtype] = "bfloat16", max_tokens: int = 8192,
-                 max_seqs: Optional[int] = None, device: str = "cuda:0", use_graphs: bool = True):
+                 max_seqs: Optional[int] = None, device: str = "cuda:0", use_graphs: bool = True, weights: Optional[str] = None):
         """model_dir: a folder with config.json and model.safetensors, or a model that is
-        already bound to its weights on `device` (see random_model)."""
+        already bound to its weights on `device` (see random_model).  weights "int8": the products of the layers in 8-bit
+        integers, weights with a scale per output channel and activations rounded row by row (a bound model's own too)."""
         if not torch.cuda.is_available():
             raise RuntimeError("tinyllama.c_b200 needs a CUDA device (NVIDIA B200); there is no CPU path")
         from . import ops
         ops.library()                                   # build / load the kernels now, loudly
         torch.cuda.set_device(torch.device(device))
-        self.model = load_model(model_dir, dtype, device) if isinstance(model_dir, (str, bytes)) else model_dir
+        if isinstance(model_dir, (str, bytes)):
+            self.model = load_model(model_dir, dtype, device, weights)
+        else:
+            self.model = model_dir
+            if weight_format(weights, self.model.dtype):
+                self.model.to_int8()
         self.config = self.model.config
         self.use_graphs = use_graphs
         self._graphs: dict = {}

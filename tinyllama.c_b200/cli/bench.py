@@ -30,7 +30,7 @@ def main(argv=None) -> int:
     n_tokens = max(1, args.tokens)
     ctx = args.ctx if args.ctx > 0 else None
     need = (len(prompt) + n_tokens + 63) // 64 * 64 * max(1, args.batch)
-    llm = tlc.LLM(args.model, dtype=args.dtype, max_tokens=max(need, 64), max_seqs=max(1, args.batch))
+    llm = tlc.LLM(args.model, dtype=args.dtype, max_tokens=max(need, 64), max_seqs=max(1, args.batch), weights=args.weights)
     if ctx:
         llm.max_context = min(llm.max_context, ctx)
     params = sampling_params(args)

@@ -24,7 +24,7 @@ def main(argv=None) -> int:
     args = ap.parse_args(argv)
     import tinyllama_c_b200 as tlc
     ctx = args.ctx if args.ctx > 0 else 0
-    llm = tlc.LLM(args.model, dtype=args.dtype, max_tokens=ctx or 4096, max_seqs=1)
+    llm = tlc.LLM(args.model, dtype=args.dtype, max_tokens=ctx or 4096, max_seqs=1, weights=args.weights)
     llm.max_context = ctx = min(ctx or llm.max_context, llm.max_context)
     params = sampling_params(args)
     system = parse_ids(args.system) if args.system else []

@@ -28,6 +28,7 @@ def add_common(ap: argparse.ArgumentParser, default_tokens: int) -> None:
     ap.add_argument("-fp", "--frequency-penalty", type=float, default=0.0)
     ap.add_argument("-pp", "--presence-penalty", type=float, default=0.0)
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weights", default=None, choices=["int8"], help="products of the layers in 8-bit integers (default: weights as stored)")
     ap.add_argument("--seed", type=int, default=0, help="seed of the sampler's draws")
     ap.add_argument("--ignore-eos", action="store_true", help="do not stop at the stop tokens")
 

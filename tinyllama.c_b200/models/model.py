@@ -134,6 +134,16 @@ class Model:
             self.head.bind(tensors, dtype, device)
         self.repeated = RepeatedLayers.of(self.layers, self.schedule) if self.device.type == "cuda" else None
 
+    def to_int8(self) -> None:
+        """The bound model with the weights of its layers' products in 8-bit integers, a scale per output channel; embedding, head,
+        norms, routers, convolutions and states stay as they are.  Once, before the first step."""
+        if self.dtype != torch.bfloat16:
+            raise ValueError("weights in 8-bit integers go with bfloat16 runs; a float32 run keeps its weights in 32 bits")
+        for layer in self.layers:
+            layer.to_int8()
+        self.expert_tables = ops.ExpertTables([p.table_entry() for p in self.by_table]) if self.by_table else None
+        self.repeated = RepeatedLayers.of(self.layers, self.schedule) if self.device.type == "cuda" else None
+
     # ---- forward ------------------------------------------------------------------------------
     def forward(self, step: StepInfo, cache, want_rows: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
         """Runs the step's rows through every scheduled layer; returns float32 logits

@@ -233,7 +233,7 @@ def _call(name: str, *args) -> None:
 REPEATABLE = frozenset(("tlc_event_record", "tlc_event_wait", "tlc_rmsnorm", "tlc_gated_rmsnorm", "tlc_gated_rmsnorm_step", "tlc_linear",
                         "tlc_linear_swiglu", "tlc_glu", "tlc_rope_kv_store", "tlc_attention", "tlc_attention_decode",
                         "tlc_attention_decode_fused", "tlc_attention_prefill", "tlc_attention_prefill_tc", "tlc_mamba_conv", "tlc_mamba_step",
-                        "tlc_ssm_scan", "tlc_ssm_scan_one_row", "tlc_ssm_scan_chunked", "tlc_ssm_scan_ssd"))
+                        "tlc_ssm_scan", "tlc_ssm_scan_one_row", "tlc_ssm_scan_chunked", "tlc_ssm_scan_ssd", "tlc_rows_int8", "tlc_linear_int8"))
 
 
 class NotedCalls:
@@ -1582,7 +1582,7 @@ def int8_empty(rows: int, k: int, device) -> torch.Tensor:
     return torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
 
 
-def _rows_int8(x, what, norm_weight=None, eps=0.0, boundary=0):
+def _rows_int8(x, what, out=None, norm_weight=None, eps=0.0, boundary=0):
     if x.dim() != 2 or x.shape[1] < 1:
         raise KernelError(f"{what}: rows [T, K] with K >= 1, got {tuple(x.shape)}")
     T, K = x.shape
@@ -1597,23 +1597,31 @@ def _rows_int8(x, what, norm_weight=None, eps=0.0, boundary=0):
     ldx, dense = x.stride()
     if T < 2 or (dense != 1 and K > 1):
         ldx = _rows(x, what + " input")
-    q = torch.empty((T, K), dtype=torch.int8, device=dev) if K % 16 == 0 else int8_empty(T, K, dev)
-    scale = torch.empty(T, dtype=torch.float32, device=dev)
-    _call("tlc_rows_int8", x.data_ptr(), code, ldx, T, K, weight, eps, q.data_ptr(), (K + 15) // 16 * 16, scale.data_ptr(), None, 1,
-          boundary, _stream())
+    if out is None:
+        q = torch.empty((T, K), dtype=torch.int8, device=dev) if K % 16 == 0 else int8_empty(T, K, dev)
+        scale = torch.empty(T, dtype=torch.float32, device=dev)
+        ldq = (K + 15) // 16 * 16
+    else:
+        q, scale = out
+        _gpu(q, scale)
+        if q.dtype != torch.int8:
+            raise KernelError(f"{what}: integers go to an int8 tensor, got {q.dtype}")
+        ldq = _out_rows(q, T, K, what)
+        _f32vec(scale, T, what + " scale")
+    _call("tlc_rows_int8", x.data_ptr(), code, ldx, T, K, weight, eps, q.data_ptr(), ldq, scale.data_ptr(), None, 1, boundary, _stream())
     return q, scale
 
 
-def rows_int8(x: torch.Tensor):
+def rows_int8(x: torch.Tensor, out=None):
     """(q int8 [T, K], scale float32 [T]) of float32 or bfloat16 rows: scale[t] = max_k |x[t, k]| / 127, q = x / scale rounded to the
     nearest integer (halves to even).  A row of zeros has scale 0; one that holds a NaN or an infinity has scale NaN and integers 0.
-    q is an operand a of linear_int8; for weights see weight_int8."""
-    return _rows_int8(x, "rows_int8")
+    q is an operand a of linear_int8; for weights see weight_int8.  out: (q, scale) to write to."""
+    return _rows_int8(x, "rows_int8", out)
 
 
-def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float):
+def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out=None):
     """rows_int8 of the RMS norm x / sqrt(mean(x^2) + eps) * weight of every row, in one pass; weight float32 [K]."""
-    return _rows_int8(x, "rmsnorm_int8", weight, float(eps))
+    return _rows_int8(x, "rmsnorm_int8", out, weight, float(eps))
 
 
 def weight_int8(w: torch.Tensor):

@@ -128,6 +128,29 @@ class Block(Part):
                     self.out_offsets.append((off, pr.in_features))
                     off += pr.in_features
 
+    def to_int8(self) -> None:
+        """The layer's products in 8-bit integers: projections that its mixers share as one matrix (the mixers' own are ranges of
+        it then too), other mixers' and the feed-forward's by themselves.  The norm in front of a product that its part shares with
+        nobody leaves integers at once (_pre_norm)."""
+        for fused, mine in ((self.fused_in, lambda m: m.input_projection()), (self.fused_out, lambda m: m.output_projection())):
+            if fused is None or fused.weight.dtype != torch.bfloat16:
+                continue
+            fused.to_int8()
+            off = 0
+            for i, m in enumerate(self.mixers):
+                pr = mine(m)
+                if fused is self.fused_in:                  # rows of the fused matrix
+                    pr.weight, pr.int8_scale = fused.weight[off:off + pr.out_features], fused.int8_scale[off:off + pr.out_features]
+                    off += pr.out_features
+                else:                                       # columns of it; a part's scale went into its input (out_scales)
+                    pr.weight, pr.int8_scale = fused.weight[:, off:off + pr.in_features], fused.int8_scale * self.out_scales[i]
+                    off += pr.in_features
+                pr.colscale = None
+        for m in self.mixers:
+            m.to_int8()                                     # (what is integers already stays so)
+        if self.ffn is not None:
+            self.ffn.to_int8()
+
     def _make_sides(self, device) -> None:
         if not hasattr(self, "_side"):
             self._side = [torch.cuda.Stream(device=device) for _ in self.mixers[1:]]
@@ -336,7 +359,12 @@ class Block(Part):
             return self._leave(next_entry, x32, "block.normed", adds)
         return {} if self.parallel_ffn else self._leave(self.ffn_norm, x32, "block.ffn_normed", adds)
 
-    def _pre_norm(self, norm, x32: torch.Tensor, tag: str, step: StepInfo, cache: LayerCache) -> torch.Tensor:
+    def _pre_norm(self, norm, x32: torch.Tensor, tag: str, step: StepInfo, cache: LayerCache, int8: bool = False):
+        """int8: whoever reads it multiplies by weights in 8 bits and nothing else: behind a plain RMS norm (integers, scales)."""
+        if int8 and type(norm) is RMSNorm and tag not in self._copied:
+            T, D = x32.shape
+            room = scratch_buf(tag + ".int8", (T, (D + 15) // 16 * 16), torch.int8, x32.device)
+            return ops.rmsnorm_int8(x32, norm.weight, norm.eps, (room[:, :D], scratch_buf(tag + ".scale", (T,), torch.float32, x32.device)))
         normed = scratch_buf(tag, x32.shape, self.dtype, x32.device)
         if tag in self._copied:                       # filled by the kernel that last added into the stream
             self._copied.discard(tag)
@@ -371,7 +399,8 @@ class Block(Part):
             self.mixer_out_norm.add_normed(y, x32, **left)
         elif self.mixers:
             normed, ffn_in = self._parallel_inputs(x32, step, cache) if self.parallel_ffn \
-                else (self._pre_norm(self.mixer_norm, x32, "block.normed", step, cache), None)
+                else (self._pre_norm(self.mixer_norm, x32, "block.normed", step, cache,
+                                     self.fused_in is not None and self.fused_in.int8_scale is not None), None)
             if self._beside(x32, step):
                 self._two_branches(normed, x32, lambda: self._run_mixers(normed, x32, step, cache), ffn_in, self._ffn_more(step))
                 return False
@@ -407,7 +436,7 @@ class Block(Part):
     def _feed_forward(self, x32: torch.Tensor, step: StepInfo, cache: LayerCache, next_entry=None) -> bool:
         """A feed-forward with a norm of its own, after the mixers.  Returns whether the kernel that added its result
         also left the next layer's input (next_entry)."""
-        normed = self._pre_norm(self.ffn_norm, x32, "block.ffn_normed", step, cache)
+        normed = self._pre_norm(self.ffn_norm, x32, "block.ffn_normed", step, cache, getattr(self.ffn, "takes_int8", False))
         left = self._leave(next_entry, x32, "block.normed", self.ffn_out_norm) if self.ffn_out_norm is not None else {}
         # without a norm in front, a feed-forward that can use them (takes_stream) also gets the 32-bit rows themselves
         more = self._ffn_more(step)

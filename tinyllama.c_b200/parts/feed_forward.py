@@ -54,6 +54,7 @@ class SwiGLU(Part):
     def bind(self, tensors: Dict[str, torch.Tensor], dtype, device) -> None:
         self.gate_up.bind(tensors, dtype, device)
         self.down.bind(tensors, dtype, device)
+        self.act_dtype = dtype
         # Rows regrouped as 8 gate rows followed by their 8 up rows, so that the product's epilogue
         # has a feature's gate and up side by side and writes silu(gate) * up directly.
         self.interleaved = self.F % 8 == 0
@@ -66,18 +67,40 @@ class SwiGLU(Part):
             if self.gate_up.colbias is not None:
                 self.gate_up.colbias = self.gate_up.colbias[idx].contiguous()
 
+    def to_int8(self) -> None:
+        if self.interleaved and self.gate_up.weight.dtype == torch.bfloat16:
+            # the 8-bit product takes the gate's rows, then the up projection's, as they are stored
+            F = self.F
+            idx = torch.arange(2 * F, device=self.gate_up.weight.device).reshape(F // 8, 2, 8).permute(1, 0, 2).reshape(-1)
+            for name in ("weight", "colscale", "colbias"):
+                v = getattr(self.gate_up, name)
+                if v is not None:
+                    setattr(self.gate_up, name, v[idx].contiguous())
+            self.interleaved = False
+        self.gate_up.to_int8()
+        self.down.to_int8()
+
+    @property
+    def takes_int8(self) -> bool:
+        """Whether forward() takes rows that are rounded already (integers, scales)."""
+        return self.gate_up.int8_scale is not None
+
     def repeats(self):
         return frozenset()
 
-    def forward(self, normed: torch.Tensor, residual: torch.Tensor, accumulate: bool = True) -> None:
+    def forward(self, normed, residual: torch.Tensor, accumulate: bool = True) -> None:
         """Adds the result into `residual` (float32 [T, D]), or overwrites it with accumulate False."""
-        T = normed.shape[0]
-        act = scratch_buf("swiglu.act", (T, self.F), normed.dtype, normed.device)
-        if self.interleaved:
+        T = residual.shape[0]
+        act = scratch_buf("swiglu.act", (T, self.F), self.act_dtype if isinstance(normed, tuple) else normed.dtype, residual.device)
+        if self.gate_up.int8_scale is not None:
+            rows, a_scale = normed if isinstance(normed, tuple) else (normed, None)
+            ops.linear_swiglu_int8(rows, self.gate_up.weight, self.gate_up.int8_scale, act, a_scale, self.gate_up.colbias, self.act,
+                                   self.limit, self.alpha)
+        elif self.interleaved:
             ops.linear_swiglu(normed, self.gate_up.weight, act, self.gate_up.colscale, self.gate_up.colbias, self.act,
                               self.limit, self.alpha)
         else:
-            gu = scratch_buf("swiglu.gate_up", (T, 2 * self.F), torch.float32, normed.device)
+            gu = scratch_buf("swiglu.gate_up", (T, 2 * self.F), torch.float32, residual.device)
             self.gate_up.forward(normed, gu)
             ops.glu(gu, act, self.act, interleaved=self.interleaved, limit=self.limit, alpha=self.alpha)
         self.down.forward(act, residual, accumulate=accumulate)
@@ -261,14 +284,24 @@ class MoEFeedForward(Part):
         else:                                    # [E, F, D]: one product an expert
             self.w_gate_up = torch.stack([to(tensors[n["up"]]) for n in names]).contiguous()
         self.w_down = torch.stack([to(tensors[n["down"]]) for n in names]).contiguous()
+        self.gate_up_scale = self.down_scale = None      # of every output channel, where the experts' weights are integers
         if self.shared is not None:
             self.shared.bind(tensors, dtype, device)
+
+    def to_int8(self) -> None:
+        """The experts' weights and the shared expert's; the router stays in its own type."""
+        if self.w_gate_up.dtype == torch.bfloat16:
+            self.w_gate_up, self.gate_up_scale = ops.weight_int8(self.w_gate_up)
+            self.w_down, self.down_scale = ops.weight_int8(self.w_down)
+            self.expert_tables = None
+        if self.shared is not None:
+            self.shared.to_int8()
 
     takes_stream = True        # forward(..., stream=x32): an expert that returns its input returns the 32-bit rows
 
     def table_entry(self):
         """This part's table as ops.ExpertTables takes it."""
-        return self.table, self.E, ops.moe_tiles_of_64(self.w_gate_up, self.dtype, self.F)
+        return self.table, self.E, self.gate_up_scale is None and ops.moe_tiles_of_64(self.w_gate_up, self.dtype, self.F)
 
     @staticmethod
     def route_step(parts, tables, step) -> None:
@@ -288,7 +321,8 @@ class MoEFeedForward(Part):
                     self.expert_tables = ops.ExpertTables([self.table_entry()])
                 routing = ops.moe_route_tables(step.tokens, self.expert_tables)[0]
             return routing, None
-        tile_rows = ops.moe_tile_rows(normed, self.w_gate_up, self.dtype, self.top, self.F)
+        # (the products in 8-bit integers make tiles of their own)
+        tile_rows = ops.moe_tile_rows(normed, self.w_gate_up, self.dtype, self.top, self.F) if self.gate_up_scale is None else 32
         logits = scratch_buf("moe.logits", (normed.shape[0], self.router.shape[0]), torch.float32, normed.device)
         ops.linear(normed, self.router, logits, None, self.router_bias)
         return ops.moe_route(logits, self.n_out, self.top, tile_rows, self.weights, self.choice_bias, self.n_identity,
@@ -308,10 +342,14 @@ class MoEFeedForward(Part):
                     self._side = SideStream(dev)
                 side = self._side
                 side.run(lambda: self.shared.forward(normed, shared_out, accumulate=False))
-        act = scratch_buf("moe.act", (T * self.top, self.F), self.dtype, dev)
         parts = scratch_buf("moe.parts", (T, self.top, self.hidden), torch.float32, dev)
-        ops.moe_experts(normed, self.w_gate_up, self.w_down, routing, self.top, act, parts, self.act, self.weight_on, self.limit,
-                        self.alpha)
+        if self.gate_up_scale is not None:
+            ops.moe_experts_int8(normed, self.w_gate_up, self.gate_up_scale, self.w_down, self.down_scale, routing, self.top, parts, self.act,
+                                 self.weight_on, self.limit, self.alpha)
+        else:
+            act = scratch_buf("moe.act", (T * self.top, self.F), self.dtype, dev)
+            ops.moe_experts(normed, self.w_gate_up, self.w_down, routing, self.top, act, parts, self.act, self.weight_on, self.limit,
+                            self.alpha)
         if self.n_identity:
             ops.moe_identity(stream if stream is not None else normed, routing, self.top, self.E, parts)
         if self.shared is None:

@@ -39,6 +39,7 @@ class StackedLinear(Editable):
             raise ValueError(f"padded input heads {self.in_heads} do not make {self.in_features} input values")
         self.segments: List[dict] = []
         self.weight: Optional[torch.Tensor] = None
+        self.int8_scale: Optional[torch.Tensor] = None      # of every output channel, where the weight is integers
         self.colscale: Optional[torch.Tensor] = None
         self.colbias: Optional[torch.Tensor] = None
 
@@ -123,6 +124,7 @@ class StackedLinear(Editable):
             self.weight = mats[0].to(device=device, dtype=mdt).contiguous()
         else:
             self.weight = torch.cat([m.to(device=device, dtype=mdt) for m in mats], dim=0).contiguous()
+        self.int8_scale = None
         scale = torch.ones(self.out_features, dtype=torch.float64)
         bias = torch.zeros(self.out_features, dtype=torch.float64)
         any_scale = any_bias = False
@@ -143,10 +145,24 @@ class StackedLinear(Editable):
     def repeats(self):
         return frozenset(("segments",))
 
-    def forward(self, x: torch.Tensor, out: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
+    def to_int8(self) -> None:
+        """From here on the weight is integers [out, in] in 8 bits with a scale per output channel (int8_scale, the column
+        scale in it) and forward() rounds its rows.  A matrix that is kept in 32 bits stays as it is."""
+        if self.weight.dtype != torch.bfloat16:
+            return
+        self.weight, self.int8_scale = ops.weight_int8(self.weight)
+        if self.colscale is not None:
+            self.int8_scale, self.colscale = self.int8_scale * self.colscale, None
+
+    def forward(self, x, out: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
+        """x: rows [T, in]; for weights in 8 bits also (integers, scales) of rows that are rounded already."""
         # a part of a product fused along K keeps its weight as a column range of the fused matrix; used on
         # its own (a mixer outside its block) it multiplies by a dense copy
         w = self.weight
+        if self.int8_scale is not None:
+            rows, a_scale = x if isinstance(x, tuple) else (x, None)
+            ops.linear_int8(rows, w, self.int8_scale, out, a_scale, self.colbias, accumulate)
+            return out
         if not w.is_contiguous():
             w = w.contiguous()
             ops.cannot_repeat()

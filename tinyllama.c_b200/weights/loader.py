@@ -80,9 +80,20 @@ def normalise(t: torch.Tensor) -> torch.Tensor:
     return t.to(torch.float32)
 
 
-def load_model(model_dir: str, dtype: Union[str, torch.dtype] = "bfloat16", device="cuda") -> Model:
-    """Model folder -> model bound to its weights on `device`, computing in `dtype`."""
+def weight_format(weights: Optional[str], dtype: torch.dtype) -> bool:
+    """Whether weights are to be laid out as 8-bit integers; raises on a format there is none of, or that `dtype` does not go with."""
+    if weights not in (None, "int8"):
+        raise ValueError(f"weights must be None (as stored) or 'int8', got {weights!r}")
+    if weights == "int8" and dtype != torch.bfloat16:
+        raise ValueError("weights 'int8' go with dtype bfloat16")
+    return weights == "int8"
+
+
+def load_model(model_dir: str, dtype: Union[str, torch.dtype] = "bfloat16", device="cuda", weights: Optional[str] = None) -> Model:
+    """Model folder -> model bound to its weights on `device`, computing in `dtype`.  weights "int8": the layers' products
+    in 8-bit integers (Model.to_int8)."""
     rd = run_dtype(dtype)
+    int8 = weight_format(weights, rd)
     config = load_config(model_dir)
     model = build_model(config)
     try:
@@ -92,6 +103,8 @@ def load_model(model_dir: str, dtype: Union[str, torch.dtype] = "bfloat16", devi
     model.adopt_shapes({k: tuple(v.shape) for k, v in tensors.items()})     # sizes that only a tensor's shape gives
     check_tensors(model, tensors)
     model.bind({k: normalise(v) for k, v in tensors.items()}, rd, torch.device(device))
+    if int8:
+        model.to_int8()
     return model
 
 
