@@ -210,6 +210,7 @@ extern "C" int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_sca
   const bool skinny = M <= (a_dtype == TLC_I8 ? 4 : 2) && (long long)p.w_rows * K <= 24 << 20;
   if (takes && (g_kernel == 0 ? skinny : g_kernel == 4)) return tlc_int8_skinny(a, a_dtype, p, out_dtype, sm_count(), stream);
   if (a_dtype != TLC_I8) {
+    if (!a_int8 || !a_scale) return 1;                     // (room is wanted)
     if (int rc = tlc_rows_int8(a, a_dtype, lda, M, K, nullptr, 0.f, a_int8, ld_int8, a_scale, nullptr, 1, 0, stream)) return rc;
     p.a = (const int8_t*)a_int8;
     p.lda = ld_int8;

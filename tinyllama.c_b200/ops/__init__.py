@@ -212,16 +212,21 @@ def count_launches(n: int) -> None:
     _launches += int(n)
 
 
-def _call(name: str, *args) -> None:
+def _call(name: str, *args, ok: int = 0) -> bool:
+    """Makes a call of the library.  ok > 0: the code by which the library may say that it did nothing; returns whether it did."""
     global _launches
     lib = library()
     _launches += 1
     rc = getattr(lib, name)(*args)
     if rc != 0:
+        if ok and rc == ok:
+            _launches -= 1
+            return False
         raise KernelError(f"{name}: {lib.tlc_last_error().decode()}")
     notes = _notes.calls
     if notes is not None:
         notes.add(name, args)
+    return True
 
 
 # ---- calls made again --------------------------------------------------------------------
@@ -1670,13 +1675,21 @@ def _linear_int8(what, a, a_scale, w, w_scale, colbias, out, N, accumulate, act,
         if a_scale is not None:
             raise KernelError(f"{what}: a_scale belongs to integer rows; a is {a.dtype}")
         code, ldq = dtype_code(a.dtype), (K + 15) // 16 * 16
-        room = torch.empty(M * (ldq + 4), dtype=torch.int8, device=a.device)       # the rows' integers, then their scales
-        if _notes.calls is not None:
-            _note_owned(room)
-        q = room.data_ptr()
-        scale = q + M * ldq
-    _call("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, w.data_ptr(), ldw, w_scale.data_ptr(), out.data_ptr(),
-          dtype_code(out.dtype), ldo, bias, accumulate, M, N, K, act, limit, alpha, _stream())
+        scale = q = None
+        if M > 2:                                        # (one or two rows mostly go without; the library says so where not)
+            scale, q = _int8_room(M, ldq, a.device)
+    args = (w.data_ptr(), ldw, w_scale.data_ptr(), out.data_ptr(), dtype_code(out.dtype), ldo, bias, accumulate, M, N, K, act, limit, alpha, _stream())
+    if not _call("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, *args, ok=1):
+        scale, q = _int8_room(M, ldq, a.device)
+        _call("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, *args)
+
+
+def _int8_room(M: int, ld: int, device):
+    """Addresses of room for the scales and the integers [M, ld] of rows that a product rounds first."""
+    room = torch.empty(M * (ld + 4), dtype=torch.int8, device=device)
+    if _notes.calls is not None:
+        _note_owned(room)
+    return room.data_ptr() + M * ld, room.data_ptr()
 
 
 def linear_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: torch.Tensor, a_scale: Optional[torch.Tensor] = None,
@@ -1703,9 +1716,11 @@ def linear_swiglu_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, 
 
 def _expert_rows(w: torch.Tensor, what: str) -> int:
     """Row stride of matrices [E, N, K] of integers whose rows are dense and follow one another."""
-    if w.dim() != 3 or w.dtype != torch.int8 or (w.shape[2] > 1 and w.stride(2) != 1)             or (w.shape[0] > 1 and w.stride(0) != w.shape[1] * w.stride(1)):
-        raise KernelError(f"{what}: int8 [E, N, K] with dense rows one after the other, got {tuple(w.shape)} {w.dtype} strides {w.stride()}")
-    return w.stride(1)
+    if w.dtype == torch.int8 and w.dim() == 3:
+        (E, N, K), (se, sn, sk) = w.shape, w.stride()
+        if (sk == 1 or K == 1) and (se == N * sn or E == 1):
+            return sn
+    raise KernelError(f"{what}: int8 [E, N, K] with dense rows one after the other, got {tuple(w.shape)} {w.dtype} strides {w.stride()}")
 
 
 def moe_experts_int8(x: torch.Tensor, w_gate_up: torch.Tensor, gate_up_scale: torch.Tensor, w_down: torch.Tensor, down_scale: torch.Tensor,
