@@ -100,7 +100,7 @@ int8_tile_kernel(Int8Args p) {
         float u = 0.f;
         if (GLU)
           u = int8_value(acc[NW - 1][i][j], rs, p.w_scale[w0 + p.N + n], p.colbias ? p.colbias[p.N + n] : 0.f);
-        v = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, pw, v, u);
+        v = int8_gated(p, p.w_in, pw, v, u);
       } else if (p.mode == I8_ADD) {
         v += to_f32(o[n]);
       }

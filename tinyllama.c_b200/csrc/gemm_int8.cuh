@@ -28,3 +28,20 @@ enum { I8_PLAIN = 0, I8_ADD = 1, I8_ACT = 2, I8_GLU = 3 };
 __device__ __forceinline__ float int8_value(int sum, float row_scale, float col_scale, float bias) {
   return __fmaf_rn(__fmul_rn(__int2float_rn(sum), row_scale), col_scale, bias);
 }
+
+// A gated activation as all kernels here make it; w: the pair's weight on gate and up, where it goes there.  SiLU is g / (1 + 2^(-g log2 e)) by
+// the special-function unit's power and reciprocal (a few units in the last place of 32 bits), written out because the general
+// forms also mend results below 2^-126, which nothing here needs.
+__device__ __forceinline__ float int8_silu(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return __fmul_rn(__fmul_rn(g, r), u);
+}
+__device__ __forceinline__ float int8_gated(const Int8Args& p, bool weighted, float w, float g, float u) {
+  if (weighted) {
+    g = __fmul_rn(g, w);
+    u = __fmul_rn(u, w);
+  }
+  return p.act == TLC_ACT_SILU ? int8_silu(g, u) : moe_pair_act<true>(p.act, 1, p.limit, p.alpha, 1.0f, g, u);
+}

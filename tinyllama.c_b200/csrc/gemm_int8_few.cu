@@ -201,11 +201,11 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const float u = __shfl_down_sync(0xffffffffu, v[i], 2);
-          v[i] = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, pw, v[i], u);
+          v[i] = int8_gated(p, GROUPED && p.w_in, pw, v[i], u);
         }
       } else if (p.mode == I8_ACT) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, pw, v[i], 0.f);
+        for (int i = 0; i < 4; i++) v[i] = int8_gated(p, GROUPED && p.w_in, pw, v[i], 0.f);
       } else if (p.mode == I8_ADD) {
 #pragma unroll
         for (int i = 0; i < 4; i++) if (writes && c0 + i < p.N) v[i] += to_f32(o[i]);

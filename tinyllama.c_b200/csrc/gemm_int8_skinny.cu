@@ -187,9 +187,9 @@ int8_skinny_kernel(const TX* __restrict__ x, Int8Args p, const int* __restrict__
       float v = int8_value(mine, rs, p.w_scale[n], p.colbias ? p.colbias[n] : 0.f);
       if (GLU) {
         const float u = int8_value(up, rs, p.w_scale[p.N + n], p.colbias ? p.colbias[p.N + n] : 0.f);
-        v = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, pw, v, u);
+        v = int8_gated(p, GROUPED && p.w_in, pw, v, u);
       } else if (p.mode == I8_ACT) {
-        v = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, pw, v, 0.f);
+        v = int8_gated(p, GROUPED && p.w_in, pw, v, 0.f);
       } else if (p.mode == I8_ADD) {
         v += to_f32(*o);
       }

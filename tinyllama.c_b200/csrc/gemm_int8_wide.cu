@@ -204,7 +204,7 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       cs = n_cs;
       cb = n_cb;
       const int col = column(at);                       // of the result
-      const bool in = col < p.N;
+      const bool in = col < p.N, inside = (GLU ? (at.n + I8_ROWS) / 2 : at.n + I8_ROWS) <= p.N;
       __syncwarp();                                     // (the last tile's numbers have been read)
 #pragma unroll
       for (int c = 0; c < CHUNKS; c++) {
@@ -244,42 +244,49 @@ int8_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
           if (lane == 0) mbar_arrive_cluster_relaxed(cluster_address(acc_empty0 + 8 * as, 0));
         }
         if (left <= 0) continue;
-        // where this lane writes row j + mine of the piece (grouped: by the row's own index)
+        // where this lane writes row j + mine of the piece: the rows' own places, or one row after the other
         TO* base = out + (size_t)(at.row0 + m0) * p.ldo + col;
-        auto target = [&](const int j, const int mine) {
-          return GROUPED ? out + (size_t)to[m1 + j + mine] * p.ldo + col : base + (unsigned)((j + mine) * p.ldo);
-        };
-        if constexpr (GLU) {
-          const int mine = is_up ? 1 : 0;
-          auto gated = [&](const auto act_of) {
+        auto leave = [&](const bool whole) {            // whole: every row and column of the piece is there
+          if constexpr (GLU) {
+            const int mine = is_up ? 1 : 0;
+            TO* t = base + (size_t)mine * p.ldo;
+            auto gated = [&](const auto act_of) {
 #pragma unroll
-            for (int j = 0; j < PIECE; j += 2) {        // of rows j and j + 1 the gate's lanes finish the first, the up projection's the second
-              const float other = __shfl_xor_sync(0xffffffffu, is_up ? v[j] : v[j + 1], 8);
-              const float w = GROUPED ? pw[m1 + j + mine] : 1.0f;
-              const float y = act_of(w, is_up ? other : v[j], is_up ? v[j + 1] : other);
-              TO* t = target(j, mine);
-              if (in && j + mine < left) *t = from_f32<TO>(y);
+              for (int j = 0; j < PIECE; j += 2) {      // of rows j and j + 1 the gate's lanes finish the first, the up projection's the second
+                const float other = __shfl_xor_sync(0xffffffffu, is_up ? v[j] : v[j + 1], 8);
+                const float y = act_of(is_up ? other : v[j], is_up ? v[j + 1] : other, j + mine);
+                if (whole || (in && j + mine < left)) t[(unsigned)(j * p.ldo)] = from_f32<TO>(y);
+              }
+            };
+            if (p.act == TLC_ACT_SILU && !(GROUPED && p.w_in)) gated([&](float g, float u, int) { return int8_silu(g, u); });
+            else gated([&](float g, float u, int j) { return int8_gated(p, GROUPED && p.w_in, GROUPED ? pw[m1 + j] : 1.0f, g, u); });
+          } else if constexpr (GROUPED) {
+#pragma unroll
+            for (int j = 0; j < PIECE; j += 4) {
+              const int4 rows = *reinterpret_cast<const int4*>(to + m1 + j);
+              const int place_of[4] = {rows.x, rows.y, rows.z, rows.w};
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                if (whole || (in && j + e < left)) out[(size_t)place_of[e] * p.ldo + col] = from_f32<TO>(v[j + e]);
             }
-          };
-          if (p.act == TLC_ACT_SILU) gated([&](float w, float g, float u) { return GROUPED ? moe_pair_act<true>(TLC_ACT_SILU, 0, 0.f, 1.f, w, g, u) : silu_quick(g) * u; });
-          else gated([&](float w, float g, float u) { return moe_pair_act<true>(p.act, 0, p.limit, p.alpha, w, g, u); });
-        } else {
-          if (p.mode == I8_ACT) {
+          } else {
 #pragma unroll
-            for (int j = 0; j < PIECE; j++) v[j] = moe_pair_act<true>(p.act, 0, p.limit, p.alpha, GROUPED ? pw[m1 + j] : 1.0f, v[j], 0.f);
-          } else if (p.mode == I8_ADD) {
-            float old[PIECE];                           // (all in flight before the first is added)
-#pragma unroll
-            for (int j = 0; j < PIECE; j++) old[j] = in && j < left ? to_f32(*target(j, 0)) : 0.f;
-#pragma unroll
-            for (int j = 0; j < PIECE; j++) v[j] += old[j];
+            for (int j = 0; j < PIECE; j++)
+              if (whole || (in && j < left)) base[(unsigned)(j * p.ldo)] = from_f32<TO>(v[j]);
           }
+        };
+        if (!GLU && p.mode == I8_ACT) {
 #pragma unroll
-          for (int j = 0; j < PIECE; j++) {
-            TO* t = target(j, 0);
-            if (in && j < left) *t = from_f32<TO>(v[j]);
-          }
+          for (int j = 0; j < PIECE; j++) v[j] = int8_gated(p, GROUPED && p.w_in, GROUPED ? pw[m1 + j] : 1.0f, v[j], 0.f);
+        } else if (!GLU && !GROUPED && p.mode == I8_ADD) {
+          float old[PIECE];                             // (all in flight before the first is added)
+#pragma unroll
+          for (int j = 0; j < PIECE; j++) old[j] = in && j < left ? to_f32(base[(unsigned)(j * p.ldo)]) : 0.f;
+#pragma unroll
+          for (int j = 0; j < PIECE; j++) v[j] += old[j];
         }
+        if (left >= PIECE && inside) leave(true);
+        else leave(false);
       }
     }
   }
