@@ -15,18 +15,16 @@
 // Both products work on tiles of 32 sorted rows of ONE expert; the grid is an upper bound (pairs / 32 + experts in
 // use) and a block past the last tile returns.
 #include "common.cuh"
+#include <algorithm>
 
 #define MOE_TM 32
 
 // A warp per token: its `top` experts by descending logit (lowest index first on ties) and their weights.  In every pass a
 // lane finds the best of its experts (lane, lane + 32, ...) that come after the last choice in that order, and the
 // warp the best of the lanes.
-__global__ void __launch_bounds__(128)
-moe_topk_kernel(const float* __restrict__ logits, int ld, int T, int E, int top, int mode, const float* __restrict__ choice_bias,
-                int* __restrict__ ids, float* __restrict__ wts, float sum_to) {
-  tlc_pdl(logits, ids, wts);
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (t >= T) return;
+__device__ __forceinline__ void moe_topk(const float* __restrict__ logits, int ld, int t, int E, int top, int mode, const float* __restrict__ choice_bias,
+                                         int* __restrict__ ids, float* __restrict__ wts, float sum_to) {
+  const int lane = threadIdx.x & 31;
   const float* lr = logits + (size_t)t * ld;
   float last = INFINITY, first = 0.f, sum = 0.f;
   int last_e = -1;
@@ -91,6 +89,14 @@ moe_topk_kernel(const float* __restrict__ logits, int ld, int T, int E, int top,
   }
 }
 
+__global__ void __launch_bounds__(128)
+moe_topk_kernel(const float* __restrict__ logits, int ld, int T, int E, int top, int mode, const float* __restrict__ choice_bias,
+                int* __restrict__ ids, float* __restrict__ wts, float sum_to) {
+  tlc_pdl(logits, ids, wts);
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (t < T) moe_topk(logits, ld, t, E, top, mode, choice_bias, ids, wts, sum_to);
+}
+
 // A block sorts the pairs by expert: counts, offsets (and every expert's first tile of `tm` sorted rows), then the list order
 // [n_pairs]: pair index (t * top + k) of every sorted position.  shi: 2 * E ints.  ids[i] is read by the thread that owns i
 // (i modulo the block) only.
@@ -100,7 +106,14 @@ __device__ __forceinline__ void moe_sort_pairs(const int* ids, int n_pairs, int 
   int* cursor = shi + E;       // [E]
   for (int e = threadIdx.x; e < E; e += blockDim.x) count[e] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n_pairs; i += blockDim.x) atomicAdd(&count[ids[i]], 1);
+  // (a thread's experts are fetched 8 at a time, all on their way before the first is counted)
+  for (int i0 = threadIdx.x; i0 < n_pairs; i0 += 8 * blockDim.x) {
+    int e[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) e[j] = i0 + j * blockDim.x < n_pairs ? ids[i0 + j * blockDim.x] : -1;
+#pragma unroll
+    for (int j = 0; j < 8; j++) if (e[j] >= 0) atomicAdd(&count[e[j]], 1);
+  }
   __syncthreads();
   if (threadIdx.x < 32) {      // running sums of pairs and tiles, 32 experts at a time
     const int lane = threadIdx.x;
@@ -127,7 +140,15 @@ __device__ __forceinline__ void moe_sort_pairs(const int* ids, int n_pairs, int 
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n_pairs; i += blockDim.x) order[atomicAdd(&cursor[ids[i]], 1)] = i;
+  for (int i0 = threadIdx.x; i0 < n_pairs; i0 += 8 * blockDim.x) {
+    int e[8], at[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) e[j] = i0 + j * blockDim.x < n_pairs ? ids[i0 + j * blockDim.x] : -1;
+#pragma unroll
+    for (int j = 0; j < 8; j++) at[j] = e[j] >= 0 ? atomicAdd(&cursor[e[j]], 1) : 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) if (e[j] >= 0) order[at[j]] = i0 + j * blockDim.x;
+  }
 }
 
 __global__ void __launch_bounds__(1024)
@@ -136,6 +157,19 @@ moe_sort_kernel(const int* __restrict__ ids, int n_pairs, int E, int E_tiled, in
   tlc_pdl(ids, order, offsets, tile_off);
   extern __shared__ int shi[];
   moe_sort_pairs(ids, n_pairs, E, E_tiled, tm, order, offsets, tile_off, shi);
+}
+
+// Both for the few rows of a decode step, a row a warp: one launch.
+__global__ void __launch_bounds__(1024)
+moe_topk_sort_kernel(const float* __restrict__ logits, int ld, int T, int E, int top, int mode, const float* __restrict__ choice_bias, int* ids,
+                     float* __restrict__ wts, float sum_to, int E_tiled, int tm, int* __restrict__ order, int* __restrict__ offsets,
+                     int* __restrict__ tile_off) {
+  tlc_pdl(logits, ids, wts, order, offsets, tile_off);
+  extern __shared__ int shi[];
+  const int t = threadIdx.x >> 5;
+  if (t < T) moe_topk(logits, ld, t, E, top, mode, choice_bias, ids, wts, sum_to);
+  __syncthreads();
+  moe_sort_pairs(ids, T * top, E, E_tiled, tm, order, offsets, tile_off, shi);
 }
 
 // Routing without a router, for all layers of a model that route this way: block p takes table p.  desc [n, 4] (64-bit): the
@@ -175,6 +209,12 @@ extern "C" int tlc_moe_route(const float* logits, int ld, int T, int E, int top,
   TLC_REQUIRE(E >= 1 && top >= 1 && top <= E && E <= 4096, "moe_route: %d experts, %d chosen", E, top);
   TLC_REQUIRE(mode == TLC_ROUTE_SIGMOID || mode == TLC_ROUTE_SOFTMAX || mode == TLC_ROUTE_SOFTMAX_ALL, "moe_route: unknown weighting %d", mode);
   TLC_REQUIRE(n_identity >= 0 && n_identity < E, "moe_route: %d of %d router outputs without an expert's weights", n_identity, E);
+  if (T <= 8) {             // (1 row 5.2 us as two launches, 4.9 as one; 8 rows 5.4; 32 rows 5.6 and, the block being larger, 10.5)
+    tlc_launch(moe_topk_sort_kernel, dim3(1), dim3(32 * std::max(T, 4)), (size_t)2 * E * sizeof(int), stream, logits, ld, T, E, top, mode, choice_bias,
+               ids, wts, sum_to, E - n_identity, tile_rows, order, offsets, tile_off);
+    TLC_CHECK_LAUNCH("moe_route");
+    return 0;
+  }
   tlc_launch(moe_topk_kernel, dim3((T + 3) / 4), dim3(128), 0, stream, logits, ld, T, E, top, mode, choice_bias, ids, wts, sum_to);
   TLC_CHECK_LAUNCH("moe_topk");
   tlc_launch(moe_sort_kernel, dim3(1), dim3(1024), (size_t)2 * E * sizeof(int), stream, (const int*)ids, T * top, E, E - n_identity, tile_rows,

@@ -1748,10 +1748,14 @@ def moe_experts_int8(x: torch.Tensor, w_gate_up: torch.Tensor, gate_up_scale: to
         raise KernelError(f"moe_experts_int8: a routing of {ids.numel()} pairs does not belong to {T} rows with {top} experts each of {E}")
     if not (x.is_cuda and w_gate_up.is_cuda and w_down.is_cuda and y.is_cuda and gate_up_scale.is_cuda and down_scale.is_cuda and ids.is_cuda):
         _gpu(x, w_gate_up, w_down, y, gate_up_scale, down_scale, ids)
-    _f32vec(gate_up_scale, E * N, "moe_experts_int8 gate and up scale")
-    _f32vec(down_scale, E * D, "moe_experts_int8 down scale")
+    for scale, n in ((gate_up_scale, E * N), (down_scale, E * D)):
+        if scale.dtype != torch.float32 or scale.numel() != n or not scale.is_contiguous():
+            _f32vec(scale, n, "moe_experts_int8 weight scale")
     if not y.is_contiguous() or y.numel() != pairs * D:
         raise KernelError("moe_experts_int8: y must be contiguous [T, top, D]")
+    ldx, dense = x.stride()
+    if T < 2 or dense != 1:
+        ldx = _rows(x, "moe_experts_int8 input")
     # the rows' integers (the activation's after them in the same place), the activation, the rows' scales
     ldq = (max(D, F) + 15) // 16 * 16
     room = torch.empty(pairs * (ldq + 4 * F + 4), dtype=torch.int8, device=x.device)
@@ -1759,7 +1763,7 @@ def moe_experts_int8(x: torch.Tensor, w_gate_up: torch.Tensor, gate_up_scale: to
         _note_owned(room)
     q = room.data_ptr()
     act = q + pairs * ldq
-    _call("tlc_moe_experts_int8", x.data_ptr(), dtype_code(x.dtype), _rows(x, "moe_experts_int8 input"), w_gate_up.data_ptr(), ld_gu,
+    _call("tlc_moe_experts_int8", x.data_ptr(), dtype_code(x.dtype), ldx, w_gate_up.data_ptr(), ld_gu,
           gate_up_scale.data_ptr(), w_down.data_ptr(), ld_d, down_scale.data_ptr(), ids.data_ptr(), order.data_ptr(), offsets.data_ptr(),
           wts.data_ptr(), T, E, top, F, D, q, ldq, act + 4 * pairs * F, act, y.data_ptr(), dtype_code(y.dtype), MOE_ACTS[act_fn],
           1 if weight_on == "output" else 0, float(limit), float(alpha), _stream())
