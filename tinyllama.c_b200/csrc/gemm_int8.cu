@@ -8,6 +8,8 @@
 #include <algorithm>
 #include <atomic>
 
+int tlc_rows_int8_pairs(const void* x, int x_dtype, int ldx, int T, int K, void* q, int ldq, float* scale, const int* order, int top, int* place,
+                        cudaStream_t stream);       // int8_rows.cu
 int tlc_int8_few(const Int8Args& p, int out_dtype, int nb, int sms, cudaStream_t stream);      // gemm_int8_few.cu
 int tlc_int8_few_split(long long tiles, int num_k, int sms);
 int tlc_int8_skinny(const void* x, int x_dtype, const Int8Args& p, int out_dtype, int sms, cudaStream_t stream);   // gemm_int8_skinny.cu
@@ -250,7 +252,8 @@ extern "C" int tlc_moe_experts_int8(const void* x, int x_dtype, int ldx, const v
     return tlc_int8_skinny_pairs(act, TLC_F32, d, ids, 1, y_dtype, sm_count(), stream);
   }
   // the chosen rows, sorted by expert, rounded; both products read their rows from q
-  if (int rc = tlc_rows_int8(x, x_dtype, ldx, (int)pairs, D, nullptr, 0.f, q, ldq, scales, order, top, 0, stream)) return rc;
+  // (the activation's place has not been written yet and lends itself to the pairs' places)
+  if (int rc = tlc_rows_int8_pairs(x, x_dtype, ldx, T, D, q, ldq, scales, order, top, (int*)act, stream)) return rc;
   if (int rc = run(p, TLC_F32, stream)) return rc;
   // the activation in 32 bits -> rounded row by row; a weight on the result only multiplies the row's scale
   if (int rc = tlc_rows_int8(act, TLC_F32, F, (int)pairs, F, nullptr, 0.f, q, ldq, scales, nullptr, 1, 0, stream)) return rc;
