@@ -166,3 +166,22 @@ def test_a_bound_model_and_what_it_holds(folders):
     before = [p.weight for p in (block.fused_in, block.ffn.gate_up)]
     llm.model.to_int8()                                   # a second time changes nothing
     assert all(a is b for a, b in zip(before, (block.fused_in.weight, block.ffn.gate_up.weight)))
+
+
+@pytest.mark.parametrize("name", ["linear_int8", "linear_swiglu_int8", "rmsnorm_int8", "_call_packed"])
+def test_a_function_around_a_product_is_called_for_every_layer(folders, name, monkeypatch):
+    llm = tlc.LLM(folders["D"], max_tokens=1024, max_seqs=4, weights="int8")
+    tokens = random_tokens(llm.model.vocab, 60, 1)
+    layers = len(llm.model.layers)
+
+    def step():
+        slot = llm.cache.acquire()
+        out = llm.step([StepEntry(slot, tokens, [59])])
+        llm.cache.release(slot)
+        return out
+
+    want = step()
+    real, calls = getattr(ops, name), []
+    monkeypatch.setattr(ops, name, lambda *a, **k: (calls.append(name), real(*a, **k))[1])
+    assert torch.equal(step(), want)
+    assert len(calls) % layers == 0 and len(calls) >= layers

@@ -43,7 +43,7 @@ const Entry kEntries[] = {
     TLC_ENTRY(tlc_rope_kv_store), TLC_ENTRY(tlc_attention), TLC_ENTRY(tlc_attention_decode), TLC_ENTRY(tlc_attention_decode_fused),
     TLC_ENTRY(tlc_attention_prefill), TLC_ENTRY(tlc_attention_prefill_tc),
     TLC_ENTRY(tlc_mamba_conv), TLC_ENTRY(tlc_mamba_step), TLC_ENTRY(tlc_ssm_scan), TLC_ENTRY(tlc_ssm_scan_one_row), TLC_ENTRY(tlc_ssm_scan_chunked), TLC_ENTRY(tlc_ssm_scan_ssd),
-    TLC_ENTRY(tlc_rows_int8), TLC_ENTRY(tlc_linear_int8),
+    TLC_ENTRY(tlc_rows_int8), TLC_ENTRY(tlc_linear_int8), TLC_ENTRY(tlc_moe_route), TLC_ENTRY(tlc_moe_experts_int8),
 };
 #undef TLC_ENTRY
 constexpr int kCount = (int)(sizeof(kEntries) / sizeof(kEntries[0]));
@@ -64,6 +64,11 @@ extern "C" int tlc_replay_index(const char* name) {
   for (int i = 0; name && i < kCount; i++)
     if (strcmp(kEntries[i].name, name) == 0) return i;
   return -1;
+}
+
+extern "C" int tlc_call(int function, const char* words) {
+  TLC_REQUIRE(function >= 0 && function < kCount, "call: there is no function %d", function);
+  return kEntries[function].run(reinterpret_cast<const unsigned long long*>(words));
 }
 
 extern "C" int tlc_replay(const int* functions, const unsigned long long* words, long long n_words, int n_calls, int times) {

@@ -53,6 +53,8 @@ void tlc_set_pdl(int on);
  * as 64-bit words (pointers and integers by value, floats by their bits; n_words in all; both arrays host).  Stops at the
  * first call that fails and returns its code. */
 int tlc_replay_index(const char* name);
+/* One such call, its arguments as words (8-byte aligned). */
+int tlc_call(int function, const char* words);
 int tlc_replay(const int* functions, const unsigned long long* words, long long n_words, int n_calls, int times);
 /* An event (cudaEvent_t) recorded on a stream; a stream that waits for one. */
 int tlc_event_record(void* event, cudaStream_t stream);

@@ -34,9 +34,11 @@ _ptr, _size, _stride, _dtype = torch.Tensor.data_ptr, torch.Tensor.size, torch.T
 _dense = torch.Tensor.is_contiguous
 
 
-# The wrappers of the kernel library as they are defined: the functions that name one of its calls, and those that they go through.
+# The wrappers of the kernel library as they are defined: the functions that name one of its calls, those that they go through, and
+# those that come to it by way of another.
+_BY_WAY = ("_call", "_call_packed", "record_event", "wait_event", "linear_int8", "linear_swiglu_int8", "rows_int8", "rmsnorm_int8")
 _OPS = {k: f for k, f in vars(ops).items() if isinstance(f, FunctionType) and
-        (k in ("_call", "record_event", "wait_event") or any(isinstance(c, str) and c in ops.REPEATABLE for c in f.__code__.co_consts))}
+        (k in _BY_WAY or any(isinstance(c, str) and c in ops.REPEATABLE for c in f.__code__.co_consts))}
 # methods that a step has no use for
 _NOT_IN_A_STEP = {"__init__", "bind", "weight_specs", "cache_requests", "step_requests", "shapes_from", "parts", "repeats", "add", "fuse_bound",
                   "fuse_bound_inputs", "out_features", "__setattr__", "__delattr__", "__init_subclass__"}

@@ -36,6 +36,7 @@ _SIGNATURES = {
     "tlc_last_error": (ctypes.c_char_p, []),
     "tlc_set_pdl": (None, [_i]),
     "tlc_replay_index": (_i, [ctypes.c_char_p]),
+    "tlc_call": (_i, [_i, ctypes.c_char_p]),
     "tlc_replay": (_i, [_vp, _vp, _ll, _i, _i]),
     "tlc_event_record": (_i, [_vp, _vp]),
     "tlc_event_wait": (_i, [_vp, _vp]),
@@ -212,21 +213,16 @@ def count_launches(n: int) -> None:
     _launches += int(n)
 
 
-def _call(name: str, *args, ok: int = 0) -> bool:
-    """Makes a call of the library.  ok > 0: the code by which the library may say that it did nothing; returns whether it did."""
+def _call(name: str, *args) -> None:
     global _launches
     lib = library()
     _launches += 1
     rc = getattr(lib, name)(*args)
     if rc != 0:
-        if ok and rc == ok:
-            _launches -= 1
-            return False
         raise KernelError(f"{name}: {lib.tlc_last_error().decode()}")
     notes = _notes.calls
     if notes is not None:
         notes.add(name, args)
-    return True
 
 
 # ---- calls made again --------------------------------------------------------------------
@@ -238,7 +234,32 @@ def _call(name: str, *args, ok: int = 0) -> bool:
 REPEATABLE = frozenset(("tlc_event_record", "tlc_event_wait", "tlc_rmsnorm", "tlc_gated_rmsnorm", "tlc_gated_rmsnorm_step", "tlc_linear",
                         "tlc_linear_swiglu", "tlc_glu", "tlc_rope_kv_store", "tlc_attention", "tlc_attention_decode",
                         "tlc_attention_decode_fused", "tlc_attention_prefill", "tlc_attention_prefill_tc", "tlc_mamba_conv", "tlc_mamba_step",
-                        "tlc_ssm_scan", "tlc_ssm_scan_one_row", "tlc_ssm_scan_chunked", "tlc_ssm_scan_ssd", "tlc_rows_int8", "tlc_linear_int8"))
+                        "tlc_ssm_scan", "tlc_ssm_scan_one_row", "tlc_ssm_scan_chunked", "tlc_ssm_scan_ssd", "tlc_rows_int8", "tlc_linear_int8", "tlc_moe_route", "tlc_moe_experts_int8"))
+
+
+# ctypes converts an argument at a time, 2.5 us for a call of 21; packed by one struct they take 0.5.
+_packs: dict = {}
+
+
+def _call_packed(name: str, *args, ok: int = 0) -> bool:
+    """_call() for a function of the library's table, its arguments plain numbers (0 for no pointer)."""
+    global _launches
+    hit = _packs.get(name)
+    if hit is None:
+        lib = library()
+        pack = struct.Struct("=" + "".join("f4x" if t is _f else "q" for t in _SIGNATURES[name][1])).pack
+        hit = _packs[name] = (lib, lib.tlc_call, lib.tlc_replay_index(name.encode()), pack)
+    lib, call, index, pack = hit
+    rc = call(index, pack(*args))
+    if rc != 0:
+        if ok and rc == ok:
+            return False
+        raise KernelError(f"{name}: {lib.tlc_last_error().decode()}")
+    _launches += 1
+    notes = _notes.calls
+    if notes is not None:
+        notes.add(name, args)
+    return True
 
 
 class NotedCalls:
@@ -1470,8 +1491,8 @@ def moe_route(logits: torch.Tensor, n_experts: int, top: int, tile_rows: int = 3
     _launches += 1                      # (two kernels)
     _f32vec(choice_bias, n_experts, "moe_route choice bias")
     _gpu(choice_bias)
-    _call("tlc_moe_route", logits.data_ptr(), _rows(logits, "router logits"), T, int(n_experts), int(top), ROUTE_WEIGHTS[weights],
-          _p(choice_bias), int(n_identity), ids.data_ptr(),
+    _call_packed("tlc_moe_route", logits.data_ptr(), _rows(logits, "router logits"), T, int(n_experts), int(top), ROUTE_WEIGHTS[weights],
+          _p(choice_bias) or 0, int(n_identity), ids.data_ptr(),
           wts.data_ptr(), order.data_ptr(), offsets.data_ptr(), tile_off.data_ptr(), int(tile_rows), float(sum_to), _stream())
     return ids, wts, order, offsets, tile_off, int(tile_rows)
 
@@ -1591,7 +1612,7 @@ def _rows_int8(x, what, out=None, norm_weight=None, eps=0.0, boundary=0):
     if x.dim() != 2 or x.shape[1] < 1:
         raise KernelError(f"{what}: rows [T, K] with K >= 1, got {tuple(x.shape)}")
     T, K = x.shape
-    weight = None
+    weight = 0
     if norm_weight is not None:
         _gpu(norm_weight)
         _f32vec(norm_weight, K, what + " weight")
@@ -1613,7 +1634,7 @@ def _rows_int8(x, what, out=None, norm_weight=None, eps=0.0, boundary=0):
             raise KernelError(f"{what}: integers go to an int8 tensor, got {q.dtype}")
         ldq = _out_rows(q, T, K, what)
         _f32vec(scale, T, what + " scale")
-    _call("tlc_rows_int8", x.data_ptr(), code, ldx, T, K, weight, eps, q.data_ptr(), ldq, scale.data_ptr(), None, 1, boundary, _stream())
+    _call_packed("tlc_rows_int8", x.data_ptr(), code, ldx, T, K, weight, eps, q.data_ptr(), ldq, scale.data_ptr(), 0, 1, boundary, _stream())
     return q, scale
 
 
@@ -1656,7 +1677,7 @@ def _linear_int8(what, a, a_scale, w, w_scale, colbias, out, N, accumulate, act,
         _gpu(a, w, out, w_scale)
     if w_scale.dtype != torch.float32 or w_scale.numel() != rows or not w_scale.is_contiguous():
         _f32vec(w_scale, rows, what + " weight scale")
-    bias = None
+    bias = 0
     if colbias is not None:
         _gpu(colbias)
         _f32vec(colbias, rows, what + " colbias")
@@ -1670,18 +1691,18 @@ def _linear_int8(what, a, a_scale, w, w_scale, colbias, out, N, accumulate, act,
             raise KernelError(f"{what}: integer rows come with their scales (a_scale)")
         _gpu(a_scale)
         _f32vec(a_scale, M, what + " a_scale")
-        code, scale, q, ldq = I8, a_scale.data_ptr(), None, 0
+        code, scale, q, ldq = I8, a_scale.data_ptr(), 0, 0
     else:
         if a_scale is not None:
             raise KernelError(f"{what}: a_scale belongs to integer rows; a is {a.dtype}")
         code, ldq = dtype_code(a.dtype), (K + 15) // 16 * 16
-        scale = q = None
+        scale = q = 0
         if M > 2:                                        # (one or two rows mostly go without; the library says so where not)
             scale, q = _int8_room(M, ldq, a.device)
     args = (w.data_ptr(), ldw, w_scale.data_ptr(), out.data_ptr(), dtype_code(out.dtype), ldo, bias, accumulate, M, N, K, act, limit, alpha, _stream())
-    if not _call("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, *args, ok=1):
+    if not _call_packed("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, *args, ok=1):
         scale, q = _int8_room(M, ldq, a.device)
-        _call("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, *args)
+        _call_packed("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, *args)
 
 
 def _int8_room(M: int, ld: int, device):
@@ -1763,7 +1784,7 @@ def moe_experts_int8(x: torch.Tensor, w_gate_up: torch.Tensor, gate_up_scale: to
         _note_owned(room)
     q = room.data_ptr()
     act = q + pairs * ldq
-    _call("tlc_moe_experts_int8", x.data_ptr(), dtype_code(x.dtype), ldx, w_gate_up.data_ptr(), ld_gu,
+    _call_packed("tlc_moe_experts_int8", x.data_ptr(), dtype_code(x.dtype), ldx, w_gate_up.data_ptr(), ld_gu,
           gate_up_scale.data_ptr(), w_down.data_ptr(), ld_d, down_scale.data_ptr(), ids.data_ptr(), order.data_ptr(), offsets.data_ptr(),
           wts.data_ptr(), T, E, top, F, D, q, ldq, act + 4 * pairs * F, act, y.data_ptr(), dtype_code(y.dtype), MOE_ACTS[act_fn],
           1 if weight_on == "output" else 0, float(limit), float(alpha), _stream())
