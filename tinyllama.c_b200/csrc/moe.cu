@@ -27,7 +27,8 @@ __device__ __forceinline__ void moe_topk(const float* __restrict__ logits, int l
   const int lane = threadIdx.x & 31;
   const float* lr = logits + (size_t)t * ld;
   float last = INFINITY, first = 0.f, sum = 0.f;
-  int last_e = -1;
+  int last_e = -1, my_id = 0;
+  float my_w = 0.f;
   // TLC_ROUTE_SOFTMAX_ALL: scores are the softmax over all E outputs; an expert is chosen by score + choice_bias[e] and
   // weighted by the score alone
   float all_max = 0.f, all_inv = 1.0f;
@@ -60,33 +61,34 @@ __device__ __forceinline__ void moe_topk(const float* __restrict__ logits, int l
       if (take) { best = ov; be = oe; }
     }
     if (be == 0x7fffffff) be = 0;            // (NaN logits: no order; keep indices valid)
-    if (lane == 0) {
-      ids[t * top + k] = be;
-      if (mode == TLC_ROUTE_SOFTMAX) {       // the first choice has the largest logit: numerators exp(z_k - z_0)
-        if (k == 0) first = lr[be];
-        const float e = expf(lr[be] - first);
-        sum += e;
-        wts[t * top + k] = e;
-      } else if (mode == TLC_ROUTE_SOFTMAX_ALL) {
-        const float w = __fmul_rn(expf(lr[be] - all_max), all_inv);
-        sum += w;
-        wts[t * top + k] = w;
-      } else {
-        wts[t * top + k] = 1.0f / (1.0f + expf(-lr[be]));
-      }
+    float w;                                 // (the same in every lane; lane k keeps choice k)
+    if (mode == TLC_ROUTE_SOFTMAX) {         // the first choice has the largest logit: numerators exp(z_k - z_0)
+      if (k == 0) first = lr[be];
+      w = expf(lr[be] - first);
+      sum += w;
+    } else if (mode == TLC_ROUTE_SOFTMAX_ALL) {
+      w = __fmul_rn(expf(lr[be] - all_max), all_inv);
+      sum += w;
+    } else {
+      w = 1.0f / (1.0f + expf(-lr[be]));
+    }
+    if (lane == (k & 31)) {
+      if (k < 32) { my_id = be; my_w = w; }
+      else { ids[t * top + k] = be; wts[t * top + k] = w; }
     }
     last = best;                             // (the value the comparison saw, not one computed anew: the same bits)
     last_e = be;
   }
-  if (mode == TLC_ROUTE_SOFTMAX && lane == 0) {
-    const float inv = 1.0f / sum;
-    for (int k = 0; k < top; k++) wts[t * top + k] *= inv;
+  // softmax: the numerators divided by their sum; all scores: divided by the chosen ones' sum (+ 1e-20, which keeps a sum of zero
+  // finite) and multiplied by sum_to
+  const bool normed = mode == TLC_ROUTE_SOFTMAX_ALL && sum_to > 0.f;
+  const float inv = normed ? 1.0f / (sum + 1e-20f) : 1.0f / sum;
+  auto final_of = [&](float w) { return normed ? w * inv * sum_to : mode == TLC_ROUTE_SOFTMAX ? w * inv : w; };
+  if (lane < top) {
+    ids[t * top + lane] = my_id;
+    wts[t * top + lane] = final_of(my_w);
   }
-  // the chosen scores divided by their sum (+ 1e-20, which keeps a sum of zero finite) and multiplied by sum_to
-  if (mode == TLC_ROUTE_SOFTMAX_ALL && sum_to > 0.f && lane == 0) {
-    const float inv = 1.0f / (sum + 1e-20f);
-    for (int k = 0; k < top; k++) wts[t * top + k] = wts[t * top + k] * inv * sum_to;
-  }
+  for (int k = 32 + lane; k < top; k += 32) wts[t * top + k] = final_of(wts[t * top + k]);
 }
 
 __global__ void __launch_bounds__(128)
@@ -106,13 +108,17 @@ __device__ __forceinline__ void moe_sort_pairs(const int* ids, int n_pairs, int 
   int* cursor = shi + E;       // [E]
   for (int e = threadIdx.x; e < E; e += blockDim.x) count[e] = 0;
   __syncthreads();
-  // (a thread's experts are fetched 8 at a time, all on their way before the first is counted)
-  for (int i0 = threadIdx.x; i0 < n_pairs; i0 += 8 * blockDim.x) {
-    int e[8];
+  // Up to 16 pairs a thread are counted once: what the counter said is the pair's place among its expert's.  Fetched together.
+  constexpr int MINE = 16;
+  const bool once = n_pairs <= MINE * (int)blockDim.x;
+  int mine[MINE], rank[MINE];
+  if (once) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) e[j] = i0 + j * blockDim.x < n_pairs ? ids[i0 + j * blockDim.x] : -1;
+    for (int j = 0; j < MINE; j++) mine[j] = threadIdx.x + j * blockDim.x < n_pairs ? ids[threadIdx.x + j * blockDim.x] : -1;
 #pragma unroll
-    for (int j = 0; j < 8; j++) if (e[j] >= 0) atomicAdd(&count[e[j]], 1);
+    for (int j = 0; j < MINE; j++) rank[j] = mine[j] >= 0 ? atomicAdd(&count[mine[j]], 1) : 0;
+  } else {
+    for (int i = threadIdx.x; i < n_pairs; i += blockDim.x) atomicAdd(&count[ids[i]], 1);
   }
   __syncthreads();
   if (threadIdx.x < 32) {      // running sums of pairs and tiles, 32 experts at a time
@@ -140,14 +146,11 @@ __device__ __forceinline__ void moe_sort_pairs(const int* ids, int n_pairs, int 
     }
   }
   __syncthreads();
-  for (int i0 = threadIdx.x; i0 < n_pairs; i0 += 8 * blockDim.x) {
-    int e[8], at[8];
+  if (once) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) e[j] = i0 + j * blockDim.x < n_pairs ? ids[i0 + j * blockDim.x] : -1;
-#pragma unroll
-    for (int j = 0; j < 8; j++) at[j] = e[j] >= 0 ? atomicAdd(&cursor[e[j]], 1) : 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) if (e[j] >= 0) order[at[j]] = i0 + j * blockDim.x;
+    for (int j = 0; j < MINE; j++) if (mine[j] >= 0) order[cursor[mine[j]] + rank[j]] = threadIdx.x + j * blockDim.x;
+  } else {
+    for (int i = threadIdx.x; i < n_pairs; i += blockDim.x) order[atomicAdd(&cursor[ids[i]], 1)] = i;
   }
 }
 
