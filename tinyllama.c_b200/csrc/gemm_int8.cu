@@ -2,8 +2,14 @@
 // the like) and grouped by expert.  The sum of integers is exact in 32 bits while K <= 131,071 (128 * 128 * K < 2^31), so neither the
 // order of a sum nor how K is cut changes a result.
 //
-// Here: the product for operands in any layout, on the CUDA cores (dp4a: four products and their sum an instruction), tiles of 32 x
-// 64 results staged through shared memory 64 values of K at a time.
+// The kernels, chosen in run() and tlc_linear_int8() by sizes, types and alignment alone:
+//   gemm_int8_skinny.cu  up to 4 rows, and experts of up to 8 pairs: CUDA cores, the rows rounded in the same kernel
+//   gemm_int8_few.cu     up to 64 rows, more where tiles are few: tensor cores, K shared among the blocks of a cluster
+//   gemm_int8_wide.cu    many rows, groups of 25 and more: tensor cores, pairs of blocks, persistent
+//   here                 operands that the copy engine does not take (rows off 16-byte boundaries; gated outputs that are no multiple of
+//                        8): CUDA cores (dp4a: four products and their sum an instruction), tiles of 32 x 64 results staged
+//                        through shared memory 64 values of K at a time.  2,048 rows of 2,048 -> 8,240 956 us, 72 TOP/s, bound by
+//                        shared memory (three reads for eight dp4a); the tensor cores take 31.
 #include "gemm_int8_tc.cuh"
 #include <algorithm>
 #include <atomic>

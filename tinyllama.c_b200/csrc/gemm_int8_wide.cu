@@ -8,9 +8,18 @@
 // products of the next; blocks are persistent and pairs walk the tiles.
 //
 // A lane holds one weight row, so its scale and bias stay in a register and neighbouring lanes write neighbouring columns of a row of
-// the result; 16-bit results are exchanged between neighbours so that a lane writes two of them at once.  Gated products have the
-// gate and up rows of 8 features in neighbouring groups of 8 lanes (load_weights): of two activation rows the gate's lanes finish
-// one and the up projection's lanes the other.
+// the result.  Gated products have the gate and up rows of 8 features in neighbouring groups of 8 lanes (load_weights): of two
+// activation rows the gate's lanes finish one and the up projection's lanes the other.  Sixteen warps take the results out, sixteen
+// rows at a time, what they need beside the sums asked for a tile ahead.
+//
+// What bounds it: the way of the operands from the L2 into shared memory.  The products of a stage take 512 clocks (the unit's 4.5 POP/s),
+// 32 KB come in at some 47 bytes a clock and SM (11 TB/s over the GPU), so a stage takes 700; without copies the largest case would
+// take 172 us, without results 205, it takes 250 to 270.  Over many milliseconds the power limit holds the clock at 1.5 GHz
+// (2.4 POP/s; bfloat16 products 1.24 GHz, 1.34).  8,192 x 2,560 -> 16,384 260 us, 2.6 POP/s; 2,048 x 2,048 -> 8,240 31 us (four rounds of 74
+// pairs for 3.57); gated 1,031 x 2,560 -> 2 x 8,192 42 us, a fifth of it for the last seven rows.
+//
+// Tiles of 128 activation rows are for groups of up to 110: the weights come in once for a group either way, the rows' stages are
+// half as long and eight of them fit.
 //
 // Waits are bounded (codes 55-59); after one that ran out both blocks of a pair go to their common end.
 #include "gemm_int8_tc.cuh"
