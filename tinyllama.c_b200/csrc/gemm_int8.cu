@@ -212,8 +212,8 @@ extern "C" int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_sca
   TLC_REQUIRE(out_dtype == TLC_F32 || out_dtype == TLC_BF16, "linear_int8: unknown output dtype %d", out_dtype);
   // Up to 4 rows of at most 8,192 values in all (2 where they are still to be rounded, which every block does), weights in 16-byte pieces
   // and up to 24 MB of them: the kernel that takes the rows as they are.  Microseconds there and on the tensor cores (rounding
-  // included): 1 x 2,048 -> 2,048 2.5, 4.5; 1 x 2,048 -> 8,240 5.2, 6.4; 1 x 8,192 -> 2,560 7.6, 7.6; 2 x 4,096 -> 2,048 5.1, 5.7;
-  // 2 x 8,192 -> 2,560 9.4, 7.6; 4 x 2,048 -> 8,240 7.5, 6.6 (integers given 5.6, 6.0); 1 x 2,560 -> 2 x 8,192 11.2, 10.1.
+  // included): 1 x 2,048 -> 2,048 2.1, 4.6; 1 x 2,048 -> 8,240 3.7, 6.2; 1 x 8,192 -> 2,560 7.4, 7.6; 2 x 4,096 -> 2,048 4.6, 5.7;
+  // 2 x 8,192 -> 2,560 9.4, 7.6; 4 x 2,048 -> 8,240 6.9, 6.5 (integers given 5.1, 5.9); 1 x 2,560 -> 2 x 8,192 11.3, 10.1.
   const bool takes = M <= 4 && (long long)(M == 3 ? 4 : M) * K <= TLC_INT8_SKINNY && ((uintptr_t)w | (uintptr_t)ldw) % 16 == 0;
   const bool skinny = M <= (a_dtype == TLC_I8 ? 4 : 2) && (long long)p.w_rows * K <= 24 << 20;
   if (takes && (g_kernel == 0 ? skinny : g_kernel == 4)) return tlc_int8_skinny(a, a_dtype, p, out_dtype, sm_count(), stream);
@@ -249,7 +249,7 @@ extern "C" int tlc_moe_experts_int8(const void* x, int x_dtype, int ldx, const v
   d.w = (const int8_t*)wd; d.w_scale = sd; d.out = y; d.ldw = ldd; d.ldo = D; d.N = D; d.K = F; d.w_rows = D;
   d.mode = I8_PLAIN; d.w_in = 0; d.w_out = w_out; d.scatter = 1;
   // A few pairs: each a product of one row, which the kernel rounds itself.  Microseconds there and in the four launches below (2,048 x
-  // 1,024, 32 experts): 4 pairs 11.6, 16.4; 8 pairs 17.1, 20.7; 12 pairs 23.4, 23.2
+  // 1,024, 32 experts): 4 pairs 11.8, 16.2; 8 pairs 17.2, 19.2; 12 pairs 23.1, 23.0
   if ((g_kernel == 0 || g_kernel == 4) && pairs <= 8 && D <= TLC_INT8_SKINNY && F <= TLC_INT8_SKINNY &&
       ((uintptr_t)wgu | (uintptr_t)wd | (uintptr_t)ldgu | (uintptr_t)ldd) % 16 == 0) {
     p.lda = ldx;

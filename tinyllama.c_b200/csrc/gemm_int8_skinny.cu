@@ -1,21 +1,22 @@
 // Products in 8-bit integers of up to 4 rows on the CUDA cores, rows rounded in the same kernel.
 //
-// The weights are streamed once, a warp two rows of them at a time (a feature's gate and up row, or neighbours), a lane 16 bytes of
-// every 512, four such pieces of both rows on their way together; dp4a multiplies them with the activation rows, which every block
-// keeps as integers in shared memory, and a warp reduction adds the lanes' sums, exactly.  Rows given in 16 or 32 bits are rounded by
-// every block for itself (they are small and come from the L2): a decode step's product is one launch, without tensor maps and without
-// room for the integers.  The first pieces of the weights are asked for before the wait on the kernel before.
+// The weights are streamed once, a lane 16 bytes of every 512 of a weight row; dp4a multiplies them with the activation rows, which every
+// block keeps as integers in shared memory, and a warp reduction adds the lanes' sums, exactly.  Rows given in 16 or 32 bits are rounded
+// by every block for itself (they are small and come from the L2): a decode step's product is one launch, without tensor maps and without
+// room for the integers.  The first pieces of the weights are asked for before the wait on the kernel before; where one item a warp
+// covers the matrix that is all of them, the scales and biases too, so that after the wait no load from HBM is left.
 //
-// What bounds it: for small matrices the way from launch to last store (1 x 2,048 -> 2,048 2.5 us, of which the 4 MB are 0.65; the
-// tensor cores' kernel and the one that rounds for it 4.5), then the weights' stream (8,240 x 2,048 5.2 us, 17 MB at 3.3 TB/s; there
-// 6.4).  From about 24 MB on the tensor cores' ring keeps more on its way (gated 16,384 x 2,560: 11.2 us here, 10.1 there).
+// What bounds it: for small matrices the way from launch to last store (1 x 2,048 -> 2,048 2.1 us, of which the 4 MB are 0.65; the
+// tensor cores' kernel and the one that rounds for it 4.6), then the weights' stream (8,240 x 2,048 3.7 us, 17 MB at 4.6 TB/s, integers
+// given 3.2; there 6.2 and 5.8).  Items that come one after another in a warp cost a wait each (two rows at a time, four or five items
+// a warp: 5.2 us there); from about 24 MB on the tensor cores' ring keeps more on its way (gated 16,384 x 2,560: 11.3 us here, 10.1).
 #include "gemm_int8.cuh"
 #include "int8_round.cuh"
 #include <algorithm>
 
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32, AHEAD = 4;      // pieces of 512 bytes of a weight row on their way together
+constexpr int THREADS = 256, WARPS = THREADS / 32;
 
 // 16 values from k on, zeros past K.
 __device__ __forceinline__ int4 sixteen(const int8_t* p, int k, int K) {
@@ -93,33 +94,20 @@ __device__ __forceinline__ void stage(const T* x, int ldx, const float*, int M, 
   __syncthreads();
 }
 
-// MR: rows the kernel is built for (M of them are there).  GROUPED (MR = 1): blocks of blockIdx.y take the pair of that number, row
+// MR: activation rows the kernel is built for (M of them are there); R: weight rows that a warp takes at a time, an item (gated: R / 2
+// features, their gate rows and then their up rows); A: pieces of 512 bytes of every one of them that are on their way together; ONCE:
+// a warp has one item at most and A pieces are its rows.  GROUPED (MR = 1): blocks of blockIdx.y take the pair of that number, row
 // pair / per_row of x times the weights of expert ids[pair].
-template <typename TX, typename TO, int MR, bool GLU, bool GROUPED>
+template <typename TX, typename TO, int MR, int R, int A, bool ONCE, bool GLU, bool GROUPED>
 __global__ void __launch_bounds__(THREADS, 2)
 int8_skinny_kernel(const TX* __restrict__ x, Int8Args p, const int* __restrict__ ids, int per_row) {
   asm volatile("griddepcontrol.launch_dependents;");
+  constexpr int C = GLU ? R / 2 : R;                      // columns of the result an item makes
   extern __shared__ __align__(16) int8_t skinny_rows[];
   __shared__ float scale[MR];
   __shared__ unsigned red[MR * WARPS];
-  const int lane = threadIdx.x & 31, ld = (p.K + 15) & ~15;
-  const int warps = gridDim.x * WARPS, items = GLU ? p.N : (p.N + 1) / 2;
-  const int8_t* rows[2];
-  auto rows_of = [&](int item) {                          // the two weight rows of an item (past the last: that one again)
-    const int n0 = GLU ? item : 2 * item, n1 = GLU ? p.N + item : min(2 * item + 1, p.N - 1);
-    rows[0] = p.w + (size_t)n0 * p.ldw;
-    rows[1] = p.w + (size_t)n1 * p.ldw;
-  };
-  int4 w[2][AHEAD];
-  auto fetch = [&](int k0) {
-#pragma unroll
-    for (int j = 0; j < AHEAD; j++)
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const int k = k0 + 512 * j + 16 * lane;
-        w[r][j] = k < p.K ? sixteen(rows[r], k, p.K) : make_int4(0, 0, 0, 0);
-      }
-  };
+  const int lane = threadIdx.x & 31, K = p.K, ld = (K + 15) & ~15;
+  const int warps = gridDim.x * WARPS, items = (p.N + C - 1) / C;
   // a warp's items: one from each block in turn, so that few items spread over all SMs
   int item = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
   const float* a_scale = p.a_scale;
@@ -136,74 +124,108 @@ int8_skinny_kernel(const TX* __restrict__ x, Int8Args p, const int* __restrict__
     out += (size_t)pair * p.ldo;
     share = wts[pair];
   }
+  int4 w[R][A];
+  auto fetch = [&](int item, int k0) {                    // (past the last column: that one again)
+#pragma unroll
+    for (int j = 0; j < A; j++)
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const int k = k0 + 512 * j + 16 * lane, n = min(C * item + (GLU ? r % C : r), p.N - 1) + (GLU && r >= C ? p.N : 0);
+        w[r][j] = k < K ? sixteen(p.w + (size_t)n * p.ldw, k, K) : make_int4(0, 0, 0, 0);
+      }
+  };
+  // lane m C + c finishes column c of row m; its scales and biases come with the weights
+  const int m_mine = lane / C, c_mine = lane % C;
+  float cs, cb, us, ub;
+  auto column = [&](int item) {
+    const int n = C * item + c_mine;
+    const bool in = n < p.N && m_mine < MR;
+    cs = in ? p.w_scale[n] : 0.f;
+    cb = in && p.colbias ? p.colbias[n] : 0.f;
+    us = GLU && in ? p.w_scale[p.N + n] : 0.f;
+    ub = GLU && in && p.colbias ? p.colbias[p.N + n] : 0.f;
+  };
   if (item < items) {
-    rows_of(item);
-    fetch(0);
+    fetch(item, 0);
+    column(item);
   }
   if (!GROUPED) tlc_wait(x, a_scale, out);
-  stage<MR>(x, p.lda, a_scale, GROUPED ? 1 : p.M, p.K, skinny_rows, ld, scale, red);
+  const int M = GROUPED ? 1 : p.M;
+  stage<MR>(x, p.lda, a_scale, M, K, skinny_rows, ld, scale, red);
   for (; item < items; item += warps) {
-    int acc[2][MR] = {};
-    for (int k0 = 0; k0 < p.K; k0 += 512 * AHEAD) {
-      int4 now[2][AHEAD];
+    const int n = C * item + c_mine, next = item + warps;
+    const bool writes = m_mine < M && n < p.N;
+    TO* o = out + (size_t)m_mine * p.ldo + n;
+    const float old = !GLU && p.mode == I8_ADD && writes ? to_f32(*o) : 0.f;
+    int acc[R][MR] = {};
+    auto multiply = [&](const int4 (&w)[R][A], int k0) {
 #pragma unroll
-      for (int j = 0; j < AHEAD; j++) { now[0][j] = w[0][j]; now[1][j] = w[1][j]; }
-      // the next pieces, of this item or the next one, under these pieces' products
-      const int next = item + warps;
-      if (k0 + 512 * AHEAD < p.K) fetch(k0 + 512 * AHEAD);
-      else if (next < items) {
-        rows_of(next);
-        fetch(0);
-      }
-#pragma unroll
-      for (int j = 0; j < AHEAD; j++) {
-        const int k = k0 + 512 * j + 16 * lane;
-        if (k0 + 512 * j >= p.K) break;
+      for (int j = 0; j < A; j++) {
+        if (k0 + 512 * j >= K) break;
+        const int k = min(k0 + 512 * j + 16 * lane, ld - 16);           // (where the row has ended, w is zeros)
 #pragma unroll
         for (int m = 0; m < MR; m++) {
-          const int4 a = k < ld ? *reinterpret_cast<const int4*>(skinny_rows + (size_t)m * ld + k) : make_int4(0, 0, 0, 0);
-          acc[0][m] = dot16(now[0][j], a, acc[0][m]);
-          acc[1][m] = dot16(now[1][j], a, acc[1][m]);
+          const int4 a = *reinterpret_cast<const int4*>(skinny_rows + (size_t)m * ld + k);
+#pragma unroll
+          for (int r = 0; r < R; r++) acc[r][m] = dot16(w[r][j], a, acc[r][m]);
         }
       }
+    };
+    if constexpr (ONCE) {
+      multiply(w, 0);
+    } else {
+      for (int k0 = 0; k0 < K; k0 += 512 * A) {
+        int4 now[R][A];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+          for (int j = 0; j < A; j++) now[r][j] = w[r][j];
+        // the next pieces, of this item or the next one, under these pieces' products
+        if (k0 + 512 * A < K) fetch(item, k0 + 512 * A);
+        else if (next < items) fetch(next, 0);
+        multiply(now, k0);
+      }
     }
-    // lane 2 m + r (gated: lane m) takes row m's result of weight row r
     int mine = 0, up = 0;
 #pragma unroll
     for (int m = 0; m < MR; m++)
 #pragma unroll
-      for (int r = 0; r < 2; r++) {
+      for (int r = 0; r < R; r++) {
         const int sum = __reduce_add_sync(0xffffffffu, acc[r][m]);
-        if (GLU) {
-          if (lane == m) { if (r == 0) mine = sum; else up = sum; }
-        } else if (lane == 2 * m + r) {
-          mine = sum;
-        }
+        if (lane == m * C + r % C) { if (GLU && r >= C) up = sum; else mine = sum; }
       }
-    const int m = GLU ? lane : lane >> 1, n = GLU ? item : 2 * item + (lane & 1);
-    if (m < (GROUPED ? 1 : p.M) && n < p.N) {
-      TO* o = out + (size_t)m * p.ldo + n;
-      const float rs = GROUPED && p.w_out ? scale[m] * share : scale[m], pw = GROUPED && p.w_in ? share : 1.0f;
-      float v = int8_value(mine, rs, p.w_scale[n], p.colbias ? p.colbias[n] : 0.f);
-      if (GLU) {
-        const float u = int8_value(up, rs, p.w_scale[p.N + n], p.colbias ? p.colbias[p.N + n] : 0.f);
-        v = int8_gated(p, GROUPED && p.w_in, pw, v, u);
-      } else if (p.mode == I8_ACT) {
-        v = int8_gated(p, GROUPED && p.w_in, pw, v, 0.f);
-      } else if (p.mode == I8_ADD) {
-        v += to_f32(*o);
-      }
+    if (writes) {
+      const float rs = GROUPED && p.w_out ? scale[m_mine] * share : scale[m_mine], pw = GROUPED && p.w_in ? share : 1.0f;
+      float v = int8_value(mine, rs, cs, cb);
+      if (GLU) v = int8_gated(p, GROUPED && p.w_in, pw, v, int8_value(up, rs, us, ub));
+      else if (p.mode == I8_ACT) v = int8_gated(p, GROUPED && p.w_in, pw, v, 0.f);
+      else if (p.mode == I8_ADD) v += old;
       *o = from_f32<TO>(v);
     }
+    if constexpr (ONCE) break;
+    if (next < items) column(next);
   }
 }
 
 template <typename TX, typename TO, int MR, bool GLU, bool GROUPED = false>
 int launch(const void* x, const Int8Args& p, const int* ids, int per_row, int sms, cudaStream_t stream) {
   const size_t smem = (size_t)MR * ((p.K + 15) & ~15);       // (TLC_INT8_SKINNY and the rows' ends at most)
-  const int items = GLU ? p.N : (p.N + 1) / 2, places = GROUPED ? std::max(1, 2 * sms / p.M) : 2 * sms;
-  tlc_launch(int8_skinny_kernel<TX, TO, MR, GLU, GROUPED>, dim3(std::min((items + WARPS - 1) / WARPS, places), GROUPED ? p.M : 1), dim3(THREADS), smem,
-             stream, (const TX*)x, p, ids, per_row);
+  const int places = GROUPED ? std::max(1, 2 * sms / p.M) : 2 * sms, rows = GLU ? 2 * p.N : p.N;
+  const long long warps = (long long)places * WARPS;
+#define TLC_SKINNY(R_, A_, ONCE_) \
+  tlc_launch(int8_skinny_kernel<TX, TO, MR, R_, A_, ONCE_, GLU, GROUPED>, dim3(std::min((rows + WARPS * R_ - 1) / (WARPS * R_), places), GROUPED ? p.M : 1), \
+             dim3(THREADS), smem, stream, (const TX*)x, p, ids, per_row)
+  // one item a warp, all of it on its way before the wait on the kernel before, where that takes no more than 16 pieces.  Microseconds so
+  // and two rows and four pieces at a time: 1 x 2,048 -> 8,240 3.7, 5.2; 2 x 2,048 -> 2 x 4,096 4.4, 6.0; 1 x 4,096 -> 2,048 3.0, 3.9.
+  // (2,048 -> 2,048 by the row, 3.0 for 2.1: half as many warps leave the next kernel room to fetch its weights meanwhile.)
+  bool done = false;
+  if constexpr (MR <= 2 && !GROUPED) {
+    if (p.K <= 2048 && rows > 2 * warps && rows <= 4 * warps) TLC_SKINNY(4, 4, true), done = true;
+    if constexpr (!GLU)
+      if (p.K > 2048 && p.K <= 4096 && rows <= warps) TLC_SKINNY(1, 8, true), done = true;
+  }
+  if (!done) TLC_SKINNY(2, 4, false);
+#undef TLC_SKINNY
   TLC_CHECK_LAUNCH("linear_int8 (up to 4 rows)");
   return 0;
 }
