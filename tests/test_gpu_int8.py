@@ -527,3 +527,55 @@ def test_every_kernel_gives_the_same_experts(kernel, T, E, top, F, D, act, weigh
                 ops.linear_int8_kernel()
         assert torch.equal(*got)
     ops.check_errors()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 200, 384), (3, 77, 2049), (8, 300, 4096), (8, 1000, 272), (6, 2050, 130), (7, 2048, 64), (2, 33, 3001), (4, 16, 4095),
+                                   (5, 9, 17), (8, 40, 4097)])
+def test_few_rows_give_the_same_bits(M, N, K):
+    """The kernel of up to 8 rows against the CUDA cores', at column counts and lengths that end inside a tile; rows of the activations on
+    16-byte boundaries and off them."""
+    g = gen(M * K)
+    a, sa, w, sw = integers(g, M, K), scales(g, M), integers(g, N, K), scales(g, N)
+    off = torch.empty(M, K + 37, dtype=torch.int8, device=DEV)[:, 3:3 + K]
+    off.copy_(a)
+    bias, w2, sw2 = normal(g, N), integers(g, 2 * 132, K), scales(g, 2 * 132) * 0.1
+    for dtype in (torch.float32, torch.bfloat16):
+        old = normal(g, M, N, dtype=dtype)
+        got = []
+        for k, rows in (((1, 0), a), ((5, 0), a), ((5, 0), off)):
+            ops.linear_int8_kernel(*k)
+            try:
+                outs = [torch.full((M, N), float("nan"), dtype=dtype, device=DEV), old.clone(), torch.full((M, 132), float("nan"), dtype=dtype, device=DEV)]
+                ops.linear_int8(rows, w, sw, outs[0], a_scale=sa, colbias=bias)
+                ops.linear_int8(rows, w, sw, outs[1], a_scale=sa, accumulate=True)
+                ops.linear_swiglu_int8(rows, w2, sw2, outs[2], a_scale=sa)
+                got.append(outs)
+            finally:
+                ops.linear_int8_kernel()
+        for other in got[1:]:
+            assert all(torch.equal(x, y) for x, y in zip(got[0], other))
+    ops.check_errors()
+
+
+@pytest.mark.parametrize("N,K", [(2048, 2048), (8240, 2048), (4738, 2041), (2368, 4096), (2369, 4096), (2048, 2064), (40, 8192), (9472, 2048), (9480, 100)])
+def test_one_row_rounded_within_gives_the_same_bits(N, K):
+    """One row in 16 or 32 bits, rounded where it is multiplied, at both sides of the rules that say how many weight rows a warp takes."""
+    g = gen(N + K)
+    w, sw, bias = integers(g, N, K), scales(g, N), normal(g, N)
+    for xt, dtype in ((torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)):
+        x = normal(g, 1, K, dtype=xt)
+        got = []
+        for k in ((1, 0), (4, 0)):
+            ops.linear_int8_kernel(*k)
+            try:
+                outs = [torch.full((1, N), float("nan"), dtype=dtype, device=DEV), torch.ones(1, N, dtype=dtype, device=DEV)]
+                ops.linear_int8(x, w, sw, outs[0], colbias=bias)
+                ops.linear_int8(x, w, sw, outs[1], accumulate=True)
+                if N % 2 == 0:
+                    outs.append(torch.full((1, N // 2), float("nan"), dtype=dtype, device=DEV))
+                    ops.linear_swiglu_int8(x, w, sw * 0.1, outs[2])
+                got.append(outs)
+            finally:
+                ops.linear_int8_kernel()
+        assert all(torch.equal(x, y) for x, y in zip(*got))
+    ops.check_errors()

@@ -3,7 +3,8 @@
 // order of a sum nor how K is cut changes a result.
 //
 // The kernels, chosen in run() and tlc_linear_int8() by sizes, types and alignment alone:
-//   gemm_int8_skinny.cu  up to 4 rows, and experts of up to 8 pairs: CUDA cores, the rows rounded in the same kernel
+//   gemm_int8_skinny.cu  one row, and experts of up to 8 pairs: CUDA cores, rows rounded in the same kernel
+//   gemm_int8_thin.cu    up to 8 rows of up to 4,096 values: mma.sync on weights that come from HBM into registers
 //   gemm_int8_few.cu     up to 64 rows, more where tiles are few: tensor cores, K shared among the blocks of a cluster
 //   gemm_int8_wide.cu    many rows, groups of 25 and more: tensor cores, pairs of blocks, persistent
 //   here                 operands that the copy engine does not take (rows off 16-byte boundaries; gated outputs that are no multiple of
@@ -20,6 +21,7 @@ int tlc_int8_few(const Int8Args& p, int out_dtype, int nb, int sms, cudaStream_t
 int tlc_int8_few_split(long long tiles, int num_k, int sms);
 int tlc_int8_skinny(const void* x, int x_dtype, const Int8Args& p, int out_dtype, int sms, cudaStream_t stream);   // gemm_int8_skinny.cu
 int tlc_int8_skinny_pairs(const void* x, int x_dtype, const Int8Args& p, const int* ids, int per_row, int out_dtype, int sms, cudaStream_t stream);
+int tlc_int8_thin(const Int8Args& p, int out_dtype, cudaStream_t stream);                        // gemm_int8_thin.cu
 int tlc_int8_wide(const Int8Args& p, int out_dtype, int nb, int pairs, cudaStream_t stream);   // gemm_int8_wide.cu
 
 namespace {
@@ -149,7 +151,13 @@ int g_kernel = 0, g_rows = 0;        // test hook: which kernel, on tiles of how
 
 int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
   const int sms = sm_count();
-  if (g_kernel != 1 && (out_dtype == TLC_F32 || out_dtype == TLC_BF16) && tensor_cores_take(p)) {
+  // Up to 8 rows: weights straight to the registers of mma.sync, for one wave of blocks before the wait.  Microseconds there and through shared
+  // memory, 8 rows: 2,048 -> 2,048 2.1, 3.6; 4,096 -> 2,048 2.5, 4.4; 2,048 -> 8,240 3.9, 6.0; 2,560 -> 2 x 8,192 9.2, 10.1; 2,048 ->
+  // 65,536 22.6, 26.1.  (12 rows in two eights 5.3 and 6.1 for 2,048 -> 8,240, but 38 and 27 for 65,536; 8,192 -> 2,560 by clusters of
+  // two blocks 7.6 and 6.8.)
+  if (!p.offsets && (g_kernel == 0 || g_kernel >= 4) && p.M <= 8 && p.K <= TLC_INT8_THIN && ((uintptr_t)p.w | (uintptr_t)p.ldw) % 16 == 0)
+    return tlc_int8_thin(p, out_dtype, stream);
+  if (g_kernel != 1 && tensor_cores_take(p)) {
     const int pairs = tlc_linear_pairs();
     if (g_kernel == 3 && pairs > 0) return tlc_int8_wide(p, out_dtype, g_rows, pairs, stream);
     if (g_kernel == 2) return tlc_int8_few(p, out_dtype, g_rows, sms, stream);
@@ -179,18 +187,17 @@ int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
     }
     return tlc_int8_few(p, out_dtype, by64 <= by128 ? 64 : 128, sms, stream);
   }
-  if (out_dtype == TLC_F32) return run_tiles<float>(p, stream);
-  if (out_dtype == TLC_BF16) return run_tiles<__nv_bfloat16>(p, stream);
-  return tlc_fail(-1, "linear_int8: unknown output dtype %d", out_dtype);
+  return out_dtype == TLC_F32 ? run_tiles<float>(p, stream) : run_tiles<__nv_bfloat16>(p, stream);
 }
 
 }  // namespace
 
 // Test hook: 0 = chosen by the sizes; 1 = the CUDA cores; 2 = tiles of 128 weight rows and 16, 32, 64 or 128 activation rows; 3 = pairs of
-// blocks on 256 weight rows and 128 or 256 activation rows; 4 = the kernel of up to 4 rows, wherever they take the operands.
+// blocks on 256 weight rows and 128 or 256 activation rows; 4 = the kernel of one row; 5 = the kernel of up to 8 rows, wherever
+// they take the operands.
 extern "C" int tlc_linear_int8_kernel(int kernel, int rows) {
   TLC_REQUIRE(kernel == 0 || kernel == 1 || (kernel == 2 && (rows == 16 || rows == 32 || rows == 64 || rows == 128)) ||
-              (kernel == 3 && (rows == 128 || rows == 256)) || kernel == 4, "linear_int8: there is no kernel %d with tiles of %d rows", kernel, rows);
+              (kernel == 3 && (rows == 128 || rows == 256)) || kernel == 4 || kernel == 5, "linear_int8: there is no kernel %d with tiles of %d rows", kernel, rows);
   g_kernel = kernel;
   g_rows = rows;
   return 0;
@@ -210,13 +217,13 @@ extern "C" int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_sca
   p.act = act; p.limit = limit; p.alpha = alpha;
   TLC_REQUIRE(a_dtype == TLC_I8 || a_dtype == TLC_F32 || a_dtype == TLC_BF16, "linear_int8: unknown type %d of the rows", a_dtype);
   TLC_REQUIRE(out_dtype == TLC_F32 || out_dtype == TLC_BF16, "linear_int8: unknown output dtype %d", out_dtype);
-  // Up to 4 rows of at most 8,192 values in all (2 where they are still to be rounded, which every block does), weights in 16-byte pieces
-  // and up to 24 MB of them: the kernel that takes the rows as they are.  Microseconds there and on the tensor cores (rounding
-  // included): 1 x 2,048 -> 2,048 2.1, 4.6; 1 x 2,048 -> 8,240 3.7, 6.2; 1 x 8,192 -> 2,560 7.4, 7.6; 2 x 4,096 -> 2,048 4.6, 5.7;
-  // 2 x 8,192 -> 2,560 9.4, 7.6; 4 x 2,048 -> 8,240 6.9, 6.5 (integers given 5.1, 5.9); 1 x 2,560 -> 2 x 8,192 11.3, 10.1.
-  const bool takes = M <= 4 && (long long)(M == 3 ? 4 : M) * K <= TLC_INT8_SKINNY && ((uintptr_t)w | (uintptr_t)ldw) % 16 == 0;
-  const bool skinny = M <= (a_dtype == TLC_I8 ? 4 : 2) && (long long)p.w_rows * K <= 24 << 20;
-  if (takes && (g_kernel == 0 ? skinny : g_kernel == 4)) return tlc_int8_skinny(a, a_dtype, p, out_dtype, sm_count(), stream);
+  // One row of at most 8,192 values, weights in 16-byte pieces and up to 24 MB of them: the kernel that takes the row as it is.
+  // Microseconds there and by gemm_int8_thin.cu (from K = 4,097 the tensor cores), a row to be rounded: 2,048 -> 2,048 2.1, 2.8; 2,048 ->
+  // 8,240 3.7, 4.5; 4,096 -> 2,048 3.0, 3.5; 2,048 -> 2 x 4,096 3.4, 4.6; 8,192 -> 2,560 7.4, 7.5; 2,560 -> 10,240 8.2, 6.8.  Integers
+  // behind the norm that makes them, both: 2,048 -> 8,240 4.5, 4.8; gated 4.5, 5.0.  (Two rows rounded in every block were 4.5 and 4.6 us
+  // for 2,048 -> 8,240 and 4,096 -> 2,048, rounded first 4.3 and 3.6.)
+  const bool takes = M == 1 && K <= TLC_INT8_SKINNY && ((uintptr_t)w | (uintptr_t)ldw) % 16 == 0;
+  if (takes && (g_kernel == 4 || (g_kernel == 0 && (long long)p.w_rows * K <= 24 << 20))) return tlc_int8_skinny(a, a_dtype, p, out_dtype, sm_count(), stream);
   if (a_dtype != TLC_I8) {
     if (!a_int8 || !a_scale) return 1;                     // (room is wanted)
     if (int rc = tlc_rows_int8(a, a_dtype, lda, M, K, nullptr, 0.f, a_int8, ld_int8, a_scale, nullptr, 1, 0, stream)) return rc;

@@ -19,9 +19,19 @@ struct Int8Args {
   int E;
   int scatter, w_out;                   // result rows go where order says, times the pair's weight
 };
-constexpr int TLC_INT8_SKINNY = 8192;     // values of activation rows in the kernel of up to 4 rows, at most
+constexpr int TLC_INT8_SKINNY = 8192;     // values of the row in the kernel of one row, at most
+constexpr int TLC_INT8_THIN = 4096;       // values of a row in the kernel of up to 8 rows, at most: 256 for each of 16 warps
 constexpr int TLC_INT8_GROUPS = 4096;     // at most (as a routing)
 enum { I8_PLAIN = 0, I8_ADD = 1, I8_ACT = 2, I8_GLU = 3 };
+
+// 16 values from k on, zeros past K; whole: on a 16-byte boundary.
+__device__ __forceinline__ int4 sixteen(const int8_t* p, int k, int K, bool whole) {
+  if (whole && k + 16 <= K) return __ldg(reinterpret_cast<const int4*>(p + k));
+  int v[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; i++) if (k + i < K) v[i >> 2] |= (int)(uint8_t)p[k + i] << (8 * (i & 3));
+  return make_int4(v[0], v[1], v[2], v[3]);
+}
 
 // One result from its integer sum.  Both scales in 32 bits, one after the other: their product alone may leave the range.  The
 // operations are spelled out, so that every kernel rounds alike and a result does not depend on which one made it.

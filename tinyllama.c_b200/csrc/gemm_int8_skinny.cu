@@ -1,15 +1,14 @@
-// Products in 8-bit integers of up to 4 rows on the CUDA cores, rows rounded in the same kernel.
+// Products in 8-bit integers of one row on the CUDA cores, a row in 16 or 32 bits rounded in the same kernel.
 //
-// The weights are streamed once, a lane 16 bytes of every 512 of a weight row; dp4a multiplies them with the activation rows, which every
-// block keeps as integers in shared memory, and a warp reduction adds the lanes' sums, exactly.  Rows given in 16 or 32 bits are rounded
-// by every block for itself (they are small and come from the L2): a decode step's product is one launch, without tensor maps and without
-// room for the integers.  The first pieces of the weights are asked for before the wait on the kernel before; where one item a warp
-// covers the matrix that is all of them, the scales and biases too, so that after the wait no load from HBM is left.
+// The weights are streamed once, a lane 16 bytes of every 512 of a weight row; dp4a multiplies them with the activation row, which every
+// block keeps as integers in shared memory, and a warp reduction adds the lanes' sums, exactly.  Every block rounds the row for itself (it
+// is small and comes from the L2): a decode step's product is one launch, without room for the integers.  The first pieces of the
+// weights are asked for before the wait on the kernel before; where one item a warp covers the matrix that is all of them, the scales
+// and biases too, so that after the wait no load from HBM is left.
 //
-// What bounds it: for small matrices the way from launch to last store (1 x 2,048 -> 2,048 2.1 us, of which the 4 MB are 0.65; the
-// tensor cores' kernel and the one that rounds for it 4.6), then the weights' stream (8,240 x 2,048 3.7 us, 17 MB at 4.6 TB/s, integers
-// given 3.2; there 6.2 and 5.8).  Items that come one after another in a warp cost a wait each (two rows at a time, four or five items
-// a warp: 5.2 us there); from about 24 MB on the tensor cores' ring keeps more on its way (gated 16,384 x 2,560: 11.3 us here, 10.1).
+// What bounds it: for small matrices the way from launch to last store (2,048 -> 2,048 2.1 us, of which the 4 MB are 0.65; rounded by
+// one kernel and multiplied by another 2.8), then the weights' stream (8,240 x 2,048 3.7 us, 17 MB at 4.6 TB/s; 4.5 so).  Items that come
+// one after another in a warp cost a wait each (two rows at a time, four or five items a warp: 5.2 us there).
 #include "gemm_int8.cuh"
 #include "int8_round.cuh"
 #include <algorithm>
@@ -18,39 +17,20 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 
-// 16 values from k on, zeros past K.
-__device__ __forceinline__ int4 sixteen(const int8_t* p, int k, int K) {
-  if (k + 16 <= K) return __ldg(reinterpret_cast<const int4*>(p + k));
-  int v[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 16; i++) if (k + i < K) v[i >> 2] |= (int)(uint8_t)p[k + i] << (8 * (i & 3));
-  return make_int4(v[0], v[1], v[2], v[3]);
-}
 __device__ __forceinline__ int dot16(int4 a, int4 b, int c) { return __dp4a(a.w, b.w, __dp4a(a.z, b.z, __dp4a(a.y, b.y, __dp4a(a.x, b.x, c)))); }
 
-// The block's copy of the activation rows: integers in xs [MR][ld], scales.
-template <int MR> __device__ __forceinline__ void stage(const int8_t* x, int ldx, const float* a_scale, int M, int K, int8_t* xs, int ld, float* scale, unsigned*) {
-  for (int i = threadIdx.x; i < MR * (ld / 16); i += THREADS) {
-    const int m = i / (ld / 16), k = 16 * (i - m * (ld / 16));
-    int4 v = make_int4(0, 0, 0, 0);
-    if (m < M && (((uintptr_t)x | (uintptr_t)ldx) & 15) == 0) v = sixteen(x + (size_t)m * ldx, k, K);
-    else if (m < M) {
-      int w[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 16; j++) if (k + j < K) w[j >> 2] |= (int)(uint8_t)x[(size_t)m * ldx + k + j] << (8 * (j & 3));
-      v = make_int4(w[0], w[1], w[2], w[3]);
-    }
-    *reinterpret_cast<int4*>(xs + (size_t)m * ld + k) = v;
-  }
-  if (threadIdx.x < MR) scale[threadIdx.x] = threadIdx.x < M ? a_scale[threadIdx.x] : 0.f;
+// The block's copy of the row: integers in xs [ld], zeros from K on; returns its scale.
+__device__ __forceinline__ float stage(const int8_t* x, const float* a_scale, int K, int8_t* xs, int ld, unsigned*) {
+  const float scale = *a_scale;
+  for (int k = 16 * threadIdx.x; k < ld; k += 16 * THREADS) *reinterpret_cast<int4*>(xs + k) = sixteen(x, k, K, (uintptr_t)x % 16 == 0);
   __syncthreads();
+  return scale;
 }
-template <int MR, typename T>
-__device__ __forceinline__ void stage(const T* x, int ldx, const float*, int M, int K, int8_t* xs, int ld, float* scale, unsigned* red) {
-  const bool whole = (uintptr_t)x % 16 == 0 && ((size_t)ldx * sizeof(T)) % 16 == 0;
-  const int pieces = ld / 8, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;      // (zeros from K to ld)
-  auto piece = [&](int m, int c, float (&v)[8]) {
-    const T* p = x + (size_t)m * ldx + 8 * c;
+template <typename T> __device__ __forceinline__ float stage(const T* x, const float*, int K, int8_t* xs, int ld, unsigned* red) {
+  const bool whole = (uintptr_t)x % 16 == 0;
+  const int pieces = ld / 8, lane = threadIdx.x & 31;
+  auto piece = [&](int c, float (&v)[8]) {
+    const T* p = x + 8 * c;
     if (whole && 8 * c + 8 <= K) {
       Piece<T> raw;
       raw.load(p);
@@ -60,57 +40,46 @@ __device__ __forceinline__ void stage(const T* x, int ldx, const float*, int M, 
       for (int i = 0; i < 8; i++) v[i] = 8 * c + i < K ? to_f32(p[i]) : 0.f;
     }
   };
-  // the largest magnitudes of all rows, one meeting of the block
+  float magnitude = 0.f;
+  for (int c = threadIdx.x; c < pieces; c += THREADS) {
+    float v[8];
+    piece(c, v);
 #pragma unroll
-  for (int m = 0; m < MR; m++) {
-    float magnitude = 0.f;
-    if (m < M)
-      for (int c = threadIdx.x; c < pieces; c += THREADS) {
-        float v[8];
-        piece(m, c, v);
-#pragma unroll
-        for (int i = 0; i < 8; i++) magnitude = larger(magnitude, v[i]);
-      }
-    const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(magnitude));
-    if (lane == 0) red[m * WARPS + warp] = most;
+    for (int i = 0; i < 8; i++) magnitude = larger(magnitude, v[i]);
   }
+  const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(magnitude));
+  if (lane == 0) red[threadIdx.x >> 5] = most;
   __syncthreads();
-#pragma unroll 1
-  for (int m = 0; m < MR; m++) {
-    bool some;
-    const unsigned largest = __reduce_max_sync(0xffffffffu, red[m * WARPS + (lane & (WARPS - 1))]);
-    const float s = int8_scale(largest, &some), inv = __frcp_rn(s);
-    if (threadIdx.x == 0) scale[m] = int8_told(largest, some, s);
-    for (int c = threadIdx.x; c < pieces; c += THREADS) {
-      uint2 n = make_uint2(0u, 0u);
-      if (some) {
-        float v[8];
-        piece(m, c, v);
-        n = eight_nearest(v, s, inv);
-      }
-      *reinterpret_cast<uint2*>(xs + (size_t)m * ld + 8 * c) = n;
+  bool some;
+  const unsigned largest = __reduce_max_sync(0xffffffffu, red[lane & (WARPS - 1)]);
+  const float s = int8_scale(largest, &some), inv = __frcp_rn(s);
+  for (int c = threadIdx.x; c < pieces; c += THREADS) {
+    uint2 n = make_uint2(0u, 0u);
+    if (some) {
+      float v[8];
+      piece(c, v);
+      n = eight_nearest(v, s, inv);
     }
+    *reinterpret_cast<uint2*>(xs + 8 * c) = n;
   }
   __syncthreads();
+  return int8_told(largest, some, s);
 }
 
-// MR: activation rows the kernel is built for (M of them are there); R: weight rows that a warp takes at a time, an item (gated: R / 2
-// features, their gate rows and then their up rows); A: pieces of 512 bytes of every one of them that are on their way together; ONCE:
-// a warp has one item at most and A pieces are its rows.  GROUPED (MR = 1): blocks of blockIdx.y take the pair of that number, row
-// pair / per_row of x times the weights of expert ids[pair].
-template <typename TX, typename TO, int MR, int R, int A, bool ONCE, bool GLU, bool GROUPED>
+// R: weight rows that a warp takes at a time, an item (gated: R / 2 features, their gate rows and then their up rows); A: pieces of 512
+// bytes of every one of them that are on their way together; ONCE: a warp has one item at most and A pieces are its rows.
+// GROUPED: blocks of blockIdx.y take the pair of that number, row pair / per_row of x times the weights of expert ids[pair].
+template <typename TX, typename TO, int R, int A, bool ONCE, bool GLU, bool GROUPED>
 __global__ void __launch_bounds__(THREADS, 2)
 int8_skinny_kernel(const TX* __restrict__ x, Int8Args p, const int* __restrict__ ids, int per_row) {
   asm volatile("griddepcontrol.launch_dependents;");
   constexpr int C = GLU ? R / 2 : R;                      // columns of the result an item makes
   extern __shared__ __align__(16) int8_t skinny_rows[];
-  __shared__ float scale[MR];
-  __shared__ unsigned red[MR * WARPS];
+  __shared__ unsigned red[WARPS];
   const int lane = threadIdx.x & 31, K = p.K, ld = (K + 15) & ~15;
   const int warps = gridDim.x * WARPS, items = (p.N + C - 1) / C;
   // a warp's items: one from each block in turn, so that few items spread over all SMs
   int item = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
-  const float* a_scale = p.a_scale;
   const float* wts = p.wts;
   TO* out = reinterpret_cast<TO*>(p.out);
   float share = 1.0f;
@@ -131,15 +100,14 @@ int8_skinny_kernel(const TX* __restrict__ x, Int8Args p, const int* __restrict__
 #pragma unroll
       for (int r = 0; r < R; r++) {
         const int k = k0 + 512 * j + 16 * lane, n = min(C * item + (GLU ? r % C : r), p.N - 1) + (GLU && r >= C ? p.N : 0);
-        w[r][j] = k < K ? sixteen(p.w + (size_t)n * p.ldw, k, K) : make_int4(0, 0, 0, 0);
+        w[r][j] = k < K ? sixteen(p.w + (size_t)n * p.ldw, k, K, true) : make_int4(0, 0, 0, 0);
       }
   };
-  // lane m C + c finishes column c of row m; its scales and biases come with the weights
-  const int m_mine = lane / C, c_mine = lane % C;
+  // lane c finishes column c of the item; its scales and biases come with the weights
   float cs, cb, us, ub;
   auto column = [&](int item) {
-    const int n = C * item + c_mine;
-    const bool in = n < p.N && m_mine < MR;
+    const int n = C * item + lane;
+    const bool in = n < p.N && lane < C;
     cs = in ? p.w_scale[n] : 0.f;
     cb = in && p.colbias ? p.colbias[n] : 0.f;
     us = GLU && in ? p.w_scale[p.N + n] : 0.f;
@@ -149,26 +117,22 @@ int8_skinny_kernel(const TX* __restrict__ x, Int8Args p, const int* __restrict__
     fetch(item, 0);
     column(item);
   }
+  const float* a_scale = p.a_scale;
   if (!GROUPED) tlc_wait(x, a_scale, out);
-  const int M = GROUPED ? 1 : p.M;
-  stage<MR>(x, p.lda, a_scale, M, K, skinny_rows, ld, scale, red);
+  const float scale = stage(x, a_scale, K, skinny_rows, ld, red);
   for (; item < items; item += warps) {
-    const int n = C * item + c_mine, next = item + warps;
-    const bool writes = m_mine < M && n < p.N;
-    TO* o = out + (size_t)m_mine * p.ldo + n;
-    const float old = !GLU && p.mode == I8_ADD && writes ? to_f32(*o) : 0.f;
-    int acc[R][MR] = {};
+    const int n = C * item + lane, next = item + warps;
+    const bool writes = lane < C && n < p.N;
+    const float old = !GLU && p.mode == I8_ADD && writes ? to_f32(out[n]) : 0.f;
+    int acc[R] = {};
     auto multiply = [&](const int4 (&w)[R][A], int k0) {
 #pragma unroll
       for (int j = 0; j < A; j++) {
         if (k0 + 512 * j >= K) break;
         const int k = min(k0 + 512 * j + 16 * lane, ld - 16);           // (where the row has ended, w is zeros)
+        const int4 a = *reinterpret_cast<const int4*>(skinny_rows + k);
 #pragma unroll
-        for (int m = 0; m < MR; m++) {
-          const int4 a = *reinterpret_cast<const int4*>(skinny_rows + (size_t)m * ld + k);
-#pragma unroll
-          for (int r = 0; r < R; r++) acc[r][m] = dot16(w[r][j], a, acc[r][m]);
-        }
+        for (int r = 0; r < R; r++) acc[r] = dot16(w[r][j], a, acc[r]);
       }
     };
     if constexpr (ONCE) {
@@ -188,74 +152,66 @@ int8_skinny_kernel(const TX* __restrict__ x, Int8Args p, const int* __restrict__
     }
     int mine = 0, up = 0;
 #pragma unroll
-    for (int m = 0; m < MR; m++)
-#pragma unroll
-      for (int r = 0; r < R; r++) {
-        const int sum = __reduce_add_sync(0xffffffffu, acc[r][m]);
-        if (lane == m * C + r % C) { if (GLU && r >= C) up = sum; else mine = sum; }
-      }
+    for (int r = 0; r < R; r++) {
+      const int sum = __reduce_add_sync(0xffffffffu, acc[r]);
+      if (lane == r % C) { if (GLU && r >= C) up = sum; else mine = sum; }
+    }
     if (writes) {
-      const float rs = GROUPED && p.w_out ? scale[m_mine] * share : scale[m_mine], pw = GROUPED && p.w_in ? share : 1.0f;
+      const float rs = GROUPED && p.w_out ? scale * share : scale, pw = GROUPED && p.w_in ? share : 1.0f;
       float v = int8_value(mine, rs, cs, cb);
       if (GLU) v = int8_gated(p, GROUPED && p.w_in, pw, v, int8_value(up, rs, us, ub));
       else if (p.mode == I8_ACT) v = int8_gated(p, GROUPED && p.w_in, pw, v, 0.f);
       else if (p.mode == I8_ADD) v += old;
-      *o = from_f32<TO>(v);
+      out[n] = from_f32<TO>(v);
     }
     if constexpr (ONCE) break;
     if (next < items) column(next);
   }
 }
 
-template <typename TX, typename TO, int MR, bool GLU, bool GROUPED = false>
+template <typename TX, typename TO, bool GLU, bool GROUPED>
 int launch(const void* x, const Int8Args& p, const int* ids, int per_row, int sms, cudaStream_t stream) {
-  const size_t smem = (size_t)MR * ((p.K + 15) & ~15);       // (TLC_INT8_SKINNY and the rows' ends at most)
+  const size_t smem = (p.K + 15) & ~15;                   // (TLC_INT8_SKINNY at most)
   const int places = GROUPED ? std::max(1, 2 * sms / p.M) : 2 * sms, rows = GLU ? 2 * p.N : p.N;
   const long long warps = (long long)places * WARPS;
 #define TLC_SKINNY(R_, A_, ONCE_) \
-  tlc_launch(int8_skinny_kernel<TX, TO, MR, R_, A_, ONCE_, GLU, GROUPED>, dim3(std::min((rows + WARPS * R_ - 1) / (WARPS * R_), places), GROUPED ? p.M : 1), \
+  tlc_launch(int8_skinny_kernel<TX, TO, R_, A_, ONCE_, GLU, GROUPED>, dim3(std::min((rows + WARPS * R_ - 1) / (WARPS * R_), places), GROUPED ? p.M : 1), \
              dim3(THREADS), smem, stream, (const TX*)x, p, ids, per_row)
   // one item a warp, all of it on its way before the wait on the kernel before, where that takes no more than 16 pieces.  Microseconds so
-  // and two rows and four pieces at a time: 1 x 2,048 -> 8,240 3.7, 5.2; 2 x 2,048 -> 2 x 4,096 4.4, 6.0; 1 x 4,096 -> 2,048 3.0, 3.9.
+  // and two rows and four pieces at a time: 2,048 -> 8,240 3.7, 5.2; 2,048 -> 2 x 4,096 3.4, 5.2; 4,096 -> 2,048 3.0, 3.9.
   // (2,048 -> 2,048 by the row, 3.0 for 2.1: half as many warps leave the next kernel room to fetch its weights meanwhile.)
   bool done = false;
-  if constexpr (MR <= 2 && !GROUPED) {
+  if constexpr (!GROUPED) {
     if (p.K <= 2048 && rows > 2 * warps && rows <= 4 * warps) TLC_SKINNY(4, 4, true), done = true;
     if constexpr (!GLU)
       if (p.K > 2048 && p.K <= 4096 && rows <= warps) TLC_SKINNY(1, 8, true), done = true;
   }
   if (!done) TLC_SKINNY(2, 4, false);
 #undef TLC_SKINNY
-  TLC_CHECK_LAUNCH("linear_int8 (up to 4 rows)");
+  TLC_CHECK_LAUNCH("linear_int8 (one row)");
   return 0;
 }
 
-template <typename TX, typename TO>
-int launch_of(const void* x, const Int8Args& p, int sms, cudaStream_t stream) {
-#define TLC_SKINNY(MR_) (p.mode == I8_GLU ? launch<TX, TO, MR_, true>(x, p, nullptr, 1, sms, stream) : launch<TX, TO, MR_, false>(x, p, nullptr, 1, sms, stream))
-  return p.M == 1 ? TLC_SKINNY(1) : p.M == 2 ? TLC_SKINNY(2) : TLC_SKINNY(4);
-#undef TLC_SKINNY
+template <typename TX, typename TO, bool GROUPED>
+int launch_of(const void* x, const Int8Args& p, const int* ids, int per_row, int sms, cudaStream_t stream) {
+  return p.mode == I8_GLU ? launch<TX, TO, true, GROUPED>(x, p, ids, per_row, sms, stream) : launch<TX, TO, false, GROUPED>(x, p, ids, per_row, sms, stream);
 }
-
-template <typename TX, typename TO>
-int launch_pairs(const void* x, const Int8Args& p, const int* ids, int per_row, int sms, cudaStream_t stream) {
-  return p.mode == I8_GLU ? launch<TX, TO, 1, true, true>(x, p, ids, per_row, sms, stream) : launch<TX, TO, 1, false, true>(x, p, ids, per_row, sms, stream);
+template <typename TO, bool GROUPED>
+int launch_from(const void* x, int x_dtype, const Int8Args& p, const int* ids, int per_row, int sms, cudaStream_t stream) {
+  if constexpr (!GROUPED)
+    if (x_dtype == TLC_I8) return launch_of<int8_t, TO, false>(x, p, ids, per_row, sms, stream);
+  return x_dtype == TLC_F32 ? launch_of<float, TO, GROUPED>(x, p, ids, per_row, sms, stream) : launch_of<__nv_bfloat16, TO, GROUPED>(x, p, ids, per_row, sms, stream);
 }
 
 }  // namespace
 
-// x [M, p.lda] of x_dtype (TLC_I8: p.a_scale holds the scales).
+// x: one row of K values, float, bfloat16 or integers (with their scale in p.a_scale).
 int tlc_int8_skinny(const void* x, int x_dtype, const Int8Args& p, int out_dtype, int sms, cudaStream_t stream) {
-  if (out_dtype == TLC_F32)
-    return x_dtype == TLC_I8 ? launch_of<int8_t, float>(x, p, sms, stream) : x_dtype == TLC_F32 ? launch_of<float, float>(x, p, sms, stream)
-                                                                          : launch_of<__nv_bfloat16, float>(x, p, sms, stream);
-  return x_dtype == TLC_I8 ? launch_of<int8_t, __nv_bfloat16>(x, p, sms, stream)
-                           : x_dtype == TLC_F32 ? launch_of<float, __nv_bfloat16>(x, p, sms, stream) : launch_of<__nv_bfloat16, __nv_bfloat16>(x, p, sms, stream);
+  return out_dtype == TLC_F32 ? launch_from<float, false>(x, x_dtype, p, nullptr, 1, sms, stream) : launch_from<__nv_bfloat16, false>(x, x_dtype, p, nullptr, 1, sms, stream);
 }
 
 // p.M pairs, each a product of its own: row pair / per_row of x (float or bfloat16), the weights of expert ids[pair], row `pair` of the result.
 int tlc_int8_skinny_pairs(const void* x, int x_dtype, const Int8Args& p, const int* ids, int per_row, int out_dtype, int sms, cudaStream_t stream) {
-  if (out_dtype == TLC_F32)
-    return x_dtype == TLC_F32 ? launch_pairs<float, float>(x, p, ids, per_row, sms, stream) : launch_pairs<__nv_bfloat16, float>(x, p, ids, per_row, sms, stream);
-  return x_dtype == TLC_F32 ? launch_pairs<float, __nv_bfloat16>(x, p, ids, per_row, sms, stream) : launch_pairs<__nv_bfloat16, __nv_bfloat16>(x, p, ids, per_row, sms, stream);
+  return out_dtype == TLC_F32 ? launch_from<float, true>(x, x_dtype, p, ids, per_row, sms, stream)
+                              : launch_from<__nv_bfloat16, true>(x, x_dtype, p, ids, per_row, sms, stream);
 }
