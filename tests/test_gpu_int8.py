@@ -579,3 +579,8 @@ def test_one_row_rounded_within_gives_the_same_bits(N, K):
                 ops.linear_int8_kernel()
         assert all(torch.equal(x, y) for x, y in zip(*got))
     ops.check_errors()
+
+
+@pytest.mark.parametrize("M,N,K", [(9, 100, 4096), (16, 2050, 2048), (13, 77, 1001), (15, 2048, 333), (12, 17, 16), (16, 8, 4081)])
+def test_up_to_sixteen_rows_give_the_same_bits(M, N, K):
+    test_few_rows_give_the_same_bits(M, N, K)

@@ -4,7 +4,7 @@
 //
 // The kernels, chosen in run() and tlc_linear_int8() by sizes, types and alignment alone:
 //   gemm_int8_skinny.cu  one row, and experts of up to 8 pairs: CUDA cores, rows rounded in the same kernel
-//   gemm_int8_thin.cu    up to 8 rows of up to 4,096 values: mma.sync on weights that come from HBM into registers
+//   gemm_int8_thin.cu    up to 16 rows of up to 4,096 values: mma.sync on weights that come from HBM into registers
 //   gemm_int8_few.cu     up to 64 rows, more where tiles are few: tensor cores, K shared among the blocks of a cluster
 //   gemm_int8_wide.cu    many rows, groups of 25 and more: tensor cores, pairs of blocks, persistent
 //   here                 operands that the copy engine does not take (rows off 16-byte boundaries; gated outputs that are no multiple of
@@ -151,11 +151,14 @@ int g_kernel = 0, g_rows = 0;        // test hook: which kernel, on tiles of how
 
 int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
   const int sms = sm_count();
-  // Up to 8 rows: weights straight to the registers of mma.sync, for one wave of blocks before the wait.  Microseconds there and through shared
-  // memory, 8 rows: 2,048 -> 2,048 2.1, 3.6; 4,096 -> 2,048 2.5, 4.4; 2,048 -> 8,240 3.9, 6.0; 2,560 -> 2 x 8,192 9.2, 10.1; 2,048 ->
-  // 65,536 22.6, 26.1.  (12 rows in two eights 5.3 and 6.1 for 2,048 -> 8,240, but 38 and 27 for 65,536; 8,192 -> 2,560 by clusters of
-  // two blocks 7.6 and 6.8.)
-  if (!p.offsets && (g_kernel == 0 || g_kernel >= 4) && p.M <= 8 && p.K <= TLC_INT8_THIN && ((uintptr_t)p.w | (uintptr_t)p.ldw) % 16 == 0)
+  // Up to 16 rows: weights straight to the registers of mma.sync, for one wave of blocks before the wait.  Microseconds there and through
+  // shared memory, 8 rows: 2,048 -> 2,048 2.1, 3.6; 4,096 -> 2,048 2.5, 4.4; 2,048 -> 8,240 3.9, 6.0; 2,560 -> 2 x 8,192 9.2, 10.1;
+  // 2,048 -> 65,536 22.6, 26.1.  12 rows: 2,048 -> 2,048 2.8, 3.7; 4,096 -> 2,048 3.2, 4.5; 2,048 -> 8,240 5.1, 6.1, but from 24 MB of
+  // weights on 2,560 -> 10,240 8.2, 8.1; 2,560 -> 2 x 8,192 12.0, 10.2; 2,048 -> 65,536 30.8, 26.3.  (8 rows of 8,192 -> 2,560 by clusters
+  // of two blocks 7.6, 6.8.)
+  const bool thin = p.M <= 8 || (p.M <= 16 && (long long)p.w_rows * p.K <= 24 << 20);
+  if (!p.offsets && (g_kernel == 5 ? p.M <= 16 : thin && (g_kernel == 0 || g_kernel == 4)) && p.K <= TLC_INT8_THIN &&
+      ((uintptr_t)p.w | (uintptr_t)p.ldw) % 16 == 0)
     return tlc_int8_thin(p, out_dtype, stream);
   if (g_kernel != 1 && tensor_cores_take(p)) {
     const int pairs = tlc_linear_pairs();
@@ -193,7 +196,7 @@ int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
 }  // namespace
 
 // Test hook: 0 = chosen by the sizes; 1 = the CUDA cores; 2 = tiles of 128 weight rows and 16, 32, 64 or 128 activation rows; 3 = pairs of
-// blocks on 256 weight rows and 128 or 256 activation rows; 4 = the kernel of one row; 5 = the kernel of up to 8 rows, wherever
+// blocks on 256 weight rows and 128 or 256 activation rows; 4 = the kernel of one row; 5 = the kernel of up to 16 rows, wherever
 // they take the operands.
 extern "C" int tlc_linear_int8_kernel(int kernel, int rows) {
   TLC_REQUIRE(kernel == 0 || kernel == 1 || (kernel == 2 && (rows == 16 || rows == 32 || rows == 64 || rows == 128)) ||

@@ -9,8 +9,8 @@
 // exactly, in whatever order.  Then scales, bias, activation or sum: a warp a row, a lane four weight rows.
 //
 // What bounds it: the weights' stream where there are enough of them (64 rows of 2,560 -> 16,384 12.0 us, 42 MB at 3.5 TB/s; 37 rows of
-// experts, 134 MB, 26 us, 5.1 TB/s), else the way in and out: set-up, first bytes, the cluster's meeting, stores (12 rows of 2,048 -> 2,048 3.7
-// us, of which the 4 MB are 0.65; 24 of 8,192 -> 2,560 7.2, 21 MB).  Two blocks an SM keep 190 to 220 KB on their way.
+// experts, 134 MB, 26 us, 5.1 TB/s), else the way in and out: set-up, first bytes, the cluster's meeting, stores (24 rows of 8,192 -> 2,560
+// 7.2 us, 21 MB; 32 of 2,048 -> 8,240 6.5, 17 MB).  Two blocks an SM keep 190 to 220 KB on their way.
 //
 // Gated products find a feature's gate and up row 8 lanes of tensor memory apart, because the copy interleaves them so
 // (load_weights).  Waits are bounded (codes 51-54); a block whose wait ran out still meets its cluster.
