@@ -24,13 +24,20 @@ constexpr int TLC_INT8_THIN = 4096;       // values of a row in the kernel of up
 constexpr int TLC_INT8_GROUPS = 4096;     // at most (as a routing)
 enum { I8_PLAIN = 0, I8_ADD = 1, I8_ACT = 2, I8_GLU = 3 };
 
-// 16 values from k on, zeros past K; whole: on a 16-byte boundary.
-__device__ __forceinline__ int4 sixteen(const int8_t* p, int k, int K, bool whole) {
-  if (whole && k + 16 <= K) return __ldg(reinterpret_cast<const int4*>(p + k));
+// 16 values of a row from k on, zeros past K.  Weights (rows on 16-byte boundaries) come through the read-only way; activations, which an
+// earlier kernel may still have been writing when this one started, by ordinary loads (whole: the row is on a 16-byte boundary).  Past the
+// L1 they would cost the blocks of an SM, which read the same rows, half a microsecond of four.
+__device__ __forceinline__ int4 int8_bytes(const int8_t* p, int k, int K) {
   int v[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < 16; i++) if (k + i < K) v[i >> 2] |= (int)(uint8_t)p[k + i] << (8 * (i & 3));
   return make_int4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ int4 int8_weights(const int8_t* p, int k, int K) {
+  return k + 16 <= K ? __ldg(reinterpret_cast<const int4*>(p + k)) : int8_bytes(p, k, K);
+}
+__device__ __forceinline__ int4 int8_row(const int8_t* p, int k, int K, bool whole) {
+  return whole && k + 16 <= K ? *reinterpret_cast<const int4*>(p + k) : int8_bytes(p, k, K);
 }
 
 // One result from its integer sum.  Both scales in 32 bits, one after the other: their product alone may leave the range.  The

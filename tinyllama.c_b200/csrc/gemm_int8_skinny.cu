@@ -22,7 +22,7 @@ __device__ __forceinline__ int dot16(int4 a, int4 b, int c) { return __dp4a(a.w,
 // The block's copy of the row: integers in xs [ld], zeros from K on; returns its scale.
 __device__ __forceinline__ float stage(const int8_t* x, const float* a_scale, int K, int8_t* xs, int ld, unsigned*) {
   const float scale = *a_scale;
-  for (int k = 16 * threadIdx.x; k < ld; k += 16 * THREADS) *reinterpret_cast<int4*>(xs + k) = sixteen(x, k, K, (uintptr_t)x % 16 == 0);
+  for (int k = 16 * threadIdx.x; k < ld; k += 16 * THREADS) *reinterpret_cast<int4*>(xs + k) = int8_row(x, k, K, (uintptr_t)x % 16 == 0);
   __syncthreads();
   return scale;
 }
@@ -100,7 +100,7 @@ int8_skinny_kernel(const TX* __restrict__ x, Int8Args p, const int* __restrict__
 #pragma unroll
       for (int r = 0; r < R; r++) {
         const int k = k0 + 512 * j + 16 * lane, n = min(C * item + (GLU ? r % C : r), p.N - 1) + (GLU && r >= C ? p.N : 0);
-        w[r][j] = k < K ? sixteen(p.w + (size_t)n * p.ldw, k, K, true) : make_int4(0, 0, 0, 0);
+        w[r][j] = k < K ? int8_weights(p.w + (size_t)n * p.ldw, k, K) : make_int4(0, 0, 0, 0);
       }
   };
   // lane c finishes column c of the item; its scales and biases come with the weights

@@ -42,7 +42,7 @@ int8_thin_kernel(Int8Args p) {
 #pragma unroll
   for (int j = 0; j < PIECES; j++)
 #pragma unroll
-    for (int r = 0; r < 2; r++) w[r][j] = k0 + 64 * j < K ? sixteen(rows[r], k0 + 64 * j, K, true) : make_int4(0, 0, 0, 0);
+    for (int r = 0; r < 2; r++) w[r][j] = k0 + 64 * j < K ? int8_weights(rows[r], k0 + 64 * j, K) : make_int4(0, 0, 0, 0);
   // thread m C + c finishes column c of row m
   const int c = threadIdx.x % C, m = threadIdx.x / C, n = n0 + c;
   const bool finishes = m < p.M && n < p.N;
@@ -74,7 +74,7 @@ int8_thin_kernel(Int8Args p) {
       if (NT > 1 && k + 16 <= K && row < p.M && whole)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from + k) : "memory");
       else
-        *to = k < K && row < p.M ? sixteen(from, k, K, whole) : make_int4(0, 0, 0, 0);
+        *to = k < K && row < p.M ? int8_row(from, k, K, whole) : make_int4(0, 0, 0, 0);
     }
   float old = 0.f, rs = 0.f;
   if (finishes) {
