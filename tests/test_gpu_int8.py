@@ -584,3 +584,30 @@ def test_one_row_rounded_within_gives_the_same_bits(N, K):
 @pytest.mark.parametrize("M,N,K", [(9, 100, 4096), (16, 2050, 2048), (13, 77, 1001), (15, 2048, 333), (12, 17, 16), (16, 8, 4081)])
 def test_up_to_sixteen_rows_give_the_same_bits(M, N, K):
     test_few_rows_give_the_same_bits(M, N, K)
+
+
+@pytest.mark.parametrize("N,K", [(2048, 2048), (8240, 2048), (4738, 2041), (9480, 100), (33, 17), (8, 2049)])
+def test_two_rows_rounded_within_give_the_same_bits(N, K):
+    """Two rows in 16 or 32 bits, on 16-byte boundaries and off them, one with a NaN, rounded where they are multiplied."""
+    g = gen(N + 2 * K)
+    w, sw, bias = integers(g, N, K), scales(g, N), normal(g, N)
+    for xt, dtype, first in ((torch.bfloat16, torch.float32, 0), (torch.float32, torch.bfloat16, 0), (torch.bfloat16, torch.bfloat16, 3)):
+        x = normal(g, 2, K + 5, dtype=xt)[:, first:first + K]
+        if first:
+            x[1, K // 2] = float("nan")
+        got = []
+        for k in ((1, 0), (4, 0)):
+            ops.linear_int8_kernel(*k)
+            try:
+                outs = [torch.full((2, N), 3.0, dtype=dtype, device=DEV), torch.ones(2, N, dtype=dtype, device=DEV)]
+                ops.linear_int8(x, w, sw, outs[0], colbias=bias)
+                ops.linear_int8(x, w, sw, outs[1], accumulate=True)
+                if N % 2 == 0:
+                    outs.append(torch.full((2, N // 2), 3.0, dtype=dtype, device=DEV))
+                    ops.linear_swiglu_int8(x, w, sw * 0.1, outs[2])
+                got.append(outs)
+            finally:
+                ops.linear_int8_kernel()
+        assert all(torch.equal(a.nan_to_num(7e30), b.nan_to_num(7e30)) for a, b in zip(*got))
+        assert not first or bool(got[0][0][1].isnan().all())
+    ops.check_errors()

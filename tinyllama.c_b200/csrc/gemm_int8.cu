@@ -3,7 +3,7 @@
 // order of a sum nor how K is cut changes a result.
 //
 // The kernels, chosen in run() and tlc_linear_int8() by sizes, types and alignment alone:
-//   gemm_int8_skinny.cu  one row, and experts of up to 8 pairs: CUDA cores, rows rounded in the same kernel
+//   gemm_int8_skinny.cu  one row (two that are to be rounded), and experts of up to 8 pairs: CUDA cores, rows rounded in the same kernel
 //   gemm_int8_thin.cu    up to 16 rows of up to 4,096 values: mma.sync on weights that come from HBM into registers
 //   gemm_int8_few.cu     up to 64 rows, more where tiles are few: tensor cores, K shared among the blocks of a cluster
 //   gemm_int8_wide.cu    many rows, groups of 25 and more: tensor cores, pairs of blocks, persistent
@@ -223,9 +223,9 @@ extern "C" int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_sca
   // One row of at most 8,192 values, weights in 16-byte pieces and up to 24 MB of them: the kernel that takes the row as it is.
   // Microseconds there and by gemm_int8_thin.cu (from K = 4,097 the tensor cores), a row to be rounded: 2,048 -> 2,048 2.1, 2.8; 2,048 ->
   // 8,240 3.7, 4.5; 4,096 -> 2,048 3.0, 3.5; 2,048 -> 2 x 4,096 3.4, 4.6; 8,192 -> 2,560 7.4, 7.5; 2,560 -> 10,240 8.2, 6.8.  Integers
-  // behind the norm that makes them, both: 2,048 -> 8,240 4.5, 4.8; gated 4.5, 5.0.  (Two rows rounded in every block were 4.5 and 4.6 us
-  // for 2,048 -> 8,240 and 4,096 -> 2,048, rounded first 4.3 and 3.6.)
-  const bool takes = M == 1 && K <= TLC_INT8_SKINNY && ((uintptr_t)w | (uintptr_t)ldw) % 16 == 0;
+  // behind the norm that makes them, both: 2,048 -> 8,240 4.5, 4.8; gated 4.5, 5.0.  Two rows that are to be rounded, up to K = 2,048: 2,048
+  // -> 2,048 2.9, 3.1, -> 8,240 4.5, 4.5, and a launch less for the host (4,096 -> 2,048 4.6, 3.7; three rows 6.8, 4.6).
+  const bool takes = (M == 1 ? K <= TLC_INT8_SKINNY : M == 2 && a_dtype != TLC_I8 && K <= TLC_INT8_SKINNY / 4) && ((uintptr_t)w | (uintptr_t)ldw) % 16 == 0;
   if (takes && (g_kernel == 4 || (g_kernel == 0 && (long long)p.w_rows * K <= 24 << 20))) return tlc_int8_skinny(a, a_dtype, p, out_dtype, sm_count(), stream);
   if (a_dtype != TLC_I8) {
     if (!a_int8 || !a_scale) return 1;                     // (room is wanted)

@@ -1696,7 +1696,7 @@ def _linear_int8(what, a, a_scale, w, w_scale, colbias, out, N, accumulate, act,
             raise KernelError(f"{what}: a_scale belongs to integer rows; a is {a.dtype}")
         code, ldq = dtype_code(a.dtype), (K + 15) // 16 * 16
         scale = q = 0
-        if M > 1:                                        # (one row mostly goes without; the library says so where not)
+        if M > 2 or (M == 2 and K > 2048):                 # (one or two rows mostly go without; the library says so where not)
             scale, q = _int8_room(M, ldq, a.device)
     args = (w.data_ptr(), ldw, w_scale.data_ptr(), out.data_ptr(), dtype_code(out.dtype), ldo, bias, accumulate, M, N, K, act, limit, alpha, _stream())
     if not _call_packed("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, *args, ok=1):
