@@ -196,7 +196,7 @@ int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
 }  // namespace
 
 // Test hook: 0 = chosen by the sizes; 1 = the CUDA cores; 2 = tiles of 128 weight rows and 16, 32, 64 or 128 activation rows; 3 = pairs of
-// blocks on 256 weight rows and 128 or 256 activation rows; 4 = the kernel of one row; 5 = the kernel of up to 16 rows, wherever
+// blocks on 256 weight rows and 128 or 256 activation rows; 4 = the kernel of one or two rows; 5 = the kernel of up to 16 rows, wherever
 // they take the operands.
 extern "C" int tlc_linear_int8_kernel(int kernel, int rows) {
   TLC_REQUIRE(kernel == 0 || kernel == 1 || (kernel == 2 && (rows == 16 || rows == 32 || rows == 64 || rows == 128)) ||

@@ -19,7 +19,7 @@ struct Int8Args {
   int E;
   int scatter, w_out;                   // result rows go where order says, times the pair's weight
 };
-constexpr int TLC_INT8_SKINNY = 8192;     // values of the row in the kernel of one row, at most
+constexpr int TLC_INT8_SKINNY = 8192;     // values of the row in the kernel of one or two rows, at most
 constexpr int TLC_INT8_THIN = 4096;       // values of a row in the kernel of up to 16 rows, at most: 256 for each of 16 warps
 constexpr int TLC_INT8_GROUPS = 4096;     // at most (as a routing)
 enum { I8_PLAIN = 0, I8_ADD = 1, I8_ACT = 2, I8_GLU = 3 };

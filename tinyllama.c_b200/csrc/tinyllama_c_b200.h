@@ -436,7 +436,7 @@ int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_scale, void* a
                     const float* w_scale, void* out, int out_dtype, int ldo, const float* colbias, int accumulate, int M,
                     int N, int K, int act, float limit, float alpha, cudaStream_t stream);
 /* Test hook: 0 = the kernel is chosen by the sizes; 1 = the CUDA cores; 2 = tiles of 128 weight rows and `rows` = 16, 32, 64 or 128
- * activation rows; 3 = pairs of blocks, 128 or 256 activation rows; 4 = the kernel of one row; 5 = of up to 16
+ * activation rows; 3 = pairs of blocks, 128 or 256 activation rows; 4 = the kernel of one or two rows; 5 = of up to 16
  * rows; where the operands allow. */
 int tlc_linear_int8_kernel(int kernel, int rows);
 /* The experts' feed-forwards over the pairs that tlc_moe_route sorted, in 8-bit integers: x [T, ldx] float or bfloat16;

@@ -1594,7 +1594,7 @@ INT8_MAX_K = 131071                      # 128 * 128 * K < 2^31: the sums of pro
 
 def linear_int8_kernel(kernel: int = 0, rows: int = 0) -> None:
     """Which kernel the products in 8-bit integers take where it takes the operands: 0 chosen by the sizes, 1 the CUDA cores, 2 tiles of
-    128 weight rows and `rows` (16, 32, 64 or 128) activation rows, 3 pairs of blocks on tiles of 128 or 256, 4 the kernel of one row, 5 that of up to 16 rows.  For tests."""
+    128 weight rows and `rows` (16, 32, 64 or 128) activation rows, 3 pairs of blocks on tiles of 128 or 256, 4 the kernel of one or two rows, 5 that of up to 16 rows.  For tests."""
     lib = library()
     if lib.tlc_linear_int8_kernel(int(kernel), int(rows)) != 0:
         raise KernelError(f"linear_int8_kernel: {lib.tlc_last_error().decode()}")
