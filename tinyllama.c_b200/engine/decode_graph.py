@@ -53,6 +53,7 @@ class DecodeGraph:
         self.out_host = torch.zeros(B, dtype=torch.int32).pin_memory()
         self.logits: Optional[torch.Tensor] = None
         self.graph: Optional[torch.cuda.CUDAGraph] = None
+        self.weights_version = -1                 # of the model, when the step was captured
         self.launches = 0
 
     def _body(self) -> None:
@@ -70,6 +71,7 @@ class DecodeGraph:
         writes only what the buffers name, and the buffers name the sequences of the first real
         step), then captures it."""
         before = ops.launch_count()
+        self.weights_version = self.model.weights_version
         stream = torch.cuda.Stream(device=self.model.device)
         stream.wait_stream(torch.cuda.current_stream())
         self.graph = torch.cuda.CUDAGraph()
@@ -102,13 +104,19 @@ class DecodeGraph:
                 if tail:
                     hh[r, :len(tail)] = tail
             self.history.copy_(self.hhost, non_blocking=True)
-        if self.graph is None:
+        if self.stale:
             self.capture()          # the capture itself does not execute; the replay below does
         self.graph.replay()
         ops.count_launches(self.launches)
         self.out_host.copy_(self.out, non_blocking=True)
         torch.cuda.current_stream().synchronize()
         return self.out_host.tolist()
+
+    @property
+    def stale(self) -> bool:
+        """Whether the step is still to be captured: not captured yet, or of weights that the model has since replaced (the graph
+        has their addresses in it, and their memory may be someone else's by now)."""
+        return self.graph is None or self.weights_version != self.model.weights_version
 
     @property
     def h2d_bytes(self) -> int:

@@ -66,6 +66,7 @@ class Model:
         self.dtype: Optional[torch.dtype] = None
         self.device: Optional[torch.device] = None
         self.repeated: Optional[RepeatedLayers] = None      # the run order's layers, where they were all alike when bound
+        self.weights_version = 0        # counts bind() and to_int8(): a captured step holds its weights' addresses, and is captured anew
 
     def _collect_chunks(self) -> None:
         """What the layers ask the step function for."""
@@ -118,6 +119,7 @@ class Model:
     def bind(self, tensors: Dict[str, torch.Tensor], dtype: torch.dtype, device) -> None:
         self.dtype, self.device = dtype, torch.device(device)
         self.repeated = None
+        self.weights_version += 1
         for layer in self.layers:
             layer.bind(tensors, dtype, device)
         self._collect_chunks()
@@ -136,9 +138,11 @@ class Model:
 
     def to_int8(self) -> None:
         """The bound model with the weights of its layers' products in 8-bit integers, a scale per output channel; embedding, head,
-        norms, routers, convolutions and states stay as they are.  Once, before the first step."""
+        norms, routers, convolutions and states stay as they are.  In place: whoever holds this model (every LLM made of it) multiplies
+        in 8-bit integers from the next step on, and the 16-bit weights are let go."""
         if self.dtype != torch.bfloat16:
             raise ValueError("weights in 8-bit integers go with bfloat16 runs; a float32 run keeps its weights in 32 bits")
+        self.weights_version += 1
         for layer in self.layers:
             layer.to_int8()
         self.expert_tables = ops.ExpertTables([p.table_entry() for p in self.by_table]) if self.by_table else None
