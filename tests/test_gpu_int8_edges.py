@@ -1,0 +1,46 @@
+"""Products in 8-bit integers where operands are at the edge of what they can be."""
+import numpy as np
+import pytest
+import torch
+
+from tinyllama_c_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _next_to_halves(exponent, K, seed):
+    """Rows [64, K] (numpy float32) whose scales are 2^exponent to 2^(exponent + 1) and whose quotients by them lie next to a half; with
+    them their scales and the integers nearest to the quotients, both by IEEE divisions."""
+    r = np.random.RandomState(seed)
+    largest = (np.float32(127) * np.ldexp(r.uniform(1.01, 1.99, (64, 1)).astype(np.float32), exponent)).astype(np.float32)
+    s = (largest / np.float32(127)).astype(np.float32)
+    half = r.randint(-126, 126, (64, K)) + 0.5
+    x = (half * s.astype(np.float64)).astype(np.float32)
+    up = np.nextafter(x, np.float32(np.inf)), np.nextafter(x, np.float32(-np.inf)), x
+    x = np.choose(r.randint(0, 3, x.shape), up).astype(np.float32)
+    x[:, :1] = largest
+    return x, s, np.rint((x / s).astype(np.float32)).astype(np.int8)
+
+
+@pytest.mark.parametrize("K", [64, 2048, 77])
+@pytest.mark.parametrize("exponent", [-126, -125, -122, -118, -103, -102, -101, -100, -99, -90, -30, 100, 119])
+def test_integers_of_small_and_large_rows_are_those_of_the_quotients(exponent, K):
+    """Down to the smallest scale that a row can have (2^-126): equal to the nearest integer of the IEEE quotient."""
+    x, s, q = _next_to_halves(exponent, K, K)
+    rows = torch.from_numpy(x).to(DEV)
+    got, scale = ops.rows_int8(rows)
+    assert np.array_equal(scale.cpu().numpy(), s[:, 0]) and np.array_equal(got.cpu().numpy(), q)
+    if exponent < 0:                                     # (the sum of squares of larger rows is infinite)
+        got, _ = ops.rmsnorm_int8(rows, torch.ones(K, device=DEV), 1e-5)
+        assert np.array_equal(got.cpu().numpy(), q)
+    # one row and two, rounded by the product itself: times the unit matrix and a power of two that brings them into range
+    w = ops.int8_empty(K, K, DEV)
+    w.copy_(torch.eye(K, dtype=torch.int8))
+    power = 2.0 ** (-exponent if exponent < 0 else 0)
+    for M in (1, 2):
+        out = torch.empty(M, K, device=DEV)
+        ops.linear_int8(rows[:M], w, torch.full((K,), power, device=DEV), out)
+        want = (q[:M].astype(np.float32) * s[:M]) * np.float32(power)
+        assert np.array_equal(out.cpu().numpy(), want)
+    ops.check_errors()
