@@ -116,12 +116,15 @@ int launch(const Int8Args& p, cudaStream_t stream) {
   const int warps = std::max(8 * NT * C / 32, (p.K + SPAN - 1) / SPAN);      // (a thread for every result, too)
   const int smem = NT == 1 ? 0 : warps * NT * PIECES * 32 * (int)sizeof(int4);      // 64 KB at most
   if (NT > 1) {
-    static std::atomic<bool> set{false};
-    if (!set) {
+    static std::atomic<unsigned long long> raised{0};       // a bit a device: the limit is the device's, and this kernel runs on any
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (!(raised & bit)) {
       const int most = MOST * NT * PIECES * 32 * (int)sizeof(int4);
       if (cudaFuncSetAttribute(int8_thin_kernel<TO, NT, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
         return tlc_fail(-2, "linear_int8: cannot reserve %d bytes of shared memory", most);
-      set = true;
+      raised |= bit;
     }
   }
   tlc_launch(int8_thin_kernel<TO, NT, GLU>, dim3((p.N + C - 1) / C), dim3(32 * warps), smem, stream, p);
