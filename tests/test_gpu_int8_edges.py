@@ -44,3 +44,31 @@ def test_integers_of_small_and_large_rows_are_those_of_the_quotients(exponent, K
         want = (q[:M].astype(np.float32) * s[:M]) * np.float32(power)
         assert np.array_equal(out.cpu().numpy(), want)
     ops.check_errors()
+
+
+def _operands(M, N, K, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    x = torch.empty(M, K, device=DEV).normal_(generator=g)
+    return x, *ops.weight_int8(torch.empty(N, K, device=DEV).normal_(0.0, 0.1, generator=g)), g
+
+
+def test_numbers_beyond_32_bits_are_infinities_as_in_the_16_bit_products():
+    """A clamp that does nothing, given as a number that only 64 bits hold."""
+    x, w, sw, g = _operands(5, 128, 64, 1)
+    outs = []
+    for limit in (1e300, float("inf"), 1e30):
+        outs.append(torch.empty(5, 64, device=DEV))
+        ops.linear_swiglu_int8(x, w, sw, outs[-1], act="swish_clamped", limit=limit, alpha=1.5)
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+    logits = torch.empty(5, 2, device=DEV).normal_(generator=g)
+    wd, sd = ops.weight_int8(torch.empty(2, 64, 64, device=DEV).normal_(generator=g))
+    wgu, sgu = torch.stack([w, w]), torch.stack([sw, sw])
+    outs = []
+    for limit in (1e300, float("inf")):
+        outs.append(torch.empty(5, 1, 64, device=DEV))
+        ops.moe_experts_int8(x, wgu, sgu, wd, sd, ops.moe_route(logits, 2, 1), 1, outs[-1], act_fn="swish_clamped", limit=limit, alpha=1.5)
+    assert torch.equal(*outs)
+    weights = [ops.moe_route(logits, 2, 1, weights="softmax_all", sum_to=s)[1] for s in (1e300, float("inf"))]
+    assert torch.equal(*weights) and bool(torch.isinf(weights[0]).all())
+    ops.check_errors()

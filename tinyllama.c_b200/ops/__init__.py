@@ -250,7 +250,11 @@ def _call_packed(name: str, *args, ok: int = 0) -> bool:
         pack = struct.Struct("=" + "".join("f4x" if t is _f else "q" for t in _SIGNATURES[name][1])).pack
         hit = _packs[name] = (lib, lib.tlc_call, lib.tlc_replay_index(name.encode()), pack)
     lib, call, index, pack = hit
-    rc = call(index, pack(*args))
+    try:
+        words = pack(*args)
+    except OverflowError:                # a float beyond the 32-bit range is infinity, as in every other call
+        words = pack(*(_f(a).value if t is _f else a for t, a in zip(_SIGNATURES[name][1], args)))
+    rc = call(index, words)
     if rc != 0:
         if ok and rc == ok:
             return False
