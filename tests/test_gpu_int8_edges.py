@@ -72,3 +72,20 @@ def test_numbers_beyond_32_bits_are_infinities_as_in_the_16_bit_products():
     weights = [ops.moe_route(logits, 2, 1, weights="softmax_all", sum_to=s)[1] for s in (1e300, float("inf"))]
     assert torch.equal(*weights) and bool(torch.isinf(weights[0]).all())
     ops.check_errors()
+
+
+def test_rows_further_apart_than_32_bits_count_are_refused():
+    """Strides of 2^32 + 64 elements, which as 32-bit numbers would be 64."""
+    far = (1 << 32) + 64
+    room = torch.zeros(far + 4096, dtype=torch.int8, device=DEV)
+    a, sa = room.as_strided((2, 64), (far, 1)), torch.ones(2, device=DEV)
+    x, w, sw, g = _operands(2, 128, 64, 2)
+    out = torch.empty(2, 128, device=DEV)
+    with pytest.raises(ops.KernelError):
+        ops.linear_int8(a, w, sw, out, a_scale=sa)
+    with pytest.raises(ops.KernelError):
+        ops.linear_int8(x, a, sa, torch.empty(2, 2, device=DEV))
+    with pytest.raises(ops.KernelError):
+        ops.rows_int8(x, (a, sa))
+    ops.linear_int8(x, w, sw, out)                       # and nothing is left of it
+    assert bool(torch.isfinite(out).all())

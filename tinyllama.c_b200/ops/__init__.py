@@ -247,13 +247,15 @@ def _call_packed(name: str, *args, ok: int = 0) -> bool:
     hit = _packs.get(name)
     if hit is None:
         lib = library()
-        pack = struct.Struct("=" + "".join("f4x" if t is _f else "q" for t in _SIGNATURES[name][1])).pack
+        pack = struct.Struct("=" + "".join("f4x" if t is _f else "i4x" if t is _i else "q" for t in _SIGNATURES[name][1])).pack
         hit = _packs[name] = (lib, lib.tlc_call, lib.tlc_replay_index(name.encode()), pack)
     lib, call, index, pack = hit
     try:
         words = pack(*args)
     except OverflowError:                # a float beyond the 32-bit range is infinity, as in every other call
         words = pack(*(_f(a).value if t is _f else a for t, a in zip(_SIGNATURES[name][1], args)))
+    except struct.error as e:            # (rows further apart than the kernels count, say)
+        raise KernelError(f"{name}: sizes and strides are whole numbers of 32 bits ({e}); got {args}") from e
     rc = call(index, words)
     if rc != 0:
         if ok and rc == ok:
