@@ -89,3 +89,27 @@ def test_rows_further_apart_than_32_bits_count_are_refused():
         ops.rows_int8(x, (a, sa))
     ops.linear_int8(x, w, sw, out)                       # and nothing is left of it
     assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("kernel", [(0, 0), (3, 128), (3, 256)])
+def test_results_whose_rows_lie_far_apart(kernel):
+    """Rows of the result 310,000,000 values apart: the sixteenth begins beyond 2^32."""
+    M, N, K, far = 16, 64, 256, 310_000_000
+    x, w, sw, g = _operands(M, N, K, 3)
+    a, sa = ops.rows_int8(x)
+    room = torch.empty((M - 1) * far + N, dtype=torch.bfloat16, device=DEV)
+    for product, n in ((ops.linear_int8, N), (ops.linear_swiglu_int8, N // 2)):
+        want = torch.empty(M, n, dtype=torch.bfloat16, device=DEV)
+        product(a, w, sw, want, a_scale=sa)
+        out = room.as_strided((M, n), (far, 1))
+        out.fill_(float("nan"))
+        ops.linear_int8_kernel(*kernel)
+        try:
+            product(a, w, sw, out, a_scale=sa)
+            if product is ops.linear_int8:
+                product(a, w, sw, out, a_scale=sa, accumulate=True)
+                product(a, w, sw, want, a_scale=sa, accumulate=True)
+        finally:
+            ops.linear_int8_kernel()
+        assert torch.equal(out, want)
+    ops.check_errors()

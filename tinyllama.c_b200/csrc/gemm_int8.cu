@@ -161,7 +161,7 @@ int run(const Int8Args& p, int out_dtype, cudaStream_t stream) {
       ((uintptr_t)p.w | (uintptr_t)p.ldw) % 16 == 0)
     return tlc_int8_thin(p, out_dtype, stream);
   if (g_kernel != 1 && tensor_cores_take(p)) {
-    const int pairs = tlc_linear_pairs();
+    const int pairs = p.ldo < 1 << 27 ? tlc_linear_pairs() : 0;      // (sixteen rows of a result are addressed in 32 bits there)
     if (g_kernel == 3 && pairs > 0) return tlc_int8_wide(p, out_dtype, g_rows, pairs, stream);
     if (g_kernel == 2) return tlc_int8_few(p, out_dtype, g_rows, sms, stream);
     if (p.offsets) {
