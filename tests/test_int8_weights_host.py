@@ -1,6 +1,7 @@
 """Models whose weights become 8-bit integers: what needs no GPU."""
 from types import SimpleNamespace
 
+import pytest
 import torch
 
 from tinyllama_c_b200.engine.decode_graph import DecodeGraph
@@ -28,3 +29,13 @@ def test_a_captured_step_is_stale_once_the_model_has_other_weights(tmp_path):
     tensors = {s.name: torch.zeros(s.shape) for s in model.weight_specs()}
     model.bind(tensors, torch.float32, "cpu")
     assert stale()
+
+
+def test_a_model_stored_in_32_bits_is_refused(tmp_path):
+    """Its matrices keep their 32 bits: asked for 8, it would run unchanged."""
+    folder = make_model_dir(tmp_path, configs.TINY_A, seed=3, dtype="float32")
+    with pytest.raises(ValueError, match="32 bits"):
+        load_model(folder, "bfloat16", "cpu", weights="int8")
+    model = load_model(folder, "bfloat16", "cpu")
+    with pytest.raises(ValueError, match="32 bits"):
+        model.to_int8()

@@ -41,7 +41,8 @@ class LLM:
                  max_seqs: Optional[int] = None, device: str = "cuda:0", use_graphs: bool = True, weights: Optional[str] = None):
         """model_dir: a folder with config.json and model.safetensors, or a model that is
         already bound to its weights on `device` (see random_model).  weights "int8": the products of the layers in 8-bit
-        integers, weights with a scale per output channel and activations rounded row by row.  A bound model is converted in place
+        integers, weights with a scale per output channel and activations rounded row by row (a matrix that is stored in 32 bits keeps
+        them; a model of nothing else is refused).  A bound model is converted in place
         (Model.to_int8): every other LLM of it multiplies in 8-bit integers from then on as well."""
         if not torch.cuda.is_available():
             raise RuntimeError("tinyllama.c_b200 needs a CUDA device (NVIDIA B200); there is no CPU path")

@@ -139,12 +139,14 @@ class Model:
     def to_int8(self) -> None:
         """The bound model with the weights of its layers' products in 8-bit integers, a scale per output channel; embedding, head,
         norms, routers, convolutions and states stay as they are.  In place: whoever holds this model (every LLM made of it) multiplies
-        in 8-bit integers from the next step on, and the 16-bit weights are let go."""
+        in 8-bit integers from the next step on, and the 16-bit weights are let go.  Matrices that are stored in 32 bits keep them; a model
+        that has no others is refused."""
         if self.dtype != torch.bfloat16:
             raise ValueError("weights in 8-bit integers go with bfloat16 runs; a float32 run keeps its weights in 32 bits")
         self.weights_version += 1
-        for layer in self.layers:
-            layer.to_int8()
+        if not sum([layer.to_int8() for layer in self.layers]):
+            raise ValueError("there is nothing to lay out in 8-bit integers: every matrix of the layers is stored in 32 bits, and such a matrix "
+                             "keeps them")
         self.expert_tables = ops.ExpertTables([p.table_entry() for p in self.by_table]) if self.by_table else None
         self.repeated = RepeatedLayers.of(self.layers, self.schedule) if self.device.type == "cuda" else None
 

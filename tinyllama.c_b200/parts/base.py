@@ -170,12 +170,11 @@ class Part(Editable):
         """What the step function must prepare for this part in every step (ChunkRequest)."""
         return []
 
-    def to_int8(self) -> None:
+    def to_int8(self) -> int:
         """Lays out the bound 16-bit matrices of this part's products as 8-bit integers with a scale per output channel; their
-        inputs are rounded to such integers row by row from then on.  What a part keeps of other kinds stays as it is."""
-        for v in list(vars(self).values()):
-            if isinstance(v, Editable) and hasattr(v, "to_int8"):
-                v.to_int8()
+        inputs are rounded to such integers row by row from then on.  What a part keeps of other kinds stays as it is.  Returns how many
+        matrices are integers now."""
+        return sum(v.to_int8() for v in list(vars(self).values()) if isinstance(v, Editable) and hasattr(v, "to_int8"))
 
 
 class Position(Part):

@@ -128,7 +128,7 @@ class Block(Part):
                     self.out_offsets.append((off, pr.in_features))
                     off += pr.in_features
 
-    def to_int8(self) -> None:
+    def to_int8(self) -> int:
         """The layer's products in 8-bit integers: projections that its mixers share as one matrix (the mixers' own are ranges of
         it then too), other mixers' and the feed-forward's by themselves.  The norm in front of a product that its part shares with
         nobody leaves integers at once (_pre_norm)."""
@@ -146,10 +146,8 @@ class Block(Part):
                     pr.weight, pr.int8_scale = fused.weight[:, off:off + pr.in_features], fused.int8_scale * self.out_scales[i]
                     off += pr.in_features
                 pr.colscale = None
-        for m in self.mixers:
-            m.to_int8()                                     # (what is integers already stays so)
-        if self.ffn is not None:
-            self.ffn.to_int8()
+        # (what is integers already stays so)
+        return sum(m.to_int8() for m in self.mixers) + (self.ffn.to_int8() if self.ffn is not None else 0)
 
     def _make_sides(self, device) -> None:
         if not hasattr(self, "_side"):

@@ -67,7 +67,7 @@ class SwiGLU(Part):
             if self.gate_up.colbias is not None:
                 self.gate_up.colbias = self.gate_up.colbias[idx].contiguous()
 
-    def to_int8(self) -> None:
+    def to_int8(self) -> int:
         if self.interleaved and self.gate_up.weight.dtype == torch.bfloat16:
             # the 8-bit product takes the gate's rows, then the up projection's, as they are stored
             F = self.F
@@ -77,8 +77,7 @@ class SwiGLU(Part):
                 if v is not None:
                     setattr(self.gate_up, name, v[idx].contiguous())
             self.interleaved = False
-        self.gate_up.to_int8()
-        self.down.to_int8()
+        return self.gate_up.to_int8() + self.down.to_int8()
 
     @property
     def takes_int8(self) -> bool:
@@ -288,14 +287,13 @@ class MoEFeedForward(Part):
         if self.shared is not None:
             self.shared.bind(tensors, dtype, device)
 
-    def to_int8(self) -> None:
+    def to_int8(self) -> int:
         """The experts' weights and the shared expert's; the router stays in its own type."""
         if self.w_gate_up.dtype == torch.bfloat16:
             self.w_gate_up, self.gate_up_scale = ops.weight_int8(self.w_gate_up)
             self.w_down, self.down_scale = ops.weight_int8(self.w_down)
             self.expert_tables = None
-        if self.shared is not None:
-            self.shared.to_int8()
+        return (2 if self.gate_up_scale is not None else 0) + (self.shared.to_int8() if self.shared is not None else 0)
 
     takes_stream = True        # forward(..., stream=x32): an expert that returns its input returns the 32-bit rows
 

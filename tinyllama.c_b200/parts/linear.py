@@ -145,14 +145,15 @@ class StackedLinear(Editable):
     def repeats(self):
         return frozenset(("segments",))
 
-    def to_int8(self) -> None:
+    def to_int8(self) -> int:
         """From here on the weight is integers [out, in] in 8 bits with a scale per output channel (int8_scale, the column
-        scale in it) and forward() rounds its rows.  A matrix that is kept in 32 bits stays as it is."""
-        if self.weight.dtype != torch.bfloat16:
-            return
-        self.weight, self.int8_scale = ops.weight_int8(self.weight)
-        if self.colscale is not None:
-            self.int8_scale, self.colscale = self.int8_scale * self.colscale, None
+        scale in it) and forward() rounds its rows.  A matrix that is kept in 32 bits stays as it is.  Returns how many matrices (1 or
+        0) are integers now."""
+        if self.weight.dtype == torch.bfloat16:
+            self.weight, self.int8_scale = ops.weight_int8(self.weight)
+            if self.colscale is not None:
+                self.int8_scale, self.colscale = self.int8_scale * self.colscale, None
+        return 1 if self.int8_scale is not None else 0
 
     def forward(self, x, out: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
         """x: rows [T, in]; for weights in 8 bits also (integers, scales) of rows that are rounded already."""
