@@ -4,7 +4,9 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from tinyllama_c_b200 import ops
 from tinyllama_c_b200.engine.decode_graph import DecodeGraph
+from tinyllama_c_b200.parts.feed_forward import MoEFeedForward
 from tinyllama_c_b200.weights import load_model
 
 import configs
@@ -39,3 +41,22 @@ def test_a_model_stored_in_32_bits_is_refused(tmp_path):
     model = load_model(folder, "bfloat16", "cpu")
     with pytest.raises(ValueError, match="32 bits"):
         model.to_int8()
+
+
+def test_experts_are_converted_as_a_whole_or_not_at_all(monkeypatch):
+    """The second of an expert's two tables may find no memory; the layer then still runs as it was, and can be asked again."""
+    moe = MoEFeedForward(64, 3, 2, 40, "router", dict(gate="e{e}.g", up="e{e}.u", down="e{e}.d"))
+    moe.bind({s.name: torch.ones(s.shape, dtype=torch.bfloat16) for s in moe.weight_specs()}, torch.bfloat16, "cpu")
+    calls = []
+
+    def weight_int8(w):
+        calls.append(w)
+        if len(calls) == 2:
+            raise torch.OutOfMemoryError("no room")
+        return w.to(torch.int8), w.float()[..., 0]
+
+    monkeypatch.setattr(ops, "weight_int8", weight_int8)
+    with pytest.raises(torch.OutOfMemoryError):
+        moe.to_int8()
+    assert moe.w_gate_up.dtype == moe.w_down.dtype == torch.bfloat16 and moe.gate_up_scale is None and moe.down_scale is None
+    assert moe.to_int8() == 2 and moe.w_gate_up.dtype == moe.w_down.dtype == torch.int8

@@ -290,8 +290,8 @@ class MoEFeedForward(Part):
     def to_int8(self) -> int:
         """The experts' weights and the shared expert's; the router stays in its own type."""
         if self.w_gate_up.dtype == torch.bfloat16:
-            self.w_gate_up, self.gate_up_scale = ops.weight_int8(self.w_gate_up)
-            self.w_down, self.down_scale = ops.weight_int8(self.w_down)
+            both = ops.weight_int8(self.w_gate_up), ops.weight_int8(self.w_down)      # (both or, out of memory, neither)
+            (self.w_gate_up, self.gate_up_scale), (self.w_down, self.down_scale) = both
             self.expert_tables = None
         return (2 if self.gate_up_scale is not None else 0) + (self.shared.to_int8() if self.shared is not None else 0)
 
