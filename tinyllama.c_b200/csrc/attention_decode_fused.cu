@@ -468,7 +468,7 @@ cudaError_t launch_fused(dim3 grid, int passes, cudaStream_t stream, Args... arg
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_tlc_pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, attention_decode_fused_kernel<HD, CK, STAGES, CLUSTER>, args...);
+  return tlc_launch_config(cfg, attention_decode_fused_kernel<HD, CK, STAGES, CLUSTER>, args...);
 }
 
 }  // namespace

@@ -7,6 +7,7 @@
 
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
+#include <atomic>
 #include <stdint.h>
 #include <stdio.h>
 
@@ -52,6 +53,15 @@ template <typename... P> __device__ __forceinline__ void tlc_pdl(P&... ptrs) {
   tlc_wait(ptrs...);
 }
 
+// Every launch of the library goes through here and is counted (tlc_launches).
+inline std::atomic<long long> g_tlc_launches{0};
+template <typename... KArgs, typename... Args>
+inline cudaError_t tlc_launch_config(const cudaLaunchConfig_t& cfg, void (*kernel)(KArgs...), Args&&... args) {
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  if (e == cudaSuccess) g_tlc_launches.fetch_add(1, std::memory_order_relaxed);
+  return e;
+}
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t tlc_launch_as(bool programmatic, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
                                  cudaStream_t stream, Args&&... args) {
@@ -65,7 +75,7 @@ inline cudaError_t tlc_launch_as(bool programmatic, void (*kernel)(KArgs...), di
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (programmatic && g_tlc_pdl) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  return tlc_launch_config(cfg, kernel, static_cast<Args&&>(args)...);
 }
 
 template <typename... KArgs, typename... Args>

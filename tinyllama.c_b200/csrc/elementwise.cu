@@ -9,6 +9,7 @@
 
 int g_tlc_pdl = 0;
 extern "C" void tlc_set_pdl(int on) { g_tlc_pdl = on; }
+extern "C" long long tlc_launches() { return g_tlc_launches; }
 
 static thread_local char g_err[512];
 extern "C" const char* tlc_last_error() { return g_err; }

@@ -275,7 +275,7 @@ int launch(const Int8Args& p, int token_tiles, int split, cudaStream_t stream) {
   }
   cfg.attrs = attr;
   cfg.numAttrs = na;
-  cudaLaunchKernelEx(&cfg, int8_few_kernel<TO, NB, GLU, GROUPED>, mw, mx, p, split, n_tiles, tlc_error_words());
+  tlc_launch_config(cfg, int8_few_kernel<TO, NB, GLU, GROUPED>, mw, mx, p, split, n_tiles, tlc_error_words());
   TLC_CHECK_LAUNCH("linear_int8 (few rows)");
   return 0;
 }

@@ -331,7 +331,7 @@ int launch(const Int8Args& p, long long tiles, int n_tiles, int pairs, cudaStrea
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_tlc_pdl ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, int8_wide_kernel<TO, NB, GLU, GROUPED>, mw, mx, p, n_tiles, tlc_error_words());
+  tlc_launch_config(cfg, int8_wide_kernel<TO, NB, GLU, GROUPED>, mw, mx, p, n_tiles, tlc_error_words());
   TLC_CHECK_LAUNCH("linear_int8 (pairs)");
   return 0;
 }

@@ -545,7 +545,7 @@ static void launch_split_f32x4(const float* a, int lda, const float* w, int ldw,
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, gemm_split_f32x4_kernel<TO, TM, NC, KS>, a, lda, w, ldw, out, ldo, colscale, colbias, accumulate, M, N, K, split);
+  tlc_launch_config(cfg, gemm_split_f32x4_kernel<TO, TM, NC, KS>, a, lda, w, ldw, out, ldo, colscale, colbias, accumulate, M, N, K, split);
 }
 
 // Which tiles 17 and more rows take, by how much work lands on the fullest SM (so the order of a sum follows from the sizes and
@@ -1175,9 +1175,9 @@ static void launch_skinny_mg(const __nv_bfloat16* a, int lda, const __nv_bfloat1
       cfg.numAttrs = g_tlc_pdl ? 2 : 1;
       const int half = (n_steps + 1) / 2;
       if (half <= SK_WARPS * 2 || MG == 2)
-        cudaLaunchKernelEx(&cfg, gemm_skinny_mma_kernel<TO, MG, 2, false, true>, a, lda, w, ldw, out, ldo, colscale, colbias, accumulate, M, N, K);
+        tlc_launch_config(cfg, gemm_skinny_mma_kernel<TO, MG, 2, false, true>, a, lda, w, ldw, out, ldo, colscale, colbias, accumulate, M, N, K);
       else
-        cudaLaunchKernelEx(&cfg, gemm_skinny_mma_kernel<TO, MG, 4, false, true>, a, lda, w, ldw, out, ldo, colscale, colbias, accumulate, M, N, K);
+        tlc_launch_config(cfg, gemm_skinny_mma_kernel<TO, MG, 4, false, true>, a, lda, w, ldw, out, ldo, colscale, colbias, accumulate, M, N, K);
       return;
     }
   }
@@ -1206,7 +1206,7 @@ static void launch_skinny_mg(const __nv_bfloat16* a, int lda, const __nv_bfloat1
       cudaLaunchAttribute attr[2];
       cudaLaunchConfig_t cfg = ring_config(blocks, attr);
       cfg.stream = stream;
-      cudaLaunchKernelEx(&cfg, gemm_skinny_ring_kernel<TO>, a, lda, w, ldw, out, ldo, colscale, colbias, accumulate, M, N, K);
+      tlc_launch_config(cfg, gemm_skinny_ring_kernel<TO>, a, lda, w, ldw, out, ldo, colscale, colbias, accumulate, M, N, K);
       return;
     }
   }

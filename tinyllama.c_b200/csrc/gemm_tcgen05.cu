@@ -745,7 +745,7 @@ int launch_pairs(const CUtensorMap& ma, const CUtensorMap& mb, void* out, int ld
   int tma_out = 0;
   if (std::is_same<TO, float>::value && !SWIGLU)
     if (int rc = get_out_map(out, M, N, ldo, ma, &mo, &tma_out)) return rc;
-  cudaLaunchKernelEx(&cfg, gemm_tcgen05_kernel<TO, PAIR_BN, PAIR_STAGES, SWIGLU, true>, ma, mb, (TO*)out, ldo, colscale, colbias,
+  tlc_launch_config(cfg, gemm_tcgen05_kernel<TO, PAIR_BN, PAIR_STAGES, SWIGLU, true>, ma, mb, (TO*)out, ldo, colscale, colbias,
                      accumulate, M, N, K, g_err_dev, 1, (float*)nullptr, (unsigned*)nullptr, mo, tma_out);
   TLC_CHECK_LAUNCH("linear(tcgen05, pairs)");
   return 0;

@@ -339,7 +339,7 @@ int launch_few(const CUtensorMap& mw, const CUtensorMap& mx, void* out, int ldo,
   }
   cfg.attrs = attr;
   cfg.numAttrs = na;
-  cudaLaunchKernelEx(&cfg, gemm_few_rows_kernel<TO, NB, STAGES, SWIGLU>, mw, mx, (TO*)out, ldo, colscale, colbias, accumulate, M, N,
+  tlc_launch_config(cfg, gemm_few_rows_kernel<TO, NB, STAGES, SWIGLU>, mw, mx, (TO*)out, ldo, colscale, colbias, accumulate, M, N,
                      K, split, tlc_error_words());
   TLC_CHECK_LAUNCH("linear(few rows)");
   return 0;

@@ -48,6 +48,8 @@ const char* tlc_last_error(void);
  * predecessor drains); 0: plain stream order.  The embedding kernel never carries it: it is the boundary
  * between steps (see tlc_embed). */
 void tlc_set_pdl(int on);
+/* How many kernels the library has launched so far, captured ones included. */
+long long tlc_launches(void);
 /* Calls made again from a table: `times` rounds of n_calls calls, the functions of a round by their index
  * (tlc_replay_index: -1 for a function that is not among those that can be) and the arguments of all rounds one after the other
  * as 64-bit words (pointers and integers by value, floats by their bits; n_words in all; both arrays host).  Stops at the

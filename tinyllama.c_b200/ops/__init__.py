@@ -35,6 +35,7 @@ _vp, _i, _f, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longl
 _SIGNATURES = {
     "tlc_last_error": (ctypes.c_char_p, []),
     "tlc_set_pdl": (None, [_i]),
+    "tlc_launches": (_ll, []),
     "tlc_replay_index": (_i, [ctypes.c_char_p]),
     "tlc_call": (_i, [_i, ctypes.c_char_p]),
     "tlc_replay": (_i, [_vp, _vp, _ll, _i, _i]),
@@ -203,9 +204,9 @@ _launches = 0
 
 
 def launch_count() -> int:
-    """How many kernel-launching library calls were made (captured calls count once at capture;
-    a graph replay adds its calls through count_launches)."""
-    return _launches
+    """How many kernels of the library were launched (captured ones count once at capture; a graph replay adds its
+    kernels through count_launches)."""
+    return _launches + (_lib.tlc_launches() if _lib is not None else 0)
 
 
 def count_launches(n: int) -> None:
@@ -214,9 +215,7 @@ def count_launches(n: int) -> None:
 
 
 def _call(name: str, *args) -> None:
-    global _launches
     lib = library()
-    _launches += 1
     rc = getattr(lib, name)(*args)
     if rc != 0:
         raise KernelError(f"{name}: {lib.tlc_last_error().decode()}")
@@ -243,7 +242,6 @@ _packs: dict = {}
 
 def _call_packed(name: str, *args, ok: int = 0) -> bool:
     """_call() for a function of the library's table, its arguments plain numbers (0 for no pointer)."""
-    global _launches
     hit = _packs.get(name)
     if hit is None:
         lib = library()
@@ -261,7 +259,6 @@ def _call_packed(name: str, *args, ok: int = 0) -> bool:
         if ok and rc == ok:
             return False
         raise KernelError(f"{name}: {lib.tlc_last_error().decode()}")
-    _launches += 1
     notes = _notes.calls
     if notes is not None:
         notes.add(name, args)
@@ -349,17 +346,10 @@ def cannot_repeat() -> None:
 
 def replay(functions, words, times: int) -> None:
     """Makes the calls of `functions` (int32 array of indices) `times` times; words: the arguments of all rounds (uint64 array)."""
-    global _launches
     lib = library()
     rc = lib.tlc_replay(functions.ctypes.data, words.ctypes.data, words.size, functions.size, int(times))
     if rc != 0:
         raise KernelError(f"tlc_replay: {lib.tlc_last_error().decode()}")
-    _launches += int(times) * int((functions >= _event_functions()).sum())
-
-
-def _event_functions() -> int:
-    """The first entries of the library's table are the events, which launch nothing."""
-    return max(_replayable("tlc_event_record")[0], _replayable("tlc_event_wait")[0]) + 1
 
 
 def record_event(event: "torch.cuda.Event", stream: "torch.cuda.Stream") -> None:
@@ -799,15 +789,12 @@ def linear_swiglu(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, colscale:
         raise KernelError(f"linear_swiglu: shapes a{tuple(a.shape)} w{tuple(w.shape)} out{tuple(out.shape)} do not agree")
     _f32vec(colscale, N, "linear colscale")
     _f32vec(colbias, N, "linear colbias")
-    global _launches
     lib = library()
-    _launches += 1
     args = (a.data_ptr(), dtype_code(a.dtype), _rows(a, "linear input"), w.data_ptr(), dtype_code(w.dtype),
             _rows(w, "linear weight"), out.data_ptr(), dtype_code(out.dtype), N // 2, _p(colscale),
             _p(colbias), M, N, K, TENSOR_CORE_MIN_ROWS, DENSE_ACTS[act], float(limit), float(alpha), _stream())
     rc = lib.tlc_linear_swiglu(*args)
     if rc == 1:                                   # no fused kernel for these operands
-        _launches -= 1
         gu = torch.empty((M, N), dtype=torch.float32, device=a.device)
         _note_owned(gu)
         linear(a, w, gu, colscale, colbias)
@@ -1493,8 +1480,6 @@ def moe_route(logits: torch.Tensor, n_experts: int, top: int, tile_rows: int = 3
     ints = torch.empty(2 * T * top + 2 * (n_experts + 1), dtype=torch.int32, device=dev)
     ids, order, offsets, tile_off = ints.split_with_sizes((T * top, T * top, n_experts + 1, n_experts + 1))
     wts = torch.empty(T * top, dtype=torch.float32, device=dev)
-    global _launches
-    _launches += 1                      # (two kernels)
     _f32vec(choice_bias, n_experts, "moe_route choice bias")
     _gpu(choice_bias)
     _call_packed("tlc_moe_route", logits.data_ptr(), _rows(logits, "router logits"), T, int(n_experts), int(top), ROUTE_WEIGHTS[weights],
@@ -1850,14 +1835,11 @@ def qkv_prepare(proj: torch.Tensor, off: int, H: int, KV: int, hd: int, inv_freq
         if k_pages.dtype != q_out.dtype or v_pages.dtype != q_out.dtype or not q_out.is_contiguous() or tuple(q_out.shape) != (T, H * hd) \
                 or not k_pages.is_contiguous() or not v_pages.is_contiguous() or tuple(k_pages.shape[1:]) != (KV, PAGE, hd):
             raise KernelError("qkv_prepare: q_out [T, H*hd] and pages [n, KV, 64, hd] contiguous and of one type")
-    global _launches
     fresh, single = _all_fresh(step), int(step.max_new == 1)
     single_kernel = single and T == step.n_seqs
     sums = None
     if not single_kernel and q_weight is not None:
         sums = torch.empty((T, 2 * library().tlc_qkv_prepare_sums(H, KV, hd)), dtype=torch.float32, device=proj.device)
-    if not single_kernel:               # (the sums' kernel; the one that writes the kept rows)
-        _launches += int(sums is not None) + int(K > 1 and not fresh)
     _call("tlc_qkv_prepare", proj.data_ptr(), ld, int(off), _p(taps), K, _window(state, K, C, "qkv_prepare"), _p(q_weight), _p(k_weight),
           int(q_count or H * hd), int(k_count or KV * hd), float(eps), inv_freq.data_ptr(), 2 * inv_freq.numel(), float(amplitude),
           step.positions.data_ptr(), step.row_seq.data_ptr(), step.cu_seqlens.data_ptr(), step.slots.data_ptr(), step.start_pos.data_ptr(),
@@ -2149,8 +2131,6 @@ def retention_chunked(proj: torch.Tensor, q_off: int, k_off: int, v_off: int, g_
     _gpu(out, seg_start, seg_seq, seq_seg_start)
     n_seg, T = seg_seq.numel(), proj.shape[0]
     scratch = torch.empty(n_seg * H * (dk * dv + 1), dtype=torch.float32, device=proj.device)
-    global _launches
-    _launches += 2                      # (three kernels)
     _call("tlc_retention_chunked", proj.data_ptr(), ld, int(q_off), int(k_off), int(v_off), int(g_off), inv_freq.data_ptr(),
           2 * inv_freq.numel(), step.positions.data_ptr(), decay.data_ptr(), float(k_scale), float(eps), state.data_ptr(), scratch.data_ptr(),
           seg_start.data_ptr(), seg_seq.data_ptr(), seq_seg_start.data_ptr(), step.slots.data_ptr(), step.start_pos.data_ptr(), step.n_seqs,
