@@ -62,14 +62,25 @@ __device__ __forceinline__ void stage(const T* x, int ldx, const float*, int K, 
     const unsigned largest = __reduce_max_sync(0xffffffffu, red[m * WARPS + (lane & (WARPS - 1))]);
     const float s = int8_scale(largest, &some), inv = __frcp_rn(s);
     scale[m] = int8_told(largest, some, s);
-    for (int c = threadIdx.x; c < pieces; c += THREADS) {
-      uint2 n = make_uint2(0u, 0u);
-      if (some) {
+    int8_t* to = xs + (size_t)m * ld;
+    if (int8_usual(largest, s)) {
+      for (int c = threadIdx.x; c < pieces; c += THREADS) {
         float v[8];
         piece(m, c, v);
-        n = eight_nearest(v, s, inv);
+        *reinterpret_cast<uint2*>(to + 8 * c) = eight_nearest(v, s, inv);
       }
-      *reinterpret_cast<uint2*>(xs + (size_t)m * ld + 8 * c) = n;
+    } else {
+      for (int c = threadIdx.x; c < pieces; c += THREADS) {
+        uint2 n = make_uint2(0u, 0u);
+        if (some) {
+          float v[8];
+          piece(m, c, v);
+#pragma unroll
+          for (int i = 0; i < 8; i++) v[i] *= INT8_LIFT;
+          n = eight_nearest(v, s * INT8_LIFT, __frcp_rn(s * INT8_LIFT));
+        }
+        *reinterpret_cast<uint2*>(to + 8 * c) = n;
+      }
     }
   }
   __syncthreads();

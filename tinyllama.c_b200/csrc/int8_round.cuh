@@ -28,22 +28,13 @@ __device__ __forceinline__ float larger(float m, float v) {
 // mended by its remainder, which a fused multiply-add gives exactly, times inv (Markstein, IBM Journal of Research and Development 34,
 // 1990): the IEEE quotient, without the general division's cases, which do not arise here (s is no denormal and |v / s| <= 127).
 // The remainder of a quotient of 1/2 or more comes in steps of 2^-47 of s's power of two or more, so it is exact down to s = 2^-102; rows of
-// smaller scales are multiplied by 2^64 first, which changes no quotient.  Adding 1.5 * 2^23 rounds it to an integer and leaves that in the sum's low bits; conversions would go through the special-function
-// unit, at a quarter of the rate.
+// smaller scales come multiplied by 2^64 (int8_usual), which changes no quotient.  Adding 1.5 * 2^23 rounds it to an integer and
+// leaves that in the sum's low bits; conversions would go through the special-function unit, at a quarter of the rate.
 __device__ __forceinline__ uint2 eight_nearest(const float (&v)[8], float s, float inv) {
   uint32_t b[8];
-  float u[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) u[i] = v[i];
-  if (s < 7.8886091e-31f) {                 // 2^-100
-    s *= 18446744073709551616.0f;           // 2^64
-    inv *= 5.4210109e-20f;                  // 2^-64
-#pragma unroll
-    for (int i = 0; i < 8; i++) u[i] *= 18446744073709551616.0f;
-  }
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const float first = __fmul_rn(u[i], inv), quotient = __fmaf_rn(__fmaf_rn(-first, s, u[i]), inv, first);
+    const float first = __fmul_rn(v[i], inv), quotient = __fmaf_rn(__fmaf_rn(-first, s, v[i]), inv, first);
     b[i] = __float_as_uint(__fadd_rn(quotient, 12582912.0f));
   }
   return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
@@ -56,6 +47,10 @@ __device__ __forceinline__ float int8_scale(unsigned largest, bool* some) {
   *some = largest < 0x7f800000u && s >= 1.17549435e-38f;
   return s;
 }
+// Rows of numbers, not all zero, whose scale is 2^-100 or more.  Of a row with a smaller scale the quotients are taken of 2^64 times its
+// values and 2^64 times its scale, exactly (see eight_nearest).
+__device__ __forceinline__ bool int8_usual(unsigned largest, float s) { return largest < 0x7f800000u && s >= 7.8886091e-31f; }
+constexpr float INT8_LIFT = 18446744073709551616.0f;
 // ... as it is told: NaN where the row holds an infinity or a NaN.
 __device__ __forceinline__ float int8_told(unsigned largest, bool some, float s) {
   return largest >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : some ? s : 0.f;

@@ -96,13 +96,26 @@ int8_rows_kernel(const T* __restrict__ x, int ldx, int rows, int K, const float*
   }
   if (!there) return;
   bool some;
-  const float s = int8_scale(largest, &some), inv = __frcp_rn(s);
+  const float s = int8_scale(largest, &some);
   if (tid == 0) {
     const float r = NORM ? rsqrtf(sum / (float)K + eps) : 1.0f;
     const float told = int8_told(largest, some, s * r);
     for (int i = 0; i < copies; i++) scale[to(i)] = told;
   }
-  if constexpr (NI > 0) {
+  const bool usual = int8_usual(largest, s);
+  if (NI == 0 || !usual) {                                   // from memory again, a value at a time
+    const float lift = usual ? 1.0f : INT8_LIFT, lifted = s * lift, inv = __frcp_rn(lifted);
+    for (int c = tid; c < pieces; c += threads) {
+      float u[8], g[8] = {};
+      row8(xr, 8 * c, K, u);
+      if (NORM) row8(w, 8 * c, K, g);
+#pragma unroll
+      for (int i = 0; i < 8; i++) u[i] = (NORM ? u[i] * g[i] : u[i]) * lift;
+      const uint2 bytes = some ? eight_nearest(u, lifted, inv) : make_uint2(0u, 0u);
+      for (int i = 0; i < copies; i++) store8(PLACED ? q + (size_t)to(i) * ldq : qr, 8 * c, K, bytes);
+    }
+  } else if constexpr (NI > 0) {
+    const float inv = __frcp_rn(s);
     uint2 bytes[PLACED ? N : 1];
 #pragma unroll
     for (int j = 0; j < N; j++) {
@@ -116,7 +129,7 @@ int8_rows_kernel(const T* __restrict__ x, int ldx, int rows, int K, const float*
 #pragma unroll
         for (int i = 0; i < 8; i++) u[i] *= g[i];
       }
-      const uint2 b = some ? eight_nearest(u, s, inv) : make_uint2(0u, 0u);
+      const uint2 b = eight_nearest(u, s, inv);
       if constexpr (PLACED) bytes[j] = b;
       else *reinterpret_cast<uint2*>(qr + 8 * c) = b;
     }
@@ -130,18 +143,6 @@ int8_rows_kernel(const T* __restrict__ x, int ldx, int rows, int K, const float*
           if (c < pieces) *reinterpret_cast<uint2*>(o + 8 * c) = bytes[j];
         }
       }
-    }
-  } else {
-    for (int c = tid; c < pieces; c += threads) {
-      float u[8], g[8] = {};
-      row8(xr, 8 * c, K, u);
-      if (NORM) {
-        row8(w, 8 * c, K, g);
-#pragma unroll
-        for (int i = 0; i < 8; i++) u[i] *= g[i];
-      }
-      const uint2 bytes = some ? eight_nearest(u, s, inv) : make_uint2(0u, 0u);
-      for (int i = 0; i < copies; i++) store8(PLACED ? q + (size_t)to(i) * ldq : qr, 8 * c, K, bytes);
     }
   }
 }
