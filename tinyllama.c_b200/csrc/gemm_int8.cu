@@ -11,6 +11,11 @@
 //                        8): CUDA cores (dp4a: four products and their sum an instruction), tiles of 32 x 64 results staged
 //                        through shared memory 64 values of K at a time.  2,048 rows of 2,048 -> 8,240 956 us, 72 TOP/s, bound by
 //                        shared memory (three reads for eight dp4a); the tensor cores take 31.
+//
+// Results added to what is there, as a model's projections back into the 32-bit stream are, cost little in the kernels of few rows
+// and much in the pairs' (the old values of a piece are asked for when its sums are there).  Microseconds added, and written in 32 bits:
+// 12 x 4,096 -> 2,048 3.3, 3.1; 64 rows 6.4, 6.3; 512 rows 12.7, 11.0; 2,048 rows 27.2, 17.1; 2,048 x 8,192 -> 2,560 56.8, 45.2; 8,192 rows 146,
+// 134; 2,048 x 2,048 -> 8,240 82.6, 32.9.
 #include "gemm_int8_tc.cuh"
 #include <algorithm>
 #include <atomic>
@@ -136,7 +141,7 @@ bool tensor_cores_take(const Int8Args& p) {
          tlc_error_words_here() != nullptr;
 }
 
-int sm_count() {
+int sm_count() {                     // (of the device that is asked first: it sizes grids, no more)
   static std::atomic<int> sms{0};
   if (sms == 0) {
     int dev = 0, n = 0;
@@ -225,7 +230,7 @@ extern "C" int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_sca
   // 8,240 3.7, 4.5; 4,096 -> 2,048 3.0, 3.5; 2,048 -> 2 x 4,096 3.4, 4.6; 8,192 -> 2,560 7.4, 7.5; 2,560 -> 10,240 8.2, 6.8.  Integers
   // behind the norm that makes them, both: 2,048 -> 8,240 4.5, 4.8; gated 4.5, 5.0.  Two rows that are to be rounded, up to K = 2,048: 2,048
   // -> 2,048 2.9, 3.1, -> 8,240 4.5, 4.5, and a launch less for the host (4,096 -> 2,048 4.6, 3.7; three rows 6.8, 4.6).
-  const bool takes = (M == 1 ? K <= TLC_INT8_SKINNY : M == 2 && a_dtype != TLC_I8 && K <= TLC_INT8_SKINNY / 4) && ((uintptr_t)w | (uintptr_t)ldw) % 16 == 0;
+  const bool takes = (M == 1 ? K <= TLC_INT8_SKINNY : M == 2 && a_dtype != TLC_I8 && K <= TLC_INT8_TWO) && ((uintptr_t)w | (uintptr_t)ldw) % 16 == 0;
   if (takes && (g_kernel == 4 || (g_kernel == 0 && (long long)p.w_rows * K <= 24 << 20))) return tlc_int8_skinny(a, a_dtype, p, out_dtype, sm_count(), stream);
   if (a_dtype != TLC_I8) {
     if (!a_int8 || !a_scale) return 1;                     // (room is wanted)

@@ -19,7 +19,8 @@ struct Int8Args {
   int E;
   int scatter, w_out;                   // result rows go where order says, times the pair's weight
 };
-constexpr int TLC_INT8_SKINNY = 8192;     // values of the row in the kernel of one or two rows, at most
+constexpr int TLC_INT8_SKINNY = 8192;     // values of one row, at most, in the kernel of one or two rows
+constexpr int TLC_INT8_TWO = 2048;        // ... of each of two (ops.linear_int8 brings room for longer ones at once)
 constexpr int TLC_INT8_THIN = 4096;       // values of a row in the kernel of up to 16 rows, at most: 256 for each of 16 warps
 constexpr int TLC_INT8_GROUPS = 4096;     // at most (as a routing)
 enum { I8_PLAIN = 0, I8_ADD = 1, I8_ACT = 2, I8_GLU = 3 };
@@ -47,8 +48,10 @@ __device__ __forceinline__ float int8_value(int sum, float row_scale, float col_
 }
 
 // A gated activation as all kernels here make it; w: the pair's weight on gate and up, where it goes there.  SiLU is g / (1 + 2^(-g log2 e)) by
-// the special-function unit's power and reciprocal (a few units in the last place of 32 bits), written out because the general
-// forms also mend results below 2^-126, which nothing here needs.
+// the special-function unit's power and reciprocal.  The product g log2 e is rounded before the power, so the error of the result grows
+// with |g| where g is negative: (4 + 1.2 |g|) 2^-24 of it at most, measured (9 at g = -10, 63 at -80), 4 where g is positive.  From
+// g = -87.4 down (results of 1e-36) it is 0.  A result in 16 bits is rounded to 2^-8 after that; the 32-bit paths elsewhere (silu_f) keep
+// the slower form.
 __device__ __forceinline__ float int8_silu(float g, float u) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));

@@ -5,11 +5,15 @@
 //
 // The norm's factor r = 1 / sqrt(mean + eps) is the same for a whole row and cancels in v / s, so the integers are those of
 // p = x w and only the scale is multiplied by r: the row's sum of squares and its largest |p| come from one trip through the
-// row's warps, and a row is read once (up to 16,384 values stay in registers).
+// row's warps, and a row is read once (up to 24,576 values stay in registers).
 //
-// Few rows: as many threads a row as it has pieces of eight values, for the shortest way through (1 x 2,048 1.4 us).  Rows that fill the
-// GPU: several pieces a thread and several rows a block, so that enough loads are on their way: 8,192 x 2,560 bfloat16 values 12.3 us
-// (63 MB, 5.1 TB/s), 16,384 x 1,024 float values 12.6 us (6.7 TB/s); a block a row took 27.5 and 18.6.
+// Few rows: as many threads a row as it has pieces of eight values, for the shortest way through (1 x 2,048 1.3 us).  Rows that fill the
+// GPU: several pieces a thread and several rows a block, so that enough loads are on their way: 8,192 x 2,560 bfloat16 values 12.5 us
+// (63 MB, 5.0 TB/s), 16,384 x 1,024 float values 12.6 us (6.7 TB/s); a block a row took 27.5 and 18.6.
+//
+// Rows that do not come in whole pieces on 16-byte boundaries are read value by value, and a second time for their integers: 1 x 2,043 1.9 us,
+// 24 x 8,187 3.7, 333 x 2,555 floats 5.2 (2.4 in pieces), 8,192 x 2,555 32, 16,384 x 1,019 floats 44.  So is a row of zeros, of an infinity or
+// a NaN, or of the smallest scales (int8_usual).
 //
 // The largest magnitude is a maximum of bit patterns without their sign: an infinity or a NaN is larger than every number there,
 // and a row that holds one gets the scale NaN and zeros, so that whatever is multiplied by it is NaN.  A row of zeros (or of values

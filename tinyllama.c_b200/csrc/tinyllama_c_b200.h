@@ -431,7 +431,8 @@ int tlc_rows_int8(const void* x, int x_dtype, int ldx, int T, int K, const float
 /* out[m, n] (+)= a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + colbias[n]: a [M, lda] int8 (a_dtype TLC_I8, a_scale [M] given), or
  * float or bfloat16 rows, which are rounded first (a_int8 [M, ld_int8] and a_scale [M] are then scratch; without it, NULL, the
  * call returns 1 and does nothing where it needs it).  w [N, ldw] int8,
- * w_scale [N], colbias [N] or NULL, out float or bfloat16; K at most 131071 (the sums are exact 32-bit integers).
+ * w_scale [N], colbias [N] or NULL (all three are fetched while the kernel before the product may still run: none may be what a kernel
+ * writes that was launched on the stream since the last step boundary), out float or bfloat16; K at most 131071 (the sums are exact 32-bit integers).
  * act >= 0 (TLC_ACT_SILU, TLC_ACT_GELU_TANH, TLC_ACT_SWISH_CLAMPED): gated, w has 2 N rows (N gate rows, then N up rows; w_scale,
  * colbias [2 N]) and out[m, n] = act(y[m, n]) * y[m, N + n], or the clamped swish's form with limit and alpha; no accumulate. */
 int tlc_linear_int8(const void* a, int a_dtype, int lda, float* a_scale, void* a_int8, int ld_int8, const void* w, int ldw,

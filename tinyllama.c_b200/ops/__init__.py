@@ -1581,6 +1581,7 @@ def moe_identity(x: torch.Tensor, routing, top: int, n_experts: int, y: torch.Te
 # functions here make them (int8_empty), which the tensor-core kernels need; operands in any other layout are multiplied on the CUDA
 # cores.
 INT8_MAX_K = 131071                      # 128 * 128 * K < 2^31: the sums of products stay exact in 32 bits
+INT8_TWO = 2048                          # values of each of two rows that are rounded where they are multiplied (TLC_INT8_TWO in gemm_int8.cuh)
 
 
 def linear_int8_kernel(kernel: int = 0, rows: int = 0) -> None:
@@ -1687,7 +1688,7 @@ def _linear_int8(what, a, a_scale, w, w_scale, colbias, out, N, accumulate, act,
             raise KernelError(f"{what}: a_scale belongs to integer rows; a is {a.dtype}")
         code, ldq = dtype_code(a.dtype), (K + 15) // 16 * 16
         scale = q = 0
-        if M > 2 or (M == 2 and K > 2048):                 # (one or two rows mostly go without; the library says so where not)
+        if M > 2 or (M == 2 and K > INT8_TWO):             # (one or two rows mostly go without; the library says so where not)
             scale, q = _int8_room(M, ldq, a.device)
     args = (w.data_ptr(), ldw, w_scale.data_ptr(), out.data_ptr(), dtype_code(out.dtype), ldo, bias, accumulate, M, N, K, act, limit, alpha, _stream())
     if not _call_packed("tlc_linear_int8", a.data_ptr(), code, lda, scale, q, ldq, *args, ok=1):
@@ -1709,15 +1710,15 @@ def linear_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: to
 
     w int8 [N, K] and w_scale float32 [N] as weight_int8 makes them; a int8 [M, K] with a_scale float32 [M] (rows_int8,
     rmsnorm_int8), or float32 or bfloat16 rows, which are rounded that way first.  out [M, N] float32 or bfloat16; a, w and out may
-    be row-strided views.  w is fetched while the kernel before may still run: it must not be the output of a kernel of the same
-    step (weight_int8 sees to that)."""
+    be row-strided views.  w, w_scale and colbias are fetched while the kernel before may still run: none may be the output of a
+    kernel of this library in the same step (weight_int8 sees to that for what it makes)."""
     _linear_int8("linear_int8", a, a_scale, w, w_scale, colbias, out, w.shape[0], 1 if accumulate else 0, -1, 0.0, 1.0)
 
 
 def linear_swiglu_int8(a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: torch.Tensor, a_scale: Optional[torch.Tensor] = None,
                        colbias: Optional[torch.Tensor] = None, act: str = "silu", limit: float = 0.0, alpha: float = 1.0) -> None:
     """out[m, f] = act(gate) * up with gate = y[m, f] and up = y[m, F + f] of the product y that linear_int8 makes with w [2F, K] (the
-    gate's rows, then the up projection's; not interleaved); act, limit and alpha as in glu()."""
+    gate's rows, then the up projection's; not interleaved); act, limit and alpha as in glu(); w, w_scale and colbias as there."""
     if act not in DENSE_ACTS:
         raise KernelError(f"linear_swiglu_int8: unknown activation '{act}'; known: {sorted(DENSE_ACTS)}")
     if w.shape[0] % 2:
