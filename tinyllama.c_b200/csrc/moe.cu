@@ -28,7 +28,6 @@ __device__ __forceinline__ void moe_topk(const float* __restrict__ logits, int l
   const float* lr = logits + (size_t)t * ld;
   float last = INFINITY, first = 0.f, sum = 0.f;
   int last_e = -1, my_id = 0;
-  float my_w = 0.f;
   // TLC_ROUTE_SOFTMAX_ALL: scores are the softmax over all E outputs; an expert is chosen by score + choice_bias[e] and
   // weighted by the score alone
   float all_max = 0.f, all_inv = 1.0f;
@@ -61,34 +60,35 @@ __device__ __forceinline__ void moe_topk(const float* __restrict__ logits, int l
       if (take) { best = ov; be = oe; }
     }
     if (be == 0x7fffffff) be = 0;            // (NaN logits: no order; keep indices valid)
-    float w;                                 // (the same in every lane; lane k keeps choice k)
-    if (mode == TLC_ROUTE_SOFTMAX) {         // the first choice has the largest logit: numerators exp(z_k - z_0)
-      if (k == 0) first = lr[be];
-      w = expf(lr[be] - first);
-      sum += w;
-    } else if (mode == TLC_ROUTE_SOFTMAX_ALL) {
-      w = __fmul_rn(expf(lr[be] - all_max), all_inv);
-      sum += w;
-    } else {
-      w = 1.0f / (1.0f + expf(-lr[be]));
-    }
-    if (lane == (k & 31)) {
-      if (k < 32) { my_id = be; my_w = w; }
-      else { ids[t * top + k] = be; wts[t * top + k] = w; }
-    }
     last = best;                             // (the value the comparison saw, not one computed anew: the same bits)
     last_e = be;
+    if (lane == (k & 31)) my_id = be;
+    if ((k & 31) < 31 && k + 1 < top) continue;
+    // the choices of 32 passes, one a lane, are weighed together
+    const int n = (k & 31) + 1;
+    const float z = lr[my_id];
+    float w;
+    if (mode == TLC_ROUTE_SOFTMAX) {         // the first choice has the largest logit: numerators exp(z_k - z_0)
+      if (k < 32) first = __shfl_sync(0xffffffffu, z, 0);
+      w = expf(z - first);
+    } else if (mode == TLC_ROUTE_SOFTMAX_ALL) {
+      w = __fmul_rn(expf(z - all_max), all_inv);
+    } else {
+      w = 1.0f / (1.0f + expf(-z));
+    }
+    if (mode != TLC_ROUTE_SIGMOID)
+      for (int i = 0; i < n; i++) sum += __shfl_sync(0xffffffffu, w, i);      // (in the order of the choices)
+    if (lane < n) {
+      ids[t * top + k + 1 - n + lane] = my_id;
+      wts[t * top + k + 1 - n + lane] = w;
+    }
   }
   // softmax: the numerators divided by their sum; all scores: divided by the chosen ones' sum (+ 1e-20, which keeps a sum of zero
   // finite) and multiplied by sum_to
   const bool normed = mode == TLC_ROUTE_SOFTMAX_ALL && sum_to > 0.f;
   const float inv = normed ? 1.0f / (sum + 1e-20f) : 1.0f / sum;
-  auto final_of = [&](float w) { return normed ? w * inv * sum_to : mode == TLC_ROUTE_SOFTMAX ? w * inv : w; };
-  if (lane < top) {
-    ids[t * top + lane] = my_id;
-    wts[t * top + lane] = final_of(my_w);
-  }
-  for (int k = 32 + lane; k < top; k += 32) wts[t * top + k] = final_of(wts[t * top + k]);
+  if (!normed && mode != TLC_ROUTE_SOFTMAX) return;
+  for (int k = lane; k < top; k += 32) wts[t * top + k] = normed ? wts[t * top + k] * inv * sum_to : wts[t * top + k] * inv;
 }
 
 __global__ void __launch_bounds__(128)
@@ -111,22 +111,32 @@ __device__ __forceinline__ void moe_sort_pairs(const int* ids, int n_pairs, int 
   // Up to 16 pairs a thread are counted once: what the counter said is the pair's place among its expert's.  Fetched together.
   constexpr int MINE = 16;
   const bool once = n_pairs <= MINE * (int)blockDim.x;
-  int mine[MINE], rank[MINE];
+  int mine[MINE];                                              // the expert (of 4096 at most) and, above it, that place
   if (once) {
 #pragma unroll
-    for (int j = 0; j < MINE; j++) mine[j] = threadIdx.x + j * blockDim.x < n_pairs ? ids[threadIdx.x + j * blockDim.x] : -1;
+    for (int j = 0; j < MINE; j++) {
+      if (j * (int)blockDim.x >= n_pairs) break;               // (the block is through)
+      mine[j] = threadIdx.x + j * blockDim.x < n_pairs ? ids[threadIdx.x + j * blockDim.x] : -1;
+    }
 #pragma unroll
-    for (int j = 0; j < MINE; j++) rank[j] = mine[j] >= 0 ? atomicAdd(&count[mine[j]], 1) : 0;
+    for (int j = 0; j < MINE; j++) {
+      if (j * (int)blockDim.x >= n_pairs) break;
+      if (mine[j] >= 0) mine[j] |= atomicAdd(&count[mine[j]], 1) << 12;
+    }
   } else {
     for (int i = threadIdx.x; i < n_pairs; i += blockDim.x) atomicAdd(&count[ids[i]], 1);
   }
   __syncthreads();
-  if (threadIdx.x < 32) {      // running sums of pairs and tiles, 32 experts at a time
+  // tiles of every expert, where its cursor goes (the others have no weights: no product visits them)
+  for (int e = threadIdx.x; e < E; e += blockDim.x) cursor[e] = e < E_tiled ? (count[e] + tm - 1) / tm : 0;
+  __syncthreads();
+  if (threadIdx.x < 32) {      // running sums of pairs and tiles, 32 experts at a time, the next ones asked for ahead of the sums
     const int lane = threadIdx.x;
-    int pairs = 0, tiles = 0;
+    int pairs = 0, tiles = 0, next_c = lane < E ? count[lane] : 0, next_k = lane < E ? cursor[lane] : 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + lane, c = e < E ? count[e] : 0;
-      const int k = e < E_tiled ? (c + tm - 1) / tm : 0;       // (the others have no weights: no product visits them)
+      const int e = e0 + lane, c = next_c, k = next_k;
+      next_c = e + 32 < E ? count[e + 32] : 0;
+      next_k = e + 32 < E ? cursor[e + 32] : 0;
       int ci = c, ki = k;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -148,7 +158,10 @@ __device__ __forceinline__ void moe_sort_pairs(const int* ids, int n_pairs, int 
   __syncthreads();
   if (once) {
 #pragma unroll
-    for (int j = 0; j < MINE; j++) if (mine[j] >= 0) order[cursor[mine[j]] + rank[j]] = threadIdx.x + j * blockDim.x;
+    for (int j = 0; j < MINE; j++) {
+      if (j * (int)blockDim.x >= n_pairs) break;
+      if (mine[j] >= 0) order[cursor[mine[j] & 4095] + (mine[j] >> 12)] = threadIdx.x + j * blockDim.x;
+    }
   } else {
     for (int i = threadIdx.x; i < n_pairs; i += blockDim.x) order[atomicAdd(&cursor[ids[i]], 1)] = i;
   }
