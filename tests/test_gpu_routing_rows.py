@@ -1,4 +1,4 @@
-"""Routing of few rows (one launch up to 8 rows, two from 9 on) and of more choices than a warp has lanes, all weightings, against the
+"""Routing of few rows (one launch up to 8 rows and 128 experts, else two) and of more choices than a warp has lanes, all weightings, against the
 definition in 64 bits.
 
 The weights' allowance, u = 2^-24: an exponential's argument is a difference of two logits of at most 6 each (12u), the exponential itself
@@ -91,3 +91,12 @@ def test_one_launch_and_two_choose_and_weigh_alike(n, top, weights, sum_to):
         assert torch.equal(torch.cat([p[1] for p in parts]).nan_to_num(9.0), wts.nan_to_num(9.0))
     if weights == "sigmoid":
         assert (ids.view(20, top)[5].cpu() == torch.arange(top)).all()
+
+
+@pytest.mark.parametrize("T,n,launches", [(1, 32, 1), (8, 128, 1), (9, 32, 2), (4, 4096, 2), (8, 129, 2)])
+def test_many_experts_are_chosen_from_in_a_launch_of_its_own(T, n, launches):
+    """Beside the lists' shared memory the rows of many experts do not stay in the L1."""
+    logits = torch.randn(T, n, device=DEV)
+    before = ops.launch_count()
+    ops.moe_route(logits, n, 2)
+    assert ops.launch_count() - before == launches

@@ -225,7 +225,10 @@ extern "C" int tlc_moe_route(const float* logits, int ld, int T, int E, int top,
   TLC_REQUIRE(E >= 1 && top >= 1 && top <= E && E <= 4096, "moe_route: %d experts, %d chosen", E, top);
   TLC_REQUIRE(mode == TLC_ROUTE_SIGMOID || mode == TLC_ROUTE_SOFTMAX || mode == TLC_ROUTE_SOFTMAX_ALL, "moe_route: unknown weighting %d", mode);
   TLC_REQUIRE(n_identity >= 0 && n_identity < E, "moe_route: %d of %d router outputs without an expert's weights", n_identity, E);
-  if (T <= 8) {             // (1 row 5.2 us as two launches, 4.9 as one; 8 rows 5.4; 32 rows 5.6 and, the block being larger, 10.5)
+  // Few rows in one launch: 1 row 5.2 us as two, 4.9 as one; 8 rows 5.4; 32 rows 5.6 and, the block being larger, 10.5.  Only up to 128 experts:
+  // the choosing alone is quicker in its own kernel (5 rows of 256 13.7 us, 14.3 as one), and the lists' shared memory comes out of the L1, which the
+  // rows are read from again and again (4 rows of 4,096 102 us as two launches, 224 as one).
+  if (T <= 8 && E <= 128) {
     tlc_launch(moe_topk_sort_kernel, dim3(1), dim3(32 * std::max(T, 4)), (size_t)2 * E * sizeof(int), stream, logits, ld, T, E, top, mode, choice_bias,
                ids, wts, sum_to, E - n_identity, tile_rows, order, offsets, tile_off);
     TLC_CHECK_LAUNCH("moe_route");
