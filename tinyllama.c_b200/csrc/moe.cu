@@ -30,6 +30,7 @@ __device__ __forceinline__ void moe_topk(const float* __restrict__ logits, int l
   const bool normed = mode == TLC_ROUTE_SOFTMAX_ALL && sum_to > 0.f;
   float last = INFINITY, first = 0.f, sum = 0.f;
   int last_e = -1, my_id = 0;
+  float my_w = 0.f;
   // TLC_ROUTE_SOFTMAX_ALL: scores are the softmax over all E outputs; an expert is chosen by score + choice_bias[e] and
   // weighted by the score alone
   float all_max = 0.f, all_inv = 1.0f;
@@ -69,7 +70,7 @@ __device__ __forceinline__ void moe_topk(const float* __restrict__ logits, int l
     // the choices of 32 passes, one a lane, are weighed together
     const int n = (k & 31) + 1;
     const float z = lr[my_id];
-    float w;
+    float& w = my_w;
     if (mode == TLC_ROUTE_SOFTMAX) {         // the first choice has the largest logit: numerators exp(z_k - z_0)
       if (k < 32) first = __shfl_sync(0xffffffffu, z, 0);
       w = expf(z - first);
@@ -80,16 +81,21 @@ __device__ __forceinline__ void moe_topk(const float* __restrict__ logits, int l
     }
     if (mode == TLC_ROUTE_SOFTMAX || normed)
       for (int i = 0; i < n; i++) sum += __shfl_sync(0xffffffffu, w, i);      // (in the order of the choices)
-    if (lane < n) {
-      ids[t * top + k + 1 - n + lane] = my_id;
-      wts[t * top + k + 1 - n + lane] = w;
+    if (k + 1 < top) {                       // (the last ones leave below)
+      ids[t * top + k - 31 + lane] = my_id;
+      wts[t * top + k - 31 + lane] = w;
     }
   }
   // softmax: the numerators divided by their sum; all scores: divided by the chosen ones' sum (+ 1e-20, which keeps a sum of zero
   // finite) and multiplied by sum_to
   const float inv = normed ? 1.0f / (sum + 1e-20f) : 1.0f / sum;
-  if (!normed && mode != TLC_ROUTE_SOFTMAX) return;
-  for (int k = lane; k < top; k += 32) wts[t * top + k] = normed ? wts[t * top + k] * inv * sum_to : wts[t * top + k] * inv;
+  auto final_of = [&](float w) { return normed ? w * inv * sum_to : mode == TLC_ROUTE_SOFTMAX ? w * inv : w; };
+  const int at = (top - 1) & ~31;
+  if (at + lane < top) {
+    ids[t * top + at + lane] = my_id;
+    wts[t * top + at + lane] = final_of(my_w);
+  }
+  for (int k = lane; k < at; k += 32) wts[t * top + k] = final_of(wts[t * top + k]);
 }
 
 __global__ void __launch_bounds__(128)
