@@ -44,6 +44,8 @@ const Entry kEntries[] = {
     TLC_ENTRY(tlc_attention_prefill), TLC_ENTRY(tlc_attention_prefill_tc),
     TLC_ENTRY(tlc_mamba_conv), TLC_ENTRY(tlc_mamba_step), TLC_ENTRY(tlc_ssm_scan), TLC_ENTRY(tlc_ssm_scan_one_row), TLC_ENTRY(tlc_ssm_scan_chunked), TLC_ENTRY(tlc_ssm_scan_ssd),
     TLC_ENTRY(tlc_rows_int8), TLC_ENTRY(tlc_linear_int8), TLC_ENTRY(tlc_moe_route), TLC_ENTRY(tlc_moe_experts_int8),
+    TLC_ENTRY(tlc_page_resize), TLC_ENTRY(tlc_row_maps), TLC_ENTRY(tlc_kv_store), TLC_ENTRY(tlc_tree_attention),
+    TLC_ENTRY(tlc_beam_select), TLC_ENTRY(tlc_beam_reorder_states), TLC_ENTRY(tlc_beam_reorder_pages),
 };
 #undef TLC_ENTRY
 constexpr int kCount = (int)(sizeof(kEntries) / sizeof(kEntries[0]));

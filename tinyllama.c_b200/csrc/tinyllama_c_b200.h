@@ -552,6 +552,65 @@ int tlc_retention_chunked(float* proj, int ld, int q_off, int k_off, int v_off, 
                           int B, int n_seg, int chunk_rows, int H, int dk, int dv, void* out, int out_dtype, int out_ld,
                           cudaStream_t stream);
 
+/* ---- pages handed out on the GPU (page_tables.cu) ------------------------------------------------------------
+ * A pool: refs [n_pages] counts the entries of block_table [n_slots, max_pages] that name a page (0: free, more than 1: shared),
+ * lengths [n_slots] the positions a slot holds, in the first ceil(lengths / 64) pages of its row.  status: a word that is raised
+ * to the largest code that occurred and stays until the caller clears it: 1 not enough free pages, 2 a length below 0 or beyond a row of the
+ * table, 3 a slot that does not exist or is named twice, 4 an entry or a count that cannot be (a page that does not exist, or is
+ * free), 5 a slot that would grow inside a page it shares.
+ * tlc_page_resize: slot slots[b] (-1: nothing) shall hold want[b] positions: pages behind them are given back (entries 0), and
+ * missing ones are the lowest free pages, request by request.  All of it, or with a code nothing.  B at most 8,192.
+ * tlc_row_maps: for the rows of a step, request b bringing rows[b] of them after its first start[b] positions: cu_seqlens [B + 1],
+ * row_seq, positions and row_map (page * 64 + offset of the row's position, -1: none) [T]; rows behind the last request have row_seq -1,
+ * position 0, no place; rows beyond T are left out.  parents (NULL: none) makes the rows drafts: parents[t] is the index, among its request's
+ * rows, of the draft that row t follows (-1: the context; always smaller than the row's own), positions are start + depth,
+ * mask [T, words] has the bits of the drafts on the way up and the row's own, and only rows that keep [T] (bytes) accepts have
+ * places; a row whose way up is broken sees nothing and has none.
+ * tlc_kv_store: row t of layer l of k and v (v may be NULL) [L, T, KV * hd] to place row_map[t] of the pages [L, n_pages, KV, 64, hd]; strides
+ * in elements. */
+int tlc_page_resize(int* block_table, int n_slots, int max_pages, int* refs, int n_pages, int* lengths, const int* slots,
+                    const int* want, int B, int* status, cudaStream_t stream);
+int tlc_row_maps(const int* block_table, int n_slots, int max_pages, const int* slots, const int* start, const int* rows, int B,
+                 int T, const int* parents, const void* keep, int words, int* cu_seqlens, int* row_seq, int* positions,
+                 int* row_map, int* mask, cudaStream_t stream);
+int tlc_kv_store(const void* k, const void* v, int dtype, long long layer_k, long long layer_v, long long ld_k, long long ld_v,
+                 const int* row_map, void* k_pages, void* v_pages, int page_dtype, int L, int T, int n_pages, int KV, int hd,
+                 cudaStream_t stream);
+
+/* ---- attention of drafted tokens (tree_attention.cu, tree_attention_tc.cu) ------------------------------------------
+ * Row t of request b sees the request's context (positions 0 .. start[b] - 1, in the pages of its slot; slot -1: none) and those
+ * of the request's new rows whose bit mask[t] has (mask [T, words]; NULL: the rows up to itself), with window > 0 those of
+ * them whose position is above positions[t] - window.  q [T, H * hd], k_new and v_new [T, KV * hd] (row strides ld_*) of the pages' type.
+ * softcap, sink and sink_values as in tlc_attention.  max_context, max_new: no context and no request's rows are longer.
+ * A row that sees nothing is 0; rows behind cu_seqlens[B] are left as they were.  scratch: tlc_tree_attention_scratch bytes, 16-byte
+ * aligned; aligned: whether q, k_new, v_new, out and the pages start on 16-byte boundaries, row by row. */
+long long tlc_tree_attention_scratch(int dtype, int aligned, int B, int T, int H, int KV, int hd, int max_context, int max_new);
+int tlc_tree_attention(const void* q, int dtype, int ld_q, const void* k_new, int ld_k, const void* v_new, int ld_v, const void* k_pages,
+                       const void* v_pages, int n_pages, const int* block_table, int n_slots, int max_pages, const int* slots,
+                       const int* start, const int* cu_seqlens, const int* positions, const int* mask, int words, void* out,
+                       int out_ld, int B, int T, int H, int KV, int hd, float scale, int window, float softcap, int sink,
+                       const float* sink_values, int max_context, int max_new, void* scratch, int aligned, cudaStream_t stream);
+
+/* ---- beam search (beam.cu) ------------------------------------------------------------------------------------------
+ * tlc_beam_select: for every request the n candidates (beam k, token v) of the largest scores[k] + logits[k, v] - log sum exp logits[k],
+ * equal ones by k * V + v; logits [R * K, V] with rows of ld, scores [R, K].  A beam whose score is not finite, or whose logits hold a NaN
+ * or +infinity, has no candidates; one that has ended (bytes [R, K], NULL: none) has one, token pad at its score.  Where there are
+ * fewer than n, the first other pairs follow with a score of -infinity.  placed (n == K): a beam's first child stays in its
+ * place and the others fill the places left; else the best comes first.  scratch: tlc_beam_select_scratch(R * K, V, n) bytes.
+ * tlc_beam_reorder_states: what slot slots[r, parents[r, k]] holds goes to slot slots[r, k], in every layer at once; strides in bytes.
+ * tlc_beam_reorder_pages: the same of a pool's keys and values: a beam with another parent than itself gives back its pages but the last,
+ * shares the parent's whole pages and takes over what the parent's last, partly filled page holds in its own last page.  A request
+ * for which that cannot be done (status as above) stays as it is.  scratch: 16 * R * K bytes.  A slot of -1 or a parent outside
+ * 0 .. K - 1 leaves a beam as it is. */
+long long tlc_beam_select_scratch(int rows, int V, int n);
+int tlc_beam_select(const float* logits, long long ld, const float* scores, const void* ended, int R, int K, int V, int n, int pad,
+                    int placed, void* scratch, int* tokens, int* parents, float* out_scores, cudaStream_t stream);
+int tlc_beam_reorder_states(void* state, long long layer_bytes, long long slot_bytes, long long bytes, int L, int n_slots,
+                            const int* slots, const int* parents, int R, int K, cudaStream_t stream);
+int tlc_beam_reorder_pages(int* block_table, int n_slots, int max_pages, int* refs, int n_pages, int* lengths, const int* slots,
+                           const int* parents, int R, int K, void* k_pages, void* v_pages, int dtype, int L, int KV, int hd,
+                           void* scratch, int* status, cudaStream_t stream);
+
 /* ---- sampling (sampling.cu) ------------------------------------------------------------------------ */
 /* out[r] = first index of the maximum of logits[r].  work: NULL (one block a row), or 12 * R bytes, 8-byte
  * aligned and zero (R 64-bit keys, R counters), which every launch leaves zero: a row is then spread over

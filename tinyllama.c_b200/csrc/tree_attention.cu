@@ -1,0 +1,363 @@
+// Attention of drafted tokens (a tree per request) over the paged cache, and the kernel that adds up partial results.
+//
+// CodeClaper/tinyllama.c attends causally, one sequence at a time (cpu_op.c:1010-1062); speculative decoding is no part of it.  Row i
+// of a request's drafts sees the request's context (positions 0 .. start - 1 in the pages) and those drafts whose bit its mask has:
+//     o_i = sum_j p_ij v_j,   p_ij = exp(s_ij) / (sum_j exp(s_ij) [+ exp(sink)]),   s_ij = cap(scale q_i . k_j)
+// with cap(s) = softcap tanh(s / softcap).  The drafts' keys and values are read where the projections left them: nothing of a draft
+// is in the cache before it is accepted.  A row that sees nothing has o = 0.
+//
+// The kernel here serves 32 bits and every head size up to 256; bfloat16 heads of 64 and 128 have their own
+// (tree_attention_tc.cu).  A block walks the tiles of 64 keys of its segments (see tree_attention.cuh) with 64 (or 16) pairs of a row and a head of the
+// group at a time, running maximum and sum per pair, all in 32 bits: scores and products by register tiles of 4 x 4
+// from shared memory.  Bound by the CUDA cores' FFMA rate for many pairs, by the tiles' way into shared memory for few.
+#include "tree_attention.cuh"
+
+namespace {
+
+constexpr int NT = 256, BN = TLC_PAGE;
+constexpr float LOG2E = 1.4426950408889634f;
+
+__host__ __device__ constexpr int padded(int hd) { return ((hd + 3) / 4) % 2 ? (hd + 3) / 4 * 4 : (hd + 3) / 4 * 4 + 4; }   // 16-byte rows, an odd number of pieces
+__host__ __device__ constexpr int smem_floats(int hd, int rows) { return (rows + BN) * padded(hd) + BN * ((hd + 63) / 64 * 64) + rows * (BN + 4); }
+
+// RM rows of pairs a thread (16 RM a tile), NJ times 64 columns of values.
+template <typename T, int RM, int NJ>
+__global__ void __launch_bounds__(NT)
+tree_attention_kernel(TreeArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  tlc_wait(a.q, a.k_new, a.v_new, a.k_pages, a.v_pages, a.block_table, a.slots, a.start, a.cu, a.positions, a.mask, a.out, a.part_o, a.part_ml,
+           a.plan);
+  constexpr int ROWS = 16 * RM;
+  extern __shared__ float4 tree_raw[];
+  const int hd = a.hd, hp = padded(hd), hv = NJ * 64, G = a.H / a.KV;
+  float* const Q = reinterpret_cast<float*>(tree_raw);
+  float* const K = Q + ROWS * hp;
+  float* const V = K + BN * hp;
+  float* const P = V + BN * hv;                            // [ROWS][BN + 4]
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const T* const q = reinterpret_cast<const T*>(a.q);
+  int b, unit;
+  long long todo;
+  tree_plan<NT>(a, blockIdx.x, &b, &unit, &todo);
+  const float scale2 = a.scale * LOG2E;
+  for (bool first_segment = true; todo > 0; first_segment = false) {
+    TreeSeq s = tree_seq(a, b);
+    while (unit >= s.units) { unit -= s.units; s = tree_seq(a, ++b); }
+    const int item = unit / s.key_tiles, kt0 = unit % s.key_tiles;
+    const int g = item / s.row_tiles, r0 = item % s.row_tiles * a.tile_rows;
+    const int kt1 = (int)min((long long)s.key_tiles, kt0 + todo);
+    const int pairs = min(a.tile_rows, s.n * G - r0);
+    const int* const table = a.block_table + (size_t)(s.context_tiles > 0 ? a.slots[b] : 0) * a.max_pages;
+    __syncthreads();                                        // the segment before has used its queries
+    // the tile's queries
+    for (int e = tid; e < ROWS * hp; e += NT) {
+      const int r = e / hp, d = e % hp;
+      float v = 0.f;
+      if (r < pairs && d < hd) {
+        const int i = (r0 + r) / G, h = g * G + (r0 + r) % G;
+        v = to_f32(q[(size_t)(s.t0 + i) * a.ld_q + (size_t)h * hd + d]);
+      }
+      Q[e] = v;
+    }
+    float m[RM], l[RM], o[RM][4 * NJ];
+    int pos[RM];
+#pragma unroll
+    for (int u = 0; u < RM; u++) {
+      m[u] = -INFINITY;
+      l[u] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4 * NJ; c++) o[u][c] = 0.f;
+      const int r = ty * RM + u;
+      pos[u] = r < pairs ? a.positions[s.t0 + (r0 + r) / G] : 0;
+    }
+    for (int kt = kt0; kt < kt1; kt++) {
+      const bool draft = kt >= s.context_tiles;
+      const int base = draft ? (kt - s.context_tiles) * BN : (s.first_tile + kt) * BN;       // first key of the tile: a draft's index, or a position
+      const int keys = min(BN, (draft ? s.n : s.context) - base);
+      const T *kr, *vr;
+      size_t ldk, ldv;
+      bool there = true;
+      if (draft) {
+        kr = reinterpret_cast<const T*>(a.k_new) + (size_t)(s.t0 + base) * a.ld_k + (size_t)g * hd;
+        vr = reinterpret_cast<const T*>(a.v_new) + (size_t)(s.t0 + base) * a.ld_v + (size_t)g * hd;
+        ldk = a.ld_k;
+        ldv = a.ld_v;
+      } else {
+        const int page = table[base / BN];
+        there = page >= 0 && page < a.n_pages;              // (a page that is none reads as zeros)
+        const size_t at = ((size_t)(there ? page : 0) * a.KV + g) * (size_t)(BN * hd);
+        kr = reinterpret_cast<const T*>(a.k_pages) + at;
+        vr = reinterpret_cast<const T*>(a.v_pages) + at;
+        ldk = ldv = hd;
+      }
+      __syncthreads();                                      // the tile before has been used
+      for (int e = tid; e < BN * hp; e += NT) {
+        const int r = e / hp, d = e % hp;
+        K[e] = there && r < keys && d < hd ? to_f32(kr[r * ldk + d]) : 0.f;
+      }
+      bool odd = false;                                     // a value that is no number must not reach rows that do not see it
+      for (int e = tid; e < BN * hv; e += NT) {
+        const int r = e / hv, d = e % hv;
+        const float v = there && r < keys && d < hd ? to_f32(vr[r * ldv + d]) : 0.f;
+        V[e] = v;
+        odd |= !isfinite(v);
+      }
+      odd = __syncthreads_or(odd);
+      float sc[RM][4];
+#pragma unroll
+      for (int u = 0; u < RM; u++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) sc[u][j] = 0.f;
+      for (int d = 0; d < hd; d += 4) {
+        float4 qv[RM], kv[4];
+#pragma unroll
+        for (int u = 0; u < RM; u++) qv[u] = *reinterpret_cast<const float4*>(Q + (ty * RM + u) * hp + d);
+#pragma unroll
+        for (int j = 0; j < 4; j++) kv[j] = *reinterpret_cast<const float4*>(K + (tx + 16 * j) * hp + d);
+#pragma unroll
+        for (int u = 0; u < RM; u++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            sc[u][j] = fmaf(qv[u].x, kv[j].x, fmaf(qv[u].y, kv[j].y, fmaf(qv[u].z, kv[j].z, fmaf(qv[u].w, kv[j].w, sc[u][j]))));
+      }
+#pragma unroll
+      for (int u = 0; u < RM; u++) {
+        const int r = ty * RM + u, i = (r0 + r) / G;
+        float mx = m[u];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int key = tx + 16 * j;
+          bool sees = r < pairs && key < keys;
+          if (sees) sees = draft ? tree_sees(a, s.t0, i, base + key) : a.window <= 0 || base + key > pos[u] - a.window;
+          float x = sc[u][j] * scale2;
+          if (a.softcap > 0.f) x = a.softcap * LOG2E * tanhf(sc[u][j] * a.scale / a.softcap);
+          sc[u][j] = sees ? x : -INFINITY;
+          mx = fmaxf(mx, sc[u][j]);
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float ref = mx == -INFINITY ? 0.f : mx, shrink = m[u] == -INFINITY ? 0.f : exp2f(m[u] - ref);
+        m[u] = mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float p = exp2f(sc[u][j] - ref);
+          sum += p;
+          P[r * (BN + 4) + tx + 16 * j] = p;
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        l[u] = (l[u] == 0.f ? 0.f : l[u] * shrink) + sum;
+#pragma unroll
+        for (int c = 0; c < 4 * NJ; c++) o[u][c] = o[u][c] == 0.f ? 0.f : o[u][c] * shrink;
+      }
+      __syncwarp();                                         // a row of P is written and read by the same 16 lanes
+      if (!odd) {
+        for (int k = 0; k < BN; k += 4) {
+          float4 p[RM];
+#pragma unroll
+          for (int u = 0; u < RM; u++) p[u] = *reinterpret_cast<const float4*>(P + (ty * RM + u) * (BN + 4) + k);
+#pragma unroll
+          for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int c = 0; c < NJ; c++) {
+              const float4 v = *reinterpret_cast<const float4*>(V + (k + x) * hv + 64 * c + tx * 4);
+#pragma unroll
+              for (int u = 0; u < RM; u++) {
+                const float w = x == 0 ? p[u].x : x == 1 ? p[u].y : x == 2 ? p[u].z : p[u].w;
+                o[u][4 * c] = fmaf(w, v.x, o[u][4 * c]);
+                o[u][4 * c + 1] = fmaf(w, v.y, o[u][4 * c + 1]);
+                o[u][4 * c + 2] = fmaf(w, v.z, o[u][4 * c + 2]);
+                o[u][4 * c + 3] = fmaf(w, v.w, o[u][4 * c + 3]);
+              }
+            }
+        }
+      } else {
+        for (int k = 0; k < BN; k++)
+#pragma unroll
+          for (int u = 0; u < RM; u++) {
+            const float w = P[(ty * RM + u) * (BN + 4) + k];
+            if (w == 0.f) continue;
+#pragma unroll
+            for (int c = 0; c < 4 * NJ; c++) o[u][c] = fmaf(w, V[k * hv + 64 * (c / 4) + tx * 4 + c % 4], o[u][c]);
+          }
+      }
+    }
+    const bool whole = kt0 == 0 && kt1 == s.key_tiles;
+    const size_t part = ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * a.part_rows;
+#pragma unroll
+    for (int u = 0; u < RM; u++) {
+      const int r = ty * RM + u;
+      if (r >= pairs) continue;
+      const int i = (r0 + r) / G, h = g * G + (r0 + r) % G;
+      if (whole) {
+        float total = l[u], mx = m[u];
+        float f = 1.f;
+        if (a.sink) {
+          const float sv = a.sink_values ? a.sink_values[h] * LOG2E : 0.f, top = fmaxf(mx, sv);
+          f = mx == -INFINITY && total == 0.f ? 0.f : exp2f(mx - top);
+          total = (total == 0.f ? 0.f : total * f) + exp2f(sv - top);
+        }
+        const float inv = l[u] == 0.f ? 0.f : f / total;
+        T* const to = reinterpret_cast<T*>(a.out) + (size_t)(s.t0 + i) * a.out_ld + (size_t)h * hd;
+#pragma unroll
+        for (int c = 0; c < 4 * NJ; c++) {
+          const int d = 64 * (c / 4) + tx * 4 + c % 4;
+          if (d < hd) to[d] = from_f32<T>(l[u] == 0.f ? 0.f : o[u][c] * inv);
+        }
+      } else {
+        if (tx == 0) { a.part_ml[(part + r) * 2] = m[u]; a.part_ml[(part + r) * 2 + 1] = l[u]; }
+#pragma unroll
+        for (int c = 0; c < 4 * NJ; c++) {
+          const int d = 64 * (c / 4) + tx * 4 + c % 4;
+          if (d < hd) a.part_o[(part + r) * hd + d] = o[u][c];
+        }
+      }
+    }
+    todo -= kt1 - kt0;
+    unit += kt1 - kt0;
+  }
+}
+
+// Items that several blocks share: o = sum_z o_z 2^(m_z - m) / (sum_z l_z 2^(m_z - m) [+ 2^(sink - m)]).  A warp per (row, head).
+template <typename T>
+__global__ void __launch_bounds__(128)
+tree_merge_kernel(TreeArgs a) {
+  tlc_pdl(a.cu, a.part_o, a.part_ml, a.plan, a.out);
+  const int t = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (h >= a.H) return;
+  const int G = a.H / a.KV, g = h / G, hd = a.hd;
+  int lo = 0, hi = a.B;                                    // the request: the last with cu[b] <= t
+  if (t < a.cu[0] || t >= a.cu[a.B]) return;               // rows behind the last request are left as they are
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu[mid] <= t) lo = mid; else hi = mid;
+  }
+  const int t0 = max(a.cu[lo], 0), n = min(a.cu[lo + 1], a.T) - t0, r = (t - t0) * G + h % G;
+  const int row_tiles = (n * G + a.tile_rows - 1) / a.tile_rows, kt = a.plan[a.B + 1 + lo];
+  const long long W = a.plan[a.B];
+  if (W <= 0 || kt <= 0) return;
+  const long long u0 = a.plan[lo] + ((long long)g * row_tiles + r / a.tile_rows) * kt;
+  const int nb = tree_blocks(W, a.blocks), c0 = tree_block_of(W, u0, nb), c1 = tree_block_of(W, u0 + kt - 1, nb);
+  if (c0 >= c1 || c0 < 0 || c1 >= nb) return;              // one block had all of it
+  auto part = [&](int c) { return ((size_t)c * 2 + (c == c0 && tree_first(W, c, nb) < u0 ? 1 : 0)) * a.part_rows + r % a.tile_rows; };
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) {
+    const size_t p = part(c);
+    if (a.part_ml[p * 2 + 1] != 0.f) m = fmaxf(m, a.part_ml[p * 2]);
+  }
+  m = warp_max(m);
+  const float sv = a.sink && a.sink_values ? a.sink_values[h] * LOG2E : 0.f;
+  if (a.sink) m = fmaxf(m, sv);
+  float l = 0.f, acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) acc[e] = 0.f;
+  for (int base = c0; base <= c1; base += 32) {
+    float w = 0.f;
+    size_t p = 0;
+    if (base + lane <= c1) {
+      p = part(base + lane);
+      const float lz = a.part_ml[p * 2 + 1];
+      if (lz != 0.f) {
+        w = exp2f(a.part_ml[p * 2] - m);
+        l += lz * w;
+      }
+    }
+    const int here = min(32, c1 - base + 1);
+    for (int z = 0; z < here; z++) {
+      const float wz = __shfl_sync(0xffffffffu, w, z);
+      const size_t pz = __shfl_sync(0xffffffffu, (unsigned long long)p, z);
+      if (wz == 0.f) continue;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int d = lane + 32 * e;
+        if (d < hd) acc[e] = fmaf(a.part_o[pz * hd + d], wz, acc[e]);
+      }
+    }
+  }
+  l = warp_sum(l);
+  const float total = a.sink ? l + exp2f(sv - m) : l;
+  const float inv = l == 0.f ? 0.f : 1.0f / total;
+  T* const to = reinterpret_cast<T*>(a.out) + (size_t)t * a.out_ld + (size_t)h * hd;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const int d = lane + 32 * e;
+    if (d < hd) to[d] = from_f32<T>(l == 0.f ? 0.f : acc[e] * inv);
+  }
+}
+
+template <typename T, int RM> int run_simt(const TreeArgs& a, cudaStream_t stream) {
+  const int nj = (a.hd + 63) / 64, smem = smem_floats(a.hd, 16 * RM) * (int)sizeof(float);
+  auto* const k = nj == 1 ? tree_attention_kernel<T, RM, 1> : nj == 2 ? tree_attention_kernel<T, RM, 2> : tree_attention_kernel<T, RM, 4>;
+  const int full = nj <= 2 ? smem : smem + BN * (256 - nj * 64) * (int)sizeof(float);
+  if (full > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, full) != cudaSuccess)
+    return tlc_fail(-2, "tree_attention: cannot reserve %d bytes of shared memory", full);
+  tlc_launch(k, dim3(a.blocks), dim3(NT), (size_t)full, stream, a);
+  TLC_CHECK_LAUNCH("tree_attention");
+  return 0;
+}
+
+}  // namespace
+
+int tlc_tree_attention_simt(const TreeArgs& a, int dtype, int rows, cudaStream_t stream) {
+  TLC_DISPATCH_DTYPE(dtype, T, return rows == 64 ? (run_simt<T, 4>(a, stream)) : (run_simt<T, 1>(a, stream)));
+}
+
+// How a call is cut: pairs of a tile (64 for many, 16 for few), blocks, and the scratch that it needs.
+namespace {
+struct Cut { int rows, tile_rows, blocks; bool tc; long long scratch; };
+Cut cut_of(int dtype, int aligned, int B, int T, int H, int KV, int hd, int max_context, int max_new) {
+  Cut c;
+  const int G = H / KV;
+  c.tc = false;
+  (void)aligned;
+  c.rows = (long long)max_new * G > 16 ? 64 : 16;
+  c.tile_rows = c.rows;
+  const long long kt = ((long long)max_context + BN - 1) / BN + (max_new + BN - 1) / BN;
+  const long long most = (((long long)T * G + c.tile_rows - 1) / c.tile_rows + B) * KV * kt;
+  const long long wave = 148 * 2;
+  c.blocks = (int)(most < wave ? (most < 1 ? 1 : most) : wave);
+  c.scratch = (long long)c.blocks * 2 * c.rows * (hd + 2) * 4 + (2ll * B + 1) * 4;
+  return c;
+}
+}  // namespace
+
+extern "C" long long tlc_tree_attention_scratch(int dtype, int aligned, int B, int T, int H, int KV, int hd, int max_context, int max_new) {
+  if (KV <= 0 || H <= 0 || H % KV) return 0;
+  return cut_of(dtype, aligned, B, T, H, KV, hd, max_context, max_new).scratch;
+}
+
+extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void* k_new, int ld_k, const void* v_new, int ld_v, const void* k_pages,
+                                  const void* v_pages, int n_pages, const int* block_table, int n_slots, int max_pages, const int* slots,
+                                  const int* start, const int* cu_seqlens, const int* positions, const int* mask, int words, void* out,
+                                  int out_ld, int B, int T, int H, int KV, int hd, float scale, int window, float softcap, int sink,
+                                  const float* sink_values, int max_context, int max_new, void* scratch, int aligned, cudaStream_t stream) {
+  if (B == 0 || T == 0) return 0;
+  TLC_REQUIRE(B > 0 && T > 0 && KV > 0 && H > 0 && H % KV == 0 && H <= 65535 * 4 && hd >= 1 && hd <= 256,
+              "tree_attention: %d rows of %d requests, %d heads over %d of size %d (at most 256)", T, B, H, KV, hd);
+  TLC_REQUIRE(max_context >= 0 && max_new >= 0 && n_pages > 0 && n_slots > 0 && max_pages > 0 && (mask == nullptr || words > 0),
+              "tree_attention: contexts of %d, %d new rows, %d pages", max_context, max_new, n_pages);
+  TLC_REQUIRE(((uintptr_t)scratch & 15) == 0, "tree_attention: scratch must start on a 16-byte boundary");
+  const Cut c = cut_of(dtype, aligned, B, T, H, KV, hd, max_context, max_new);
+  TreeArgs a = {};
+  a.q = q; a.k_new = k_new; a.v_new = v_new; a.k_pages = k_pages; a.v_pages = v_pages;
+  a.ld_q = ld_q; a.ld_k = ld_k; a.ld_v = ld_v; a.n_pages = n_pages;
+  a.block_table = block_table; a.slots = slots; a.start = start; a.cu = cu_seqlens; a.positions = positions; a.mask = mask;
+  a.n_slots = n_slots; a.max_pages = max_pages; a.words = words;
+  a.out = out; a.out_ld = out_ld; a.B = B; a.T = T; a.H = H; a.KV = KV; a.hd = hd;
+  a.scale = scale; a.window = window > 0 ? window : 0; a.softcap = softcap; a.sink = sink; a.sink_values = sink_values;
+  a.max_context = max_context;
+  a.tile_rows = c.tile_rows;
+  a.blocks = c.blocks;
+  a.part_rows = c.rows;
+  a.part_o = (float*)scratch;
+  a.part_ml = a.part_o + (size_t)c.blocks * 2 * c.rows * hd;
+  a.plan = (int*)(a.part_ml + (size_t)c.blocks * 2 * c.rows * 2);
+  const long long kt = ((long long)max_context + BN - 1) / BN + (max_new + BN - 1) / BN;
+  TLC_REQUIRE((((long long)T * (H / KV) + c.tile_rows - 1) / c.tile_rows + B) * KV * kt < (1ll << 31), "tree_attention: %d rows over %d keys are too many", T,
+              max_context);
+  if (const int rc = tlc_tree_attention_simt(a, dtype, c.rows, stream)) return rc;
+  TLC_DISPATCH_DTYPE(dtype, E, tlc_launch(tree_merge_kernel<E>, dim3(T, (H + 3) / 4), dim3(128), 0, stream, a));
+  TLC_CHECK_LAUNCH("tree_attention(merge)");
+  return 0;
+}

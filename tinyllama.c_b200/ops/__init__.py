@@ -9,9 +9,11 @@ cannot be built, the call raises.  Parts of the model call these through the mod
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 import threading
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -167,6 +169,16 @@ _SIGNATURES = {
     "tlc_linear_int8_kernel": (_i, [_i, _i]),
     "tlc_moe_experts_int8": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i,
                                   _i, _i, _f, _f, _vp]),
+    "tlc_page_resize": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp]),
+    "tlc_row_maps": (_i, [_vp, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "tlc_kv_store": (_i, [_vp, _vp, _i, _ll, _ll, _ll, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "tlc_tree_attention_scratch": (_ll, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "tlc_tree_attention": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i,
+                                _i, _i, _f, _i, _f, _i, _vp, _i, _i, _vp, _i, _vp]),
+    "tlc_beam_select_scratch": (_ll, [_i, _i, _i]),
+    "tlc_beam_select": (_i, [_vp, _ll, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "tlc_beam_reorder_states": (_i, [_vp, _ll, _ll, _ll, _i, _i, _vp, _vp, _i, _i, _vp]),
+    "tlc_beam_reorder_pages": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp]),
     "tlc_argmax": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
     "tlc_sample": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _i, _f, _f, _f, _i, _f, _f, _vp, _vp]),
     "tlc_attention_decode_no_alloc": (_i, [_vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _i, _i,
@@ -233,7 +245,9 @@ def _call(name: str, *args) -> None:
 REPEATABLE = frozenset(("tlc_event_record", "tlc_event_wait", "tlc_rmsnorm", "tlc_gated_rmsnorm", "tlc_gated_rmsnorm_step", "tlc_linear",
                         "tlc_linear_swiglu", "tlc_glu", "tlc_rope_kv_store", "tlc_attention", "tlc_attention_decode",
                         "tlc_attention_decode_fused", "tlc_attention_prefill", "tlc_attention_prefill_tc", "tlc_mamba_conv", "tlc_mamba_step",
-                        "tlc_ssm_scan", "tlc_ssm_scan_one_row", "tlc_ssm_scan_chunked", "tlc_ssm_scan_ssd", "tlc_rows_int8", "tlc_linear_int8", "tlc_moe_route", "tlc_moe_experts_int8"))
+                        "tlc_ssm_scan", "tlc_ssm_scan_one_row", "tlc_ssm_scan_chunked", "tlc_ssm_scan_ssd", "tlc_rows_int8", "tlc_linear_int8", "tlc_moe_route", "tlc_moe_experts_int8",
+                        "tlc_page_resize", "tlc_row_maps", "tlc_kv_store", "tlc_tree_attention", "tlc_beam_select", "tlc_beam_reorder_states",
+                        "tlc_beam_reorder_pages"))
 
 
 # ctypes converts an argument at a time, 2.5 us for a call of 21; packed by one struct they take 0.5.
@@ -2137,3 +2151,324 @@ def retention_chunked(proj: torch.Tensor, q_off: int, k_off: int, v_off: int, g_
           seg_start.data_ptr(), seg_seq.data_ptr(), seq_seg_start.data_ptr(), step.slots.data_ptr(), step.start_pos.data_ptr(), step.n_seqs,
           n_seg, int(chunk_rows), int(H), int(dk), int(dv), out.data_ptr(), dtype_code(out.dtype), _out_rows(out, T, H * dv, "retention_chunked"),
           _stream())
+
+
+# ---- several candidates of a request over one paged cache: drafted tokens, beams ---------------------------------------------
+MAX_TABLE_REQUESTS = 8192      # page_tables.cu: MAX_REQUESTS
+MAX_BEAMS = 64                 # beam.cu: beams of a request, and candidates of one
+MAX_POOL_PAGES = 1 << 25       # places (page * 64 + offset) are 32-bit numbers
+POOL_STATUS = {0: "done", 1: "not enough free pages", 2: "a length below 0 or beyond a row of the block table",
+               3: "a slot that does not exist or is named twice", 4: "an entry or a count that cannot be",
+               5: "a slot that would grow inside a page it shares"}
+
+
+def _here(what: str, *tensors) -> None:
+    """Tensors that one launch names lie on the device that it goes to."""
+    dev = _get_device() if _get_device is not None and torch.cuda.is_available() else None
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.get_device() != dev):
+            _gpu(t)
+            raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{dev}")
+
+
+def _ints_of(t: torch.Tensor, n: int, what: str) -> None:
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+        raise KernelError(f"{what}: expected {n} contiguous int32 values, got {t.dtype} of shape {tuple(t.shape)}")
+
+
+def _flags(t: Optional[torch.Tensor], n: int, what: str) -> int:
+    if t is None:
+        return 0
+    if t.dtype != torch.bool or t.numel() != n or not t.is_contiguous():
+        raise KernelError(f"{what}: expected {n} contiguous truth values (torch.bool), got {t.dtype} of shape {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _table(block_table: torch.Tensor, what: str):
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous() or block_table.numel() == 0:
+        raise KernelError(f"{what}: the block table is a contiguous int32 [slots, pages], got {block_table.dtype} {tuple(block_table.shape)}")
+    return block_table.shape
+
+
+def _pool(block_table, refs, lengths, status, what: str):
+    n_slots, max_pages = _table(block_table, what)
+    _ints_of(lengths, n_slots, what + " lengths")
+    if refs.dtype != torch.int32 or refs.dim() != 1 or not refs.is_contiguous() or not 1 <= refs.numel() <= MAX_POOL_PAGES:
+        raise KernelError(f"{what}: refs are 1 to {MAX_POOL_PAGES} contiguous int32 counts, got {refs.dtype} {tuple(refs.shape)}")
+    if status.dtype != torch.int32 or status.numel() < 1 or not status.is_contiguous():
+        raise KernelError(f"{what}: status is an int32 word")
+    return n_slots, max_pages
+
+
+def page_resize(block_table: torch.Tensor, refs: torch.Tensor, lengths: torch.Tensor, slots: torch.Tensor, want: torch.Tensor,
+                status: torch.Tensor) -> None:
+    """Makes slot slots[b] hold want[b] positions, for every request at once: what Cache.reserve and Cache.release do, on the GPU.
+
+    The pool is three int32 tensors: refs [pages] counts the entries of block_table [slots, pages a slot] that name a page (0: free),
+    lengths [slots] the positions that a slot holds, in the first ceil(length / 64) pages of its row.  Pages behind the positions
+    wanted are given back (their entries become 0); missing ones are the lowest free pages, in the order of the requests.  slots and
+    want are int32 [B] (at most 8,192; slot -1: nothing to do).  All of it is done or, with a code, nothing: status[0] is raised to the
+    largest code that occurred (POOL_STATUS) and stays until the caller clears it."""
+    n_slots, max_pages = _pool(block_table, refs, lengths, status, "page_resize")
+    B = slots.numel()
+    _ints_of(slots, B, "page_resize slots")
+    _ints_of(want, B, "page_resize want")
+    if B > MAX_TABLE_REQUESTS:
+        raise KernelError(f"page_resize: {B} requests; a call takes {MAX_TABLE_REQUESTS}")
+    _here("page_resize", block_table, refs, lengths, slots, want, status)
+    _call_packed("tlc_page_resize", block_table.data_ptr(), n_slots, max_pages, refs.data_ptr(), refs.numel(), lengths.data_ptr(),
+                 slots.data_ptr(), want.data_ptr(), B, status.data_ptr(), _stream())
+
+
+@dataclass
+class RowMaps:
+    """What the rows of a step are told (row_maps): int32 tensors on the device."""
+    cu_seqlens: torch.Tensor                 # [B + 1]: request b has rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1
+    row_seq: torch.Tensor                    # [T]: the row's request, -1 behind the last one
+    positions: torch.Tensor                  # [T]: its position in the sequence
+    row_map: torch.Tensor                    # [T]: its place in the pages, page * 64 + offset, -1: none
+    mask: Optional[torch.Tensor] = None      # [T, ceil(max_new / 32)]: which drafts of its request the row sees (bit j % 32 of word j // 32)
+
+
+def row_maps(block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor, new: torch.Tensor, n_rows: int,
+             parents: Optional[torch.Tensor] = None, keep: Optional[torch.Tensor] = None, max_new: int = 0) -> RowMaps:
+    """Sequences, positions and places of a step's rows from the requests' lengths: request b brings new[b] rows after its first
+    start[b] positions (int32 [B] each, in packed order), n_rows is how many rows the step's tensors have (more are left out; rows behind
+    the last request have request -1, position 0 and no place).
+
+    parents (int32 [n_rows]) makes the rows drafted tokens: parents[t] is the index, among its request's rows, of the draft that row t
+    follows (-1: the request's last position; always smaller than the row's own index).  Positions are then start + depth, mask says which
+    drafts a row sees (those above it and itself; max_new: the most rows of a request) and no row has a place, but those that
+    keep (torch.bool [n_rows]) accepts.  A row whose way up is broken sees nothing and has no place.  Without parents, keep leaves out rows."""
+    n_slots, max_pages = _table(block_table, "row_maps")
+    B, T = slots.numel(), int(n_rows)
+    if B > MAX_TABLE_REQUESTS or T < 0:
+        raise KernelError(f"row_maps: {B} requests (a call takes {MAX_TABLE_REQUESTS}) of {T} rows")
+    for t, what in ((slots, "row_maps slots"), (start, "row_maps start"), (new, "row_maps new")):
+        _ints_of(t, B, what)
+    words = 0
+    if parents is not None:
+        _ints_of(parents, T, "row_maps parents")
+        if max_new < 1:
+            raise KernelError("row_maps: max_new, the most rows of a request, says how wide the drafts' masks are")
+        words = (int(max_new) + 31) // 32
+    kept = _flags(keep, T, "row_maps keep")
+    _here("row_maps", block_table, slots, start, new, parents, keep)
+    # (cut by as_strided: a tensor's own slicing costs three times as much)
+    ints = torch.empty(B + 1 + T * (3 + words), dtype=torch.int32, device=block_table.device)
+    view, at = ints.as_strided, B + 1
+    maps = RowMaps(view((B + 1,), (1,), 0), view((T,), (1,), at), view((T,), (1,), at + T), view((T,), (1,), at + 2 * T),
+                   view((T, words), (words, 1), at + 3 * T) if words else None)
+    p = ints.data_ptr()
+    _call_packed("tlc_row_maps", block_table.data_ptr(), n_slots, max_pages, slots.data_ptr(), start.data_ptr(), new.data_ptr(), B, T,
+                 0 if parents is None else parents.data_ptr(), kept, words, p, p + 4 * at, p + 4 * (at + T), p + 4 * (at + 2 * T),
+                 p + 4 * (at + 3 * T) if words else 0, _stream())
+    _note_owned(ints)
+    return maps
+
+
+def _layers_of_rows(t: torch.Tensor, what: str):
+    """(layers, rows, width, layer stride, row stride) of rows [T, C] or [L, T, C]."""
+    if t.dim() not in (2, 3) or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise KernelError(f"{what}: rows [T, C] or, layer by layer, [L, T, C], dense within a row; got {tuple(t.shape)} strides {t.stride()}")
+    L, T, C = (1, *t.shape) if t.dim() == 2 else t.shape
+    return L, T, C, t.stride(0) if t.dim() == 3 and L > 1 else 0, t.stride(-2) if T > 1 else max(C, 1)
+
+
+def _page_shape(pages: torch.Tensor, what: str):
+    """(layers, pages, kv heads, head size) of pages [n, KV, 64, hd] or [L, n, KV, 64, hd]."""
+    if pages.dim() not in (4, 5) or pages.shape[-2] != PAGE or not pages.is_contiguous():
+        raise KernelError(f"{what}: contiguous pages [n, KV, {PAGE}, hd] or, layer by layer, [L, n, KV, {PAGE}, hd]; got {tuple(pages.shape)}")
+    L, n, KV, _, hd = pages.shape if pages.dim() == 5 else (1, *pages.shape)
+    if not 1 <= n <= MAX_POOL_PAGES or KV < 1 or hd < 1:
+        raise KernelError(f"{what}: {n} pages of {KV} heads of size {hd}")
+    return L, n, KV, hd
+
+
+def kv_store(k: torch.Tensor, v: Optional[torch.Tensor], row_map: torch.Tensor, k_pages: torch.Tensor,
+             v_pages: Optional[torch.Tensor]) -> None:
+    """Stores rows of keys and values at the places of row_map (int32 [T], see row_maps), of all layers in one launch: k and v [T, KV * hd] with
+    pages [n, KV, 64, hd], or [L, T, KV * hd] with pages [L, n, KV, 64, hd]; float32 or bfloat16, rounded where the pages are
+    narrower; v and v_pages may be None (pages without values).  Rows of k and v may be strided.  A row without a place (-1, or one
+    that does not exist) is not stored.  Places are distinct, as row_maps makes them: of two rows for one place either may stay."""
+    L, n, KV, hd = _page_shape(k_pages, "kv_store")
+    if (v is None) != (v_pages is None) or (v_pages is not None and (v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype)):
+        raise KernelError("kv_store: values and their pages come together, the pages alike")
+    l, T, C, layer_k, ld_k = _layers_of_rows(k, "kv_store keys")
+    layer_v = ld_v = 0
+    if v is not None:
+        lv, tv, cv, layer_v, ld_v = _layers_of_rows(v, "kv_store values")
+        if (lv, tv, cv) != (l, T, C) or v.dtype != k.dtype:
+            raise KernelError(f"kv_store: keys {tuple(k.shape)} {k.dtype} and values {tuple(v.shape)} {v.dtype} do not agree")
+        if not v_pages.is_contiguous():
+            raise KernelError("kv_store: pages must be contiguous")
+    if l != L or C != KV * hd or k.dim() != k_pages.dim() - 2:
+        raise KernelError(f"kv_store: rows {tuple(k.shape)} do not fit pages {tuple(k_pages.shape)}")
+    _ints_of(row_map, T, "kv_store row_map")
+    _here("kv_store", k, v, row_map, k_pages, v_pages)
+    _call_packed("tlc_kv_store", k.data_ptr(), 0 if v is None else v.data_ptr(), dtype_code(k.dtype), layer_k, layer_v, ld_k, ld_v,
+                 row_map.data_ptr(), k_pages.data_ptr(), 0 if v is None else v_pages.data_ptr(), dtype_code(k_pages.dtype), L, T, n, KV, hd,
+                 _stream())
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_scratch(*args) -> int:
+    return library().tlc_tree_attention_scratch(*args)
+
+
+def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                   block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor, cu_seqlens: torch.Tensor,
+                   positions: torch.Tensor, out: torch.Tensor, H: int, KV: int, hd: int, scale: float, max_context: int, max_new: int,
+                   mask: Optional[torch.Tensor] = None, window: int = 0, softcap: float = 0.0, sink: bool = False,
+                   sink_values: Optional[torch.Tensor] = None) -> None:
+    """Grouped-query attention of drafted tokens over the paged cache: row t of request b (rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1) sees the
+    request's context, positions 0 .. start[b] - 1 in the pages of slot slots[b], and those of the request's own new rows whose
+    bit mask[t] has (int32 [T, words], as row_maps makes it; None: the rows up to itself).  The new rows' keys and values are k_new and
+    v_new [T, KV * hd] (rotated, of the pages' type; rows may be strided): nothing of a draft needs to be in the cache (kv_store puts
+    the accepted ones there).  q [T, H * hd], out [T, H * hd] (a range of the columns of a wider buffer will do).
+
+    positions int32 [T]: the rows' positions, none below its request's start; with window > 0 a row sees the keys whose
+    position is above its own - window.  softcap, sink and sink_values as in attention().  max_context and max_new bound the contexts and the
+    requests' new rows (a longer context is cut).  A row that sees nothing is 0; rows behind the last request are left as they were;
+    a key or value that a row does not see does not touch it, whatever it holds.  float32 or bfloat16, heads of up to 256."""
+    T, B = q.shape[0], slots.numel()
+    dt = q.dtype
+    if not (1 <= hd <= MAX_HEAD_DIM) or H < 1 or KV < 1 or H % KV:
+        raise KernelError(f"tree_attention: {H} heads over {KV} key/value heads of size {hd} (at most {MAX_HEAD_DIM})")
+    if q.dim() != 2 or q.shape[1] != H * hd or tuple(k_new.shape) != (T, KV * hd) or tuple(v_new.shape) != (T, KV * hd):
+        raise KernelError(f"tree_attention: q{tuple(q.shape)}, k_new{tuple(k_new.shape)}, v_new{tuple(v_new.shape)} for {H} and {KV} heads of size {hd}")
+    if k_new.dtype != dt or v_new.dtype != dt or k_pages.dtype != dt or v_pages.dtype != dt or out.dtype != dt:
+        raise KernelError("tree_attention: queries, new keys and values, pages and output share one element type")
+    if k_pages.dim() != 4 or tuple(k_pages.shape[1:]) != (KV, PAGE, hd) or v_pages.shape != k_pages.shape or k_pages.shape[0] < 1 \
+            or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+        raise KernelError(f"tree_attention: contiguous pages [n, {KV}, {PAGE}, {hd}], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    if max_context < 0 or max_new < 0 or window < 0 or softcap < 0:
+        raise KernelError("tree_attention: max_context, max_new, window and softcap are not negative")
+    if softcap > 0 and scale == 0:
+        raise KernelError("tree_attention: capped scores need a scale")
+    n_slots, max_pages = _table(block_table, "tree_attention")
+    _ints_of(slots, B, "tree_attention slots")
+    _ints_of(start, B, "tree_attention start")
+    _ints_of(cu_seqlens, B + 1, "tree_attention cu_seqlens")
+    _ints_of(positions, T, "tree_attention positions")
+    words = 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[1] * 32 < max_new:
+            raise KernelError(f"tree_attention: masks are int32 [T, words] with a bit for each of {max_new} rows, got {tuple(mask.shape)}")
+        words = mask.shape[1]
+        _ints_of(mask, T * words, "tree_attention mask")
+    if sink_values is not None:
+        _f32vec(sink_values, H, "tree_attention sink scores")
+    ld_q, ld_k, ld_v, ld_o = _rows(q, "tree_attention q"), _rows(k_new, "tree_attention k_new"), _rows(v_new, "tree_attention v_new"), \
+        _out_rows(out, T, H * hd, "tree_attention")
+    _here("tree_attention", q, k_new, v_new, k_pages, v_pages, block_table, slots, start, cu_seqlens, positions, out, mask, sink_values)
+    if T == 0 or B == 0:
+        return
+    code = dtype_code(dt)
+    pq, pk, pv, pkp, pvp, po = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
+    aligned = 0 if (pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7 else 1
+    max_context, max_new = min(int(max_context), max_pages * PAGE), int(max_new)
+    scratch = torch.empty(_tree_scratch(code, aligned, B, T, H, KV, hd, max_context, max_new), dtype=torch.uint8, device=q.device)
+    _note_owned(scratch)
+    _call_packed("tlc_tree_attention", pq, code, ld_q, pk, ld_k, pv, ld_v, pkp, pvp, k_pages.shape[0], block_table.data_ptr(), n_slots, max_pages,
+                 slots.data_ptr(), start.data_ptr(), cu_seqlens.data_ptr(), positions.data_ptr(), 0 if mask is None else mask.data_ptr(), words,
+                 po, ld_o, B, T, H, KV, hd, scale, int(window), softcap, 1 if sink or sink_values is not None else 0,
+                 0 if sink_values is None else sink_values.data_ptr(), max_context, max_new, scratch.data_ptr(), aligned, _stream())
+
+
+@functools.lru_cache(maxsize=4096)
+def _beam_scratch(*args) -> int:
+    return library().tlc_beam_select_scratch(*args)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, ended: Optional[torch.Tensor] = None, pad: int = 0,
+                placed: bool = False):
+    """A beam search's step: (tokens int32 [R, n], parents int32 [R, n], scores float32 [R, n]) of the n best candidates of every request.
+
+    A candidate is a beam k and a token v, worth scores[r, k] + logits[r * K + k, v] - log sum exp logits[r * K + k]; equal ones go by the lowest
+    k * V + v.  logits float32 [R * K, V] (rows may be strided), scores float32 [R, K].  ended (torch.bool [R, K]): such a beam has one
+    candidate, token `pad` at the score it has.  A beam whose score is not finite has none (at a search's first step all but one beam
+    have a score of -infinity), nor has one with a NaN or +infinity among its logits; where fewer than n are left, the first other
+    pairs follow with a score of -infinity.  The best comes first; placed (n = K): the first child of a beam takes its parent's
+    place and the others, in order, the places that are left, so that only beams without children are overwritten (beam_reorder_*).
+    K and n at most 64."""
+    if scores.dim() != 2 or logits.dim() != 2 or logits.dtype != torch.float32:
+        raise KernelError(f"beam_select: float32 logits [R * K, V] and scores [R, K], got {logits.dtype} {tuple(logits.shape)} and {tuple(scores.shape)}")
+    (R, K), (rows, V), n = scores.shape, logits.shape, int(n)
+    if rows != R * K or not 1 <= K <= MAX_BEAMS or V < 1 or not 1 <= n <= min(MAX_BEAMS, K * V) or (placed and n != K):
+        raise KernelError(f"beam_select: {n} candidates of {R} requests with {K} beams (at most {MAX_BEAMS}) from logits {tuple(logits.shape)}"
+                          + (" in the beams' places" if placed else ""))
+    if not 0 <= pad < V:
+        raise KernelError(f"beam_select: token {pad} of {V}")
+    _f32vec(scores, R * K, "beam_select scores")
+    ld, gone = _rows(logits, "beam_select logits"), _flags(ended, R * K, "beam_select ended")
+    _here("beam_select", logits, scores, ended)
+    ints = torch.empty(3 * R * n, dtype=torch.int32, device=logits.device)
+    view = ints.as_strided
+    tokens, parents, best = view((R, n), (n, 1), 0), view((R, n), (n, 1), R * n), view((R, n), (n, 1), 2 * R * n).view(torch.float32)
+    if R:
+        scratch = torch.empty(_beam_scratch(rows, V, n), dtype=torch.uint8, device=logits.device)
+        _note_owned(ints, scratch)
+        p = ints.data_ptr()
+        _call_packed("tlc_beam_select", logits.data_ptr(), ld, scores.data_ptr(), gone, R, K, V, n, int(pad), 1 if placed else 0, scratch.data_ptr(),
+                     p, p + 4 * R * n, p + 8 * R * n, _stream())
+    return tokens, parents, best
+
+
+def _beams(slots: torch.Tensor, parents: torch.Tensor, what: str):
+    if slots.dim() != 2 or parents.shape != slots.shape or not 1 <= slots.shape[1] <= MAX_BEAMS:
+        raise KernelError(f"{what}: slots and parents are int32 [R, K] with K at most {MAX_BEAMS}, got {tuple(slots.shape)} and {tuple(parents.shape)}")
+    _ints_of(slots, slots.numel(), what + " slots")
+    _ints_of(parents, slots.numel(), what + " parents")
+    return slots.shape
+
+
+def beam_reorder_states(state: torch.Tensor, slots: torch.Tensor, parents: torch.Tensor) -> None:
+    """Beam k of request r, in slot slots[r, k], goes on from beam parents[r, k]: state [layers, slots, ...] (any type; what a slot holds is
+    dense) is permuted in place, every layer in one launch.  Any map of beams to parents will do; slot -1 or a parent outside 0 .. K - 1
+    leaves a beam as it is.  The slots of a call are distinct."""
+    R, K = _beams(slots, parents, "beam_reorder_states")
+    if state.dim() < 2:
+        raise KernelError(f"beam_reorder_states: states are [layers, slots, ...], got {tuple(state.shape)}")
+    size, values = state.element_size(), 1
+    for d in range(state.dim() - 1, 1, -1):
+        if state.shape[d] > 1 and state.stride(d) != values:
+            raise KernelError(f"beam_reorder_states: what a slot holds must be dense, got {tuple(state.shape)} strides {state.stride()}")
+        values *= state.shape[d]
+    L, n_slots = state.shape[:2]
+    if n_slots > 1 and state.stride(1) < values:
+        raise KernelError(f"beam_reorder_states: slots overlap, got {tuple(state.shape)} strides {state.stride()}")
+    if values * size >= (1 << 31) - (1 << 20) or (L > 1 and state.stride(0) < values):
+        raise KernelError(f"beam_reorder_states: {values * size} bytes a slot, strides {state.stride()}")
+    _here("beam_reorder_states", state, slots, parents)
+    if L and n_slots and values and R:
+        _call_packed("tlc_beam_reorder_states", state.data_ptr(), state.stride(0) * size, state.stride(1) * size, values * size, L, n_slots,
+                     slots.data_ptr(), parents.data_ptr(), R, K, _stream())
+
+
+def beam_reorder_pages(block_table: torch.Tensor, refs: torch.Tensor, lengths: torch.Tensor, slots: torch.Tensor, parents: torch.Tensor,
+                       k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], status: torch.Tensor) -> None:
+    """Beam k of request r, in slot slots[r, k], goes on from beam parents[r, k], over a pool as page_resize keeps it: the beam gives back its
+    pages but the last, its row names the parent's whole pages (shared: refs counts them), and what the parent's last, partly
+    filled page holds is copied into the beam's own last page, in every layer of k_pages and v_pages ([n, KV, 64, hd] or [L, n, KV, 64, hd];
+    v_pages may be None).  Lengths follow.  A beam needs a page of its own only where the parent's last page is partly filled: a search
+    starts from one sequence by giving each other beam a slot of length 1 and the parent 0.
+
+    slots and parents int32 [R, K]; slot -1 or a parent outside 0 .. K - 1 leaves a beam as it is.  A request for which it cannot be done
+    (no page of its own, one that others share, a slot named twice) stays as it is, with a code in status (see page_resize)."""
+    R, K = _beams(slots, parents, "beam_reorder_pages")
+    n_slots, max_pages = _pool(block_table, refs, lengths, status, "beam_reorder_pages")
+    L, n, KV, hd = _page_shape(k_pages, "beam_reorder_pages")
+    if n != refs.numel():
+        raise KernelError(f"beam_reorder_pages: {n} pages and {refs.numel()} counts")
+    if v_pages is not None and (v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or not v_pages.is_contiguous()):
+        raise KernelError("beam_reorder_pages: pages of keys and of values are alike")
+    _here("beam_reorder_pages", block_table, refs, lengths, slots, parents, k_pages, v_pages, status)
+    if not R:
+        return
+    code = dtype_code(k_pages.dtype)
+    own = torch.empty(4 * R * K, dtype=torch.int32, device=block_table.device)
+    _note_owned(own)
+    _call_packed("tlc_beam_reorder_pages", block_table.data_ptr(), n_slots, max_pages, refs.data_ptr(), n, lengths.data_ptr(), slots.data_ptr(),
+                 parents.data_ptr(), R, K, k_pages.data_ptr(), 0 if v_pages is None else v_pages.data_ptr(), code, L, KV, hd, own.data_ptr(),
+                 status.data_ptr(), _stream())
