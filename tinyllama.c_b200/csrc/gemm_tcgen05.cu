@@ -661,6 +661,21 @@ int tlc_tensor_map_bf16(const void* p, long long rows, long long cols, long long
   return 0;
 }
 
+// The same of `rank` dimensions, innermost first; strides in bytes, of all dimensions but the innermost.
+int tlc_tensor_map_bf16_nd(const void* p, int rank, const unsigned long long* dims, const unsigned long long* strides, const unsigned* box,
+                           CUtensorMap* out) {
+  if (int rc = init_once()) return rc;
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], e[5];
+  for (int i = 0; i < rank; i++) { d[i] = dims[i]; b[i] = box[i]; e[i] = 1; if (i) st[i - 1] = strides[i - 1]; }
+  CUresult r = g_encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(p), d, st, b, e,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return tlc_fail(-3, "cuTensorMapEncodeTiled failed with %d (rank %d, %llu x %llu)", (int)r, rank, dims[0], dims[1]);
+  return 0;
+}
+
 // The same for 8-bit values (gemm_int8_few.cu, gemm_int8_wide.cu) of `rank` dimensions.
 int tlc_tensor_map_int8(const void* p, int rank, const unsigned long long* dims, const unsigned long long* strides, const unsigned* box,
                         CUtensorMap* out) {

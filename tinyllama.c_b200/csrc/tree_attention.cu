@@ -303,28 +303,29 @@ int tlc_tree_attention_simt(const TreeArgs& a, int dtype, int rows, cudaStream_t
   TLC_DISPATCH_DTYPE(dtype, T, return rows == 64 ? (run_simt<T, 4>(a, stream)) : (run_simt<T, 1>(a, stream)));
 }
 
-// How a call is cut: pairs of a tile (64 for many, 16 for few), blocks, and the scratch that it needs.
+// How a call is cut: by which kernel, pairs of a tile, blocks, and the scratch that it needs.
 namespace {
-struct Cut { int rows, tile_rows, blocks; bool tc; long long scratch; };
-Cut cut_of(int dtype, int aligned, int B, int T, int H, int KV, int hd, int max_context, int max_new) {
+struct Cut { bool tc; int rows, tile_rows, blocks; long long units, scratch; };
+Cut cut_of(int dtype, int aligned, int n_pages, int B, int T, int H, int KV, int hd, int max_context, int max_new) {
+  static int sms = 0;
+  if (sms == 0) { int dev = 0; cudaGetDevice(&dev); cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev); }
   Cut c;
   const int G = H / KV;
-  c.tc = false;
-  (void)aligned;
-  c.rows = (long long)max_new * G > 16 ? 64 : 16;
-  c.tile_rows = c.rows;
+  c.tc = tlc_tree_attention_tc_takes(dtype, aligned, H, KV, hd, n_pages);
+  c.rows = c.tc ? 128 : (long long)max_new * G > 16 ? 64 : 16;
+  c.tile_rows = c.tc ? 128 / G * G : c.rows;
   const long long kt = ((long long)max_context + BN - 1) / BN + (max_new + BN - 1) / BN;
-  const long long most = (((long long)T * G + c.tile_rows - 1) / c.tile_rows + B) * KV * kt;
-  const long long wave = 148 * 2;
-  c.blocks = (int)(most < wave ? (most < 1 ? 1 : most) : wave);
+  c.units = (((long long)T * G + c.tile_rows - 1) / c.tile_rows + B) * KV * kt;
+  const long long wave = (long long)sms * (c.tc ? 1 : 2);
+  c.blocks = (int)(c.units < wave ? (c.units < 1 ? 1 : c.units) : wave);
   c.scratch = (long long)c.blocks * 2 * c.rows * (hd + 2) * 4 + (2ll * B + 1) * 4;
   return c;
 }
 }  // namespace
 
-extern "C" long long tlc_tree_attention_scratch(int dtype, int aligned, int B, int T, int H, int KV, int hd, int max_context, int max_new) {
+extern "C" long long tlc_tree_attention_scratch(int dtype, int aligned, int n_pages, int B, int T, int H, int KV, int hd, int max_context, int max_new) {
   if (KV <= 0 || H <= 0 || H % KV) return 0;
-  return cut_of(dtype, aligned, B, T, H, KV, hd, max_context, max_new).scratch;
+  return cut_of(dtype, aligned, n_pages, B, T, H, KV, hd, max_context, max_new).scratch;
 }
 
 extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void* k_new, int ld_k, const void* v_new, int ld_v, const void* k_pages,
@@ -338,7 +339,8 @@ extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void
   TLC_REQUIRE(max_context >= 0 && max_new >= 0 && n_pages > 0 && n_slots > 0 && max_pages > 0 && (mask == nullptr || words > 0),
               "tree_attention: contexts of %d, %d new rows, %d pages", max_context, max_new, n_pages);
   TLC_REQUIRE(((uintptr_t)scratch & 15) == 0, "tree_attention: scratch must start on a 16-byte boundary");
-  const Cut c = cut_of(dtype, aligned, B, T, H, KV, hd, max_context, max_new);
+  const Cut c = cut_of(dtype, aligned, n_pages, B, T, H, KV, hd, max_context, max_new);
+  TLC_REQUIRE(c.units < (1ll << 31), "tree_attention: %d rows over %d keys are too many", T, max_context);
   TreeArgs a = {};
   a.q = q; a.k_new = k_new; a.v_new = v_new; a.k_pages = k_pages; a.v_pages = v_pages;
   a.ld_q = ld_q; a.ld_k = ld_k; a.ld_v = ld_v; a.n_pages = n_pages;
@@ -353,10 +355,7 @@ extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void
   a.part_o = (float*)scratch;
   a.part_ml = a.part_o + (size_t)c.blocks * 2 * c.rows * hd;
   a.plan = (int*)(a.part_ml + (size_t)c.blocks * 2 * c.rows * 2);
-  const long long kt = ((long long)max_context + BN - 1) / BN + (max_new + BN - 1) / BN;
-  TLC_REQUIRE((((long long)T * (H / KV) + c.tile_rows - 1) / c.tile_rows + B) * KV * kt < (1ll << 31), "tree_attention: %d rows over %d keys are too many", T,
-              max_context);
-  if (const int rc = tlc_tree_attention_simt(a, dtype, c.rows, stream)) return rc;
+  if (const int rc = c.tc ? tlc_tree_attention_tc(a, stream) : tlc_tree_attention_simt(a, dtype, c.rows, stream)) return rc;
   TLC_DISPATCH_DTYPE(dtype, E, tlc_launch(tree_merge_kernel<E>, dim3(T, (H + 3) / 4), dim3(128), 0, stream, a));
   TLC_CHECK_LAUNCH("tree_attention(merge)");
   return 0;

@@ -100,3 +100,4 @@ __device__ __forceinline__ bool tree_sees(const TreeArgs& a, int t0, int i, int 
 
 int tlc_tree_attention_simt(const TreeArgs& a, int dtype, int rows, cudaStream_t stream);
 int tlc_tree_attention_tc(const TreeArgs& a, cudaStream_t stream);
+bool tlc_tree_attention_tc_takes(int dtype, int aligned, int H, int KV, int hd, long long n_pages);

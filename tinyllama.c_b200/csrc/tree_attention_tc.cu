@@ -1,0 +1,480 @@
+// Attention of drafted tokens on the 5th-generation tensor cores (sm_100a): bfloat16, heads of 64 and 128.
+//
+// The mathematics is tree_attention.cu's.  A tile is 128 pairs of a drafted row and one of the G query heads that share a key/value head,
+// 128 / G rows with all of their heads, so that a key tile is fetched once for all of them: pairs a key/value head x 2 operations
+// per byte of keys and values, HBM bound up to some 250 pairs (measured peaks, 1,648 TFLOP/s over 6,553 GB/s), tensor bound above.
+// Queries come by TMA as a box of {64 columns, G heads, 128 / G rows}, key tiles as boxes of 64 rows from the pages, or, the drafts', from
+// the projections' own rows.  The walk over the key tiles is the one of the prompts' kernel (attention_prefill_tc.cu): an agent warp each
+// for copies, S = Q K^T and O += P V, and two groups of four worker warps, a thread a row, that take every second key tile with
+// a score buffer, a P buffer and an output accumulator of their own.
+// What is different: a block takes an equal share of all requests' key tiles (see tree_attention.cuh) instead of a tile and a head; keys
+// are masked by a bit per (row, draft); and values that some row of the tile does not see are looked over first, since 0 x NaN is
+// NaN on the tensor cores: rows past the keys' end become zeros, and a value that is no number becomes 0 and is added, at the end, to
+// the rows that do see it.
+// Every wait on an mbarrier is bounded (codes 61-69 of the error word), as in the prompts' kernel.
+#include "tree_attention.cuh"
+#include "mbarrier.cuh"
+#include "tcgen05.cuh"
+
+int tlc_tensor_map_bf16_nd(const void* p, int rank, const unsigned long long* dims, const unsigned long long* strides, const unsigned* box,
+                           CUtensorMap* out);
+
+namespace {
+
+constexpr int BM = 128, BN = TLC_PAGE;
+constexpr int KS = 4, VS = 3;            // stages of the K and V rings
+constexpr int WORKERS = 256, THREADS = WORKERS + 96, NG = 2;
+constexpr float TAU = 8.0f;              // how far (in powers of two) a row's maximum may run ahead of its reference
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float ex2_quick(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// a bfloat16 pair's halves that are infinite or NaN become 0; whether there was one
+__device__ __forceinline__ bool make_finite(uint32_t& w) {
+  bool odd = false;
+  if ((w & 0x7f80u) == 0x7f80u) { w &= 0xffff0000u; odd = true; }
+  if ((w & 0x7f800000u) == 0x7f800000u) { w &= 0x0000ffffu; odd = true; }
+  return odd;
+}
+
+template <int HD>
+struct TreeSmem {
+  static constexpr int Q_SLAB = BM * 128, Q = 0, Q_BYTES = (HD / 64) * Q_SLAB;
+  static constexpr int K_SLAB = BN * 128, K_STAGE = (HD / 64) * K_SLAB, K = Q + Q_BYTES;
+  static constexpr int V_STAGE = HD * 128, V = K + KS * K_STAGE;
+  static constexpr int P_BUF = BM * 128, P = V + VS * V_STAGE;
+  static constexpr int X = P + 2 * P_BUF;                 // [2][NG][128] floats: the groups' reference maxima and sums, at the end
+  static constexpr int BARS = X + 2 * NG * BM * 4;        // mbarriers, tmem slot, dead flag
+  static constexpr int N_BARS = 1 + 2 * KS + 2 * VS + 8;
+  static constexpr int TOTAL = BARS + N_BARS * 8 + 16 + 1024;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(THREADS, 1)
+tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kn,
+                         const __grid_constant__ CUtensorMap map_vn, TreeArgs a, float cap_in, float cap_out, ErrWords* err) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  tlc_wait(a.v_new, a.v_pages, a.block_table, a.slots, a.start, a.cu, a.positions, a.mask, a.out, a.part_o, a.part_ml, a.plan);
+  using L_ = TreeSmem<HD>;
+  constexpr int TCOLS = HD == 128 ? 512 : 256;            // the groups' scores at 0 and 64, their outputs at 128 and 128 + hd
+  extern __shared__ uint8_t tree_tc_raw[];
+  uint8_t* sm = (uint8_t*)(((uintptr_t)tree_tc_raw + 1023) & ~(uintptr_t)1023);
+  float* xch = reinterpret_cast<float*>(sm + L_::X);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L_::BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L_::N_BARS);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ int s_last_pos, s_odd;                       // the tile's largest position; whether a value was no number
+  const uint32_t sm0 = smem_u32(sm);
+  const uint32_t bar_q = smem_u32(bars);
+  auto k_full = [&](int s) { return smem_u32(bars + 1 + s); };
+  auto k_empty = [&](int s) { return smem_u32(bars + 1 + KS + s); };
+  auto v_full = [&](int s) { return smem_u32(bars + 1 + 2 * KS + s); };
+  auto v_empty = [&](int s) { return smem_u32(bars + 1 + 2 * KS + VS + s); };
+  auto s_full = [&](int i) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + i); };
+  auto s_free = [&](int i) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + 2 + i); };
+  auto p_ready = [&](int i) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + 4 + i); };
+  auto pv_done = [&](int i) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + 6 + i); };
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long wait_limit = mbar_wait_limit(err);
+  if (tid == 0) *dead = 0;
+  int b, unit;
+  long long todo;
+  tree_plan<THREADS>(a, blockIdx.x, &b, &unit, &todo);
+  if (todo == 0) return;
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TCOLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+    if (*dead) return;
+    if (!mbar_wait(bar, parity, err, code, wait_limit)) *dead = 1;
+  };
+  const int G = a.H / a.KV, NI = BM / G;                  // rows of a tile
+  const float scale_log2 = a.scale * LOG2E;
+#pragma unroll 1
+  for (bool first_segment = true; todo > 0; first_segment = false) {
+  TreeSeq s = tree_seq(a, b);
+  while (unit >= s.units) { unit -= s.units; s = tree_seq(a, ++b); }
+  const int item = unit / s.key_tiles, kt0 = unit % s.key_tiles;
+  const int g = item / s.row_tiles, i0 = item % s.row_tiles * NI;
+  const int n = (int)min((long long)(s.key_tiles - kt0), todo);        // key tiles of this segment
+  const int rows = min(NI, s.n - i0);
+  if (tid == 0) {
+    s_last_pos = 0;
+    s_odd = 0;
+    for (int i = 0; i < L_::N_BARS; i++) {
+      const uint32_t bar = bar_q + 8 * i;               // every worker warp arrives once on s_free and p_ready, one agent on the rest
+      if (!first_segment) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");   // nothing is pending on it (see the loader's last waits)
+      mbar_init(bar, (bar == s_free(0) || bar == s_free(1) || bar == p_ready(0) || bar == p_ready(1)) ? 4 : 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+  if (a.window > 0) {
+    for (int i = tid; i < rows; i += THREADS) atomicMax(&s_last_pos, a.positions[s.t0 + i0 + i]);
+    __syncthreads();
+  }
+
+  if (warp >= WORKERS / 32) {
+    const int role = warp - WORKERS / 32;
+    constexpr uint32_t DESC_HI = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);      // see smem_desc
+    auto desc_lo = [](uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | (1u << 16); };
+    if (role == 0) {
+      // the copies: the warp reads 32 entries of the block table at a time, its first lane starts the copies
+      if (lane == 0) {
+        mbar_expect_tx(bar_q, (HD / 64) * NI * G * 128);
+        for (int c = 0; c < HD / 64; c++) tma_load_3d(sm0 + L_::Q + c * L_::Q_SLAB, &map_q, bar_q, 64 * c, g * G, s.t0 + i0);
+      }
+      const int* table = a.block_table + (size_t)(s.context_tiles > 0 ? a.slots[b] : 0) * a.max_pages;
+      int entry = 0;
+      for (int t = 0; t < n; t++) {
+        const int kt = kt0 + t;
+        if (t % 32 == 0 && kt + lane < s.context_tiles) entry = table[s.first_tile + kt + lane];
+        const int page = __shfl_sync(0xffffffffu, entry, t % 32);
+        const bool draft = kt >= s.context_tiles;
+        // (a page that is none: behind the map's last row, which reads as zeros)
+        const int row = draft ? s.t0 + (kt - s.context_tiles) * BN : ((page >= 0 && page < a.n_pages ? page * a.KV + g : a.n_pages * a.KV)) * BN;
+        {
+          const int st = t % KS;
+          if (t >= KS) wait(k_empty(st), (uint32_t)(((t - KS) / KS) & 1), 66);       // S of tile t - KS is done
+          if (lane == 0) {
+            mbar_expect_tx(k_full(st), L_::K_STAGE);
+            for (int c = 0; c < HD / 64; c++)
+              tma_load_2d(sm0 + L_::K + st * L_::K_STAGE + c * L_::K_SLAB, draft ? &map_kn : &map_k, k_full(st), (draft ? g * HD : 0) + 64 * c, row);
+          }
+        }
+        {
+          const int st = t % VS;
+          if (t >= VS) wait(v_empty(st), (uint32_t)(((t - VS) / VS) & 1), 67);       // P V of tile t - VS is done
+          if (lane == 0) {
+            mbar_expect_tx(v_full(st), L_::V_STAGE);
+            for (int c = 0; c < HD / 64; c++)
+              tma_load_2d(sm0 + L_::V + st * L_::V_STAGE + c * L_::K_SLAB, draft ? &map_vn : &map_v, v_full(st), (draft ? g * HD : 0) + 64 * c, row);
+          }
+        }
+        __syncwarp();
+      }
+      // the last arrivals on the stages' barriers (the products' commits), which nothing else waits for: after
+      // them no barrier of this segment has anything pending, and the next one may make them anew
+      for (int t = max(0, n - KS); t < n; t++) wait(k_empty(t % KS), (uint32_t)((t / KS) & 1), 66);
+      for (int t = max(0, n - VS); t < n; t++) wait(v_empty(t % VS), (uint32_t)((t / VS) & 1), 67);
+    } else if (lane == 0 && role == 1) {
+      // the scores run two tiles ahead of the workers: both score buffers are in use from the start
+      constexpr uint32_t idesc_s = instr_desc(BM, BN);
+      const uint32_t q_lo = desc_lo(sm0 + L_::Q);
+      wait(bar_q, 0, 61);
+      for (int t = 0; t < n; t++) {
+        const int st = t % KS;
+        wait(k_full(st), (uint32_t)((t / KS) & 1), 62);
+        if (t >= 2) wait(s_free(t & 1), (uint32_t)(((t - 2) >> 1) & 1), 63);         // the workers hold scores t - 2 in registers
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem + (uint32_t)((t & 1) * BN);
+        const uint32_t k_lo = desc_lo(sm0 + L_::K + st * L_::K_STAGE);
+#pragma unroll
+        for (int c = 0; c < HD / 64; c++)
+#pragma unroll
+          for (int kk = 0; kk < 4; kk++)
+            umma_halves(d, q_lo + (uint32_t)((c * L_::Q_SLAB + kk * 32) >> 4), k_lo + (uint32_t)((c * L_::K_SLAB + kk * 32) >> 4),
+                        DESC_HI, idesc_s, (c > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(s_full(t & 1));
+        umma_commit(k_empty(st));
+      }
+    } else if (lane == 0 && role == 2) {
+      constexpr uint32_t idesc_o = instr_desc(BM, HD) | (1u << 16);                   // V is MN-major: hd runs along its rows
+      for (int j = 0; j < n; j++) {
+        const int st = j % VS;
+        wait(v_full(st), (uint32_t)((j / VS) & 1), 65);
+        wait(p_ready(j & 1), (uint32_t)((j >> 1) & 1), 64);                          // P of tile j is in shared memory
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t p_lo = desc_lo(sm0 + L_::P + (j & 1) * L_::P_BUF), v_lo = (desc_lo(sm0 + L_::V + st * L_::V_STAGE) & 0xFFFFu) | ((uint32_t)(L_::K_SLAB >> 4) << 16);
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++)
+          umma_halves(tmem + 128u + (uint32_t)((j & 1) * HD), p_lo + (uint32_t)(kk * 2), v_lo + (uint32_t)(kk * (16 * 128 >> 4)), DESC_HI, idesc_o,
+                      (j >= 2 || kk > 0) ? 1u : 0u);
+        umma_commit(pv_done(j & 1));
+        umma_commit(v_empty(st));
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- the workers: thread (quarter, lane) of a group owns pair r of the tile: row i0 + r / G, head r % G of the group.  It holds all 64 scores of a
+    // key tile and its row of the group's output. ----
+    const int wg = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int i = i0 + r / G;                             // the row among the request's drafts
+    const bool live = r < rows * G;
+    const int t = s.t0 + (live ? i : 0);
+    const int lo_r = a.window > 0 ? a.positions[t] - a.window + 1 : 0;                 // the first position it sees
+    const int lo_most = a.window > 0 ? s_last_pos - a.window + 1 : 0;
+    const uint32_t s_at = tmem + lanes + (uint32_t)(wg * BN);
+    const uint32_t o_at = tmem + lanes + 128u + (uint32_t)(wg * HD);
+    float m_ref = -INFINITY, l = 0.f;                     // the maximum the numerators refer to (scaled, log2), the sum
+    int mine = 0;                                         // tiles this group has done
+    for (int j = wg; j < n; j += NG, mine++) {
+      const bool draft = kt0 + j >= s.context_tiles;
+      const int base = draft ? (kt0 + j - s.context_tiles) * BN : (s.first_tile + kt0 + j) * BN;      // a draft's index, or a position
+      const int keys = (draft ? s.n : s.context) - base;
+      const bool edge = draft || keys < BN || base < lo_most;       // some row of the tile may not see some key of it
+      uint32_t seen_lo = 0xffffffffu, seen_hi = 0xffffffffu;
+      if (edge) {
+        if (draft) {
+          const int word = base >> 5;
+          if (a.mask) {
+            const int* bits = a.mask + (size_t)t * a.words;
+            seen_lo = word < a.words ? (uint32_t)bits[word] : 0u;
+            seen_hi = word + 1 < a.words ? (uint32_t)bits[word + 1] : 0u;
+          } else {                                        // a chain: the rows up to its own
+            const int upto = i - base + 1;
+            seen_lo = upto >= 32 ? 0xffffffffu : upto > 0 ? (1u << upto) - 1 : 0u;
+            seen_hi = upto >= 64 ? 0xffffffffu : upto > 32 ? (1u << (upto - 32)) - 1 : 0u;
+          }
+          if (a.window > 0) {
+            const int* at = a.positions + s.t0 + base;
+            for (int c = 0; c < min(keys, BN); c++)
+              if (at[c] < lo_r) { if (c < 32) seen_lo &= ~(1u << c); else seen_hi &= ~(1u << (c - 32)); }
+          }
+        } else if (lo_r > base) {
+          const int from = min(lo_r - base, BN);
+          seen_lo = from >= 32 ? 0u : 0xffffffffu << from;
+          seen_hi = from >= 64 ? 0u : from > 32 ? 0xffffffffu << (from - 32) : 0xffffffffu;
+        }
+        if (keys < 32) seen_lo &= keys > 0 ? (1u << keys) - 1 : 0u;
+        if (keys < 64) seen_hi &= keys > 32 ? (1u << (keys - 32)) - 1 : 0u;
+      }
+      if (!live) seen_lo = seen_hi = 0u;
+      uint32_t sr[64];
+      wait(s_full(wg), (uint32_t)(mine & 1), 68);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      __syncwarp();
+      tmem_ld32_nowait(s_at, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
+      tmem_ld32_nowait(s_at + 32u, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free(wg));             // the scores are in registers: the buffer may take tile j + 2
+      if (cap_in > 0.f) {
+        // a capped score: s <- cap tanh(s scale / cap), left divided by the scale (what follows multiplies by it);
+        // tanh(x) = 1 - 2 / (e^(2x) + 1), cap_in = 2 log2(e) scale / cap, cap_out = cap / scale
+#pragma unroll
+        for (int c = 0; c < 64; c++) {
+          const float e = ex2_quick(__uint_as_float(sr[c]) * cap_in);
+          sr[c] = __float_as_uint(fmaf(-cap_out, __fdividef(2.0f, e + 1.0f), cap_out));
+        }
+      }
+      if (__any_sync(0xffffffffu, (seen_lo & seen_hi) != 0xffffffffu)) {
+#pragma unroll
+        for (int c = 0; c < 64; c++)
+          if (!((c < 32 ? seen_lo >> c : seen_hi >> (c - 32)) & 1u)) sr[c] = 0xff800000u;     // -inf
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 64; c++) mx = fmaxf(mx, __uint_as_float(sr[c]));
+      mx *= scale_log2;
+      // the reference maximum moves only when the true one has run ahead of it by more than 2^TAU
+      const bool grow = mx > m_ref + TAU || (m_ref == -INFINITY && mx > -INFINITY);
+      if (__any_sync(0xffffffffu, grow)) {
+        float factor = 1.f;
+        if (grow) {
+          factor = m_ref == -INFINITY ? 0.f : ex2_quick(m_ref - mx);
+          m_ref = mx;
+          l *= factor;
+        }
+        if (mine > 0) {
+          wait(pv_done(wg), (uint32_t)((mine - 1) & 1), 69);                          // every product into this output so far is done
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          __syncwarp();
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; c++) {
+            uint32_t o[32];
+            tmem_ld32(o_at + (uint32_t)(32 * c), o);
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st32(o_at + (uint32_t)(32 * c), o);
+          }
+        }
+      }
+      const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+      float sum = 0.f;
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 32; c++) {
+        const float x = ex2_quick(fmaf(__uint_as_float(sr[2 * c]), scale_log2, neg));
+        const float y = ex2_quick(fmaf(__uint_as_float(sr[2 * c + 1]), scale_log2, neg));
+        sum += x + y;
+        pk[c] = pack_bf16(x, y);
+      }
+      l += sum;
+      if (mine > 0) wait(pv_done(wg), (uint32_t)((mine - 1) & 1), 69);               // the group's P buffer is free
+      uint8_t* prow = sm + L_::P + wg * L_::P_BUF + r * 128;
+#pragma unroll
+      for (int q = 0; q < 8; q++)
+        *reinterpret_cast<uint4*>(prow + ((q ^ (r & 7)) << 4)) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+      if (edge) {
+        // the tile's values: rows past the keys' end become zeros, and so does what is no number (it is looked at again at the end)
+        wait(v_full(j % VS), (uint32_t)((j / VS) & 1), 65);
+        uint4* const v = reinterpret_cast<uint4*>(sm + L_::V + (j % VS) * L_::V_STAGE);
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < HD / 16; e++) {
+          const int at = e * 128 + r;                     // pieces of 16 bytes, eight a key, the 64-column halves one after the other
+          if (at / 8 % BN >= keys) v[at] = make_uint4(0u, 0u, 0u, 0u);
+          else {
+            uint4 w = v[at];
+            const bool x = make_finite(w.x), y = make_finite(w.y), z = make_finite(w.z), u = make_finite(w.w);
+            if (x || y || z || u) { v[at] = w; odd = true; }
+          }
+        }
+        if (odd) s_odd = 1;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();                                         // the warp's rows of P are written and fenced
+      if (lane == 0) mbar_arrive(p_ready(wg));
+    }
+    // ---- the two groups' results meet: O = (O_0 2^(m_0 - m) + O_1 2^(m_1 - m)) / (l_0 2^(m_0 - m) + l_1 2^(m_1 - m)) ----
+    if (mine > 0) wait(pv_done(wg), (uint32_t)((mine - 1) & 1), 69);
+    xch[wg * BM + r] = m_ref;
+    xch[(NG + wg) * BM + r] = l;
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    workers_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const bool whole = n == s.key_tiles;                  // else the sums stay unnormalised: another kernel adds the segments
+    const int h = g * G + r % G;
+    const bool with_sink = a.sink && whole;
+    const float sv = with_sink && a.sink_values ? a.sink_values[live ? h : 0] * LOG2E : 0.f;
+    const float m0 = xch[r], m1 = xch[BM + r], l0 = xch[NG * BM + r], l1 = xch[(NG + 1) * BM + r];
+    const float m_keys = fmaxf(m0, m1), m_all = with_sink ? fmaxf(m_keys, sv) : m_keys;
+    const float w0 = m0 == -INFINITY ? 0.f : ex2_quick(m0 - m_all), w1 = m1 == -INFINITY ? 0.f : ex2_quick(m1 - m_all);
+    const float l_keys = l0 * w0 + l1 * w1;
+    const bool none = l0 == 0.f && l1 == 0.f;             // it sees nothing
+    const float inv = whole ? 1.0f / (l_keys + (with_sink ? ex2_quick(sv - m_all) : 0.f)) : 1.0f;
+    const float f0 = w0 * inv, f1 = w1 * inv;
+    const bool has1 = n > 1;                              // the second group had a tile at all (else its accumulator was never written)
+    const size_t part = ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * BM + r;
+    if (!whole && wg == 0 && live) {
+      a.part_ml[part * 2] = m_all;
+      a.part_ml[part * 2 + 1] = l_keys;
+    }
+    const bool odd = s_odd != 0;
+    __syncwarp();
+#pragma unroll 1
+    for (int c = 0; c < HD / 64; c++) {                   // the group's half of the output columns, 32 at a time
+      const int col = wg * (HD / 2) + 32 * c;
+      uint32_t o[32];
+      float acc[32];
+      tmem_ld32(tmem + lanes + 128u + (uint32_t)col, o);
+#pragma unroll
+      for (int e = 0; e < 32; e++) acc[e] = __uint_as_float(o[e]) * f0;
+      if (has1) {
+        tmem_ld32(tmem + lanes + 128u + (uint32_t)(HD + col), o);
+#pragma unroll
+        for (int e = 0; e < 32; e++) acc[e] = fmaf(__uint_as_float(o[e]), f1, acc[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e++) acc[e] = none ? 0.f : acc[e];
+      if (odd && live) {
+        // values that are no numbers, for the rows that see them (a positive weight times NaN or infinity is that again)
+        for (int j = 0; j < n; j++) {
+          const bool draft = kt0 + j >= s.context_tiles;
+          const int base = draft ? (kt0 + j - s.context_tiles) * BN : (s.first_tile + kt0 + j) * BN;
+          const int keys = min(BN, (draft ? s.n : s.context) - base);
+          if (!(draft || keys < BN || base < lo_most)) continue;
+          const int page = draft ? 0 : a.block_table[(size_t)a.slots[b] * a.max_pages + base / BN];
+          if (page < 0 || page >= a.n_pages) continue;
+          for (int k = 0; k < keys; k++) {
+            if (!(draft ? tree_sees(a, s.t0, i, base + k) : base + k >= lo_r)) continue;
+            const __nv_bfloat16* v = draft ? (const __nv_bfloat16*)a.v_new + (size_t)(s.t0 + base + k) * a.ld_v + (size_t)g * HD + col
+                                           : (const __nv_bfloat16*)a.v_pages + (((size_t)page * a.KV + g) * BN + k) * HD + col;
+#pragma unroll 1
+            for (int q = 0; q < 4; q++) {
+              const uint4 w = *reinterpret_cast<const uint4*>(v + 8 * q);
+              uint32_t x[4] = {w.x, w.y, w.z, w.w}, y[4] = {w.x, w.y, w.z, w.w};
+              bool any = false;
+#pragma unroll
+              for (int e = 0; e < 4; e++) any |= make_finite(y[e]);
+              if (!any) continue;
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                if (e / 8 == q) {
+                  const float f = __uint_as_float(e % 2 ? x[e % 8 / 2] & 0xffff0000u : x[e % 8 / 2] << 16);
+                  if (!isfinite(f)) acc[e] += f;
+                }
+            }
+          }
+        }
+      }
+      if (!live) continue;
+      if (!whole) {
+        float4* dst = reinterpret_cast<float4*>(a.part_o + part * HD + col);
+#pragma unroll
+        for (int q = 0; q < 8; q++) dst[q] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (size_t)t * a.out_ld + (size_t)h * HD + col);
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+          dst[q] = make_uint4(pack_bf16(acc[8 * q], acc[8 * q + 1]), pack_bf16(acc[8 * q + 2], acc[8 * q + 3]),
+                              pack_bf16(acc[8 * q + 4], acc[8 * q + 5]), pack_bf16(acc[8 * q + 6], acc[8 * q + 7]));
+      }
+    }
+  }
+  // every agent is done with the segment: its copies have landed, its products have completed (the workers read
+  // their last results, the loader saw the last commits), tensor memory and shared memory may be written again
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  todo -= n;
+  unit += n;
+  }
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TCOLS) : "memory");
+}
+
+template <int HD> int run(const TreeArgs& a, cudaStream_t stream) {
+  auto* const kernel = tree_attention_tc_kernel<HD>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeSmem<HD>::TOTAL) != cudaSuccess)
+    return tlc_fail(-2, "tree_attention(tcgen05): cannot reserve shared memory");
+  const int G = a.H / a.KV, NI = BM / G;
+  CUtensorMap mq, mk, mv, mkn, mvn;
+  const unsigned long long dims[3] = {HD, (unsigned long long)a.H, (unsigned long long)a.T}, strides[2] = {HD * 2, (unsigned long long)a.ld_q * 2};
+  const unsigned box[3] = {64, (unsigned)G, (unsigned)NI};
+  if (int rc = tlc_tensor_map_bf16_nd(a.q, 3, dims, strides, box, &mq)) return rc;
+  const long long page_rows = (long long)a.n_pages * a.KV * BN;
+  if (int rc = tlc_tensor_map_bf16(a.k_pages, page_rows, HD, HD, 64, BN, &mk)) return rc;
+  if (int rc = tlc_tensor_map_bf16(a.v_pages, page_rows, HD, HD, 64, BN, &mv)) return rc;
+  if (int rc = tlc_tensor_map_bf16(a.k_new, a.T, a.KV * HD, a.ld_k, 64, BN, &mkn)) return rc;
+  if (int rc = tlc_tensor_map_bf16(a.v_new, a.T, a.KV * HD, a.ld_v, 64, BN, &mvn)) return rc;
+  tlc_launch(kernel, dim3(a.blocks), dim3(THREADS), (size_t)TreeSmem<HD>::TOTAL, stream, mq, mk, mv, mkn, mvn, a,
+             a.softcap > 0.f ? 2.0f * LOG2E * a.scale / a.softcap : 0.f, a.softcap > 0.f ? a.softcap / a.scale : 0.f, tlc_error_words());
+  TLC_CHECK_LAUNCH("tree_attention(tcgen05)");
+  return 0;
+}
+
+}  // namespace
+
+bool tlc_tree_attention_tc_takes(int dtype, int aligned, int H, int KV, int hd, long long n_pages) {
+  return dtype == TLC_BF16 && aligned && (hd == 64 || hd == 128) && H / KV <= BM && n_pages * KV * BN < (1ll << 31) - BN && tlc_error_words_here() != nullptr;
+}
+
+int tlc_tree_attention_tc(const TreeArgs& a, cudaStream_t stream) { return a.hd == 64 ? run<64>(a, stream) : run<128>(a, stream); }

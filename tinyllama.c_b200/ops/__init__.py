@@ -172,7 +172,7 @@ _SIGNATURES = {
     "tlc_page_resize": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp]),
     "tlc_row_maps": (_i, [_vp, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "tlc_kv_store": (_i, [_vp, _vp, _i, _ll, _ll, _ll, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
-    "tlc_tree_attention_scratch": (_ll, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "tlc_tree_attention_scratch": (_ll, [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "tlc_tree_attention": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i,
                                 _i, _i, _f, _i, _f, _i, _vp, _i, _i, _vp, _i, _vp]),
     "tlc_beam_select_scratch": (_ll, [_i, _i, _i]),
@@ -827,7 +827,7 @@ def check_errors() -> None:
         raise KernelError(f"a kernel gave up on a bounded wait (code {code}: 1 loader, 2 issuer, 3 epilogue, 4 drain, "
                           f"5 accumulator of the tensor-core product; 9 the self-test; 11-16 the scan of prompts; 21-29 "
                           f"attention of prompts; 31-34 the product of few rows; 41 the state of a one-token Mamba2 step; 51-59 "
-                          f"products in 8-bit integers); "
+                          f"products in 8-bit integers; 61-69 attention of drafts); "
                           f"its output is incomplete")
 
 
@@ -2312,7 +2312,7 @@ def kv_store(k: torch.Tensor, v: Optional[torch.Tensor], row_map: torch.Tensor, 
 
 
 @functools.lru_cache(maxsize=4096)
-def _tree_scratch(*args) -> int:
+def _tree_scratch(device: int, *args) -> int:            # (which kernel takes a call is a device's choice)
     return library().tlc_tree_attention_scratch(*args)
 
 
@@ -2368,7 +2368,7 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     pq, pk, pv, pkp, pvp, po = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
     aligned = 0 if (pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7 else 1
     max_context, max_new = min(int(max_context), max_pages * PAGE), int(max_new)
-    scratch = torch.empty(_tree_scratch(code, aligned, B, T, H, KV, hd, max_context, max_new), dtype=torch.uint8, device=q.device)
+    scratch = torch.empty(_tree_scratch(q.get_device(), code, aligned, k_pages.shape[0], B, T, H, KV, hd, max_context, max_new), dtype=torch.uint8, device=q.device)
     _note_owned(scratch)
     _call_packed("tlc_tree_attention", pq, code, ld_q, pk, ld_k, pv, ld_v, pkp, pvp, k_pages.shape[0], block_table.data_ptr(), n_slots, max_pages,
                  slots.data_ptr(), start.data_ptr(), cu_seqlens.data_ptr(), positions.data_ptr(), 0 if mask is None else mask.data_ptr(), words,
