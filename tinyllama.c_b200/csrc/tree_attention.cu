@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(NT)
 tree_attention_kernel(TreeArgs a) {
   asm volatile("griddepcontrol.launch_dependents;");
   tlc_wait(a.q, a.k_new, a.v_new, a.k_pages, a.v_pages, a.block_table, a.slots, a.start, a.cu, a.positions, a.mask, a.out, a.part_o, a.part_ml,
-           a.plan);
+           a.splits);
   constexpr int ROWS = 16 * RM;
   extern __shared__ float4 tree_raw[];
   const int hd = a.hd, hp = padded(hd), hv = NJ * 64, G = a.H / a.KV;
@@ -36,16 +36,15 @@ tree_attention_kernel(TreeArgs a) {
   float* const P = V + BN * hv;                            // [ROWS][BN + 4]
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const T* const q = reinterpret_cast<const T*>(a.q);
-  int b, unit;
-  long long todo;
-  tree_plan<NT>(a, blockIdx.x, &b, &unit, &todo);
+  const TreeTake take = tree_plan<NT>(a, blockIdx.x, reinterpret_cast<int*>(tree_raw));
+  int b = take.b, unit = take.unit, todo = take.todo;
+  TreeSeq s = take.s;
   const float scale2 = a.scale * LOG2E;
   for (bool first_segment = true; todo > 0; first_segment = false) {
-    TreeSeq s = tree_seq(a, b);
     while (unit >= s.units) { unit -= s.units; s = tree_seq(a, ++b); }
     const int item = unit / s.key_tiles, kt0 = unit % s.key_tiles;
     const int g = item / s.row_tiles, r0 = item % s.row_tiles * a.tile_rows;
-    const int kt1 = (int)min((long long)s.key_tiles, kt0 + todo);
+    const int kt1 = min(s.key_tiles, kt0 + todo);
     const int pairs = min(a.tile_rows, s.n * G - r0);
     const int* const table = a.block_table + (size_t)(s.context_tiles > 0 ? a.slots[b] : 0) * a.max_pages;
     __syncthreads();                                        // the segment before has used its queries
@@ -219,71 +218,215 @@ tree_attention_kernel(TreeArgs a) {
   }
 }
 
-// Items that several blocks share: o = sum_z o_z 2^(m_z - m) / (sum_z l_z 2^(m_z - m) [+ 2^(sink - m)]).  A warp per (row, head).
-template <typename T>
-__global__ void __launch_bounds__(128)
+// Items that several blocks share: o = sum_z o_z 2^(m_z - m) / (sum_z l_z 2^(m_z - m) [+ 2^(sink - m)]).  Every block reads which items those
+// are (an entry of splits for each block of the kernel before) and takes its share of their rows: a row a block, the segments shared out
+// over the warps, where there are few rows in many segments, else four rows a warp.  Bound by trips to the L2, of which rows take two (the
+// statistics, then twelve segments' values at a time); a launch with nothing to add up is over after one.
+constexpr int MG_T = 256, MG_WARPS = MG_T / 32, MG_MOST = 512;           // MG_MOST: blocks of the kernel before, at most
+constexpr int MG_ROWS = 4;                                               // of a warp
+template <typename T, int VEC, int NV>
+__global__ void __launch_bounds__(MG_T)
 tree_merge_kernel(TreeArgs a) {
-  tlc_pdl(a.cu, a.part_o, a.part_ml, a.plan, a.out);
-  const int t = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (h >= a.H) return;
-  const int G = a.H / a.KV, g = h / G, hd = a.hd;
-  int lo = 0, hi = a.B;                                    // the request: the last with cu[b] <= t
-  if (t < a.cu[0] || t >= a.cu[a.B]) return;               // rows behind the last request are left as they are
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= t) lo = mid; else hi = mid;
-  }
-  const int t0 = max(a.cu[lo], 0), n = min(a.cu[lo + 1], a.T) - t0, r = (t - t0) * G + h % G;
-  const int row_tiles = (n * G + a.tile_rows - 1) / a.tile_rows, kt = a.plan[a.B + 1 + lo];
-  const long long W = a.plan[a.B];
-  if (W <= 0 || kt <= 0) return;
-  const long long u0 = a.plan[lo] + ((long long)g * row_tiles + r / a.tile_rows) * kt;
-  const int nb = tree_blocks(W, a.blocks), c0 = tree_block_of(W, u0, nb), c1 = tree_block_of(W, u0 + kt - 1, nb);
-  if (c0 >= c1 || c0 < 0 || c1 >= nb) return;              // one block had all of it
-  auto part = [&](int c) { return ((size_t)c * 2 + (c == c0 && tree_first(W, c, nb) < u0 ? 1 : 0)) * a.part_rows + r % a.tile_rows; };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) {
-    const size_t p = part(c);
-    if (a.part_ml[p * 2 + 1] != 0.f) m = fmaxf(m, a.part_ml[p * 2]);
-  }
-  m = warp_max(m);
-  const float sv = a.sink && a.sink_values ? a.sink_values[h] * LOG2E : 0.f;
-  if (a.sink) m = fmaxf(m, sv);
-  float l = 0.f, acc[8];
+  tlc_pdl(a.part_o, a.part_ml, a.splits, a.out);
+  __shared__ int s_before[MG_MOST], s_warp[MG_WARPS], s_most;
+  __shared__ TreeSplit s_split[MG_MOST];
+  __shared__ float s_w[MG_MOST], s_red[2 * MG_WARPS], s_acc[MG_WARPS][NV * 32 * VEC];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.H / a.KV, hd = a.hd;
+  // the items' rows, in fours
+  constexpr int EACH = MG_MOST / MG_T;
+  int total = 0;
+  if (tid == 0) s_most = 0;
+  __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 8; e++) acc[e] = 0.f;
-  for (int base = c0; base <= c1; base += 32) {
-    float w = 0.f;
-    size_t p = 0;
-    if (base + lane <= c1) {
-      p = part(base + lane);
-      const float lz = a.part_ml[p * 2 + 1];
-      if (lz != 0.f) {
-        w = exp2f(a.part_ml[p * 2] - m);
-        l += lz * w;
+  for (int i = 0; i < EACH; i++) {
+    const int c = i * MG_T + tid;
+    if (i * MG_T >= a.blocks) {
+      s_before[c] = 0x7fffffff;
+      continue;
+    }
+    TreeSplit sp = {};
+    if (c < a.blocks) sp = a.splits[c];
+    s_split[c] = sp;
+    const int n = sp.n > 1 ? (sp.pairs + MG_ROWS - 1) / MG_ROWS * MG_ROWS : 0;
+    if (sp.n > 1) atomicMax(&s_most, sp.n);
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (i > 0) __syncthreads();
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    int before = total + x - n;
+#pragma unroll
+    for (int w = 0; w < MG_WARPS; w++) {
+      if (w < warp) before += s_warp[w];
+      total += s_warp[w];
+    }
+    s_before[c] = before;
+  }
+  __syncthreads();
+  // rounds of some three trips for a row a block; of one, and one for every three segments, for four rows a warp
+  const int grid = gridDim.x, wide = grid * MG_WARPS * MG_ROWS;
+  const bool together = (total + grid - 1) / grid * 3 < (total + wide - 1) / wide * (1 + (s_most + 2) / 3) || total <= grid;
+  for (int at = together ? blockIdx.x : (blockIdx.x * MG_WARPS + warp) * MG_ROWS; at < total; at += together ? grid : wide) {
+    int c = 0;                                             // the last block whose rows start at or before this one
+#pragma unroll
+    for (int step = MG_MOST / 2; step > 0; step >>= 1)
+      if (s_before[c + step] <= at) c += step;
+    const TreeSplit& item = s_split[c];
+    const int c0 = item.c0, n = item.n, r = at - s_before[c];
+    auto part = [&](int z, int row) { return ((size_t)(c0 + z) * 2 + (z == 0 ? item.slot0 : 0)) * a.part_rows + row; };
+    auto sink_of = [&](int row) { return a.sink && a.sink_values ? a.sink_values[item.g * G + (item.r0 + row) % G] * LOG2E : 0.f; };
+    auto place = [&](int row) {
+      return reinterpret_cast<T*>(a.out) + (size_t)(item.t0 + (item.r0 + row) / G) * a.out_ld + (size_t)(item.g * G + (item.r0 + row) % G) * hd;
+    };
+    auto stats = [&](int z, int row) { return z < n && row < item.pairs ? *reinterpret_cast<const float2*>(a.part_ml + part(z, row) * 2) : make_float2(-INFINITY, 0.f); };
+    auto values = [&](int z, int row, float (&v)[NV][VEC]) {
+      const float* const p = a.part_o + part(z, row) * hd;
+#pragma unroll
+      for (int e = 0; e < NV; e++) {
+        const int d = (lane + 32 * e) * VEC;
+        if constexpr (VEC == 4) {
+          const float4 f = d < hd ? *reinterpret_cast<const float4*>(p + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[e][0] = f.x; v[e][1] = f.y; v[e][2] = f.z; v[e][3] = f.w;
+        } else v[e][0] = d < hd ? p[d] : 0.f;
+      }
+    };
+    if (together) {
+      if (r >= item.pairs) continue;                       // (filled up to four)
+      __syncthreads();                                     // the row before has been read
+      const float sv = sink_of(r);
+      float m = -INFINITY, l = 0.f, acc[NV][VEC];
+#pragma unroll
+      for (int e = 0; e < NV; e++)
+#pragma unroll
+        for (int q = 0; q < VEC; q++) acc[e][q] = 0.f;
+      float2 ml[EACH];
+#pragma unroll
+      for (int i = 0; i < EACH; i++) {
+        ml[i] = stats(i * MG_T + tid, r);
+        if (ml[i].y != 0.f) m = fmaxf(m, ml[i].x);
+      }
+      m = warp_max(m);
+      if (lane == 0) s_red[warp] = m;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < MG_WARPS; w++) m = fmaxf(m, s_red[w]);
+      if (a.sink) m = fmaxf(m, sv);
+#pragma unroll
+      for (int i = 0; i < EACH; i++)
+        if (i * MG_T + tid < n) {
+          const float w = ml[i].y != 0.f ? exp2f(ml[i].x - m) : 0.f;
+          s_w[i * MG_T + tid] = w;
+          if (ml[i].y != 0.f) l += ml[i].y * w;
+        }
+      l = warp_sum(l);
+      if (lane == 0) s_red[MG_WARPS + warp] = l;
+      __syncthreads();
+      l = 0.f;
+#pragma unroll
+      for (int w = 0; w < MG_WARPS; w++) l += s_red[MG_WARPS + w];
+      constexpr int Z = NV == 1 ? 12 : 4;                  // segments on their way at a time
+      for (int z0 = warp; z0 < n; z0 += Z * MG_WARPS) {
+        float v[Z][NV][VEC];
+#pragma unroll
+        for (int z = 0; z < Z; z++)
+          if (z0 + z * MG_WARPS < n) values(z0 + z * MG_WARPS, r, v[z]);
+#pragma unroll
+        for (int z = 0; z < Z; z++) {
+          const float w = z0 + z * MG_WARPS < n ? s_w[z0 + z * MG_WARPS] : 0.f;
+          if (w == 0.f) continue;
+#pragma unroll
+          for (int e = 0; e < NV; e++)
+#pragma unroll
+            for (int q = 0; q < VEC; q++) acc[e][q] = fmaf(v[z][e][q], w, acc[e][q]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < NV; e++)
+#pragma unroll
+        for (int q = 0; q < VEC; q++) s_acc[warp][(lane + 32 * e) * VEC + q] = acc[e][q];
+      __syncthreads();
+      if (tid < hd) {
+        const float inv = l == 0.f ? 0.f : 1.0f / (a.sink ? l + exp2f(sv - m) : l);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < MG_WARPS; w++) sum += s_acc[w][tid];
+        place(r)[tid] = from_f32<T>(l == 0.f ? 0.f : sum * inv);
+      }
+      continue;
+    }
+    // four rows a warp, eight lanes a row for its segments' weights
+    constexpr int LANES = 32 / MG_ROWS;
+    const int own = r + lane / LANES;
+    const float sv = own < item.pairs ? sink_of(own) : 0.f;
+    float2 ml = stats(lane % LANES, own);
+    float m = ml.y != 0.f ? ml.x : -INFINITY, l = 0.f, acc[MG_ROWS][NV][VEC];
+    for (int z = LANES + lane % LANES; z < n; z += LANES) {
+      const float2 o = stats(z, own);
+      if (o.y != 0.f) m = fmaxf(m, o.x);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (a.sink) m = fmaxf(m, sv);
+#pragma unroll
+    for (int x = 0; x < MG_ROWS; x++)
+#pragma unroll
+      for (int e = 0; e < NV; e++)
+#pragma unroll
+        for (int q = 0; q < VEC; q++) acc[x][e][q] = 0.f;
+    for (int base = 0; base < n; base += LANES) {
+      if (base > 0) ml = stats(base + lane % LANES, own);
+      const float w = ml.y != 0.f ? exp2f(ml.x - m) : 0.f;
+      if (ml.y != 0.f) l += ml.y * w;
+      constexpr int Z = NV == 1 ? 3 : 1;                   // segments of the four rows on their way at a time
+      const int stop = min(n, base + LANES);
+      for (int z0 = base; z0 < stop; z0 += Z) {
+        float v[Z][MG_ROWS][NV][VEC];
+#pragma unroll
+        for (int z = 0; z < Z; z++)
+#pragma unroll
+          for (int x = 0; x < MG_ROWS; x++)
+            if (z0 + z < stop && r + x < item.pairs) values(z0 + z, r + x, v[z][x]);
+#pragma unroll
+        for (int z = 0; z < Z; z++)
+#pragma unroll
+          for (int x = 0; x < MG_ROWS; x++) {
+            const float wz = __shfl_sync(0xffffffffu, w, x * LANES + (z0 + z) % LANES);
+            if (z0 + z >= stop || wz == 0.f || r + x >= item.pairs) continue;
+#pragma unroll
+            for (int e = 0; e < NV; e++)
+#pragma unroll
+              for (int q = 0; q < VEC; q++) acc[x][e][q] = fmaf(v[z][x][e][q], wz, acc[x][e][q]);
+          }
       }
     }
-    const int here = min(32, c1 - base + 1);
-    for (int z = 0; z < here; z++) {
-      const float wz = __shfl_sync(0xffffffffu, w, z);
-      const size_t pz = __shfl_sync(0xffffffffu, (unsigned long long)p, z);
-      if (wz == 0.f) continue;
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int d = lane + 32 * e;
-        if (d < hd) acc[e] = fmaf(a.part_o[pz * hd + d], wz, acc[e]);
-      }
+    for (int o = LANES / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const float inv = l == 0.f ? 0.f : 1.0f / (a.sink ? l + exp2f(sv - m) : l);
+#pragma unroll
+    for (int x = 0; x < MG_ROWS; x++) {
+      const float f = __shfl_sync(0xffffffffu, inv, x * LANES);
+      const bool none = __shfl_sync(0xffffffffu, l, x * LANES) == 0.f;
+      if (r + x >= item.pairs) continue;
+      T* const to = place(r + x);
+#pragma unroll
+      for (int e = 0; e < NV; e++)
+#pragma unroll
+        for (int q = 0; q < VEC; q++) {
+          const int d = (lane + 32 * e) * VEC + q;
+          if (d < hd) to[d] = from_f32<T>(none ? 0.f : acc[x][e][q] * f);
+        }
     }
   }
-  l = warp_sum(l);
-  const float total = a.sink ? l + exp2f(sv - m) : l;
-  const float inv = l == 0.f ? 0.f : 1.0f / total;
-  T* const to = reinterpret_cast<T*>(a.out) + (size_t)t * a.out_ld + (size_t)h * hd;
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-    const int d = lane + 32 * e;
-    if (d < hd) to[d] = from_f32<T>(l == 0.f ? 0.f : acc[e] * inv);
-  }
+}
+
+template <typename T> void run_merge(const TreeArgs& a, cudaStream_t stream) {
+  auto* const k = a.hd % 4 != 0 ? tree_merge_kernel<T, 1, 8> : a.hd <= 128 ? tree_merge_kernel<T, 4, 1> : tree_merge_kernel<T, 4, 2>;
+  const long long rows = (long long)a.T * a.H, most = 148 * 4;           // a block a row at most, four to an SM
+  tlc_launch(k, dim3((unsigned)(rows < most ? rows : most)), dim3(MG_T), 0, stream, a);
 }
 
 template <typename T, int RM> int run_simt(const TreeArgs& a, cudaStream_t stream) {
@@ -312,13 +455,14 @@ Cut cut_of(int dtype, int aligned, int n_pages, int B, int T, int H, int KV, int
   Cut c;
   const int G = H / KV;
   c.tc = tlc_tree_attention_tc_takes(dtype, aligned, H, KV, hd, n_pages);
-  c.rows = c.tc ? 128 : (long long)max_new * G > 16 ? 64 : 16;
-  c.tile_rows = c.tc ? 128 / G * G : c.rows;
+  c.rows = c.tc ? 256 : (long long)max_new * G > 16 ? 64 : 16;
+  c.tile_rows = c.tc ? 128 / G * G * 2 : c.rows;
   const long long kt = ((long long)max_context + BN - 1) / BN + (max_new + BN - 1) / BN;
   c.units = (((long long)T * G + c.tile_rows - 1) / c.tile_rows + B) * KV * kt;
   const long long wave = (long long)sms * (c.tc ? 1 : 2);
   c.blocks = (int)(c.units < wave ? (c.units < 1 ? 1 : c.units) : wave);
-  c.scratch = (long long)c.blocks * 2 * c.rows * (hd + 2) * 4 + (2ll * B + 1) * 4;
+  if (c.blocks > MG_MOST) c.blocks = MG_MOST;
+  c.scratch = (long long)c.blocks * (2 * c.rows * (hd + 2) * 4 + (long long)sizeof(TreeSplit));
   return c;
 }
 }  // namespace
@@ -354,9 +498,9 @@ extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void
   a.part_rows = c.rows;
   a.part_o = (float*)scratch;
   a.part_ml = a.part_o + (size_t)c.blocks * 2 * c.rows * hd;
-  a.plan = (int*)(a.part_ml + (size_t)c.blocks * 2 * c.rows * 2);
+  a.splits = (TreeSplit*)(a.part_ml + (size_t)c.blocks * 2 * c.rows * 2);
   if (const int rc = c.tc ? tlc_tree_attention_tc(a, stream) : tlc_tree_attention_simt(a, dtype, c.rows, stream)) return rc;
-  TLC_DISPATCH_DTYPE(dtype, E, tlc_launch(tree_merge_kernel<E>, dim3(T, (H + 3) / 4), dim3(128), 0, stream, a));
+  TLC_DISPATCH_DTYPE(dtype, E, run_merge<E>(a, stream));
   TLC_CHECK_LAUNCH("tree_attention(merge)");
   return 0;
 }

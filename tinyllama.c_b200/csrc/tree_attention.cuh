@@ -2,6 +2,13 @@
 #pragma once
 #include "common.cuh"
 
+// What block c leaves for the kernel that adds up partial results: an item whose segments are those of blocks c0 .. c0 + n - 1 (n 0: none).
+struct TreeSplit {
+  int n, c0, slot0;                                       // slot0: where block c0's is (the others' are in slot 0)
+  int t0, r0, pairs, g;                                   // the request's first row, the item's first pair of it, how many, the key/value head
+  int pad;
+};
+
 struct TreeArgs {
   const void *q, *k_new, *v_new, *k_pages, *v_pages;      // [T, H * hd], [T, KV * hd] twice, [n_pages, KV, 64, hd] twice
   int ld_q, ld_k, ld_v, n_pages;                          // row strides in elements
@@ -19,7 +26,7 @@ struct TreeArgs {
   int blocks;
   float *part_o, *part_ml;                                // [blocks, 2, most rows of a tile, hd] and the same with 2 for hd
   int part_rows;                                          // most rows of a tile
-  int* plan;                                              // [B + 1] units before each request, [B] key tiles of each
+  struct TreeSplit* splits;                               // [blocks]
 };
 
 // A request: its rows, how much of its context there is to see, and in how many units of work (one key/value head, one tile of
@@ -42,52 +49,124 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
   return s;
 }
 
-// Units are numbered request by request, within it key/value head by head, tile by tile of rows, and tile by tile of keys; block c of n takes
-// [c W / n, (c + 1) W / n) of all W (n at most W): every block the same work, however unequal the requests are, and the tiles of keys of one (request, head, row
-// tile) - an item - lie in consecutive blocks.  What a block has of an item is a segment.  The item that a block begins with may have
-// started in an earlier block and the one it ends with may go on in a later one: these segments' sums are left in part_o (slot 0 for the first
-// segment, 1 for the last), and another kernel adds them up.
-__device__ __forceinline__ int tree_blocks(long long W, int n) { return (int)(W < n ? W : n); }      // fewer units than blocks: one each, and the rest none
-__device__ __forceinline__ long long tree_first(long long W, int c, int n) { return c * W / n; }
-__device__ __forceinline__ int tree_block_of(long long W, long long u, int n) { return (int)(((u + 1) * n - 1) / W); }
+// Units are numbered request by request, within it key/value head by head, tile by tile of rows, and tile by tile of keys; the tiles of keys of one
+// (request, head, row tile) are an item, what a block has of an item is a segment.  Segments whose item other blocks share leave their sums in
+// part_o, and another kernel adds them up.  Two ways to give the n blocks their work:
+//   * items in equal pieces of at most P units, a piece a block, with the smallest P for which the pieces are at most n;
+//   * where that P is more than SLACK above the mean W / n (many items, of unequal lengths): block c takes the next W / n units, whatever
+//     they belong to; the item that it begins with may have started in an earlier block and the one it ends with may go on in a
+//     later one (part_o has a slot for each).
+// A second segment costs a block about what SLACK units do (its queries, the products' way in, its sums: 16 requests of 150 to 6,000 keys in
+// pieces 35 us, in equal shares 50).
+constexpr int TREE_SLACK = 4, TREE_MOST_SEQS = 2048;      // requests whose pieces are looked at
 
-// All threads of a block of NT call it: which request the first unit of block c is in, and which of that request's it is.
-// count: how many units the block takes.  Block 0 leaves the plan that the merging kernel reads.
-template <int NT> __device__ __forceinline__ void tree_plan(const TreeArgs& a, int c, int* at_seq, int* at_unit, long long* count) {
-  __shared__ long long red[NT / 32 + 1];
-  __shared__ int s_seq, s_unit;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int each = (a.B + NT - 1) / NT, b0 = min(a.B, tid * each), b1 = min(a.B, b0 + each);
-  long long mine = 0;
-  for (int b = b0; b < b1; b++) mine += tree_seq(a, b).units;
-  long long x = mine;
+struct TreeShare {
+  int n, per, more;
+  __device__ __forceinline__ TreeShare(int W, int blocks) : n(min(W, blocks)), per(n > 0 ? W / n : 0), more(n > 0 ? W % n : 0) {}
+  __device__ __forceinline__ int first(int c) const { return c * per + min(c, more); }
+  __device__ __forceinline__ int block_of(int u) const { return u < more * (per + 1) ? u / (per + 1) : more + (u - more * (per + 1)) / per; }
+};
+
+struct TreeTake {
+  int b, unit, todo;                                      // the block begins with unit `unit` of request b and takes `todo` units
+  TreeSeq s;                                              // request b
+};
+
+template <int NT> __device__ __forceinline__ int tree_before(int mine, int* red) {     // the sum over the threads before; red: NT / 32 ints
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
-  if (tid == 0) s_seq = -1;
   if (lane == 31) red[warp] = x;
   __syncthreads();
-  long long before = x - mine, W = 0;
+  int before = x - mine;
 #pragma unroll
-  for (int w = 0; w < NT / 32; w++) {
+  for (int w = 0; w < NT / 32; w++)
     if (w < warp) before += red[w];
-    W += red[w];
-  }
-  const int n = tree_blocks(W, a.blocks);
-  const long long first = c < n ? tree_first(W, c, n) : -1;
+  return before;
+}
+
+// All threads of a block of NT call it.  room: 2 * min(B, TREE_MOST_SEQS) ints of shared memory.  Leaves block c's entry of splits.
+template <int NT> __device__ __forceinline__ TreeTake tree_plan(const TreeArgs& a, int c, int* room) {
+  __shared__ int red_w[NT / 32], red_i[NT / 32], red_b[NT / 32], s_piece;
+  __shared__ TreeTake s_take;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int each = (a.B + NT - 1) / NT, b0 = min(a.B, tid * each), b1 = min(a.B, b0 + each);
+  const bool look = a.B <= TREE_MOST_SEQS;
+  TreeSeq s = {};
+  int units = 0, items = 0;
   for (int b = b0; b < b1; b++) {
-    const TreeSeq s = tree_seq(a, b);
-    if (first >= before && first < before + s.units) { s_seq = b; s_unit = (int)(first - before); }
-    if (c == 0) { a.plan[b] = (int)before; a.plan[a.B + 1 + b] = s.key_tiles; }
-    before += s.units;
+    s = tree_seq(a, b);
+    units += s.units;
+    items += a.KV * s.row_tiles;
+    if (look) { room[2 * b] = a.KV * s.row_tiles; room[2 * b + 1] = s.key_tiles; }
   }
-  if (c == 0 && tid == 0) a.plan[a.B] = (int)W;
+  const int w_sum = __reduce_add_sync(0xffffffffu, units), i_sum = __reduce_add_sync(0xffffffffu, items);
+  if (lane == 0) { red_w[warp] = w_sum; red_i[warp] = i_sum; }
+  if (tid == 0) s_take.todo = 0;
   __syncthreads();
-  *at_seq = s_seq;
-  *at_unit = s_unit;
-  *count = c < n ? tree_first(W, c + 1, n) - first : 0;
+  int W = 0, I = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; w++) { W += red_w[w]; I += red_i[w]; }
+  const TreeShare share(W, a.blocks);
+  if (warp == 0) {
+    int piece = 0;
+    if (look && I <= a.blocks && W > 0) {
+      const int mean = (W + a.blocks - 1) / a.blocks;
+      for (int p = mean; p <= mean + TREE_SLACK && piece == 0; p++) {
+        int n = 0;
+        for (int b = lane; b < a.B; b += 32) n += room[2 * b] * ((room[2 * b + 1] + p - 1) / p);
+        if ((int)__reduce_add_sync(0xffffffffu, n) <= a.blocks) piece = p;
+      }
+    }
+    if (lane == 0) s_piece = piece;
+  }
+  __syncthreads();
+  const int piece = s_piece;
+  TreeSplit split = {};
+  if (piece > 0) {
+    int mine = 0;
+    for (int b = b0; b < b1; b++) mine += room[2 * b] * ((room[2 * b + 1] + piece - 1) / piece);
+    int before = tree_before<NT>(mine, red_b);
+    for (int b = b0; b < b1; b++) {
+      const int n = (room[2 * b + 1] + piece - 1) / piece, here = room[2 * b] * n;
+      if (c >= before && c < before + here) {
+        if (each > 1) s = tree_seq(a, b);
+        const int item = (c - before) / n, k = (c - before) % n, lo = k * s.key_tiles / n;
+        s_take = TreeTake{b, item * s.key_tiles + lo, (k + 1) * s.key_tiles / n - lo, s};
+        if (k == 0 && n > 1) {
+          const int g = item / s.row_tiles, r0 = item % s.row_tiles * a.tile_rows;
+          split = TreeSplit{n, c, 0, s.t0, r0, min(a.tile_rows, s.n * (a.H / a.KV) - r0), g, 0};
+        }
+        a.splits[c] = split;
+      }
+      before += here;
+    }
+  } else {
+    int before = tree_before<NT>(units, red_b);
+    const int first = c < share.n ? share.first(c) : -1;
+    for (int b = b0; b < b1; b++) {
+      if (each > 1) s = tree_seq(a, b);
+      if (first >= before && first < before + s.units) {
+        const int unit = first - before, tile = unit % s.key_tiles, u0 = first - tile;
+        s_take = TreeTake{b, unit, share.first(c + 1) - first, s};
+        if (tile > 0 && share.block_of(u0) == c - 1) {
+          const int item = unit / s.key_tiles, g = item / s.row_tiles, r0 = item % s.row_tiles * a.tile_rows;
+          split = TreeSplit{share.block_of(u0 + s.key_tiles - 1) - c + 2, c - 1, share.first(c - 1) < u0 ? 1 : 0, s.t0, r0,
+                            min(a.tile_rows, s.n * (a.H / a.KV) - r0), g, 0};
+        }
+        a.splits[c] = split;
+      }
+      before += s.units;
+    }
+  }
+  __syncthreads();
+  const TreeTake take = s_take;
+  if (take.todo == 0 && tid == 0) a.splits[c] = TreeSplit{};             // nothing to do
+  return take;
 }
 
 // Whether the draft's row i (position pos) sees draft j (position pos_j).

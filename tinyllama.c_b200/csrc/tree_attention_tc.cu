@@ -1,16 +1,18 @@
 // Attention of drafted tokens on the 5th-generation tensor cores (sm_100a): bfloat16, heads of 64 and 128.
 //
 // The mathematics is tree_attention.cu's.  A tile is 128 pairs of a drafted row and one of the G query heads that share a key/value head,
-// 128 / G rows with all of their heads, so that a key tile is fetched once for all of them: pairs a key/value head x 2 operations
-// per byte of keys and values, HBM bound up to some 250 pairs (measured peaks, 1,648 TFLOP/s over 6,553 GB/s), tensor bound above.
-// Queries come by TMA as a box of {64 columns, G heads, 128 / G rows}, key tiles as boxes of 64 rows from the pages, or, the drafts', from
-// the projections' own rows.  The walk over the key tiles is the one of the prompts' kernel (attention_prefill_tc.cu): an agent warp each
-// for copies, S = Q K^T and O += P V, and two groups of four worker warps, a thread a row, that take every second key tile with
-// a score buffer, a P buffer and an output accumulator of their own.
-// What is different: a block takes an equal share of all requests' key tiles (see tree_attention.cuh) instead of a tile and a head; keys
-// are masked by a bit per (row, draft); and values that some row of the tile does not see are looked over first, since 0 x NaN is
-// NaN on the tensor cores: rows past the keys' end become zeros, and a value that is no number becomes 0 and is added, at the end, to
-// the rows that do see it.
+// 128 / G rows with all of their heads, and a block takes two such tiles with every key tile that it fetches: 2 operations a pair and
+// byte of keys and values, so it is bound by HBM up to some 250 pairs (measured peaks, 1,648 TFLOP/s over 6,553 GB/s).
+// Queries come by TMA as boxes of {64 columns, G heads, 128 / G rows}, key tiles as boxes of 64 rows from the pages or, the drafts', from
+// the projections' own rows.  One agent warp each starts the copies, issues S = Q K^T (M 128, N 64, K hd; operands as in the prompts'
+// kernel, attention_prefill_tc.cu) and O += P V (M 128, N hd, K 64; V an MN-major operand); one for both products was half as quick.  Two groups of four worker warps have a score
+// buffer, two buffers of weights and an output accumulator each, all in tensor memory (a thread a row): they take one row tile each, or, of a
+// request with one row tile, every second key tile; either way products alternate between the groups, and step u is group u % 2's.
+// The weights P = 2^(s - m) go to the second product from tensor memory too, which
+// leaves shared memory to four key and six value tiles on their way (160 KB: HBM's latency at a block's share of its bandwidth is some 70 KB).
+// A block takes an equal share of all requests' key tiles (see tree_attention.cuh); keys are masked by a bit per (row, draft); and values that some
+// row of the tile does not see are looked over first, since 0 x NaN is NaN on the tensor cores: rows past the keys' end become
+// zeros, and a value that is no number becomes 0 and is added, at the end, to the rows that do see it.
 // Every wait on an mbarrier is bounded (codes 61-69 of the error word), as in the prompts' kernel.
 #include "tree_attention.cuh"
 #include "mbarrier.cuh"
@@ -22,7 +24,7 @@ int tlc_tensor_map_bf16_nd(const void* p, int rank, const unsigned long long* di
 namespace {
 
 constexpr int BM = 128, BN = TLC_PAGE;
-constexpr int KS = 4, VS = 3;            // stages of the K and V rings
+constexpr int KS = 4, VS = 6;            // stages of the K and V rings: scores are made two tiles ahead, so keys leave earlier
 constexpr int WORKERS = 256, THREADS = WORKERS + 96, NG = 2;
 constexpr float TAU = 8.0f;              // how far (in powers of two) a row's maximum may run ahead of its reference
 constexpr float LOG2E = 1.4426950408889634f;
@@ -36,6 +38,19 @@ __device__ __forceinline__ float ex2_quick(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+// two 32-bit operations at a time
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
   asm volatile(
@@ -51,17 +66,27 @@ __device__ __forceinline__ bool make_finite(uint32_t& w) {
   return odd;
 }
 
+// D += A B with A (128 rows, 16 columns of 16-bit values, two to a 32-bit column) in tensor memory
+__device__ __forceinline__ void umma_a_in_tmem(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 template <int HD>
 struct TreeSmem {
-  static constexpr int Q_SLAB = BM * 128, Q = 0, Q_BYTES = (HD / 64) * Q_SLAB;
-  static constexpr int K_SLAB = BN * 128, K_STAGE = (HD / 64) * K_SLAB, K = Q + Q_BYTES;
+  static constexpr int Q_SLAB = BM * 128, Q = 0, Q_TILE = (HD / 64) * Q_SLAB;
+  static constexpr int X = Q;                             // [2][NG][128] floats: the groups' reference maxima and sums, when the queries have been used
+  static constexpr int K_SLAB = BN * 128, K_STAGE = (HD / 64) * K_SLAB, K = Q + 2 * Q_TILE;
   static constexpr int V_STAGE = HD * 128, V = K + KS * K_STAGE;
-  static constexpr int P_BUF = BM * 128, P = V + VS * V_STAGE;
-  static constexpr int X = P + 2 * P_BUF;                 // [2][NG][128] floats: the groups' reference maxima and sums, at the end
-  static constexpr int BARS = X + 2 * NG * BM * 4;        // mbarriers, tmem slot, dead flag
-  static constexpr int N_BARS = 1 + 2 * KS + 2 * VS + 8;
+  static constexpr int BARS = V + VS * V_STAGE;           // mbarriers, tmem slot, dead flag
+  static constexpr int N_BARS = 1 + 2 * KS + 2 * VS + 12;
   static constexpr int TOTAL = BARS + N_BARS * 8 + 16 + 1024;
 };
+static_assert(TreeSmem<128>::TOTAL <= 227 * 1024 - 512, "shared memory of a block");
 
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -69,9 +94,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kn,
                          const __grid_constant__ CUtensorMap map_vn, TreeArgs a, float cap_in, float cap_out, ErrWords* err) {
   asm volatile("griddepcontrol.launch_dependents;");
-  tlc_wait(a.v_new, a.v_pages, a.block_table, a.slots, a.start, a.cu, a.positions, a.mask, a.out, a.part_o, a.part_ml, a.plan);
   using L_ = TreeSmem<HD>;
-  constexpr int TCOLS = HD == 128 ? 512 : 256;            // the groups' scores at 0 and 64, their outputs at 128 and 128 + hd
+  constexpr uint32_t T_O = 2 * BN, T_P = T_O + 2 * HD, TCOLS = 512;     // tensor memory: the groups' scores, outputs, weights (BN / 2 columns a buffer)
+  static_assert(T_P + 2 * BN <= TCOLS, "tensor memory");
   extern __shared__ uint8_t tree_tc_raw[];
   uint8_t* sm = (uint8_t*)(((uintptr_t)tree_tc_raw + 1023) & ~(uintptr_t)1023);
   float* xch = reinterpret_cast<float*>(sm + L_::X);
@@ -87,15 +112,28 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   auto v_empty = [&](int s) { return smem_u32(bars + 1 + 2 * KS + VS + s); };
   auto s_full = [&](int i) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + i); };
   auto s_free = [&](int i) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + 2 + i); };
-  auto p_ready = [&](int i) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + 4 + i); };
-  auto pv_done = [&](int i) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + 6 + i); };
+  auto p_ready = [&](int w, int buffer) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + 4 + 2 * w + buffer); };
+  auto pv_done = [&](int w, int buffer) { return smem_u32(bars + 1 + 2 * KS + 2 * VS + 8 + 2 * w + buffer); };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long wait_limit = mbar_wait_limit(err);
   if (tid == 0) *dead = 0;
-  int b, unit;
-  long long todo;
-  tree_plan<THREADS>(a, blockIdx.x, &b, &unit, &todo);
+  if (warp == 8 && lane < 5) {
+    const CUtensorMap* const m = lane == 0 ? &map_q : lane == 1 ? &map_k : lane == 2 ? &map_v : lane == 3 ? &map_kn : &map_vn;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+  }
+  tlc_wait(a.v_new, a.v_pages, a.block_table, a.slots, a.start, a.cu, a.positions, a.mask, a.out, a.part_o, a.part_ml, a.splits);
+  if (warp == 9) {                                        // every worker warp arrives once on s_free and p_ready, one agent on the rest
+    for (int i = lane; i < L_::N_BARS; i += 32) {
+      const int own = i - (1 + 2 * KS + 2 * VS);
+      mbar_init(bar_q + 8 * i, own >= 2 && own < 8 ? 4 : 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  const TreeTake take = tree_plan<THREADS>(a, blockIdx.x, reinterpret_cast<int*>(sm));
+  int b = take.b, unit = take.unit, todo = take.todo;
+  TreeSeq s = take.s;
   if (todo == 0) return;
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TCOLS)
@@ -107,29 +145,27 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   auto wait = [&](uint32_t bar, uint32_t parity, int code) {
-    if (*dead) return;
+    if (mbar_try(bar, parity) || *dead) return;
     if (!mbar_wait(bar, parity, err, code, wait_limit)) *dead = 1;
   };
-  const int G = a.H / a.KV, NI = BM / G;                  // rows of a tile
+  const int G = a.H / a.KV, NI = BM / G;                  // drafted rows of a tile
   const float scale_log2 = a.scale * LOG2E;
+  // Barriers are made once: what each agent counts goes on from segment to segment.  done: key tiles of earlier segments; used0, used1:
+  // how often a group's buffers have been used in them.
+  int done = 0, used0 = 0, used1 = 0, segment = 0;
 #pragma unroll 1
-  for (bool first_segment = true; todo > 0; first_segment = false) {
-  TreeSeq s = tree_seq(a, b);
+  for (; todo > 0; segment++) {
+  const bool first_segment = segment == 0;
   while (unit >= s.units) { unit -= s.units; s = tree_seq(a, ++b); }
   const int item = unit / s.key_tiles, kt0 = unit % s.key_tiles;
-  const int g = item / s.row_tiles, i0 = item % s.row_tiles * NI;
-  const int n = (int)min((long long)(s.key_tiles - kt0), todo);        // key tiles of this segment
-  const int rows = min(NI, s.n - i0);
+  const int g = item / s.row_tiles, i0 = item % s.row_tiles * 2 * NI;
+  const int n = min(s.key_tiles - kt0, todo);             // key tiles of this segment
+  const int rows = min(2 * NI, s.n - i0);
+  const bool pair = rows > NI;                            // two row tiles: a group each; else every second key tile for each group
   if (tid == 0) {
     s_last_pos = 0;
     s_odd = 0;
-    for (int i = 0; i < L_::N_BARS; i++) {
-      const uint32_t bar = bar_q + 8 * i;               // every worker warp arrives once on s_free and p_ready, one agent on the rest
-      if (!first_segment) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");   // nothing is pending on it (see the loader's last waits)
-      mbar_init(bar, (bar == s_free(0) || bar == s_free(1) || bar == p_ready(0) || bar == p_ready(1)) ? 4 : 1);
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // (the queries' memory has held statistics and results)
   }
   __syncthreads();
   if (a.window > 0) {
@@ -144,8 +180,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (role == 0) {
       // the copies: the warp reads 32 entries of the block table at a time, its first lane starts the copies
       if (lane == 0) {
-        mbar_expect_tx(bar_q, (HD / 64) * NI * G * 128);
-        for (int c = 0; c < HD / 64; c++) tma_load_3d(sm0 + L_::Q + c * L_::Q_SLAB, &map_q, bar_q, 64 * c, g * G, s.t0 + i0);
+        mbar_expect_tx(bar_q, (pair ? 2 : 1) * (HD / 64) * NI * G * 128);
+        for (int w = 0; w < (pair ? 2 : 1); w++)
+          for (int c = 0; c < HD / 64; c++) tma_load_3d(sm0 + L_::Q + w * L_::Q_TILE + c * L_::Q_SLAB, &map_q, bar_q, 64 * c, g * G, s.t0 + i0 + w * NI);
       }
       const int* table = a.block_table + (size_t)(s.context_tiles > 0 ? a.slots[b] : 0) * a.max_pages;
       int entry = 0;
@@ -157,8 +194,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         // (a page that is none: behind the map's last row, which reads as zeros)
         const int row = draft ? s.t0 + (kt - s.context_tiles) * BN : ((page >= 0 && page < a.n_pages ? page * a.KV + g : a.n_pages * a.KV)) * BN;
         {
-          const int st = t % KS;
-          if (t >= KS) wait(k_empty(st), (uint32_t)(((t - KS) / KS) & 1), 66);       // S of tile t - KS is done
+          const int st = (done + t) % KS;
+          if (done + t >= KS) wait(k_empty(st), (uint32_t)(((done + t) / KS - 1) & 1), 66);       // S of the tile KS before is done
           if (lane == 0) {
             mbar_expect_tx(k_full(st), L_::K_STAGE);
             for (int c = 0; c < HD / 64; c++)
@@ -166,8 +203,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
         }
         {
-          const int st = t % VS;
-          if (t >= VS) wait(v_empty(st), (uint32_t)(((t - VS) / VS) & 1), 67);       // P V of tile t - VS is done
+          const int st = (done + t) % VS;
+          if (done + t >= VS) wait(v_empty(st), (uint32_t)(((done + t) / VS - 1) & 1), 67);       // P V of the tile VS before is done
           if (lane == 0) {
             mbar_expect_tx(v_full(st), L_::V_STAGE);
             for (int c = 0; c < HD / 64; c++)
@@ -177,44 +214,45 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         __syncwarp();
       }
       // the last arrivals on the stages' barriers (the products' commits), which nothing else waits for: after
-      // them no barrier of this segment has anything pending, and the next one may make them anew
-      for (int t = max(0, n - KS); t < n; t++) wait(k_empty(t % KS), (uint32_t)((t / KS) & 1), 66);
-      for (int t = max(0, n - VS); t < n; t++) wait(v_empty(t % VS), (uint32_t)((t / VS) & 1), 67);
-    } else if (lane == 0 && role == 1) {
-      // the scores run two tiles ahead of the workers: both score buffers are in use from the start
-      constexpr uint32_t idesc_s = instr_desc(BM, BN);
-      const uint32_t q_lo = desc_lo(sm0 + L_::Q);
-      wait(bar_q, 0, 61);
-      for (int t = 0; t < n; t++) {
-        const int st = t % KS;
-        wait(k_full(st), (uint32_t)((t / KS) & 1), 62);
-        if (t >= 2) wait(s_free(t & 1), (uint32_t)(((t - 2) >> 1) & 1), 63);         // the workers hold scores t - 2 in registers
+      // them the segment's products are done and no barrier has anything pending
+      for (int t = max(0, n - KS); t < n; t++) wait(k_empty((done + t) % KS), (uint32_t)(((done + t) / KS) & 1), 66);
+      for (int t = max(0, n - VS); t < n; t++) wait(v_empty((done + t) % VS), (uint32_t)(((done + t) / VS) & 1), 67);
+    } else if (lane == 0) {
+      constexpr uint32_t idesc_s = instr_desc(BM, BN), idesc_o = instr_desc(BM, HD) | (1u << 16);             // V is MN-major: hd runs along its rows
+      const int steps = pair ? 2 * n : n;                 // step u: group u % 2, key tile u / 2 of a pair, else u
+      auto scores = [&](int u) {
+        const int w = u & 1, tile = done + (pair ? u >> 1 : u), st = tile % KS, all = (u >> 1) + (w ? used1 : used0);
+        if (!pair || w == 0) wait(k_full(st), (uint32_t)((tile / KS) & 1), 62);
+        if (all > 0) wait(s_free(w), (uint32_t)((all - 1) & 1), 63);                 // the workers hold the scores before in registers
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t d = tmem + (uint32_t)((t & 1) * BN);
-        const uint32_t k_lo = desc_lo(sm0 + L_::K + st * L_::K_STAGE);
+        const uint32_t q_lo = desc_lo(sm0 + L_::Q + (pair ? w * L_::Q_TILE : 0)), k_lo = desc_lo(sm0 + L_::K + st * L_::K_STAGE);
 #pragma unroll
         for (int c = 0; c < HD / 64; c++)
 #pragma unroll
           for (int kk = 0; kk < 4; kk++)
-            umma_halves(d, q_lo + (uint32_t)((c * L_::Q_SLAB + kk * 32) >> 4), k_lo + (uint32_t)((c * L_::K_SLAB + kk * 32) >> 4),
+            umma_halves(tmem + (uint32_t)(w * BN), q_lo + (uint32_t)((c * L_::Q_SLAB + kk * 32) >> 4), k_lo + (uint32_t)((c * L_::K_SLAB + kk * 32) >> 4),
                         DESC_HI, idesc_s, (c > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(s_full(t & 1));
-        umma_commit(k_empty(st));
-      }
-    } else if (lane == 0 && role == 2) {
-      constexpr uint32_t idesc_o = instr_desc(BM, HD) | (1u << 16);                   // V is MN-major: hd runs along its rows
-      for (int j = 0; j < n; j++) {
-        const int st = j % VS;
-        wait(v_full(st), (uint32_t)((j / VS) & 1), 65);
-        wait(p_ready(j & 1), (uint32_t)((j >> 1) & 1), 64);                          // P of tile j is in shared memory
+        umma_commit(s_full(w));
+        if (!pair || w == 1) umma_commit(k_empty(st));
+      };
+      if (role == 1) {
+        wait(bar_q, (uint32_t)(segment & 1), 61);
+#pragma unroll 1
+        for (int u = 0; u < steps; u++) scores(u);
+      } else
+#pragma unroll 1
+      for (int u = 0; u < steps; u++) {
+        const int w = u & 1, tile = done + (pair ? u >> 1 : u), st = tile % VS, use = u >> 1, all = use + (w ? used1 : used0);
+        if (!pair || w == 0) wait(v_full(st), (uint32_t)((tile / VS) & 1), 65);
+        wait(p_ready(w, all & 1), (uint32_t)(all / 2 & 1), 64);                                   // the step's weights are in tensor memory
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t p_lo = desc_lo(sm0 + L_::P + (j & 1) * L_::P_BUF), v_lo = (desc_lo(sm0 + L_::V + st * L_::V_STAGE) & 0xFFFFu) | ((uint32_t)(L_::K_SLAB >> 4) << 16);
+        const uint32_t v_lo = (desc_lo(sm0 + L_::V + st * L_::V_STAGE) & 0xFFFFu) | ((uint32_t)(L_::K_SLAB >> 4) << 16);
 #pragma unroll
         for (int kk = 0; kk < 4; kk++)
-          umma_halves(tmem + 128u + (uint32_t)((j & 1) * HD), p_lo + (uint32_t)(kk * 2), v_lo + (uint32_t)(kk * (16 * 128 >> 4)), DESC_HI, idesc_o,
-                      (j >= 2 || kk > 0) ? 1u : 0u);
-        umma_commit(pv_done(j & 1));
-        umma_commit(v_empty(st));
+          umma_a_in_tmem(tmem + T_O + (uint32_t)(w * HD), tmem + T_P + (uint32_t)((2 * w + (all & 1)) * (BN / 2) + kk * 8), v_lo + (uint32_t)(kk * (16 * 128 >> 4)), DESC_HI,
+                         idesc_o, (use > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(pv_done(w, all & 1));
+        if (!pair || w == 1) umma_commit(v_empty(st));
       }
     }
     __syncwarp();
@@ -223,16 +261,18 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // key tile and its row of the group's output. ----
     const int wg = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const int i = i0 + r / G;                             // the row among the request's drafts
-    const bool live = r < rows * G;
+    const int first_row = i0 + (pair ? wg * NI : 0), i = first_row + r / G;            // the row among the request's drafts
+    const int live_rows = min(NI, s.n - first_row) * G;
+    const bool live = r < live_rows;
     const int t = s.t0 + (live ? i : 0);
     const int lo_r = a.window > 0 ? a.positions[t] - a.window + 1 : 0;                 // the first position it sees
     const int lo_most = a.window > 0 ? s_last_pos - a.window + 1 : 0;
     const uint32_t s_at = tmem + lanes + (uint32_t)(wg * BN);
-    const uint32_t o_at = tmem + lanes + 128u + (uint32_t)(wg * HD);
+    const uint32_t o_at = tmem + lanes + T_O + (uint32_t)(wg * HD), p_at = tmem + lanes + T_P + (uint32_t)(wg * BN);
     float m_ref = -INFINITY, l = 0.f;                     // the maximum the numerators refer to (scaled, log2), the sum
-    int mine = 0;                                         // tiles this group has done
-    for (int j = wg; j < n; j += NG, mine++) {
+    int mine = 0;                                         // tiles this group has done, and in earlier segments
+    const int used = wg ? used1 : used0;
+    for (int j = pair ? 0 : wg; j < n; j += pair ? 1 : NG, mine++) {
       const bool draft = kt0 + j >= s.context_tiles;
       const int base = draft ? (kt0 + j - s.context_tiles) * BN : (s.first_tile + kt0 + j) * BN;      // a draft's index, or a position
       const int keys = (draft ? s.n : s.context) - base;
@@ -265,7 +305,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       if (!live) seen_lo = seen_hi = 0u;
       uint32_t sr[64];
-      wait(s_full(wg), (uint32_t)(mine & 1), 68);
+      wait(s_full(wg), (uint32_t)((used + mine) & 1), 68);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       __syncwarp();
       tmem_ld32_nowait(s_at, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
@@ -273,7 +313,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(s_free(wg));             // the scores are in registers: the buffer may take tile j + 2
+      if (lane == 0) mbar_arrive(s_free(wg));             // the scores are in registers: the buffer may take the next
+      const int all = used + mine;
+      const bool p_free = all < 2 || mbar_try(pv_done(wg, all & 1), (uint32_t)((all / 2 - 1) & 1));       // the weights of two steps before have been used
       if (cap_in > 0.f) {
         // a capped score: s <- cap tanh(s scale / cap), left divided by the scale (what follows multiplies by it);
         // tanh(x) = 1 - 2 / (e^(2x) + 1), cap_in = 2 log2(e) scale / cap, cap_out = cap / scale
@@ -288,10 +330,10 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (int c = 0; c < 64; c++)
           if (!((c < 32 ? seen_lo >> c : seen_hi >> (c - 32)) & 1u)) sr[c] = 0xff800000u;     // -inf
       }
-      float mx = -INFINITY;
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 64; c++) mx = fmaxf(mx, __uint_as_float(sr[c]));
-      mx *= scale_log2;
+      for (int c = 0; c < 64; c++) mx4[c % 4] = fmaxf(mx4[c % 4], __uint_as_float(sr[c]));
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
       // the reference maximum moves only when the true one has run ahead of it by more than 2^TAU
       const bool grow = mx > m_ref + TAU || (m_ref == -INFINITY && mx > -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {
@@ -302,7 +344,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           l *= factor;
         }
         if (mine > 0) {
-          wait(pv_done(wg), (uint32_t)((mine - 1) & 1), 69);                          // every product into this output so far is done
+          wait(pv_done(wg, (all - 1) & 1), (uint32_t)((all - 1) / 2 & 1), 69);        // every product into this output so far is done
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           __syncwarp();
 #pragma unroll 1
@@ -316,25 +358,26 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
       }
       const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
-      float sum = 0.f;
+      float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       uint32_t pk[32];
 #pragma unroll
       for (int c = 0; c < 32; c++) {
-        const float x = ex2_quick(fmaf(__uint_as_float(sr[2 * c]), scale_log2, neg));
-        const float y = ex2_quick(fmaf(__uint_as_float(sr[2 * c + 1]), scale_log2, neg));
-        sum += x + y;
-        pk[c] = pack_bf16(x, y);
+        float2 x = fma2(make_float2(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1])), make_float2(scale_log2, scale_log2), make_float2(neg, neg));
+        x.x = ex2_quick(x.x);
+        x.y = ex2_quick(x.y);
+        sums[c % 2] = add2(sums[c % 2], x);
+        pk[c] = pack_bf16(x.x, x.y);
       }
-      l += sum;
-      if (mine > 0) wait(pv_done(wg), (uint32_t)((mine - 1) & 1), 69);               // the group's P buffer is free
-      uint8_t* prow = sm + L_::P + wg * L_::P_BUF + r * 128;
-#pragma unroll
-      for (int q = 0; q < 8; q++)
-        *reinterpret_cast<uint4*>(prow + ((q ^ (r & 7)) << 4)) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
-      if (edge) {
+      const float2 sum = add2(sums[0], sums[1]);
+      l += sum.x + sum.y;
+      if (!p_free) wait(pv_done(wg, all & 1), (uint32_t)((all / 2 - 1) & 1), 69);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      __syncwarp();
+      tmem_st32(p_at + (uint32_t)((all & 1) * (BN / 2)), pk);
+      if (edge && !(pair && wg == 1)) {                     // (of a pair the first group: both products come after it)
         // the tile's values: rows past the keys' end become zeros, and so does what is no number (it is looked at again at the end)
-        wait(v_full(j % VS), (uint32_t)((j / VS) & 1), 65);
-        uint4* const v = reinterpret_cast<uint4*>(sm + L_::V + (j % VS) * L_::V_STAGE);
+        wait(v_full((done + j) % VS), (uint32_t)(((done + j) / VS) & 1), 65);
+        uint4* const v = reinterpret_cast<uint4*>(sm + L_::V + (done + j) % VS * L_::V_STAGE);
         bool odd = false;
 #pragma unroll
         for (int e = 0; e < HD / 16; e++) {
@@ -347,48 +390,53 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
         }
         if (odd) s_odd = 1;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();                                         // the warp's rows of P are written and fenced
-      if (lane == 0) mbar_arrive(p_ready(wg));
+      if (lane == 0) mbar_arrive(p_ready(wg, all & 1));
     }
-    // ---- the two groups' results meet: O = (O_0 2^(m_0 - m) + O_1 2^(m_1 - m)) / (l_0 2^(m_0 - m) + l_1 2^(m_1 - m)) ----
-    if (mine > 0) wait(pv_done(wg), (uint32_t)((mine - 1) & 1), 69);
-    xch[wg * BM + r] = m_ref;
-    xch[(NG + wg) * BM + r] = l;
+    // ---- the end: a pair's groups have a result each, else the two meet: O = (O_0 2^(m_0 - m) + O_1 2^(m_1 - m)) / (l_0 2^(m_0 - m) + l_1 2^(m_1 - m)) ----
+    if (mine > 0) wait(pv_done(wg, (used + mine - 1) & 1), (uint32_t)((used + mine - 1) / 2 & 1), 69);
+    float m0 = m_ref, m1 = -INFINITY, l0 = l, l1 = 0.f;
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     workers_sync();
+    if (!pair) {                                          // (every product with the queries is done: their memory takes the statistics)
+      xch[wg * BM + r] = m_ref;
+      xch[(NG + wg) * BM + r] = l;
+      workers_sync();
+      m0 = xch[r]; m1 = xch[BM + r]; l0 = xch[NG * BM + r]; l1 = xch[(NG + 1) * BM + r];
+      workers_sync();                                     // (read, before it takes results)
+    }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const bool whole = n == s.key_tiles;                  // else the sums stay unnormalised: another kernel adds the segments
     const int h = g * G + r % G;
     const bool with_sink = a.sink && whole;
     const float sv = with_sink && a.sink_values ? a.sink_values[live ? h : 0] * LOG2E : 0.f;
-    const float m0 = xch[r], m1 = xch[BM + r], l0 = xch[NG * BM + r], l1 = xch[(NG + 1) * BM + r];
     const float m_keys = fmaxf(m0, m1), m_all = with_sink ? fmaxf(m_keys, sv) : m_keys;
     const float w0 = m0 == -INFINITY ? 0.f : ex2_quick(m0 - m_all), w1 = m1 == -INFINITY ? 0.f : ex2_quick(m1 - m_all);
     const float l_keys = l0 * w0 + l1 * w1;
     const bool none = l0 == 0.f && l1 == 0.f;             // it sees nothing
     const float inv = whole ? 1.0f / (l_keys + (with_sink ? ex2_quick(sv - m_all) : 0.f)) : 1.0f;
     const float f0 = w0 * inv, f1 = w1 * inv;
-    const bool has1 = n > 1;                              // the second group had a tile at all (else its accumulator was never written)
-    const size_t part = ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * BM + r;
-    if (!whole && wg == 0 && live) {
+    const bool second = !pair && n > 1;                   // the second group had a tile at all (else its accumulator was never written)
+    const size_t part = ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * (2 * BM) + (pair ? wg * NI * G : 0) + r;
+    if (!whole && live && (pair || wg == 0)) {
       a.part_ml[part * 2] = m_all;
       a.part_ml[part * 2 + 1] = l_keys;
     }
     const bool odd = s_odd != 0;
     __syncwarp();
 #pragma unroll 1
-    for (int c = 0; c < HD / 64; c++) {                   // the group's half of the output columns, 32 at a time
-      const int col = wg * (HD / 2) + 32 * c;
+    for (int c = 0; c < (pair ? HD / 32 : HD / 64); c++) {               // 32 output columns at a time: of a pair all, else the group's half
+      const int col = (pair ? 0 : wg * (HD / 2)) + 32 * c;
       uint32_t o[32];
       float acc[32];
-      tmem_ld32(tmem + lanes + 128u + (uint32_t)col, o);
+      tmem_ld32(tmem + lanes + T_O + (uint32_t)((pair ? wg * HD : 0) + col), o);
 #pragma unroll
       for (int e = 0; e < 32; e++) acc[e] = __uint_as_float(o[e]) * f0;
-      if (has1) {
-        tmem_ld32(tmem + lanes + 128u + (uint32_t)(HD + col), o);
+      if (second) {
+        tmem_ld32(tmem + lanes + T_O + (uint32_t)(HD + col), o);
 #pragma unroll
         for (int e = 0; e < 32; e++) acc[e] = fmaf(__uint_as_float(o[e]), f1, acc[e]);
       }
@@ -425,17 +473,35 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
         }
       }
-      if (!live) continue;
+      // through 4 KB of the queries' memory of the warp's own, pieces of 16 bytes in turned order, so that a store covers whole lines
+      uint8_t* const mem = sm + L_::Q + warp * 4096;
+      __syncwarp();
       if (!whole) {
-        float4* dst = reinterpret_cast<float4*>(a.part_o + part * HD + col);
 #pragma unroll
-        for (int q = 0; q < 8; q++) dst[q] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+        for (int q = 0; q < 8; q++)
+          *reinterpret_cast<float4*>(mem + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+        __syncwarp();
+        const size_t part0 = part - r + 32 * quarter;     // of the warp's first row
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+          const int row = q * 4 + (lane >> 3), piece = lane & 7;
+          const float4 x = *reinterpret_cast<const float4*>(mem + row * 128 + ((piece ^ (row & 7)) << 4));
+          if (32 * quarter + row < live_rows) *reinterpret_cast<float4*>(a.part_o + (part0 + row) * HD + col + 4 * piece) = x;
+        }
       } else {
-        uint4* dst = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (size_t)t * a.out_ld + (size_t)h * HD + col);
 #pragma unroll
         for (int q = 0; q < 4; q++)
-          dst[q] = make_uint4(pack_bf16(acc[8 * q], acc[8 * q + 1]), pack_bf16(acc[8 * q + 2], acc[8 * q + 3]),
-                              pack_bf16(acc[8 * q + 4], acc[8 * q + 5]), pack_bf16(acc[8 * q + 6], acc[8 * q + 7]));
+          *reinterpret_cast<uint4*>(mem + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
+              make_uint4(pack_bf16(acc[8 * q], acc[8 * q + 1]), pack_bf16(acc[8 * q + 2], acc[8 * q + 3]), pack_bf16(acc[8 * q + 4], acc[8 * q + 5]),
+                         pack_bf16(acc[8 * q + 6], acc[8 * q + 7]));
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const int row = q * 8 + (lane >> 2), piece = lane & 3, at = 32 * quarter + row;
+          const uint4 x = *reinterpret_cast<const uint4*>(mem + row * 64 + ((piece ^ (row >> 1 & 3)) << 4));
+          if (at < live_rows)
+            *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (size_t)(s.t0 + first_row + at / G) * a.out_ld + (size_t)(g * G + at % G) * HD + col + 8 * piece) = x;
+        }
       }
     }
   }
@@ -446,6 +512,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   todo -= n;
   unit += n;
+  done += n;
+  used0 += pair ? n : (n + 1) >> 1;
+  used1 += pair ? n : n >> 1;
   }
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TCOLS) : "memory");
