@@ -6,14 +6,14 @@
 //     c_kv = s_k + x_kv - log(sum_u exp x_ku),
 // and the n best of a request's K * V are wanted, equal values by the lowest k * V + v.  Two kernels:
 //   * beam_scan_kernel reads every logit once.  A warp takes a piece of a row, 64 (or 16) values a lane in registers, and leaves the
-//     piece's maximum, its sum of exponentials and its n largest logits in order.  Nothing crosses warps.  Which values can be
-//     among the n largest: those not below the n-th largest of the maxima of 128 groups (four a lane), which a bitwise search by
-//     ballots finds; some n to 2n values pass and are ranked by counting.
-//   * beam_merge_kernel, a block a request, makes the rows' logarithms of sums and takes the n best of all lists the same way.
+//     piece's maximum and its sum of exponentials; nothing crosses warps.
+//   * beam_merge_kernel, a block a request, makes the rows' logarithms of sums.  The n-th largest of the pieces' maxima bounds the n best from below,
+//     so that only the pieces whose maximum reaches it (n to 2 n of hundreds, by a threshold that a few counts find) can hold
+//     any: those are read again, a warp each, and what reaches the threshold is ranked by counting.  (With the n largest of every piece
+//     left by the first kernel it took twice as long: 34 of 66 us went into values that no request wanted.)
 // Bound by HBM for a batch (256 rows of 130,048 logits: 133 MB, 20 us of loads), by the two launches for one request.
-// Arithmetic: sums of exponentials in 32 bits over 16 values at most, from there on, and of the piece's largest values, in
-// 64 bits, as are the logarithm and the values that are compared; two candidates change places only where they are nearer than
-// the 2^-24 or so that this leaves.
+// Arithmetic: exponentials and sums in 32 bits over 16 values at most, the sums of those, the logarithm and the values that are compared in
+// 64 bits: two candidates change places only where they are nearer than the 2^-22 or so that this leaves.
 #include "common.cuh"
 #include <type_traits>
 
@@ -21,11 +21,12 @@ namespace {
 
 constexpr int MAX_N = 64;                // candidates of a request
 constexpr int MAX_BEAMS = 64;
-constexpr int GROUPS = 4;                // groups of a lane's values
-constexpr int CAP = 128;                 // values of a piece that pass the threshold and are ranked side by side
 constexpr int SCAN_WARPS = 4;
-constexpr int MERGE_T = 512, MERGE_CAP = 1024;
-constexpr int MAX_LISTS = 40960;
+constexpr int MERGE_T = 512, MERGE_WARPS = MERGE_T / 32;
+constexpr int MERGE_CAP = 4096;          // values that may reach the threshold; more (of equal values) are taken one after the other
+constexpr int MERGE_RANK = 512;          // and of which so many are ranked side by side, after a second threshold
+constexpr int MERGE_LISTS = 512;         // pieces that reach the threshold and are shared out evenly
+constexpr int MAX_LISTS = 36864;         // pieces of a request: a word of shared memory each
 
 struct Stats { double sum; float max; int pad; };      // of a piece: sum exp(x - max) and max
 
@@ -34,7 +35,6 @@ __device__ __forceinline__ unsigned ordered(float x) {
   const unsigned u = __float_as_uint(x);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-constexpr unsigned ORD_NEG_INF = 0x007fffffu;          // ordered(-infinity)
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -46,124 +46,55 @@ __device__ __forceinline__ bool alive(const float* scores, const unsigned char* 
   return isfinite(scores[row]) && !(ended && ended[row]);
 }
 
-// grid: pieces of all rows, SCAN_WARPS a block.  VPL values a lane; VEC 4: rows start on 16-byte boundaries.
+// A piece's values, VPL a lane: index_of(q) = (q / VEC * 32 + lane) * VEC + q % VEC; -infinity behind the row's end (left: values from
+// the piece's start on).  VEC 4: the row starts on a 16-byte boundary.
+template <int VPL, int VEC>
+__device__ __forceinline__ void load_piece(const float* __restrict__ x, int left, int lane, float (&v)[VPL]) {
+  if (left >= 32 * VPL) {
+#pragma unroll
+    for (int q = 0; q < VPL; q += VEC) {
+      if constexpr (VEC == 4) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(x) + q / 4 * 32 + lane);
+        v[q] = f.x; v[q + 1] = f.y; v[q + 2] = f.z; v[q + 3] = f.w;
+      } else v[q] = __ldcs(x + q * 32 + lane);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < VPL; q++) {
+      const int at = (q / VEC * 32 + lane) * VEC + q % VEC;
+      v[q] = at < left ? __ldcs(x + at) : -INFINITY;
+    }
+  }
+}
+
+// grid: pieces of all rows, SCAN_WARPS a block.
 template <int VPL, int VEC>
 __global__ void __launch_bounds__(SCAN_WARPS * 32)
 beam_scan_kernel(const float* __restrict__ logits, long long ld, const float* __restrict__ scores, const unsigned char* __restrict__ ended,
-                 int rows, int V, int n_pieces, int n, Stats* __restrict__ stats, int2* __restrict__ cand) {
+                 int rows, int V, int n_pieces, Stats* __restrict__ stats) {
   asm volatile("griddepcontrol.launch_dependents;");
-  tlc_wait(logits, scores, ended, stats, cand);
-  __shared__ float2 s_buf[SCAN_WARPS][CAP];
+  tlc_wait(logits, scores, ended, stats);
   const int lane = threadIdx.x & 31;
-  float2* const buf = s_buf[threadIdx.x >> 5];
   const long long piece = (long long)blockIdx.x * SCAN_WARPS + (threadIdx.x >> 5);
-  const int row = (int)(piece / n_pieces), p = (int)(piece % n_pieces);
+  const int row = (int)(piece / n_pieces), base = (int)(piece % n_pieces) * 32 * VPL;
   if (row >= rows || !alive(scores, ended, row)) return;
-  const int base = p * 32 * VPL;
-  const float* const x = logits + (size_t)row * ld + base;
-  const int left = V - base;                           // values of the row from here on
   float v[VPL];
+  load_piece<VPL, VEC>(logits + (size_t)row * ld + base, V - base, lane, v);
+  float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};          // (a NaN is nobody's maximum; it shows in the sum)
 #pragma unroll
-  for (int q = 0; q < VPL; q += VEC) {
-    const int at = (q / VEC * 32 + lane) * VEC;
-    if constexpr (VEC == 4) {
-      if (at + 4 <= left) {
-        const float4 f = __ldcs(reinterpret_cast<const float4*>(x + at));
-        v[q] = f.x; v[q + 1] = f.y; v[q + 2] = f.z; v[q + 3] = f.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[q + e] = at + e < left ? __ldcs(x + at + e) : -INFINITY;
-      }
-    } else v[q] = at < left ? __ldcs(x + at) : -INFINITY;
-  }
-  auto index_of = [&](int q) { return base + (q / VEC * 32 + lane) * VEC + q % VEC; };
-  // the groups' maxima (a NaN is nobody's maximum; it shows in the sum)
-  unsigned key[GROUPS];
-  float m = -INFINITY;
-#pragma unroll
-  for (int g = 0; g < GROUPS; g++) {
-    float a = -INFINITY;
-#pragma unroll
-    for (int q = 0; q < VPL / GROUPS; q++) a = fmaxf(a, v[g * (VPL / GROUPS) + q]);
-    key[g] = ordered(a);
-    m = fmaxf(m, a);
-  }
-  m = warp_max(m);
-  // the n-th largest of the 128 maxima: its bits from the highest down (any threshold that exactly n reach will do)
-  unsigned least = 0;
-  for (int bit = 31; bit >= 0; bit--) {
-    const unsigned trial = least | 1u << bit;
-    int reach = 0;
-#pragma unroll
-    for (int g = 0; g < GROUPS; g++) reach += __popc(__ballot_sync(0xffffffffu, key[g] >= trial));
-    if (reach >= n) least = trial;
-    if (reach == n) break;
-  }
-  least = max(least, ORD_NEG_INF + 1);                 // values of -infinity are nobody's candidates
-  // as a float, larger than every value that does not pass
-  const float bar = __uint_as_float(least & 0x80000000u ? least & 0x7fffffffu : ~least);
-  int count = 0;
-#pragma unroll
-  for (int q = 0; q < VPL; q++) {
-    const bool in = v[q] >= bar;
-    const unsigned who = __ballot_sync(0xffffffffu, in);
-    if (who) {
-      const int at = count + __popc(who & ((1u << lane) - 1));
-      if (in && at < CAP) buf[at] = make_float2(v[q], __int_as_float(index_of(q)));
-      count += __popc(who);
-    }
-  }
-  // sums: the values that did not pass in 32 bits, group by group, the others in 64 (they are what a peaked row consists of)
-  const float top = m == -INFINITY ? 0.f : m;
+  for (int q = 0; q < VPL; q++) part[q % 4] = fmaxf(part[q % 4], v[q]);
+  const float m = warp_max(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))), top = m == -INFINITY ? 0.f : m;
+  // (the largest is taken off first: a multiple of it would bring its own rounding into every term)
   double sum = 0.0;
 #pragma unroll
-  for (int g = 0; g < GROUPS; g++) {
-    float a = 0.f;
+  for (int g = 0; g < VPL; g += 16) {
+    float a = 0.f, b = 0.f;
 #pragma unroll
-    for (int q = 0; q < VPL / GROUPS; q++) {
-      const float u = v[g * (VPL / GROUPS) + q];
-      a += count <= CAP && u >= bar ? 0.f : ex2((u - top) * 1.4426950408889634f);
+    for (int q = g; q < g + 16; q += 2) {
+      a += ex2((v[q] - top) * 1.4426950408889634f);
+      b += ex2((v[q + 1] - top) * 1.4426950408889634f);
     }
-    sum += (double)a;
-  }
-  __syncwarp();
-  int2* const out = cand + (size_t)piece * n;
-  if (count <= CAP) {
-    for (int e = lane; e < count; e += 32) {
-      const float2 mine = buf[e];
-      const int idx = __float_as_int(mine.y);
-      int rank = 0;
-      for (int i = 0; i < count; i++) {
-        const float2 o = buf[i];
-        rank += o.x > mine.x || (o.x == mine.x && __float_as_int(o.y) < idx);
-      }
-      if (rank < n) out[rank] = make_int2(__float_as_int(mine.x), idx);
-      sum += exp((double)mine.x - (double)top);
-    }
-    for (int e = count + lane; e < n; e += 32) out[e] = make_int2(0, -1);
-  } else {
-    // many equal values (or all of the largest in one group): one after the other, the best that comes after the last
-    float last = INFINITY;
-    int last_at = -1;
-    for (int r = 0; r < n; r++) {
-      float best = -INFINITY;
-      int best_at = 0x7fffffff;
-#pragma unroll
-      for (int q = 0; q < VPL; q++) {
-        const int idx = index_of(q);
-        const bool after = v[q] < last || (v[q] == last && idx > last_at);
-        if (after && v[q] > -INFINITY && (v[q] > best || (v[q] == best && idx < best_at))) { best = v[q]; best_at = idx; }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float f = __shfl_xor_sync(0xffffffffu, best, o);
-        const int at = __shfl_xor_sync(0xffffffffu, best_at, o);
-        if (f > best || (f == best && at < best_at)) { best = f; best_at = at; }
-      }
-      if (lane == 0) out[r] = best > -INFINITY ? make_int2(__float_as_int(best), best_at) : make_int2(0, -1);
-      last = best;
-      last_at = best_at;
-    }
+    sum += (double)(a + b);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -173,28 +104,32 @@ beam_scan_kernel(const float* __restrict__ logits, long long ld, const float* __
 // Candidates by value, equal ones by index.
 __device__ __forceinline__ bool better(double a, int ai, double b, int bi) { return a > b || (a == b && ai < bi); }
 
+template <int VPL, int VEC>
 __global__ void __launch_bounds__(MERGE_T)
-beam_merge_kernel(const float* __restrict__ scores, const unsigned char* __restrict__ ended, int K, int V, int n_pieces, int n, int pad,
-                  int placed, const Stats* __restrict__ stats, const int2* __restrict__ cand, int* __restrict__ tokens,
+beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* __restrict__ scores, const unsigned char* __restrict__ ended, int K,
+                  int V, int n_pieces, int n, int pad, int placed, const Stats* __restrict__ stats, int* __restrict__ tokens,
                   int* __restrict__ parents, float* __restrict__ out_scores) {
-  tlc_pdl(scores, ended, stats, cand, tokens, parents, out_scores);
-  extern __shared__ unsigned heads[];                  // of every list: the value of its first candidate, as an ordered integer
-  __shared__ double s_off[MAX_BEAMS], s_value[MERGE_CAP], s_best[MERGE_T / 32];
-  __shared__ int s_index[MERGE_CAP], s_at[MERGE_T / 32], s_count, s_alive[MAX_BEAMS];
+  tlc_pdl(logits, scores, ended, stats, tokens, parents, out_scores);
+  extern __shared__ int merge_room[];
+  float* const c_value = reinterpret_cast<float*>(merge_room);           // [MERGE_CAP] logits that reach the threshold
+  int* const c_index = merge_room + MERGE_CAP;                           // [MERGE_CAP] k * V + v of them; of ended beams -1 - k
+  unsigned* const heads = reinterpret_cast<unsigned*>(merge_room + 2 * MERGE_CAP);     // of every piece: what its maximum is worth, as an ordered integer
+  __shared__ double s_off[MAX_BEAMS], s_value[MERGE_RANK], s_best[MERGE_WARPS];
+  __shared__ int s_index[MERGE_RANK], s_at[MERGE_WARPS], s_count, s_ranked, s_alive[MAX_BEAMS], s_list[MERGE_LISTS], s_lists, s_reach[2];
   __shared__ unsigned s_least;
   __shared__ double s_out[MAX_N];
   __shared__ int s_out_at[MAX_N];
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lists = K * n_pieces;
-  if (tid == 0) s_count = 0;
+  if (tid == 0) s_count = s_lists = s_ranked = s_reach[0] = s_reach[1] = 0;
   // what a row's logits are raised by: the beam's score less the logarithm of the row's sum
-  for (int k = warp; k < K; k += MERGE_T / 32) {
+  for (int k = warp; k < K; k += MERGE_WARPS) {
     const int row = r * K + k;
+    const Stats* st = stats + (size_t)row * n_pieces;
+    float m = -INFINITY;
+    for (int i = lane; i < n_pieces; i += 32) m = fmaxf(m, st[i].max);   // (of a row that is not alive whatever is there)
     bool on = alive(scores, ended, row);
     double off = 0.0;
     if (on) {
-      const Stats* st = stats + (size_t)row * n_pieces;
-      float m = -INFINITY;
-      for (int i = lane; i < n_pieces; i += 32) m = fmaxf(m, st[i].max);
       m = warp_max(m);
       double sum = 0.0;
       for (int i = lane; i < n_pieces; i += 32) {
@@ -210,80 +145,153 @@ beam_merge_kernel(const float* __restrict__ scores, const unsigned char* __restr
     if (lane == 0) { s_off[k] = off; s_alive[k] = on; }
   }
   __syncthreads();
-  auto key_of = [&](int k, int bits) { return ordered((float)(s_off[k] + (double)__int_as_float(bits))); };
-  const int2* const mine = cand + (size_t)r * lists * n;
+  auto key_of = [&](int k, float x) { return ordered((float)(s_off[k] + (double)x)); };
+  const Stats* const mine = stats + (size_t)r * lists;
   for (int l = tid; l < lists; l += MERGE_T) {
     const int k = l / n_pieces;
     unsigned h = 0;
     if (s_alive[k]) {
-      const int2 c = mine[(size_t)l * n];
-      if (c.y >= 0) h = key_of(k, c.x);
+      const float m = mine[l].max;
+      if (m > -INFINITY) h = key_of(k, m);
     }
     heads[l] = h;
   }
   __syncthreads();
-  // the n-th largest of the first candidates: nothing below it can be among the n best
+  // a threshold that at least n of the pieces' maxima reach (and 2 n at most, where that can be found)
   if (warp == 0) {
-    unsigned least = 0;
-    for (int bit = 31; bit >= 0; bit--) {
-      const unsigned trial = least | 1u << bit;
-      int reach = 0;
-      for (int l = lane; l < lists; l += 32) reach += heads[l] >= trial;
-      reach = __reduce_add_sync(0xffffffffu, reach);
-      if (reach >= n) least = trial;
-      if (reach == n) break;
+    constexpr int HELD = 16;                           // of the first 512 pieces in registers
+    unsigned held[HELD], least = 0xffffffffu, above = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+      held[i] = i * 32 + lane < lists ? heads[i * 32 + lane] : 0u;
+      if (i * 32 + lane < lists) least = min(least, held[i]);
+      above = max(above, held[i]);
     }
+    for (int l = HELD * 32 + lane; l < lists; l += 32) { least = min(least, heads[l]); above = max(above, heads[l]); }
+    least = __reduce_min_sync(0xffffffffu, least);
+    above = __reduce_max_sync(0xffffffffu, above);
+    if (lists < n) least = 0;
+    else
+      while (least < above) {                          // (least is reached by n, above + 1 by none)
+        const unsigned trial = least + (above - least + 1) / 2;       // (at least 1: what is past the lists does not count)
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < HELD; i++) reach += held[i] >= trial;
+        for (int l = HELD * 32 + lane; l < lists; l += 32) reach += heads[l] >= trial;
+        reach = __reduce_add_sync(0xffffffffu, reach);
+        if (reach >= n) least = trial; else above = trial - 1;
+        if (reach >= n && reach <= 2 * n) break;
+      }
     if (lane == 0) s_least = max(least, 1u);
   }
   __syncthreads();
-  const unsigned least = s_least;
-  for (int l = tid; l < lists; l += MERGE_T) {
-    if (heads[l] < least) continue;
-    const int k = l / n_pieces;
-    for (int i = 0; i < n; i++) {
-      const int2 c = mine[(size_t)l * n + i];
-      if (c.y < 0 || key_of(k, c.x) < least) break;
-      const int at = atomicAdd(&s_count, 1);
-      if (at < MERGE_CAP) { s_value[at] = s_off[k] + (double)__int_as_float(c.x); s_index[at] = k * V + c.y; }
+  unsigned least = s_least;
+  // the pieces that reach it, again
+  for (int l = tid; l < lists; l += MERGE_T)
+    if (heads[l] >= least) {
+      const int at = atomicAdd(&s_lists, 1);
+      if (at < MERGE_LISTS) s_list[at] = l;
     }
+  __syncthreads();
+  const int passing = s_lists;
+  auto collect = [&](int l) {
+    const int k = l / n_pieces, base = l % n_pieces * 32 * VPL;
+    const float* const x = logits + (size_t)(r * K + k) * ld + base;
+    float v[VPL];
+    load_piece<VPL, VEC>(x, V - base, lane, v);
+#pragma unroll
+    for (int q = 0; q < VPL; q++)
+      if (v[q] > -INFINITY && key_of(k, v[q]) >= least) {
+        const int at = atomicAdd(&s_count, 1);         // (in any order: they are ranked below)
+        if (at < MERGE_CAP) { c_value[at] = v[q]; c_index[at] = k * V + base + (q / VEC * 32 + lane) * VEC + q % VEC; }
+      }
+  };
+  if (passing <= MERGE_LISTS) {
+    for (int i = warp; i < passing; i += MERGE_WARPS) collect(s_list[i]);
+  } else {
+    for (int l = warp; l < lists; l += MERGE_WARPS)
+      if (heads[l] >= least) collect(l);
   }
   if (ended)                                           // a beam that has ended stands for itself
     for (int k = tid; k < K; k += MERGE_T)
       if (ended[r * K + k] && isfinite(scores[r * K + k])) {
         const int at = atomicAdd(&s_count, 1);
-        if (at < MERGE_CAP) { s_value[at] = (double)scores[r * K + k]; s_index[at] = k * V + pad; }
+        if (at < MERGE_CAP) c_index[at] = -1 - k;
       }
   __syncthreads();
   const int count = s_count;
-  int found;
-  if (count <= MERGE_CAP) {
-    found = min(count, n);
-    for (int e = tid; e < count; e += MERGE_T) {
-      const double a = s_value[e];
-      const int ai = s_index[e];
-      int rank = 0;
-      for (int i = 0; i < count; i++) rank += better(s_value[i], s_index[i], a, ai);
-      if (rank < n) { s_out[rank] = a; s_out_at[rank] = ai; }
+  auto value_of = [&](int e, int* index) {
+    const int at = c_index[e];
+    if (at < 0) {
+      *index = (-1 - at) * V + pad;
+      return (double)scores[r * K + -1 - at];
     }
-  } else {
-    // more than there is room for (equal values in many lists): one after the other
+    *index = at;
+    return s_off[at / V] + (double)c_value[e];
+  };
+  int found = -1;
+  if (count <= MERGE_CAP) {
+    // of many a second threshold, found the same way by the whole block
+    unsigned bar = 0;
+    if (count > MERGE_RANK) {
+      constexpr int HELD = MERGE_CAP / MERGE_T;
+      unsigned held[HELD], low = 1u, high = 0xffffffffu;
+#pragma unroll
+      for (int i = 0; i < HELD; i++) {
+        int index;
+        held[i] = i * MERGE_T + tid < count ? ordered((float)value_of(i * MERGE_T + tid, &index)) : 0u;
+      }
+      for (int turn = 0; low < high; turn++) {         // (low is reached by n)
+        const unsigned trial = low + (high - low) / 2 + 1;
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < HELD; i++) reach += held[i] >= trial;
+        reach = __reduce_add_sync(0xffffffffu, reach);
+        if (lane == 0) atomicAdd(&s_reach[turn & 1], reach);
+        __syncthreads();
+        reach = s_reach[turn & 1];
+        if (tid == 0) s_reach[(turn + 1) & 1] = 0;
+        __syncthreads();
+        if (reach >= n) low = trial; else high = trial - 1;
+        if (reach >= n && reach <= MERGE_RANK) break;
+      }
+      bar = low;
+    }
+    for (int e = tid; e < count; e += MERGE_T) {
+      int index;
+      const double a = value_of(e, &index);
+      if (bar > 0 && ordered((float)a) < bar) continue;
+      const int at = atomicAdd(&s_ranked, 1);
+      if (at < MERGE_RANK) { s_value[at] = a; s_index[at] = index; }
+    }
+    __syncthreads();
+    const int ranked = s_ranked;
+    if (ranked <= MERGE_RANK) {
+      found = min(ranked, n);
+      for (int e = tid; e < ranked; e += MERGE_T) {
+        const double a = s_value[e];
+        const int ai = s_index[e];
+        int rank = 0;
+        for (int i = 0; i < ranked; i++) rank += better(s_value[i], s_index[i], a, ai);
+        if (rank < n) { s_out[rank] = a; s_out_at[rank] = ai; }
+      }
+    }
+  }
+  if (found < 0) {
+    // more than there is room for (equal values): one after the other, each the best of all logits that comes after the last
     double last = INFINITY;
     int last_at = -1;
-    found = 0;
-    for (; found < n; found++) {
+    for (found = 0; found < n; found++) {
       double best = -INFINITY;
       int best_at = 0x7fffffff;
       auto take = [&](double a, int ai) {
         if (better(last, last_at, a, ai) && better(a, ai, best, best_at)) { best = a; best_at = ai; }
       };
-      for (int l = tid; l < lists; l += MERGE_T) {
-        if (heads[l] < least) continue;
-        const int k = l / n_pieces;
-        for (int i = 0; i < n; i++) {
-          const int2 c = mine[(size_t)l * n + i];
-          if (c.y < 0) break;
-          take(s_off[k] + (double)__int_as_float(c.x), k * V + c.y);
-        }
+      for (int k = 0; k < K; k++) {
+        if (!s_alive[k]) continue;
+        const float* const x = logits + (size_t)(r * K + k) * ld;
+        for (int i = tid; i < V; i += MERGE_T)
+          if (x[i] > -INFINITY) take(s_off[k] + (double)x[i], k * V + i);
       }
       if (ended)
         for (int k = tid; k < K; k += MERGE_T)
@@ -298,7 +306,7 @@ beam_merge_kernel(const float* __restrict__ scores, const unsigned char* __restr
       __syncthreads();
       best = s_best[0];
       best_at = s_at[0];
-      for (int w = 1; w < MERGE_T / 32; w++)
+      for (int w = 1; w < MERGE_WARPS; w++)
         if (better(s_best[w], s_at[w], best, best_at)) { best = s_best[w]; best_at = s_at[w]; }
       __syncthreads();
       if (best == -INFINITY) break;
@@ -564,10 +572,38 @@ beam_pages_kernel(char* k_pages, char* v_pages, long long layer_bytes, int KV, i
 // values of a piece: 64 a lane make few lists of long pieces; 16 spread a few rows over the SMs (4 rows of 65,536: 512 warps, not 128)
 static int piece_values(long long rows, int V) { return rows * V >= 2048ll * 148 * 4 ? 2048 : 512; }
 
-extern "C" long long tlc_beam_select_scratch(int rows, int V, int n) {
+extern "C" long long tlc_beam_select_scratch(int rows, int V) {
   const int per = piece_values(rows, V);
-  return rows * (((long long)V + per - 1) / per) * ((long long)sizeof(Stats) + 8ll * n);
+  return rows * (((long long)V + per - 1) / per) * (long long)sizeof(Stats);
 }
+
+namespace {
+struct SelectArgs {
+  const float* logits;
+  long long ld;
+  const float* scores;
+  const unsigned char* ended;
+  int R, K, V, pieces, n, pad, placed;
+  Stats* stats;
+  int *tokens, *parents;
+  float* out_scores;
+};
+template <int VPL, int VEC> int run_select(const SelectArgs& a, cudaStream_t stream) {
+  static OncePerDevice ready;
+  if (!ready.done([] {
+        return cudaFuncSetAttribute(beam_merge_kernel<VPL, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * MERGE_CAP + MAX_LISTS) * (int)sizeof(int));
+      }))
+    return tlc_fail(-2, "beam_select: cannot reserve shared memory");
+  const unsigned blocks = (unsigned)(((long long)a.R * a.K * a.pieces + SCAN_WARPS - 1) / SCAN_WARPS);
+  tlc_launch(beam_scan_kernel<VPL, VEC>, dim3(blocks), dim3(SCAN_WARPS * 32), 0, stream, a.logits, a.ld, a.scores, a.ended, a.R * a.K, a.V, a.pieces,
+             a.stats);
+  TLC_CHECK_LAUNCH("beam_select(scan)");
+  tlc_launch(beam_merge_kernel<VPL, VEC>, dim3(a.R), dim3(MERGE_T), (2 * MERGE_CAP + (size_t)a.K * a.pieces) * sizeof(int), stream, a.logits, a.ld, a.scores,
+             a.ended, a.K, a.V, a.pieces, a.n, a.pad, a.placed, a.stats, a.tokens, a.parents, a.out_scores);
+  TLC_CHECK_LAUNCH("beam_select(merge)");
+  return 0;
+}
+}  // namespace
 
 extern "C" int tlc_beam_select(const float* logits, long long ld, const float* scores, const void* ended, int R, int K, int V, int n, int pad,
                                int placed, void* scratch, int* tokens, int* parents, float* out_scores, cudaStream_t stream) {
@@ -580,21 +616,10 @@ extern "C" int tlc_beam_select(const float* logits, long long ld, const float* s
   TLC_REQUIRE((long long)K * pieces <= MAX_LISTS && (long long)K * V < (1ll << 31), "beam_select: %d beams of %d tokens are too many", K, V);
   TLC_REQUIRE((long long)R * K * pieces < (1ll << 31) * SCAN_WARPS, "beam_select: %d rows of %d logits are too many", R * K, V);
   TLC_REQUIRE(((uintptr_t)scratch & 15) == 0, "beam_select: scratch must start on a 16-byte boundary");
-  Stats* const stats = (Stats*)scratch;
-  int2* const cand = (int2*)(stats + (size_t)R * K * pieces);
+  const SelectArgs a{logits, ld, scores, (const unsigned char*)ended, R, K, V, pieces, n, pad, placed, (Stats*)scratch, tokens, parents, out_scores};
   const bool vec = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
-  const dim3 grid((unsigned)(((long long)R * K * pieces + SCAN_WARPS - 1) / SCAN_WARPS)), block(SCAN_WARPS * 32);
-  auto* const k = per == 2048 ? (vec ? beam_scan_kernel<64, 4> : beam_scan_kernel<64, 1>) : (vec ? beam_scan_kernel<16, 4> : beam_scan_kernel<16, 1>);
-  tlc_launch(k, grid, block, 0, stream, logits, ld, scores, (const unsigned char*)ended, R * K, V, pieces, n, stats, cand);
-  TLC_CHECK_LAUNCH("beam_select(scan)");
-  const int smem = K * pieces * (int)sizeof(unsigned);
-  if (smem > 16 * 1024 &&
-      cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_LISTS * (int)sizeof(unsigned)) != cudaSuccess)
-    return tlc_fail(-2, "beam_select: cannot reserve shared memory");
-  tlc_launch(beam_merge_kernel, dim3(R), dim3(MERGE_T), (size_t)smem, stream, scores, (const unsigned char*)ended, K, V, pieces, n, pad, placed,
-             stats, cand, tokens, parents, out_scores);
-  TLC_CHECK_LAUNCH("beam_select(merge)");
-  return 0;
+  if (per == 2048) return vec ? run_select<64, 4>(a, stream) : run_select<64, 1>(a, stream);
+  return vec ? run_select<16, 4>(a, stream) : run_select<16, 1>(a, stream);
 }
 
 extern "C" int tlc_beam_reorder_states(void* state, long long layer_bytes, long long slot_bytes, long long bytes, int L, int n_slots,

@@ -98,6 +98,21 @@ inline cudaError_t tlc_launch_step_boundary(void (*kernel)(KArgs...), dim3 grid,
   return tlc_launch_as(false, kernel, grid, block, smem, stream, static_cast<Args&&>(args)...);
 }
 
+// Set-up that every device needs once (a kernel's shared memory): done() runs it on the current device unless it has been run there, and
+// says whether it has succeeded.
+struct OncePerDevice {
+  std::atomic<unsigned long long> devices{0};
+  template <typename F> bool done(F set_up) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;           // (beyond 64 devices: every time)
+    if (devices.load(std::memory_order_relaxed) & bit) return true;
+    if (set_up() != cudaSuccess) return false;
+    devices.fetch_or(bit, std::memory_order_relaxed);
+    return true;
+  }
+};
+
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }

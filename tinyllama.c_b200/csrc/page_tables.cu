@@ -14,7 +14,7 @@
 namespace {
 
 constexpr int RT = 1024;                 // threads of the resizing block
-constexpr int MAX_REQUESTS = 8192;       // of one call: two sums a request in shared memory
+constexpr int MAX_REQUESTS = 4096;       // of one call: their sums and pages lie in shared memory
 constexpr int PER = 16;                  // entries of refs a thread looks at a time (four 16-byte loads)
 
 // codes of the status word (the largest that occurred stays until the caller clears it)
@@ -61,15 +61,21 @@ __device__ __forceinline__ int find_sum(const int* sum, int n, int at) {
 }
 
 // One block does all of it: which page is the p-th lowest free one depends on every page before it, and what a step takes is
-// few pages of a pool that is looked through from the start (150,000 pages: ten rounds of one load and one sum each).
-// Everything another thread of the block may have changed is read past the L1 (__ldcg).
+// few pages of a pool that is looked through from the start.  Bound by trips to the L2: the requests, their lengths, the last pages'
+// counts, then a round for every 16,384 pages looked at (the first round's counts are fetched at the start); in a round the free pages go
+// into a list, and the list into the table, a page a thread (700 requests that take 800 pages: 22 us where a thread placed all the pages
+// it had found, one after the other).  Everything another thread of the block may have changed is read past the L1 (__ldcg).
+struct Request { int slot, have, need; };             // slot -1: nothing to do
+
 __global__ void __launch_bounds__(RT)
 page_resize_kernel(int* block_table, int n_slots, int max_pages, int* refs, int n_pages, int* lengths, const int* slots,
                    const int* want, int B, int* status) {
   tlc_wait(block_table, refs, lengths, slots, want, status);
-  extern __shared__ int sums[];                       // [2][B + 1]: pages taken and pages given back by the requests before
-  int* const take = sums;
-  int* const give = sums + B + 1;
+  extern __shared__ int resize_room[];
+  int* const list = resize_room;                      // [RT * PER] free pages of a round
+  int* const take = list + RT * PER;                  // [B + 1] pages taken by the requests before
+  int* const give = take + B + 1;                     // [B + 1] pages given back by them
+  Request* const request = reinterpret_cast<Request*>(give + B + 1);
   __shared__ long long red[33];
   __shared__ int s_bad;
   const int tid = threadIdx.x;
@@ -81,29 +87,45 @@ page_resize_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
     __syncthreads();
     return c;
   };
+  const bool vec = (reinterpret_cast<uintptr_t>(refs) & 15) == 0;
+  auto load = [&](int at, int (&v)[PER]) {
+    if (vec && at + PER <= n_pages) {
+#pragma unroll
+      for (int q = 0; q < PER / 4; q++) {
+        const int4 x = __ldcg(reinterpret_cast<const int4*>(refs + at) + q);
+        v[4 * q] = x.x; v[4 * q + 1] = x.y; v[4 * q + 2] = x.z; v[4 * q + 3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < PER; q++) v[q] = at + q < n_pages ? __ldcg(refs + at + q) : 1;
+    }
+  };
+  int v[PER];
+  load(tid * PER, v);                                 // (loaded again where pages are given back)
   // 1. each request's slot is claimed (by the sign of its length); what the request takes or gives back is added up
   const int each = (B + RT - 1) / RT, b0 = min(B, tid * each), b1 = min(B, b0 + each);
-  int slot[MINE], t_of[MINE], g_of[MINE], bad = 0;    // slot -1: none, or not claimed here
+  int slot[MINE], last[MINE], old[MINE], t_of[MINE], g_of[MINE], bad = 0;    // slot -1: none, or not claimed here; last: a page that is grown in
   long long mine = 0;                                 // pages taken, and pages given back in the upper half
 #pragma unroll
   for (int i = 0; i < MINE; i++) {
-    slot[i] = -1;
-    t_of[i] = g_of[i] = 0;
+    slot[i] = last[i] = -1;
+    t_of[i] = g_of[i] = old[i] = 0;
     const int b = b0 + i;
     if (b >= b1) continue;
     const int s = slots[b], w = want[b];
-    if (s < 0) continue;
-    if (s >= n_slots) { bad = max(bad, (int)ST_SLOT); continue; }
-    const int old = atomicOr(lengths + s, ~LENGTH);
-    if (old < 0) { bad = max(bad, (int)ST_SLOT); continue; }             // named twice (or no length at all)
+    if (s >= n_slots) bad = max(bad, (int)ST_SLOT);
+    if (s < 0 || s >= n_slots) { request[b] = Request{-1, 0, 0}; continue; }
+    old[i] = atomicOr(lengths + s, ~LENGTH);
+    const int have = pages_of(old[i] & LENGTH), need = pages_of(max(w, 0));
+    request[b] = Request{s, have, need};
+    if (old[i] < 0) { bad = max(bad, (int)ST_SLOT); continue; }          // named twice (or no length at all)
     slot[i] = s;
-    const int have = pages_of(old), need = pages_of(max(w, 0));
     if (w < 0 || need > max_pages || have > max_pages) { bad = max(bad, (int)ST_LENGTH); continue; }
     t_of[i] = max(0, need - have);
     g_of[i] = max(0, have - need);
-    if (w > old && old % TLC_PAGE != 0) {
-      const int p = __ldcg(block_table + (size_t)s * max_pages + have - 1);
-      if (p < 0 || p >= n_pages) bad = max(bad, (int)ST_TABLE);
+    if (w > old[i] && old[i] % TLC_PAGE != 0) {
+      last[i] = __ldcg(block_table + (size_t)s * max_pages + have - 1);
+      if (last[i] < 0 || last[i] >= n_pages) { bad = max(bad, (int)ST_TABLE); last[i] = -1; }
     }
     mine += (long long)t_of[i] | ((long long)g_of[i] << 32);
   }
@@ -124,65 +146,53 @@ page_resize_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
   // the table entry of the i-th page given back, and of the i-th page taken
   auto given = [&](int i) {
     const int b = find_sum(give, B + 1, i);
-    return block_table + (size_t)slots[b] * max_pages + pages_of(want[b]) + i - give[b];
+    return block_table + (size_t)request[b].slot * max_pages + request[b].need + i - give[b];
   };
   auto taken = [&](int i) {
-    const int b = find_sum(take, B + 1, i), s = slots[b];
-    return block_table + (size_t)s * max_pages + pages_of(__ldcg(lengths + s) & LENGTH) + i - take[b];
+    const int b = find_sum(take, B + 1, i);
+    return block_table + (size_t)request[b].slot * max_pages + request[b].have + i - take[b];
   };
   if (bad_so_far() == 0) {
     // 2. pages given back: one entry less each that names them
-    for (int i = tid; i < n_give; i += RT) {
-      const int p = __ldcg(given(i));
-      if (p < 0 || p >= n_pages || atomicSub(refs + p, 1) <= 0) atomicMax(&s_bad, (int)ST_TABLE);
+    if (n_give > 0) {
+      for (int i = tid; i < n_give; i += RT) {
+        const int p = __ldcg(given(i));
+        if (p < 0 || p >= n_pages || atomicSub(refs + p, 1) <= 0) atomicMax(&s_bad, (int)ST_TABLE);
+      }
+      __syncthreads();
+      load(tid * PER, v);
     }
-    __syncthreads();
     // a slot that grows inside its last page must have that page to itself
 #pragma unroll
     for (int i = 0; i < MINE; i++) {
-      if (slot[i] < 0) continue;
-      const int old = __ldcg(lengths + slot[i]) & LENGTH;
-      if (want[b0 + i] <= old || old % TLC_PAGE == 0) continue;
-      const int n = __ldcg(refs + __ldcg(block_table + (size_t)slot[i] * max_pages + pages_of(old) - 1));
+      if (last[i] < 0) continue;
+      const int n = __ldcg(refs + last[i]);
       if (n != 1) atomicMax(&s_bad, n < 1 ? (int)ST_TABLE : (int)ST_SHARED);
     }
     int code = bad_so_far();
     // 3. the lowest free pages, request by request
     int found = 0;
     if (code == 0 && n_take > 0) {
-      const bool vec = (reinterpret_cast<uintptr_t>(refs) & 15) == 0;
-      auto load = [&](int at, int (&v)[PER]) {
-        if (vec && at + PER <= n_pages) {
-#pragma unroll
-          for (int q = 0; q < PER / 4; q++) {
-            const int4 x = __ldcg(reinterpret_cast<const int4*>(refs + at) + q);
-            v[4 * q] = x.x; v[4 * q + 1] = x.y; v[4 * q + 2] = x.z; v[4 * q + 3] = x.w;
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < PER; q++) v[q] = at + q < n_pages ? __ldcg(refs + at + q) : 1;
-        }
-      };
-      int v[PER], next[PER];
-      load(tid * PER, v);
       for (int base = 0; base < n_pages && found < n_take; base += RT * PER) {
         const int at = base + tid * PER;
-        load(at + RT * PER, next);                     // the next round's, on their way during this one's sum
         int n = 0;
-#pragma unroll
-        for (int q = 0; q < PER; q++) n += v[q] == 0;
-        long long all;
-        int rank = found + (int)block_prefix<long long>(n, red, &all);
+        unsigned free = 0;
 #pragma unroll
         for (int q = 0; q < PER; q++) {
-          if (v[q] == 0 && rank < n_take) {
-            *taken(rank) = at + q;
-            refs[at + q] = 1;
-            rank++;
-          }
-          v[q] = next[q];
+          n += v[q] == 0;
+          free |= (v[q] == 0 ? 1u : 0u) << q;
         }
-        found += (int)all;
+        load(at + RT * PER, v);                        // the next round's, on their way during this one's sum
+        long long all;
+        int rank = (int)block_prefix<long long>(n, red, &all);
+        const int most = min((int)all, n_take - found);
+        for (; free != 0 && rank < most; free &= free - 1, rank++) list[rank] = at + __ffs(free) - 1;
+        __syncthreads();
+        for (int i = tid; i < most; i += RT) {
+          *taken(found + i) = list[i];
+          refs[list[i]] = 1;
+        }
+        found += most;                                 // (the list is written again after the next sum's barriers)
       }
       if (found < n_take) code = ST_FULL;              // (every thread knows)
     }
@@ -191,7 +201,7 @@ page_resize_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
     if (code == 0) {
       for (int i = tid; i < n_give; i += RT) *given(i) = 0;
     } else {
-      for (int i = tid; i < min(found, n_take); i += RT) {
+      for (int i = tid; i < found; i += RT) {
         int* const e = taken(i);
         refs[__ldcg(e)] = 0;
         *e = 0;
@@ -207,7 +217,7 @@ page_resize_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
   const int code = bad_so_far();
 #pragma unroll
   for (int i = 0; i < MINE; i++)
-    if (slot[i] >= 0) lengths[slot[i]] = code == 0 ? want[b0 + i] : __ldcg(lengths + slot[i]) & LENGTH;
+    if (slot[i] >= 0) lengths[slot[i]] = code == 0 ? want[b0 + i] : old[i];
   if (code != 0 && tid == 0) atomicMax(status, code);
 }
 
@@ -397,10 +407,11 @@ extern "C" int tlc_page_resize(int* block_table, int n_slots, int max_pages, int
   TLC_REQUIRE(B > 0 && B <= MAX_REQUESTS, "page_resize: %d requests (at most %d a call)", B, MAX_REQUESTS);
   TLC_REQUIRE(n_slots > 0 && max_pages > 0 && n_pages > 0 && n_pages <= (1 << 25), "page_resize: %d slots of %d pages, %d pages (at most 2^25)",
               n_slots, max_pages, n_pages);
-  const int smem = 2 * (B + 1) * (int)sizeof(int);
-  if (smem > 40 * 1024 &&
-      cudaFuncSetAttribute(page_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (MAX_REQUESTS + 1) * (int)sizeof(int)) != cudaSuccess)
+  static OncePerDevice ready;
+  constexpr int most = (RT * PER + 2 * (MAX_REQUESTS + 1)) * (int)sizeof(int) + MAX_REQUESTS * (int)sizeof(Request);
+  if (!ready.done([&] { return cudaFuncSetAttribute(page_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most); }))
     return tlc_fail(-2, "page_resize: cannot reserve shared memory");
+  const int smem = (RT * PER + 2 * (B + 1)) * (int)sizeof(int) + B * (int)sizeof(Request);
   tlc_launch(page_resize_kernel, dim3(1), dim3(RT), (size_t)smem, stream, block_table, n_slots, max_pages, refs, n_pages, lengths, slots, want, B,
              status);
   TLC_CHECK_LAUNCH("page_resize");

@@ -559,7 +559,7 @@ int tlc_retention_chunked(float* proj, int ld, int q_off, int k_off, int v_off, 
  * table, 3 a slot that does not exist or is named twice, 4 an entry or a count that cannot be (a page that does not exist, or is
  * free), 5 a slot that would grow inside a page it shares.
  * tlc_page_resize: slot slots[b] (-1: nothing) shall hold want[b] positions: pages behind them are given back (entries 0), and
- * missing ones are the lowest free pages, request by request.  All of it, or with a code nothing.  B at most 8,192.
+ * missing ones are the lowest free pages, request by request.  All of it, or with a code nothing.  B at most 4,096.
  * tlc_row_maps: for the rows of a step, request b bringing rows[b] of them after its first start[b] positions: cu_seqlens [B + 1],
  * row_seq, positions and row_map (page * 64 + offset of the row's position, -1: none) [T]; rows behind the last request have row_seq -1,
  * position 0, no place; rows beyond T are left out.  parents (NULL: none) makes the rows drafts: parents[t] is the index, among its request's
@@ -596,13 +596,13 @@ int tlc_tree_attention(const void* q, int dtype, int ld_q, const void* k_new, in
  * equal ones by k * V + v; logits [R * K, V] with rows of ld, scores [R, K].  A beam whose score is not finite, or whose logits hold a NaN
  * or +infinity, has no candidates; one that has ended (bytes [R, K], NULL: none) has one, token pad at its score.  Where there are
  * fewer than n, the first other pairs follow with a score of -infinity.  placed (n == K): a beam's first child stays in its
- * place and the others fill the places left; else the best comes first.  scratch: tlc_beam_select_scratch(R * K, V, n) bytes.
+ * place and the others fill the places left; else the best comes first.  scratch: tlc_beam_select_scratch(R * K, V) bytes.
  * tlc_beam_reorder_states: what slot slots[r, parents[r, k]] holds goes to slot slots[r, k], in every layer at once; strides in bytes.
  * tlc_beam_reorder_pages: the same of a pool's keys and values: a beam with another parent than itself gives back its pages but the last,
  * shares the parent's whole pages and takes over what the parent's last, partly filled page holds in its own last page.  A request
  * for which that cannot be done (status as above) stays as it is.  scratch: 16 * R * K bytes.  A slot of -1 or a parent outside
  * 0 .. K - 1 leaves a beam as it is. */
-long long tlc_beam_select_scratch(int rows, int V, int n);
+long long tlc_beam_select_scratch(int rows, int V);
 int tlc_beam_select(const float* logits, long long ld, const float* scores, const void* ended, int R, int K, int V, int n, int pad,
                     int placed, void* scratch, int* tokens, int* parents, float* out_scores, cudaStream_t stream);
 int tlc_beam_reorder_states(void* state, long long layer_bytes, long long slot_bytes, long long bytes, int L, int n_slots,

@@ -20,6 +20,14 @@ constexpr float LOG2E = 1.4426950408889634f;
 __host__ __device__ constexpr int padded(int hd) { return ((hd + 3) / 4) % 2 ? (hd + 3) / 4 * 4 : (hd + 3) / 4 * 4 + 4; }   // 16-byte rows, an odd number of pieces
 __host__ __device__ constexpr int smem_floats(int hd, int rows) { return (rows + BN) * padded(hd) + BN * ((hd + 63) / 64 * 64) + rows * (BN + 4); }
 
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ bool finite4(float4 v) { return isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w); }
+
 // RM rows of pairs a thread (16 RM a tile), NJ times 64 columns of values.
 template <typename T, int RM, int NJ>
 __global__ void __launch_bounds__(NT)
@@ -37,26 +45,25 @@ tree_attention_kernel(TreeArgs a) {
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const T* const q = reinterpret_cast<const T*>(a.q);
   const TreeTake take = tree_plan<NT>(a, blockIdx.x, reinterpret_cast<int*>(tree_raw));
-  int b = take.b, unit = take.unit, todo = take.todo;
+  int b = take.b, item = take.item, kt0 = take.tile, todo = take.todo;
   TreeSeq s = take.s;
   const float scale2 = a.scale * LOG2E;
   for (bool first_segment = true; todo > 0; first_segment = false) {
-    while (unit >= s.units) { unit -= s.units; s = tree_seq(a, ++b); }
-    const int item = unit / s.key_tiles, kt0 = unit % s.key_tiles;
+    while (item >= a.KV * s.row_tiles) { item -= a.KV * s.row_tiles; s = tree_seq(a, ++b); }
     const int g = item / s.row_tiles, r0 = item % s.row_tiles * a.tile_rows;
     const int kt1 = min(s.key_tiles, kt0 + todo);
     const int pairs = min(a.tile_rows, s.n * G - r0);
     const int* const table = a.block_table + (size_t)(s.context_tiles > 0 ? a.slots[b] : 0) * a.max_pages;
     __syncthreads();                                        // the segment before has used its queries
     // the tile's queries
-    for (int e = tid; e < ROWS * hp; e += NT) {
-      const int r = e / hp, d = e % hp;
-      float v = 0.f;
-      if (r < pairs && d < hd) {
-        const int i = (r0 + r) / G, h = g * G + (r0 + r) % G;
-        v = to_f32(q[(size_t)(s.t0 + i) * a.ld_q + (size_t)h * hd + d]);
+    for (int r = ty; r < ROWS; r += 16) {
+      const int i = (r0 + r) / G, h = g * G + (r0 + r) % G;
+      const T* const from = q + (size_t)(s.t0 + i) * a.ld_q + (size_t)h * hd;
+      if (a.vec) {
+        for (int d = tx * 4; d < hd; d += 64) *reinterpret_cast<float4*>(Q + r * hp + d) = r < pairs ? load4(from + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        for (int d = tx; d < hp; d += 16) Q[r * hp + d] = r < pairs && d < hd ? to_f32(from[d]) : 0.f;
       }
-      Q[e] = v;
     }
     float m[RM], l[RM], o[RM][4 * NJ];
     int pos[RM];
@@ -89,17 +96,45 @@ tree_attention_kernel(TreeArgs a) {
         vr = reinterpret_cast<const T*>(a.v_pages) + at;
         ldk = ldv = hd;
       }
-      __syncthreads();                                      // the tile before has been used
-      for (int e = tid; e < BN * hp; e += NT) {
-        const int r = e / hp, d = e % hp;
-        K[e] = there && r < keys && d < hd ? to_f32(kr[r * ldk + d]) : 0.f;
-      }
       bool odd = false;                                     // a value that is no number must not reach rows that do not see it
-      for (int e = tid; e < BN * hv; e += NT) {
-        const int r = e / hv, d = e % hv;
-        const float v = there && r < keys && d < hd ? to_f32(vr[r * ldv + d]) : 0.f;
-        V[e] = v;
-        odd |= !isfinite(v);
+      if (a.vec) {
+        // all of a thread's loads, then its stores (heads above 128: keys first)
+        constexpr int HALVES = NJ > 2 ? 2 : 1;
+#pragma unroll
+        for (int half = 0; half < HALVES; half++) {
+          float4 kv[4][NJ], vv[4][NJ];
+#pragma unroll
+          for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int c = 0; c < NJ; c++) {
+              const int r = ty + 16 * x, d = 64 * c + tx * 4;
+              const bool in = there && r < keys && d < hd;
+              if (HALVES == 1 || half == 0) kv[x][c] = in ? load4(kr + r * ldk + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+              if (HALVES == 1 || half == 1) vv[x][c] = in ? load4(vr + r * ldv + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+          if (half == 0) __syncthreads();                   // the tile before has been used
+#pragma unroll
+          for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int c = 0; c < NJ; c++) {
+              const int r = ty + 16 * x, d = 64 * c + tx * 4;
+              if ((HALVES == 1 || half == 0) && d < hd) *reinterpret_cast<float4*>(K + r * hp + d) = kv[x][c];
+              if (HALVES == 1 || half == 1) {
+                *reinterpret_cast<float4*>(V + r * hv + d) = vv[x][c];
+                odd |= !finite4(vv[x][c]);
+              }
+            }
+        }
+      } else {
+        __syncthreads();                                    // the tile before has been used
+        for (int r = ty; r < BN; r += 16) {
+          for (int d = tx; d < hp; d += 16) K[r * hp + d] = there && r < keys && d < hd ? to_f32(kr[r * ldk + d]) : 0.f;
+          for (int d = tx; d < hv; d += 16) {
+            const float v = there && r < keys && d < hd ? to_f32(vr[r * ldv + d]) : 0.f;
+            V[r * hv + d] = v;
+            odd |= !isfinite(v);
+          }
+        }
       }
       odd = __syncthreads_or(odd);
       float sc[RM][4];
@@ -183,7 +218,6 @@ tree_attention_kernel(TreeArgs a) {
       }
     }
     const bool whole = kt0 == 0 && kt1 == s.key_tiles;
-    const size_t part = ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * a.part_rows;
 #pragma unroll
     for (int u = 0; u < RM; u++) {
       const int r = ty * RM + u;
@@ -205,38 +239,37 @@ tree_attention_kernel(TreeArgs a) {
           if (d < hd) to[d] = from_f32<T>(l[u] == 0.f ? 0.f : o[u][c] * inv);
         }
       } else {
-        if (tx == 0) { a.part_ml[(part + r) * 2] = m[u]; a.part_ml[(part + r) * 2 + 1] = l[u]; }
+        const int slot = first_segment ? 0 : 1;
+        if (tx == 0) *tree_part_ml(a, blockIdx.x, slot, r) = make_float2(m[u], l[u]);
 #pragma unroll
-        for (int c = 0; c < 4 * NJ; c++) {
-          const int d = 64 * (c / 4) + tx * 4 + c % 4;
-          if (d < hd) a.part_o[(part + r) * hd + d] = o[u][c];
-        }
+        for (int c = 0; c < NJ; c++)
+          if (64 * c + tx * 4 < hd) *tree_part(a, blockIdx.x, slot, 16 * c + tx, r) = make_float4(o[u][4 * c], o[u][4 * c + 1], o[u][4 * c + 2], o[u][4 * c + 3]);
       }
     }
     todo -= kt1 - kt0;
-    unit += kt1 - kt0;
+    kt0 = 0;
+    item++;
   }
 }
 
 // Items that several blocks share: o = sum_z o_z 2^(m_z - m) / (sum_z l_z 2^(m_z - m) [+ 2^(sink - m)]).  Every block reads which items those
-// are (an entry of splits for each block of the kernel before) and takes its share of their rows: a row a block, the segments shared out
-// over the warps, where there are few rows in many segments, else four rows a warp.  Bound by trips to the L2, of which rows take two (the
-// statistics, then twelve segments' values at a time); a launch with nothing to add up is over after one.
+// are (an entry of splits for each block of the kernel before) and takes its share of their rows, four at a time, which lie side by
+// side: of few rows in many segments a block, or one for some of the columns, the segments shared out over its warps, else a warp.  Bound by trips to
+// the L2, of which rows take two (the statistics, then the values of some segments at a time); a launch with nothing to add up is over
+// after one.
 constexpr int MG_T = 256, MG_WARPS = MG_T / 32, MG_MOST = 512;           // MG_MOST: blocks of the kernel before, at most
-constexpr int MG_ROWS = 4;                                               // of a warp
-template <typename T, int VEC, int NV>
+constexpr int MG_ROWS = 4, MG_LANES = 32 / MG_ROWS;                      // rows of a task, lanes that look after a row's statistics
+template <typename T, int NV>
 __global__ void __launch_bounds__(MG_T)
 tree_merge_kernel(TreeArgs a) {
   tlc_pdl(a.part_o, a.part_ml, a.splits, a.out);
-  __shared__ int s_before[MG_MOST], s_warp[MG_WARPS], s_most;
-  __shared__ TreeSplit s_split[MG_MOST];
-  __shared__ float s_w[MG_MOST], s_red[2 * MG_WARPS], s_acc[MG_WARPS][NV * 32 * VEC];
+  __shared__ int s_before[MG_MOST], s_warp[MG_WARPS], s_most[MG_WARPS];
+  __shared__ float s_w[MG_MOST][MG_ROWS], s_red[2 * MG_WARPS][MG_ROWS];
+  __shared__ float4 s_acc[2][MG_WARPS][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.H / a.KV, hd = a.hd;
-  // the items' rows, in fours
+  // the items' rows, in fours, and the most segments of an item
   constexpr int EACH = MG_MOST / MG_T;
-  int total = 0;
-  if (tid == 0) s_most = 0;
-  __syncthreads();
+  int total = 0, most = 0;
 #pragma unroll
   for (int i = 0; i < EACH; i++) {
     const int c = i * MG_T + tid;
@@ -246,194 +279,221 @@ tree_merge_kernel(TreeArgs a) {
     }
     TreeSplit sp = {};
     if (c < a.blocks) sp = a.splits[c];
-    s_split[c] = sp;
-    const int n = sp.n > 1 ? (sp.pairs + MG_ROWS - 1) / MG_ROWS * MG_ROWS : 0;
-    if (sp.n > 1) atomicMax(&s_most, sp.n);
+    const int n = sp.n > 1 ? (sp.pairs + MG_ROWS - 1) / MG_ROWS : 0;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
+    const int segments = __reduce_max_sync(0xffffffffu, sp.n);
     if (i > 0) __syncthreads();
-    if (lane == 31) s_warp[warp] = x;
+    if (lane == 31) { s_warp[warp] = x; s_most[warp] = segments; }
     __syncthreads();
     int before = total + x - n;
 #pragma unroll
     for (int w = 0; w < MG_WARPS; w++) {
       if (w < warp) before += s_warp[w];
       total += s_warp[w];
+      most = max(most, s_most[w]);
     }
     s_before[c] = before;
   }
+  if (total == 0) return;
   __syncthreads();
-  // rounds of some three trips for a row a block; of one, and one for every three segments, for four rows a warp
-  const int grid = gridDim.x, wide = grid * MG_WARPS * MG_ROWS;
-  const bool together = (total + grid - 1) / grid * 3 < (total + wide - 1) / wide * (1 + (s_most + 2) / 3) || total <= grid;
-  for (int at = together ? blockIdx.x : (blockIdx.x * MG_WARPS + warp) * MG_ROWS; at < total; at += together ? grid : wide) {
-    int c = 0;                                             // the last block whose rows start at or before this one
+  auto task_of = [&](int at) {                             // the last block whose rows start at or before these
+    int c = 0;
 #pragma unroll
     for (int step = MG_MOST / 2; step > 0; step >>= 1)
       if (s_before[c + step] <= at) c += step;
-    const TreeSplit& item = s_split[c];
-    const int c0 = item.c0, n = item.n, r = at - s_before[c];
-    auto part = [&](int z, int row) { return ((size_t)(c0 + z) * 2 + (z == 0 ? item.slot0 : 0)) * a.part_rows + row; };
-    auto sink_of = [&](int row) { return a.sink && a.sink_values ? a.sink_values[item.g * G + (item.r0 + row) % G] * LOG2E : 0.f; };
-    auto place = [&](int row) {
-      return reinterpret_cast<T*>(a.out) + (size_t)(item.t0 + (item.r0 + row) / G) * a.out_ld + (size_t)(item.g * G + (item.r0 + row) % G) * hd;
-    };
-    auto stats = [&](int z, int row) { return z < n && row < item.pairs ? *reinterpret_cast<const float2*>(a.part_ml + part(z, row) * 2) : make_float2(-INFINITY, 0.f); };
-    auto values = [&](int z, int row, float (&v)[NV][VEC]) {
-      const float* const p = a.part_o + part(z, row) * hd;
+    return c;
+  };
+  // what a task takes, in trips to the L2: of a warp three and one for every segment (which is some hundred instructions to a warp by itself), of a
+  // block, which reads eight segments at a time, two and one or more for every 32 columns.  (4 x 60,000 keys, 2,048 rows in 19 segments: a
+  // warp a task 27 us, a block 10; 16 x 3,000 keys, 5,000 rows in 5 segments: a warp 8 us, a block 14.)
+  const int grid = gridDim.x, wide = grid * MG_WARPS, chunks = (hd + 31) / 32;
+  int parts = 0, trips = (total + wide - 1) / wide * (3 + most);                         // parts: blocks that share a row's columns
+  for (int p = chunks; p > 0; p = (p + 1) / 2) {
+    const int t = (total * p + grid - 1) / grid * (2 + (chunks + p - 1) / p * (32 + most) / 32);
+    if (t < trips) { trips = t; parts = p; }
+    if (p == 1) break;
+  }
+  if (parts > 0) {
+    // a lane has four columns of a row, 32 columns at a time, the warps have every eighth segment
+    for (int at = blockIdx.x; at < total * parts; at += grid) {
+      const int c = task_of(at / parts), per = (chunks + parts - 1) / parts, chunk0 = at % parts * per;
+      const TreeSplit item = a.splits[c];
+      const int n = item.n, r = (at / parts - s_before[c]) * MG_ROWS, row = r + lane % MG_ROWS, own = min(row, item.pairs - 1), h = item.g * G + (item.r0 + own) % G;
+      auto stats = [&](int z) { return *tree_part_ml(a, item.c0 + z, z == 0 ? item.slot0 : 0, own); };
+      // the statistics of the lane's row, every 64th segment a thread
+      float2 ml[MG_MOST / (MG_T / MG_ROWS)];
+      float m = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int e = 0; e < NV; e++) {
-        const int d = (lane + 32 * e) * VEC;
-        if constexpr (VEC == 4) {
-          const float4 f = d < hd ? *reinterpret_cast<const float4*>(p + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-          v[e][0] = f.x; v[e][1] = f.y; v[e][2] = f.z; v[e][3] = f.w;
-        } else v[e][0] = d < hd ? p[d] : 0.f;
-      }
-    };
-    if (together) {
-      if (r >= item.pairs) continue;                       // (filled up to four)
-      __syncthreads();                                     // the row before has been read
-      const float sv = sink_of(r);
-      float m = -INFINITY, l = 0.f, acc[NV][VEC];
-#pragma unroll
-      for (int e = 0; e < NV; e++)
-#pragma unroll
-        for (int q = 0; q < VEC; q++) acc[e][q] = 0.f;
-      float2 ml[EACH];
-#pragma unroll
-      for (int i = 0; i < EACH; i++) {
-        ml[i] = stats(i * MG_T + tid, r);
+      for (int i = 0; i < MG_MOST / (MG_T / MG_ROWS); i++) {
+        const int z = i * (MG_T / MG_ROWS) + tid / MG_ROWS;
+        ml[i] = z < n ? stats(z) : make_float2(-INFINITY, 0.f);
         if (ml[i].y != 0.f) m = fmaxf(m, ml[i].x);
       }
-      m = warp_max(m);
-      if (lane == 0) s_red[warp] = m;
+#pragma unroll
+      for (int o = MG_ROWS; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      __syncthreads();                                     // the task before has been read
+      if (lane < MG_ROWS) s_red[warp][lane] = m;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < MG_WARPS; w++) m = fmaxf(m, s_red[w]);
+      for (int w = 0; w < MG_WARPS; w++) m = fmaxf(m, s_red[w][lane % MG_ROWS]);
+      const float sv = a.sink && a.sink_values ? a.sink_values[h] * LOG2E : 0.f;
       if (a.sink) m = fmaxf(m, sv);
 #pragma unroll
-      for (int i = 0; i < EACH; i++)
-        if (i * MG_T + tid < n) {
-          const float w = ml[i].y != 0.f ? exp2f(ml[i].x - m) : 0.f;
-          s_w[i * MG_T + tid] = w;
-          if (ml[i].y != 0.f) l += ml[i].y * w;
-        }
-      l = warp_sum(l);
-      if (lane == 0) s_red[MG_WARPS + warp] = l;
+      for (int i = 0; i < MG_MOST / (MG_T / MG_ROWS); i++) {
+        const int z = i * (MG_T / MG_ROWS) + tid / MG_ROWS;
+        if (z >= n) continue;
+        const float w = ml[i].y != 0.f ? exp2f(ml[i].x - m) : 0.f;
+        s_w[z][lane % MG_ROWS] = w;
+        if (ml[i].y != 0.f) l += ml[i].y * w;
+      }
+#pragma unroll
+      for (int o = MG_ROWS; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      if (lane < MG_ROWS) s_red[MG_WARPS + warp][lane] = l;
       __syncthreads();
       l = 0.f;
 #pragma unroll
-      for (int w = 0; w < MG_WARPS; w++) l += s_red[MG_WARPS + w];
-      constexpr int Z = NV == 1 ? 12 : 4;                  // segments on their way at a time
-      for (int z0 = warp; z0 < n; z0 += Z * MG_WARPS) {
-        float v[Z][NV][VEC];
+      for (int w = 0; w < MG_WARPS; w++) l += s_red[MG_WARPS + w][lane % MG_ROWS];
+      const float inv = l == 0.f ? 0.f : 1.0f / (a.sink ? l + exp2f(sv - m) : l);
+      T* const to = reinterpret_cast<T*>(a.out) + (size_t)(item.t0 + (item.r0 + own) / G) * a.out_ld + (size_t)h * hd;
+      for (int part = chunk0; part < min(chunks, chunk0 + per); part++) {
+        const int chunk = part * 8 + lane / MG_ROWS;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int Z = 10;
+        for (int z0 = warp; z0 < n; z0 += Z * MG_WARPS) {
+          float4 v[Z];
 #pragma unroll
-        for (int z = 0; z < Z; z++)
-          if (z0 + z * MG_WARPS < n) values(z0 + z * MG_WARPS, r, v[z]);
+          for (int i = 0; i < Z; i++) {
+            const int z = min(z0 + i * MG_WARPS, n - 1);
+            v[i] = *tree_part(a, item.c0 + z, z == 0 ? item.slot0 : 0, min(chunk, (hd + 3) / 4 - 1), own);
+          }
 #pragma unroll
-        for (int z = 0; z < Z; z++) {
-          const float w = z0 + z * MG_WARPS < n ? s_w[z0 + z * MG_WARPS] : 0.f;
-          if (w == 0.f) continue;
-#pragma unroll
-          for (int e = 0; e < NV; e++)
-#pragma unroll
-            for (int q = 0; q < VEC; q++) acc[e][q] = fmaf(v[z][e][q], w, acc[e][q]);
+          for (int i = 0; i < Z; i++) {
+            const float w = z0 + i * MG_WARPS < n ? s_w[z0 + i * MG_WARPS][lane % MG_ROWS] : 0.f;
+            if (w == 0.f) continue;
+            sum.x = fmaf(v[i].x, w, sum.x);
+            sum.y = fmaf(v[i].y, w, sum.y);
+            sum.z = fmaf(v[i].z, w, sum.z);
+            sum.w = fmaf(v[i].w, w, sum.w);
+          }
         }
+        float4 (*const room)[32] = s_acc[part & 1];        // (read while the next 32 columns' are written)
+        room[warp][lane] = sum;
+        __syncthreads();
+        if (warp != part % MG_WARPS || row >= item.pairs) continue;
+        sum = room[0][lane];
+#pragma unroll
+        for (int w = 1; w < MG_WARPS; w++) {
+          const float4 o = room[w][lane];
+          sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
+        }
+        const float o[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+          if (chunk * 4 + q < hd) to[chunk * 4 + q] = from_f32<T>(l == 0.f ? 0.f : o[q] * inv);
       }
-#pragma unroll
-      for (int e = 0; e < NV; e++)
-#pragma unroll
-        for (int q = 0; q < VEC; q++) s_acc[warp][(lane + 32 * e) * VEC + q] = acc[e][q];
-      __syncthreads();
-      if (tid < hd) {
-        const float inv = l == 0.f ? 0.f : 1.0f / (a.sink ? l + exp2f(sv - m) : l);
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < MG_WARPS; w++) sum += s_acc[w][tid];
-        place(r)[tid] = from_f32<T>(l == 0.f ? 0.f : sum * inv);
-      }
-      continue;
     }
-    // four rows a warp, eight lanes a row for its segments' weights
-    constexpr int LANES = 32 / MG_ROWS;
-    const int own = r + lane / LANES;
-    const float sv = own < item.pairs ? sink_of(own) : 0.f;
-    float2 ml = stats(lane % LANES, own);
-    float m = ml.y != 0.f ? ml.x : -INFINITY, l = 0.f, acc[MG_ROWS][NV][VEC];
-    for (int z = LANES + lane % LANES; z < n; z += LANES) {
-      const float2 o = stats(z, own);
+    return;
+  }
+  for (int at = blockIdx.x * MG_WARPS + warp; at < total; at += wide) {
+    const int c = task_of(at);
+    const TreeSplit item = a.splits[c];
+    const int n = item.n, r = (at - s_before[c]) * MG_ROWS, rows = min(MG_ROWS, item.pairs - r);
+    // the weights of the rows' segments, eight lanes a row
+    const int own = r + min(lane / MG_LANES, rows - 1);
+    auto stats = [&](int z) { return z < n ? *tree_part_ml(a, item.c0 + z, z == 0 ? item.slot0 : 0, own) : make_float2(-INFINITY, 0.f); };
+    auto head = [&](int row) { return item.g * G + (item.r0 + row) % G; };
+    const float sv = a.sink && a.sink_values ? a.sink_values[head(own)] * LOG2E : 0.f;
+    float2 ml = stats(lane % MG_LANES);
+    float m = ml.y != 0.f ? ml.x : -INFINITY, l = 0.f;
+    for (int z = MG_LANES + lane % MG_LANES; z < n; z += MG_LANES) {
+      const float2 o = stats(z);
       if (o.y != 0.f) m = fmaxf(m, o.x);
     }
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = MG_LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (a.sink) m = fmaxf(m, sv);
+    float4 acc[MG_ROWS][NV];
 #pragma unroll
     for (int x = 0; x < MG_ROWS; x++)
 #pragma unroll
-      for (int e = 0; e < NV; e++)
-#pragma unroll
-        for (int q = 0; q < VEC; q++) acc[x][e][q] = 0.f;
-    for (int base = 0; base < n; base += LANES) {
-      if (base > 0) ml = stats(base + lane % LANES, own);
+      for (int e = 0; e < NV; e++) acc[x][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int base = 0; base < n; base += MG_LANES) {
+      if (base > 0) ml = stats(base + lane % MG_LANES);
       const float w = ml.y != 0.f ? exp2f(ml.x - m) : 0.f;
       if (ml.y != 0.f) l += ml.y * w;
-      constexpr int Z = NV == 1 ? 3 : 1;                   // segments of the four rows on their way at a time
-      const int stop = min(n, base + LANES);
+      const int stop = min(n, base + MG_LANES);
+      constexpr int Z = 2;                   // segments on their way at a time
       for (int z0 = base; z0 < stop; z0 += Z) {
-        float v[Z][MG_ROWS][NV][VEC];
+        float4 v[Z][MG_ROWS][NV];
 #pragma unroll
-        for (int z = 0; z < Z; z++)
+        for (int z = 0; z < Z; z++) {
+          const int at_z = z0 + z;
+          if (at_z >= stop) continue;
 #pragma unroll
-          for (int x = 0; x < MG_ROWS; x++)
-            if (z0 + z < stop && r + x < item.pairs) values(z0 + z, r + x, v[z][x]);
+          for (int e = 0; e < NV; e++) {
+            const float4* const p = tree_part(a, item.c0 + at_z, at_z == 0 ? item.slot0 : 0, min(lane + 32 * e, (hd + 3) / 4 - 1), r);
+#pragma unroll
+            for (int x = 0; x < MG_ROWS; x++) v[z][x][e] = p[min(x, rows - 1)];
+          }
+        }
 #pragma unroll
         for (int z = 0; z < Z; z++)
 #pragma unroll
           for (int x = 0; x < MG_ROWS; x++) {
-            const float wz = __shfl_sync(0xffffffffu, w, x * LANES + (z0 + z) % LANES);
-            if (z0 + z >= stop || wz == 0.f || r + x >= item.pairs) continue;
+            const float wz = __shfl_sync(0xffffffffu, w, x * MG_LANES + (z0 + z) % MG_LANES);
+            if (z0 + z >= stop || wz == 0.f) continue;
 #pragma unroll
-            for (int e = 0; e < NV; e++)
-#pragma unroll
-              for (int q = 0; q < VEC; q++) acc[x][e][q] = fmaf(v[z][x][e][q], wz, acc[x][e][q]);
+            for (int e = 0; e < NV; e++) {
+              acc[x][e].x = fmaf(v[z][x][e].x, wz, acc[x][e].x);
+              acc[x][e].y = fmaf(v[z][x][e].y, wz, acc[x][e].y);
+              acc[x][e].z = fmaf(v[z][x][e].z, wz, acc[x][e].z);
+              acc[x][e].w = fmaf(v[z][x][e].w, wz, acc[x][e].w);
+            }
           }
       }
     }
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    for (int o = MG_LANES / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     const float inv = l == 0.f ? 0.f : 1.0f / (a.sink ? l + exp2f(sv - m) : l);
 #pragma unroll
     for (int x = 0; x < MG_ROWS; x++) {
-      const float f = __shfl_sync(0xffffffffu, inv, x * LANES);
-      const bool none = __shfl_sync(0xffffffffu, l, x * LANES) == 0.f;
-      if (r + x >= item.pairs) continue;
-      T* const to = place(r + x);
+      const float f = __shfl_sync(0xffffffffu, inv, x * MG_LANES);
+      const bool none = __shfl_sync(0xffffffffu, l, x * MG_LANES) == 0.f;
+      if (x >= rows) continue;
+      T* const to = reinterpret_cast<T*>(a.out) + (size_t)(item.t0 + (item.r0 + r + x) / G) * a.out_ld + (size_t)head(r + x) * hd;
 #pragma unroll
-      for (int e = 0; e < NV; e++)
+      for (int e = 0; e < NV; e++) {
+        const float o[4] = {acc[x][e].x, acc[x][e].y, acc[x][e].z, acc[x][e].w};
 #pragma unroll
-        for (int q = 0; q < VEC; q++) {
-          const int d = (lane + 32 * e) * VEC + q;
-          if (d < hd) to[d] = from_f32<T>(none ? 0.f : acc[x][e][q] * f);
+        for (int q = 0; q < 4; q++) {
+          const int d = (lane + 32 * e) * 4 + q;
+          if (d < hd) to[d] = from_f32<T>(none ? 0.f : o[q] * f);
         }
+      }
     }
   }
 }
 
 template <typename T> void run_merge(const TreeArgs& a, cudaStream_t stream) {
-  auto* const k = a.hd % 4 != 0 ? tree_merge_kernel<T, 1, 8> : a.hd <= 128 ? tree_merge_kernel<T, 4, 1> : tree_merge_kernel<T, 4, 2>;
-  const long long rows = (long long)a.T * a.H, most = 148 * 4;           // a block a row at most, four to an SM
-  tlc_launch(k, dim3((unsigned)(rows < most ? rows : most)), dim3(MG_T), 0, stream, a);
+  const long long tasks = ((long long)a.T * a.H + MG_ROWS - 1) / MG_ROWS * ((a.hd + 31) / 32), most = 148 * 2;     // two to an SM
+  const dim3 grid((unsigned)(tasks < most ? tasks : most));
+  if (a.hd <= 128) tlc_launch(tree_merge_kernel<T, 1>, grid, dim3(MG_T), 0, stream, a);
+  else tlc_launch(tree_merge_kernel<T, 2>, grid, dim3(MG_T), 0, stream, a);
 }
 
+constexpr int SIMT_MOST_SMEM = 227 * 1024 - 1024;
+static_assert(smem_floats(256, 64) * 4 <= SIMT_MOST_SMEM && (smem_floats(192, 64) + BN * 64) * 4 <= SIMT_MOST_SMEM, "shared memory of a block");
 template <typename T, int RM> int run_simt(const TreeArgs& a, cudaStream_t stream) {
   const int nj = (a.hd + 63) / 64, smem = smem_floats(a.hd, 16 * RM) * (int)sizeof(float);
   auto* const k = nj == 1 ? tree_attention_kernel<T, RM, 1> : nj == 2 ? tree_attention_kernel<T, RM, 2> : tree_attention_kernel<T, RM, 4>;
   const int full = nj <= 2 ? smem : smem + BN * (256 - nj * 64) * (int)sizeof(float);
-  if (full > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, full) != cudaSuccess)
+  static OncePerDevice ready[3];
+  if (!ready[nj == 1 ? 0 : nj == 2 ? 1 : 2].done([&] { return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SIMT_MOST_SMEM); }))
     return tlc_fail(-2, "tree_attention: cannot reserve %d bytes of shared memory", full);
   tlc_launch(k, dim3(a.blocks), dim3(NT), (size_t)full, stream, a);
   TLC_CHECK_LAUNCH("tree_attention");
@@ -462,7 +522,7 @@ Cut cut_of(int dtype, int aligned, int n_pages, int B, int T, int H, int KV, int
   const long long wave = (long long)sms * (c.tc ? 1 : 2);
   c.blocks = (int)(c.units < wave ? (c.units < 1 ? 1 : c.units) : wave);
   if (c.blocks > MG_MOST) c.blocks = MG_MOST;
-  c.scratch = (long long)c.blocks * (2 * c.rows * (hd + 2) * 4 + (long long)sizeof(TreeSplit));
+  c.scratch = (long long)c.blocks * (2 * c.rows * ((hd + 3) / 4 * 4 + 2) * 4 + (long long)sizeof(TreeSplit));
   return c;
 }
 }  // namespace
@@ -493,11 +553,13 @@ extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void
   a.out = out; a.out_ld = out_ld; a.B = B; a.T = T; a.H = H; a.KV = KV; a.hd = hd;
   a.scale = scale; a.window = window > 0 ? window : 0; a.softcap = softcap; a.sink = sink; a.sink_values = sink_values;
   a.max_context = max_context;
+  const uintptr_t starts = (uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new | (uintptr_t)k_pages | (uintptr_t)v_pages;
+  a.vec = hd % 4 == 0 && ((ld_q | ld_k | ld_v) & 3) == 0 && (starts & (dtype == TLC_F32 ? 15 : 7)) == 0;
   a.tile_rows = c.tile_rows;
   a.blocks = c.blocks;
   a.part_rows = c.rows;
   a.part_o = (float*)scratch;
-  a.part_ml = a.part_o + (size_t)c.blocks * 2 * c.rows * hd;
+  a.part_ml = a.part_o + (size_t)c.blocks * 2 * c.rows * ((hd + 3) / 4 * 4);
   a.splits = (TreeSplit*)(a.part_ml + (size_t)c.blocks * 2 * c.rows * 2);
   if (const int rc = c.tc ? tlc_tree_attention_tc(a, stream) : tlc_tree_attention_simt(a, dtype, c.rows, stream)) return rc;
   TLC_DISPATCH_DTYPE(dtype, E, run_merge<E>(a, stream));

@@ -22,9 +22,10 @@ struct TreeArgs {
   int sink;
   const float* sink_values;
   int max_context;
+  int vec;                                                // every row starts on a boundary of four elements and holds a multiple of four
   int tile_rows;                                          // (row, head of the group) pairs of a tile
   int blocks;
-  float *part_o, *part_ml;                                // [blocks, 2, most rows of a tile, hd] and the same with 2 for hd
+  float *part_o, *part_ml;                                // [blocks, 2, hd in fours, most rows of a tile, 4] and [blocks, 2, most rows of a tile, 2]
   int part_rows;                                          // most rows of a tile
   struct TreeSplit* splits;                               // [blocks]
 };
@@ -49,6 +50,15 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
   return s;
 }
 
+// a / b of numbers that are not negative: by a 32-bit reciprocal where they are small (a plan is a chain of divisions, an integer one
+// takes four times as long)
+__device__ __forceinline__ int tree_div(int a, int b) {
+  if (a >= 1 << 22) return a / b;
+  int q = (int)__fdividef((float)a, (float)b);            // off by one at most
+  const int r = a - q * b;
+  return q + (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+
 // Units are numbered request by request, within it key/value head by head, tile by tile of rows, and tile by tile of keys; the tiles of keys of one
 // (request, head, row tile) are an item, what a block has of an item is a segment.  Segments whose item other blocks share leave their sums in
 // part_o, and another kernel adds them up.  Two ways to give the n blocks their work:
@@ -62,13 +72,13 @@ constexpr int TREE_SLACK = 4, TREE_MOST_SEQS = 2048;      // requests whose piec
 
 struct TreeShare {
   int n, per, more;
-  __device__ __forceinline__ TreeShare(int W, int blocks) : n(min(W, blocks)), per(n > 0 ? W / n : 0), more(n > 0 ? W % n : 0) {}
+  __device__ __forceinline__ TreeShare(int W, int blocks) : n(min(W, blocks)), per(n > 0 ? tree_div(W, n) : 0), more(W - per * n) {}
   __device__ __forceinline__ int first(int c) const { return c * per + min(c, more); }
-  __device__ __forceinline__ int block_of(int u) const { return u < more * (per + 1) ? u / (per + 1) : more + (u - more * (per + 1)) / per; }
+  __device__ __forceinline__ int block_of(int u) const { return u < more * (per + 1) ? tree_div(u, per + 1) : more + tree_div(u - more * (per + 1), per); }
 };
 
 struct TreeTake {
-  int b, unit, todo;                                      // the block begins with unit `unit` of request b and takes `todo` units
+  int b, item, tile, todo;                                // the block begins with key tile `tile` of item `item` of request b and takes `todo` units
   TreeSeq s;                                              // request b
 };
 
@@ -91,7 +101,7 @@ template <int NT> __device__ __forceinline__ int tree_before(int mine, int* red)
 
 // All threads of a block of NT call it.  room: 2 * min(B, TREE_MOST_SEQS) ints of shared memory.  Leaves block c's entry of splits.
 template <int NT> __device__ __forceinline__ TreeTake tree_plan(const TreeArgs& a, int c, int* room) {
-  __shared__ int red_w[NT / 32], red_i[NT / 32], red_b[NT / 32], s_piece;
+  __shared__ int red_w[NT / 32], red_i[NT / 32], red_b[NT / 32], s_piece[TREE_SLACK + 1];
   __shared__ TreeTake s_take;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (a.B + NT - 1) / NT, b0 = min(a.B, tid * each), b1 = min(a.B, b0 + each);
@@ -112,33 +122,35 @@ template <int NT> __device__ __forceinline__ TreeTake tree_plan(const TreeArgs& 
 #pragma unroll
   for (int w = 0; w < NT / 32; w++) { W += red_w[w]; I += red_i[w]; }
   const TreeShare share(W, a.blocks);
-  if (warp == 0) {
-    int piece = 0;
+  // the smallest P of mean .. mean + SLACK for which there are blocks enough, a warp each
+  static_assert(NT / 32 > TREE_SLACK, "a warp for every candidate");
+  if (warp <= TREE_SLACK) {
+    int n = 0x7fffffff;
+    const int p = tree_div(W + a.blocks - 1, a.blocks) + warp;
     if (look && I <= a.blocks && W > 0) {
-      const int mean = (W + a.blocks - 1) / a.blocks;
-      for (int p = mean; p <= mean + TREE_SLACK && piece == 0; p++) {
-        int n = 0;
-        for (int b = lane; b < a.B; b += 32) n += room[2 * b] * ((room[2 * b + 1] + p - 1) / p);
-        if ((int)__reduce_add_sync(0xffffffffu, n) <= a.blocks) piece = p;
-      }
+      n = 0;
+      for (int b = lane; b < a.B; b += 32) n += room[2 * b] * tree_div(room[2 * b + 1] + p - 1, p);
+      n = (int)__reduce_add_sync(0xffffffffu, n);
     }
-    if (lane == 0) s_piece = piece;
+    if (lane == 0) s_piece[warp] = n <= a.blocks ? p : 0;
   }
   __syncthreads();
-  const int piece = s_piece;
+  int piece = 0;
+#pragma unroll
+  for (int w = TREE_SLACK; w >= 0; w--) piece = s_piece[w] > 0 ? s_piece[w] : piece;
   TreeSplit split = {};
   if (piece > 0) {
     int mine = 0;
-    for (int b = b0; b < b1; b++) mine += room[2 * b] * ((room[2 * b + 1] + piece - 1) / piece);
+    for (int b = b0; b < b1; b++) mine += room[2 * b] * tree_div(room[2 * b + 1] + piece - 1, piece);
     int before = tree_before<NT>(mine, red_b);
     for (int b = b0; b < b1; b++) {
-      const int n = (room[2 * b + 1] + piece - 1) / piece, here = room[2 * b] * n;
+      const int n = tree_div(room[2 * b + 1] + piece - 1, piece), here = room[2 * b] * n;
       if (c >= before && c < before + here) {
         if (each > 1) s = tree_seq(a, b);
-        const int item = (c - before) / n, k = (c - before) % n, lo = k * s.key_tiles / n;
-        s_take = TreeTake{b, item * s.key_tiles + lo, (k + 1) * s.key_tiles / n - lo, s};
+        const int item = tree_div(c - before, n), k = c - before - item * n, lo = tree_div(k * s.key_tiles, n);
+        s_take = TreeTake{b, item, lo, tree_div((k + 1) * s.key_tiles, n) - lo, s};
         if (k == 0 && n > 1) {
-          const int g = item / s.row_tiles, r0 = item % s.row_tiles * a.tile_rows;
+          const int g = tree_div(item, s.row_tiles), r0 = (item - g * s.row_tiles) * a.tile_rows;
           split = TreeSplit{n, c, 0, s.t0, r0, min(a.tile_rows, s.n * (a.H / a.KV) - r0), g, 0};
         }
         a.splits[c] = split;
@@ -151,10 +163,10 @@ template <int NT> __device__ __forceinline__ TreeTake tree_plan(const TreeArgs& 
     for (int b = b0; b < b1; b++) {
       if (each > 1) s = tree_seq(a, b);
       if (first >= before && first < before + s.units) {
-        const int unit = first - before, tile = unit % s.key_tiles, u0 = first - tile;
-        s_take = TreeTake{b, unit, share.first(c + 1) - first, s};
+        const int unit = first - before, item = tree_div(unit, s.key_tiles), tile = unit - item * s.key_tiles, u0 = first - tile;
+        s_take = TreeTake{b, item, tile, share.first(c + 1) - first, s};
         if (tile > 0 && share.block_of(u0) == c - 1) {
-          const int item = unit / s.key_tiles, g = item / s.row_tiles, r0 = item % s.row_tiles * a.tile_rows;
+          const int g = tree_div(item, s.row_tiles), r0 = (item - g * s.row_tiles) * a.tile_rows;
           split = TreeSplit{share.block_of(u0 + s.key_tiles - 1) - c + 2, c - 1, share.first(c - 1) < u0 ? 1 : 0, s.t0, r0,
                             min(a.tile_rows, s.n * (a.H / a.KV) - r0), g, 0};
         }
@@ -175,6 +187,14 @@ __device__ __forceinline__ bool tree_sees(const TreeArgs& a, int t0, int i, int 
     if ((j >> 5) >= a.words || !((unsigned)a.mask[(size_t)(t0 + i) * a.words + (j >> 5)] >> (j & 31) & 1)) return false;
   } else if (j > i) return false;
   return a.window <= 0 || a.positions[t0 + j] > a.positions[t0 + i] - a.window;
+}
+
+// The four values from column 4 c on of row r in block z's slot: lanes that have a row each write whole lines, and readers take four rows.
+__device__ __forceinline__ float4* tree_part(const TreeArgs& a, int z, int slot, int c, int r) {
+  return reinterpret_cast<float4*>(a.part_o) + (((size_t)z * 2 + slot) * ((a.hd + 3) / 4) + c) * a.part_rows + r;
+}
+__device__ __forceinline__ float2* tree_part_ml(const TreeArgs& a, int z, int slot, int r) {
+  return reinterpret_cast<float2*>(a.part_ml) + ((size_t)z * 2 + slot) * a.part_rows + r;
 }
 
 int tlc_tree_attention_simt(const TreeArgs& a, int dtype, int rows, cudaStream_t stream);

@@ -118,6 +118,11 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long wait_limit = mbar_wait_limit(err);
   if (tid == 0) *dead = 0;
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TCOLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   if (warp == 8 && lane < 5) {
     const CUtensorMap* const m = lane == 0 ? &map_q : lane == 1 ? &map_k : lane == 2 ? &map_v : lane == 3 ? &map_kn : &map_vn;
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
@@ -132,14 +137,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   const TreeTake take = tree_plan<THREADS>(a, blockIdx.x, reinterpret_cast<int*>(sm));
-  int b = take.b, unit = take.unit, todo = take.todo;
+  int b = take.b, item = take.item, kt0 = take.tile, todo = take.todo;
   TreeSeq s = take.s;
-  if (todo == 0) return;
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TCOLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -156,9 +155,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll 1
   for (; todo > 0; segment++) {
   const bool first_segment = segment == 0;
-  while (unit >= s.units) { unit -= s.units; s = tree_seq(a, ++b); }
-  const int item = unit / s.key_tiles, kt0 = unit % s.key_tiles;
-  const int g = item / s.row_tiles, i0 = item % s.row_tiles * 2 * NI;
+  while (item >= a.KV * s.row_tiles) { item -= a.KV * s.row_tiles; s = tree_seq(a, ++b); }
+  const int g = tree_div(item, s.row_tiles), i0 = (item - g * s.row_tiles) * 2 * NI;
   const int n = min(s.key_tiles - kt0, todo);             // key tiles of this segment
   const int rows = min(2 * NI, s.n - i0);
   const bool pair = rows > NI;                            // two row tiles: a group each; else every second key tile for each group
@@ -420,12 +418,16 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const float inv = whole ? 1.0f / (l_keys + (with_sink ? ex2_quick(sv - m_all) : 0.f)) : 1.0f;
     const float f0 = w0 * inv, f1 = w1 * inv;
     const bool second = !pair && n > 1;                   // the second group had a tile at all (else its accumulator was never written)
-    const size_t part = ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * (2 * BM) + (pair ? wg * NI * G : 0) + r;
-    if (!whole && live && (pair || wg == 0)) {
-      a.part_ml[part * 2] = m_all;
-      a.part_ml[part * 2 + 1] = l_keys;
-    }
+    const int slot = first_segment ? 0 : 1, part_row = (pair ? wg * NI * G : 0) + r;
+    if (!whole && live && (pair || wg == 0)) *tree_part_ml(a, blockIdx.x, slot, part_row) = make_float2(m_all, l_keys);
     const bool odd = s_odd != 0;
+    // where the pieces of 16 bytes that the lane stores belong: rows 8 q + lane / 4 of the warp's
+    __nv_bfloat16* to[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int at = min(32 * quarter + q * 8 + (lane >> 2), BM - 1);
+      to[q] = (__nv_bfloat16*)a.out + (size_t)(s.t0 + first_row + at / G) * a.out_ld + (size_t)(g * G + at % G) * HD + 8 * (lane & 3);
+    }
     __syncwarp();
 #pragma unroll 1
     for (int c = 0; c < (pair ? HD / 32 : HD / 64); c++) {               // 32 output columns at a time: of a pair all, else the group's half
@@ -473,22 +475,16 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
         }
       }
-      // through 4 KB of the queries' memory of the warp's own, pieces of 16 bytes in turned order, so that a store covers whole lines
-      uint8_t* const mem = sm + L_::Q + warp * 4096;
-      __syncwarp();
       if (!whole) {
+        if (live) {
+          float4* const p = tree_part(a, blockIdx.x, slot, col / 4, part_row);
 #pragma unroll
-        for (int q = 0; q < 8; q++)
-          *reinterpret_cast<float4*>(mem + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
-        __syncwarp();
-        const size_t part0 = part - r + 32 * quarter;     // of the warp's first row
-#pragma unroll
-        for (int q = 0; q < 8; q++) {
-          const int row = q * 4 + (lane >> 3), piece = lane & 7;
-          const float4 x = *reinterpret_cast<const float4*>(mem + row * 128 + ((piece ^ (row & 7)) << 4));
-          if (32 * quarter + row < live_rows) *reinterpret_cast<float4*>(a.part_o + (part0 + row) * HD + col + 4 * piece) = x;
+          for (int q = 0; q < 8; q++) p[q * (2 * BM)] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
         }
       } else {
+        // through 2 KB of the queries' memory of the warp's own, pieces of 16 bytes in turned order, so that a store covers whole sectors
+        uint8_t* const mem = sm + L_::Q + warp * 2048;
+        __syncwarp();
 #pragma unroll
         for (int q = 0; q < 4; q++)
           *reinterpret_cast<uint4*>(mem + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
@@ -499,8 +495,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (int q = 0; q < 4; q++) {
           const int row = q * 8 + (lane >> 2), piece = lane & 3, at = 32 * quarter + row;
           const uint4 x = *reinterpret_cast<const uint4*>(mem + row * 64 + ((piece ^ (row >> 1 & 3)) << 4));
-          if (at < live_rows)
-            *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (size_t)(s.t0 + first_row + at / G) * a.out_ld + (size_t)(g * G + at % G) * HD + col + 8 * piece) = x;
+          if (at < live_rows) *reinterpret_cast<uint4*>(to[q] + col) = x;
         }
       }
     }
@@ -511,7 +506,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   todo -= n;
-  unit += n;
+  kt0 = 0;
+  item++;
   done += n;
   used0 += pair ? n : (n + 1) >> 1;
   used1 += pair ? n : n >> 1;
@@ -522,7 +518,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
 template <int HD> int run(const TreeArgs& a, cudaStream_t stream) {
   auto* const kernel = tree_attention_tc_kernel<HD>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeSmem<HD>::TOTAL) != cudaSuccess)
+  static OncePerDevice ready;
+  if (!ready.done([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeSmem<HD>::TOTAL); }))
     return tlc_fail(-2, "tree_attention(tcgen05): cannot reserve shared memory");
   const int G = a.H / a.KV, NI = BM / G;
   CUtensorMap mq, mk, mv, mkn, mvn;

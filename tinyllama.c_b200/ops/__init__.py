@@ -175,7 +175,7 @@ _SIGNATURES = {
     "tlc_tree_attention_scratch": (_ll, [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "tlc_tree_attention": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i,
                                 _i, _i, _f, _i, _f, _i, _vp, _i, _i, _vp, _i, _vp]),
-    "tlc_beam_select_scratch": (_ll, [_i, _i, _i]),
+    "tlc_beam_select_scratch": (_ll, [_i, _i]),
     "tlc_beam_select": (_i, [_vp, _ll, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "tlc_beam_reorder_states": (_i, [_vp, _ll, _ll, _ll, _i, _i, _vp, _vp, _i, _i, _vp]),
     "tlc_beam_reorder_pages": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp]),
@@ -2154,7 +2154,7 @@ def retention_chunked(proj: torch.Tensor, q_off: int, k_off: int, v_off: int, g_
 
 
 # ---- several candidates of a request over one paged cache: drafted tokens, beams ---------------------------------------------
-MAX_TABLE_REQUESTS = 8192      # page_tables.cu: MAX_REQUESTS
+MAX_TABLE_REQUESTS = 4096      # page_tables.cu: MAX_REQUESTS
 MAX_BEAMS = 64                 # beam.cu: beams of a request, and candidates of one
 MAX_POOL_PAGES = 1 << 25       # places (page * 64 + offset) are 32-bit numbers
 POOL_STATUS = {0: "done", 1: "not enough free pages", 2: "a length below 0 or beyond a row of the block table",
@@ -2164,11 +2164,13 @@ POOL_STATUS = {0: "done", 1: "not enough free pages", 2: "a length below 0 or be
 
 def _here(what: str, *tensors) -> None:
     """Tensors that one launch names lie on the device that it goes to."""
-    dev = _get_device() if _get_device is not None and torch.cuda.is_available() else None
+    dev = tensors[0].get_device()
+    if dev >= 0 and _get_device is not None and dev != _get_device():
+        raise KernelError(f"{what}: tensors on {tensors[0].device} while the current device is cuda:{_get_device()}")
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != dev):
-            _gpu(t)
-            raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{dev}")
+        if t is not None and (t.get_device() != dev or dev < 0):
+            _gpu(*tensors)
+            raise KernelError(f"{what}: tensors on {tensors[0].device} and on {t.device}")
 
 
 def _ints_of(t: torch.Tensor, n: int, what: str) -> None:
@@ -2207,7 +2209,7 @@ def page_resize(block_table: torch.Tensor, refs: torch.Tensor, lengths: torch.Te
     The pool is three int32 tensors: refs [pages] counts the entries of block_table [slots, pages a slot] that name a page (0: free),
     lengths [slots] the positions that a slot holds, in the first ceil(length / 64) pages of its row.  Pages behind the positions
     wanted are given back (their entries become 0); missing ones are the lowest free pages, in the order of the requests.  slots and
-    want are int32 [B] (at most 8,192; slot -1: nothing to do).  All of it is done or, with a code, nothing: status[0] is raised to the
+    want are int32 [B] (at most 4,096; slot -1: nothing to do).  All of it is done or, with a code, nothing: status[0] is raised to the
     largest code that occurred (POOL_STATUS) and stays until the caller clears it."""
     n_slots, max_pages = _pool(block_table, refs, lengths, status, "page_resize")
     B = slots.numel()
@@ -2407,7 +2409,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, ended: Optio
     view = ints.as_strided
     tokens, parents, best = view((R, n), (n, 1), 0), view((R, n), (n, 1), R * n), view((R, n), (n, 1), 2 * R * n).view(torch.float32)
     if R:
-        scratch = torch.empty(_beam_scratch(rows, V, n), dtype=torch.uint8, device=logits.device)
+        scratch = torch.empty(_beam_scratch(rows, V), dtype=torch.uint8, device=logits.device)
         _note_owned(ints, scratch)
         p = ints.data_ptr()
         _call_packed("tlc_beam_select", logits.data_ptr(), ld, scores.data_ptr(), gone, R, K, V, n, int(pad), 1 if placed else 0, scratch.data_ptr(),
