@@ -194,16 +194,25 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
     }
   __syncthreads();
   const int passing = s_lists;
+  // (the threshold as a logit of row k, a little lower: whatever is worth as much passes, and what is worth hardly less does no harm)
+  const float worth = __uint_as_float(least & 0x80000000u ? least & 0x7fffffffu : ~least);
+  auto push = [&](double value, float logit, int index, int mark) {
+    const int at = atomicAdd(&s_count, 1);             // (in any order: they are ranked below)
+    if (at < MERGE_CAP) { c_value[at] = logit; c_index[at] = mark; }
+    if (at < MERGE_RANK) { s_value[at] = value; s_index[at] = index; }
+  };
   auto collect = [&](int l) {
     const int k = l / n_pieces, base = l % n_pieces * 32 * VPL;
     const float* const x = logits + (size_t)(r * K + k) * ld + base;
     float v[VPL];
     load_piece<VPL, VEC>(x, V - base, lane, v);
+    const double off = s_off[k];
+    const float exact = (float)((double)worth - off), bar = least == 1u ? -3.402823466e38f : exact - 1e-6f * (fabsf(exact) + fabsf(worth));
 #pragma unroll
     for (int q = 0; q < VPL; q++)
-      if (v[q] > -INFINITY && key_of(k, v[q]) >= least) {
-        const int at = atomicAdd(&s_count, 1);         // (in any order: they are ranked below)
-        if (at < MERGE_CAP) { c_value[at] = v[q]; c_index[at] = k * V + base + (q / VEC * 32 + lane) * VEC + q % VEC; }
+      if (v[q] >= bar) {
+        const int index = k * V + base + (q / VEC * 32 + lane) * VEC + q % VEC;
+        push(off + (double)v[q], v[q], index, index);
       }
   };
   if (passing <= MERGE_LISTS) {
@@ -214,10 +223,7 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
   }
   if (ended)                                           // a beam that has ended stands for itself
     for (int k = tid; k < K; k += MERGE_T)
-      if (ended[r * K + k] && isfinite(scores[r * K + k])) {
-        const int at = atomicAdd(&s_count, 1);
-        if (at < MERGE_CAP) c_index[at] = -1 - k;
-      }
+      if (ended[r * K + k] && isfinite(scores[r * K + k])) push((double)scores[r * K + k], 0.f, k * V + pad, -1 - k);
   __syncthreads();
   const int count = s_count;
   auto value_of = [&](int e, int* index) {
@@ -231,9 +237,9 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
   };
   int found = -1;
   if (count <= MERGE_CAP) {
-    // of many a second threshold, found the same way by the whole block
-    unsigned bar = 0;
+    int ranked = count;
     if (count > MERGE_RANK) {
+      // of many a second threshold, found the same way by the whole block
       constexpr int HELD = MERGE_CAP / MERGE_T;
       unsigned held[HELD], low = 1u, high = 0xffffffffu;
 #pragma unroll
@@ -255,17 +261,16 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
         if (reach >= n) low = trial; else high = trial - 1;
         if (reach >= n && reach <= MERGE_RANK) break;
       }
-      bar = low;
+      for (int e = tid; e < count; e += MERGE_T) {
+        int index;
+        const double a = value_of(e, &index);
+        if (ordered((float)a) < low) continue;
+        const int at = atomicAdd(&s_ranked, 1);
+        if (at < MERGE_RANK) { s_value[at] = a; s_index[at] = index; }
+      }
+      __syncthreads();
+      ranked = s_ranked;
     }
-    for (int e = tid; e < count; e += MERGE_T) {
-      int index;
-      const double a = value_of(e, &index);
-      if (bar > 0 && ordered((float)a) < bar) continue;
-      const int at = atomicAdd(&s_ranked, 1);
-      if (at < MERGE_RANK) { s_value[at] = a; s_index[at] = index; }
-    }
-    __syncthreads();
-    const int ranked = s_ranked;
     if (ranked <= MERGE_RANK) {
       found = min(ranked, n);
       for (int e = tid; e < ranked; e += MERGE_T) {

@@ -2162,15 +2162,18 @@ POOL_STATUS = {0: "done", 1: "not enough free pages", 2: "a length below 0 or be
                5: "a slot that would grow inside a page it shares"}
 
 
+_I32, _BOOL = torch.int32, torch.bool
+
+
+# The functions below first ask in one expression whether a call is in order (a chain of them takes a microsecond or two); only one that is not
+# goes through the checks one by one, which say what is wrong with it.
 def _here(what: str, *tensors) -> None:
     """Tensors that one launch names lie on the device that it goes to."""
-    dev = tensors[0].get_device()
-    if dev >= 0 and _get_device is not None and dev != _get_device():
-        raise KernelError(f"{what}: tensors on {tensors[0].device} while the current device is cuda:{_get_device()}")
-    for t in tensors:
-        if t is not None and (t.get_device() != dev or dev < 0):
-            _gpu(*tensors)
-            raise KernelError(f"{what}: tensors on {tensors[0].device} and on {t.device}")
+    given = [t for t in tensors if t is not None]
+    _gpu(*given)
+    for t in given:
+        if t.get_device() != _get_device():
+            raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{_get_device()}")
 
 
 def _ints_of(t: torch.Tensor, n: int, what: str) -> None:
@@ -2178,12 +2181,9 @@ def _ints_of(t: torch.Tensor, n: int, what: str) -> None:
         raise KernelError(f"{what}: expected {n} contiguous int32 values, got {t.dtype} of shape {tuple(t.shape)}")
 
 
-def _flags(t: Optional[torch.Tensor], n: int, what: str) -> int:
-    if t is None:
-        return 0
+def _flags(t: torch.Tensor, n: int, what: str) -> None:
     if t.dtype != torch.bool or t.numel() != n or not t.is_contiguous():
         raise KernelError(f"{what}: expected {n} contiguous truth values (torch.bool), got {t.dtype} of shape {tuple(t.shape)}")
-    return t.data_ptr()
 
 
 def _table(block_table: torch.Tensor, what: str):
@@ -2202,6 +2202,17 @@ def _pool(block_table, refs, lengths, status, what: str):
     return n_slots, max_pages
 
 
+def _pool_ok(block_table, refs, lengths, status, dev: int) -> bool:
+    return (block_table.dtype is _I32 and block_table.dim() == 2 and block_table.is_contiguous() and refs.dtype is _I32 and refs.dim() == 1
+            and refs.is_contiguous() and 1 <= refs.numel() <= MAX_POOL_PAGES and lengths.dtype is _I32 and lengths.is_contiguous()
+            and lengths.numel() == block_table.shape[0] and block_table.shape[1] > 0 and status.dtype is _I32 and status.numel() > 0
+            and status.is_contiguous() and dev >= 0 and refs.get_device() == dev and lengths.get_device() == dev and status.get_device() == dev)
+
+
+def _ok(t: torch.Tensor, dtype: torch.dtype, n: int, dev: int) -> bool:
+    return t.dtype is dtype and t.numel() == n and t.is_contiguous() and t.get_device() == dev
+
+
 def page_resize(block_table: torch.Tensor, refs: torch.Tensor, lengths: torch.Tensor, slots: torch.Tensor, want: torch.Tensor,
                 status: torch.Tensor) -> None:
     """Makes slot slots[b] hold want[b] positions, for every request at once: what Cache.reserve and Cache.release do, on the GPU.
@@ -2211,13 +2222,16 @@ def page_resize(block_table: torch.Tensor, refs: torch.Tensor, lengths: torch.Te
     wanted are given back (their entries become 0); missing ones are the lowest free pages, in the order of the requests.  slots and
     want are int32 [B] (at most 4,096; slot -1: nothing to do).  All of it is done or, with a code, nothing: status[0] is raised to the
     largest code that occurred (POOL_STATUS) and stays until the caller clears it."""
-    n_slots, max_pages = _pool(block_table, refs, lengths, status, "page_resize")
-    B = slots.numel()
-    _ints_of(slots, B, "page_resize slots")
-    _ints_of(want, B, "page_resize want")
-    if B > MAX_TABLE_REQUESTS:
-        raise KernelError(f"page_resize: {B} requests; a call takes {MAX_TABLE_REQUESTS}")
-    _here("page_resize", block_table, refs, lengths, slots, want, status)
+    dev, B = block_table.get_device(), slots.numel()
+    if not (_pool_ok(block_table, refs, lengths, status, dev) and _ok(slots, _I32, B, dev) and _ok(want, _I32, B, dev) and B <= MAX_TABLE_REQUESTS
+            and dev == _get_device()):
+        _pool(block_table, refs, lengths, status, "page_resize")
+        _ints_of(slots, B, "page_resize slots")
+        _ints_of(want, B, "page_resize want")
+        if B > MAX_TABLE_REQUESTS:
+            raise KernelError(f"page_resize: {B} requests; a call takes {MAX_TABLE_REQUESTS}")
+        _here("page_resize", block_table, refs, lengths, slots, want, status)
+    n_slots, max_pages = block_table.shape
     _call_packed("tlc_page_resize", block_table.data_ptr(), n_slots, max_pages, refs.data_ptr(), refs.numel(), lengths.data_ptr(),
                  slots.data_ptr(), want.data_ptr(), B, status.data_ptr(), _stream())
 
@@ -2242,39 +2256,42 @@ def row_maps(block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor
     follows (-1: the request's last position; always smaller than the row's own index).  Positions are then start + depth, mask says which
     drafts a row sees (those above it and itself; max_new: the most rows of a request) and no row has a place, but those that
     keep (torch.bool [n_rows]) accepts.  A row whose way up is broken sees nothing and has no place.  Without parents, keep leaves out rows."""
-    n_slots, max_pages = _table(block_table, "row_maps")
-    B, T = slots.numel(), int(n_rows)
-    if B > MAX_TABLE_REQUESTS or T < 0:
-        raise KernelError(f"row_maps: {B} requests (a call takes {MAX_TABLE_REQUESTS}) of {T} rows")
-    for t, what in ((slots, "row_maps slots"), (start, "row_maps start"), (new, "row_maps new")):
-        _ints_of(t, B, what)
-    words = 0
-    if parents is not None:
-        _ints_of(parents, T, "row_maps parents")
-        if max_new < 1:
-            raise KernelError("row_maps: max_new, the most rows of a request, says how wide the drafts' masks are")
-        words = (int(max_new) + 31) // 32
-    kept = _flags(keep, T, "row_maps keep")
-    _here("row_maps", block_table, slots, start, new, parents, keep)
-    # (cut by as_strided: a tensor's own slicing costs three times as much)
-    ints = torch.empty(B + 1 + T * (3 + words), dtype=torch.int32, device=block_table.device)
+    B, T, dev = slots.numel(), int(n_rows), block_table.get_device()
+    words = 0 if parents is None else (int(max_new) + 31) // 32
+    if not (block_table.dtype is _I32 and block_table.dim() == 2 and block_table.is_contiguous() and block_table.numel() > 0 and dev >= 0
+            and dev == _get_device() and _ok(slots, _I32, B, dev) and _ok(start, _I32, B, dev) and _ok(new, _I32, B, dev) and B <= MAX_TABLE_REQUESTS
+            and T >= 0 and (parents is None or (words > 0 and _ok(parents, _I32, T, dev))) and (keep is None or _ok(keep, _BOOL, T, dev))):
+        _table(block_table, "row_maps")
+        if B > MAX_TABLE_REQUESTS or T < 0:
+            raise KernelError(f"row_maps: {B} requests (a call takes {MAX_TABLE_REQUESTS}) of {T} rows")
+        for t, what in ((slots, "row_maps slots"), (start, "row_maps start"), (new, "row_maps new")):
+            _ints_of(t, B, what)
+        if parents is not None:
+            _ints_of(parents, T, "row_maps parents")
+            if words < 1:
+                raise KernelError("row_maps: max_new, the most rows of a request, says how wide the drafts' masks are")
+        if keep is not None:
+            _flags(keep, T, "row_maps keep")
+        _here("row_maps", block_table, slots, start, new, parents, keep)
+    n_slots, max_pages = block_table.shape
+    # (cut by as_strided: a tensor's own slicing costs more)
+    ints = torch.empty(B + 1 + T * (3 + words), dtype=_I32, device=block_table.device)
     view, at = ints.as_strided, B + 1
-    maps = RowMaps(view((B + 1,), (1,), 0), view((T,), (1,), at), view((T,), (1,), at + T), view((T,), (1,), at + 2 * T),
-                   view((T, words), (words, 1), at + 3 * T) if words else None)
     p = ints.data_ptr()
     _call_packed("tlc_row_maps", block_table.data_ptr(), n_slots, max_pages, slots.data_ptr(), start.data_ptr(), new.data_ptr(), B, T,
-                 0 if parents is None else parents.data_ptr(), kept, words, p, p + 4 * at, p + 4 * (at + T), p + 4 * (at + 2 * T),
-                 p + 4 * (at + 3 * T) if words else 0, _stream())
-    _note_owned(ints)
-    return maps
+                 0 if parents is None else parents.data_ptr(), 0 if keep is None else keep.data_ptr(), words, p, p + 4 * at, p + 4 * (at + T),
+                 p + 4 * (at + 2 * T), p + 4 * (at + 3 * T) if words else 0, _stream())
+    if _notes.calls is not None:
+        _note_owned(ints)
+    return RowMaps(view((B + 1,), (1,), 0), view((T,), (1,), at), view((T,), (1,), at + T), view((T,), (1,), at + 2 * T),
+                   view((T, words), (words, 1), at + 3 * T) if words else None)
 
 
 def _layers_of_rows(t: torch.Tensor, what: str):
-    """(layers, rows, width, layer stride, row stride) of rows [T, C] or [L, T, C]."""
+    """(layers, rows, width) of rows [T, C] or [L, T, C] that are dense within a row."""
     if t.dim() not in (2, 3) or (t.shape[-1] > 1 and t.stride(-1) != 1):
         raise KernelError(f"{what}: rows [T, C] or, layer by layer, [L, T, C], dense within a row; got {tuple(t.shape)} strides {t.stride()}")
-    L, T, C = (1, *t.shape) if t.dim() == 2 else t.shape
-    return L, T, C, t.stride(0) if t.dim() == 3 and L > 1 else 0, t.stride(-2) if T > 1 else max(C, 1)
+    return (1, *t.shape) if t.dim() == 2 else tuple(t.shape)
 
 
 def _page_shape(pages: torch.Tensor, what: str):
@@ -2293,14 +2310,35 @@ def kv_store(k: torch.Tensor, v: Optional[torch.Tensor], row_map: torch.Tensor, 
     pages [n, KV, 64, hd], or [L, T, KV * hd] with pages [L, n, KV, 64, hd]; float32 or bfloat16, rounded where the pages are
     narrower; v and v_pages may be None (pages without values).  Rows of k and v may be strided.  A row without a place (-1, or one
     that does not exist) is not stored.  Places are distinct, as row_maps makes them: of two rows for one place either may stay."""
+    dev, dims = k.get_device(), k.dim()
+    if not (dims in (2, 3) and k_pages.dim() == dims + 2 and k_pages.is_contiguous() and k_pages.shape[-2] == PAGE and k_pages.get_device() == dev
+            and dev >= 0 and dev == _get_device() and k.stride(-1) == 1 and k.shape[-1] == k_pages.shape[-3] * k_pages.shape[-1]
+            and _ok(row_map, _I32, k.shape[-2], dev) and (dims == 2 or k.shape[0] == k_pages.shape[0]) and 1 <= k_pages.shape[-4] <= MAX_POOL_PAGES
+            and k_pages.numel() > 0
+            and ((v is None and v_pages is None) or (v is not None and v_pages is not None and v.shape == k.shape and v.dtype is k.dtype
+                 and v_pages.shape == k_pages.shape and v_pages.dtype is k_pages.dtype and v_pages.is_contiguous() and v.stride(-1) == 1
+                 and v.get_device() == dev and v_pages.get_device() == dev))):
+        _kv_store_checks(k, v, row_map, k_pages, v_pages)
+    if dims == 3:
+        L, T, C = k.shape
+        n, KV, _, hd = k_pages.shape[1:]
+    else:
+        (T, C), L = k.shape, 1
+        n, KV, _, hd = k_pages.shape
+    sk = k.stride()
+    sv = (0,) * dims if v is None else v.stride()
+    _call_packed("tlc_kv_store", k.data_ptr(), 0 if v is None else v.data_ptr(), dtype_code(k.dtype), sk[0] if L > 1 else 0, sv[0] if L > 1 else 0, sk[-2],
+                 sv[-2], row_map.data_ptr(), k_pages.data_ptr(), 0 if v is None else v_pages.data_ptr(), dtype_code(k_pages.dtype), L, T, n, KV, hd,
+                 _stream())
+
+
+def _kv_store_checks(k, v, row_map, k_pages, v_pages) -> None:
     L, n, KV, hd = _page_shape(k_pages, "kv_store")
     if (v is None) != (v_pages is None) or (v_pages is not None and (v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype)):
         raise KernelError("kv_store: values and their pages come together, the pages alike")
-    l, T, C, layer_k, ld_k = _layers_of_rows(k, "kv_store keys")
-    layer_v = ld_v = 0
+    l, T, C = _layers_of_rows(k, "kv_store keys")
     if v is not None:
-        lv, tv, cv, layer_v, ld_v = _layers_of_rows(v, "kv_store values")
-        if (lv, tv, cv) != (l, T, C) or v.dtype != k.dtype:
+        if _layers_of_rows(v, "kv_store values") != (l, T, C) or v.dtype != k.dtype:
             raise KernelError(f"kv_store: keys {tuple(k.shape)} {k.dtype} and values {tuple(v.shape)} {v.dtype} do not agree")
         if not v_pages.is_contiguous():
             raise KernelError("kv_store: pages must be contiguous")
@@ -2308,9 +2346,6 @@ def kv_store(k: torch.Tensor, v: Optional[torch.Tensor], row_map: torch.Tensor, 
         raise KernelError(f"kv_store: rows {tuple(k.shape)} do not fit pages {tuple(k_pages.shape)}")
     _ints_of(row_map, T, "kv_store row_map")
     _here("kv_store", k, v, row_map, k_pages, v_pages)
-    _call_packed("tlc_kv_store", k.data_ptr(), 0 if v is None else v.data_ptr(), dtype_code(k.dtype), layer_k, layer_v, ld_k, ld_v,
-                 row_map.data_ptr(), k_pages.data_ptr(), 0 if v is None else v_pages.data_ptr(), dtype_code(k_pages.dtype), L, T, n, KV, hd,
-                 _stream())
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2333,8 +2368,42 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     position is above its own - window.  softcap, sink and sink_values as in attention().  max_context and max_new bound the contexts and the
     requests' new rows (a longer context is cut).  A row that sees nothing is 0; rows behind the last request are left as they were;
     a key or value that a row does not see does not touch it, whatever it holds.  float32 or bfloat16, heads of up to 256."""
-    T, B = q.shape[0], slots.numel()
-    dt = q.dtype
+    T, B, dt, dev = q.shape[0], slots.numel(), q.dtype, q.get_device()
+    words = 0 if mask is None or mask.dim() != 2 else mask.shape[1]
+    sq, sk, sv, so = q.stride(), k_new.stride(), v_new.stride(), out.stride()
+    if not (1 <= hd <= MAX_HEAD_DIM and KV >= 1 and H >= 1 and H % KV == 0 and T > 0 and B > 0 and dev >= 0 and dev == _get_device()
+            and q.shape == out.shape == (T, H * hd) and k_new.shape == v_new.shape == (T, KV * hd)
+            and sq[1] == sk[1] == sv[1] == so[1] == 1 and k_new.dtype is dt and v_new.dtype is dt and out.dtype is dt and k_pages.dtype is dt
+            and v_pages.dtype is dt and k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.dim() == 4 and v_pages.shape == k_pages.shape
+            and k_pages.shape[1:] == (KV, PAGE, hd) and k_pages.shape[0] > 0 and block_table.dtype is _I32 and block_table.dim() == 2
+            and block_table.is_contiguous() and block_table.numel() > 0 and _ok(slots, _I32, B, dev) and _ok(start, _I32, B, dev)
+            and _ok(cu_seqlens, _I32, B + 1, dev) and _ok(positions, _I32, T, dev)
+            and (mask is None or (words > 0 and 32 * words >= max_new and _ok(mask, _I32, T * words, dev)))
+            and (sink_values is None or _ok(sink_values, torch.float32, H, dev)) and max_context >= 0 and max_new >= 0 and window >= 0
+            and (softcap == 0 or (softcap > 0 and scale != 0)) and k_new.get_device() == dev and v_new.get_device() == dev and out.get_device() == dev
+            and k_pages.get_device() == dev and v_pages.get_device() == dev and block_table.get_device() == dev):
+        _tree_attention_checks(q, k_new, v_new, k_pages, v_pages, block_table, slots, start, cu_seqlens, positions, out, H, KV, hd, scale, max_context,
+                               max_new, mask, window, softcap, sink_values)
+        if T == 0 or B == 0:
+            return
+    ld_q, ld_k, ld_v, ld_o = (sq[0], sk[0], sv[0], so[0]) if T > 1 else (H * hd, KV * hd, KV * hd, H * hd)
+    n_slots, max_pages = block_table.shape
+    code = dtype_code(dt)
+    pq, pk, pv, pkp, pvp, po = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
+    aligned = 0 if (pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7 else 1
+    max_context, max_new = min(int(max_context), max_pages * PAGE), int(max_new)
+    scratch = torch.empty(_tree_scratch(dev, code, aligned, k_pages.shape[0], B, T, H, KV, hd, max_context, max_new), dtype=torch.uint8, device=q.device)
+    if _notes.calls is not None:
+        _note_owned(scratch)
+    _call_packed("tlc_tree_attention", pq, code, ld_q, pk, ld_k, pv, ld_v, pkp, pvp, k_pages.shape[0], block_table.data_ptr(), n_slots, max_pages,
+                 slots.data_ptr(), start.data_ptr(), cu_seqlens.data_ptr(), positions.data_ptr(), 0 if mask is None else mask.data_ptr(), words,
+                 po, ld_o, B, T, H, KV, hd, scale, int(window), softcap, 1 if sink or sink_values is not None else 0,
+                 0 if sink_values is None else sink_values.data_ptr(), max_context, max_new, scratch.data_ptr(), aligned, _stream())
+
+
+def _tree_attention_checks(q, k_new, v_new, k_pages, v_pages, block_table, slots, start, cu_seqlens, positions, out, H, KV, hd, scale, max_context,
+                           max_new, mask, window, softcap, sink_values) -> None:
+    T, B, dt = q.shape[0], slots.numel(), q.dtype
     if not (1 <= hd <= MAX_HEAD_DIM) or H < 1 or KV < 1 or H % KV:
         raise KernelError(f"tree_attention: {H} heads over {KV} key/value heads of size {hd} (at most {MAX_HEAD_DIM})")
     if q.dim() != 2 or q.shape[1] != H * hd or tuple(k_new.shape) != (T, KV * hd) or tuple(v_new.shape) != (T, KV * hd):
@@ -2348,34 +2417,22 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
         raise KernelError("tree_attention: max_context, max_new, window and softcap are not negative")
     if softcap > 0 and scale == 0:
         raise KernelError("tree_attention: capped scores need a scale")
-    n_slots, max_pages = _table(block_table, "tree_attention")
+    _table(block_table, "tree_attention")
     _ints_of(slots, B, "tree_attention slots")
     _ints_of(start, B, "tree_attention start")
     _ints_of(cu_seqlens, B + 1, "tree_attention cu_seqlens")
     _ints_of(positions, T, "tree_attention positions")
-    words = 0
     if mask is not None:
         if mask.dim() != 2 or mask.shape[1] * 32 < max_new:
             raise KernelError(f"tree_attention: masks are int32 [T, words] with a bit for each of {max_new} rows, got {tuple(mask.shape)}")
-        words = mask.shape[1]
-        _ints_of(mask, T * words, "tree_attention mask")
+        _ints_of(mask, T * mask.shape[1], "tree_attention mask")
     if sink_values is not None:
         _f32vec(sink_values, H, "tree_attention sink scores")
-    ld_q, ld_k, ld_v, ld_o = _rows(q, "tree_attention q"), _rows(k_new, "tree_attention k_new"), _rows(v_new, "tree_attention v_new"), \
-        _out_rows(out, T, H * hd, "tree_attention")
+    for t, what in ((q, "q"), (k_new, "k_new"), (v_new, "v_new")):
+        _rows(t, "tree_attention " + what)
+    _out_rows(out, T, H * hd, "tree_attention")
+    dtype_code(dt)
     _here("tree_attention", q, k_new, v_new, k_pages, v_pages, block_table, slots, start, cu_seqlens, positions, out, mask, sink_values)
-    if T == 0 or B == 0:
-        return
-    code = dtype_code(dt)
-    pq, pk, pv, pkp, pvp, po = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
-    aligned = 0 if (pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7 else 1
-    max_context, max_new = min(int(max_context), max_pages * PAGE), int(max_new)
-    scratch = torch.empty(_tree_scratch(q.get_device(), code, aligned, k_pages.shape[0], B, T, H, KV, hd, max_context, max_new), dtype=torch.uint8, device=q.device)
-    _note_owned(scratch)
-    _call_packed("tlc_tree_attention", pq, code, ld_q, pk, ld_k, pv, ld_v, pkp, pvp, k_pages.shape[0], block_table.data_ptr(), n_slots, max_pages,
-                 slots.data_ptr(), start.data_ptr(), cu_seqlens.data_ptr(), positions.data_ptr(), 0 if mask is None else mask.data_ptr(), words,
-                 po, ld_o, B, T, H, KV, hd, scale, int(window), softcap, 1 if sink or sink_values is not None else 0,
-                 0 if sink_values is None else sink_values.data_ptr(), max_context, max_new, scratch.data_ptr(), aligned, _stream())
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2394,27 +2451,38 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, ended: Optio
     pairs follow with a score of -infinity.  The best comes first; placed (n = K): the first child of a beam takes its parent's
     place and the others, in order, the places that are left, so that only beams without children are overwritten (beam_reorder_*).
     K and n at most 64."""
+    n, dev = int(n), logits.get_device()
+    if not (scores.dim() == 2 and logits.dim() == 2 and logits.dtype is torch.float32 and dev >= 0 and dev == _get_device()
+            and _ok(scores, torch.float32, scores.numel(), dev) and logits.shape[0] == scores.numel() and 1 <= scores.shape[1] <= MAX_BEAMS
+            and 1 <= n <= MAX_BEAMS and n <= scores.shape[1] * logits.shape[1] and (not placed or n == scores.shape[1]) and 0 <= pad < logits.shape[1]
+            and logits.stride(1) == 1 and (ended is None or _ok(ended, _BOOL, scores.numel(), dev))):
+        _beam_select_checks(logits, scores, n, ended, pad, placed)
+    (R, K), (rows, V) = scores.shape, logits.shape
+    size = 4 * (3 * R * n + (-3 * R * n) % 4)              # tokens, parents and scores, then room for the kernels on a 16-byte boundary
+    room = torch.empty((size + (_beam_scratch(rows, V) if R else 0)) // 4, dtype=_I32, device=logits.device)
+    view, p = room.as_strided, room.data_ptr()
+    if R:
+        if _notes.calls is not None:
+            _note_owned(room)
+        _call_packed("tlc_beam_select", logits.data_ptr(), logits.stride(0) if rows > 1 else V, scores.data_ptr(), 0 if ended is None else ended.data_ptr(), R, K, V, n,
+                     int(pad), 1 if placed else 0, p + size, p, p + 4 * R * n, p + 8 * R * n, _stream())
+    return view((R, n), (n, 1), 0), view((R, n), (n, 1), R * n), view((R, n), (n, 1), 2 * R * n).view(torch.float32)
+
+
+def _beam_select_checks(logits, scores, n, ended, pad, placed) -> None:
     if scores.dim() != 2 or logits.dim() != 2 or logits.dtype != torch.float32:
         raise KernelError(f"beam_select: float32 logits [R * K, V] and scores [R, K], got {logits.dtype} {tuple(logits.shape)} and {tuple(scores.shape)}")
-    (R, K), (rows, V), n = scores.shape, logits.shape, int(n)
+    (R, K), (rows, V) = scores.shape, logits.shape
     if rows != R * K or not 1 <= K <= MAX_BEAMS or V < 1 or not 1 <= n <= min(MAX_BEAMS, K * V) or (placed and n != K):
         raise KernelError(f"beam_select: {n} candidates of {R} requests with {K} beams (at most {MAX_BEAMS}) from logits {tuple(logits.shape)}"
                           + (" in the beams' places" if placed else ""))
     if not 0 <= pad < V:
         raise KernelError(f"beam_select: token {pad} of {V}")
     _f32vec(scores, R * K, "beam_select scores")
-    ld, gone = _rows(logits, "beam_select logits"), _flags(ended, R * K, "beam_select ended")
+    _rows(logits, "beam_select logits")
+    if ended is not None:
+        _flags(ended, R * K, "beam_select ended")
     _here("beam_select", logits, scores, ended)
-    ints = torch.empty(3 * R * n, dtype=torch.int32, device=logits.device)
-    view = ints.as_strided
-    tokens, parents, best = view((R, n), (n, 1), 0), view((R, n), (n, 1), R * n), view((R, n), (n, 1), 2 * R * n).view(torch.float32)
-    if R:
-        scratch = torch.empty(_beam_scratch(rows, V), dtype=torch.uint8, device=logits.device)
-        _note_owned(ints, scratch)
-        p = ints.data_ptr()
-        _call_packed("tlc_beam_select", logits.data_ptr(), ld, scores.data_ptr(), gone, R, K, V, n, int(pad), 1 if placed else 0, scratch.data_ptr(),
-                     p, p + 4 * R * n, p + 8 * R * n, _stream())
-    return tokens, parents, best
 
 
 def _beams(slots: torch.Tensor, parents: torch.Tensor, what: str):
@@ -2429,7 +2497,19 @@ def beam_reorder_states(state: torch.Tensor, slots: torch.Tensor, parents: torch
     """Beam k of request r, in slot slots[r, k], goes on from beam parents[r, k]: state [layers, slots, ...] (any type; what a slot holds is
     dense) is permuted in place, every layer in one launch.  Any map of beams to parents will do; slot -1 or a parent outside 0 .. K - 1
     leaves a beam as it is.  The slots of a call are distinct."""
-    R, K = _beams(slots, parents, "beam_reorder_states")
+    dev = state.get_device()
+    if not (slots.dim() == 2 and parents.shape == slots.shape and 1 <= slots.shape[1] <= MAX_BEAMS and _ok(slots, _I32, slots.numel(), dev)
+            and _ok(parents, _I32, slots.numel(), dev) and state.dim() >= 2 and state.is_contiguous() and dev >= 0 and dev == _get_device()
+            and state.numel() * state.element_size() < 1 << 30):
+        _beam_states_checks(state, slots, parents)
+    (R, K), (L, n_slots), strides, size = slots.shape, state.shape[:2], state.stride(), state.element_size()
+    if state.numel() and R:
+        _call_packed("tlc_beam_reorder_states", state.data_ptr(), strides[0] * size, strides[1] * size, state.numel() // (L * n_slots) * size, L, n_slots,
+                     slots.data_ptr(), parents.data_ptr(), R, K, _stream())
+
+
+def _beam_states_checks(state, slots, parents) -> None:
+    _beams(slots, parents, "beam_reorder_states")
     if state.dim() < 2:
         raise KernelError(f"beam_reorder_states: states are [layers, slots, ...], got {tuple(state.shape)}")
     size, values = state.element_size(), 1
@@ -2443,9 +2523,6 @@ def beam_reorder_states(state: torch.Tensor, slots: torch.Tensor, parents: torch
     if values * size >= (1 << 31) - (1 << 20) or (L > 1 and state.stride(0) < values):
         raise KernelError(f"beam_reorder_states: {values * size} bytes a slot, strides {state.stride()}")
     _here("beam_reorder_states", state, slots, parents)
-    if L and n_slots and values and R:
-        _call_packed("tlc_beam_reorder_states", state.data_ptr(), state.stride(0) * size, state.stride(1) * size, values * size, L, n_slots,
-                     slots.data_ptr(), parents.data_ptr(), R, K, _stream())
 
 
 def beam_reorder_pages(block_table: torch.Tensor, refs: torch.Tensor, lengths: torch.Tensor, slots: torch.Tensor, parents: torch.Tensor,
@@ -2458,19 +2535,30 @@ def beam_reorder_pages(block_table: torch.Tensor, refs: torch.Tensor, lengths: t
 
     slots and parents int32 [R, K]; slot -1 or a parent outside 0 .. K - 1 leaves a beam as it is.  A request for which it cannot be done
     (no page of its own, one that others share, a slot named twice) stays as it is, with a code in status (see page_resize)."""
-    R, K = _beams(slots, parents, "beam_reorder_pages")
-    n_slots, max_pages = _pool(block_table, refs, lengths, status, "beam_reorder_pages")
-    L, n, KV, hd = _page_shape(k_pages, "beam_reorder_pages")
+    dev, dims = k_pages.get_device(), k_pages.dim()
+    if not (slots.dim() == 2 and parents.shape == slots.shape and 1 <= slots.shape[1] <= MAX_BEAMS and _pool_ok(block_table, refs, lengths, status, dev)
+            and block_table.get_device() == dev and dev == _get_device() and _ok(slots, _I32, slots.numel(), dev) and _ok(parents, _I32, slots.numel(), dev)
+            and dims in (4, 5) and k_pages.is_contiguous() and k_pages.numel() > 0 and k_pages.shape[-2] == PAGE and k_pages.shape[-4] == refs.numel()
+            and (v_pages is None or (v_pages.shape == k_pages.shape and v_pages.dtype is k_pages.dtype and v_pages.is_contiguous()
+                                     and v_pages.get_device() == dev))):
+        _beam_pages_checks(block_table, refs, lengths, slots, parents, k_pages, v_pages, status)
+    (R, K), (n_slots, max_pages), (n, KV, _, hd) = slots.shape, block_table.shape, k_pages.shape[-4:]
+    if not R:
+        return
+    own = torch.empty(4 * R * K, dtype=_I32, device=block_table.device)
+    if _notes.calls is not None:
+        _note_owned(own)
+    _call_packed("tlc_beam_reorder_pages", block_table.data_ptr(), n_slots, max_pages, refs.data_ptr(), n, lengths.data_ptr(), slots.data_ptr(),
+                 parents.data_ptr(), R, K, k_pages.data_ptr(), 0 if v_pages is None else v_pages.data_ptr(), dtype_code(k_pages.dtype),
+                 k_pages.shape[0] if dims == 5 else 1, KV, hd, own.data_ptr(), status.data_ptr(), _stream())
+
+
+def _beam_pages_checks(block_table, refs, lengths, slots, parents, k_pages, v_pages, status) -> None:
+    _beams(slots, parents, "beam_reorder_pages")
+    _pool(block_table, refs, lengths, status, "beam_reorder_pages")
+    _, n, _, _ = _page_shape(k_pages, "beam_reorder_pages")
     if n != refs.numel():
         raise KernelError(f"beam_reorder_pages: {n} pages and {refs.numel()} counts")
     if v_pages is not None and (v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or not v_pages.is_contiguous()):
         raise KernelError("beam_reorder_pages: pages of keys and of values are alike")
     _here("beam_reorder_pages", block_table, refs, lengths, slots, parents, k_pages, v_pages, status)
-    if not R:
-        return
-    code = dtype_code(k_pages.dtype)
-    own = torch.empty(4 * R * K, dtype=torch.int32, device=block_table.device)
-    _note_owned(own)
-    _call_packed("tlc_beam_reorder_pages", block_table.data_ptr(), n_slots, max_pages, refs.data_ptr(), n, lengths.data_ptr(), slots.data_ptr(),
-                 parents.data_ptr(), R, K, k_pages.data_ptr(), 0 if v_pages is None else v_pages.data_ptr(), code, L, KV, hd, own.data_ptr(),
-                 status.data_ptr(), _stream())
