@@ -4,8 +4,10 @@
 // 128 / G rows with all of their heads, and a block takes two such tiles with every key tile that it fetches: 2 operations a pair and
 // byte of keys and values, so it is bound by HBM up to some 250 pairs (measured peaks, 1,648 TFLOP/s over 6,553 GB/s).
 // Queries come by TMA as boxes of {64 columns, G heads, 128 / G rows}, key tiles as boxes of 64 rows from the pages or, the drafts', from
-// the projections' own rows.  One agent warp each starts the copies, issues S = Q K^T (M 128, N 64, K hd; operands as in the prompts'
-// kernel, attention_prefill_tc.cu) and O += P V (M 128, N hd, K 64; V an MN-major operand); one for both products was half as quick.  Two groups of four worker warps have a score
+// the projections' own rows.  One agent warp starts the copies, one issues O += P V (M 128, N hd, K 64; V an MN-major operand), and two issue
+// S = Q K^T (M 128, N 64, K hd; operands as in the prompts' kernel, attention_prefill_tc.cu): such a product keeps the thread that issues
+// it for the 540 cycles that it runs, and 600 more go by in waits and commits before the thread's next (one agent for the scores of both row
+// tiles took 2,300 cycles a key tile, one for all products 3,400).  Two groups of four worker warps have a score
 // buffer, two buffers of weights and an output accumulator each, all in tensor memory (a thread a row): they take one row tile each, or, of a
 // request with one row tile, every second key tile; either way products alternate between the groups, and step u is group u % 2's.
 // The weights P = 2^(s - m) go to the second product from tensor memory too, which
@@ -25,7 +27,7 @@ namespace {
 
 constexpr int BM = 128, BN = TLC_PAGE;
 constexpr int KS = 4, VS = 6;            // stages of the K and V rings: scores are made two tiles ahead, so keys leave earlier
-constexpr int WORKERS = 256, THREADS = WORKERS + 96, NG = 2;
+constexpr int WORKERS = 256, THREADS = WORKERS + 128, NG = 2;
 constexpr float TAU = 8.0f;              // how far (in powers of two) a row's maximum may run ahead of its reference
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -128,10 +130,10 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
   tlc_wait(a.v_new, a.v_pages, a.block_table, a.slots, a.start, a.cu, a.positions, a.mask, a.out, a.part_o, a.part_ml, a.splits);
-  if (warp == 9) {                                        // every worker warp arrives once on s_free and p_ready, one agent on the rest
+  if (warp == 9) {                                        // every worker warp arrives once on s_free and p_ready, two agents on k_empty, one on the rest
     for (int i = lane; i < L_::N_BARS; i += 32) {
       const int own = i - (1 + 2 * KS + 2 * VS);
-      mbar_init(bar_q + 8 * i, own >= 2 && own < 8 ? 4 : 1);
+      mbar_init(bar_q + 8 * i, own >= 2 && own < 8 ? 4 : i >= 1 + KS && i < 1 + 2 * KS ? 2 : 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -218,25 +220,27 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     } else if (lane == 0) {
       constexpr uint32_t idesc_s = instr_desc(BM, BN), idesc_o = instr_desc(BM, HD) | (1u << 16);             // V is MN-major: hd runs along its rows
       const int steps = pair ? 2 * n : n;                 // step u: group u % 2, key tile u / 2 of a pair, else u
-      auto scores = [&](int u) {
-        const int w = u & 1, tile = done + (pair ? u >> 1 : u), st = tile % KS, all = (u >> 1) + (w ? used1 : used0);
-        if (!pair || w == 0) wait(k_full(st), (uint32_t)((tile / KS) & 1), 62);
-        if (all > 0) wait(s_free(w), (uint32_t)((all - 1) & 1), 63);                 // the workers hold the scores before in registers
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t q_lo = desc_lo(sm0 + L_::Q + (pair ? w * L_::Q_TILE : 0)), k_lo = desc_lo(sm0 + L_::K + st * L_::K_STAGE);
-#pragma unroll
-        for (int c = 0; c < HD / 64; c++)
-#pragma unroll
-          for (int kk = 0; kk < 4; kk++)
-            umma_halves(tmem + (uint32_t)(w * BN), q_lo + (uint32_t)((c * L_::Q_SLAB + kk * 32) >> 4), k_lo + (uint32_t)((c * L_::K_SLAB + kk * 32) >> 4),
-                        DESC_HI, idesc_s, (c > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(s_full(w));
-        if (!pair || w == 1) umma_commit(k_empty(st));
-      };
-      if (role == 1) {
+      if (role < 3) {
+        const int w = role - 1;
         wait(bar_q, (uint32_t)(segment & 1), 61);
+        const uint32_t q_lo = desc_lo(sm0 + L_::Q + (pair ? w * L_::Q_TILE : 0));
 #pragma unroll 1
-        for (int u = 0; u < steps; u++) scores(u);
+        for (int u = w; u < steps; u += 2) {
+          const int tile = done + (pair ? u >> 1 : u), st = tile % KS, all = (u >> 1) + (w ? used1 : used0);
+          wait(k_full(st), (uint32_t)((tile / KS) & 1), 62);
+          if (all > 0) wait(s_free(w), (uint32_t)((all - 1) & 1), 63);               // the workers hold the scores before in registers
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t k_lo = desc_lo(sm0 + L_::K + st * L_::K_STAGE);
+#pragma unroll
+          for (int c = 0; c < HD / 64; c++)
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+              umma_halves(tmem + (uint32_t)(w * BN), q_lo + (uint32_t)((c * L_::Q_SLAB + kk * 32) >> 4), k_lo + (uint32_t)((c * L_::K_SLAB + kk * 32) >> 4),
+                          DESC_HI, idesc_s, (c > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(s_full(w));
+          umma_commit(k_empty(st));                       // (two arrivals: the agents' of a pair, else both by the one whose tile it is)
+          if (!pair) mbar_arrive(k_empty(st));
+        }
       } else
 #pragma unroll 1
       for (int u = 0; u < steps; u++) {
