@@ -208,12 +208,15 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
     load_piece<VPL, VEC>(x, V - base, lane, v);
     const double off = s_off[k];
     const float exact = (float)((double)worth - off), bar = least == 1u ? -3.402823466e38f : exact - 1e-6f * (fabsf(exact) + fabsf(worth));
+    // which of them reach it; those few are read once more (a body for each of 64 values would not fit the instruction cache)
+    unsigned long long who = 0;
 #pragma unroll
-    for (int q = 0; q < VPL; q++)
-      if (v[q] >= bar) {
-        const int index = k * V + base + (q / VEC * 32 + lane) * VEC + q % VEC;
-        push(off + (double)v[q], v[q], index, index);
-      }
+    for (int q = 0; q < VPL; q++) who |= (unsigned long long)(v[q] >= bar) << q;
+    for (; who != 0; who &= who - 1) {
+      const int q = __ffsll((long long)who) - 1, at = (q / VEC * 32 + lane) * VEC + q % VEC;
+      const float f = x[at];
+      push(off + (double)f, f, k * V + base + at, k * V + base + at);
+    }
   };
   if (passing <= MERGE_LISTS) {
     for (int i = warp; i < passing; i += MERGE_WARPS) collect(s_list[i]);
