@@ -90,7 +90,7 @@ struct TreeSmem {
 };
 static_assert(TreeSmem<128>::TOTAL <= 227 * 1024 - 512, "shared memory of a block");
 
-template <int HD>
+template <int HD, bool CAPPED>
 __global__ void __launch_bounds__(THREADS, 1)
 tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kn,
@@ -318,7 +318,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (lane == 0) mbar_arrive(s_free(wg));             // the scores are in registers: the buffer may take the next
       const int all = used + mine;
       const bool p_free = all < 2 || mbar_try(pv_done(wg, all & 1), (uint32_t)((all / 2 - 1) & 1));       // the weights of two steps before have been used
-      if (cap_in > 0.f) {
+      if constexpr (CAPPED) {
         // a capped score: s <- cap tanh(s scale / cap), left divided by the scale (what follows multiplies by it);
         // tanh(x) = 1 - 2 / (e^(2x) + 1), cap_in = 2 log2(e) scale / cap, cap_out = cap / scale
 #pragma unroll
@@ -448,37 +448,6 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
 #pragma unroll
       for (int e = 0; e < 32; e++) acc[e] = none ? 0.f : acc[e];
-      if (odd && live) {
-        // values that are no numbers, for the rows that see them (a positive weight times NaN or infinity is that again)
-        for (int j = 0; j < n; j++) {
-          const bool draft = kt0 + j >= s.context_tiles;
-          const int base = draft ? (kt0 + j - s.context_tiles) * BN : (s.first_tile + kt0 + j) * BN;
-          const int keys = min(BN, (draft ? s.n : s.context) - base);
-          if (!(draft || keys < BN || base < lo_most)) continue;
-          const int page = draft ? 0 : a.block_table[(size_t)a.slots[b] * a.max_pages + base / BN];
-          if (page < 0 || page >= a.n_pages) continue;
-          for (int k = 0; k < keys; k++) {
-            if (!(draft ? tree_sees(a, s.t0, i, base + k) : base + k >= lo_r)) continue;
-            const __nv_bfloat16* v = draft ? (const __nv_bfloat16*)a.v_new + (size_t)(s.t0 + base + k) * a.ld_v + (size_t)g * HD + col
-                                           : (const __nv_bfloat16*)a.v_pages + (((size_t)page * a.KV + g) * BN + k) * HD + col;
-#pragma unroll 1
-            for (int q = 0; q < 4; q++) {
-              const uint4 w = *reinterpret_cast<const uint4*>(v + 8 * q);
-              uint32_t x[4] = {w.x, w.y, w.z, w.w}, y[4] = {w.x, w.y, w.z, w.w};
-              bool any = false;
-#pragma unroll
-              for (int e = 0; e < 4; e++) any |= make_finite(y[e]);
-              if (!any) continue;
-#pragma unroll
-              for (int e = 0; e < 32; e++)
-                if (e / 8 == q) {
-                  const float f = __uint_as_float(e % 2 ? x[e % 8 / 2] & 0xffff0000u : x[e % 8 / 2] << 16);
-                  if (!isfinite(f)) acc[e] += f;
-                }
-            }
-          }
-        }
-      }
       if (!whole) {
         if (live) {
           float4* const p = tree_part(a, blockIdx.x, slot, col / 4, part_row);
@@ -503,6 +472,34 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
       }
     }
+    if (odd) {
+      // values that are no numbers, into the results of the rows that see them (a positive weight times NaN or infinity is that again).
+      // In line and without unrolling: a function of its own, with the arguments in memory, costs every launch 1.5 us.
+      __syncwarp();                                       // (a row's result was stored by several lanes of its warp)
+      __nv_bfloat16* const result = (__nv_bfloat16*)a.out + (size_t)t * a.out_ld + (size_t)h * HD;
+      const int col = pair ? 0 : wg * (HD / 2), cols = pair ? HD : HD / 2;
+#pragma unroll 1
+      for (int j = live ? 0 : n; j < n; j++) {
+        const bool draft = kt0 + j >= s.context_tiles;
+        const int base = draft ? (kt0 + j - s.context_tiles) * BN : (s.first_tile + kt0 + j) * BN;
+        const int keys = min(BN, (draft ? s.n : s.context) - base);
+        const int page = draft ? 0 : a.block_table[(size_t)a.slots[b] * a.max_pages + base / BN];
+        if (!(draft || keys < BN || base < lo_most) || page < 0 || page >= a.n_pages) continue;
+        const __nv_bfloat16* v = draft ? (const __nv_bfloat16*)a.v_new + (size_t)(s.t0 + base) * a.ld_v + (size_t)g * HD
+                                       : (const __nv_bfloat16*)a.v_pages + ((size_t)page * a.KV + g) * BN * HD;
+#pragma unroll 1
+        for (int k = 0; k < keys; k++, v += draft ? a.ld_v : HD) {
+          if (!(draft ? tree_sees(a, s.t0, i, base + k) : base + k >= lo_r)) continue;
+#pragma unroll 1
+          for (int d = col; d < col + cols; d++) {
+            const float f = __bfloat162float(v[d]);
+            if (isfinite(f)) continue;
+            if (whole) result[d] = __float2bfloat16_rn(__bfloat162float(result[d]) + f);
+            else reinterpret_cast<float*>(tree_part(a, blockIdx.x, slot, d / 4, part_row))[d % 4] += f;
+          }
+        }
+      }
+    }
   }
   // every agent is done with the segment: its copies have landed, its products have completed (the workers read
   // their last results, the loader saw the last commits), tensor memory and shared memory may be written again
@@ -520,8 +517,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TCOLS) : "memory");
 }
 
-template <int HD> int run(const TreeArgs& a, cudaStream_t stream) {
-  auto* const kernel = tree_attention_tc_kernel<HD>;
+template <int HD, bool CAPPED> int run(const TreeArgs& a, cudaStream_t stream) {
+  auto* const kernel = tree_attention_tc_kernel<HD, CAPPED>;
   static OncePerDevice ready;
   if (!ready.done([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeSmem<HD>::TOTAL); }))
     return tlc_fail(-2, "tree_attention(tcgen05): cannot reserve shared memory");
@@ -547,4 +544,7 @@ bool tlc_tree_attention_tc_takes(int dtype, int aligned, int H, int KV, int hd, 
   return dtype == TLC_BF16 && aligned && (hd == 64 || hd == 128) && H / KV <= BM && n_pages * KV * BN < (1ll << 31) - BN && tlc_error_words_here() != nullptr;
 }
 
-int tlc_tree_attention_tc(const TreeArgs& a, cudaStream_t stream) { return a.hd == 64 ? run<64>(a, stream) : run<128>(a, stream); }
+int tlc_tree_attention_tc(const TreeArgs& a, cudaStream_t stream) {
+  if (a.softcap > 0.f) return a.hd == 64 ? run<64, true>(a, stream) : run<128, true>(a, stream);
+  return a.hd == 64 ? run<64, false>(a, stream) : run<128, false>(a, stream);
+}
