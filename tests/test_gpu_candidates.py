@@ -352,6 +352,97 @@ def test_tree_attention_bad_values_stay_where_they_are_seen(dtype, hd, bad):
     assert bool((got[T0:c["cu"][2], 2:][~hit] == clean[T0:c["cu"][2], 2:][~hit]).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tree_attention_many_requests_and_long_chains(dtype):
+    """More requests than the pieces are looked at for; rows that fill several tiles of keys and of queries."""
+    B = 2100
+    c = attention_case(dtype, [b % 70 for b in range(B)], [1 + b % 2 for b in range(B)], 2, 1, 64, seed=11)
+    out = attention_run(c)
+    full = attention_run(dict(c, slots=c["slots"], new=c["new"]))
+    assert torch.equal(out, full)
+    got = out.float().cpu().double().view(c["T"], 2, 64)
+    for b in range(0, B, 97):
+        rows, ctx = slice(c["cu"][b], c["cu"][b + 1]), c["context"][b]
+        at = [c["table"][c["slots"][b]][j // PAGE] * PAGE + j % PAGE for j in range(ctx)]
+        k, v = (torch.cat([p.transpose(1, 2).reshape(-1, 1, 64)[at], r[rows].reshape(-1, 1, 64)]) for p, r in ((c["kp"], c["k"]), (c["vp"], c["v"])))
+        part = plain.tree_sees([0, c["new"][b]], [ctx], c["positions"][rows], c["parents"][rows], [ctx], 0, c["new"][b])[0]
+        o, A, S = plain.tree_attention(c["q"][rows].reshape(-1, 2, 64), k, v, part, c["scale"])
+        E = 2 * 68 * U * S[..., None] + 2 * (168 + len(k)) * U
+        assert bool(((got[rows] - o).abs() <= E * A + (HALF * (o.abs() + A) if dtype == torch.bfloat16 else U * o.abs()) + 1e-30).all())
+    c = attention_case(dtype, [70, 3], [300, 190], 4, 2, 64, drafts=False, seed=12)
+    attention_check(c, attention_run(c))
+    attention_check(c, attention_run(c, window=100), 100)
+
+
+def test_offsets_beyond_32_bits():
+    """A pool of 4.6 GB of keys and as many of values, the last pages in use: places, rows, attention and reordering at its far end."""
+    n, KV, hd = 140000, 2, 128
+    pages = [torch.empty(n, KV, PAGE, hd, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    assert pages[0].numel() > 1 << 31
+    pool = plain.Pool(2, 3, n)
+    pool.refs = [1] * (n - 4) + [0] * 4                               # all but the last pages are somebody else's
+    dev = DevicePool(pool)
+    assert pool.resize([0, 1], [100, 100]) == 0
+    dev.resize([0, 1], [100, 100])
+    dev.equals(pool)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    k, v = (torch.randn(200, KV * hd, device=DEV, generator=g).bfloat16() for _ in range(2))
+    maps = ops.row_maps(dev.table, ints([0, 1]), ints([0, 0]), ints([100, 100]), 200)
+    assert int(maps.row_map.min()) >= (n - 4) * PAGE
+    ops.kv_store(k, v, maps.row_map, *pages)
+    where = maps.row_map.long()
+    assert torch.equal(pages[0][where // PAGE, :, where % PAGE].view(200, -1), k) and torch.equal(pages[1][where // PAGE, :, where % PAGE].view(200, -1), v)
+    q = torch.randn(2, 4 * hd, device=DEV, generator=g).bfloat16()
+    outs = [torch.empty_like(q) for _ in range(2)]
+    wide = torch.empty(2, 4 * hd + 1, dtype=torch.bfloat16, device=DEV)[:, 1:]                  # off 16-byte boundaries: the other kernel
+    wide.copy_(q)
+    for o, x in zip(outs, (q, wide)):
+        ops.tree_attention(x, k[:2], v[:2], *pages, dev.table, ints([0, 1]), ints([100, 100]), ints([0, 1, 2]), ints([100, 100]), o, 4, KV, hd, 0.088,
+                           max_context=100, max_new=1, mask=ints([[0], [0]]))
+    for r in range(2):
+        K, V = (x[100 * r:100 * r + 100].view(100, KV, hd).cpu() for x in (k, v))
+        o, A, S = plain.tree_attention(q[r:r + 1].view(1, 4, hd).cpu(), K, V, torch.ones(1, 100, dtype=torch.bool), 0.088)
+        allow = (2 * (hd + 4) * U * S[..., None] + 2 * 268 * U) * A + HALF * (o.abs() + A)
+        for out in outs:
+            assert bool(((out[r].view(1, 4, hd).cpu().double() - o).abs() <= allow).all())
+    ops.beam_reorder_pages(dev.table, dev.refs, dev.lengths, ints([[0, 1]]), ints([[0, 0]]), *pages, dev.status)
+    pool.reorder([0, 1], [0, 0])
+    dev.equals(pool)
+    a, b = pool.table[0][1], pool.table[1][1]
+    assert a != b and torch.equal(pages[0][a, :, :36], pages[0][b, :, :36]) and dev.status.tolist() == [0]
+
+
+def test_calls_made_again_and_tensors_elsewhere(monkeypatch):
+    """Calls noted and made again from the library's table; a call while another device is current is refused."""
+    import numpy as np
+    pool = plain.Pool(2, 2, 8)
+    dev = DevicePool(pool)
+    q = torch.randn(3, 64, device=DEV)
+    pages = torch.zeros(8, 1, PAGE, 64, device=DEV)
+    out, state, logits = torch.zeros(3, 64, device=DEV), torch.randn(1, 2, 5, device=DEV), torch.randn(2, 30, device=DEV)
+    slots, length, three, beams, up, scores = ints([0]), ints([3]), ints([3]), ints([[0, 1]]), ints([[0, 0]]), torch.zeros(1, 2, device=DEV)
+    zero, cu, pos, place = ints([0]), ints([0, 3]), ints([0, 1, 2]), ints([64, 65, 66])
+    calls = [lambda: ops.page_resize(dev.table, dev.refs, dev.lengths, slots, length, dev.status), lambda: ops.row_maps(dev.table, slots, zero, three, 3),
+             lambda: ops.kv_store(q, q, place, pages, pages), lambda: ops.beam_select(logits, scores, 2), lambda: ops.beam_reorder_states(state, beams, up),
+             lambda: ops.tree_attention(q, q, q, pages, pages, dev.table, slots, zero, cu, pos, out, 1, 1, 64, 0.1, max_context=0, max_new=3),
+             lambda: ops.beam_reorder_pages(dev.table, dev.refs, dev.lengths, beams, ints([[0, 1]]), pages, None, dev.status)]
+    with ops.noting() as notes:
+        for call in calls:
+            call()
+    assert notes.complete and len(notes.functions) == len(calls)
+    first = out.clone()
+    out.zero_()
+    dev.lengths.zero_()
+    dev.refs.zero_()
+    ops.replay(np.array(notes.functions, dtype=np.int32), np.array(notes.words, dtype=np.uint64), 1)
+    torch.cuda.synchronize()
+    assert torch.equal(out, first) and dev.lengths.tolist() == [3, 0] and dev.refs.tolist() == [1] + [0] * 7 and dev.status.tolist() == [0]
+    monkeypatch.setattr(ops, "_get_device", lambda: 1)
+    for call in calls:
+        with pytest.raises(ops.KernelError, match="current device"):
+            call()
+
+
 def test_tree_attention_repeats_itself_and_replays():
     c = attention_case(torch.bfloat16, [900, 64, 2000], [33, 5, 64], 8, 2, 128, seed=8)
     first = attention_run(c)

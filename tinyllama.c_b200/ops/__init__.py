@@ -2221,7 +2221,8 @@ def page_resize(block_table: torch.Tensor, refs: torch.Tensor, lengths: torch.Te
     lengths [slots] the positions that a slot holds, in the first ceil(length / 64) pages of its row.  Pages behind the positions
     wanted are given back (their entries become 0); missing ones are the lowest free pages, in the order of the requests.  slots and
     want are int32 [B] (at most 4,096; slot -1: nothing to do).  All of it is done or, with a code, nothing: status[0] is raised to the
-    largest code that occurred (POOL_STATUS) and stays until the caller clears it."""
+    largest code that occurred (POOL_STATUS) and stays until the caller clears it.  Calls on one pool follow one another (on one stream, or
+    ordered by events)."""
     dev, B = block_table.get_device(), slots.numel()
     if not (_pool_ok(block_table, refs, lengths, status, dev) and _ok(slots, _I32, B, dev) and _ok(want, _I32, B, dev) and B <= MAX_TABLE_REQUESTS
             and dev == _get_device()):
@@ -2367,8 +2368,10 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     positions int32 [T]: the rows' positions, none below its request's start; with window > 0 a row sees the keys whose
     position is above its own - window.  softcap, sink and sink_values as in attention().  max_context and max_new bound the contexts and the
     requests' new rows (a longer context is cut).  A row that sees nothing is 0; rows behind the last request are left as they were;
-    a key or value that a row does not see does not touch it, whatever it holds.  float32 or bfloat16, heads of up to 256."""
+    a key or value that a row does not see does not touch it, whatever it holds.  float32 or bfloat16, heads of up to 256.  How the
+    keys are cut among blocks goes by the whole call: a row's sums may be added up in another order beside other requests."""
     T, B, dt, dev = q.shape[0], slots.numel(), q.dtype, q.get_device()
+    window, softcap = int(window or 0), float(softcap or 0.0)
     words = 0 if mask is None or mask.dim() != 2 else mask.shape[1]
     sq, sk, sv, so = q.stride(), k_new.stride(), v_new.stride(), out.stride()
     if not (1 <= hd <= MAX_HEAD_DIM and KV >= 1 and H >= 1 and H % KV == 0 and T > 0 and B > 0 and dev >= 0 and dev == _get_device()
@@ -2397,7 +2400,7 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
         _note_owned(scratch)
     _call_packed("tlc_tree_attention", pq, code, ld_q, pk, ld_k, pv, ld_v, pkp, pvp, k_pages.shape[0], block_table.data_ptr(), n_slots, max_pages,
                  slots.data_ptr(), start.data_ptr(), cu_seqlens.data_ptr(), positions.data_ptr(), 0 if mask is None else mask.data_ptr(), words,
-                 po, ld_o, B, T, H, KV, hd, scale, int(window), softcap, 1 if sink or sink_values is not None else 0,
+                 po, ld_o, B, T, H, KV, hd, scale, window, softcap, 1 if sink or sink_values is not None else 0,
                  0 if sink_values is None else sink_values.data_ptr(), max_context, max_new, scratch.data_ptr(), aligned, _stream())
 
 
@@ -2534,7 +2537,8 @@ def beam_reorder_pages(block_table: torch.Tensor, refs: torch.Tensor, lengths: t
     starts from one sequence by giving each other beam a slot of length 1 and the parent 0.
 
     slots and parents int32 [R, K]; slot -1 or a parent outside 0 .. K - 1 leaves a beam as it is.  A request for which it cannot be done
-    (no page of its own, one that others share, a slot named twice) stays as it is, with a code in status (see page_resize)."""
+    (no page of its own, one that others share, a slot named twice) stays as it is, with a code in status (see page_resize).  No two
+    requests of a call name one slot; calls on one pool follow one another."""
     dev, dims = k_pages.get_device(), k_pages.dim()
     if not (slots.dim() == 2 and parents.shape == slots.shape and 1 <= slots.shape[1] <= MAX_BEAMS and _pool_ok(block_table, refs, lengths, status, dev)
             and block_table.get_device() == dev and dev == _get_device() and _ok(slots, _I32, slots.numel(), dev) and _ok(parents, _I32, slots.numel(), dev)
