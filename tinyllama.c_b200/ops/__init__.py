@@ -2275,17 +2275,17 @@ def row_maps(block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor
             _flags(keep, T, "row_maps keep")
         _here("row_maps", block_table, slots, start, new, parents, keep)
     n_slots, max_pages = block_table.shape
-    # (cut by as_strided: a tensor's own slicing costs more)
-    ints = torch.empty(B + 1 + T * (3 + words), dtype=_I32, device=block_table.device)
-    view, at = ints.as_strided, B + 1
-    p = ints.data_ptr()
+    ints = block_table.new_empty(B + 1 + T * (3 + words))
+    at, p = B + 1, ints.data_ptr()
     _call_packed("tlc_row_maps", block_table.data_ptr(), n_slots, max_pages, slots.data_ptr(), start.data_ptr(), new.data_ptr(), B, T,
                  0 if parents is None else parents.data_ptr(), 0 if keep is None else keep.data_ptr(), words, p, p + 4 * at, p + 4 * (at + T),
                  p + 4 * (at + 2 * T), p + 4 * (at + 3 * T) if words else 0, _stream())
     if _notes.calls is not None:
         _note_owned(ints)
-    return RowMaps(view((B + 1,), (1,), 0), view((T,), (1,), at), view((T,), (1,), at + T), view((T,), (1,), at + 2 * T),
-                   view((T, words), (words, 1), at + 3 * T) if words else None)
+    if not words:                                          # (one call that cuts: half the time of four slices)
+        return RowMaps(*ints.split_with_sizes((at, T, T, T)))
+    cu_seqlens, row_seq, positions, row_map, mask = ints.split_with_sizes((at, T, T, T, T * words))
+    return RowMaps(cu_seqlens, row_seq, positions, row_map, mask.view(T, words))
 
 
 def _layers_of_rows(t: torch.Tensor, what: str):
@@ -2311,25 +2311,25 @@ def kv_store(k: torch.Tensor, v: Optional[torch.Tensor], row_map: torch.Tensor, 
     pages [n, KV, 64, hd], or [L, T, KV * hd] with pages [L, n, KV, 64, hd]; float32 or bfloat16, rounded where the pages are
     narrower; v and v_pages may be None (pages without values).  Rows of k and v may be strided.  A row without a place (-1, or one
     that does not exist) is not stored.  Places are distinct, as row_maps makes them: of two rows for one place either may stay."""
-    dev, dims = k.get_device(), k.dim()
-    if not (dims in (2, 3) and k_pages.dim() == dims + 2 and k_pages.is_contiguous() and k_pages.shape[-2] == PAGE and k_pages.get_device() == dev
-            and dev >= 0 and dev == _get_device() and k.stride(-1) == 1 and k.shape[-1] == k_pages.shape[-3] * k_pages.shape[-1]
-            and _ok(row_map, _I32, k.shape[-2], dev) and (dims == 2 or k.shape[0] == k_pages.shape[0]) and 1 <= k_pages.shape[-4] <= MAX_POOL_PAGES
-            and k_pages.numel() > 0
-            and ((v is None and v_pages is None) or (v is not None and v_pages is not None and v.shape == k.shape and v.dtype is k.dtype
-                 and v_pages.shape == k_pages.shape and v_pages.dtype is k_pages.dtype and v_pages.is_contiguous() and v.stride(-1) == 1
-                 and v.get_device() == dev and v_pages.get_device() == dev))):
+    dev, rows, sk, pages, sv = k.get_device(), k.shape, k.stride(), k_pages.shape, ()
+    dims, ok = len(rows), False
+    if (dims == 2 or dims == 3) and len(pages) == dims + 2:
+        n, KV, size, hd = pages[-4:]
+        ok = (size == PAGE and rows[-1] == KV * hd > 0 and sk[-1] == 1 and (dims == 2 or rows[0] == pages[0]) and 1 <= n <= MAX_POOL_PAGES
+              and k_pages.is_contiguous() and k_pages.get_device() == dev and dev >= 0 and dev == _get_device() and _ok(row_map, _I32, rows[-2], dev))
+        if ok and v is not None and v_pages is not None:
+            sv = v.stride()
+            ok = (v.shape == rows and v.dtype is k.dtype and sv[-1] == 1 and v_pages.shape == pages and v_pages.dtype is k_pages.dtype
+                  and v_pages.is_contiguous() and v.get_device() == dev and v_pages.get_device() == dev)
+        else:
+            ok = ok and v is None and v_pages is None
+    if not ok:
         _kv_store_checks(k, v, row_map, k_pages, v_pages)
-    if dims == 3:
-        L, T, C = k.shape
-        n, KV, _, hd = k_pages.shape[1:]
-    else:
-        (T, C), L = k.shape, 1
-        n, KV, _, hd = k_pages.shape
-    sk = k.stride()
-    sv = (0,) * dims if v is None else v.stride()
-    _call_packed("tlc_kv_store", k.data_ptr(), 0 if v is None else v.data_ptr(), dtype_code(k.dtype), sk[0] if L > 1 else 0, sv[0] if L > 1 else 0, sk[-2],
-                 sv[-2], row_map.data_ptr(), k_pages.data_ptr(), 0 if v is None else v_pages.data_ptr(), dtype_code(k_pages.dtype), L, T, n, KV, hd,
+        n, KV, _, hd = pages[-4:]
+        sv = () if v is None else v.stride()
+    L, T = rows[0] if dims == 3 else 1, rows[-2]
+    _call_packed("tlc_kv_store", k.data_ptr(), v.data_ptr() if sv else 0, dtype_code(k.dtype), sk[0] if L > 1 else 0, sv[0] if sv and L > 1 else 0, sk[-2],
+                 sv[-2] if sv else 0, row_map.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr() if sv else 0, dtype_code(k_pages.dtype), L, T, n, KV, hd,
                  _stream())
 
 
