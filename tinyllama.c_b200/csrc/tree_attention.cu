@@ -37,7 +37,7 @@ tree_attention_kernel(TreeArgs a) {
            a.splits);
   constexpr int ROWS = 16 * RM;
   extern __shared__ float4 tree_raw[];
-  const int hd = a.hd, hp = padded(hd), hv = NJ * 64, G = a.H / a.KV;
+  const int hd = a.hd, hp = padded(hd), hv = NJ * 64, G = a.G;
   float* const Q = reinterpret_cast<float*>(tree_raw);
   float* const K = Q + ROWS * hp;
   float* const V = K + BN * hp;
@@ -252,6 +252,24 @@ tree_attention_kernel(TreeArgs a) {
   }
 }
 
+__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
+  const __nv_bfloat162 u[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+  *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(u);
+}
+// four columns from d on of a row of hd, times f
+template <typename T> __device__ __forceinline__ void put4(const TreeArgs& a, T* row, int d, float4 v, float f, bool none) {
+  v = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+  if (a.vec_out) {
+    if (d < a.hd) store4(row + d, v);
+    return;
+  }
+  const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int q = 0; q < 4; q++)
+    if (d + q < a.hd) row[d + q] = from_f32<T>(o[q]);
+}
+
 // Items that several blocks share: o = sum_z o_z 2^(m_z - m) / (sum_z l_z 2^(m_z - m) [+ 2^(sink - m)]).  Every block reads which items those
 // are (an entry of splits for each block of the kernel before) and takes its share of their rows, four at a time, which lie side by
 // side: of few rows in many segments a block, or one for some of the columns, the segments shared out over its warps, else a warp.  Bound by trips to
@@ -266,7 +284,7 @@ tree_merge_kernel(TreeArgs a) {
   __shared__ int s_before[MG_MOST], s_warp[MG_WARPS], s_most[MG_WARPS];
   __shared__ float s_w[MG_MOST][MG_ROWS], s_red[2 * MG_WARPS][MG_ROWS];
   __shared__ float4 s_acc[2][MG_WARPS][32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.H / a.KV, hd = a.hd;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.G, hd = a.hd;
   // the items' rows, in fours, and the most segments of an item
   constexpr int EACH = MG_MOST / MG_T;
   int total = 0, most = 0;
@@ -391,10 +409,7 @@ tree_merge_kernel(TreeArgs a) {
           const float4 o = room[w][lane];
           sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
         }
-        const float o[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-          if (chunk * 4 + q < hd) to[chunk * 4 + q] = from_f32<T>(l == 0.f ? 0.f : o[q] * inv);
+        put4(a, to, chunk * 4, sum, inv, l == 0.f);
       }
     }
     return;
@@ -467,14 +482,7 @@ tree_merge_kernel(TreeArgs a) {
       if (x >= rows) continue;
       T* const to = reinterpret_cast<T*>(a.out) + (size_t)(item.t0 + (item.r0 + r + x) / G) * a.out_ld + (size_t)head(r + x) * hd;
 #pragma unroll
-      for (int e = 0; e < NV; e++) {
-        const float o[4] = {acc[x][e].x, acc[x][e].y, acc[x][e].z, acc[x][e].w};
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const int d = (lane + 32 * e) * 4 + q;
-          if (d < hd) to[d] = from_f32<T>(none ? 0.f : o[q] * f);
-        }
-      }
+      for (int e = 0; e < NV; e++) put4(a, to, (lane + 32 * e) * 4, acc[x][e], f, none);
     }
   }
 }
@@ -554,6 +562,8 @@ extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void
   a.scale = scale; a.window = window > 0 ? window : 0; a.softcap = softcap; a.sink = sink; a.sink_values = sink_values;
   a.max_context = max_context;
   const uintptr_t starts = (uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new | (uintptr_t)k_pages | (uintptr_t)v_pages;
+  a.G = H / KV;
+  a.vec_out = hd % 4 == 0 && (out_ld & 3) == 0 && ((uintptr_t)out & (dtype == TLC_F32 ? 15 : 7)) == 0;
   a.vec = hd % 4 == 0 && ((ld_q | ld_k | ld_v) & 3) == 0 && (starts & (dtype == TLC_F32 ? 15 : 7)) == 0;
   a.tile_rows = c.tile_rows;
   a.blocks = c.blocks;

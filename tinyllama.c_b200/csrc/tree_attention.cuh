@@ -22,13 +22,23 @@ struct TreeArgs {
   int sink;
   const float* sink_values;
   int max_context;
-  int vec;                                                // every row starts on a boundary of four elements and holds a multiple of four
+  int G;                                                  // query heads of a key/value head
+  int vec, vec_out;                                       // every input row, every output row starts on a boundary of four elements, with heads of fours
   int tile_rows;                                          // (row, head of the group) pairs of a tile
   int blocks;
   float *part_o, *part_ml;                                // [blocks, 2, hd in fours, most rows of a tile, 4] and [blocks, 2, most rows of a tile, 2]
   int part_rows;                                          // most rows of a tile
   struct TreeSplit* splits;                               // [blocks]
 };
+
+// a / b of numbers that are not negative: by a 32-bit reciprocal where they are small (a plan is a chain of divisions, an integer one
+// takes four times as long)
+__device__ __forceinline__ int tree_div(int a, int b) {
+  if (a >= 1 << 22) return a / b;
+  int q = (int)__fdividef((float)a, (float)b);            // off by one at most
+  const int r = a - q * b;
+  return q + (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
+}
 
 // A request: its rows, how much of its context there is to see, and in how many units of work (one key/value head, one tile of
 // rows, one tile of 64 keys) it comes.
@@ -45,18 +55,9 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
   s.first_tile = a.window > 0 ? max(0, s.context + 1 - a.window) / TLC_PAGE : 0;
   s.context_tiles = (s.context + TLC_PAGE - 1) / TLC_PAGE - s.first_tile;
   s.key_tiles = s.context_tiles + (s.n + TLC_PAGE - 1) / TLC_PAGE;
-  s.row_tiles = (s.n * (a.H / a.KV) + a.tile_rows - 1) / a.tile_rows;
+  s.row_tiles = tree_div(s.n * a.G + a.tile_rows - 1, a.tile_rows);
   s.units = a.KV * s.row_tiles * s.key_tiles;
   return s;
-}
-
-// a / b of numbers that are not negative: by a 32-bit reciprocal where they are small (a plan is a chain of divisions, an integer one
-// takes four times as long)
-__device__ __forceinline__ int tree_div(int a, int b) {
-  if (a >= 1 << 22) return a / b;
-  int q = (int)__fdividef((float)a, (float)b);            // off by one at most
-  const int r = a - q * b;
-  return q + (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
 }
 
 // Units are numbered request by request, within it key/value head by head, tile by tile of rows, and tile by tile of keys; the tiles of keys of one
@@ -151,7 +152,7 @@ template <int NT> __device__ __forceinline__ TreeTake tree_plan(const TreeArgs& 
         s_take = TreeTake{b, item, lo, tree_div((k + 1) * s.key_tiles, n) - lo, s};
         if (k == 0 && n > 1) {
           const int g = tree_div(item, s.row_tiles), r0 = (item - g * s.row_tiles) * a.tile_rows;
-          split = TreeSplit{n, c, 0, s.t0, r0, min(a.tile_rows, s.n * (a.H / a.KV) - r0), g, 0};
+          split = TreeSplit{n, c, 0, s.t0, r0, min(a.tile_rows, s.n * a.G - r0), g, 0};
         }
         a.splits[c] = split;
       }
@@ -168,7 +169,7 @@ template <int NT> __device__ __forceinline__ TreeTake tree_plan(const TreeArgs& 
         if (tile > 0 && share.block_of(u0) == c - 1) {
           const int g = tree_div(item, s.row_tiles), r0 = (item - g * s.row_tiles) * a.tile_rows;
           split = TreeSplit{share.block_of(u0 + s.key_tiles - 1) - c + 2, c - 1, share.first(c - 1) < u0 ? 1 : 0, s.t0, r0,
-                            min(a.tile_rows, s.n * (a.H / a.KV) - r0), g, 0};
+                            min(a.tile_rows, s.n * a.G - r0), g, 0};
         }
         a.splits[c] = split;
       }

@@ -149,7 +149,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (mbar_try(bar, parity) || *dead) return;
     if (!mbar_wait(bar, parity, err, code, wait_limit)) *dead = 1;
   };
-  const int G = a.H / a.KV, NI = BM / G;                  // drafted rows of a tile
+  const int G = a.G, NI = tree_div(BM, G);                // drafted rows of a tile
   const float scale_log2 = a.scale * LOG2E;
   // Barriers are made once: what each agent counts goes on from segment to segment.  done: key tiles of earlier segments; used0, used1:
   // how often a group's buffers have been used in them.
