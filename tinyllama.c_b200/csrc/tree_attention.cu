@@ -276,8 +276,9 @@ template <typename T> __device__ __forceinline__ void put4(const TreeArgs& a, T*
 // the L2, of which rows take two (the statistics, then the values of some segments at a time); a launch with nothing to add up is over
 // after one.
 constexpr int MG_T = 256, MG_WARPS = MG_T / 32, MG_MOST = 512;           // MG_MOST: blocks of the kernel before, at most
-constexpr int MG_ROWS = 4, MG_LANES = 32 / MG_ROWS;                      // rows of a task, lanes that look after a row's statistics
-template <typename T, int NV>
+constexpr int MG_ROWS = 4, MG_LANES = 32 / MG_ROWS;                      // rows of a task, lanes to a row
+constexpr int MG_E = 2;                                                  // fours of columns of a lane where a warp has the task
+template <typename T>
 __global__ void __launch_bounds__(MG_T)
 tree_merge_kernel(TreeArgs a) {
   tlc_pdl(a.part_o, a.part_ml, a.splits, a.out);
@@ -326,13 +327,14 @@ tree_merge_kernel(TreeArgs a) {
       if (s_before[c + step] <= at) c += step;
     return c;
   };
-  // what a task takes, in trips to the L2: of a warp three and one for every segment (which is some hundred instructions to a warp by itself), of a
-  // block, which reads eight segments at a time, two and one or more for every 32 columns.  (4 x 60,000 keys, 2,048 rows in 19 segments: a
-  // warp a task 27 us, a block 10; 16 x 3,000 keys, 5,000 rows in 5 segments: a warp 8 us, a block 14.)
-  const int grid = gridDim.x, wide = grid * MG_WARPS, chunks = (hd + 31) / 32;
-  int parts = 0, trips = (total + wide - 1) / wide * (3 + most);                         // parts: blocks that share a row's columns
+  // what a task takes, in half trips to the L2: of a warp, which reads eight segments at a time, six and four for each eight; of a block, which has
+  // eight warps do that, four and two or more for every 32 columns.  (4 x 60,000 keys, 2,048 rows in 19 segments: warps 88 us with the kernel before,
+  // blocks 97; 60,000 keys, 512 rows in 74 segments: warps 57, blocks 40; 16 x 1,000 keys, 2,048 rows in 2 segments: warps 17, blocks 38; 45,000 and
+  // 60,000 keys, 888 rows in 37 segments: warps 64, blocks 59.)
+  const int grid = gridDim.x, wide = grid * MG_WARPS, chunks = (hd + 31) / 32, cuts = (hd + 32 * MG_E - 1) / (32 * MG_E);
+  int parts = 0, trips = (total * cuts + wide - 1) / wide * (6 + (most + 7) / 8 * 4);  // parts: blocks that share a row's columns
   for (int p = chunks; p > 0; p = (p + 1) / 2) {
-    const int t = (total * p + grid - 1) / grid * (2 + (chunks + p - 1) / p * (32 + most) / 32);
+    const int t = (total * p + grid - 1) / grid * (4 + (chunks + p - 1) / p * (32 + most) / 16);
     if (t < trips) { trips = t; parts = p; }
     if (p == 1) break;
   }
@@ -414,84 +416,63 @@ tree_merge_kernel(TreeArgs a) {
     }
     return;
   }
-  for (int at = blockIdx.x * MG_WARPS + warp; at < total; at += wide) {
-    const int c = task_of(at);
+  for (int at = blockIdx.x * MG_WARPS + warp; at < total * cuts; at += wide) {
+    const int c = task_of(at / cuts), chunk = at % cuts * (8 * MG_E) + lane / MG_ROWS, last = (hd + 3) / 4 - 1;
     const TreeSplit item = a.splits[c];
-    const int n = item.n, r = (at - s_before[c]) * MG_ROWS, rows = min(MG_ROWS, item.pairs - r);
-    // the weights of the rows' segments, eight lanes a row
-    const int own = r + min(lane / MG_LANES, rows - 1);
+    const int n = item.n, row = (at / cuts - s_before[c]) * MG_ROWS + lane % MG_ROWS, own = min(row, item.pairs - 1), h = item.g * G + (item.r0 + own) % G;
+    // a lane has every eighth four columns of a row, and the statistics of every eighth segment
     auto stats = [&](int z) { return z < n ? *tree_part_ml(a, item.c0 + z, z == 0 ? item.slot0 : 0, own) : make_float2(-INFINITY, 0.f); };
-    auto head = [&](int row) { return item.g * G + (item.r0 + row) % G; };
-    const float sv = a.sink && a.sink_values ? a.sink_values[head(own)] * LOG2E : 0.f;
-    float2 ml = stats(lane % MG_LANES);
+    const float sv = a.sink && a.sink_values ? a.sink_values[h] * LOG2E : 0.f;
+    float2 ml = stats(lane / MG_ROWS);
     float m = ml.y != 0.f ? ml.x : -INFINITY, l = 0.f;
-    for (int z = MG_LANES + lane % MG_LANES; z < n; z += MG_LANES) {
+    for (int z = MG_LANES + lane / MG_ROWS; z < n; z += MG_LANES) {
       const float2 o = stats(z);
       if (o.y != 0.f) m = fmaxf(m, o.x);
     }
 #pragma unroll
-    for (int o = MG_LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = MG_ROWS; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (a.sink) m = fmaxf(m, sv);
-    float4 acc[MG_ROWS][NV];
+    float4 acc[MG_E];
 #pragma unroll
-    for (int x = 0; x < MG_ROWS; x++)
-#pragma unroll
-      for (int e = 0; e < NV; e++) acc[x][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int e = 0; e < MG_E; e++) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int base = 0; base < n; base += MG_LANES) {
-      if (base > 0) ml = stats(base + lane % MG_LANES);
+      if (base > 0) ml = stats(base + lane / MG_ROWS);
       const float w = ml.y != 0.f ? exp2f(ml.x - m) : 0.f;
       if (ml.y != 0.f) l += ml.y * w;
-      const int stop = min(n, base + MG_LANES);
-      constexpr int Z = 2;                   // segments on their way at a time
-      for (int z0 = base; z0 < stop; z0 += Z) {
-        float4 v[Z][MG_ROWS][NV];
+      float4 v[MG_LANES][MG_E];                            // all eight segments on their way
 #pragma unroll
-        for (int z = 0; z < Z; z++) {
-          const int at_z = z0 + z;
-          if (at_z >= stop) continue;
+      for (int z = 0; z < MG_LANES; z++) {
+        if (base + z >= n) continue;
 #pragma unroll
-          for (int e = 0; e < NV; e++) {
-            const float4* const p = tree_part(a, item.c0 + at_z, at_z == 0 ? item.slot0 : 0, min(lane + 32 * e, (hd + 3) / 4 - 1), r);
+        for (int e = 0; e < MG_E; e++) v[z][e] = *tree_part(a, item.c0 + base + z, base + z == 0 ? item.slot0 : 0, min(chunk + 8 * e, last), own);
+      }
 #pragma unroll
-            for (int x = 0; x < MG_ROWS; x++) v[z][x][e] = p[min(x, rows - 1)];
-          }
+      for (int z = 0; z < MG_LANES; z++) {
+        const float wz = __shfl_sync(0xffffffffu, w, z * MG_ROWS + lane % MG_ROWS);
+        if (base + z >= n || wz == 0.f) continue;
+#pragma unroll
+        for (int e = 0; e < MG_E; e++) {
+          acc[e].x = fmaf(v[z][e].x, wz, acc[e].x);
+          acc[e].y = fmaf(v[z][e].y, wz, acc[e].y);
+          acc[e].z = fmaf(v[z][e].z, wz, acc[e].z);
+          acc[e].w = fmaf(v[z][e].w, wz, acc[e].w);
         }
-#pragma unroll
-        for (int z = 0; z < Z; z++)
-#pragma unroll
-          for (int x = 0; x < MG_ROWS; x++) {
-            const float wz = __shfl_sync(0xffffffffu, w, x * MG_LANES + (z0 + z) % MG_LANES);
-            if (z0 + z >= stop || wz == 0.f) continue;
-#pragma unroll
-            for (int e = 0; e < NV; e++) {
-              acc[x][e].x = fmaf(v[z][x][e].x, wz, acc[x][e].x);
-              acc[x][e].y = fmaf(v[z][x][e].y, wz, acc[x][e].y);
-              acc[x][e].z = fmaf(v[z][x][e].z, wz, acc[x][e].z);
-              acc[x][e].w = fmaf(v[z][x][e].w, wz, acc[x][e].w);
-            }
-          }
       }
     }
 #pragma unroll
-    for (int o = MG_LANES / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    for (int o = MG_ROWS; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     const float inv = l == 0.f ? 0.f : 1.0f / (a.sink ? l + exp2f(sv - m) : l);
+    if (row >= item.pairs) continue;
+    T* const to = reinterpret_cast<T*>(a.out) + (size_t)(item.t0 + (item.r0 + row) / G) * a.out_ld + (size_t)h * hd;
 #pragma unroll
-    for (int x = 0; x < MG_ROWS; x++) {
-      const float f = __shfl_sync(0xffffffffu, inv, x * MG_LANES);
-      const bool none = __shfl_sync(0xffffffffu, l, x * MG_LANES) == 0.f;
-      if (x >= rows) continue;
-      T* const to = reinterpret_cast<T*>(a.out) + (size_t)(item.t0 + (item.r0 + r + x) / G) * a.out_ld + (size_t)head(r + x) * hd;
-#pragma unroll
-      for (int e = 0; e < NV; e++) put4(a, to, (lane + 32 * e) * 4, acc[x][e], f, none);
-    }
+    for (int e = 0; e < MG_E; e++) put4(a, to, (chunk + 8 * e) * 4, acc[e], inv, l == 0.f);
   }
 }
 
 template <typename T> void run_merge(const TreeArgs& a, cudaStream_t stream) {
   const long long tasks = ((long long)a.T * a.H + MG_ROWS - 1) / MG_ROWS * ((a.hd + 31) / 32), most = 148 * 2;     // two to an SM
   const dim3 grid((unsigned)(tasks < most ? tasks : most));
-  if (a.hd <= 128) tlc_launch(tree_merge_kernel<T, 1>, grid, dim3(MG_T), 0, stream, a);
-  else tlc_launch(tree_merge_kernel<T, 2>, grid, dim3(MG_T), 0, stream, a);
+  tlc_launch(tree_merge_kernel<T>, grid, dim3(MG_T), 0, stream, a);
 }
 
 constexpr int SIMT_MOST_SMEM = 227 * 1024 - 1024;
