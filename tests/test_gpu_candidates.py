@@ -547,6 +547,27 @@ def test_beam_select_clustered_values():
     select_check(logits, torch.zeros(4, 1, device=DEV), 64)
 
 
+@pytest.mark.parametrize("R,K,V,n", [(16, 4, 30000, 16), (3, 2, 20001, 64), (24, 8, 9000, 16), (1, 1, 130048, 64), (2, 16, 65537, 32)])
+def test_beam_select_of_few_alive_beams(R, K, V, n):
+    """A first step (one beam is alive), beams of which only a few tokens are allowed, and values that rise from token to token."""
+    g = torch.Generator(device=DEV).manual_seed(V + n)
+    inf = float("inf")
+    logits = torch.randn(R * K, V, device=DEV, generator=g) * 3
+    first = torch.full((R, K), -inf, device=DEV)
+    first[torch.arange(R), torch.arange(R) % K] = -0.5
+    select_check(logits, first, n)
+    zeros = torch.zeros(R, K, device=DEV)
+    allowed = logits.clone()
+    allowed[:, 5000:] = -inf
+    select_check(allowed, first, n)
+    lowest = logits.clone()
+    lowest[:, 3:] = torch.finfo(torch.float32).min
+    select_check(lowest, first, n)
+    rising = (torch.arange(V, device=DEV) * 2.0 ** -10).expand(R * K, V).contiguous()
+    select_check(rising, zeros, n)
+    select_check(rising.flip(1).contiguous(), first, n)
+
+
 # ---- beams that go on from another one ------------------------------------------------------------------
 MAPS = {"copies": lambda K, rng: [0] * K, "cycle": lambda K, rng: [(k + 1) % K for k in range(K)], "swap": lambda K, rng: list(range(K))[::-1],
         "any": lambda K, rng: [rng.randrange(K) for _ in range(K)], "none": lambda K, rng: [rng.choice([k, -1, K, 99]) for k in range(K)]}

@@ -23,9 +23,10 @@ constexpr int MAX_N = 64;                // candidates of a request
 constexpr int MAX_BEAMS = 64;
 constexpr int SCAN_WARPS = 4;
 constexpr int MERGE_T = 512, MERGE_WARPS = MERGE_T / 32;
-constexpr int MERGE_CAP = 4096;          // values that may reach the threshold; more (of equal values) are taken one after the other
+constexpr int MERGE_CAP = 4096;          // values that may reach the threshold; more equal ones are taken one after the other
 constexpr int MERGE_RANK = 512;          // and of which so many are ranked side by side, after a second threshold
 constexpr int MERGE_LISTS = 512;         // pieces that reach the threshold and are shared out evenly
+constexpr int SHARES = 16;               // parts of a request's logits where values are taken one after the other
 constexpr int MAX_LISTS = 36864;         // pieces of a request: a word of shared memory each
 
 struct Stats { double sum; float max; int pad; };      // of a piece: sum exp(x - max) and max
@@ -117,8 +118,8 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
   __shared__ double s_off[MAX_BEAMS], s_value[MERGE_RANK], s_best[MERGE_WARPS];
   __shared__ int s_index[MERGE_RANK], s_at[MERGE_WARPS], s_count, s_ranked, s_alive[MAX_BEAMS], s_list[MERGE_LISTS], s_lists, s_reach[2];
   __shared__ unsigned s_least;
-  __shared__ double s_out[MAX_N];
-  __shared__ int s_out_at[MAX_N];
+  __shared__ double s_out[MAX_N], s_share[SHARES];
+  __shared__ int s_out_at[MAX_N], s_share_at[SHARES];
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lists = K * n_pieces;
   if (tid == 0) s_count = s_lists = s_ranked = s_reach[0] = s_reach[1] = 0;
   // what a row's logits are raised by: the beam's score less the logarithm of the row's sum
@@ -186,6 +187,28 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
   }
   __syncthreads();
   unsigned least = s_least;
+  // a threshold of `low` or more that at least n and, where that can be found, at most `enough` of the block's keys reach
+  auto search = [&](const auto& keys, unsigned low, int enough) {
+    unsigned high = 0xffffffffu;
+    __syncthreads();
+    if (tid == 0) s_reach[0] = s_reach[1] = 0;
+    __syncthreads();
+    for (int turn = 0; low < high; turn++) {
+      const unsigned trial = low + (high - low) / 2 + 1;
+      int reach = 0;
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(keys) / sizeof(keys[0])); i++) reach += keys[i] >= trial;
+      reach = __reduce_add_sync(0xffffffffu, reach);
+      if (lane == 0) atomicAdd(&s_reach[turn & 1], reach);
+      __syncthreads();
+      reach = s_reach[turn & 1];
+      if (tid == 0) s_reach[(turn + 1) & 1] = 0;
+      __syncthreads();
+      if (reach >= n) low = trial; else high = trial - 1;
+      if (reach >= n && reach <= enough) break;
+    }
+    return low;
+  };
   // the pieces that reach it, again
   for (int l = tid; l < lists; l += MERGE_T)
     if (heads[l] >= least) {
@@ -194,8 +217,6 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
     }
   __syncthreads();
   const int passing = s_lists;
-  // (the threshold as a logit of row k, a little lower: whatever is worth as much passes, and what is worth hardly less does no harm)
-  const float worth = __uint_as_float(least & 0x80000000u ? least & 0x7fffffffu : ~least);
   auto push = [&](double value, float logit, int index, int mark) {
     const int at = atomicAdd(&s_count, 1);             // (in any order: they are ranked below)
     if (at < MERGE_CAP) { c_value[at] = logit; c_index[at] = mark; }
@@ -207,7 +228,11 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
     float v[VPL];
     load_piece<VPL, VEC>(x, V - base, lane, v);
     const double off = s_off[k];
-    const float exact = (float)((double)worth - off), bar = least == 1u ? -3.402823466e38f : exact - 1e-6f * (fabsf(exact) + fabsf(worth));
+    // (the threshold as a logit of row k, a little lower: whatever is worth as much passes, and what is worth hardly less does no harm)
+    const float worth = __uint_as_float(least & 0x80000000u ? least & 0x7fffffffu : ~least);
+    // (never below the lowest number: load_piece has -infinity behind a row's end, and a threshold under every number's key is worth a NaN)
+    constexpr float LOWEST = -3.402823466e38f;
+    const float exact = (float)((double)worth - off), bar = least == 1u ? LOWEST : fmaxf(LOWEST, exact - 1e-6f * (fabsf(exact) + fabsf(worth)));
     // which of them reach it; those few are read once more (a body for each of 64 values would not fit the instruction cache)
     unsigned long long who = 0;
 #pragma unroll
@@ -218,17 +243,46 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
       push(off + (double)f, f, k * V + base + at, k * V + base + at);
     }
   };
-  if (passing <= MERGE_LISTS) {
-    for (int i = warp; i < passing; i += MERGE_WARPS) collect(s_list[i]);
-  } else {
-    for (int l = warp; l < lists; l += MERGE_WARPS)
-      if (heads[l] >= least) collect(l);
+  // Fewer pieces than n hold anything (one beam is alive: 15 pieces of 30,000 logits for 16 candidates), or those that reach the threshold
+  // hold more than there is room for: then the maxima of the pieces' lanes make the threshold (64 such requests: 830 us one value after the
+  // other, 18 this way).
+  const bool few = passing * 32 <= MERGE_CAP;
+  bool finer = few && least == 1u && passing * 32 * VPL > MERGE_CAP;
+  int count;
+  for (;;) {
+    if (finer) {
+      unsigned* const tops = reinterpret_cast<unsigned*>(c_value);       // [32 * passing]
+      for (int i = warp; i < passing; i += MERGE_WARPS) {
+        const int l = s_list[i], k = l / n_pieces, base = l % n_pieces * 32 * VPL;
+        float v[VPL], m = -INFINITY;
+        load_piece<VPL, VEC>(logits + (size_t)(r * K + k) * ld + base, V - base, lane, v);
+#pragma unroll
+        for (int q = 0; q < VPL; q++) m = fmaxf(m, v[q]);
+        tops[i * 32 + lane] = m > -INFINITY ? key_of(k, m) : 0u;
+      }
+      __syncthreads();
+      unsigned held[MERGE_CAP / MERGE_T];
+#pragma unroll
+      for (int i = 0; i < MERGE_CAP / MERGE_T; i++) held[i] = i * MERGE_T + tid < passing * 32 ? tops[i * MERGE_T + tid] : 0u;
+      least = search(held, least, 2 * n);              // (its barriers come between these reads and what collect writes)
+    }
+    if (passing <= MERGE_LISTS) {
+      for (int i = warp; i < passing; i += MERGE_WARPS) collect(s_list[i]);
+    } else {
+      for (int l = warp; l < lists; l += MERGE_WARPS)
+        if (heads[l] >= least) collect(l);
+    }
+    if (ended)                                         // a beam that has ended stands for itself
+      for (int k = tid; k < K; k += MERGE_T)
+        if (ended[r * K + k] && isfinite(scores[r * K + k])) push((double)scores[r * K + k], 0.f, k * V + pad, -1 - k);
+    __syncthreads();
+    count = s_count;
+    if (count <= MERGE_CAP || finer || !few) break;
+    finer = true;
+    __syncthreads();
+    if (tid == 0) s_count = 0;
+    __syncthreads();
   }
-  if (ended)                                           // a beam that has ended stands for itself
-    for (int k = tid; k < K; k += MERGE_T)
-      if (ended[r * K + k] && isfinite(scores[r * K + k])) push((double)scores[r * K + k], 0.f, k * V + pad, -1 - k);
-  __syncthreads();
-  const int count = s_count;
   auto value_of = [&](int e, int* index) {
     const int at = c_index[e];
     if (at < 0) {
@@ -243,27 +297,13 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
     int ranked = count;
     if (count > MERGE_RANK) {
       // of many a second threshold, found the same way by the whole block
-      constexpr int HELD = MERGE_CAP / MERGE_T;
-      unsigned held[HELD], low = 1u, high = 0xffffffffu;
+      unsigned held[MERGE_CAP / MERGE_T];
 #pragma unroll
-      for (int i = 0; i < HELD; i++) {
+      for (int i = 0; i < MERGE_CAP / MERGE_T; i++) {
         int index;
         held[i] = i * MERGE_T + tid < count ? ordered((float)value_of(i * MERGE_T + tid, &index)) : 0u;
       }
-      for (int turn = 0; low < high; turn++) {         // (low is reached by n)
-        const unsigned trial = low + (high - low) / 2 + 1;
-        int reach = 0;
-#pragma unroll
-        for (int i = 0; i < HELD; i++) reach += held[i] >= trial;
-        reach = __reduce_add_sync(0xffffffffu, reach);
-        if (lane == 0) atomicAdd(&s_reach[turn & 1], reach);
-        __syncthreads();
-        reach = s_reach[turn & 1];
-        if (tid == 0) s_reach[(turn + 1) & 1] = 0;
-        __syncthreads();
-        if (reach >= n) low = trial; else high = trial - 1;
-        if (reach >= n && reach <= MERGE_RANK) break;
-      }
+      const unsigned low = search(held, 1u, MERGE_RANK);
       for (int e = tid; e < count; e += MERGE_T) {
         int index;
         const double a = value_of(e, &index);
@@ -286,10 +326,18 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
     }
   }
   if (found < 0) {
-    // more than there is room for (equal values): one after the other, each the best of all logits that comes after the last
+    // more than there is room for (equal values): one after the other, each the best of what comes after the last.  The best of every 16th 512
+    // tokens is known; the share that had the last is looked through again (480,000 equal values, 16 of them: 1.6 ms over all of them each
+    // time, 0.55 this way).
     double last = INFINITY;
     int last_at = -1;
-    for (found = 0; found < n; found++) {
+    auto best_of = [&](const double* value, const int* at, int of) {
+      int x = 0;
+      for (int w = 1; w < of; w++)
+        if (better(value[w], at[w], value[x], at[x])) x = w;
+      return x;
+    };
+    auto look = [&](int share) {
       double best = -INFINITY;
       int best_at = 0x7fffffff;
       auto take = [&](double a, int ai) {
@@ -298,10 +346,14 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
       for (int k = 0; k < K; k++) {
         if (!s_alive[k]) continue;
         const float* const x = logits + (size_t)(r * K + k) * ld;
-        for (int i = tid; i < V; i += MERGE_T)
-          if (x[i] > -INFINITY) take(s_off[k] + (double)x[i], k * V + i);
+        const double off = s_off[k];
+#pragma unroll 4
+        for (int i = share * MERGE_T + tid; i < V; i += SHARES * MERGE_T) {
+          const float f = x[i];
+          if (f > -INFINITY) take(off + (double)f, k * V + i);
+        }
       }
-      if (ended)
+      if (ended && share == 0)
         for (int k = tid; k < K; k += MERGE_T)
           if (ended[r * K + k] && isfinite(scores[r * K + k])) take((double)scores[r * K + k], k * V + pad);
 #pragma unroll
@@ -312,15 +364,22 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
       }
       if (lane == 0) { s_best[warp] = best; s_at[warp] = best_at; }
       __syncthreads();
-      best = s_best[0];
-      best_at = s_at[0];
-      for (int w = 1; w < MERGE_WARPS; w++)
-        if (better(s_best[w], s_at[w], best, best_at)) { best = s_best[w]; best_at = s_at[w]; }
+      if (tid == 0) {
+        const int x = best_of(s_best, s_at, MERGE_WARPS);
+        s_share[share] = s_best[x];
+        s_share_at[share] = s_at[x];
+      }
       __syncthreads();
-      if (best == -INFINITY) break;
-      if (tid == 0) { s_out[found] = best; s_out_at[found] = best_at; }
-      last = best;
-      last_at = best_at;
+    };
+    for (int share = 0; share < SHARES; share++) look(share);
+    for (found = 0; found < n; found++) {
+      const int x = best_of(s_share, s_share_at, SHARES);
+      last = s_share[x];
+      last_at = s_share_at[x];
+      __syncthreads();
+      if (last == -INFINITY) break;
+      if (tid == 0) { s_out[found] = last; s_out_at[found] = last_at; }
+      look(x);
     }
   }
   __syncthreads();
