@@ -182,9 +182,10 @@ def beam_select(logits, scores, n, ended=None, pad=0, placed=False):
                 c[k, pad] = s
                 continue
             x = logits[r * K + k].double()
-            lse = torch.logsumexp(x, 0)
+            top = x.max()
+            lse = torch.log(torch.exp(x - top).sum())
             if torch.isfinite(lse):
-                c[k] = s + (x - lse)
+                c[k] = s + ((x - top) - lse)
         flat = c.flatten()
         order = torch.sort(flat, descending=True, stable=True).indices[:n].tolist()
         if placed:

@@ -563,6 +563,8 @@ def test_beam_select_of_few_alive_beams(R, K, V, n):
     lowest = logits.clone()
     lowest[:, 3:] = torch.finfo(torch.float32).min
     select_check(lowest, first, n)
+    lowest[:, :3] = torch.finfo(torch.float32).min
+    select_check(lowest, torch.arange(R * K, device=DEV).view(R, K) * -0.25, n)
     rising = (torch.arange(V, device=DEV) * 2.0 ** -10).expand(R * K, V).contiguous()
     select_check(rising, zeros, n)
     select_check(rising.flip(1).contiguous(), first, n)

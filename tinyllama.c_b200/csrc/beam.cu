@@ -11,7 +11,8 @@
 //     so that only the pieces whose maximum reaches it (n to 2 n of hundreds, by a threshold that a few counts find) can hold
 //     any: those are read again, a warp each, and what reaches the threshold is ranked by counting.  (With the n largest of every piece
 //     left by the first kernel it took twice as long: 34 of 66 us went into values that no request wanted.)
-// Bound by HBM for a batch (256 rows of 130,048 logits: 133 MB, 20 us of loads), by the two launches for one request.
+// Bound by HBM for a batch (192 rows of 130,048 logits: 100 MB in 16.5 us, 6.1 TB/s; the merge, 16 candidates of 32 requests, some 9 more, of which
+// half are trips to the L2 and half the counts that find the threshold), by the two launches for one request (7.4 us for 4 rows of 65,536).
 // Arithmetic: exponentials and sums in 32 bits over 16 values at most, the sums of those, the logarithm and the values that are compared in
 // 64 bits: two candidates change places only where they are nearer than the 2^-22 or so that this leaves.
 #include "common.cuh"
@@ -115,14 +116,15 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
   float* const c_value = reinterpret_cast<float*>(merge_room);           // [MERGE_CAP] logits that reach the threshold
   int* const c_index = merge_room + MERGE_CAP;                           // [MERGE_CAP] k * V + v of them; of ended beams -1 - k
   unsigned* const heads = reinterpret_cast<unsigned*>(merge_room + 2 * MERGE_CAP);     // of every piece: what its maximum is worth, as an ordered integer
-  __shared__ double s_off[MAX_BEAMS], s_value[MERGE_RANK], s_best[MERGE_WARPS];
+  __shared__ double s_off[MAX_BEAMS], s_top[MAX_BEAMS], s_value[MERGE_RANK], s_best[MERGE_WARPS];
   __shared__ int s_index[MERGE_RANK], s_at[MERGE_WARPS], s_count, s_ranked, s_alive[MAX_BEAMS], s_list[MERGE_LISTS], s_lists, s_reach[2];
   __shared__ unsigned s_least;
   __shared__ double s_out[MAX_N], s_share[SHARES];
   __shared__ int s_out_at[MAX_N], s_share_at[SHARES];
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lists = K * n_pieces;
   if (tid == 0) s_count = s_lists = s_ranked = s_reach[0] = s_reach[1] = 0;
-  // what a row's logits are raised by: the beam's score less the logarithm of the row's sum
+  // a logit x of row k is worth s_off + (x - s_top), with the row's largest in s_top and the beam's score less the logarithm of the sum of
+  // exp(x - s_top) in s_off (one number for both would lose the score where a row holds nothing but the lowest number)
   for (int k = warp; k < K; k += MERGE_WARPS) {
     const int row = r * K + k;
     const Stats* st = stats + (size_t)row * n_pieces;
@@ -140,13 +142,14 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      off = (double)scores[row] - ((double)m + log(sum));
+      off = (double)scores[row] - log(sum);
       on = isfinite(off);                              // no candidates of a row with a NaN, an infinity or nothing in it
     }
-    if (lane == 0) { s_off[k] = off; s_alive[k] = on; }
+    if (lane == 0) { s_off[k] = off; s_top[k] = m; s_alive[k] = on; }
   }
   __syncthreads();
-  auto key_of = [&](int k, float x) { return ordered((float)(s_off[k] + (double)x)); };
+  auto worth_of = [&](int k, float x) { return s_off[k] + ((double)x - s_top[k]); };
+  auto key_of = [&](int k, float x) { return ordered((float)worth_of(k, x)); };
   const Stats* const mine = stats + (size_t)r * lists;
   for (int l = tid; l < lists; l += MERGE_T) {
     const int k = l / n_pieces;
@@ -227,12 +230,11 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
     const float* const x = logits + (size_t)(r * K + k) * ld + base;
     float v[VPL];
     load_piece<VPL, VEC>(x, V - base, lane, v);
-    const double off = s_off[k];
     // (the threshold as a logit of row k, a little lower: whatever is worth as much passes, and what is worth hardly less does no harm)
     const float worth = __uint_as_float(least & 0x80000000u ? least & 0x7fffffffu : ~least);
     // (never below the lowest number: load_piece has -infinity behind a row's end, and a threshold under every number's key is worth a NaN)
     constexpr float LOWEST = -3.402823466e38f;
-    const float exact = (float)((double)worth - off), bar = least == 1u ? LOWEST : fmaxf(LOWEST, exact - 1e-6f * (fabsf(exact) + fabsf(worth)));
+    const float exact = (float)((double)worth - s_off[k] + s_top[k]), bar = least == 1u ? LOWEST : fmaxf(LOWEST, exact - 1e-6f * (fabsf(exact) + fabsf(worth)));
     // which of them reach it; those few are read once more (a body for each of 64 values would not fit the instruction cache)
     unsigned long long who = 0;
 #pragma unroll
@@ -240,7 +242,7 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
     for (; who != 0; who &= who - 1) {
       const int q = __ffsll((long long)who) - 1, at = (q / VEC * 32 + lane) * VEC + q % VEC;
       const float f = x[at];
-      push(off + (double)f, f, k * V + base + at, k * V + base + at);
+      push(worth_of(k, f), f, k * V + base + at, k * V + base + at);
     }
   };
   // Fewer pieces than n hold anything (one beam is alive: 15 pieces of 30,000 logits for 16 candidates), or those that reach the threshold
@@ -290,7 +292,7 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
       return (double)scores[r * K + -1 - at];
     }
     *index = at;
-    return s_off[at / V] + (double)c_value[e];
+    return worth_of(at / V, c_value[e]);
   };
   int found = -1;
   if (count <= MERGE_CAP) {
@@ -346,11 +348,10 @@ beam_merge_kernel(const float* __restrict__ logits, long long ld, const float* _
       for (int k = 0; k < K; k++) {
         if (!s_alive[k]) continue;
         const float* const x = logits + (size_t)(r * K + k) * ld;
-        const double off = s_off[k];
 #pragma unroll 4
         for (int i = share * MERGE_T + tid; i < V; i += SHARES * MERGE_T) {
           const float f = x[i];
-          if (f > -INFINITY) take(off + (double)f, k * V + i);
+          if (f > -INFINITY) take(worth_of(k, f), k * V + i);
         }
       }
       if (ended && share == 0)
@@ -487,7 +488,7 @@ __device__ __forceinline__ void copy_part(char* base, const Move* moves, int cou
   }
 }
 
-// grid (parts of a slot's state, requests, layers)
+// grid (parts of a slot's state, requests, layers).  Bound by HBM: 16 moved states of 6 layers of 3 MB, 604 MB in and out in 102 us (5.9 TB/s).
 template <typename Vec>
 __global__ void __launch_bounds__(CP_T)
 beam_states_kernel(char* state, long long layer_bytes, long long slot_bytes, int bytes, int n_slots, const int* __restrict__ slots,
