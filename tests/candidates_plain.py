@@ -70,12 +70,10 @@ class Pool:
         if any(slots[parents[k]] < 0 for k in moved):
             return 3, {}
         own = {k: old.table[s][pages_of(old.lengths[s]) - 1] if s >= 0 and old.lengths[s] else None for k, s in enumerate(slots)}
-        for k in moved:
-            if old.lengths[slots[parents[k]]] % PAGE:
-                if own[k] is None:
-                    return 4, {}
-                if old.refs[own[k]] != 1:
-                    return 5, {}
+        needs = [own[k] for k in moved if old.lengths[slots[parents[k]]] % PAGE]
+        code = max([4 if page is None else 5 if old.refs[page] != 1 else 0 for page in needs] + [0])
+        if code:
+            return code, {}
         copies = {}
         for k in moved:
             s, p = slots[k], slots[parents[k]]

@@ -2538,7 +2538,8 @@ def beam_reorder_pages(block_table: torch.Tensor, refs: torch.Tensor, lengths: t
 
     slots and parents int32 [R, K]; slot -1 or a parent outside 0 .. K - 1 leaves a beam as it is.  A request for which it cannot be done
     (no page of its own, one that others share, a slot named twice) stays as it is, with a code in status (see page_resize).  No two
-    requests of a call name one slot; calls on one pool follow one another."""
+    requests of a call name one slot, and none fills a page that a beam of another names (whole pages may be anybody's); calls on one pool
+    follow one another."""
     dev, dims = k_pages.get_device(), k_pages.dim()
     if not (slots.dim() == 2 and parents.shape == slots.shape and 1 <= slots.shape[1] <= MAX_BEAMS and _pool_ok(block_table, refs, lengths, status, dev)
             and block_table.get_device() == dev and dev == _get_device() and _ok(slots, _I32, slots.numel(), dev) and _ok(parents, _I32, slots.numel(), dev)
