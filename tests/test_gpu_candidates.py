@@ -166,6 +166,8 @@ def test_row_maps_of_nothing():
     assert (got.cu_seqlens.tolist(), got.row_seq.tolist(), got.row_map.tolist()) == ([0], [-1, -1], [-1, -1])
     got = ops.row_maps(ints([[3]]), ints([0]), ints([5]), ints([4]), 0)
     assert got.cu_seqlens.tolist() == [0, 0]
+    got = ops.row_maps(ints([[3]]), ints([0]), ints([5]), ints([0]), 0, ints([]), torch.zeros(0, dtype=torch.bool, device=DEV), 40)
+    assert got.cu_seqlens.tolist() == [0, 0] and got.mask.shape == (0, 2)
 
 
 # ---- rows to their places -----------------------------------------------------------------------------
@@ -655,6 +657,27 @@ def test_beam_reorder_pages_that_cannot_be():
         ops.beam_reorder_pages(dev.table, dev.refs, dev.lengths, ints(slots), ints(parents), pages, None, dev.status)
         dev.equals(mine)
         assert dev.status.tolist() == [code] and torch.equal(pages, want)
+
+
+def test_calls_of_nothing():
+    """No requests, no rows, states of no values: nothing is launched that would touch anything."""
+    zeros = lambda *shape, dtype=torch.int32: torch.zeros(*shape, dtype=dtype, device=DEV)
+    table, refs, lengths, status, none = zeros(2, 3), zeros(6), zeros(2), zeros(1), zeros(0)
+    pages = zeros(3, 6, 2, PAGE, 64, dtype=torch.bfloat16)
+    rows = zeros(3, 0, 128, dtype=torch.bfloat16)
+    ops.page_resize(table, refs, lengths, none, none, status)
+    ops.kv_store(rows, rows, none, pages, pages)
+    for n, slots in ((0, [0]), (2, [])):                               # a request of no rows, rows of no request
+        q, kv, out = zeros(n, 256, dtype=torch.bfloat16), zeros(n, 128, dtype=torch.bfloat16), torch.full((n, 256), 3.0, dtype=torch.bfloat16, device=DEV)
+        ops.tree_attention(q, kv, kv, pages[0], pages[0], table, ints(slots), ints(slots), zeros(len(slots) + 1), zeros(n), out, 4, 2, 64, 0.1,
+                           max_context=10, max_new=2)
+        assert bool((out == 3.0).all())
+    assert ops.beam_select(zeros(0, 50, dtype=torch.float32), zeros(0, 4, dtype=torch.float32), 4)[0].shape == (0, 4)
+    ops.beam_reorder_states(zeros(2, 3, 8), zeros(0, 4), zeros(0, 4))
+    ops.beam_reorder_states(zeros(2, 3, 0), ints([[0, 1]]), ints([[1, 1]]))
+    ops.beam_reorder_pages(table, refs, lengths, zeros(0, 4), zeros(0, 4), pages, pages, status)
+    assert status.tolist() == [0] and not bool(pages.any()) and not bool(table.any())
+    ops.check_errors()
 
 
 # ---- together --------------------------------------------------------------------------------------------

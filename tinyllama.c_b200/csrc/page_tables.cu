@@ -423,7 +423,7 @@ extern "C" int tlc_row_maps(const int* block_table, int n_slots, int max_pages, 
                             int T, const int* parents, const void* keep, int words, int* cu_seqlens, int* row_seq, int* positions,
                             int* row_map, int* mask, cudaStream_t stream) {
   TLC_REQUIRE(B >= 0 && B <= MAX_REQUESTS, "row_maps: %d requests (at most %d a call)", B, MAX_REQUESTS);
-  TLC_REQUIRE(T >= 0 && n_slots > 0 && max_pages > 0 && (parents == nullptr) == (mask == nullptr) && words >= 0, "row_maps: %d rows, %d slots of %d pages",
+  TLC_REQUIRE(T >= 0 && n_slots > 0 && max_pages > 0 && (T == 0 || (parents == nullptr) == (mask == nullptr)) && words >= 0, "row_maps: %d rows, %d slots of %d pages",
               T, n_slots, max_pages);
   if (!mask) words = 0;
   tlc_launch(row_maps_kernel, dim3(T > 0 ? (T + MT - 1) / MT : 1), dim3(MT), (size_t)(B + 1) * sizeof(int), stream, block_table, n_slots, max_pages,
