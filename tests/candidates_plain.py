@@ -74,6 +74,14 @@ class Pool:
         code = max([4 if page is None else 5 if old.refs[page] != 1 else 0 for page in needs] + [0])
         if code:
             return code, {}
+        # a last page that is whole and that a child of the beam takes over cannot be filled by the beam too: it fills a page that the beams give
+        # back, the last one of a beam that fills none and whose child does not take it, in order
+        fills = [k for k in moved if old.lengths[slots[parents[k]]] % PAGE]
+        taken = {parents[k] for k in moved if old.lengths[slots[parents[k]]] % PAGE == 0}
+        lost = [k for k in fills if k in taken]
+        spare = [own[k] for k in moved if k not in fills and k not in taken and own[k] is not None and old.refs[own[k]] == 1]
+        if len(spare) < len(lost):
+            return 5, {}
         copies = {}
         for k in moved:
             s, p = slots[k], slots[parents[k]]
@@ -89,6 +97,12 @@ class Pool:
                 self.table[s][full] = own[k]
                 copies[k] = (own[parents[k]], own[k], used)
             self.lengths[s] = old.lengths[p]
+        for k, page in zip(lost, spare):
+            source, mine, used = copies[k]
+            self.refs[mine] -= 1
+            self.refs[page] += 1
+            self.table[slots[k]][old.lengths[slots[parents[k]]] // PAGE] = page
+            copies[k] = (source, page, used)
         return 0, copies
 
 

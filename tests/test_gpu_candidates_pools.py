@@ -1,0 +1,112 @@
+"""The pool's operators by what they leave behind: what a beam's table row reads after a reordering, whose pages a step writes."""
+import random
+
+import pytest
+import torch
+
+from tinyllama_c_b200 import ops
+
+import candidates_plain as plain
+from test_gpu_candidates import DEV, PAGE, DevicePool, ints
+
+pytestmark = pytest.mark.gpu
+
+
+def histories(dev, slots, pages):
+    """What each slot's row reads: [L, KV, length, hd] of pages [L, n, KV, 64, hd]."""
+    out = []
+    for s in slots:
+        n = int(dev.lengths[s])
+        row = dev.table[s, :plain.pages_of(n)].long()
+        out.append(pages[:, row].transpose(1, 2).flatten(2, 3)[:, :, :n].clone())
+    return out
+
+
+def reordered(dev, slots, parents, pages):
+    """One call of all requests; its code.  With code 0 every beam reads what its parent read, else what it read before; the counts are those of the table."""
+    before = [[histories(dev, row, p) for row in slots] for p in pages]
+    ops.beam_reorder_pages(dev.table, dev.refs, dev.lengths, ints(slots), ints(parents), pages[0], pages[1], dev.status)
+    code = int(dev.status)
+    dev.status.zero_()
+    for p, old in zip(pages, before):
+        for r, row in enumerate(slots):
+            now = histories(dev, row, p)
+            same = [all(torch.equal(a, b) for a, b in zip(now, want)) for want in ([old[r][k] for k in parents[r]], old[r])]
+            assert same[0] or (code and same[1]), (r, code)
+    counts = torch.zeros_like(dev.refs)
+    for s, n in enumerate(dev.lengths.tolist()):
+        row = dev.table[s, :plain.pages_of(n)].long()
+        counts.index_add_(0, row, torch.ones_like(row, dtype=torch.int32))
+    assert torch.equal(counts, dev.refs)
+    return code
+
+
+@pytest.mark.parametrize("lengths,parents", [([64, 100], [1, 0]), ([100, 64], [1, 0]), ([64, 100, 100], [1, 0, 2]), ([128, 70, 64], [1, 2, 0]), ([64, 64, 100], [2, 0, 2]),
+                                             ([64, 128, 100, 5], [2, 0, 1, 1]), ([64, 64, 64, 90], [3, 0, 0, 1]), ([128, 128, 70, 71], [2, 3, 0, 1])])
+def test_whole_last_pages_that_a_child_takes_over(lengths, parents):
+    K = len(lengths)
+    pool = plain.Pool(2 * K, 4, 8 * K)
+    slots = [list(range(K)), list(range(K, 2 * K))[::-1]]
+    for row in slots:
+        assert pool.resize(row, lengths) == 0
+    dev = DevicePool(pool)
+    pages = [torch.randint(0, 250, (2, 8 * K, 2, PAGE, 9), device=DEV).bfloat16() for _ in range(2)]
+    assert reordered(dev, slots, [parents, list(range(K))], pages) == 0
+    for row, up in zip(slots, [parents, list(range(K))]):
+        assert pool.reorder(row, up)[0] == 0
+    dev.equals(pool)
+    # every beam may go on
+    dev.resize([s for row in slots for s in row], [n + 1 for row in slots for n in dev.lengths[ints(row).long()].tolist()])
+    assert dev.status.tolist() == [0]
+
+
+@pytest.mark.parametrize("K,hd,dtype", [(2, 128, torch.bfloat16), (4, 5, torch.float32), (7, 16, torch.bfloat16), (20, 7, torch.bfloat16)])
+def test_histories_of_random_lengths(K, hd, dtype):
+    rng, R, codes = random.Random(K), 3, []
+    for _ in range(8):
+        n_slots = R * K + 1
+        pool = plain.Pool(n_slots, 5, 5 * n_slots)
+        taken = rng.sample(range(n_slots), R * K)
+        slots = [taken[r * K:(r + 1) * K] for r in range(R)]
+        assert pool.resize(taken, [rng.choice([64, 128, 320, rng.randint(1, 320)]) for _ in taken]) == 0
+        dev = DevicePool(pool)
+        pages = [torch.randint(0, 250, (1, 5 * n_slots, 2, PAGE, hd), device=DEV).to(dtype) for _ in range(2)]
+        for _ in range(3):
+            parents = [[rng.randrange(K) for _ in range(K)] for _ in range(R)]
+            want = max(pool.reorder(row, up)[0] for row, up in zip(slots, parents))
+            codes.append(reordered(dev, slots, parents, pages))
+            assert codes[-1] == want
+            dev.equals(pool)
+    assert 0 in codes
+
+
+def test_no_page_to_spare():
+    """The only page that the beams give back is another slot's too: refused, nothing changes."""
+    pool = plain.Pool(4, 4, 16)
+    assert pool.resize([0, 1, 2], [64, 64, 100]) == 0
+    pool.table[3], pool.lengths[3] = list(pool.table[1]), 64
+    pool.refs[pool.table[1][0]] = 2
+    dev = DevicePool(pool)
+    pages = [torch.randn(1, 16, 1, PAGE, 8, device=DEV) for _ in range(2)]
+    before = [p.clone() for p in pages]
+    assert reordered(dev, [[0, 1, 2]], [[2, 0, 2]], pages) == 5
+    dev.equals(pool)
+    assert all(torch.equal(a, b) for a, b in zip(before, pages))
+
+
+def test_requests_that_share_whole_pages():
+    """Two requests over one whole prompt page, whose beams give it back and take it over at once: nobody fills it."""
+    pool = plain.Pool(6, 4, 24)
+    assert pool.resize([0, 2, 3, 5], [64, 100, 64, 100]) == 0
+    for s in (1, 4):
+        assert pool.resize([s], [64]) == 0
+    prompt = pool.table[1][0]
+    for s in (3, 4):                                                     # slots 1, 3 and 4 name one page
+        pool.refs[pool.table[s][0]] = 0
+        pool.table[s][0] = prompt
+    pool.refs[prompt] = 3
+    dev = DevicePool(pool)
+    pages = [torch.randn(2, 24, 1, PAGE, 8, device=DEV) for _ in range(2)]
+    # request 0: beam 0 fills a page that its child, beam 1, takes over, and beam 1's page is the prompt's; request 1 moves the prompt's page about
+    assert reordered(dev, [[0, 1, 2], [3, 4, 5]], [[2, 0, 2], [1, 0, 2]], pages) == 5
+    assert int(dev.refs[prompt]) == 3

@@ -521,14 +521,18 @@ beam_states_kernel(char* state, long long layer_bytes, long long slot_bytes, int
 }
 
 // A block a request.  Whole pages of the parent are shared; the page that the parent is filling is copied into the beam's own last
-// page.  own [R, K]: what the copy needs: {page it comes from, page it goes to, positions}.
+// page.  Where that page is whole and a child of the beam takes it over (lengths that differ: beam 0 of 64 positions goes on from beam 1 of 100,
+// and beam 1 from beam 0), the copy goes into another page, one that the request's beams give back: the last page of a beam that fills none itself
+// and that no child takes over.  Such beams take these pages in order; where there are too few the request is refused.
+// own [R, K]: what the copy needs: {page it comes from, page it goes to, positions}.
 constexpr int RO_T = 256, RO_COLS = 64;
 enum { RO_LENGTH = 2, RO_SLOT = 3, RO_TABLE = 4, RO_SHARED = 5 };   // codes of the status word, as of page_resize
 __global__ void __launch_bounds__(RO_T)
 beam_tables_kernel(int* block_table, int n_slots, int max_pages, int* refs, int n_pages, int* lengths, const int* __restrict__ slots,
                    const int* __restrict__ parents, int K, int4* __restrict__ own, int* status) {
   tlc_wait(block_table, refs, lengths, slots, parents, own, status);
-  __shared__ int s_slot[MAX_BEAMS], s_parent[MAX_BEAMS], s_len[MAX_BEAMS], s_last[MAX_BEAMS], s_tile[MAX_BEAMS][RO_COLS], s_bad, s_cols;
+  __shared__ int s_slot[MAX_BEAMS], s_parent[MAX_BEAMS], s_len[MAX_BEAMS], s_last[MAX_BEAMS], s_fill[MAX_BEAMS], s_tile[MAX_BEAMS][RO_COLS], s_bad, s_cols;
+  __shared__ unsigned char s_lost[MAX_BEAMS], s_spare[MAX_BEAMS];
   const int r = blockIdx.x, tid = threadIdx.x;
   if (tid == 0) s_bad = s_cols = 0;
   __syncthreads();
@@ -569,13 +573,34 @@ beam_tables_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
       const int page = block_table[(size_t)s_slot[k] * max_pages + c];
       if (page < 0 || page >= n_pages) atomicMax(&s_bad, (int)RO_TABLE);
     }
+    __syncthreads();
+    const bool sound = s_bad == 0;
+    // s_lost: the beam's last page goes to a child, and it fills one; s_spare: its last page is nobody's after the move
+    if (sound && tid < K) {
+      const int p = s_parent[tid], n = s_len[tid], last = s_last[tid];
+      const bool moves = p != tid && s_slot[tid] >= 0, fills = moves && s_len[p] % TLC_PAGE != 0;
+      bool taken = false;
+      if (n % TLC_PAGE == 0)
+        for (int k = 0; k < K; k++) taken |= k != tid && s_parent[k] == tid && s_slot[k] >= 0;
+      s_lost[tid] = fills && taken;
+      s_spare[tid] = moves && !fills && !taken && n > 0 && refs[last] == 1;
+      s_fill[tid] = last;
+    }
+    __syncthreads();
+    if (sound && tid < K && s_lost[tid]) {
+      int before = 0, at = 0;
+      for (int k = 0; k < tid; k++) before += s_lost[k];
+      for (; at < K; at++)
+        if (s_spare[at] && before-- == 0) break;
+      if (at < K) s_fill[tid] = s_last[at]; else atomicMax(&s_bad, (int)RO_SHARED);
+    }
   }
   __syncthreads();
   const bool go = s_bad == 0 && moved;
   if (tid < K) {
     const int p = s_parent[tid], used = s_len[p] % TLC_PAGE;
     int4 mv = make_int4(0, 0, 0, 0);
-    if (go && p != tid && s_slot[tid] >= 0 && used > 0) mv = make_int4(s_last[p], s_last[tid], used, 0);
+    if (go && p != tid && s_slot[tid] >= 0 && used > 0) mv = make_int4(s_last[p], s_fill[tid], used, 0);
     own[r * K + tid] = mv;
     if (go && p != tid && s_slot[tid] >= 0) lengths[s_slot[tid]] = s_len[p];
   }
@@ -583,25 +608,32 @@ beam_tables_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
   if (!go) return;
   const int cols = s_cols;
   for (int c0 = 0; c0 < cols; c0 += RO_COLS) {
-    __syncthreads();
     for (int e = tid; e < K * RO_COLS; e += RO_T) {
       const int k = e / RO_COLS, c = c0 + e % RO_COLS;
       if (s_slot[k] >= 0 && c < pages_of(s_len[k])) s_tile[k][e % RO_COLS] = block_table[(size_t)s_slot[k] * max_pages + c];
     }
     __syncthreads();
-    for (int e = tid; e < K * RO_COLS; e += RO_T) {
-      const int k = e / RO_COLS, i = e % RO_COLS, c = c0 + i, p = s_parent[k];
-      if (p == k || s_slot[k] < 0) continue;
-      const int have = pages_of(s_len[k]), full = s_len[p] / TLC_PAGE, used = s_len[p] % TLC_PAGE;
-      const bool had = c < have, keeps = used > 0 && c == have - 1;      // keeps: the page stays the beam's, in its new last place
-      const int before = had ? s_tile[k][i] : -1;
-      int after = 0;
-      if (c < full) after = s_tile[p][i];
-      else if (c == full && used > 0) after = s_last[k];
-      if (!had && c > full) continue;
-      if (c < full && !(had && !keeps && before == after)) atomicAdd(refs + after, 1);
-      if (had && !keeps && !(c < full && before == after)) atomicSub(refs + before, 1);
-      if (c < full || had || (c == full && used > 0)) block_table[(size_t)s_slot[k] * max_pages + c] = after;
+    // what is taken is counted before what is given back: a page that stays in use is never seen as somebody's alone by another request's block
+    for (int give = 0; give < 2; give++) {
+      for (int e = tid; e < K * RO_COLS; e += RO_T) {
+        const int k = e / RO_COLS, i = e % RO_COLS, c = c0 + i, p = s_parent[k];
+        if (p == k || s_slot[k] < 0) continue;
+        const int have = pages_of(s_len[k]), full = s_len[p] / TLC_PAGE, used = s_len[p] % TLC_PAGE;
+        const bool had = c < have, other = s_fill[k] != s_last[k];
+        const bool keeps = used > 0 && c == have - 1 && !other;          // the page stays the beam's, in its new last place
+        const int before = had ? s_tile[k][i] : -1;
+        int after = 0;
+        if (c < full) after = s_tile[p][i];
+        else if (c == full && used > 0) after = s_fill[k];
+        if (!had && c > full) continue;
+        if (!give) {
+          if (c < full ? !(had && !keeps && before == after) : c == full && used > 0 && other) atomicAdd(refs + after, 1);
+        } else {
+          if (had && !keeps && !(c < full && before == after)) atomicSub(refs + before, 1);
+          if (c < full || had || (c == full && used > 0)) block_table[(size_t)s_slot[k] * max_pages + c] = after;
+        }
+      }
+      __syncthreads();
     }
   }
 }

@@ -599,7 +599,8 @@ int tlc_tree_attention(const void* q, int dtype, int ld_q, const void* k_new, in
  * place and the others fill the places left; else the best comes first.  scratch: tlc_beam_select_scratch(R * K, V) bytes.
  * tlc_beam_reorder_states: what slot slots[r, parents[r, k]] holds goes to slot slots[r, k], in every layer at once; strides in bytes.
  * tlc_beam_reorder_pages: the same of a pool's keys and values: a beam with another parent than itself gives back its pages but the last,
- * shares the parent's whole pages and takes over what the parent's last, partly filled page holds in its own last page.  A request
+ * shares the parent's whole pages and takes over what the parent's last, partly filled page holds in its own last page, or, where that
+ * is whole and goes to another beam, in a last page that a beam of the request gives back.  A request
  * for which that cannot be done (status as above) stays as it is.  scratch: 16 * R * K bytes.  A slot of -1 or a parent outside
  * 0 .. K - 1 leaves a beam as it is. */
 long long tlc_beam_select_scratch(int rows, int V);

@@ -2534,10 +2534,11 @@ def beam_reorder_pages(block_table: torch.Tensor, refs: torch.Tensor, lengths: t
     pages but the last, its row names the parent's whole pages (shared: refs counts them), and what the parent's last, partly
     filled page holds is copied into the beam's own last page, in every layer of k_pages and v_pages ([n, KV, 64, hd] or [L, n, KV, 64, hd];
     v_pages may be None).  Lengths follow.  A beam needs a page of its own only where the parent's last page is partly filled: a search
-    starts from one sequence by giving each other beam a slot of length 1 and the parent 0.
+    starts from one sequence by giving each other beam a slot of length 1 and the parent 0.  Lengths of a request may differ: where a beam's
+    last page is whole and another beam takes it over, what the beam fills is a last page that a beam of the request gives back.
 
     slots and parents int32 [R, K]; slot -1 or a parent outside 0 .. K - 1 leaves a beam as it is.  A request for which it cannot be done
-    (no page of its own, one that others share, a slot named twice) stays as it is, with a code in status (see page_resize).  No two
+    (no page of its own, one that others share or take over and none given back, a slot named twice) stays as it is, with a code in status (see page_resize).  No two
     requests of a call name one slot, and none fills a page that a beam of another names (whole pages may be anybody's); calls on one pool
     follow one another."""
     dev, dims = k_pages.get_device(), k_pages.dim()
