@@ -110,3 +110,19 @@ def test_requests_that_share_whole_pages():
     # request 0: beam 0 fills a page that its child, beam 1, takes over, and beam 1's page is the prompt's; request 1 moves the prompt's page about
     assert reordered(dev, [[0, 1, 2], [3, 4, 5]], [[2, 0, 2], [1, 0, 2]], pages) == 5
     assert int(dev.refs[prompt]) == 3
+
+
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 63, 2 ** 31 - 64, 4 * 64 + 1, -1, -2 ** 31])
+def test_lengths_that_no_row_can_hold(length):
+    """The largest numbers too (63 more than they are is beyond 32 bits): code 2, the request stays as it is."""
+    pool = plain.Pool(4, 4, 16)
+    assert pool.resize([0, 1, 2, 3], [100, 100, 70, 70]) == 0
+    for parents in ([1, 0], [1, 1], [0, 0]):
+        mine = pool.copy()
+        mine.lengths[0] = length
+        dev = DevicePool(mine)
+        pages = torch.randn(16, 1, PAGE, 8, device=DEV)
+        before = pages.clone()
+        ops.beam_reorder_pages(dev.table, dev.refs, dev.lengths, ints([[0, 1], [2, 3]]), ints([parents, [0, 1]]), pages, None, dev.status)
+        dev.equals(mine)
+        assert dev.status.tolist() == [2] and torch.equal(pages, before)

@@ -535,6 +535,7 @@ beam_tables_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
   __shared__ unsigned char s_lost[MAX_BEAMS], s_spare[MAX_BEAMS];
   const int r = blockIdx.x, tid = threadIdx.x;
   if (tid == 0) s_bad = s_cols = 0;
+  auto pages_of = [](int n) { return (int)(((unsigned)n + (TLC_PAGE - 1)) / TLC_PAGE); };      // (of a length up to 2^31 - 1)
   __syncthreads();
   if (tid < K) {
     const int s = slots[r * K + tid], p = parents[r * K + tid];
@@ -542,10 +543,9 @@ beam_tables_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
     s_parent[tid] = p >= 0 && p < K ? p : tid;         // (a parent that is none: the beam stays as it is)
     const int n = s >= 0 && s < n_slots ? lengths[s] : 0;
     s_len[tid] = n;
-    if (s >= n_slots || n < 0 || (n + TLC_PAGE - 1) / TLC_PAGE > max_pages) atomicMax(&s_bad, s >= n_slots ? (int)RO_SLOT : (int)RO_LENGTH);
+    if (s >= n_slots || n < 0 || pages_of(n) > max_pages) atomicMax(&s_bad, s >= n_slots ? (int)RO_SLOT : (int)RO_LENGTH);
   }
   __syncthreads();
-  auto pages_of = [](int n) { return (n + TLC_PAGE - 1) / TLC_PAGE; };
   if (tid < K && s_slot[tid] >= 0) {
     for (int k = 0; k < K; k++)
       if (k != tid && s_slot[k] == s_slot[tid]) atomicMax(&s_bad, (int)RO_SLOT);
