@@ -126,3 +126,16 @@ def test_lengths_that_no_row_can_hold(length):
         ops.beam_reorder_pages(dev.table, dev.refs, dev.lengths, ints([[0, 1], [2, 3]]), ints([parents, [0, 1]]), pages, None, dev.status)
         dev.equals(mine)
         assert dev.status.tolist() == [2] and torch.equal(pages, before)
+
+
+@pytest.mark.parametrize("bad", [5, 2 ** 25 - 2])
+def test_entries_of_the_longest_rows(bad):
+    """64 beams, two of them with 2^25 pages each: an entry that names no page is found wherever it is."""
+    n = 2 ** 31 - 1
+    table = torch.zeros(2, 2 ** 25, dtype=torch.int32, device=DEV)
+    table[0, -1], table[1, -1], table[1, bad] = 1, 2, 3
+    refs, lengths, status = ints([2 ** 26 - 3, 1, 1]), ints([n, n]), ints([0])
+    before = table.clone()
+    pages = torch.zeros(3, 1, PAGE, 1, dtype=torch.bfloat16, device=DEV)
+    ops.beam_reorder_pages(table, refs, lengths, ints([[0, 1] + [-1] * 62]), ints([[1] + list(range(1, 64))]), pages, None, status)
+    assert status.tolist() == [4] and torch.equal(table, before) and refs.tolist() == [2 ** 26 - 3, 1, 1] and lengths.tolist() == [n, n]

@@ -566,9 +566,9 @@ beam_tables_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
       }
     }
     __syncthreads();
-    // every entry that is going to be used names a page
-    for (int e = tid; e < K * s_cols; e += RO_T) {
-      const int k = e / s_cols, c = e % s_cols;
+    // every entry that is going to be used names a page (64 rows of 2^25 entries are 2^31)
+    for (unsigned e = tid, n = (unsigned)s_cols; e < K * n; e += RO_T) {
+      const int k = (int)(e / n), c = (int)(e % n);
       if (s_slot[k] < 0 || c >= pages_of(s_len[k])) continue;
       const int page = block_table[(size_t)s_slot[k] * max_pages + c];
       if (page < 0 || page >= n_pages) atomicMax(&s_bad, (int)RO_TABLE);
