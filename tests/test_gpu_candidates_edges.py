@@ -1,0 +1,36 @@
+"""Calls of the operators for several candidates at the ends of their ranges, against what the formulas say."""
+import random
+
+import pytest
+import torch
+
+from tinyllama_c_b200 import ops
+
+import candidates_plain as plain
+from test_gpu_candidates import DEV, HALF, PAGE, TYPES, U, DevicePool, attention_case, attention_check, attention_run, ints
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.float32, 16)])
+@pytest.mark.parametrize("context", [2 ** 31 - 1, 2 ** 31 - 64, 2 ** 30 + 5])
+def test_tree_attention_longest_contexts(dtype, hd, context):
+    """A context of up to 2^31 - 1 positions, every page of it the same one.  With queries of 0 every weight is 1: sums of whole numbers, exact in every
+    block, and the result the mean of the page's values (what the last, partly filled page lacks is less than 2^-24 of it), off by the additions of the
+    parts' sums (296 at most, of sums and of results) and its own rounding."""
+    table = torch.zeros(1, 2 ** 25, dtype=torch.int32, device=DEV)
+    k = torch.ones(1, 1, PAGE, hd, dtype=dtype, device=DEV)
+    v = torch.randint(-4, 5, (1, 1, PAGE, hd), device=DEV).to(dtype)
+    zero = torch.zeros(1, hd, dtype=dtype, device=DEV)
+    out = torch.full((1, hd), 7.0, dtype=dtype, device=DEV)
+    ops.tree_attention(zero, zero, zero, k, v, table, ints([0]), ints([context]), ints([0, 1]), ints([context]), out, 1, 1, hd, 0.5, max_context=2 ** 31 - 1, max_new=1)
+    want = v[0, 0].double().mean(0)
+    allow = (2 * 296 + 8) * U * v[0, 0].double().abs().mean(0) + (HALF if dtype == torch.bfloat16 else U) * want.abs() + 1e-30
+    assert bool(((out[0].double() - want).abs() <= allow).all())
+    # a window that only the last positions are in
+    ops.tree_attention(zero, zero, zero, k, v, table, ints([0]), ints([context]), ints([0, 1]), ints([context]), out, 1, 1, hd, 0.5, max_context=2 ** 31 - 1, max_new=1,
+                       window=PAGE + 1)
+    at = torch.arange(context - PAGE, context, device=DEV) % PAGE
+    want = v[0, 0][at].double().sum(0) / (PAGE + 1)
+    assert bool(((out[0].double() - want).abs() <= 8 * U * v[0, 0].double().abs().sum(0) + (HALF if dtype == torch.bfloat16 else U) * want.abs() + 1e-30).all())
+    ops.check_errors()

@@ -52,8 +52,8 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
   s.n = min(max(a.cu[b + 1], s.t0), a.T) - s.t0;
   const int slot = a.slots[b];
   s.context = slot >= 0 && slot < a.n_slots ? min(max(a.start[b], 0), min(a.max_context, (int)min((long long)a.max_pages * TLC_PAGE, 2147483647ll))) : 0;
-  s.first_tile = a.window > 0 ? max(0, s.context + 1 - a.window) / TLC_PAGE : 0;
-  s.context_tiles = (s.context + TLC_PAGE - 1) / TLC_PAGE - s.first_tile;
+  s.first_tile = a.window > 0 ? max(0, s.context - (a.window - 1)) / TLC_PAGE : 0;
+  s.context_tiles = (int)(((unsigned)s.context + (TLC_PAGE - 1)) / TLC_PAGE) - s.first_tile;     // (of a context up to 2^31 - 1)
   s.key_tiles = s.context_tiles + (s.n + TLC_PAGE - 1) / TLC_PAGE;
   s.row_tiles = tree_div(s.n * a.G + a.tile_rows - 1, a.tile_rows);
   s.units = a.KV * s.row_tiles * s.key_tiles;
@@ -148,8 +148,10 @@ template <int NT> __device__ __forceinline__ TreeTake tree_plan(const TreeArgs& 
       const int n = tree_div(room[2 * b + 1] + piece - 1, piece), here = room[2 * b] * n;
       if (c >= before && c < before + here) {
         if (each > 1) s = tree_seq(a, b);
-        const int item = tree_div(c - before, n), k = c - before - item * n, lo = tree_div(k * s.key_tiles, n);
-        s_take = TreeTake{b, item, lo, tree_div((k + 1) * s.key_tiles, n) - lo, s};
+        const int item = tree_div(c - before, n), k = c - before - item * n;
+        const int whole = tree_div(s.key_tiles, n), rest = s.key_tiles - whole * n;      // (k key_tiles / n in parts: the product may pass 32 bits)
+        const int lo = k * whole + tree_div(k * rest, n);
+        s_take = TreeTake{b, item, lo, (k + 1) * whole + tree_div((k + 1) * rest, n) - lo, s};
         if (k == 0 && n > 1) {
           const int g = tree_div(item, s.row_tiles), r0 = (item - g * s.row_tiles) * a.tile_rows;
           split = TreeSplit{n, c, 0, s.t0, r0, min(a.tile_rows, s.n * a.G - r0), g, 0};
