@@ -139,3 +139,63 @@ def test_entries_of_the_longest_rows(bad):
     pages = torch.zeros(3, 1, PAGE, 1, dtype=torch.bfloat16, device=DEV)
     ops.beam_reorder_pages(table, refs, lengths, ints([[0, 1] + [-1] * 62]), ints([[1] + list(range(1, 64))]), pages, None, status)
     assert status.tolist() == [4] and torch.equal(table, before) and refs.tolist() == [2 ** 26 - 3, 1, 1] and lengths.tolist() == [n, n]
+
+
+# ---- whose pages a step writes ------------------------------------------------------------------------------------
+def step(dev, slots, start, new, pages):
+    """Room for a step's rows, their places, their values stored; the places."""
+    dev.resize(slots, [a + n for a, n in zip(start, new)])
+    T = sum(new)
+    rows = torch.randn(T, pages.shape[1] * pages.shape[3], device=DEV)
+    maps = ops.row_maps(dev.table, ints(slots), ints(start), ints(new), T, lengths=dev.lengths)
+    ops.kv_store(rows, rows, maps.row_map, pages, pages.clone())
+    return maps.row_map.tolist()
+
+
+def test_a_refused_step_stores_nothing():
+    """The pool is full (1), or a request would grow in a page that it shares (5): no row beyond what the slots hold has a place."""
+    pool = plain.Pool(3, 4, 4)
+    assert pool.resize([0, 1, 2], [62, 100, 20]) == 0                    # four pages of four
+    pages = torch.randn(4, 2, PAGE, 8, device=DEV)
+    before, dev = pages.clone(), DevicePool(pool)
+    assert step(dev, [0, 1], [62, 100], [4, 1], pages) == [-1] * 5
+    assert dev.status.tolist() == [1] and torch.equal(pages, before)
+    dev.equals(pool)
+    assert step(dev, [0, 1], [62, 100], [2, 1], pages) == [pool.table[0][0] * 64 + 62, pool.table[0][0] * 64 + 63, pool.table[1][1] * 64 + 36]
+    pool = plain.Pool(3, 4, 9)
+    assert pool.resize([0, 2], [100, 64]) == 0
+    pool.table[1], pool.lengths[1] = list(pool.table[0]), 100            # both pages shared
+    for p in pool.table[0][:2]:
+        pool.refs[p] = 2
+    pages = torch.randn(9, 2, PAGE, 8, device=DEV)
+    before, dev = pages.clone(), DevicePool(pool)
+    assert step(dev, [1, 2], [100, 64], [1, 3], pages) == [-1] * 4
+    assert dev.status.tolist() == [5] and torch.equal(pages, before)
+    # rows that the slot does hold have places all the same, whatever has become of the step
+    maps = ops.row_maps(dev.table, ints([1, -1, 0]), ints([98, 0, 99]), ints([4, 1, 2]), 7, lengths=dev.lengths)
+    last = pool.table[0][1] * 64
+    assert maps.row_map.tolist() == [last + 34, last + 35, -1, -1, -1, last + 35, -1]
+    assert maps.positions.tolist() == [98, 99, 100, 101, 0, 99, 100]
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_places_of_what_slots_hold(seed):
+    """Random lengths, slots and drafts: the plain form's places, but for positions that the slot does not hold."""
+    rng = random.Random(seed)
+    B, width = rng.randint(1, 40), rng.randint(1, 6)
+    pool = plain.Pool(B + 2, width, (B + 2) * width)
+    assert pool.resize(list(range(B + 2)), [rng.randint(0, width * PAGE) for _ in range(B + 2)]) == 0
+    slots = [rng.choice([-1, rng.randrange(B + 2), B + 2]) if rng.random() < 0.2 else s for s in rng.sample(range(B + 2), B)]
+    start = [rng.randint(0, width * PAGE) if not 0 <= s < B + 2 or rng.random() < 0.3 else max(0, pool.lengths[s] - rng.randint(0, 9)) for s in slots]
+    new = [rng.randint(0, 20) for _ in slots]
+    T = sum(new) + 2
+    dev = DevicePool(pool)
+    for drafts in (False, True):
+        parents = [p for n in new for p in plain.draft(rng, n)] + [-1, -1] if drafts else None
+        keep = [rng.random() < 0.6 for _ in range(T)] if drafts or seed % 2 else None
+        got = ops.row_maps(dev.table, ints(slots), ints(start), ints(new), T, ints(parents) if drafts else None,
+                           None if keep is None else torch.tensor(keep, device=DEV), 20, lengths=dev.lengths)
+        cu, seq, pos, place, mask = plain.row_maps(pool.table, slots, start, new, T, parents, keep, 1)
+        place = [-1 if b < 0 or p < 0 or at >= pool.lengths[slots[b]] else p for b, p, at in zip(seq, place, pos)]
+        assert (got.cu_seqlens.tolist(), got.row_seq.tolist(), got.positions.tolist(), got.row_map.tolist()) == (cu, seq, pos, place)
+        assert not drafts or got.mask.tolist() == mask

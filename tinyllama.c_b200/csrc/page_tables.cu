@@ -227,15 +227,16 @@ constexpr int MT = 256;
 // Row t of request b (its i-th): sequence b, position start[b] + i, place page * 64 + offset of that position.  With parents a row is
 // a drafted token: parent[t] is the draft it follows (by its index among the request's, always a smaller one; -1: the context), its
 // depth is the number of drafts above it, its position start[b] + depth, and mask [T, words] has a bit for each of those and itself.
-// Such rows have no place unless `keep` accepts them.  Every block adds up the requests' rows by itself (a few loads a
+// Such rows have no place unless `keep` accepts them.  With lengths [n_slots] a row has a place only where its slot holds the position: entries behind
+// a slot's pages are 0, and page 0 is somebody's.  Every block adds up the requests' rows by itself (a few loads a
 // thread), so nothing has to be handed from block to block.  Bound by trips to the L2, three after one another: 3.4 us for 8 rows, 4.3 for
 // 53,000 rows of 700 requests.
 __global__ void __launch_bounds__(MT)
 row_maps_kernel(const int* __restrict__ block_table, int n_slots, int max_pages, const int* __restrict__ slots,
-                const int* __restrict__ start, const int* __restrict__ rows_of, int B, int T, const int* __restrict__ parents,
-                const unsigned char* __restrict__ keep, int words, int* __restrict__ cu, int* __restrict__ row_seq,
+                const int* __restrict__ lengths, const int* __restrict__ start, const int* __restrict__ rows_of, int B, int T,
+                const int* __restrict__ parents, const unsigned char* __restrict__ keep, int words, int* __restrict__ cu, int* __restrict__ row_seq,
                 int* __restrict__ positions, int* __restrict__ row_map, int* __restrict__ mask) {
-  tlc_wait(block_table, slots, start, rows_of, parents, keep, cu, row_seq, positions, row_map, mask);
+  tlc_wait(block_table, slots, lengths, start, rows_of, parents, keep, cu, row_seq, positions, row_map, mask);
   extern __shared__ int sum[];                        // [B + 1]
   __shared__ long long red[33];
   const int tid = threadIdx.x, each = (B + MT - 1) / MT, b0 = min(B, tid * each), b1 = min(B, b0 + each);
@@ -297,7 +298,7 @@ row_maps_kernel(const int* __restrict__ block_table, int n_slots, int max_pages,
   const int s = slots[b];
   if (!lost && (keep ? keep[t] != 0 : parents == nullptr) && s >= 0 && s < n_slots && position < (long long)max_pages * TLC_PAGE) {
     const int p = block_table[(size_t)s * max_pages + position / TLC_PAGE];
-    if (p >= 0 && p < (1 << 25)) place = p * TLC_PAGE + (int)(position % TLC_PAGE);
+    if (p >= 0 && p < (1 << 25) && (!lengths || position < lengths[s])) place = p * TLC_PAGE + (int)(position % TLC_PAGE);
   }
   row_map[t] = place;
 }
@@ -419,15 +420,15 @@ extern "C" int tlc_page_resize(int* block_table, int n_slots, int max_pages, int
   return 0;
 }
 
-extern "C" int tlc_row_maps(const int* block_table, int n_slots, int max_pages, const int* slots, const int* start, const int* rows, int B,
-                            int T, const int* parents, const void* keep, int words, int* cu_seqlens, int* row_seq, int* positions,
+extern "C" int tlc_row_maps(const int* block_table, int n_slots, int max_pages, const int* slots, const int* lengths, const int* start,
+                            const int* rows, int B, int T, const int* parents, const void* keep, int words, int* cu_seqlens, int* row_seq, int* positions,
                             int* row_map, int* mask, cudaStream_t stream) {
   TLC_REQUIRE(B >= 0 && B <= MAX_REQUESTS, "row_maps: %d requests (at most %d a call)", B, MAX_REQUESTS);
   TLC_REQUIRE(T >= 0 && n_slots > 0 && max_pages > 0 && (T == 0 || (parents == nullptr) == (mask == nullptr)) && words >= 0, "row_maps: %d rows, %d slots of %d pages",
               T, n_slots, max_pages);
   if (!mask) words = 0;
   tlc_launch(row_maps_kernel, dim3(T > 0 ? (T + MT - 1) / MT : 1), dim3(MT), (size_t)(B + 1) * sizeof(int), stream, block_table, n_slots, max_pages,
-             slots, start, rows, B, T, parents, (const unsigned char*)keep, words, cu_seqlens, row_seq, positions, row_map, mask);
+             slots, lengths, start, rows, B, T, parents, (const unsigned char*)keep, words, cu_seqlens, row_seq, positions, row_map, mask);
   TLC_CHECK_LAUNCH("row_maps");
   return 0;
 }

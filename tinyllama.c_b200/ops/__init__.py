@@ -170,7 +170,7 @@ _SIGNATURES = {
     "tlc_moe_experts_int8": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i,
                                   _i, _i, _f, _f, _vp]),
     "tlc_page_resize": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp]),
-    "tlc_row_maps": (_i, [_vp, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "tlc_row_maps": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "tlc_kv_store": (_i, [_vp, _vp, _i, _ll, _ll, _ll, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "tlc_tree_attention_scratch": (_ll, [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "tlc_tree_attention": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i,
@@ -2248,7 +2248,8 @@ class RowMaps:
 
 
 def row_maps(block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor, new: torch.Tensor, n_rows: int,
-             parents: Optional[torch.Tensor] = None, keep: Optional[torch.Tensor] = None, max_new: int = 0) -> RowMaps:
+             parents: Optional[torch.Tensor] = None, keep: Optional[torch.Tensor] = None, max_new: int = 0,
+             lengths: Optional[torch.Tensor] = None) -> RowMaps:
     """Sequences, positions and places of a step's rows from the requests' lengths: request b brings new[b] rows after its first
     start[b] positions (int32 [B] each, in packed order), n_rows is how many rows the step's tensors have (more are left out; rows behind
     the last request have request -1, position 0 and no place).
@@ -2256,12 +2257,18 @@ def row_maps(block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor
     parents (int32 [n_rows]) makes the rows drafted tokens: parents[t] is the index, among its request's rows, of the draft that row t
     follows (-1: the request's last position; always smaller than the row's own index).  Positions are then start + depth, mask says which
     drafts a row sees (those above it and itself; max_new: the most rows of a request) and no row has a place, but those that
-    keep (torch.bool [n_rows]) accepts.  A row whose way up is broken sees nothing and has no place.  Without parents, keep leaves out rows."""
+    keep (torch.bool [n_rows]) accepts.  A row whose way up is broken sees nothing and has no place.  Without parents, keep leaves out rows.
+
+    lengths (int32 [slots], the pool's): a row has a place only where its slot holds the position.  Places are read from the table as it is: the
+    pages must be there before (page_resize first), and an entry that a slot does not hold is 0, which is another's page.  So over a pool pass
+    its lengths; where page_resize then refuses a step, the step's rows have no places and nothing is stored.  None is for tables that name a
+    page for every row's position (a Cache's)."""
     B, T, dev = slots.numel(), int(n_rows), block_table.get_device()
     words = 0 if parents is None else (int(max_new) + 31) // 32
     if not (block_table.dtype is _I32 and block_table.dim() == 2 and block_table.is_contiguous() and block_table.numel() > 0 and dev >= 0
             and dev == _get_device() and _ok(slots, _I32, B, dev) and _ok(start, _I32, B, dev) and _ok(new, _I32, B, dev) and B <= MAX_TABLE_REQUESTS
-            and T >= 0 and (parents is None or (words > 0 and _ok(parents, _I32, T, dev))) and (keep is None or _ok(keep, _BOOL, T, dev))):
+            and T >= 0 and (parents is None or (words > 0 and _ok(parents, _I32, T, dev))) and (keep is None or _ok(keep, _BOOL, T, dev))
+            and (lengths is None or _ok(lengths, _I32, block_table.shape[0], dev))):
         _table(block_table, "row_maps")
         if B > MAX_TABLE_REQUESTS or T < 0:
             raise KernelError(f"row_maps: {B} requests (a call takes {MAX_TABLE_REQUESTS}) of {T} rows")
@@ -2273,12 +2280,14 @@ def row_maps(block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor
                 raise KernelError("row_maps: max_new, the most rows of a request, says how wide the drafts' masks are")
         if keep is not None:
             _flags(keep, T, "row_maps keep")
-        _here("row_maps", block_table, slots, start, new, parents, keep)
+        if lengths is not None:
+            _ints_of(lengths, block_table.shape[0], "row_maps lengths")
+        _here("row_maps", block_table, slots, start, new, parents, keep, lengths)
     n_slots, max_pages = block_table.shape
     ints = block_table.new_empty(B + 1 + T * (3 + words))
     at, p = B + 1, ints.data_ptr()
-    _call_packed("tlc_row_maps", block_table.data_ptr(), n_slots, max_pages, slots.data_ptr(), start.data_ptr(), new.data_ptr(), B, T,
-                 0 if parents is None else parents.data_ptr(), 0 if keep is None else keep.data_ptr(), words, p, p + 4 * at, p + 4 * (at + T),
+    _call_packed("tlc_row_maps", block_table.data_ptr(), n_slots, max_pages, slots.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+                 start.data_ptr(), new.data_ptr(), B, T, 0 if parents is None else parents.data_ptr(), 0 if keep is None else keep.data_ptr(), words, p, p + 4 * at, p + 4 * (at + T),
                  p + 4 * (at + 2 * T), p + 4 * (at + 3 * T) if words else 0, _stream())
     if _notes.calls is not None:
         _note_owned(ints)
