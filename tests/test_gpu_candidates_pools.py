@@ -199,3 +199,23 @@ def test_places_of_what_slots_hold(seed):
         place = [-1 if b < 0 or p < 0 or at >= pool.lengths[slots[b]] else p for b, p, at in zip(seq, place, pos)]
         assert (got.cu_seqlens.tolist(), got.row_seq.tolist(), got.positions.tolist(), got.row_map.tolist()) == (cu, seq, pos, place)
         assert not drafts or got.mask.tolist() == mask
+
+
+def test_room_comes_before_places():
+    """Accepted rows that cross into a new page: after page_resize they have places there; asked before it they have none, and are not stored into page 0."""
+    pool = plain.Pool(2, 3, 6)
+    assert pool.resize([1, 0], [64, 62]) == 0                            # page 0 is slot 1's
+    parents, keep, slots, start, new = ints([-1, 0, 1, 2]), torch.tensor([True] * 4, device=DEV), ints([0]), ints([62]), ints([4])
+    rows = torch.randn(4, 2 * 8, device=DEV)
+    for early in (False, True):
+        dev, pages = DevicePool(pool), torch.zeros(6, 2, PAGE, 8, device=DEV)
+        if not early:
+            dev.resize([0], [66])
+        maps = ops.row_maps(dev.table, slots, start, new, 4, parents, keep, 4, lengths=dev.lengths)
+        if early:
+            dev.resize([0], [66])
+        ops.kv_store(rows, None, maps.row_map, pages, None)
+        assert dev.status.tolist() == [0] and dev.table.tolist() == [[1, 2, 0], [0, 0, 0]]
+        assert maps.row_map.tolist() == ([-1] * 4 if early else [64 + 62, 64 + 63, 128, 129])
+        assert not bool(pages[0].any()) and bool(pages[1:].any()) != early
+        assert maps.mask.tolist() == [[1], [3], [7], [15]] and maps.positions.tolist() == [62, 63, 64, 65]
