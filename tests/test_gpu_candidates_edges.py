@@ -34,3 +34,18 @@ def test_tree_attention_longest_contexts(dtype, hd, context):
     want = v[0, 0][at].double().sum(0) / (PAGE + 1)
     assert bool(((out[0].double() - want).abs() <= 8 * U * v[0, 0].double().abs().sum(0) + (HALF if dtype == torch.bfloat16 else U) * want.abs() + 1e-30).all())
     ops.check_errors()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 40])
+@pytest.mark.parametrize("scale", [0.0, -0.2, -1e-30, 1e-30, 1e-50])
+@pytest.mark.parametrize("window,softcap,sink", [(0, 0.0, False), (50, 0.0, True), (0, 3.0, False)])
+def test_tree_attention_scales(dtype, hd, scale, window, softcap, sink):
+    """Scales that are not positive, and tiny ones: hidden keys stay hidden, the scores' order is what the scale makes it."""
+    if softcap and scale == 0:
+        pytest.skip("refused")
+    c = dict(attention_case(dtype, [300, 0, 64, 129], [20, 9, 70, 1], 4, 2, hd, seed=21), scale=scale)
+    values = torch.linspace(-1.0, 1.0, 4) if sink else None
+    out = attention_run(c, window=window, softcap=softcap, sink_values=values.to(DEV) if sink else None)
+    attention_check(c, out, window, softcap, values)
+    ops.check_errors()

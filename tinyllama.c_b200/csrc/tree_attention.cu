@@ -6,7 +6,7 @@
 // with cap(s) = softcap tanh(s / softcap).  The drafts' keys and values are read where the projections left them: nothing of a draft
 // is in the cache before it is accepted.  A row that sees nothing has o = 0.
 //
-// The kernel here serves 32 bits and every head size up to 256; bfloat16 heads of 64 and 128 have their own
+// The kernel here serves 32 bits and every head size up to 256; bfloat16 heads of 64 and 128 with a scale above 0 have their own
 // (tree_attention_tc.cu).  A block walks the tiles of 64 keys of its segments (see tree_attention.cuh) with 64 (or 16) pairs of a row and a head of the
 // group at a time, running maximum and sum per pair, all in 32 bits: scores and products by register tiles of 4 x 4
 // from shared memory.  Bound by the CUDA cores' FFMA rate for many pairs, by the tiles' way into shared memory for few
@@ -535,6 +535,7 @@ extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void
               "tree_attention: contexts of %d, %d new rows, %d pages", max_context, max_new, n_pages);
   TLC_REQUIRE(((uintptr_t)scratch & 15) == 0, "tree_attention: scratch must start on a 16-byte boundary");
   const Cut c = cut_of(dtype, aligned, n_pages, B, T, H, KV, hd, max_context, max_new);
+  TLC_REQUIRE(!c.tc || scale > 0.f, "tree_attention: a scale of %g with `aligned` set", (double)scale);
   TLC_REQUIRE(c.units < (1ll << 31), "tree_attention: %d rows over %d keys are too many", T, max_context);
   TreeArgs a = {};
   a.q = q; a.k_new = k_new; a.v_new = v_new; a.k_pages = k_pages; a.v_pages = v_pages;

@@ -327,6 +327,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           sr[c] = __float_as_uint(fmaf(-cap_out, __fdividef(2.0f, e + 1.0f), cap_out));
         }
       }
+      // (hidden before the scale, which is above 0: 0 x -inf would be NaN, and a negative one would make them the largest)
       if (__any_sync(0xffffffffu, (seen_lo & seen_hi) != 0xffffffffu)) {
 #pragma unroll
         for (int c = 0; c < 64; c++)

@@ -2402,7 +2402,8 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     n_slots, max_pages = block_table.shape
     code = dtype_code(dt)
     pq, pk, pv, pkp, pvp, po = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
-    aligned = 0 if (pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7 else 1
+    # (the tensor cores' kernel hides keys before it scales, which is right for scales above 0: the other one has the rest, NaN among them)
+    aligned = 1 if scale >= 2.0 ** -126 and not ((pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7) else 0
     max_context, max_new = min(int(max_context), max_pages * PAGE), int(max_new)
     scratch = torch.empty(_tree_scratch(dev, code, aligned, k_pages.shape[0], B, T, H, KV, hd, max_context, max_new), dtype=torch.uint8, device=q.device)
     if _notes.calls is not None:
