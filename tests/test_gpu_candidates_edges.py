@@ -49,3 +49,13 @@ def test_tree_attention_scales(dtype, hd, scale, window, softcap, sink):
     out = attention_run(c, window=window, softcap=softcap, sink_values=values.to(DEV) if sink else None)
     attention_check(c, out, window, softcap, values)
     ops.check_errors()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 40])
+@pytest.mark.parametrize("softcap,scale", [(0.01, 1.0), (1024.0, 0.3), (1025.0, 0.3), (1e5, 0.3), (1e30, 0.1), (50.0, 1e-37), (1e4, -0.3), (1e-35, 0.3)])
+def test_tree_attention_caps(dtype, hd, softcap, scale):
+    """Caps far above and below the scores, and scales that a cap cannot be divided by in 32 bits."""
+    c = dict(attention_case(dtype, [300, 0, 64, 129], [20, 9, 70, 1], 4, 2, hd, seed=22), scale=scale)
+    attention_check(c, attention_run(c, softcap=softcap), 0, softcap)
+    ops.check_errors()

@@ -584,7 +584,8 @@ int tlc_kv_store(const void* k, const void* v, int dtype, long long layer_k, lon
  * them whose position is above positions[t] - window.  q [T, H * hd], k_new and v_new [T, KV * hd] (row strides ld_*) of the pages' type.
  * softcap, sink and sink_values as in tlc_attention.  max_context, max_new: no context and no request's rows are longer.
  * A row that sees nothing is 0; rows behind cu_seqlens[B] are left as they were.  scratch: tlc_tree_attention_scratch bytes, 16-byte
- * aligned; aligned: whether q, k_new, v_new, out and the pages start on 16-byte boundaries, row by row, and the scale is above 0. */
+ * aligned; aligned: whether q, k_new, v_new, out and the pages start on 16-byte boundaries, row by row, the scale is above 0 and a
+ * softcap at most 1,024, neither more than 2^100 times the other. */
 long long tlc_tree_attention_scratch(int dtype, int aligned, int n_pages, int B, int T, int H, int KV, int hd, int max_context, int max_new);
 int tlc_tree_attention(const void* q, int dtype, int ld_q, const void* k_new, int ld_k, const void* v_new, int ld_v, const void* k_pages,
                        const void* v_pages, int n_pages, const int* block_table, int n_slots, int max_pages, const int* slots,

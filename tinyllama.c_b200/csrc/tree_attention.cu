@@ -535,7 +535,7 @@ extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void
               "tree_attention: contexts of %d, %d new rows, %d pages", max_context, max_new, n_pages);
   TLC_REQUIRE(((uintptr_t)scratch & 15) == 0, "tree_attention: scratch must start on a 16-byte boundary");
   const Cut c = cut_of(dtype, aligned, n_pages, B, T, H, KV, hd, max_context, max_new);
-  TLC_REQUIRE(!c.tc || scale > 0.f, "tree_attention: a scale of %g with `aligned` set", (double)scale);
+  TLC_REQUIRE(!c.tc || (scale > 0.f && softcap <= 1024.f), "tree_attention: a scale of %g, scores capped at %g, with `aligned` set", (double)scale, (double)softcap);
   TLC_REQUIRE(c.units < (1ll << 31), "tree_attention: %d rows over %d keys are too many", T, max_context);
   TreeArgs a = {};
   a.q = q; a.k_new = k_new; a.v_new = v_new; a.k_pages = k_pages; a.v_pages = v_pages;

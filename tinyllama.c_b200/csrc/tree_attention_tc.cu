@@ -320,7 +320,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const bool p_free = all < 2 || mbar_try(pv_done(wg, all & 1), (uint32_t)((all / 2 - 1) & 1));       // the weights of two steps before have been used
       if constexpr (CAPPED) {
         // a capped score: s <- cap tanh(s scale / cap), left divided by the scale (what follows multiplies by it);
-        // tanh(x) = 1 - 2 / (e^(2x) + 1), cap_in = 2 log2(e) scale / cap, cap_out = cap / scale
+        // tanh(x) = 1 - 2 / (e^(2x) + 1), cap_in = 2 log2(e) scale / cap, cap_out = cap / scale.  Off by some 2^-21 of the cap, since scores far below it
+        // are a difference of 1s: caps of more than 1,024 go to the other kernel.
 #pragma unroll
         for (int c = 0; c < 64; c++) {
           const float e = ex2_quick(__uint_as_float(sr[c]) * cap_in);

@@ -2402,8 +2402,9 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     n_slots, max_pages = block_table.shape
     code = dtype_code(dt)
     pq, pk, pv, pkp, pvp, po = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
-    # (the tensor cores' kernel hides keys before it scales, which is right for scales above 0: the other one has the rest, NaN among them)
-    aligned = 1 if scale >= 2.0 ** -126 and not ((pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7) else 0
+    # The tensor cores' kernel hides keys before it scales, which is right for scales above 0, and its capped scores are off by 2^-21 of the cap: up to 1,024
+    # that is a quarter of what rounding the weights to 16 bits leaves.  The other kernel has the rest, NaN among them.
+    aligned = 1 if scale >= 2.0 ** -126 and (not softcap or (softcap <= 1024.0 and 2.0 ** -100 <= scale / softcap <= 2.0 ** 100)) and not ((pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7) else 0
     max_context, max_new = min(int(max_context), max_pages * PAGE), int(max_new)
     scratch = torch.empty(_tree_scratch(dev, code, aligned, k_pages.shape[0], B, T, H, KV, hd, max_context, max_new), dtype=torch.uint8, device=q.device)
     if _notes.calls is not None:
