@@ -17,3 +17,14 @@ def test_refused(i):
     with pytest.raises(ops.KernelError) as e:
         call(**change)
     assert "CUDA device" not in str(e.value)             # refused for what is wrong with it, not for where it runs
+
+
+@pytest.mark.parametrize("n_slots,max_pages,B,refused", [(64, 1 << 25, 64, True), (4096, 1 << 19, 4096, True), (4096, 1 << 19, 4095, False), (63, 1 << 25, 4096, False),
+                                                         (1 << 20, 4096, 4096, False)])
+def test_pages_of_a_call_fit_32_bits(n_slots, max_pages, B, refused, monkeypatch):
+    """The library refuses before it looks at anything; what it does not refuse fails here for want of a device, not by a launch."""
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    lib = ops.library()
+    code = lib.tlc_page_resize(None, n_slots, max_pages, None, 1 << 20, None, None, None, B, None, None)
+    assert code != 0 and ("2^31" in lib.tlc_last_error().decode()) == refused

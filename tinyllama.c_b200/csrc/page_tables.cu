@@ -105,7 +105,7 @@ page_resize_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
   // 1. each request's slot is claimed (by the sign of its length); what the request takes or gives back is added up
   const int each = (B + RT - 1) / RT, b0 = min(B, tid * each), b1 = min(B, b0 + each);
   int slot[MINE], last[MINE], old[MINE], t_of[MINE], g_of[MINE], bad = 0;    // slot -1: none, or not claimed here; last: a page that is grown in
-  long long mine = 0;                                 // pages taken, and pages given back in the upper half
+  long long mine = 0;                                 // pages taken, and pages given back in the upper half: below 2^31 each, see tlc_page_resize
 #pragma unroll
   for (int i = 0; i < MINE; i++) {
     slot[i] = last[i] = -1;
@@ -409,6 +409,9 @@ extern "C" int tlc_page_resize(int* block_table, int n_slots, int max_pages, int
   TLC_REQUIRE(B > 0 && B <= MAX_REQUESTS, "page_resize: %d requests (at most %d a call)", B, MAX_REQUESTS);
   TLC_REQUIRE(n_slots > 0 && max_pages > 0 && n_pages > 0 && n_pages <= (1 << 25), "page_resize: %d slots of %d pages, %d pages (at most 2^25)",
               n_slots, max_pages, n_pages);
+  // (the kernel adds up pages taken, and pages given back, in 32 bits each; slots are distinct)
+  TLC_REQUIRE((long long)(B < n_slots ? B : n_slots) * max_pages < (1ll << 31), "page_resize: %d requests of up to %d pages, 2^31 or more together",
+              B < n_slots ? B : n_slots, max_pages);
   static OncePerDevice ready;
   constexpr int most = (RT * PER + 2 * (MAX_REQUESTS + 1)) * (int)sizeof(int) + MAX_REQUESTS * (int)sizeof(Request);
   if (!ready.done([&] { return cudaFuncSetAttribute(page_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most); }))

@@ -559,7 +559,8 @@ int tlc_retention_chunked(float* proj, int ld, int q_off, int k_off, int v_off, 
  * table, 3 a slot that does not exist or is named twice, 4 an entry or a count that cannot be (a page that does not exist, or is
  * free), 5 a slot that would grow inside a page it shares.
  * tlc_page_resize: slot slots[b] (-1: nothing) shall hold want[b] positions: pages behind them are given back (entries 0), and
- * missing ones are the lowest free pages, request by request.  All of it, or with a code nothing.  B at most 4,096.
+ * missing ones are the lowest free pages, request by request.  All of it, or with a code nothing.  B at most 4,096, and the rows
+ * of the table that B requests can name fewer than 2^31 entries together.
  * tlc_row_maps: for the rows of a step, request b bringing rows[b] of them after its first start[b] positions: cu_seqlens [B + 1],
  * row_seq, positions and row_map (page * 64 + offset of the row's position, -1: none) [T]; rows behind the last request have row_seq -1,
  * position 0, no place; rows beyond T are left out.  parents (NULL: none) makes the rows drafts: parents[t] is the index, among its request's

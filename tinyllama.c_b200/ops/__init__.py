@@ -2220,7 +2220,7 @@ def page_resize(block_table: torch.Tensor, refs: torch.Tensor, lengths: torch.Te
     The pool is three int32 tensors: refs [pages] counts the entries of block_table [slots, pages a slot] that name a page (0: free),
     lengths [slots] the positions that a slot holds, in the first ceil(length / 64) pages of its row.  Pages behind the positions
     wanted are given back (their entries become 0); missing ones are the lowest free pages, in the order of the requests.  slots and
-    want are int32 [B] (at most 4,096; slot -1: nothing to do).  All of it is done or, with a code, nothing: status[0] is raised to the
+    want are int32 [B] (at most 4,096, whose rows of the table have fewer than 2^31 entries; slot -1: nothing to do).  All of it is done or, with a code, nothing: status[0] is raised to the
     largest code that occurred (POOL_STATUS) and stays until the caller clears it.  Calls on one pool follow one another (on one stream, or
     ordered by events)."""
     dev, B = block_table.get_device(), slots.numel()
