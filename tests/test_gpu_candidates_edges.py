@@ -59,3 +59,32 @@ def test_tree_attention_caps(dtype, hd, softcap, scale):
     c = dict(attention_case(dtype, [300, 0, 64, 129], [20, 9, 70, 1], 4, 2, hd, seed=22), scale=scale)
     attention_check(c, attention_run(c, softcap=softcap), 0, softcap)
     ops.check_errors()
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 24)])
+@pytest.mark.parametrize("drafts", [True, False])
+def test_tree_attention_more_rows_than_said(dtype, hd, drafts):
+    """Requests of 70, 3 and 33 rows where 33 were announced: what is within is right, rows beyond stay as they were, and it is reported."""
+    c = attention_case(dtype, [100, 5, 64], [70, 3, 33], 4, 2, hd, drafts=drafts, seed=31)
+    full = attention_run(c)
+    ops.check_errors()
+    cut = attention_run(dict(c, new=[33, 3, 33], mask=c["mask"]))
+    with pytest.raises(ops.KernelError, match="code 60"):
+        torch.cuda.synchronize()
+        ops.check_errors()
+    ops.check_errors()                                                   # (said once)
+    rows = torch.zeros(c["T"], dtype=torch.bool, device=DEV)
+    for b, n in enumerate([33, 3, 33]):
+        rows[c["cu"][b]:c["cu"][b] + n] = True
+    assert bool((cut[~rows] == 3.0).all())
+    # (the rows within see none beyond: their own results, which other shares may have added up in another order)
+    assert float((cut[rows].float() - full[rows].float()).abs().max()) <= 4 * (HALF if dtype == torch.bfloat16 else 2000 * U) * float(c["v"][:c["cu"][-1]].float().abs().max().clamp(min=6.0))
+
+
+def test_row_maps_of_more_rows_than_the_mask_has_bits():
+    parents = [-1] + list(range(39))
+    maps = ops.row_maps(ints([[0, 1], [2, 3]]), ints([0, 1]), ints([10, 20]), ints([40, 2]), 42, ints(parents + [-1, 0]), torch.ones(42, dtype=torch.bool, device=DEV), 32)
+    assert maps.mask.shape == (42, 1) and maps.mask[32:40].tolist() == [[0]] * 8 and maps.row_map[32:40].tolist() == [-1] * 8
+    assert maps.positions[32:40].tolist() == [10] * 8 and maps.positions[:32].tolist() == list(range(10, 42))
+    assert [v & 0xFFFFFFFF for v in maps.mask[:32, 0].tolist()] == [(2 << i) - 1 for i in range(32)] and maps.row_map[:32].tolist() == list(range(10, 42))
+    assert maps.row_map[40:].tolist() == [2 * 64 + 20, 2 * 64 + 21] and maps.mask[40:].tolist() == [[1], [3]]

@@ -267,10 +267,11 @@ row_maps_kernel(const int* __restrict__ block_table, int n_slots, int max_pages,
   if (parents) {
     const int* const up = parents + sum[b];
     depth = 0;
+    lost = i >> 5 >= words;                           // (the mask has no bit for it)
     int word = i >> 5, here = i;
     unsigned acc = 1u << (i & 31);
     for (int w = words - 1; w > word; w--) bits[w] = 0;
-    for (;;) {                                        // up the tree: indices fall, so the words are finished from the last to the first
+    while (!lost) {                                   // up the tree: indices fall, so the words are finished from the last to the first
       const int p = up[here];
       if (p == -1) break;
       if (p < 0 || p >= here) { lost = true; break; }
@@ -286,7 +287,7 @@ row_maps_kernel(const int* __restrict__ block_table, int n_slots, int max_pages,
     }
     if (word < words) bits[word] = (int)acc;
     for (int w = min(word, words) - 1; w >= 0; w--) bits[w] = 0;
-    if (lost) {                                       // no parent that could be: the row sees no draft and is not kept
+    if (lost) {                                       // no bit, or no parent that could be: the row sees no draft and is not kept
       for (int w = 0; w < words; w++) bits[w] = 0;
       depth = 0;
     }

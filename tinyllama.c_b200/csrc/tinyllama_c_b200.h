@@ -566,7 +566,7 @@ int tlc_retention_chunked(float* proj, int ld, int q_off, int k_off, int v_off, 
  * position 0, no place; rows beyond T are left out.  parents (NULL: none) makes the rows drafts: parents[t] is the index, among its request's
  * rows, of the draft that row t follows (-1: the context; always smaller than the row's own), positions are start + depth,
  * mask [T, words] has the bits of the drafts on the way up and the row's own, and only rows that keep [T] (bytes) accepts have
- * places; a row whose way up is broken sees nothing and has none.  lengths [n_slots] (NULL: the table names a page for every row's position):
+ * places; a row whose way up is broken, or for which the mask has no bit, sees nothing and has none.  lengths [n_slots] (NULL: the table names a page for every row's position):
  * a position that its slot does not hold has no place.  Places are read from the table as it is: room first (tlc_page_resize), then places.
  * tlc_kv_store: row t of layer l of k and v (v may be NULL) [L, T, KV * hd] to place row_map[t] of the pages [L, n_pages, KV, 64, hd]; strides
  * in elements. */
@@ -583,7 +583,8 @@ int tlc_kv_store(const void* k, const void* v, int dtype, long long layer_k, lon
  * Row t of request b sees the request's context (positions 0 .. start[b] - 1, in the pages of its slot; slot -1: none) and those
  * of the request's new rows whose bit mask[t] has (mask [T, words]; NULL: the rows up to itself), with window > 0 those of
  * them whose position is above positions[t] - window.  q [T, H * hd], k_new and v_new [T, KV * hd] (row strides ld_*) of the pages' type.
- * softcap, sink and sink_values as in tlc_attention.  max_context, max_new: no context and no request's rows are longer.
+ * softcap, sink and sink_values as in tlc_attention.  max_context: a longer context is cut.  max_new: of a request with more rows those beyond
+ * are left as they were, nobody sees them, and the error word says 60 (tlc_linear_error).
  * A row that sees nothing is 0; rows behind cu_seqlens[B] are left as they were.  scratch: tlc_tree_attention_scratch bytes, 16-byte
  * aligned; aligned: whether q, k_new, v_new, out and the pages start on 16-byte boundaries, row by row, the scale is above 0 and a
  * softcap at most 1,024, neither more than 2^100 times the other. */

@@ -544,7 +544,8 @@ extern "C" int tlc_tree_attention(const void* q, int dtype, int ld_q, const void
   a.n_slots = n_slots; a.max_pages = max_pages; a.words = words;
   a.out = out; a.out_ld = out_ld; a.B = B; a.T = T; a.H = H; a.KV = KV; a.hd = hd;
   a.scale = scale; a.window = window > 0 ? window : 0; a.softcap = softcap; a.sink = sink; a.sink_values = sink_values;
-  a.max_context = max_context;
+  a.max_context = max_context; a.max_new = max_new;
+  a.err = tlc_error_words_here();
   const uintptr_t starts = (uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new | (uintptr_t)k_pages | (uintptr_t)v_pages;
   a.G = H / KV;
   a.vec_out = hd % 4 == 0 && (out_ld & 3) == 0 && ((uintptr_t)out & (dtype == TLC_F32 ? 15 : 7)) == 0;

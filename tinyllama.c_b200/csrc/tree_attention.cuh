@@ -1,6 +1,7 @@
 // What the kernels of tree attention share: the arguments, which work a block takes, and where its partial results go.
 #pragma once
 #include "common.cuh"
+#include "mbarrier.cuh"
 
 // What block c leaves for the kernel that adds up partial results: an item whose segments are those of blocks c0 .. c0 + n - 1 (n 0: none).
 struct TreeSplit {
@@ -21,7 +22,7 @@ struct TreeArgs {
   float softcap;
   int sink;
   const float* sink_values;
-  int max_context;
+  int max_context, max_new;                               // a longer context is cut, and so is a request of more rows (TREE_MORE_ROWS is reported)
   int G;                                                  // query heads of a key/value head
   int vec, vec_out;                                       // every input row, every output row starts on a boundary of four elements, with heads of fours
   int tile_rows;                                          // (row, head of the group) pairs of a tile
@@ -29,7 +30,10 @@ struct TreeArgs {
   float *part_o, *part_ml;                                // [blocks, 2, hd in fours, most rows of a tile, 4] and [blocks, 2, most rows of a tile, 2]
   int part_rows;                                          // most rows of a tile
   struct TreeSplit* splits;                               // [blocks]
+  ErrWords* err;                                          // or NULL
 };
+
+constexpr int TREE_MORE_ROWS = 60;                        // code of the error word
 
 // a / b of numbers that are not negative: by a 32-bit reciprocal where they are small (a plan is a chain of divisions, an integer one
 // takes four times as long)
@@ -49,7 +53,7 @@ struct TreeSeq {
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
   TreeSeq s;
   s.t0 = min(max(a.cu[b], 0), a.T);
-  s.n = min(max(a.cu[b + 1], s.t0), a.T) - s.t0;
+  s.n = min(min(max(a.cu[b + 1], s.t0), a.T) - s.t0, a.max_new);
   const int slot = a.slots[b];
   s.context = slot >= 0 && slot < a.n_slots ? min(max(a.start[b], 0), min(a.max_context, (int)min((long long)a.max_pages * TLC_PAGE, 2147483647ll))) : 0;
   s.first_tile = a.window > 0 ? max(0, s.context - (a.window - 1)) / TLC_PAGE : 0;
@@ -113,6 +117,10 @@ template <int NT> __device__ __forceinline__ TreeTake tree_plan(const TreeArgs& 
     s = tree_seq(a, b);
     units += s.units;
     items += a.KV * s.row_tiles;
+    if (c == 0 && a.err && min(a.cu[b + 1], a.T) - s.t0 > a.max_new) {
+      atomicExch(&a.err->flag, TREE_MORE_ROWS);
+      *(volatile int*)a.err->host = TREE_MORE_ROWS;
+    }
     if (look) { room[2 * b] = a.KV * s.row_tiles; room[2 * b + 1] = s.key_tiles; }
   }
   const int w_sum = __reduce_add_sync(0xffffffffu, units), i_sum = __reduce_add_sync(0xffffffffu, items);
@@ -149,7 +157,9 @@ template <int NT> __device__ __forceinline__ TreeTake tree_plan(const TreeArgs& 
       if (c >= before && c < before + here) {
         if (each > 1) s = tree_seq(a, b);
         const int item = tree_div(c - before, n), k = c - before - item * n;
-        const int whole = tree_div(s.key_tiles, n), rest = s.key_tiles - whole * n;      // (k key_tiles / n in parts: the product may pass 32 bits)
+        // (n is at most 512: the products of more tiles may pass 32 bits)
+        const bool small = s.key_tiles < 1 << 22;
+        const int whole = small ? 0 : s.key_tiles / n, rest = s.key_tiles - whole * n;
         const int lo = k * whole + tree_div(k * rest, n);
         s_take = TreeTake{b, item, lo, (k + 1) * whole + tree_div((k + 1) * rest, n) - lo, s};
         if (k == 0 && n > 1) {

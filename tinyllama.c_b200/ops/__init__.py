@@ -827,7 +827,7 @@ def check_errors() -> None:
         raise KernelError(f"a kernel gave up on a bounded wait (code {code}: 1 loader, 2 issuer, 3 epilogue, 4 drain, "
                           f"5 accumulator of the tensor-core product; 9 the self-test; 11-16 the scan of prompts; 21-29 "
                           f"attention of prompts; 31-34 the product of few rows; 41 the state of a one-token Mamba2 step; 51-59 "
-                          f"products in 8-bit integers; 61-69 attention of drafts); "
+                          f"products in 8-bit integers; 61-69 attention of drafts), or attention of drafts was given a request of more rows than max_new (code 60); "
                           f"its output is incomplete")
 
 
@@ -2257,7 +2257,7 @@ def row_maps(block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor
     parents (int32 [n_rows]) makes the rows drafted tokens: parents[t] is the index, among its request's rows, of the draft that row t
     follows (-1: the request's last position; always smaller than the row's own index).  Positions are then start + depth, mask says which
     drafts a row sees (those above it and itself; max_new: the most rows of a request) and no row has a place, but those that
-    keep (torch.bool [n_rows]) accepts.  A row whose way up is broken sees nothing and has no place.  Without parents, keep leaves out rows.
+    keep (torch.bool [n_rows]) accepts.  A row whose way up is broken, or of an index for which max_new leaves no bit, sees nothing and has no place.  Without parents, keep leaves out rows.
 
     lengths (int32 [slots], the pool's): a row has a place only where its slot holds the position.  Places are read from the table as it is: the
     pages must be there before (page_resize first), and an entry that a slot does not hold is 0, which is another's page.  So over a pool pass
@@ -2376,7 +2376,8 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
 
     positions int32 [T]: the rows' positions, none below its request's start; with window > 0 a row sees the keys whose
     position is above its own - window.  softcap, sink and sink_values as in attention().  max_context and max_new bound the contexts and the
-    requests' new rows (a longer context is cut).  A row that sees nothing is 0; rows behind the last request are left as they were;
+    requests' new rows: a longer context is cut; of a request with more rows those beyond are left as they were and nobody sees them, which
+    check_errors() reports.  A row that sees nothing is 0; rows behind the last request are left as they were;
     a key or value that a row does not see does not touch it, whatever it holds.  float32 or bfloat16, heads of up to 256.  How the
     keys are cut among blocks goes by the whole call: a row's sums may be added up in another order beside other requests."""
     T, B, dt, dev = q.shape[0], slots.numel(), q.dtype, q.get_device()
