@@ -28,3 +28,13 @@ def test_pages_of_a_call_fit_32_bits(n_slots, max_pages, B, refused, monkeypatch
     lib = ops.library()
     code = lib.tlc_page_resize(None, n_slots, max_pages, None, 1 << 20, None, None, None, B, None, None)
     assert code != 0 and ("2^31" in lib.tlc_last_error().decode()) == refused
+
+
+@pytest.mark.parametrize("args,blocks,rows", [((0, 1, 50, 4, 64, 8, 2, 128, 4096, 64), 296, 64), ((0, 1, 50, 1, 3, 4, 2, 64, 100, 3), 12, 16),
+                                              ((0, 1, 50, 4, 64, 8, 2, 37, 4096, 64), 296, 64)])
+def test_scratch_by_the_current_device(args, blocks, rows):
+    """Asked anew in every call, a B200's 148 SMs where there is no device: two blocks of partial results to an SM at most, each two slots of
+    `rows` rows of heads in fours and two statistics, and the 32-byte split."""
+    hd = args[7]
+    assert ops.library().tlc_tree_attention_scratch(*args) == blocks * (2 * rows * ((hd + 3) // 4 * 4 + 2) * 4 + 32)
+    assert ops.library().tlc_beam_select_scratch(8, 151551) == 8 * 296 * 16 and ops.library().tlc_beam_select_scratch(8, 151552) == 8 * 74 * 16

@@ -670,7 +670,7 @@ beam_pages_kernel(char* k_pages, char* v_pages, long long layer_bytes, int KV, i
 }  // namespace
 
 // values of a piece: 64 a lane make few lists of long pieces; 16 spread a few rows over the SMs (4 rows of 65,536: 512 warps, not 128)
-static int piece_values(long long rows, int V) { return rows * V >= 2048ll * 148 * 4 ? 2048 : 512; }
+static int piece_values(long long rows, int V) { return rows * V >= 2048ll * 4 * tlc_sm_count() ? 2048 : 512; }
 
 extern "C" long long tlc_beam_select_scratch(int rows, int V) {
   const int per = piece_values(rows, V);

@@ -472,7 +472,7 @@ tree_merge_kernel(TreeArgs a) {
 }
 
 template <typename T> void run_merge(const TreeArgs& a, cudaStream_t stream) {
-  const long long tasks = ((long long)a.T * a.H + MG_ROWS - 1) / MG_ROWS * ((a.hd + 31) / 32), most = 148 * 2;     // two to an SM
+  const long long tasks = ((long long)a.T * a.H + MG_ROWS - 1) / MG_ROWS * ((a.hd + 31) / 32), most = 2 * tlc_sm_count();     // two to an SM
   const dim3 grid((unsigned)(tasks < most ? tasks : most));
   tlc_launch(tree_merge_kernel<T>, grid, dim3(MG_T), 0, stream, a);
 }
@@ -501,8 +501,6 @@ int tlc_tree_attention_simt(const TreeArgs& a, int dtype, int rows, cudaStream_t
 namespace {
 struct Cut { bool tc; int rows, tile_rows, blocks; long long units, scratch; };
 Cut cut_of(int dtype, int aligned, int n_pages, int B, int T, int H, int KV, int hd, int max_context, int max_new) {
-  static int sms = 0;
-  if (sms == 0) { int dev = 0; cudaGetDevice(&dev); cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev); }
   Cut c;
   const int G = H / KV;
   c.tc = tlc_tree_attention_tc_takes(dtype, aligned, H, KV, hd, n_pages);
@@ -510,7 +508,7 @@ Cut cut_of(int dtype, int aligned, int n_pages, int B, int T, int H, int KV, int
   c.tile_rows = c.tc ? 128 / G * G * 2 : c.rows;
   const long long kt = ((long long)max_context + BN - 1) / BN + (max_new + BN - 1) / BN;
   c.units = (((long long)T * G + c.tile_rows - 1) / c.tile_rows + B) * KV * kt;
-  const long long wave = (long long)sms * (c.tc ? 1 : 2);
+  const long long wave = (long long)tlc_sm_count() * (c.tc ? 1 : 2);
   c.blocks = (int)(c.units < wave ? (c.units < 1 ? 1 : c.units) : wave);
   if (c.blocks > MG_MOST) c.blocks = MG_MOST;
   c.scratch = (long long)c.blocks * (2 * c.rows * ((hd + 3) / 4 * 4 + 2) * 4 + (long long)sizeof(TreeSplit));

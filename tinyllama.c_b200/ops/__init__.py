@@ -2451,8 +2451,8 @@ def _tree_attention_checks(q, k_new, v_new, k_pages, v_pages, block_table, slots
 
 
 @functools.lru_cache(maxsize=4096)
-def _beam_scratch(*args) -> int:
-    return library().tlc_beam_select_scratch(*args)
+def _beam_scratch(device: int, rows: int, V: int) -> int:   # (how a row is cut goes by the device's SMs)
+    return library().tlc_beam_select_scratch(rows, V)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, ended: Optional[torch.Tensor] = None, pad: int = 0,
@@ -2474,7 +2474,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, ended: Optio
         _beam_select_checks(logits, scores, n, ended, pad, placed)
     (R, K), (rows, V) = scores.shape, logits.shape
     size = 4 * (3 * R * n + (-3 * R * n) % 4)              # tokens, parents and scores, then room for the kernels on a 16-byte boundary
-    room = torch.empty((size + (_beam_scratch(rows, V) if R else 0)) // 4, dtype=_I32, device=logits.device)
+    room = torch.empty((size + (_beam_scratch(dev, rows, V) if R else 0)) // 4, dtype=_I32, device=logits.device)
     view, p = room.as_strided, room.data_ptr()
     if R:
         if _notes.calls is not None:
