@@ -88,3 +88,10 @@ def test_row_maps_of_more_rows_than_the_mask_has_bits():
     assert maps.positions[32:40].tolist() == [10] * 8 and maps.positions[:32].tolist() == list(range(10, 42))
     assert [v & 0xFFFFFFFF for v in maps.mask[:32, 0].tolist()] == [(2 << i) - 1 for i in range(32)] and maps.row_map[:32].tolist() == list(range(10, 42))
     assert maps.row_map[40:].tolist() == [2 * 64 + 20, 2 * 64 + 21] and maps.mask[40:].tolist() == [[1], [3]]
+
+
+@pytest.mark.parametrize("R,K,V,n", [(1, 4, 65536, 4), (5, 8, 130048, 3), (0, 2, 9, 2)])
+def test_beam_select_results_keep_little_else(R, K, V, n):
+    """Tokens and parents are kept for every step of a search: with them their own bytes and 16 KB at most."""
+    got = ops.beam_select(torch.randn(R * K, V, device=DEV), torch.zeros(R, K, device=DEV), n)
+    assert all(t.untyped_storage().nbytes() <= 12 * R * n + 12 + 16384 and t.shape == (R, n) for t in got)

@@ -2156,6 +2156,7 @@ def retention_chunked(proj: torch.Tensor, q_off: int, k_off: int, v_off: int, g_
 # ---- several candidates of a request over one paged cache: drafted tokens, beams ---------------------------------------------
 MAX_TABLE_REQUESTS = 4096      # page_tables.cu: MAX_REQUESTS
 MAX_BEAMS = 64                 # beam.cu: beams of a request, and candidates of one
+MAX_KEPT = 16384               # bytes of a call's scratch that may lie behind its results
 MAX_POOL_PAGES = 1 << 25       # places (page * 64 + offset) are 32-bit numbers
 POOL_STATUS = {0: "done", 1: "not enough free pages", 2: "a length below 0 or beyond a row of the block table",
                3: "a slot that does not exist or is named twice", 4: "an entry or a count that cannot be",
@@ -2473,14 +2474,20 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, ended: Optio
             and logits.stride(1) == 1 and (ended is None or _ok(ended, _BOOL, scores.numel(), dev))):
         _beam_select_checks(logits, scores, n, ended, pad, placed)
     (R, K), (rows, V) = scores.shape, logits.shape
-    size = 4 * (3 * R * n + (-3 * R * n) % 4)              # tokens, parents and scores, then room for the kernels on a 16-byte boundary
-    room = torch.empty((size + (_beam_scratch(dev, rows, V) if R else 0)) // 4, dtype=_I32, device=logits.device)
+    # Tokens, parents and scores, then room for the kernels on a 16-byte boundary; more of it than MAX_KEPT lies apart, so that whoever keeps a
+    # search's tokens does not keep that (a second allocation is 2 us of the host's time, a seventh of a call for one request).
+    size, work = 4 * (3 * R * n + (-3 * R * n) % 4), _beam_scratch(dev, rows, V) if R else 0
+    apart = work > MAX_KEPT
+    room = torch.empty((size if apart else size + work) // 4, dtype=_I32, device=logits.device)
     view, p = room.as_strided, room.data_ptr()
     if R:
+        scratch = torch.empty(work, dtype=torch.uint8, device=logits.device) if apart else None
         if _notes.calls is not None:
             _note_owned(room)
+            if apart:
+                _note_owned(scratch)
         _call_packed("tlc_beam_select", logits.data_ptr(), logits.stride(0) if rows > 1 else V, scores.data_ptr(), 0 if ended is None else ended.data_ptr(), R, K, V, n,
-                     int(pad), 1 if placed else 0, p + size, p, p + 4 * R * n, p + 8 * R * n, _stream())
+                     int(pad), 1 if placed else 0, scratch.data_ptr() if apart else p + size, p, p + 4 * R * n, p + 8 * R * n, _stream())
     return view((R, n), (n, 1), 0), view((R, n), (n, 1), R * n), view((R, n), (n, 1), 2 * R * n).view(torch.float32)
 
 
