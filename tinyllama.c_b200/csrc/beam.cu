@@ -555,15 +555,20 @@ beam_tables_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
   __syncthreads();
   if (bad == 0 && moved) {
     // the beams' own last pages, and how many columns there are to look at
+    int count = 0;
+    bool moves = false, fills = false;
     if (tid < K && s_slot[tid] >= 0) {
       const int have = pages_of(s_len[tid]), p = s_parent[tid];
-      s_last[tid] = have > 0 ? block_table[(size_t)s_slot[tid] * max_pages + have - 1] : -1;
+      const int last = have > 0 ? block_table[(size_t)s_slot[tid] * max_pages + have - 1] : -1;
+      const bool there = last >= 0 && last < n_pages;
+      s_last[tid] = s_fill[tid] = last;
       atomicMax(&s_cols, have);
-      if (p != tid && s_len[p] % TLC_PAGE != 0) {
-        const int last = s_last[tid];
-        if (last < 0 || last >= n_pages) atomicMax(&s_bad, (int)RO_TABLE);
-        else if (refs[last] != 1) atomicMax(&s_bad, refs[last] < 1 ? (int)RO_TABLE : (int)RO_SHARED);
+      if (p != tid) {
+        count = there ? refs[last] : 0;
+        fills = s_len[p] % TLC_PAGE != 0;
+        if (fills && count != 1) atomicMax(&s_bad, count < 1 ? (int)RO_TABLE : (int)RO_SHARED);
       }
+      moves = p != tid;
     }
     __syncthreads();
     // every entry that is going to be used names a page (64 rows of 2^25 entries are 2^31)
@@ -573,26 +578,24 @@ beam_tables_kernel(int* block_table, int n_slots, int max_pages, int* refs, int 
       const int page = block_table[(size_t)s_slot[k] * max_pages + c];
       if (page < 0 || page >= n_pages) atomicMax(&s_bad, (int)RO_TABLE);
     }
-    __syncthreads();
-    const bool sound = s_bad == 0;
-    // s_lost: the beam's last page goes to a child, and it fills one; s_spare: its last page is nobody's after the move
-    if (sound && tid < K) {
-      const int p = s_parent[tid], n = s_len[tid], last = s_last[tid];
-      const bool moves = p != tid && s_slot[tid] >= 0, fills = moves && s_len[p] % TLC_PAGE != 0;
-      bool taken = false;
-      if (n % TLC_PAGE == 0)
-        for (int k = 0; k < K; k++) taken |= k != tid && s_parent[k] == tid && s_slot[k] >= 0;
-      s_lost[tid] = fills && taken;
-      s_spare[tid] = moves && !fills && !taken && n > 0 && refs[last] == 1;
-      s_fill[tid] = last;
-    }
-    __syncthreads();
-    if (sound && tid < K && s_lost[tid]) {
-      int before = 0, at = 0;
-      for (int k = 0; k < tid; k++) before += s_lost[k];
-      for (; at < K; at++)
-        if (s_spare[at] && before-- == 0) break;
-      if (at < K) s_fill[tid] = s_last[at]; else atomicMax(&s_bad, (int)RO_SHARED);
+    const bool whole = tid < K && s_len[tid] % TLC_PAGE == 0;
+    if (__syncthreads_or(fills && whole) && s_bad == 0) {
+      // s_lost: the beam's last page goes to a child, and it fills one; s_spare: its last page is nobody's after the move
+      if (tid < K) {
+        bool taken = false;
+        if (whole)
+          for (int k = 0; k < K; k++) taken |= k != tid && s_parent[k] == tid && s_slot[k] >= 0;
+        s_lost[tid] = fills && taken;
+        s_spare[tid] = moves && !fills && !taken && s_len[tid] > 0 && count == 1;
+      }
+      __syncthreads();
+      if (tid < K && s_lost[tid]) {
+        int before = 0, at = 0;
+        for (int k = 0; k < tid; k++) before += s_lost[k];
+        for (; at < K; at++)
+          if (s_spare[at] && before-- == 0) break;
+        if (at < K) s_fill[tid] = s_last[at]; else atomicMax(&s_bad, (int)RO_SHARED);
+      }
     }
   }
   __syncthreads();
