@@ -10,7 +10,7 @@
 // (tree_attention_tc.cu).  A block walks the tiles of 64 keys of its segments (see tree_attention.cuh) with 64 (or 16) pairs of a row and a head of the
 // group at a time, running maximum and sum per pair, all in 32 bits: scores and products by register tiles of 4 x 4
 // from shared memory.  Bound by the CUDA cores' FFMA rate for many pairs, by the tiles' way into shared memory for few
-// (32 bits, 3 requests of up to 1,900 keys, heads of 80: 18 us, of which the first tile's way in, two tiles a block and the sums' way out;
+// (32 bits, 3 requests of up to 1,900 keys, heads of 80: 20 us, of which the first tile's way in, two tiles a block and the sums' way out;
 // bfloat16 heads of 256, 2 x 30,000 keys, 16 drafts of 16 heads: 637 us, 25 TFLOP/s).
 #include "tree_attention.cuh"
 

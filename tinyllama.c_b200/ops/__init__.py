@@ -2258,7 +2258,8 @@ def row_maps(block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor
     parents (int32 [n_rows]) makes the rows drafted tokens: parents[t] is the index, among its request's rows, of the draft that row t
     follows (-1: the request's last position; always smaller than the row's own index).  Positions are then start + depth, mask says which
     drafts a row sees (those above it and itself; max_new: the most rows of a request) and no row has a place, but those that
-    keep (torch.bool [n_rows]) accepts.  A row whose way up is broken, or of an index for which max_new leaves no bit, sees nothing and has no place.  Without parents, keep leaves out rows.
+    keep (torch.bool [n_rows]) accepts.  A row whose way up is broken, or of an index for which max_new leaves no bit, sees no
+    draft and has no place.  Without parents, keep leaves out rows.
 
     lengths (int32 [slots], the pool's): a row has a place only where its slot holds the position.  Places are read from the table as it is: the
     pages must be there before (page_resize first), and an entry that a slot does not hold is 0, which is another's page.  So over a pool pass
@@ -2320,7 +2321,8 @@ def kv_store(k: torch.Tensor, v: Optional[torch.Tensor], row_map: torch.Tensor, 
     """Stores rows of keys and values at the places of row_map (int32 [T], see row_maps), of all layers in one launch: k and v [T, KV * hd] with
     pages [n, KV, 64, hd], or [L, T, KV * hd] with pages [L, n, KV, 64, hd]; float32 or bfloat16, rounded where the pages are
     narrower; v and v_pages may be None (pages without values).  Rows of k and v may be strided.  A row without a place (-1, or one
-    that does not exist) is not stored.  Places are distinct, as row_maps makes them: of two rows for one place either may stay."""
+    that does not exist) is not stored.  Places are distinct, as row_maps makes them of rows at positions of their own: of two rows for one place (two
+    accepted drafts of one depth) any mixture may stay."""
     dev, rows, sk, pages, sv = k.get_device(), k.shape, k.stride(), k_pages.shape, ()
     dims, ok = len(rows), False
     if (dims == 2 or dims == 3) and len(pages) == dims + 2:
