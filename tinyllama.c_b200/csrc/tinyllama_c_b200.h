@@ -566,8 +566,8 @@ int tlc_retention_chunked(float* proj, int ld, int q_off, int k_off, int v_off, 
  * position 0, no place; rows beyond T are left out.  parents (NULL: none) makes the rows drafts: parents[t] is the index, among its request's
  * rows, of the draft that row t follows (-1: the context; always smaller than the row's own), positions are start + depth,
  * mask [T, words] has the bits of the drafts on the way up and the row's own, and only rows that keep [T] (bytes) accepts have
- * places; a row whose way up is broken, or for which the mask has no bit, sees no draft and has none.  lengths [n_slots] (NULL: the table names a page for every row's position):
- * a position that its slot does not hold has no place.  Places are read from the table as it is: room first (tlc_page_resize), then places.
+ * places; a row whose way up is broken, or for which the mask has no bit, sees no draft and has none.  lengths [n_slots] (NULL: the
+ * table names a page for every row's position): a position that its slot does not hold has no place.  Places are read from the table as it is: room first (tlc_page_resize), then places.
  * tlc_kv_store: row t of layer l of k and v (v may be NULL) [L, T, KV * hd] to place row_map[t] of the pages [L, n_pages, KV, 64, hd]; strides
  * in elements. */
 int tlc_page_resize(int* block_table, int n_slots, int max_pages, int* refs, int n_pages, int* lengths, const int* slots,

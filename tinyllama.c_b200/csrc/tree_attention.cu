@@ -6,7 +6,7 @@
 // with cap(s) = softcap tanh(s / softcap).  The drafts' keys and values are read where the projections left them: nothing of a draft
 // is in the cache before it is accepted.  A row that sees nothing has o = 0.
 //
-// The kernel here serves 32 bits and every head size up to 256; bfloat16 heads of 64 and 128 with a scale above 0 have their own
+// The kernel here serves 32 bits and every head size up to 256; bfloat16 heads of 64 and 128 with a scale above 0 and no cap above 1,024 have their own
 // (tree_attention_tc.cu).  A block walks the tiles of 64 keys of its segments (see tree_attention.cuh) with 64 (or 16) pairs of a row and a head of the
 // group at a time, running maximum and sum per pair, all in 32 bits: scores and products by register tiles of 4 x 4
 // from shared memory.  Bound by the CUDA cores' FFMA rate for many pairs, by the tiles' way into shared memory for few

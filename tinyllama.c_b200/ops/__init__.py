@@ -2221,8 +2221,8 @@ def page_resize(block_table: torch.Tensor, refs: torch.Tensor, lengths: torch.Te
     The pool is three int32 tensors: refs [pages] counts the entries of block_table [slots, pages a slot] that name a page (0: free),
     lengths [slots] the positions that a slot holds, in the first ceil(length / 64) pages of its row.  Pages behind the positions
     wanted are given back (their entries become 0); missing ones are the lowest free pages, in the order of the requests.  slots and
-    want are int32 [B] (at most 4,096, whose rows of the table have fewer than 2^31 entries; slot -1: nothing to do).  All of it is done or, with a code, nothing: status[0] is raised to the
-    largest code that occurred (POOL_STATUS) and stays until the caller clears it.  Calls on one pool follow one another (on one stream, or
+    want are int32 [B] (at most 4,096, whose rows of the table have fewer than 2^31 entries; slot -1: nothing to do).  All of it is
+    done or, with a code, nothing: status[0] is raised to the largest code that occurred (POOL_STATUS) and stays until the caller clears it.  Calls on one pool follow one another (on one stream, or
     ordered by events)."""
     dev, B = block_table.get_device(), slots.numel()
     if not (_pool_ok(block_table, refs, lengths, status, dev) and _ok(slots, _I32, B, dev) and _ok(want, _I32, B, dev) and B <= MAX_TABLE_REQUESTS
@@ -2289,8 +2289,8 @@ def row_maps(block_table: torch.Tensor, slots: torch.Tensor, start: torch.Tensor
     ints = block_table.new_empty(B + 1 + T * (3 + words))
     at, p = B + 1, ints.data_ptr()
     _call_packed("tlc_row_maps", block_table.data_ptr(), n_slots, max_pages, slots.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-                 start.data_ptr(), new.data_ptr(), B, T, 0 if parents is None else parents.data_ptr(), 0 if keep is None else keep.data_ptr(), words, p, p + 4 * at, p + 4 * (at + T),
-                 p + 4 * (at + 2 * T), p + 4 * (at + 3 * T) if words else 0, _stream())
+                 start.data_ptr(), new.data_ptr(), B, T, 0 if parents is None else parents.data_ptr(), 0 if keep is None else keep.data_ptr(), words,
+                 p, p + 4 * at, p + 4 * (at + T), p + 4 * (at + 2 * T), p + 4 * (at + 3 * T) if words else 0, _stream())
     if _notes.calls is not None:
         _note_owned(ints)
     if not words:                                          # (one call that cuts: half the time of four slices)
@@ -2408,7 +2408,9 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     pq, pk, pv, pkp, pvp, po = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
     # The tensor cores' kernel hides keys before it scales, which is right for scales above 0, and its capped scores are off by 2^-21 of the cap: up to 1,024
     # that is a quarter of what rounding the weights to 16 bits leaves.  The other kernel has the rest, NaN among them.
-    aligned = 1 if scale >= 2.0 ** -126 and (not softcap or (softcap <= 1024.0 and 2.0 ** -100 <= scale / softcap <= 2.0 ** 100)) and not ((pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7) else 0
+    aligned = 0 if (pq | pk | pv | pkp | pvp | po) & 15 or (ld_q | ld_k | ld_v | ld_o) & 7 or not scale >= 2.0 ** -126 else 1
+    if softcap and not (softcap <= 1024.0 and 2.0 ** -100 <= scale / softcap <= 2.0 ** 100):
+        aligned = 0
     max_context, max_new = min(int(max_context), max_pages * PAGE), int(max_new)
     scratch = torch.empty(_tree_scratch(dev, code, aligned, k_pages.shape[0], B, T, H, KV, hd, max_context, max_new), dtype=torch.uint8, device=q.device)
     if _notes.calls is not None:
@@ -2559,9 +2561,10 @@ def beam_reorder_pages(block_table: torch.Tensor, refs: torch.Tensor, lengths: t
     last page is whole and another beam takes it over, what the beam fills is a last page that a beam of the request gives back.
 
     slots and parents int32 [R, K]; slot -1 or a parent outside 0 .. K - 1 leaves a beam as it is.  A request for which it cannot be done
-    (no page of its own, one that others share or take over and none given back, a slot named twice) stays as it is, with a code in status (see page_resize).  No two
-    requests of a call name one slot, and none fills a page that a beam of another names (whole pages may be anybody's); calls on one pool
-    follow one another."""
+    (no page of its own, one that others share or take over and none given back, a slot named twice) stays as it is, with a code in
+    status (see page_resize).  No two requests of a call name one slot, and none fills a page that a beam of another names (whole pages
+    may be anybody's; one that two requests give back in a call may be found free by the later one, or by neither); calls on one
+    pool follow one another."""
     dev, dims = k_pages.get_device(), k_pages.dim()
     if not (slots.dim() == 2 and parents.shape == slots.shape and 1 <= slots.shape[1] <= MAX_BEAMS and _pool_ok(block_table, refs, lengths, status, dev)
             and block_table.get_device() == dev and dev == _get_device() and _ok(slots, _I32, slots.numel(), dev) and _ok(parents, _I32, slots.numel(), dev)
